@@ -94,6 +94,31 @@ int sglb200_silu_and_mul_masked_quant_fp8(const void* input, int dtype, void* ou
                                           float eps, const int32_t* masked_m, void* stream);
 
 /*
+ * 4-bit floating point.  A value is an e2m1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two to a byte, the even column
+ * in the low half.  A group of a row's columns shares a scale of one byte:
+ *   group_size 16: e4m3, s = e4m3(amax * g / 6), code = e2m1(x * g / s), value = code * s / g, with one float32 scale g of the
+ *                  tensor (device memory; NULL = 1; customarily 448 * 6 / the tensor's largest magnitude; 2^-100 <= g <= 2^100);
+ *   group_size 32: e8m0, s = 2^(floor(log2 amax) - 2) (at least 2^-127), code = e2m1(x / s), value = code * s; g must be NULL.
+ * Roundings are to nearest with ties to even and saturate; they are decided on the exact quotients.  A zero scale has zero codes;
+ * a group that holds a NaN or an infinity has the scale NaN (0x7f, 0xff) and zero codes.
+ * Scales lie in blocked order, in which the products read them: the scale of row r and group c is byte
+ *   ((r / 128) * GB + c / 4) * 512 + (r % 32) * 16 + (r / 32 % 4) * 4 + c % 4,   GB = ceil(hidden / group_size / 4),
+ * of ceil(rows / 128) * GB * 512 bytes.  Bytes of groups past the last are written as zeros, bytes of rows past the last are left
+ * as they were.  hidden % group_size == 0, hidden <= 2^20; every pointer 16-byte aligned.
+ * No counterpart in the reference's block-FP8 path, whose quantizers these stand beside.
+ *
+ * input [num_tokens, hidden] (bf16, fp16, fp32), output_q [num_tokens, hidden / 2] bytes.
+ */
+int sglb200_per_token_group_quant_fp4(const void* input, int in_dtype, void* output_q, void* output_s, const float* global_scale,
+                                      int64_t num_tokens, int64_t hidden, int group_size, void* stream);
+/* h = silu(x[:, :d]) * x[:, d:], unrounded in float32, quantised as above; input [rows, 2d] (bf16, fp16). */
+int sglb200_silu_and_mul_quant_fp4(const void* input, int dtype, void* output_q, void* output_s, const float* global_scale,
+                                   int64_t rows, int64_t d, int group_size, void* stream);
+/* output [num_tokens, hidden] (bf16, fp16, fp32) = code * s / g. */
+int sglb200_per_token_group_dequant_fp4(const void* input_q, const void* input_s, const float* global_scale, void* output,
+                                        int out_dtype, int64_t num_tokens, int64_t hidden, int group_size, void* stream);
+
+/*
  * Counting sort of flat topk_ids into block-padded expert segments; deterministic: within an expert,
  * entries keep ascending flat index.  Ids are shifted by +1 so that id -1 lands in bucket 0 and is
  * reported as expert -1; `num_experts` here is the bucket count, i.e. (model experts + 1), exactly

@@ -1,0 +1,133 @@
+// The 4-bit format and its conversions, shared by the fp4 kernels.
+//
+// A value is an e2m1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two to a byte, the even column in the low half.  A
+// group of a row's columns shares a scale: 16 columns an e4m3 one (beside one float32 scale of the whole tensor), or 32 columns a
+// power of two (e8m0).  Scales of the products' operands lie in blocked order, the order in which tensor memory takes them: blocks
+// of 128 rows x 4 groups, 512 bytes each, a block's rows r, r + 32, r + 64 and r + 96 side by side.
+#pragma once
+#include "common.cuh"
+
+namespace sglb200 {
+namespace fp4 {
+
+constexpr int kUnit = 16;         // columns that a thread of the elementwise kernels takes
+constexpr int kBlockBytes = 512;  // 128 rows x 4 groups of scales
+constexpr uint32_t kNanE4m3 = 0x7f, kNanE8m0 = 0xff;
+
+// Where the scale of (row, group) lies, with `group_blocks` blocks in a row.
+__host__ __device__ __forceinline__ int64_t scale_at(int64_t row, int group, int group_blocks) {
+  return ((row >> 7) * group_blocks + (group >> 2)) * kBlockBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (group & 3);
+}
+
+// n / d for n < 2^31 by a multiplication (d >= 1).
+struct FastDiv {
+  uint32_t d, mul, shift;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t div) : d(div), mul(0), shift(0) {
+    while ((1ull << shift) < div) ++shift;
+    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - div)) / div + 1);
+  }
+  __device__ __forceinline__ uint32_t quot(uint32_t n) const { return (__umulhi(mul, n) + n) >> shift; }
+};
+
+// (lo, hi) -> two codes, lo in bits 0-3; to nearest, ties to even, saturating.
+__device__ __forceinline__ uint32_t cvt_e2m1x2(float lo, float hi) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %2, %1;\n\t"
+      "cvt.u32.u8 %0, b;\n\t}"
+      : "=r"(r)
+      : "f"(lo), "f"(hi));
+  return r;
+}
+
+// Eight float32 -> eight codes.
+__device__ __forceinline__ uint32_t cvt_e2m1x8(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+
+// Eight codes -> four pairs of fp16 (exact), even columns in the low halves.
+__device__ __forceinline__ void cvt_f16x2_e2m1x8(uint32_t codes, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(codes));
+}
+
+// Two e4m3 codes (bits 0-7, 8-15) -> a pair of fp16 (exact; NaN stays NaN).
+__device__ __forceinline__ uint32_t cvt_f16x2_e4m3x2(uint32_t two) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 t;\n\t"
+      "cvt.u16.u32 t, %1;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, t;\n\t}"
+      : "=r"(r)
+      : "r"(two));
+  return r;
+}
+__device__ __forceinline__ float2 f16x2_to_f32(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
+
+// e8m0 code -> float32 (255 is NaN).
+__device__ __forceinline__ float e8m0_to_f32(uint32_t code) {
+  return __uint_as_float(code == kNanE8m0 ? 0x7fc00000u : code == 0 ? 0x00400000u : code << 23);
+}
+
+// The smallest e2m1 magnitude above each border between two neighbours is decided by the border itself: twice the border
+// between codes c and c + 1 (a multiple of 1/2 that float32 holds exactly), c in 0..6.
+__device__ __forceinline__ float e2m1_border(uint32_t c) {
+  const uint32_t quarters = c < 4 ? 2 * c + 1 : c == 4 ? 10 : c == 5 ? 14 : 20;  // 0.25 0.75 1.25 1.75 2.5 3.5 5
+  return 0.25f * (float)quarters;
+}
+
+// The scale of a group of 16: the e4m3 value nearest to amax * g / 6 (ties to even, saturating), decided on the exact product.
+// float32 alone would round amax * g / 6 onto a border it is only near to, which happens whenever g is a short number: the
+// quotient is therefore taken a little too small and a little too large, and where that matters the sign of the exact
+// amax * g - 6 * border, one fused multiply-add, decides.
+__device__ __forceinline__ uint32_t group_scale_e4m3(float amax, float g) {
+  const float v = amax * g * 0.16666667f;
+  const uint32_t two = cvt_e4m3x2(v * (1.0f - 0x1p-20f), v * (1.0f + 0x1p-20f));
+  uint32_t lo = two & 0xff;
+  const uint32_t hi = two >> 8;
+  if (lo != hi) {
+    const float2 f = f16x2_to_f32(cvt_f16x2_e4m3x2(two));
+    const float over = fmaf(amax, g, -3.0f * (f.x + f.y));
+    if (over > 0.f || (over == 0.f && (lo & 1))) lo = hi;
+  }
+  return lo;
+}
+
+// Codes of eight values x under scale s (not 0) and the tensor's scale g: e2m1 nearest to x * g / s, decided likewise.
+// `r_lo`, `r_hi`: g / s a little too small and too large.
+__device__ __forceinline__ uint32_t codes_x8(const float (&x)[8], float r_lo, float r_hi, float s, float g) {
+  float a[8], b[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a[i] = x[i] * r_lo, b[i] = x[i] * r_hi;
+  uint32_t lo = cvt_e2m1x8(a);
+  const uint32_t hi = cvt_e2m1x8(b);
+  if (lo != hi) {  // some value is within 2^-20 of a border
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t c = lo >> (4 * i) & 7;
+      if (c != (hi >> (4 * i) & 7)) {
+        const float over = fmaf(fabsf(x[i]), g, -e2m1_border(c) * s);
+        if (over > 0.f || (over == 0.f && (c & 1))) lo += 1u << (4 * i);
+      }
+    }
+  }
+  return lo;
+}
+
+}  // namespace fp4
+}  // namespace sglb200

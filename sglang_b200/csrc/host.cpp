@@ -26,6 +26,9 @@ namespace {
   X(sglb200_last_error)                  \
   X(sglb200_per_token_group_quant_fp8)   \
   X(sglb200_silu_and_mul_quant_fp8)      \
+  X(sglb200_per_token_group_quant_fp4)   \
+  X(sglb200_silu_and_mul_quant_fp4)      \
+  X(sglb200_per_token_group_dequant_fp4) \
   X(sglb200_gemm_workspace_bytes)        \
   X(sglb200_fp8_blockwise_scaled_mm)     \
   X(sglb200_block_fp8_linear_workspace_bytes) \
@@ -111,6 +114,9 @@ PyObject* pair(Tensor a, Tensor b) {
   return r;
 }
 
+// Whether the tensor's device is the current one: the runtime launches there, whatever the stream's device.
+bool here(const Tensor& t) { return t.get_device() == c10::cuda::current_device(); }
+
 constexpr float kFp8Max = 448.0f;
 
 // ---- quantizer ------------------------------------------------------------------------------------------------
@@ -172,6 +178,77 @@ PyObject* silu_mul_quant(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                                                       nr ? static_cast<const int32_t*>(nr->data_ptr()) : nullptr, stream_of(x));
     if (rc) return raise_last(rc);
     return pair(std::move(q), std::move(s));
+  });
+}
+
+// ---- 4-bit quantizers -----------------------------------------------------------------------------------------
+// One float32 on x's device, or absent; false when it is anything else.
+bool scalar_ok(PyObject* o, const Tensor& x, const float** value) {
+  *value = nullptr;
+  if (o == Py_None) return true;
+  const Tensor* t = cuda_contig(o);
+  if (t == nullptr || t->numel() != 1 || t->scalar_type() != at::kFloat || t->device() != x.device()) return false;
+  *value = static_cast<const float*>(t->data_ptr());
+  return true;
+}
+
+at::ScalarType fp4_scale_type(int64_t group) { return group == 32 ? at::kFloat8_e8m0fnu : at::kFloat8_e4m3fn; }
+
+// x [.., hidden] or [.., 2 hidden] -> (codes uint8 [.., hidden / 2], scales in blocked order)
+template <bool kSilu>
+PyObject* quant_fp4_any(PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 3) Py_RETURN_NONE;
+  const Tensor* xp = cuda_contig(args[0]);
+  const int64_t group = PyLong_AsLongLong(args[2]);
+  if (PyErr_Occurred()) return nullptr;
+  const float* g;
+  if (xp == nullptr || xp->dim() < 1 || !scalar_ok(args[1], *xp, &g) || !here(*xp)) Py_RETURN_NONE;
+  const Tensor& x = *xp;
+  const int dt = dtype_code(x.scalar_type());
+  const int64_t hidden = x.size(-1) / (kSilu ? 2 : 1);
+  if (dt < 0 || (kSilu && (dt > 1 || x.size(-1) % 2)) || hidden <= 0 || (group != 16 && group != 32) || hidden % group ||
+      x.numel() == 0)
+    Py_RETURN_NONE;
+  return guarded([&]() -> PyObject* {
+    const int64_t rows = x.numel() / x.size(-1);
+    c10::DimVector shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = hidden / 2;
+    Tensor q = make(shape, at::kByte, x.device());
+    Tensor s = make({(rows + 127) / 128 * 128, (hidden / group + 3) / 4 * 4}, fp4_scale_type(group), x.device());
+    const int rc = (kSilu ? abi.sglb200_silu_and_mul_quant_fp4 : abi.sglb200_per_token_group_quant_fp4)(
+        x.data_ptr(), dt, q.data_ptr(), s.data_ptr(), g, rows, hidden, (int)group, stream_of(x));
+    if (rc) return raise_last(rc);
+    return pair(std::move(q), std::move(s));
+  });
+}
+
+// quant_fp4(x [.., hidden], global_scale | None, group_size) -> (codes, scales)
+PyObject* quant_fp4(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return quant_fp4_any<false>(args, nargs); }
+// silu_mul_quant_fp4(x [.., 2 hidden], global_scale | None, group_size) -> (codes, scales)
+PyObject* silu_mul_quant_fp4(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return quant_fp4_any<true>(args, nargs); }
+
+// dequant_fp4(codes [.., hidden / 2], scales, global_scale | None, dtype) -> values [.., hidden]
+PyObject* dequant_fp4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 4) Py_RETURN_NONE;
+  const Tensor *q = cuda_contig(args[0]), *s = cuda_contig(args[1]);
+  const float* g;
+  if (!q || !s || q->dim() < 1 || s->dim() != 2 || !THPDtype_Check(args[3]) || !scalar_ok(args[2], *q, &g) || !here(*q)) Py_RETURN_NONE;
+  const at::ScalarType out_t = reinterpret_cast<THPDtype*>(args[3])->scalar_type;
+  const int dt = dtype_code(out_t);
+  const int64_t group = s->scalar_type() == at::kFloat8_e8m0fnu ? 32 : 16, hidden = q->size(-1) * 2;
+  if (dt < 0 || q->scalar_type() != at::kByte || s->scalar_type() != fp4_scale_type(group) || s->device() != q->device() ||
+      q->numel() == 0 || hidden % group || (g && group == 32))
+    Py_RETURN_NONE;
+  const int64_t rows = q->numel() / q->size(-1);
+  if (s->size(0) != (rows + 127) / 128 * 128 || s->size(1) != (hidden / group + 3) / 4 * 4) Py_RETURN_NONE;
+  return guarded([&]() -> PyObject* {
+    c10::DimVector shape(q->sizes().begin(), q->sizes().end());
+    shape.back() = hidden;
+    Tensor out = make(shape, out_t, q->device());
+    const int rc = abi.sglb200_per_token_group_dequant_fp4(q->data_ptr(), s->data_ptr(), g, out.data_ptr(), dt, rows, hidden,
+                                                           (int)group, stream_of(*q));
+    if (rc) return raise_last(rc);
+    return THPVariable_Wrap(std::move(out));
   });
 }
 
@@ -333,7 +410,7 @@ PyObject* fused_experts(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 PyMethodDef methods[] = {
     {"bind", bind, METH_O, "Bind the C ABI of the library at this path."},
 #define M(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-    M(quant), M(silu_mul_quant), M(linear), M(matmul), M(topk_softmax), M(fused_gate), M(fused_experts),
+    M(quant), M(silu_mul_quant), M(quant_fp4), M(silu_mul_quant_fp4), M(dequant_fp4), M(linear), M(matmul), M(topk_softmax), M(fused_gate), M(fused_experts),
 #undef M
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

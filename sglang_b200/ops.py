@@ -99,6 +99,117 @@ def per_token_group_quant_fp8(
 
 
 # --------------------------------------------------------------------------------------------
+# 4-bit floating point
+# --------------------------------------------------------------------------------------------
+
+_FP4_SCALE = {16: torch.float8_e4m3fn, 32: torch.float8_e8m0fnu}
+
+
+def _fp4_group(group_size: int, what: str) -> int:
+    if group_size not in _FP4_SCALE:
+        raise NotImplementedError(f"{what}: group_size must be 16 (e4m3 scales) or 32 (e8m0 scales), not {group_size}")
+    return int(group_size)
+
+
+def _scalar_f32(t: Optional[torch.Tensor], like: torch.Tensor, name: str) -> int:
+    if t is None:
+        return 0
+    if not t.is_cuda or t.dtype != torch.float32 or t.numel() != 1 or t.device != like.device:
+        raise RuntimeError(f"{name} must be one float32 on the device of the other tensors")
+    return t.data_ptr()
+
+
+def fp4_scale_shape(rows: int, hidden: int, group_size: int = 16) -> Tuple[int, int]:
+    """Shape of the scales of [rows, hidden] values in blocked order: whole blocks of 128 rows x 4 groups."""
+    return (rows + 127) // 128 * 128, (hidden // group_size + 3) // 4 * 4
+
+
+def fp4_blocked_scales(scales: torch.Tensor) -> torch.Tensor:
+    """Scales [rows, groups] in rows' order (as a checkpoint stores a weight's) -> blocked order, padded with zeros: what
+    the 4-bit products read.  Laid out once, when the weight is loaded."""
+    if scales.dim() != 2 or scales.dtype not in _FP4_SCALE.values():
+        raise RuntimeError("fp4_blocked_scales: scales must be float8_e4m3fn or float8_e8m0fnu [rows, groups]")
+    rows, groups = scales.shape
+    mb, gb = (rows + 127) // 128, (groups + 3) // 4
+    padded = torch.zeros(mb * 128, gb * 4, dtype=torch.uint8, device=scales.device)
+    padded[:rows, :groups] = scales.contiguous().view(torch.uint8)
+    return padded.view(mb, 4, 32, gb, 4).permute(0, 3, 2, 1, 4).reshape(mb * 128, gb * 4).view(scales.dtype)
+
+
+def _quant_fp4(x, global_scale, group_size, silu, what):
+    group = _fp4_group(group_size, what)
+    _cuda_contig(x, "input")
+    if x.dim() < 1 or x.shape[-1] == 0 or (silu and x.shape[-1] % 2):
+        raise RuntimeError(f"{what}: the last dimension is empty" + (" or odd" if silu else ""))
+    hidden = x.shape[-1] // (2 if silu else 1)
+    rows = x.numel() // x.shape[-1]
+    q = torch.empty(x.shape[:-1] + (hidden // 2,), device=x.device, dtype=torch.uint8)
+    s = torch.empty(fp4_scale_shape(rows, hidden, group), device=x.device, dtype=_FP4_SCALE[group])
+    g = _scalar_f32(global_scale, x, "global_scale")
+    fn = lib.sglb200_silu_and_mul_quant_fp4 if silu else lib.sglb200_per_token_group_quant_fp4
+    with torch.cuda.device(x.device):
+        check(fn(x.data_ptr(), _dt(x, _DT if not silu else (torch.bfloat16, torch.float16)), q.data_ptr(), s.data_ptr(), g, rows,
+                 hidden, group, _stream(x)))
+    return q, s
+
+
+def per_token_group_quant_fp4(
+    x: torch.Tensor, global_scale: Optional[torch.Tensor] = None, group_size: int = 16,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """x [..., hidden] -> (codes uint8 [..., hidden / 2], scales in blocked order, `fp4_scale_shape`).
+
+    `group_size` 16: s = e4m3(amax * global_scale / 6), code = e2m1(x * global_scale / s); `global_scale` is one float32 on
+    the device (None: 1), customarily 448 * 6 / the tensor's largest magnitude.  `group_size` 32: s = 2^(floor(log2 amax) - 2),
+    code = e2m1(x / s), no global scale.  A group that holds a NaN or an infinity gets the scale NaN."""
+    out = host.quant_fp4(x, global_scale, group_size)
+    return out if out is not None else _quant_fp4(x, global_scale, group_size, False, "per_token_group_quant_fp4")
+
+
+def silu_and_mul_quant_fp4(
+    x: torch.Tensor, global_scale: Optional[torch.Tensor] = None, group_size: int = 16,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """silu(x[..., :d]) * x[..., d:], unrounded in float32, quantised as `per_token_group_quant_fp4` does; x [..., 2d]."""
+    out = host.silu_mul_quant_fp4(x, global_scale, group_size)
+    return out if out is not None else _quant_fp4(x, global_scale, group_size, True, "silu_and_mul_quant_fp4")
+
+
+def _fp4_scales_ok(codes: torch.Tensor, scales: torch.Tensor, name: str) -> int:
+    """The group size that the type of `scales` says, once their shape fits codes [..., hidden / 2]."""
+    _cuda_contig(codes, name)
+    _cuda_contig(scales, f"{name}'s scales")
+    if codes.dtype != torch.uint8 or codes.dim() < 1 or codes.shape[-1] == 0:
+        raise RuntimeError(f"{name} must be uint8 [..., hidden / 2]")
+    group = next((g for g, t in _FP4_SCALE.items() if t == scales.dtype), None)
+    if group is None:
+        raise RuntimeError(f"{name}'s scales must be float8_e4m3fn (groups of 16) or float8_e8m0fnu (groups of 32)")
+    hidden = codes.shape[-1] * 2
+    want = fp4_scale_shape(codes.numel() // codes.shape[-1], hidden, group)
+    if hidden % group or tuple(scales.shape) != want or scales.device != codes.device:
+        raise RuntimeError(f"{name}'s scales have shape {tuple(scales.shape)}, expected {want} in blocked order")
+    return group
+
+
+def per_token_group_dequant_fp4(
+    codes: torch.Tensor, scales: torch.Tensor, global_scale: Optional[torch.Tensor] = None,
+    dtype: torch.dtype = torch.bfloat16,
+) -> torch.Tensor:
+    """The values code * s / global_scale [..., hidden] of codes [..., hidden / 2] with scales in blocked order."""
+    out = host.dequant_fp4(codes, scales, global_scale, dtype)
+    if out is not None:
+        return out
+    group = _fp4_scales_ok(codes, scales, "codes")
+    if dtype not in _DT:
+        raise RuntimeError(f"unsupported dtype {dtype}")
+    hidden = codes.shape[-1] * 2
+    out = torch.empty(codes.shape[:-1] + (hidden,), device=codes.device, dtype=dtype)
+    g = _scalar_f32(global_scale, codes, "global_scale")
+    with torch.cuda.device(codes.device):
+        check(lib.sglb200_per_token_group_dequant_fp4(codes.data_ptr(), scales.data_ptr(), g, out.data_ptr(), _DT[dtype],
+                                                      codes.numel() // codes.shape[-1], hidden, group, _stream(codes)))
+    return out
+
+
+# --------------------------------------------------------------------------------------------
 # activation / reduction / gather
 # --------------------------------------------------------------------------------------------
 

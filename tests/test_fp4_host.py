@@ -1,0 +1,93 @@
+"""What the 4-bit operators refuse, and their host-side pieces (no GPU needed)."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import fp4_oracle as F
+
+
+def _err():
+    from sglang_b200._lib import lib
+    return lib.sglb200_last_error().decode()
+
+
+QUANTIZERS = ["sglb200_per_token_group_quant_fp4", "sglb200_silu_and_mul_quant_fp4"]
+
+
+@pytest.mark.parametrize("name", QUANTIZERS)
+def test_quantizers_refuse(name):
+    from sglang_b200._lib import lib
+    fn, A = getattr(lib, name), 4096  # A: an aligned address that is never touched
+    assert fn(A, 0, A, A, None, 4, 64, 64, None) == -2 and "group_size" in _err()
+    assert fn(A, 0, A, A, None, 4, 72, 16, None) == -1 and "not divisible" in _err()
+    assert fn(A, 0, A, A, None, 4, 48, 32, None) == -1 and "not divisible" in _err()
+    assert fn(A, 0, A, A, None, 4, 0, 16, None) == -1
+    assert fn(A, 0, A, A, None, -1, 64, 16, None) == -1
+    assert fn(A, 0, A, A, None, 4, (1 << 20) + 32, 32, None) == -1 and "2^20" in _err()
+    assert fn(A, 0, A, A, A, 4, 64, 32, None) == -1 and "no global scale" in _err()
+    assert fn(A, 0, A, A, A + 2, 4, 64, 16, None) == -1 and "aligned" in _err()
+    assert fn(A, 3, A, A, None, 4, 64, 16, None) == -2 and "dtype" in _err()
+    assert fn(None, 0, A, A, None, 4, 64, 16, None) == -1 and "null" in _err()
+    assert fn(A + 8, 0, A, A, None, 4, 64, 16, None) == -1 and "16-byte" in _err()
+    assert fn(A, 0, A, A, None, 0, 64, 16, None) == 0  # no rows: nothing to do
+    if "silu" in name:
+        assert fn(A, 2, A, A, None, 4, 64, 16, None) == -2 and "dtype" in _err()
+
+
+def test_dequantizer_refuses():
+    from sglang_b200._lib import lib
+    fn, A = lib.sglb200_per_token_group_dequant_fp4, 4096
+    assert fn(A, A, None, A, 0, 4, 64, 8, None) == -2
+    assert fn(A, A, None, A, 0, 4, 40, 16, None) == -1
+    assert fn(A, A, A, A, 0, 4, 64, 32, None) == -1
+    assert fn(A, A, None, A, 5, 4, 64, 16, None) == -2
+    assert fn(A, None, None, A, 0, 4, 64, 16, None) == -1
+    assert fn(A, A, None, A + 4, 0, 4, 64, 16, None) == -1
+    assert fn(A, A, None, A, 0, 0, 64, 16, None) == 0
+
+
+def test_python_forms_refuse_cpu_tensors_and_bad_arguments():
+    from sglang_b200 import ops
+    x = torch.zeros(4, 64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.per_token_group_quant_fp4(x)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.silu_and_mul_quant_fp4(x)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.per_token_group_dequant_fp4(torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(128, 4).to(torch.float8_e4m3fn))
+    with pytest.raises(NotImplementedError, match="group_size"):
+        ops.per_token_group_quant_fp4(x, None, 128)
+    with pytest.raises(RuntimeError, match="float8"):
+        ops.fp4_blocked_scales(torch.zeros(4, 4))
+
+
+@pytest.mark.parametrize("rows,groups", [(1, 1), (3, 5), (128, 4), (129, 7), (300, 132)])
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.float8_e8m0fnu])
+def test_blocked_scales(rows, groups, dtype):
+    from sglang_b200 import ops
+    codes = np.random.default_rng(rows).integers(0, 255, size=(rows, groups)).astype(np.uint8)
+    got = ops.fp4_blocked_scales(torch.from_numpy(codes).view(dtype))
+    assert got.dtype == dtype and tuple(got.shape) == ops.fp4_scale_shape(rows, groups * 16)
+    got = got.view(torch.uint8).numpy()
+    assert np.array_equal(got, F.blocked(codes))
+    assert np.array_equal(F.unblocked(got, rows, groups), codes)
+
+
+def test_oracle_format():
+    """Known answers of the format: every code round-trips, ties go to the even mantissa, magnitudes saturate."""
+    x = np.array([[0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, -0.25, -0.75, 0.2500001, 4.99, 5.01, 6.9, 0.0, -6.0]])
+    codes, s = F.quantize(x * 1.0, 1.0, 16)
+    # amax 6.9 / 6 = 1.15 -> e4m3 1.125
+    assert s[0, 0] == 0x39
+    full = x.copy()
+    full[0, 13] = 6.0
+    codes, s = F.quantize(full, 1.0, 16)
+    assert s[0, 0] == 0x38
+    v = F.dequantize(codes, s, 16)[0]
+    assert v.tolist() == [0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0, 6.0, -0.0, -1.0, 0.5, 4.0, 6.0, 6.0, 0.0, -6.0]
+    codes, s = F.quantize(np.array([[7.9] + [1.0] * 31]), 1.0, 32)
+    assert s[0, 0] == 127 and F.dequantize(codes, s, 32)[0, 0] == 6.0
+    codes, s = F.quantize(np.array([[8.0] + [1.0] * 31]), 1.0, 32)
+    assert s[0, 0] == 128 and F.dequantize(codes, s, 32)[0, 0] == 8.0
+    t = torch.arange(0, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()
+    assert np.array_equal(t, F.E4M3)

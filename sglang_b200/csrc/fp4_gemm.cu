@@ -1,0 +1,266 @@
+// Products of 4-bit operands:  C[m, n] = out_t( alpha * sum_k a[m, k] * b[n, k] + bias[n] ),  a and b e2m1 codes times the scale of
+// their group, on tcgen05.mma.kind::mxf4nvf4, which takes the scales from tensor memory and applies them inside the MMA.
+//
+// fp4_rows_kernel: the weights on the M side (128 of their rows), NT activation rows on the N side, so that nothing is multiplied
+// for padding of few rows up to 128; K split over the CTAs of a cluster, which add their partial sums through distributed shared
+// memory in a fixed order.
+#include <algorithm>
+
+#include "fp4_gemm.cuh"
+
+namespace sglb200 {
+namespace fp4 {
+
+__device__ int g_fp4_status = 0;  // 0 ok, 1 = a pipeline wait expired
+
+constexpr int kRowsThreads = 192;  // four warps for the epilogue, one that loads, one that multiplies
+
+template <int kNT, int kG>
+struct RowsCfg {
+  static constexpr int NT = kNT, G = kG;
+  static constexpr uint32_t kTokBytes = NT * kBK / 2;
+  static constexpr uint32_t kScaleBytes = kStageBlocks<G> * kBlockBytes;  // of one operand
+  static constexpr uint32_t kStage = kOperandBytes + kTokBytes + 2 * kScaleBytes;
+  static constexpr uint32_t kPart = NT * kPartPitch * 4;
+  static constexpr int kStages = 104 * 1024 / kStage;  // two CTAs per SM
+  static constexpr uint32_t kRing = kStages * kStage > kPart ? kStages * kStage : kPart;
+  // tensor memory: the sums, then two sets of scales (weights', activations'), used in turn
+  static constexpr int kSet = 2 * kStageBlocks<G> * 4;
+  static constexpr int kUsed = NT + 2 * kSet;
+  static constexpr int kTmem = kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : 256;
+  static_assert(kStages >= 2 && kUsed <= 256);
+};
+
+struct RowsCtl {
+  uint64_t full[8], empty[8], acc_full;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+template <class Cfg>
+__global__ void __launch_bounds__(kRowsThreads, 2)
+    fp4_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Params p) {
+  constexpr int NT = Cfg::NT, G = Cfg::G, S = Cfg::kStages;
+  static_assert(S <= 8);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  RowsCtl* ctl = reinterpret_cast<RowsCtl*>(ring + Cfg::kRing);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int* abort_flag = &ctl->abort_flag;
+  const int splits = p.splits, rank = (int)(blockIdx.x % splits), tile = (int)(blockIdx.x / splits);
+  int m_tile, n_tile;
+  tile_coord(tile, p.tiles_m, p.tiles_n, p.group_m, m_tile, n_tile);
+  const int kb0 = (int)((int64_t)rank * p.kb_total / splits), kb1 = (int)((int64_t)(rank + 1) * p.kb_total / splits);
+  const uint32_t bar_full = ptx::smem_u32(ctl->full), bar_empty = ptx::smem_u32(ctl->empty), bar_acc = ptx::smem_u32(&ctl->acc_full);
+
+  if (tid == 0) {
+    for (int s = 0; s < S; ++s) ptx::mbar_init(bar_full + s * 8, 1), ptx::mbar_init(bar_empty + s * 8, 1);
+    ptx::mbar_init(bar_acc, 1);
+    ctl->abort_flag = 0;
+    ptx::mbar_fence_init();
+  }
+  // Tensor memory is taken once the kernel in front has ended, so that no CTA holds some while it waits for CTAs that need it;
+  // the kernel behind may start when every CTA has its own.
+  ptx::grid_dependency_wait();
+  if (warp == 5) {
+    ptx::tmem_alloc(ptx::smem_u32(&ctl->tmem_base), Cfg::kTmem);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  ptx::launch_dependents();
+  const uint32_t tmem = ctl->tmem_base;
+
+  if (warp == 4) {
+    if (ptx::elect_one()) {
+      const int x_block = (int)((int64_t)m_tile * NT / 128);
+      for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+        const int s = i % S;
+        if (i >= S && !FP4_WAIT(bar_empty + s * 8, ((i / S) & 1) ^ 1)) {
+          *abort_flag = 1;
+          break;
+        }
+        const uint32_t at = ptx::smem_u32(ring) + s * Cfg::kStage, bar = bar_full + s * 8;
+        const uint32_t scale_bytes = stage_blocks<G>(p, kb) * kBlockBytes;
+        ptx::mbar_arrive_expect_tx(bar, kOperandBytes + Cfg::kTokBytes + 2 * scale_bytes);
+        ptx::tma_load_3d(at, &map_w, bar, kb * (kBK / 2), n_tile * 128, 0);
+        ptx::tma_load_2d(at + kOperandBytes, &map_x, bar, kb * (kBK / 2), m_tile * NT);
+        const int64_t block = (int64_t)kb * kStageBlocks<G>;
+        const uint32_t sc = at + kOperandBytes + Cfg::kTokBytes;
+        bulk_load(sc, p.b_s + ((int64_t)n_tile * p.group_blocks + block) * kBlockBytes, scale_bytes, bar);
+        bulk_load(sc + Cfg::kScaleBytes, p.a_s + ((int64_t)x_block * p.group_blocks + block) * kBlockBytes, scale_bytes, bar);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 5) {
+    if (ptx::elect_one()) {
+      // rows 32 j .. of a block of activation scales have column j of each four
+      const uint32_t x_col = (uint32_t)(m_tile * NT % 128 / 32);
+      bool ok = true;
+      for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+        const int s = i % S;
+        ok = FP4_WAIT(bar_full + s * 8, (i / S) & 1);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        const uint32_t at = ptx::smem_u32(ring) + s * Cfg::kStage, sc = at + kOperandBytes + Cfg::kTokBytes;
+        const uint32_t sfw = tmem + NT + (i & 1) * Cfg::kSet, sfx = sfw + kStageBlocks<G> * 4;
+        const int blocks = stage_blocks<G>(p, kb), mmas = stage_mmas(p, kb);
+        for (int b = 0; b < blocks; ++b) {
+          copy_scales<1>(sfw + 4 * b, ptx::pack_f32x2(desc_lo(sc + b * kBlockBytes), kDescHiScale));
+          copy_scales<1>(sfx + 4 * b, ptx::pack_f32x2(desc_lo(sc + Cfg::kScaleBytes + b * kBlockBytes), kDescHiScale));
+        }
+        const uint32_t w_lo = desc_lo(at), x_lo = desc_lo(at + kOperandBytes);
+        for (int k = 0; k < mmas; ++k) {
+          const int b = G == 16 ? k : k >> 1;
+          mma<1, G>(tmem, ptx::pack_f32x2(w_lo + 2 * k, kDescHiTile), ptx::pack_f32x2(x_lo + 2 * k, kDescHiTile),
+                    idesc<G>(128, NT) | (G == 32 && (k & 1) ? kSecondHalf : 0u), sfw + 4 * b, sfx + 4 * b + x_col,
+                    i > 0 || k > 0 ? 1u : 0u);
+        }
+        ptx::mma_commit(bar_empty + s * 8);
+      }
+      if (!ok) *abort_flag = 1;
+      ptx::mma_commit(bar_acc);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------ sums out of tensor memory: lane = weight row, column = activation row ------------------------------
+    if (!FP4_WAIT(bar_acc, 0)) {
+      *abort_flag = 1;
+    } else {
+      ptx::tc_fence_after();
+      const float alpha = p.alpha ? *p.alpha : 1.0f;
+      float* part = reinterpret_cast<float*>(ring) + warp * 32 + lane;  // the operands have been consumed
+#pragma unroll
+      for (int c = 0; c < NT; c += 16) {
+        uint32_t r[16];
+        ptx::tmem_ld_32x16(tmem + ((uint32_t)(warp * 32) << 16) + c, r);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) part[(c + j) * kPartPitch] = alpha * __uint_as_float(r[j]);
+      }
+      ptx::tc_fence_before();
+    }
+  }
+
+  __syncwarp();
+  RowsParams rp{};
+  rp.C = p.C, rp.bias = p.bias, rp.M = p.M, rp.N = p.N, rp.splits = splits, rp.out_fp16 = p.out_fp16;
+  const RowsTile t{n_tile, m_tile * NT, NT, 0};
+  if (splits > 1) ptx::cluster_sync(); else __syncthreads();
+  if (ctl->abort_flag == 0) rows_cluster_sum<kMostClusterCtas>(rp, t, rank, ptx::smem_u32(ring), tid, kRowsThreads);
+  if (splits > 1) ptx::cluster_sync();  // no CTA leaves while another reads its shared memory
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (ctl->abort_flag != 0 && tid == 0) {
+    atomicExch(&g_fp4_status, 1);
+    // give copies that may still be in flight time to land before the CTA's shared memory is released
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000ll) {
+    }
+  }
+  __syncthreads();
+  if (warp == 5) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, Cfg::kTmem);
+  }
+}
+
+template <class Cfg>
+static int launch_rows(const void* A, const void* B, Params& p, cudaStream_t st) {
+  CUtensorMap mw, mx;
+  int rc = get_tensor_map(B, (uint64_t)p.K / 2, (uint64_t)p.N, 1, 128, 3, &mw);
+  if (rc) return rc;
+  rc = get_tensor_map(A, (uint64_t)p.K / 2, (uint64_t)p.M, 1, Cfg::NT, 2, &mx);
+  if (rc) return rc;
+  p.tiles_m = (int)((p.M + Cfg::NT - 1) / Cfg::NT), p.tiles_n = (int)((p.N + 127) / 128);
+  p.group_m = choose_group_m(p.M, p.K / 2, Cfg::NT);
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+  p.splits = rows_splits(tiles, p.kb_total, p.M, cluster_fits());
+  constexpr size_t kSmem = 1024 + Cfg::kRing + sizeof(RowsCtl);
+  static_assert(kSmem <= 113 * 1024);
+  auto kern = fp4_rows_kernel<Cfg>;
+  static thread_local bool attr_set[64] = {false};  // the opt-ins are per function and per device
+  int dev = 0;
+  SGLB_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    SGLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
+    SGLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  SGLB_REQUIRE(tiles * p.splits < (1ll << 31), "fp4_scaled_mm: %lld tiles are too many", (long long)tiles);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * p.splits), 1, 1);
+  cfg.blockDim = dim3(kRowsThreads, 1, 1);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)p.splits, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  SGLB_CUDA(cudaLaunchKernelEx(&cfg, kern, mw, mx, p));
+  return SGLB200_OK;
+}
+
+template <int G>
+static int scaled_mm(const void* A, const void* B, Params& p, cudaStream_t st) {
+  if (p.M <= 16) return launch_rows<RowsCfg<16, G>>(A, B, p, st);
+  if (p.M <= 32) return launch_rows<RowsCfg<32, G>>(A, B, p, st);
+  if (p.M <= 64) return launch_rows<RowsCfg<64, G>>(A, B, p, st);
+  return launch_rows<RowsCfg<128, G>>(A, B, p, st);
+}
+
+}  // namespace fp4
+
+int fp4_gemm_status() {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, fp4::g_fp4_status, sizeof(int)) != cudaSuccess) return -1;
+  return v;
+}
+int fp4_gemm_status_clear() {
+  const int zero = 0;
+  SGLB_CUDA(cudaMemcpyToSymbol(fp4::g_fp4_status, &zero, sizeof(int)));
+  return SGLB200_OK;
+}
+
+}  // namespace sglb200
+
+using namespace sglb200;
+
+extern "C" {
+
+int64_t sglb200_group_fp4_workspace_bytes(int64_t M, int64_t N, int64_t K) { return 0; }
+
+int sglb200_group_fp4_scaled_mm(const void* A, const void* B, const void* a_s, const void* b_s, const float* alpha, void* C,
+                                const void* bias, int64_t M, int64_t N, int64_t K, int group_size, int out_dtype, void* workspace,
+                                int64_t workspace_bytes, void* stream) {
+  if (group_size != 16 && group_size != 32)
+    return fail(SGLB200_E_UNSUPPORTED, "group_fp4_scaled_mm: group_size %d is neither 16 nor 32", group_size);
+  if (out_dtype != 0 && out_dtype != 1)
+    return fail(SGLB200_E_UNSUPPORTED, "group_fp4_scaled_mm: output dtype must be bfloat16 or float16");
+  SGLB_REQUIRE(M >= 0 && N > 0 && K > 0, "group_fp4_scaled_mm: M %lld, N %lld, K %lld", (long long)M, (long long)N, (long long)K);
+  SGLB_REQUIRE(K % 32 == 0 && N % 8 == 0, "group_fp4_scaled_mm: K (%lld) must be divisible by 32 and N (%lld) by 8", (long long)K,
+               (long long)N);
+  SGLB_REQUIRE(M < (1ll << 31) - 256 && N < (1ll << 31) - 256 && K <= 1 << 20, "group_fp4_scaled_mm: M %lld, N %lld or K %lld is too large",
+               (long long)M, (long long)N, (long long)K);
+  if (M == 0) return SGLB200_OK;
+  SGLB_REQUIRE(A && B && a_s && b_s && C, "group_fp4_scaled_mm: null pointer");
+  SGLB_REQUIRE(aligned16(A) && aligned16(B) && aligned16(a_s) && aligned16(b_s) && aligned16(C) && aligned16(bias),
+               "group_fp4_scaled_mm: pointers must be 16-byte aligned");
+  SGLB_REQUIRE(((uintptr_t)alpha & 3) == 0, "group_fp4_scaled_mm: alpha is not aligned to 4 bytes");
+  fp4::Params p{};
+  p.a_s = static_cast<const uint8_t*>(a_s), p.b_s = static_cast<const uint8_t*>(b_s);
+  p.alpha = alpha, p.C = C, p.bias = bias;
+  p.M = M, p.N = N, p.K = K;
+  p.group_blocks = (int)((K / group_size + 3) / 4), p.kb_total = (int)((K + fp4::kBK - 1) / fp4::kBK);
+  p.out_fp16 = out_dtype;
+  p.wait_probes = g_gemm_wait_probes;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return group_size == 16 ? fp4::scaled_mm<16>(A, B, p, st) : fp4::scaled_mm<32>(A, B, p, st);
+}
+
+}  // extern "C"

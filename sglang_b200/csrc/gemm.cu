@@ -1683,7 +1683,8 @@ using namespace sglb200;
 extern "C" int sglb200_gemm_status_clear(void) {
   const int zero = 0;
   SGLB_CUDA(cudaMemcpyToSymbol(g_gemm_status, &zero, sizeof(int)));
-  const int rc = rows_gemm_status_clear();
+  int rc = rows_gemm_status_clear();
+  if (rc == SGLB200_OK) rc = fp4_gemm_status_clear();
   return rc != SGLB200_OK ? rc : small_linear_status_clear();
 }
 
@@ -1691,6 +1692,7 @@ extern "C" int sglb200_gemm_status(void) {
   int v = 0;
   if (cudaMemcpyFromSymbol(&v, g_gemm_status, sizeof(int)) != cudaSuccess) return -1;
   if (v == 0) v = rows_gemm_status();
+  if (v == 0) v = fp4_gemm_status();
   return v != 0 ? v : small_linear_status();
 }
 

@@ -108,6 +108,10 @@ int small_linear(const void* x, int dtype, const void* B, const float* b_s, void
 int small_linear_status();
 int small_linear_status_clear();
 
+// fp4_gemm.cu: status word of its kernels (0 ok, 1 a wait expired, -1 not readable), and its reset.
+int fp4_gemm_status();
+int fp4_gemm_status_clear();
+
 // gemm_rows.cu: status word of its kernels (0 ok, 1 a wait expired, -1 not readable), and its reset.
 int rows_gemm_status();
 int rows_gemm_status_clear();

@@ -29,6 +29,8 @@ namespace {
   X(sglb200_per_token_group_quant_fp4)   \
   X(sglb200_silu_and_mul_quant_fp4)      \
   X(sglb200_per_token_group_dequant_fp4) \
+  X(sglb200_group_fp4_workspace_bytes)   \
+  X(sglb200_group_fp4_scaled_mm)         \
   X(sglb200_gemm_workspace_bytes)        \
   X(sglb200_fp8_blockwise_scaled_mm)     \
   X(sglb200_block_fp8_linear_workspace_bytes) \
@@ -194,6 +196,15 @@ bool scalar_ok(PyObject* o, const Tensor& x, const float** value) {
 
 at::ScalarType fp4_scale_type(int64_t group) { return group == 32 ? at::kFloat8_e8m0fnu : at::kFloat8_e4m3fn; }
 
+// Codes [.., K / 2] of `rows` rows with scales in blocked order; the group size, or 0 when it is anything else.
+int64_t fp4_group(const Tensor* q, const Tensor* s) {
+  if (!q || !s || q->dim() < 1 || s->dim() != 2 || q->scalar_type() != at::kByte || q->numel() == 0 || s->device() != q->device()) return 0;
+  const int64_t group = s->scalar_type() == at::kFloat8_e8m0fnu ? 32 : s->scalar_type() == at::kFloat8_e4m3fn ? 16 : 0;
+  const int64_t hidden = q->size(-1) * 2, rows = q->numel() / q->size(-1);
+  if (!group || hidden % group || s->size(0) != (rows + 127) / 128 * 128 || s->size(1) != (hidden / group + 3) / 4 * 4) return 0;
+  return group;
+}
+
 // x [.., hidden] or [.., 2 hidden] -> (codes uint8 [.., hidden / 2], scales in blocked order)
 template <bool kSilu>
 PyObject* quant_fp4_any(PyObject* const* args, Py_ssize_t nargs) {
@@ -231,16 +242,13 @@ PyObject* silu_mul_quant_fp4(PyObject*, PyObject* const* args, Py_ssize_t nargs)
 PyObject* dequant_fp4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 4) Py_RETURN_NONE;
   const Tensor *q = cuda_contig(args[0]), *s = cuda_contig(args[1]);
+  const int64_t group = fp4_group(q, s);
   const float* g;
-  if (!q || !s || q->dim() < 1 || s->dim() != 2 || !THPDtype_Check(args[3]) || !scalar_ok(args[2], *q, &g) || !here(*q)) Py_RETURN_NONE;
+  if (!group || !THPDtype_Check(args[3]) || !scalar_ok(args[2], *q, &g) || !here(*q) || (g && group == 32)) Py_RETURN_NONE;
   const at::ScalarType out_t = reinterpret_cast<THPDtype*>(args[3])->scalar_type;
   const int dt = dtype_code(out_t);
-  const int64_t group = s->scalar_type() == at::kFloat8_e8m0fnu ? 32 : 16, hidden = q->size(-1) * 2;
-  if (dt < 0 || q->scalar_type() != at::kByte || s->scalar_type() != fp4_scale_type(group) || s->device() != q->device() ||
-      q->numel() == 0 || hidden % group || (g && group == 32))
-    Py_RETURN_NONE;
-  const int64_t rows = q->numel() / q->size(-1);
-  if (s->size(0) != (rows + 127) / 128 * 128 || s->size(1) != (hidden / group + 3) / 4 * 4) Py_RETURN_NONE;
+  if (dt < 0) Py_RETURN_NONE;
+  const int64_t hidden = q->size(-1) * 2, rows = q->numel() / q->size(-1);
   return guarded([&]() -> PyObject* {
     c10::DimVector shape(q->sizes().begin(), q->sizes().end());
     shape.back() = hidden;
@@ -328,6 +336,33 @@ PyObject* matmul(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
+// matmul_fp4(A [.., K/2], B [N, K/2], As, Bs, alpha | None, out_dtype, bias | None) -> [.., N]
+PyObject* matmul_fp4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 7) Py_RETURN_NONE;
+  const Tensor *a = cuda_contig(args[0]), *b = cuda_contig(args[1]), *as = cuda_contig(args[2]), *bs = cuda_contig(args[3]), *bias;
+  const int64_t group = fp4_group(a, as);
+  const float* alpha;
+  if (!group || fp4_group(b, bs) != group || b->dim() != 2 || b->size(1) != a->size(-1) || b->device() != a->device() ||
+      !THPDtype_Check(args[5]) || !scalar_ok(args[4], *a, &alpha) || !here(*a))
+    Py_RETURN_NONE;
+  const at::ScalarType out_t = reinterpret_cast<THPDtype*>(args[5])->scalar_type;
+  const int dt = dtype_code(out_t);
+  const int64_t K = a->size(-1) * 2, N = b->size(0), M = a->numel() / a->size(-1);
+  if (dt < 0 || dt > 1 || !bias_ok(args[6], N, out_t, &bias) || (bias && bias->device() != a->device())) Py_RETURN_NONE;
+  return guarded([&]() -> PyObject* {
+    const int64_t scratch = abi.sglb200_group_fp4_workspace_bytes(M, N, K);
+    c10::DimVector shape(a->sizes().begin(), a->sizes().end());
+    shape.back() = N;
+    Tensor out = make(shape, out_t, a->device()), mem;
+    if (scratch) mem = workspace(scratch, a->device());
+    const int rc = abi.sglb200_group_fp4_scaled_mm(a->data_ptr(), b->data_ptr(), as->data_ptr(), bs->data_ptr(), alpha, out.data_ptr(),
+                                                   bias ? bias->data_ptr() : nullptr, M, N, K, (int)group, dt,
+                                                   scratch ? mem.data_ptr() : nullptr, scratch, stream_of(*a));
+    if (rc) return raise_last(rc);
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
 // ---- routing --------------------------------------------------------------------------------------------------
 // topk_softmax(logits [T, E], k, renormalize) -> (weights, ids)
 PyObject* topk_softmax(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -410,7 +445,7 @@ PyObject* fused_experts(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 PyMethodDef methods[] = {
     {"bind", bind, METH_O, "Bind the C ABI of the library at this path."},
 #define M(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-    M(quant), M(silu_mul_quant), M(quant_fp4), M(silu_mul_quant_fp4), M(dequant_fp4), M(linear), M(matmul), M(topk_softmax), M(fused_gate), M(fused_experts),
+    M(quant), M(silu_mul_quant), M(quant_fp4), M(silu_mul_quant_fp4), M(dequant_fp4), M(linear), M(matmul), M(matmul_fp4), M(topk_softmax), M(fused_gate), M(fused_experts),
 #undef M
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

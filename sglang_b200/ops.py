@@ -521,6 +521,41 @@ def w8a8_block_fp8_matmul(
     return C
 
 
+def w4a4_group_fp4_matmul(
+    A: torch.Tensor, B: torch.Tensor, As: torch.Tensor, Bs: torch.Tensor, alpha: Optional[torch.Tensor] = None,
+    output_dtype: torch.dtype = torch.bfloat16, bias: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """alpha * (A @ B.T) + bias of 4-bit operands: A [..., K / 2], B [N, K / 2] codes, As and Bs their scales in blocked order
+    (`per_token_group_quant_fp4`, `fp4_blocked_scales`), both of groups of 16 or both of 32.  `alpha`: one float32 on the device,
+    1 / (A's global scale * B's); None: 1.  K % 32 == 0, N % 8 == 0."""
+    C = host.matmul_fp4(A, B, As, Bs, alpha, output_dtype, bias)
+    if C is not None:
+        return C
+    if output_dtype not in (torch.bfloat16, torch.float16):
+        raise RuntimeError("output dtype must be bfloat16 or float16")
+    group = _fp4_scales_ok(A, As, "A")
+    if _fp4_scales_ok(B, Bs, "B") != group:
+        raise RuntimeError("A and B have different group sizes")
+    if B.dim() != 2 or B.shape[1] != A.shape[-1] or B.device != A.device:
+        raise RuntimeError("B must be [N, K / 2] with K matching A, on A's device")
+    K, N = A.shape[-1] * 2, B.shape[0]
+    M = A.numel() // A.shape[-1]
+    C = torch.empty(A.shape[:-1] + (N,), device=A.device, dtype=output_dtype)
+    a = _scalar_f32(alpha, A, "alpha")
+    if bias is not None:
+        bias = bias.to(output_dtype).contiguous()
+        if not bias.is_cuda or bias.device != A.device or bias.numel() != N:
+            raise RuntimeError(f"bias must be {N} values on A's device")
+    ws_bytes = lib.sglb200_group_fp4_workspace_bytes(M, N, K)
+    with torch.cuda.device(A.device):
+        ws = torch.empty(ws_bytes, device=A.device, dtype=torch.uint8) if ws_bytes else None
+        check(lib.sglb200_group_fp4_scaled_mm(
+            A.data_ptr(), B.data_ptr(), As.data_ptr(), Bs.data_ptr(), a, C.data_ptr(),
+            bias.data_ptr() if bias is not None else None, M, N, K, group, 0 if output_dtype == torch.bfloat16 else 1,
+            ws.data_ptr() if ws is not None else None, ws_bytes, _stream(A)))
+    return C
+
+
 def grouped_block_fp8_matmul(
     A: torch.Tensor, As: torch.Tensor, B: torch.Tensor, Bs: torch.Tensor, sorted_token_ids: torch.Tensor,
     expert_ids: torch.Tensor, num_rows: torch.Tensor, *, numel: int, scatter: bool,

@@ -91,3 +91,24 @@ def test_oracle_format():
     assert s[0, 0] == 128 and F.dequantize(codes, s, 32)[0, 0] == 8.0
     t = torch.arange(0, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()
     assert np.array_equal(t, F.E4M3)
+
+
+def test_product_refuses():
+    from sglang_b200._lib import lib
+    A = 4096
+
+    def call(M=4, N=16, K=64, group=16, dt=0, a=A, b=A, sa=A, sb=A, alpha=None, c=A, bias=None):
+        return lib.sglb200_group_fp4_scaled_mm(a, b, sa, sb, alpha, c, bias, M, N, K, group, dt, None, 0, None)
+
+    assert call(group=64) == -2 and "group_size" in _err()
+    assert call(dt=2) == -2 and "output dtype" in _err()
+    assert call(K=48) == -1 and "divisible" in _err()
+    assert call(N=12) == -1 and "divisible" in _err()
+    assert call(K=0) == -1 and call(N=0) == -1 and call(M=-1) == -1
+    assert call(K=(1 << 20) + 32) == -1 and "too large" in _err()
+    assert call(M=(1 << 31)) == -1 and "too large" in _err()
+    assert call(sa=None) == -1 and "null" in _err()
+    assert call(c=A + 8) == -1 and "16-byte" in _err()
+    assert call(bias=A + 2) == -1 and "16-byte" in _err()
+    assert call(alpha=A + 1) == -1 and "alpha" in _err()
+    assert call(M=0) == 0

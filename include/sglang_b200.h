@@ -133,6 +133,26 @@ int sglb200_group_fp4_scaled_mm(const void* A, const void* B, const void* a_s, c
                                 int64_t workspace_bytes, void* stream);
 
 /*
+ * The routed experts of a few tokens with 4-bit weights (groups of 16) and 16-bit activations, in two launches:
+ *   h[t, j]  = silu(a13[e] * G_e x[t]) * (a13[e] * U_e x[t]),  e = topk_ids[t, j]
+ *   out[t]   = factor * sum_j topk_weights[t, j] * a2[e] * W2_e h[t, j]
+ * x, out [tokens, hidden] (dtype 0 bf16, 1 fp16).  w13 [E, 2 * intermediate, hidden / 2] codes (G_e's rows, then U_e's), w2 [E, hidden,
+ * intermediate / 2]; their scales e4m3 in rows' order, as a checkpoint stores them, [E, rows, columns / 16].  w13_alpha, w2_alpha: a
+ * float32 per expert (1 / the global scale of its weights), NULL = 1.  topk_ids int32 [tokens, topk]; an id outside [0, E) (an expert
+ * of another rank) contributes nothing, the same id twice in a row counts twice.  Activations are not quantised: products with weights are exact in
+ * fp16 (bf16 activations under a power of two per row; what is below 2^-28 of a row's largest magnitude is rounded to 2^-39 of
+ * it), sums are float32, h is rounded to 11 bits for the second product, the output once.
+ * tokens * topk <= 1024, E <= 1024, hidden and intermediate divisible by 32; pointers 16-byte aligned.
+ * workspace: device scratch of at least sglb200_fused_experts_fp4_workspace_bytes, 16-byte aligned, needs no initialisation.
+ * Stands beside sglb200_fused_experts; no counterpart in the reference's block-FP8 path.
+ */
+int64_t sglb200_fused_experts_fp4_workspace_bytes(int64_t tokens, int64_t topk, int64_t hidden, int64_t intermediate);
+int sglb200_fused_experts_fp4(const void* x, int dtype, const void* w13, const void* w13_scale, const float* w13_alpha, const void* w2,
+                              const void* w2_scale, const float* w2_alpha, const float* topk_weights, const int32_t* topk_ids, void* out,
+                              int64_t tokens, int64_t topk, int num_experts, int64_t hidden, int64_t intermediate, float factor,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Counting sort of flat topk_ids into block-padded expert segments; deterministic: within an expert,
  * entries keep ascending flat index.  Ids are shifted by +1 so that id -1 lands in bucket 0 and is
  * reported as expert -1; `num_experts` here is the bucket count, i.e. (model experts + 1), exactly

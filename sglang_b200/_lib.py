@@ -35,6 +35,8 @@ SIGNATURES = {
     "sglb200_per_token_group_dequant_fp4": (_i32, [_vp, _vp, _vp, _vp, _i32, _i64, _i64, _i32, _vp]),
     "sglb200_group_fp4_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "sglb200_group_fp4_scaled_mm": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _i64, _vp]),
+    "sglb200_fused_experts_fp4_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "sglb200_fused_experts_fp4": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i64, _i64, _f32, _vp, _i64, _vp]),
     "sglb200_moe_align_workspace_bytes": (_i64, [_i64, _i32]),
     "sglb200_moe_align_block_size": (_i32, [_vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _i64, _vp]),
     "sglb200_moe_align_set_cooperative": (None, [_i32]),

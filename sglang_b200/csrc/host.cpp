@@ -31,6 +31,8 @@ namespace {
   X(sglb200_per_token_group_dequant_fp4) \
   X(sglb200_group_fp4_workspace_bytes)   \
   X(sglb200_group_fp4_scaled_mm)         \
+  X(sglb200_fused_experts_fp4_workspace_bytes) \
+  X(sglb200_fused_experts_fp4)           \
   X(sglb200_gemm_workspace_bytes)        \
   X(sglb200_fp8_blockwise_scaled_mm)     \
   X(sglb200_block_fp8_linear_workspace_bytes) \
@@ -442,10 +444,57 @@ PyObject* fused_experts(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
+// Experts' 4-bit weights [E, n, k / 2] with e4m3 scales [E, n, k / 16] in rows' order.
+bool experts_fp4_ok(const Tensor* w, const Tensor* s) {
+  return w && s && w->dim() == 3 && s->dim() == 3 && w->scalar_type() == at::kByte && s->scalar_type() == at::kFloat8_e4m3fn &&
+         s->size(0) == w->size(0) && s->size(1) == w->size(1) && s->size(2) * 8 == w->size(2) && s->device() == w->device();
+}
+
+// One float32 per expert on x's device, or absent.
+bool factors_ok(PyObject* o, int64_t n, const Tensor& x, const float** value) {
+  *value = nullptr;
+  if (o == Py_None) return true;
+  const Tensor* t = cuda_contig(o);
+  if (t == nullptr || t->numel() != n || t->scalar_type() != at::kFloat || t->device() != x.device()) return false;
+  *value = static_cast<const float*>(t->data_ptr());
+  return true;
+}
+
+// fused_experts_fp4(x [T, H] 16-bit, w13, w2, w13_scale, w2_scale, weights [T, k] f32, ids [T, k] i32, w13_alpha | None,
+//                   w2_alpha | None, factor) -> [T, H]
+PyObject* fused_experts_fp4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 10) Py_RETURN_NONE;
+  const Tensor *xp = cuda_contig(args[0]), *w1 = cuda_contig(args[1]), *w2 = cuda_contig(args[2]), *s1 = cuda_contig(args[3]),
+               *s2 = cuda_contig(args[4]), *wt = cuda_contig(args[5]), *id = cuda_contig(args[6]);
+  const double factor = PyFloat_AsDouble(args[9]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!xp || !wt || !id || !experts_fp4_ok(w1, s1) || !experts_fp4_ok(w2, s2) || !here(*xp)) Py_RETURN_NONE;
+  const Tensor& x = *xp;
+  const int dt = dtype_code(x.scalar_type());
+  if (dt < 0 || dt > 1 || x.dim() != 2 || id->dim() != 2 || id->scalar_type() != at::kInt || wt->scalar_type() != at::kFloat ||
+      wt->sizes() != id->sizes() || id->size(0) != x.size(0) || w1->device() != x.device() || w2->device() != x.device() ||
+      id->device() != x.device() || wt->device() != x.device())
+    Py_RETURN_NONE;
+  const int64_t T = x.size(0), H = x.size(1), E = w1->size(0), I = w1->size(1) / 2, k = id->size(1);
+  const float *a1, *a2;
+  if (T == 0 || k == 0 || w1->size(1) % 2 || w1->size(2) * 2 != H || w2->size(0) != E || w2->size(1) != H || w2->size(2) * 2 != I ||
+      !factors_ok(args[7], E, x, &a1) || !factors_ok(args[8], E, x, &a2))
+    Py_RETURN_NONE;
+  return guarded([&]() -> PyObject* {
+    const int64_t bytes = abi.sglb200_fused_experts_fp4_workspace_bytes(T, k, H, I);
+    Tensor out = make({T, H}, x.scalar_type(), x.device()), mem = workspace(bytes, x.device());
+    const int rc = abi.sglb200_fused_experts_fp4(x.data_ptr(), dt, w1->data_ptr(), s1->data_ptr(), a1, w2->data_ptr(), s2->data_ptr(), a2,
+                                                 static_cast<const float*>(wt->data_ptr()), static_cast<const int32_t*>(id->data_ptr()),
+                                                 out.data_ptr(), T, k, (int)E, H, I, (float)factor, mem.data_ptr(), bytes, stream_of(x));
+    if (rc) return raise_last(rc);
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
 PyMethodDef methods[] = {
     {"bind", bind, METH_O, "Bind the C ABI of the library at this path."},
 #define M(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-    M(quant), M(silu_mul_quant), M(quant_fp4), M(silu_mul_quant_fp4), M(dequant_fp4), M(linear), M(matmul), M(matmul_fp4), M(topk_softmax), M(fused_gate), M(fused_experts),
+    M(quant), M(silu_mul_quant), M(quant_fp4), M(silu_mul_quant_fp4), M(dequant_fp4), M(linear), M(matmul), M(matmul_fp4), M(topk_softmax), M(fused_gate), M(fused_experts), M(fused_experts_fp4),
 #undef M
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

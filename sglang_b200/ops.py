@@ -583,6 +583,64 @@ def grouped_block_fp8_matmul(
     return out
 
 
+def fused_experts_fp4(
+    hidden_states: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, w13_scale: torch.Tensor, w2_scale: torch.Tensor,
+    topk_weights: torch.Tensor, topk_ids: torch.Tensor, w13_alpha: Optional[torch.Tensor] = None,
+    w2_alpha: Optional[torch.Tensor] = None, routed_scaling_factor: float = 1.0,
+) -> torch.Tensor:
+    """The routed experts of a few tokens (at most 1024 tokens x experts a token), 4-bit weights and 16-bit activations:
+
+        h   = silu(w13_alpha[e] * G_e x) * (w13_alpha[e] * U_e x)
+        out = routed_scaling_factor * sum over a token's experts of topk_weights * w2_alpha[e] * W2_e h
+
+    hidden_states [T, H] bf16 or fp16; w13 uint8 [E, 2I, H / 2] (G_e's rows, then U_e's), w2 uint8 [E, H, I / 2]; their scales
+    float8_e4m3fn in rows' order, [E, 2I, H / 16] and [E, H, I / 16]; topk_weights and topk_ids [T, k].  An id outside
+    [0, E) contributes nothing.  The alphas are float32 [E] (None: 1).  H and I divisible by 32."""
+    if topk_ids.dtype != torch.int32:  # (an id that does not fit an int32 names no expert)
+        topk_ids = topk_ids.clamp(-1, 2**31 - 1).to(torch.int32)
+    if topk_weights.dtype != torch.float32:
+        topk_weights = topk_weights.float()
+    out = host.fused_experts_fp4(hidden_states, w13, w2, w13_scale, w2_scale, topk_weights, topk_ids, w13_alpha, w2_alpha,
+                                 routed_scaling_factor)
+    if out is not None:
+        return out
+    x = hidden_states
+    for t, n in ((x, "hidden_states"), (w13, "w13"), (w2, "w2"), (w13_scale, "w13_scale"), (w2_scale, "w2_scale"),
+                 (topk_weights, "topk_weights"), (topk_ids, "topk_ids")):
+        _cuda_contig(t, n)
+        if t.device != x.device:
+            raise RuntimeError(f"{n} is on another device than hidden_states")
+    if x.dim() != 2 or w13.dim() != 3 or w2.dim() != 3 or w13.dtype != torch.uint8 or w2.dtype != torch.uint8:
+        raise RuntimeError("fused_experts_fp4: hidden_states [T, H], w13 uint8 [E, 2I, H / 2], w2 uint8 [E, H, I / 2]")
+    T, H = x.shape
+    E, rows, _ = w13.shape
+    I = rows // 2
+    if rows % 2 or w13.shape[2] * 2 != H or tuple(w2.shape) != (E, H, I // 2) or I % 2:
+        raise RuntimeError(f"fused_experts_fp4: w13 {tuple(w13.shape)} and w2 {tuple(w2.shape)} do not fit {H} columns")
+    for w, s, n in ((w13, w13_scale, "w13_scale"), (w2, w2_scale, "w2_scale")):
+        if s.dtype != torch.float8_e4m3fn or tuple(s.shape) != (E, w.shape[1], w.shape[2] // 8):
+            raise RuntimeError(f"{n} must be float8_e4m3fn {(E, w.shape[1], w.shape[2] // 8)} in rows' order")
+    if topk_ids.dim() != 2 or topk_ids.shape[0] != T or topk_weights.shape != topk_ids.shape:
+        raise RuntimeError("fused_experts_fp4: topk_weights and topk_ids must be [T, k]")
+    for a, n in ((w13_alpha, "w13_alpha"), (w2_alpha, "w2_alpha")):
+        if a is not None and (not a.is_cuda or a.device != x.device or not a.is_contiguous() or a.dtype != torch.float32 or a.numel() != E):
+            raise RuntimeError(f"{n} must be {E} contiguous float32 on the device of hidden_states")
+    k = topk_ids.shape[1]
+    out = torch.empty_like(x)
+    if T == 0:
+        return out
+    if k == 0:
+        return out.zero_()
+    bytes_ = lib.sglb200_fused_experts_fp4_workspace_bytes(T, k, H, I)
+    with torch.cuda.device(x.device):
+        ws = torch.empty(bytes_, device=x.device, dtype=torch.uint8)
+        check(lib.sglb200_fused_experts_fp4(
+            x.data_ptr(), _dt(x), w13.data_ptr(), w13_scale.data_ptr(), w13_alpha.data_ptr() if w13_alpha is not None else None,
+            w2.data_ptr(), w2_scale.data_ptr(), w2_alpha.data_ptr() if w2_alpha is not None else None, topk_weights.data_ptr(),
+            topk_ids.data_ptr(), out.data_ptr(), T, k, E, H, I, float(routed_scaling_factor), ws.data_ptr(), bytes_, _stream(x)))
+    return out
+
+
 def gemm_status() -> int:
     """0, or 1 if a pipeline wait inside a GEMM kernel expired since the library was loaded (synchronises)."""
     return lib.sglb200_gemm_status()

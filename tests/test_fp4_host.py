@@ -112,3 +112,28 @@ def test_product_refuses():
     assert call(bias=A + 2) == -1 and "16-byte" in _err()
     assert call(alpha=A + 1) == -1 and "alpha" in _err()
     assert call(M=0) == 0
+
+
+def test_experts_refuse():
+    from sglang_b200._lib import lib
+    A = 4096
+    size = lib.sglb200_fused_experts_fp4_workspace_bytes
+
+    def call(T=2, k=2, E=8, H=256, I=128, dt=0, x=A, w13=A, s13=A, a13=None, w2=A, s2=A, a2=None, w=A, ids=A, out=A, ws=A, ws_bytes=None):
+        if ws_bytes is None:
+            ws_bytes = size(T, k, H, I)
+        return lib.sglb200_fused_experts_fp4(x, dt, w13, s13, a13, w2, s2, a2, w, ids, out, T, k, E, H, I, 1.0, ws, ws_bytes, None)
+
+    assert size(0, 2, 256, 128) == 0 and size(2, 2, 256, 128) >= 4 * (256 + 128) * 4
+    assert call(dt=2) == -2
+    assert call(H=240) == -1 and "divisible" in _err()
+    assert call(I=80) == -1 and "divisible" in _err()
+    assert call(E=0) == -1 and call(E=1025) == -1 and "experts" in _err()
+    assert call(T=600) == -1 and "at most" in _err()
+    assert call(T=1 << 40, k=1 << 40, ws_bytes=0) == -1 and "at most" in _err()
+    assert call(k=0, ws_bytes=0) == -1 and call(T=-1, ws_bytes=0) == -1
+    assert call(ids=None) == -1 and "null" in _err()
+    assert call(x=A + 8) == -1 and "16-byte" in _err()
+    assert call(ws=None) == -4 and "workspace" in _err()
+    assert call(ws_bytes=16) == -4 and call(ws=A + 8) == -4
+    assert call(T=0) == 0

@@ -19,19 +19,27 @@
 #include <type_traits>
 
 #include "fp4_math.cuh"
+#include "gemm_common.cuh"
 #include "ptx_sm100.cuh"
 
 namespace sglb200 {
 namespace fp4 {
 
-constexpr int kMoeWarps = 8, kMoeThreads = kMoeWarps * 32;
+constexpr int kMoeWarps = 16, kMoeConsumers = kMoeWarps * 32, kMoeThreads = kMoeConsumers + 32;  // one more warp fetches the weights
 constexpr int kMoeMaxExperts = 1024, kMoeMaxSlots = 1024;
-constexpr int kChunk = 128;   // columns per step: four lanes of 16 bytes of codes
-constexpr int kMoeRows = 8;   // activation rows per pass
+constexpr int kStep = 256;                    // columns per step: a lane takes 64 of a row, 32 bytes of codes and four scales
+constexpr int kMoeRows = 8;                   // activation rows per pass, at most
+constexpr uint32_t kTileBytes = 16 * kStep / 2;                  // of a tile and step
+constexpr uint32_t kCodeBytes = kMoeWarps * kTileBytes;    // of a stage: 32 KB, and 4 KB of scales
+constexpr uint32_t kTileScales = 16 * kStep / 16;
+constexpr uint32_t kStageBytes = kCodeBytes + kMoeWarps * kTileScales;
+constexpr int kMoeMaxStages = 6;
+constexpr int kUsualShift = 6;                // rows whose largest magnitude lies in [2^-5, 2^9) are staged under 2^6
+
+__device__ int g_fp4_moe_status = 0;  // 0 ok, 1 = a wait for weights expired
 
 struct MoeParams {
   const void* x;            // up: [tokens, K] 16-bit; down: h [slots, K] float32
-  const uint8_t* w;         // [experts, rows, K / 2]
   const uint8_t* ws;        // [experts, rows, K / 16]
   const float* alpha;       // [experts] or nullptr
   const int32_t* ids;       // [slots]
@@ -42,89 +50,141 @@ struct MoeParams {
   int done_count;
   int64_t K, rows;          // rows of w: 2 I or H
   int slots, topk, experts, tokens;
-  int chunks;               // of K
+  int steps;                // of K
   int warps_k;              // warps that split K; the others split tiles
   int sets;                 // items per expert
+  int pass_rows;            // activation rows per pass
+  int stages;
   float factor;
+  uint32_t wait_probes;
 };
 
-struct MoeTables {
+struct MoeCtl {
+  uint64_t full[kMoeMaxStages], empty[kMoeMaxStages];
   uint16_t count[kMoeMaxExperts];   // slots of an expert, then where they begin
-  uint16_t live[kMoeMaxExperts];    // experts that are named, ascending
+  uint16_t live[kMoeMaxExperts];    // experts that are named
   uint16_t begin[kMoeMaxExperts + 1];
   uint16_t slot[kMoeMaxSlots];      // slots in experts' order
-  int warp_sum[kMoeWarps];
-  int row_exp[kMoeRows][kMoeWarps]; // largest magnitudes, as float bits
-  int num_live, last;
+  int warp_sum[8];
+  int amax[2][kMoeRows];            // largest magnitudes of the staged rows, as float bits; used in turn
+  int num_live, complete[2], abort_flag;
 };
 
-// Which experts are named and by which slots; ids outside the experts are skipped.  (The order of an expert's slots depends on the
-// order of the atomics; it decides only which column of an instruction a slot takes, and columns do not mix.)
-__device__ __forceinline__ void route(const MoeParams& p, MoeTables* tb) {
+__device__ __forceinline__ int ld_fresh(const int32_t* at) {  // (past the first-level cache)
+  int v;
+  asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(at));
+  return v;
+}
+
+// Which experts are named and by which slots; ids outside the experts are skipped.  (The order of an expert's slots can depend on the
+// order of atomics; it decides only which column of an instruction a slot takes, and columns do not mix.)  All threads.
+__device__ __forceinline__ void route(const MoeParams& p, MoeCtl* ctl) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  uint32_t* count32 = reinterpret_cast<uint32_t*>(tb->count);
-  for (int i = tid; i < kMoeMaxExperts / 2; i += kMoeThreads) count32[i] = 0;
-  __syncthreads();
-  int place[kMoeMaxSlots / kMoeThreads], id[kMoeMaxSlots / kMoeThreads];
+  if (p.slots <= 32) {  // a slot a lane: its expert's slots are those lanes whose id is the same
+    if (warp == 0) {
+      const int id = lane < p.slots ? ld_fresh(p.ids + lane) : -1;
+      const bool in = (uint32_t)id < (uint32_t)p.experts;
+      const uint32_t same = __match_any_sync(0xffffffffu, in ? id : -1 - lane), before = (1u << lane) - 1;
+      const bool first = in && (same & before) == 0;
+      const uint32_t firsts = __ballot_sync(0xffffffffu, first);
+      int incl = first ? __popc(same) : 0;
 #pragma unroll
-  for (int j = 0; j < kMoeMaxSlots / kMoeThreads; ++j) {
-    const int s = tid + j * kMoeThreads;
-    id[j] = s < p.slots ? p.ids[s] : -1;
-    if ((uint32_t)id[j] < (uint32_t)p.experts) {
-      const uint32_t shift = (id[j] & 1) * 16;
-      place[j] = (int)(atomicAdd(&count32[id[j] >> 1], 1u << shift) >> shift & 0xffffu);
-    } else {
-      id[j] = -1;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      const int begin = __shfl_sync(0xffffffffu, incl - (first ? __popc(same) : 0), in ? __ffs(same) - 1 : lane);
+      if (first) {
+        const int j = __popc(firsts & before);
+        ctl->live[j] = (uint16_t)id;
+        ctl->begin[j] = (uint16_t)begin;
+      }
+      if (in) ctl->slot[begin + __popc(same & before)] = (uint16_t)lane;
+      if (lane == 31) {
+        ctl->num_live = __popc(firsts);
+        ctl->begin[__popc(firsts)] = (uint16_t)incl;
+      }
+    }
+    __syncthreads();
+    return;
+  }
+  constexpr int kRouters = 256, kIds = kMoeMaxSlots / kRouters, kExperts = kMoeMaxExperts / kRouters;
+  uint32_t* count32 = reinterpret_cast<uint32_t*>(ctl->count);
+  int place[kIds], id[kIds];
+  if (tid < kRouters) {
+#pragma unroll
+    for (int j = 0; j < kIds; ++j) id[j] = tid + j * kRouters < p.slots ? ld_fresh(p.ids + tid + j * kRouters) : -1;
+    for (int i = tid; i < kMoeMaxExperts / 2; i += kRouters) count32[i] = 0;
+  }
+  __syncthreads();
+  if (tid < kRouters) {
+#pragma unroll
+    for (int j = 0; j < kIds; ++j) {
+      if ((uint32_t)id[j] < (uint32_t)p.experts) {
+        const uint32_t shift = (id[j] & 1) * 16;
+        place[j] = (int)(atomicAdd(&count32[id[j] >> 1], 1u << shift) >> shift & 0xffffu);
+      } else {
+        id[j] = -1;
+      }
     }
   }
   __syncthreads();
   // exclusive scan over the experts, four a thread: (named, slots) packed
-  int mine = 0, c[4];
+  int mine = 0, c[kExperts], incl = 0;
+  if (tid < kRouters) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int e = tid * 4 + k;
-    c[k] = tb->count[e];
-    mine += c[k] ? (1 << 16) + c[k] : 0;
-  }
-  int incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += up;
-  }
-  if (lane == 31) tb->warp_sum[warp] = incl;
-  __syncthreads();
-  int before = incl - mine;
-  for (int w = 0; w < warp; ++w) before += tb->warp_sum[w];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if (c[k]) {
-      tb->live[before >> 16] = (uint16_t)(tid * 4 + k);
-      tb->begin[before >> 16] = (uint16_t)(before & 0xffff);
+    for (int k = 0; k < kExperts; ++k) {
+      c[k] = ctl->count[tid * kExperts + k];
+      mine += c[k] ? (1 << 16) + c[k] : 0;
     }
-    tb->count[tid * 4 + k] = (uint16_t)(before & 0xffff);
-    before += c[k] ? (1 << 16) + c[k] : 0;
-  }
-  if (tid == kMoeThreads - 1) {
-    tb->num_live = before >> 16;
-    tb->begin[before >> 16] = (uint16_t)(before & 0xffff);
+    incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    if (lane == 31) ctl->warp_sum[warp] = incl;
   }
   __syncthreads();
+  if (tid < kRouters) {
+    int before = incl - mine;
+    for (int w = 0; w < warp; ++w) before += ctl->warp_sum[w];
 #pragma unroll
-  for (int j = 0; j < kMoeMaxSlots / kMoeThreads; ++j)
-    if (id[j] >= 0) tb->slot[tb->count[id[j]] + place[j]] = (uint16_t)(tid + j * kMoeThreads);
+    for (int k = 0; k < kExperts; ++k) {
+      if (c[k]) {
+        ctl->live[before >> 16] = (uint16_t)(tid * kExperts + k);
+        ctl->begin[before >> 16] = (uint16_t)(before & 0xffff);
+      }
+      ctl->count[tid * kExperts + k] = (uint16_t)(before & 0xffff);
+      before += c[k] ? (1 << 16) + c[k] : 0;
+    }
+    if (tid == kRouters - 1) {
+      ctl->num_live = before >> 16;
+      ctl->begin[before >> 16] = (uint16_t)(before & 0xffff);
+    }
+  }
+  __syncthreads();
+  if (tid < kRouters) {
+#pragma unroll
+    for (int j = 0; j < kIds; ++j)
+      if (id[j] >= 0) ctl->slot[ctl->count[id[j]] + place[j]] = (uint16_t)(tid + j * kRouters);
+  }
   __syncthreads();
 }
 
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
 }
-__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2, int c3, int c4) {
+  asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+               : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Barrier of the warps that multiply.
+__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kMoeConsumers) : "memory"); }
 
 __device__ __forceinline__ uint32_t lds_32(uint32_t addr) {
   uint32_t v;
@@ -170,271 +230,421 @@ __device__ __forceinline__ void load8(const T* src, float (&v)[8]) {
   }
 }
 
-// The power of two that brings `amax` into [2^14, 2^15); 1 where it is zero or not finite.
-__device__ __forceinline__ int row_shift(float amax) {
-  const int e = (int)(__float_as_uint(amax) >> 23) & 0xff;
-  return e == 0xff || amax == 0.f ? 0 : min(max(14 + 127 - e, -126), 126);
-}
 __device__ __forceinline__ float pow2(int k) { return __uint_as_float((uint32_t)(127 + k) << 23); }
+// The power of two under which a row with this largest magnitude is staged: the usual one, or the one that brings it into [2^14,
+// 2^15); 1 where it is not finite.  fp16 rows are taken as they are.
+template <typename T>
+__device__ __forceinline__ int row_shift(int amax_bits) {
+  if constexpr (std::is_same<T, __half>::value) return 0;
+  const int e = amax_bits >> 23;
+  if (amax_bits == 0 || (e >= 127 - 5 && e < 127 + 9)) return kUsualShift;
+  return e == 0xff ? 0 : min(max(14 + 127 - e, -126), 126);
+}
+
+// One piece of a row, as fp16 under the factor f, to its place.
+__device__ __forceinline__ uint4 to_f16(const float (&v)[8], float f, bool fine) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a = v[2 * i] * f, b = v[2 * i + 1] * f;
+    if (!fine) {  // an infinite row: its finite values stay finite
+      if (fabsf(a) < __int_as_float(0x7f800000)) a = fminf(fmaxf(a, -65504.f), 65504.f);
+      if (fabsf(b) < __int_as_float(0x7f800000)) b = fminf(fmaxf(b, -65504.f), 65504.f);
+    }
+    const __half2 h = __floats2half2_rn(a, b);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
 
 // Rows [r0, r0 + n) of the expert's slots, as fp16 in the order in which lanes take them: 16-byte pieces of 8 columns, piece
-// (chunk, jj, row, t) = columns chunk * 128 + t * 32 + jj * 8 ..; columns past K are zeros.  All threads; ends with a barrier.
+// (step, jj, row, t) = columns step * 256 + t * 64 + jj * 8 ..; columns past K are zeros.  The multiplying warps; ends with a barrier.
 template <typename T>
-__device__ __forceinline__ void stage_rows(const MoeParams& p, MoeTables* tb, int r0, int n, uint4* xs) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int pieces = p.chunks * 16;  // of a row
-  __syncthreads();                   // the rows before these have been used
-  if constexpr (!std::is_same<T, __half>::value) {
-    for (int r = 0; r < n; ++r) {
-      const T* src = act_row<T>(p, tb->slot[r0 + r]);
-      float amax = 0.f;
-      for (int q = tid; q * 8 < p.K; q += kMoeThreads) {
-        float v[8];
-        load8(src + q * 8, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
-        // a NaN is not seen here and stays one under any power of two
-      }
-      amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
-      if (lane == 0) tb->row_exp[r][warp] = __float_as_int(amax);
-    }
-    __syncthreads();
-    if (tid < n) {
-      int m = 0;
-      for (int w = 0; w < kMoeWarps; ++w) m = max(m, tb->row_exp[tid][w]);
-      tb->row_exp[tid][0] = m;
-    }
-    __syncthreads();
-  }
-  for (int r = 0; r < n; ++r) {
-    const T* src = act_row<T>(p, tb->slot[r0 + r]);
-    float f = 1.f;
-    bool fine = true;
+__device__ __forceinline__ void stage_rows(const MoeParams& p, MoeCtl* ctl, int first, int n, int turn, uint4* xs) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int pieces = p.steps * 32;  // of a row: a multiple of the warp, so that a warp's pieces are of one row
+  int* amax = ctl->amax[turn & 1];
+  consumer_sync();  // the rows before these have been used
+  if (tid < kMoeRows) ctl->amax[(turn + 1) & 1][tid] = 0;
+  for (int i = tid; i < n * pieces; i += kMoeConsumers) {
+    const int r = i / pieces, q = i - r * pieces;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (q * 8 < p.K) load8(act_row<T>(p, ctl->slot[first + r]) + q * 8, v);
     if constexpr (!std::is_same<T, __half>::value) {
-      const float amax = __int_as_float(tb->row_exp[r][0]);
-      f = pow2(row_shift(amax));
-      fine = amax < __int_as_float(0x7f800000);
-    }
-    for (int q = tid; q < pieces; q += kMoeThreads) {
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (q * 8 < p.K) load8(src + q * 8, v);
-      uint32_t w[4];
+      float m = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float a = v[2 * i] * f, b = v[2 * i + 1] * f;
-        if (!fine) {  // an infinite row: its finite values stay finite
-          if (fabsf(a) < __int_as_float(0x7f800000)) a = fminf(fmaxf(a, -65504.f), 65504.f);
-          if (fabsf(b) < __int_as_float(0x7f800000)) b = fminf(fmaxf(b, -65504.f), 65504.f);
-        }
-        const __half2 h = __floats2half2_rn(a, b);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-      }
-      const int chunk = q >> 4, t = (q >> 2) & 3, jj = q & 3;
-      xs[((chunk * 4 + jj) * kMoeRows + r) * 4 + t] = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(v[k]));  // (a NaN is not seen here and stays one under any power of two)
+      const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+      if (lane == 0) atomicMax(&amax[r], (int)most);
     }
+    xs[(((q >> 5) * 8 + (q & 7)) * p.pass_rows + r) * 4 + ((q >> 3) & 3)] = to_f16(v, std::is_same<T, __half>::value ? 1.f : pow2(kUsualShift), true);
   }
-  __syncthreads();
-}
-
-template <typename T>
-__device__ __forceinline__ float row_unscale(const MoeTables* tb, int r) {
-  if constexpr (std::is_same<T, __half>::value) return 1.f;
-  return pow2(-row_shift(__int_as_float(tb->row_exp[r][0])));
-}
-
-// kUp: T is the activations' type and a tile is 8 gate and the 8 matching up rows; else T is float (h) and OutT the output's type.
-template <typename T, typename OutT, bool kUp, int MT, int D>
-__global__ void __launch_bounds__(kMoeThreads)
-    fp4_experts_kernel(const MoeParams p) {
-  extern __shared__ uint8_t smem_raw[];
-  MoeTables* tb = reinterpret_cast<MoeTables*>(smem_raw);
-  uint8_t* rest = smem_raw + (sizeof(MoeTables) + 15) / 16 * 16;
-  constexpr uint32_t kStage = MT * 1280;  // a warp's chunk: per tile 2 x 512 bytes of codes, 2 x 128 of scales
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t ring = ptx::smem_u32(rest) + warp * (D * kStage);
-  float* red = reinterpret_cast<float*>(rest + kMoeWarps * D * kStage);  // [warp][MT][4][32]
-  uint4* xs = reinterpret_cast<uint4*>(red + kMoeWarps * MT * 128);
-
-  ptx::grid_dependency_wait();
-  if (kUp && blockIdx.x == 0)
-    for (int i = tid; i < p.done_count; i += kMoeThreads) p.done[i] = 0;
-  route(p, tb);
-  const int warps_m = kMoeWarps / p.warps_k, wk = warp % p.warps_k, wm = warp / p.warps_k;
-  const int c0 = wk * p.chunks / p.warps_k, c1 = (wk + 1) * p.chunks / p.warps_k;
-  const int tiles = (int)(p.rows / 16);  // of an expert (16 rows of w each)
-  const int64_t code_row = p.K / 2, scale_row = p.K / 16;
-  const int items = tb->num_live * p.sets;
-  int staged_live = -1, staged_r0 = -1;
-
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    const int live = item / p.sets, set = item - live * p.sets;
-    const int expert = tb->live[live], first = tb->begin[live], rows_n = tb->begin[live + 1] - first;
-    const int tile0 = (set * warps_m + wm) * MT;
-    // this lane's two rows of each tile
-    const uint8_t *wp[MT][2], *sp[MT][2];
-    bool tile_live[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      tile_live[m] = tile0 + m < tiles;
-      const int tile = tile_live[m] ? tile0 + m : 0;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int64_t row = (int64_t)expert * p.rows + (kUp ? (int64_t)tile * 8 + g + u * (p.rows / 2) : (int64_t)tile * 16 + g + u * 8);
-        wp[m][u] = p.w + row * code_row + t * 16;
-        sp[m][u] = p.ws + row * scale_row + t * 2;
+  consumer_sync();
+  if constexpr (!std::is_same<T, __half>::value) {
+    bool again = false;
+    for (int r = 0; r < n; ++r) {
+      const int bits = amax[r], shift = row_shift<T>(bits);
+      if (shift == kUsualShift) continue;
+      again = true;
+      const bool fine = (bits >> 23) != 0xff;
+      for (int q = tid; q * 8 < p.K; q += kMoeConsumers) {
+        float v[8];
+        load8(act_row<T>(p, ctl->slot[first + r]) + q * 8, v);
+        xs[(((q >> 5) * 8 + (q & 7)) * p.pass_rows + r) * 4 + ((q >> 3) & 3)] = to_f16(v, pow2(shift), fine);
       }
     }
-    for (int r0 = 0; r0 < rows_n; r0 += kMoeRows) {
-      const int n = min(kMoeRows, rows_n - r0);
-      const auto issue = [&](int c, int d) {
-        const bool in = c * kChunk + t * 32 < p.K;
-        const uint32_t at = ring + d * kStage + lane * 16, sat = ring + d * kStage + MT * 1024 + lane * 4;
+    if (again) consumer_sync();  // (the same for all threads)
+  }
+}
+
+// A lane's scales of 64 columns of a row, of which `left` are there; zeros for the others.
+__device__ __forceinline__ uint32_t load_scales(const uint8_t* at, int left) {
+  uint32_t v = 0;
+  if (left > 0) v = __ldg(reinterpret_cast<const uint16_t*>(at));
+  if (left > 32) v |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(at) + 1) << 16;
+  return v;
+}
+
+// The tokens' slots of the columns [col0, col0 + cols), added in their order, by the CTA whose item was the last of those columns.
+template <typename OutT>
+__device__ __noinline__ void sum_slots(const MoeParams& p, int col0, int cols) {
+  __threadfence();
+  for (int j = threadIdx.x * 4; j < p.tokens * cols; j += kMoeConsumers * 4) {  // four columns a thread
+    const int token = j / cols, col = col0 + j - token * cols;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 0; k0 < p.topk; k0 += 8) {  // eight slots are asked for before the first is added
+      float4 v[8];
+      int id[8];
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const bool ok = in && tile_live[m];
-            cp_async_16(at + (m * 2 + u) * 512, ok ? wp[m][u] + c * 64 : p.w, ok);
-            cp_async_4(sat + (m * 2 + u) * 128, ok ? reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(sp[m][u] + c * 8) & ~uintptr_t(3)) : p.ws, ok);
-          }
-      };
-#pragma unroll
-      for (int d = 0; d < D; ++d) {
-        if (c0 + d < c1) issue(c0 + d, d);
-        cp_async_commit();
+      for (int k = 0; k < 8; ++k) {
+        const int s = token * p.topk + min(k0 + k, p.topk - 1);
+        v[k] = __ldcg(reinterpret_cast<const float4*>(p.h + (int64_t)s * p.rows + col)), id[k] = p.ids[s];
       }
-      if (staged_live != live || staged_r0 != r0) {
-        stage_rows<T>(p, tb, first + r0, n, xs);
-        staged_live = live, staged_r0 = r0;
-      }
-      float acc[MT][4];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
-      int d = 0;
-      for (int c = c0; c < c1; ++c) {
-        cp_async_wait<D - 1>();
-        uint4 code[MT][2];
-        uint32_t sc[MT][2];
+      for (int k = 0; k < 8; ++k)  // (a slot of no expert has not been written)
+        if (k0 + k < p.topk && (uint32_t)id[k] < (uint32_t)p.experts)
+          sum[0] += v[k].x, sum[1] += v[k].y, sum[2] += v[k].z, sum[3] += v[k].w;
+    }
+    OutT o[4];
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+    for (int k = 0; k < 4; ++k) o[k] = ElemTraits<OutT>::from_f32(sum[k] * p.factor);
+    *reinterpret_cast<uint2*>(static_cast<OutT*>(p.out) + (int64_t)token * p.rows + col) = *reinterpret_cast<const uint2*>(o);
+  }
+}
+
+// acc += weights of a step times the staged rows (`b`: this lane's pieces, `stride` apart).  181 instructions with the loads from
+// shared memory, 64 of them conversions and 64 scalings, for 16 x 256 weights: an SM that does nothing else takes 8.2 TB/s of weights so
+// (two tiles a warp, which share the pieces of x: 9.3, but half as many stages fit).
+__device__ __forceinline__ void multiply(float (&acc)[4], const uint4 (&code)[2][2], const uint32_t (&scale)[2], const uint4* b, int stride) {
+  uint32_t s2[2][2];
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            code[m][u] = ptx::lds_128(ring + d * kStage + lane * 16 + (m * 2 + u) * 512);
-            const uint32_t word = lds_32(ring + d * kStage + MT * 1024 + lane * 4 + (m * 2 + u) * 128);
-            sc[m][u] = cvt_f16x2_e4m3x2(word >> ((reinterpret_cast<uintptr_t>(sp[m][u]) & 2) * 8) & 0xffffu);
-          }
-        if (c + D < c1) issue(c + D, d);
-        cp_async_commit();
-        d = d + 1 == D ? 0 : d + 1;
+  for (int u = 0; u < 2; ++u) s2[u][0] = cvt_f16x2_e4m3x2(scale[u]), s2[u][1] = cvt_f16x2_e4m3x2(scale[u] >> 16);
 #pragma unroll
-        for (int jj = 0; jj < 4; ++jj) {
-          const uint4 b = g < n ? xs[((c * 4 + jj) * kMoeRows + g) * 4 + t] : make_uint4(0, 0, 0, 0);
+  for (int jj = 0; jj < 8; ++jj) {
+    const uint4 x = b[jj * stride];
+    uint32_t a[2][4];
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            uint32_t a[2][4];
+    for (int u = 0; u < 2; ++u) {
+      const uint32_t s = __byte_perm(s2[u][jj >> 2], 0, (jj >> 1) & 1 ? 0x3232 : 0x1010);
+      const uint4 c = code[u][jj >> 2];
+      cvt_f16x2_e2m1x8((jj & 3) == 0 ? c.x : (jj & 3) == 1 ? c.y : (jj & 3) == 2 ? c.z : c.w, a[u]);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const uint32_t word = jj == 0 ? code[m][u].x : jj == 1 ? code[m][u].y : jj == 2 ? code[m][u].z : code[m][u].w;
-              const uint32_t s = __byte_perm(sc[m][u], 0, jj < 2 ? 0x1010 : 0x3232);
-              cvt_f16x2_e2m1x8(word, a[u]);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) a[u][i] = hmul2(a[u][i], s);
+      for (int i = 0; i < 4; ++i) a[u][i] = hmul2(a[u][i], s);
+    }
+    mma_f16(acc, a[0][0], a[1][0], a[0][1], a[1][1], x.x, x.y);
+    mma_f16(acc, a[0][2], a[1][2], a[0][3], a[1][3], x.z, x.w);
+  }
+}
+
+// kWhole: K is a multiple of a step.  kUp: T is the activations' type and a tile is 8 gate and the 8 matching up rows; else T is float (h) and OutT the output's type.
+template <typename T, typename OutT, bool kUp, bool kWhole>
+__global__ void __launch_bounds__(kMoeThreads, 1)
+    fp4_experts_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s, const MoeParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint4* xs = reinterpret_cast<uint4*>(ring + p.stages * kStageBytes);
+  float* red = reinterpret_cast<float*>(xs + p.steps * 32 * p.pass_rows);  // [warp][4][32]
+  MoeCtl* ctl = reinterpret_cast<MoeCtl*>(red + kMoeWarps * 128);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t bar_full = ptx::smem_u32(ctl->full), bar_empty = ptx::smem_u32(ctl->empty);
+  const int S = p.stages;
+
+  if (tid == 0) {
+    for (int s = 0; s < S; ++s) ptx::mbar_init(bar_full + s * 8, 1), ptx::mbar_init(bar_empty + s * 8, kMoeWarps);
+    ctl->abort_flag = 0;
+    ptx::mbar_fence_init();
+  }
+  if (tid < kMoeRows) ctl->amax[0][tid] = 0;
+  // The down launch may begin when every CTA of the up launch runs, which is after all that is in front of both: it finds its experts
+  // and asks for its first weights, neither of which the up launch writes, before it waits for that.
+  if constexpr (kUp) {
+    ptx::grid_dependency_wait();
+    ptx::launch_dependents();
+    if (blockIdx.x == 0)
+      for (int i = tid; i < p.done_count; i += kMoeThreads) p.done[i] = 0;
+  }
+  route(p, ctl);
+
+  const int warps_k = p.warps_k, warps_m = kMoeWarps / warps_k;
+  const int tiles = (int)(p.rows / 16);  // of an expert (16 rows of w each)
+  const int items = ctl->num_live * p.sets, turns = (p.steps + warps_k - 1) / warps_k;
+  // A CTA takes neighbouring items, which are mostly of one expert.
+  const int item0 = (int)((int64_t)blockIdx.x * items / gridDim.x), item1 = (int)((int64_t)(blockIdx.x + 1) * items / gridDim.x);
+
+  if (warp == kMoeWarps) {
+    // ------------------------------ weights ------------------------------
+    if (ptx::elect_one()) {
+      bool ok = true;
+      int s = 0;                      // stage
+      uint32_t ph = 1, part_bytes = warps_m * kTileBytes;  // (the first round of stages is free)
+      for (int item = item0; item < item1 && ok; ++item) {
+        const int live = item / p.sets, tile0 = (item - live * p.sets) * warps_m, expert = ctl->live[live];
+        const int passes = (ctl->begin[live + 1] - ctl->begin[live] + p.pass_rows - 1) / p.pass_rows;
+        for (int i = 0, step0 = 0; i < passes * turns; ++i) {
+          ok = p.wait_probes != ptx::kProbesNone && ptx::mbar_wait_quiet(bar_empty + s * 8, ph);
+          if (!ok) break;
+          const uint32_t bar = bar_full + s * 8, at = ptx::smem_u32(ring) + s * kStageBytes;
+          if constexpr (kWhole) {  // one load for the codes of all parts of K, one for their scales (a box is counted whole)
+            ptx::mbar_arrive_expect_tx(bar, kStageBytes);
+            if constexpr (kUp) {
+              tma_load_5d(at, &map_w, bar, 0, tile0 * 8, 0, step0, expert);
+              tma_load_5d(at + kCodeBytes, &map_s, bar, 0, tile0 * 8, 0, step0, expert);
+            } else {
+              tma_load_4d(at, &map_w, bar, 0, tile0 * 16, step0, expert);
+              tma_load_4d(at + kCodeBytes, &map_s, bar, 0, tile0 * 16, step0, expert);
             }
-            mma_f16(acc[m], a[0][0], a[1][0], a[0][1], a[1][1], b.x, b.y);
-            mma_f16(acc[m], a[0][2], a[1][2], a[0][3], a[1][3], b.z, b.w);
+          } else {
+            const int parts = min(warps_k, p.steps - step0);
+            ptx::mbar_arrive_expect_tx(bar, parts * part_bytes);
+            for (int k = 0; k < parts; ++k) {
+              if constexpr (kUp)
+                tma_load_4d(at + k * part_bytes, &map_w, bar, (step0 + k) * (kStep / 2), tile0 * 8, 0, expert);
+              else
+                ptx::tma_load_3d(at + k * part_bytes, &map_w, bar, (step0 + k) * (kStep / 2), tile0 * 16, expert);
+            }
+          }
+          step0 += warps_k;
+          if (step0 >= p.steps) step0 = 0;
+          if (++s == S) s = 0, ph ^= 1;
+        }
+      }
+      if (!ok) ctl->abort_flag = 1;
+    }
+    __syncwarp();
+    if constexpr (!kUp) ptx::grid_dependency_wait();
+  } else {
+    // ------------------------------ products ------------------------------
+    const int wk = warp % warps_k, wm = warp / warps_k;
+    // this lane's codes in a stage: rows g and g + 8 of its tiles, pieces 2 t and 2 t + 1 of 128 swizzled bytes; a part of K has
+    // its tiles' gate rows, then their up rows, or its tiles
+    const uint32_t part = ptx::smem_u32(ring) + wk * warps_m * kTileBytes + g * 128;
+    const uint32_t tile_step = kUp ? 8 * 128 : 16 * 128, row_step = kUp ? warps_m * 8 * 128 : 8 * 128;
+    const uint32_t code_lo = part + wm * tile_step + ((uint32_t)(2 * t) ^ g) * 16;
+    const uint32_t code_hi = part + wm * tile_step + ((uint32_t)(2 * t + 1) ^ g) * 16;
+    const uint32_t row_a = (kUp ? wm * 8 : wm * 16) + g, row_b = row_a + (kUp ? warps_m * 8 : 8);
+    const uint32_t scale_a = ptx::smem_u32(ring) + kCodeBytes + wk * warps_m * kTileScales + row_a * 16 + t * 4;
+    const uint32_t scale_b = scale_a + (row_b - row_a) * 16;
+    const int64_t scale_row = p.K / 16;
+    const int skip = warps_k * kStep;  // columns between two steps of this warp
+
+    if constexpr (!kUp) ptx::grid_dependency_wait();
+    const auto sum_set = [&](int set) {
+      const int col0 = set * warps_m * 16;
+      sum_slots<OutT>(p, col0, min(warps_m * 16, (int)p.rows - col0));
+    };
+    bool ok = p.wait_probes != ptx::kProbesNone;
+    int staged_live = -1, staged_r0 = -1, stagings = 0, s = 0;
+    uint32_t ph = 0;
+    for (int item = item0; item < item1; ++item) {
+      const int live = item / p.sets, set = item - live * p.sets;
+      const int expert = ctl->live[live], first = ctl->begin[live], rows_n = ctl->begin[live + 1] - first;
+      const int my_tile = set * warps_m + wm;
+      // scales of this lane's rows (of the expert's first ones where there is no tile)
+      const int64_t row0 = (int64_t)expert * p.rows + (my_tile < tiles ? kUp ? (int64_t)my_tile * 8 + g : (int64_t)my_tile * 16 + g : 0);
+      const uint8_t* sp[2] = {p.ws + row0 * scale_row, p.ws + (row0 + (kUp ? p.rows / 2 : 8)) * scale_row};
+      for (int r0 = 0; r0 < rows_n; r0 += p.pass_rows) {
+        const int n = min(p.pass_rows, rows_n - r0);
+        // where K is not whole steps, scales are asked for in global memory, two steps ahead
+        uint32_t sc[2][2];
+        const uint8_t *sa = sp[0] + (wk * kStep + t * 64) / 16, *sb = sp[1] + (wk * kStep + t * 64) / 16;
+        int left = (int)p.K - (wk * kStep + t * 64);  // columns of the row from those whose scales are asked for next
+        const auto ask = [&](uint32_t (&to)[2]) {
+          to[0] = load_scales(sa, left), to[1] = load_scales(sb, left);
+          sa += skip / 16, sb += skip / 16, left -= skip;
+        };
+        if constexpr (!kWhole) ask(sc[0]), ask(sc[1]);
+        if (staged_live != live || staged_r0 != r0) {
+          stage_rows<T>(p, ctl, first + r0, n, stagings, xs);
+          ++stagings, staged_live = live, staged_r0 = r0;
+        }
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint4* b = xs + (wk * 8 * p.pass_rows + (g < n ? g : 0)) * 4 + t;  // (columns without a row are not looked at)
+        const int stride = p.pass_rows * 4;
+        const auto step = [&](uint32_t (&scale)[2], bool mine) {
+          if (ok && !ptx::mbar_test(bar_full + s * 8, ph)) ok = ptx::mbar_wait_quiet(bar_full + s * 8, ph);
+          const uint32_t lo = code_lo + s * kStageBytes, hi = code_hi + s * kStageBytes;
+          const uint4 code[2][2] = {{ptx::lds_128(lo), ptx::lds_128(hi)}, {ptx::lds_128(lo + row_step), ptx::lds_128(hi + row_step)}};
+          if constexpr (kWhole) scale[0] = lds_32(scale_a + s * kStageBytes), scale[1] = lds_32(scale_b + s * kStageBytes);
+          __syncwarp();
+          ptx::mbar_arrive_if(bar_empty + s * 8, lane == 0);
+          if (++s == S) s = 0, ph ^= 1;
+          if (mine) multiply(acc, code, scale, b, stride);
+          b += warps_k * 8 * stride;
+          if constexpr (!kWhole) ask(scale);
+        };
+        const int mine = (p.steps - wk + warps_k - 1) / warps_k;  // (the last turn may have no step for this warp)
+        for (int i = 0; i < turns; i += 2) {
+          step(sc[0], i < mine);
+          if (i + 1 < turns) step(sc[1], i + 1 < mine);
+        }
+        // Lane (g, t) has rows g (acc 0, 1) and g + 8 (2, 3) of columns 2 t, 2 t + 1.  A warp of those that split K adds up two
+        // values of each of their lanes.
+        const float alpha = p.alpha ? p.alpha[expert] : 1.f;
+        const auto finish = [&](int tile, int r, int row, float lo, float hi) {
+          if (tile >= tiles || r >= n) return;
+          const float f = pow2(-row_shift<T>(ctl->amax[(stagings - 1) & 1][r]));
+          lo = lo * alpha * f, hi = hi * alpha * f;
+          const int slot = ctl->slot[first + r0 + r];
+          if constexpr (kUp) {
+            p.h[(int64_t)slot * (p.rows / 2) + tile * 8 + row] = lo / (1.f + expf(-lo)) * hi;
+          } else {
+            const float weight = p.weights[slot];
+            float* at = p.h + (int64_t)slot * p.rows + tile * 16 + row;
+            at[0] = weight * lo, at[8] = weight * hi;
+          }
+        };
+        if (warps_k == 1) {
+          finish(my_tile, 2 * t, g, acc[0], acc[2]);
+          finish(my_tile, 2 * t + 1, g, acc[1], acc[3]);
+        } else {
+          consumer_sync();  // (the sums before these have been read)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) red[(warp * 4 + j) * 32 + lane] = acc[j];
+          consumer_sync();
+          for (int i = tid; i < warps_m * 64; i += kMoeConsumers) {
+            const int j = (i >> 5) & 1, m = i >> 6;  // (i % 32 == lane)
+            float lo = 0.f, hi = 0.f;
+            for (int k = 0; k < warps_k; ++k) {
+              const float* at = red + ((m * warps_k + k) * 4 + j) * 32 + lane;
+              lo += at[0], hi += at[64];
+            }
+            finish(set * warps_m + m, 2 * t + j, g, lo, hi);
           }
         }
       }
-      // sums over the warps of a K split: lane (g, t) has rows g (0, 1) and g + 8 (2, 3), columns 2 t, 2 t + 1
-      __syncthreads();  // (the sums before these have been read)
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) red[((warp * MT + m) * 4 + j) * 32 + lane] = acc[m][j];
-      __syncthreads();
-      const float alpha = p.alpha ? p.alpha[expert] : 1.f;
-      // thread -> (tile of the item, pair of values): j = 0, 1 with 2, 3
-      for (int i = tid; i < warps_m * MT * 64; i += kMoeThreads) {
-        const int l = i & 31, j = (i >> 5) & 1, m = (i >> 6) % MT, w = (i >> 6) / MT;
-        const int tile = (set * warps_m + w) * MT + m, r = 2 * (l & 3) + j;
-        if (tile >= tiles || r >= n) continue;
-        float lo = 0.f, hi = 0.f;
-        for (int k = 0; k < p.warps_k; ++k) {
-          const float* at = red + (((w * p.warps_k + k) * MT + m) * 4 + j) * 32 + l;
-          lo += at[0], hi += at[64];
+      if constexpr (!kUp) {
+        // One thread counts the item once everybody's products are on their way; what it learns is looked at behind the next
+        // item's weights, so that nobody waits for it.
+        consumer_sync();
+        const bool sum = item > item0 && ctl->complete[(item - 1) & 1];
+        if (tid == 0) {
+          __threadfence();
+          ctl->complete[item & 1] = atomicAdd(&p.done[set], 1) == ctl->num_live - 1;
         }
-        const float f = row_unscale<T>(tb, r);
-        lo = lo * alpha * f, hi = hi * alpha * f;
-        const int slot = tb->slot[first + r0 + r];
-        if constexpr (kUp) {
-          p.h[(int64_t)slot * (p.rows / 2) + tile * 8 + (l >> 2)] = lo / (1.f + expf(-lo)) * hi;
-        } else {
-          const float w8 = p.weights[slot];
-          float* at = p.h + (int64_t)slot * p.rows + tile * 16 + (l >> 2);
-          at[0] = w8 * lo, at[8] = w8 * hi;
-        }
+        if (sum) sum_set((item - 1) % p.sets);
       }
     }
     if constexpr (!kUp) {
-      // the last of the experts' CTAs to reach a set of columns adds up its tokens
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) tb->last = atomicAdd(&p.done[set], 1) == tb->num_live - 1;
-      __syncthreads();
-      if (tb->last) {
-        __threadfence();
-        const int col0 = set * warps_m * MT * 16, cols = min(warps_m * MT * 16, (int)p.rows - col0);
-        for (int i = tid; i < p.tokens * cols; i += kMoeThreads) {
-          const int token = i / cols, col = col0 + i % cols;
-          float sum = 0.f;
-          for (int j = 0; j < p.topk; ++j) {
-            const int s = token * p.topk + j;
-            if ((uint32_t)p.ids[s] < (uint32_t)p.experts) sum += __ldcg(p.h + (int64_t)s * p.rows + col);
-          }
-          static_cast<OutT*>(p.out)[(int64_t)token * p.rows + col] = ElemTraits<OutT>::from_f32(sum * p.factor);
-        }
-      }
+      consumer_sync();
+      if (item0 < item1 && ctl->complete[(item1 - 1) & 1]) sum_set((item1 - 1) % p.sets);
+      if (items == 0)  // no expert is named: zeros
+        for (int64_t i = (int64_t)blockIdx.x * kMoeConsumers + tid; i < (int64_t)p.tokens * p.rows; i += (int64_t)gridDim.x * kMoeConsumers)
+          static_cast<OutT*>(p.out)[i] = ElemTraits<OutT>::from_f32(0.f);
     }
+    if (!ok) ctl->abort_flag = 1;
   }
-  if constexpr (!kUp) {
-    if (tb->num_live == 0)  // no expert is named: zeros
-      for (int64_t i = blockIdx.x * kMoeThreads + tid; i < (int64_t)p.tokens * p.rows; i += (int64_t)gridDim.x * kMoeThreads)
-        static_cast<OutT*>(p.out)[i] = ElemTraits<OutT>::from_f32(0.f);
+  __syncthreads();
+  if (ctl->abort_flag != 0 && tid == 0) {
+    atomicExch(&g_fp4_moe_status, 1);
+    // give copies that may still be in flight time to land before the CTA's shared memory is released
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000ll) {
+    }
   }
 }
 
-template <typename T, typename OutT, bool kUp, int MT, int D>
-static int launch_experts(MoeParams& p, cudaStream_t st) {
-  auto kern = fp4_experts_kernel<T, OutT, kUp, MT, D>;
-  const size_t smem = (sizeof(MoeTables) + 15) / 16 * 16 + (size_t)kMoeWarps * D * MT * 1280 + kMoeWarps * MT * 512 +
-                      (size_t)p.chunks * 4 * kMoeRows * 4 * 16;
-  SGLB_REQUIRE(smem <= 227 * 1024, "fused_experts_fp4: %lld columns are too many", (long long)p.K);
-  static thread_local size_t attr_set[64] = {0};
-  int dev = 0;
-  SGLB_CUDA(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64 || attr_set[dev] < smem) {
-    SGLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    if (dev >= 0 && dev < 64) attr_set[dev] = smem;
-  }
-  const int per_sm = std::max(1, std::min(4, (int)(224 * 1024 / (smem + 1024))));
-  const int64_t most = (int64_t)std::min(p.slots, p.experts) * p.sets;
-  const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)sm_count() * per_sm));
-  SGLB_CUDA(launch_pdl(kern, grid, kMoeThreads, smem, st, p));
+constexpr int64_t moe_smem(int steps, int pass_rows, int stages) {
+  return 1024 + (int64_t)stages * kStageBytes + (int64_t)steps * 512 * pass_rows + kMoeWarps * 512 + (int64_t)sizeof(MoeCtl);
+}
+constexpr int64_t kMoeMostSmem = 227 * 1024;
+
+// Experts that `slots` picks name, taken as spread evenly.
+static double expected_live(const MoeParams& p) {
+  double none = 1.0;
+  for (int i = 0; i < p.slots; ++i) none *= 1.0 - 1.0 / p.experts;
+  return p.experts * (1.0 - none);
+}
+
+static int plan_product(MoeParams& p, int64_t K, int64_t rows) {
+  p.K = K, p.rows = rows, p.steps = (int)((K + kStep - 1) / kStep);
+  // Warps that split K, the others taking tiles of their own: as few as give nine in ten SMs an item (sums of a split K cost two
+  // barriers and the shared memory between).  us over 1, 2, 4, 8 and 16 for the first product: 8 named experts of 7168 x 256 41, 31, 26,
+  // 24, 24; 8 of 7168 x 2048 61, 62, 62, 65, 70; 101 of them 451, 475, 475, 497, 557.
+  const double live = expected_live(p);
+  p.warps_k = 1;
+  while (p.warps_k < kMoeWarps && p.warps_k < p.steps && live * (double)(rows / 16) * p.warps_k / kMoeWarps < 0.85 * sm_count()) p.warps_k *= 2;
+  const int per = kMoeWarps / p.warps_k;
+  p.sets = (int)((rows / 16 + per - 1) / per);
+  p.pass_rows = kMoeRows;
+  while (p.pass_rows > 1 && (moe_smem(p.steps, p.pass_rows, 4) > kMoeMostSmem || p.pass_rows >= 2 * p.slots)) p.pass_rows /= 2;
+  p.stages = kMoeMaxStages;
+  while (p.stages > 2 && moe_smem(p.steps, p.pass_rows, p.stages) > kMoeMostSmem) --p.stages;
+  SGLB_REQUIRE(moe_smem(p.steps, p.pass_rows, p.stages) <= kMoeMostSmem, "fused_experts_fp4: %lld columns are too many", (long long)K);
   return SGLB200_OK;
 }
 
-struct MoeShape {
-  int64_t T, topk, H, I;
-  int E;
-};
-constexpr int kMoeMT = 2, kMoeD = 3;
-static int warps_k_for(int chunks) { return chunks >= 16 ? 8 : chunks >= 8 ? 4 : chunks >= 4 ? 2 : 1; }
-static int64_t down_sets(int64_t H, int64_t I) {
-  const int wm = kMoeWarps / warps_k_for((int)((I + kChunk - 1) / kChunk));
-  return (H / 16 + wm * kMoeMT - 1) / (wm * kMoeMT);
+template <typename T, typename OutT, bool kUp, bool kWhole>
+static int launch_experts(const CUtensorMap& map_w, const CUtensorMap& map_s, const MoeParams& p, cudaStream_t st) {
+  auto kern = fp4_experts_kernel<T, OutT, kUp, kWhole>;
+  static thread_local bool attr_set[64] = {false};  // the opt-in is per function and per device
+  int dev = 0;
+  SGLB_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    SGLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMoeMostSmem));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  const int64_t most = (int64_t)std::min(p.slots, p.experts) * p.sets;
+  const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, sm_count()));
+  SGLB_CUDA(launch_pdl(kern, grid, kMoeThreads, (size_t)moe_smem(p.steps, p.pass_rows, p.stages), st, map_w, map_s, p));
+  return SGLB200_OK;
+}
+
+template <typename T, typename OutT, bool kUp>
+static int launch_product(const void* w, const MoeParams& p, cudaStream_t st) {
+  // Dimensions: bytes (of a step), rows, for w13 its two halves, steps where rows are whole ones, experts.
+  const bool whole = p.K % kStep == 0;
+  const uint64_t rows = (uint64_t)(kUp ? p.rows / 2 : p.rows);
+  const uint32_t tile_rows = (uint32_t)((kUp ? 8 : 16) * (kMoeWarps / p.warps_k));
+  const auto map_of = [&](const void* at, uint64_t row_bytes, uint32_t step_bytes, bool swizzled, CUtensorMap* out) {
+    uint64_t dims[5] = {whole ? (uint64_t)step_bytes : row_bytes, rows}, strides[4] = {row_bytes};
+    uint32_t box[5] = {step_bytes, tile_rows}, rank = 2;
+    const auto add = [&](uint64_t n, uint64_t stride, uint32_t b) { dims[rank] = n, strides[rank - 1] = stride, box[rank++] = b; };
+    if (kUp) add(2, rows * row_bytes, 2);
+    if (whole) add((uint64_t)p.steps, step_bytes, (uint32_t)p.warps_k);
+    add((uint64_t)p.experts, (uint64_t)p.rows * row_bytes, 1);
+    return get_tile_map(at, rank, dims, strides, box, swizzled, out);
+  };
+  CUtensorMap map_w, map_s;
+  int rc = map_of(w, (uint64_t)p.K / 2, kStep / 2, true, &map_w);
+  if (rc) return rc;
+  if (!whole) return launch_experts<T, OutT, kUp, false>(map_w, map_w, p, st);
+  rc = map_of(p.ws, (uint64_t)p.K / 16, kStep / 16, false, &map_s);
+  return rc ? rc : launch_experts<T, OutT, kUp, true>(map_w, map_s, p, st);
 }
 
 }  // namespace fp4
+
+int fp4_moe_status() {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, fp4::g_fp4_moe_status, sizeof(int)) != cudaSuccess) return -1;
+  return v;
+}
+int fp4_moe_status_clear() {
+  const int zero = 0;
+  SGLB_CUDA(cudaMemcpyToSymbol(fp4::g_fp4_moe_status, &zero, sizeof(int)));
+  return SGLB200_OK;
+}
+
 }  // namespace sglb200
 
 using namespace sglb200;
@@ -444,7 +654,7 @@ extern "C" {
 int64_t sglb200_fused_experts_fp4_workspace_bytes(int64_t tokens, int64_t topk, int64_t hidden, int64_t intermediate) {
   if (tokens <= 0 || topk <= 0 || hidden <= 0 || intermediate <= 0) return 0;
   const int64_t slots = tokens * topk;
-  return (slots * intermediate + slots * hidden) * 4 + (fp4::down_sets(hidden, intermediate) * 4 + 15) / 16 * 16;
+  return (slots * intermediate + slots * hidden) * 4 + (hidden / 16 * 4 + 15) / 16 * 16;  // h, products, counters
 }
 
 int sglb200_fused_experts_fp4(const void* x, int dtype, const void* w13, const void* w13_scale, const float* w13_alpha, const void* w2,
@@ -474,22 +684,18 @@ int sglb200_fused_experts_fp4(const void* x, int dtype, const void* w13, const v
   fp4::MoeParams p{};
   p.ids = topk_ids, p.weights = topk_weights;
   p.slots = (int)slots, p.topk = (int)topk, p.experts = num_experts, p.tokens = (int)tokens;
-  p.done = reinterpret_cast<int32_t*>(y + slots * hidden), p.done_count = (int)fp4::down_sets(hidden, intermediate);
+  p.done = reinterpret_cast<int32_t*>(y + slots * hidden), p.done_count = (int)(hidden / 16);
   p.factor = factor;
-  const auto plan = [&](int64_t K, int64_t rows) {
-    p.K = K, p.rows = rows, p.chunks = (int)((K + fp4::kChunk - 1) / fp4::kChunk), p.warps_k = fp4::warps_k_for(p.chunks);
-    const int per = fp4::kMoeWarps / p.warps_k * fp4::kMoeMT;
-    p.sets = (int)((rows / 16 + per - 1) / per);
-  };
-  p.x = x, p.w = static_cast<const uint8_t*>(w13), p.ws = static_cast<const uint8_t*>(w13_scale), p.alpha = w13_alpha, p.h = h;
-  plan(hidden, 2 * intermediate);
-  int rc = dtype == 0 ? fp4::launch_experts<__nv_bfloat16, __nv_bfloat16, true, fp4::kMoeMT, fp4::kMoeD>(p, st)
-                      : fp4::launch_experts<__half, __half, true, fp4::kMoeMT, fp4::kMoeD>(p, st);
-  if (rc) return rc;
-  p.x = h, p.w = static_cast<const uint8_t*>(w2), p.ws = static_cast<const uint8_t*>(w2_scale), p.alpha = w2_alpha, p.h = y, p.out = out;
-  plan(intermediate, hidden);
-  return dtype == 0 ? fp4::launch_experts<float, __nv_bfloat16, false, fp4::kMoeMT, fp4::kMoeD>(p, st)
-                    : fp4::launch_experts<float, __half, false, fp4::kMoeMT, fp4::kMoeD>(p, st);
+  p.wait_probes = g_gemm_wait_probes;
+  p.x = x, p.ws = static_cast<const uint8_t*>(w13_scale), p.alpha = w13_alpha, p.h = h;
+  int rc = fp4::plan_product(p, hidden, 2 * intermediate);
+  fp4::MoeParams q = p;
+  q.x = h, q.ws = static_cast<const uint8_t*>(w2_scale), q.alpha = w2_alpha, q.h = y, q.out = out;
+  if (rc == SGLB200_OK) rc = fp4::plan_product(q, intermediate, hidden);
+  if (rc != SGLB200_OK) return rc;
+  rc = dtype == 0 ? fp4::launch_product<__nv_bfloat16, __nv_bfloat16, true>(w13, p, st) : fp4::launch_product<__half, __half, true>(w13, p, st);
+  if (rc != SGLB200_OK) return rc;
+  return dtype == 0 ? fp4::launch_product<float, __nv_bfloat16, false>(w2, q, st) : fp4::launch_product<float, __half, false>(w2, q, st);
 }
 
 }  // extern "C"

@@ -44,9 +44,11 @@
 // (sglb200_gemm_status() reports it).
 #include <cuda.h>
 
+#include <cstring>
 #include <mutex>
 #include <type_traits>
 #include <unordered_map>
+#include <vector>
 
 #include "common.cuh"
 #include "gemm_common.cuh"
@@ -1397,6 +1399,64 @@ int get_tensor_map(const void* ptr, uint64_t d0, uint64_t d1, uint64_t d2, uint3
   return SGLB200_OK;
 }
 
+int get_tile_map(const void* ptr, uint32_t rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box, bool swizzled,
+                 CUtensorMap* out) {
+  struct Entry {
+    const void* ptr;
+    uint32_t rank, box[5];
+    bool swizzled;
+    uint64_t dims[5], strides[4];
+    CUtensorMap map;
+  };
+  // The maps of the last calls, most programs having a few of them; the oldest gives way.
+  constexpr int kKept = 512;
+  static thread_local std::vector<Entry> cache;
+  static thread_local std::unordered_multimap<uintptr_t, size_t> at;
+  static thread_local size_t oldest = 0;
+  Entry e{};
+  e.ptr = ptr, e.rank = rank, e.swizzled = swizzled;
+  for (uint32_t i = 0; i < rank; ++i) {
+    e.dims[i] = dims[i], e.box[i] = box[i];
+    if (i + 1 < rank) e.strides[i] = strides[i];
+  }
+  const auto same = [&](const Entry& a) {
+    return a.ptr == e.ptr && a.rank == e.rank && a.swizzled == e.swizzled && memcmp(a.box, e.box, sizeof(e.box)) == 0 && memcmp(a.dims, e.dims, sizeof(e.dims)) == 0 &&
+           memcmp(a.strides, e.strides, sizeof(e.strides)) == 0;
+  };
+  const auto range = at.equal_range(reinterpret_cast<uintptr_t>(ptr));
+  for (auto it = range.first; it != range.second; ++it)
+    if (same(cache[it->second])) {
+      *out = cache[it->second].map;
+      return SGLB200_OK;
+    }
+  EncodeTiledFn enc = get_encode_fn();
+  if (enc == nullptr) return fail(SGLB200_E_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t d[5], st[4];
+  cuuint32_t bx[5], estr[5] = {1, 1, 1, 1, 1};
+  for (uint32_t i = 0; i < 5; ++i) d[i] = e.dims[i], bx[i] = e.box[i];
+  for (uint32_t i = 0; i < 4; ++i) st[i] = e.strides[i];
+  const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(ptr), d, st, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(SGLB200_E_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  e.map = *out;
+  size_t slot = cache.size();
+  if (slot < kKept) {
+    cache.push_back(e);
+  } else {
+    slot = oldest, oldest = (oldest + 1) % kKept;
+    const auto old = at.equal_range(reinterpret_cast<uintptr_t>(cache[slot].ptr));
+    for (auto it = old.first; it != old.second; ++it)
+      if (it->second == slot) {
+        at.erase(it);
+        break;
+      }
+    cache[slot] = e;
+  }
+  at.emplace(reinterpret_cast<uintptr_t>(ptr), slot);
+  return SGLB200_OK;
+}
+
 int get_out_map(const void* ptr, uint64_t N, uint64_t rows, int out_fp16, uint32_t box_rows, CUtensorMap* out) {
   static thread_local std::unordered_map<MapKey, CUtensorMap, MapKeyHash> cache;
   const MapKey key{ptr, N, rows, (uint64_t)out_fp16, box_rows, 0};
@@ -1685,6 +1745,7 @@ extern "C" int sglb200_gemm_status_clear(void) {
   SGLB_CUDA(cudaMemcpyToSymbol(g_gemm_status, &zero, sizeof(int)));
   int rc = rows_gemm_status_clear();
   if (rc == SGLB200_OK) rc = fp4_gemm_status_clear();
+  if (rc == SGLB200_OK) rc = fp4_moe_status_clear();
   return rc != SGLB200_OK ? rc : small_linear_status_clear();
 }
 
@@ -1693,6 +1754,7 @@ extern "C" int sglb200_gemm_status(void) {
   if (cudaMemcpyFromSymbol(&v, g_gemm_status, sizeof(int)) != cudaSuccess) return -1;
   if (v == 0) v = rows_gemm_status();
   if (v == 0) v = fp4_gemm_status();
+  if (v == 0) v = fp4_moe_status();
   return v != 0 ? v : small_linear_status();
 }
 

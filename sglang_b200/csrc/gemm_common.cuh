@@ -23,6 +23,11 @@ __device__ __forceinline__ void tile_coord(int t, int tiles_m, int tiles_n, int 
 // 128-byte swizzle, out-of-range elements read as zero.  Cached per argument tuple and thread.
 int get_tensor_map(const void* ptr, uint64_t d0, uint64_t d1, uint64_t d2, uint32_t box_rows, uint32_t rank, CUtensorMap* out);
 
+// uint8 tensor of `rank` (2 to 5) dimensions, innermost first, `strides` of all but the innermost in bytes; out-of-range elements read as zero; with `swizzled` the box's
+// rows are 128 bytes.  Cached likewise.
+int get_tile_map(const void* ptr, uint32_t rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box, bool swizzled,
+                 CUtensorMap* out);
+
 // Output tensor [rows][N] of 2-byte elements, box = 64 columns x box_rows, 128-byte swizzle (matches the staging layout
 // written by the epilogues).  Cached likewise.
 int get_out_map(const void* ptr, uint64_t N, uint64_t rows, int out_fp16, uint32_t box_rows, CUtensorMap* out);
@@ -111,6 +116,9 @@ int small_linear_status_clear();
 // fp4_gemm.cu: status word of its kernels (0 ok, 1 a wait expired, -1 not readable), and its reset.
 int fp4_gemm_status();
 int fp4_gemm_status_clear();
+// fp4_moe.cu: the same.
+int fp4_moe_status();
+int fp4_moe_status_clear();
 
 // gemm_rows.cu: status word of its kernels (0 ok, 1 a wait expired, -1 not readable), and its reset.
 int rows_gemm_status();

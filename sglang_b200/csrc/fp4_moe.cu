@@ -28,7 +28,7 @@ namespace fp4 {
 constexpr int kMoeWarps = 16, kMoeConsumers = kMoeWarps * 32, kMoeThreads = kMoeConsumers + 32;  // one more warp fetches the weights
 constexpr int kMoeMaxExperts = 1024, kMoeMaxSlots = 1024;
 constexpr int kStep = 256;                    // columns per step: a lane takes 64 of a row, 32 bytes of codes and four scales
-constexpr int kMoeRows = 8;                   // activation rows per pass, at most
+constexpr int kMoeRows = 32;                  // activation rows per pass, at most: four times the eight of an instruction
 constexpr uint32_t kTileBytes = 16 * kStep / 2;                  // of a tile and step
 constexpr uint32_t kCodeBytes = kMoeWarps * kTileBytes;    // of a stage: 32 KB, and 4 KB of scales
 constexpr uint32_t kTileScales = 16 * kStep / 16;
@@ -67,6 +67,7 @@ struct MoeCtl {
   uint16_t slot[kMoeMaxSlots];      // slots in experts' order
   int warp_sum[8];
   int amax[2][kMoeRows];            // largest magnitudes of the staged rows, as float bits; used in turn
+  float factor[kMoeRows];           // of the staged rows: alpha (times the routing weight)
   int num_live, complete[2], abort_flag;
 };
 
@@ -209,26 +210,34 @@ __device__ __forceinline__ const T* act_row(const MoeParams& p, int slot) {
   return static_cast<const T*>(p.x) + (int64_t)row * p.K;
 }
 
-// Eight activations as float32.
+// Eight activations as they lie in memory, as float32, and the largest of their magnitudes' bits (NaN above infinity).
 template <typename T>
-__device__ __forceinline__ void load8(const T* src, float (&v)[8]) {
-  if constexpr (std::is_same<T, float>::value) {
-    const float4 a = __ldcg(reinterpret_cast<const float4*>(src)), b = __ldcg(reinterpret_cast<const float4*>(src) + 1);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else {
-    const uint4 q = __ldcg(reinterpret_cast<const uint4*>(src));
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (std::is_same<T, __half>::value) {
-        const float2 f = f16x2_to_f32(w[i]);
-        v[2 * i] = f.x, v[2 * i + 1] = f.y;
-      } else {
-        v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      }
+struct Piece {
+  uint32_t w[std::is_same<T, float>::value ? 8 : 4];
+  __device__ __forceinline__ void load(const T* src) {
+    const uint4 a = __ldcg(reinterpret_cast<const uint4*>(src));
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+    if constexpr (std::is_same<T, float>::value) {
+      const uint4 b = __ldcg(reinterpret_cast<const uint4*>(src) + 1);
+      w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
     }
   }
-}
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (uint32_t& v : w) v = 0;
+  }
+  __device__ __forceinline__ float2 pair(int i) const {  // values 2 i, 2 i + 1
+    if constexpr (std::is_same<T, float>::value) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    if constexpr (std::is_same<T, __half>::value) return f16x2_to_f32(w[i]);
+    return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  }
+  // two 16-bit maxima for bf16, one for float32
+  __device__ __forceinline__ uint32_t most(uint32_t m) const {
+#pragma unroll
+    for (uint32_t v : w) m = std::is_same<T, float>::value ? max(m, v & 0x7fffffffu) : __vmaxu2(m, v & 0x7fff7fffu);
+    return m;
+  }
+};
 
 __device__ __forceinline__ float pow2(int k) { return __uint_as_float((uint32_t)(127 + k) << 23); }
 // The power of two under which a row with this largest magnitude is staged: the usual one, or the one that brings it into [2^14,
@@ -236,48 +245,80 @@ __device__ __forceinline__ float pow2(int k) { return __uint_as_float((uint32_t)
 template <typename T>
 __device__ __forceinline__ int row_shift(int amax_bits) {
   if constexpr (std::is_same<T, __half>::value) return 0;
-  const int e = amax_bits >> 23;
+  const int e = min(amax_bits >> 23, 0xff);
   if (amax_bits == 0 || (e >= 127 - 5 && e < 127 + 9)) return kUsualShift;
   return e == 0xff ? 0 : min(max(14 + 127 - e, -126), 126);
 }
 
-// One piece of a row, as fp16 under the factor f, to its place.
-__device__ __forceinline__ uint4 to_f16(const float (&v)[8], float f, bool fine) {
+// A piece as fp16 under the factor f.
+template <typename T>
+__device__ __forceinline__ uint4 to_f16(const Piece<T>& x, float f) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float a = v[2 * i] * f, b = v[2 * i + 1] * f;
-    if (!fine) {  // an infinite row: its finite values stay finite
-      if (fabsf(a) < __int_as_float(0x7f800000)) a = fminf(fmaxf(a, -65504.f), 65504.f);
-      if (fabsf(b) < __int_as_float(0x7f800000)) b = fminf(fmaxf(b, -65504.f), 65504.f);
+    if constexpr (std::is_same<T, __half>::value) {
+      w[i] = x.w[i];
+    } else {
+      const float2 v = x.pair(i);
+      const __half2 h = __floats2half2_rn(v.x * f, v.y * f);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
-    const __half2 h = __floats2half2_rn(a, b);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The same of a row that is not finite: its finite values stay finite.
+template <typename T>
+__device__ __forceinline__ uint4 to_f16_clamped(const Piece<T>& x) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 v = x.pair(i);
+    if (fabsf(v.x) < __int_as_float(0x7f800000)) v.x = fminf(fmaxf(v.x, -65504.f), 65504.f);
+    if (fabsf(v.y) < __int_as_float(0x7f800000)) v.y = fminf(fmaxf(v.y, -65504.f), 65504.f);
+    const __half2 h = __floats2half2_rn(v.x, v.y);
     w[i] = *reinterpret_cast<const uint32_t*>(&h);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Rows [r0, r0 + n) of the expert's slots, as fp16 in the order in which lanes take them: 16-byte pieces of 8 columns, piece
-// (step, jj, row, t) = columns step * 256 + t * 64 + jj * 8 ..; columns past K are zeros.  The multiplying warps; ends with a barrier.
+// Rows [first, first + n) of the slots, as fp16 in the order in which lanes take them: 16-byte pieces of 8 columns, piece
+// (step, jj, row, t) = columns step * 256 + t * 64 + jj * 8 ..; columns past K are zeros.  The multiplying warps, which share out the
+// rows, several to a row where there are few; ends with a barrier.
 template <typename T>
-__device__ __forceinline__ void stage_rows(const MoeParams& p, MoeCtl* ctl, int first, int n, int turn, uint4* xs) {
-  const int tid = threadIdx.x, lane = tid & 31;
-  const int pieces = p.steps * 32;  // of a row: a multiple of the warp, so that a warp's pieces are of one row
+__device__ __noinline__ void stage_rows(const MoeParams& p, MoeCtl* ctl, int expert, int first, int n, int turn, uint4* xs) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int pieces = p.steps * 32, K = (int)p.K, row_pitch = p.pass_rows * 4;
   int* amax = ctl->amax[turn & 1];
-  consumer_sync();  // the rows before these have been used
+  if (turn > 0) consumer_sync();  // the rows before these have been used
   if (tid < kMoeRows) ctl->amax[(turn + 1) & 1][tid] = 0;
-  for (int i = tid; i < n * pieces; i += kMoeConsumers) {
-    const int r = i / pieces, q = i - r * pieces;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (q * 8 < p.K) load8(act_row<T>(p, ctl->slot[first + r]) + q * 8, v);
-    if constexpr (!std::is_same<T, __half>::value) {
-      float m = 0.f;
+  if (tid < n) {
+    const float alpha = p.alpha ? __ldg(p.alpha + expert) : 1.f;
+    ctl->factor[tid] = std::is_same<T, float>::value ? alpha * __ldg(p.weights + ctl->slot[first + tid]) : alpha;
+  }
+  const int share = n > 8 ? 0 : n > 4 ? 1 : n > 2 ? 2 : n > 1 ? 3 : 4;  // 2^share warps to a row
+  constexpr int kAhead = 4;  // pieces that are asked for before the first is converted
+  for (int r = warp >> share; r < n; r += kMoeWarps >> share) {
+    const T* src = act_row<T>(p, ctl->slot[first + r]);
+    uint32_t most = 0;
+    for (int q0 = (warp & ((1 << share) - 1)) * 32 + lane; q0 < pieces; q0 += (kAhead * 32) << share) {
+      Piece<T> x[kAhead];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(v[k]));  // (a NaN is not seen here and stays one under any power of two)
-      const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+      for (int k = 0; k < kAhead; ++k) {
+        const int q = q0 + ((k * 32) << share);
+        if (q * 8 < K) x[k].load(src + q * 8); else x[k].zero();
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int q = q0 + ((k * 32) << share);
+        if constexpr (!std::is_same<T, __half>::value) most = x[k].most(most);
+        if (q < pieces) xs[((q >> 5) * 8 + (q & 7)) * row_pitch + r * 4 + ((q >> 3) & 3)] = to_f16(x[k], pow2(kUsualShift));
+      }
+    }
+    if constexpr (!std::is_same<T, __half>::value) {
+      if constexpr (!std::is_same<T, float>::value) most = max(most << 16, most & 0xffff0000u);
+      most = __reduce_max_sync(0xffffffffu, most);
       if (lane == 0) atomicMax(&amax[r], (int)most);
     }
-    xs[(((q >> 5) * 8 + (q & 7)) * p.pass_rows + r) * 4 + ((q >> 3) & 3)] = to_f16(v, std::is_same<T, __half>::value ? 1.f : pow2(kUsualShift), true);
   }
   consumer_sync();
   if constexpr (!std::is_same<T, __half>::value) {
@@ -286,11 +327,12 @@ __device__ __forceinline__ void stage_rows(const MoeParams& p, MoeCtl* ctl, int 
       const int bits = amax[r], shift = row_shift<T>(bits);
       if (shift == kUsualShift) continue;
       again = true;
-      const bool fine = (bits >> 23) != 0xff;
-      for (int q = tid; q * 8 < p.K; q += kMoeConsumers) {
-        float v[8];
-        load8(act_row<T>(p, ctl->slot[first + r]) + q * 8, v);
-        xs[(((q >> 5) * 8 + (q & 7)) * p.pass_rows + r) * 4 + ((q >> 3) & 3)] = to_f16(v, pow2(shift), fine);
+      const bool fine = bits < 0x7f800000;
+      const T* src = act_row<T>(p, ctl->slot[first + r]);
+      for (int q = tid; q * 8 < K; q += kMoeConsumers) {
+        Piece<T> x;
+        x.load(src + q * 8);
+        xs[((q >> 5) * 8 + (q & 7)) * row_pitch + r * 4 + ((q >> 3) & 3)] = fine ? to_f16(x, pow2(shift)) : to_f16_clamped(x);
       }
     }
     if (again) consumer_sync();  // (the same for all threads)
@@ -332,16 +374,16 @@ __device__ __noinline__ void sum_slots(const MoeParams& p, int col0, int cols) {
   }
 }
 
-// acc += weights of a step times the staged rows (`b`: this lane's pieces, `stride` apart).  181 instructions with the loads from
+// acc += weights of a step times the staged rows, 8 NT of them (`b`: this lane's pieces, `stride` apart).  181 instructions with the loads from
 // shared memory, 64 of them conversions and 64 scalings, for 16 x 256 weights: an SM that does nothing else takes 8.2 TB/s of weights so
 // (two tiles a warp, which share the pieces of x: 9.3, but half as many stages fit).
-__device__ __forceinline__ void multiply(float (&acc)[4], const uint4 (&code)[2][2], const uint32_t (&scale)[2], const uint4* b, int stride) {
+template <int NT>
+__device__ __forceinline__ void multiply(float (&acc)[NT][4], const uint4 (&code)[2][2], const uint32_t (&scale)[2], const uint4* b, int stride) {
   uint32_t s2[2][2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) s2[u][0] = cvt_f16x2_e4m3x2(scale[u]), s2[u][1] = cvt_f16x2_e4m3x2(scale[u] >> 16);
 #pragma unroll
   for (int jj = 0; jj < 8; ++jj) {
-    const uint4 x = b[jj * stride];
     uint32_t a[2][4];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -351,25 +393,32 @@ __device__ __forceinline__ void multiply(float (&acc)[4], const uint4 (&code)[2]
 #pragma unroll
       for (int i = 0; i < 4; ++i) a[u][i] = hmul2(a[u][i], s);
     }
-    mma_f16(acc, a[0][0], a[1][0], a[0][1], a[1][1], x.x, x.y);
-    mma_f16(acc, a[0][2], a[1][2], a[0][3], a[1][3], x.z, x.w);
+#pragma unroll
+    for (int q = 0; q < NT; ++q) {
+      const uint4 x = b[jj * stride + q * 32];
+      mma_f16(acc[q], a[0][0], a[1][0], a[0][1], a[1][1], x.x, x.y);
+      mma_f16(acc[q], a[0][2], a[1][2], a[0][3], a[1][3], x.z, x.w);
+    }
   }
 }
 
 // kWhole: K is a multiple of a step.  kUp: T is the activations' type and a tile is 8 gate and the 8 matching up rows; else T is float (h) and OutT the output's type.
-template <typename T, typename OutT, bool kUp, bool kWhole>
+template <typename T, typename OutT, bool kUp, bool kWhole, int NT>
 __global__ void __launch_bounds__(kMoeThreads, 1)
-    fp4_experts_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s, const MoeParams p) {
+    fp4_experts_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s,
+                       const __grid_constant__ MoeParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint4* xs = reinterpret_cast<uint4*>(ring + p.stages * kStageBytes);
-  float* red = reinterpret_cast<float*>(xs + p.steps * 32 * p.pass_rows);  // [warp][4][32]
-  MoeCtl* ctl = reinterpret_cast<MoeCtl*>(red + kMoeWarps * 128);
+  float* red = reinterpret_cast<float*>(xs + p.steps * 32 * p.pass_rows);  // [warp][4 NT][32]
+  MoeCtl* ctl = reinterpret_cast<MoeCtl*>(red + kMoeWarps * NT * 128);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const uint32_t bar_full = ptx::smem_u32(ctl->full), bar_empty = ptx::smem_u32(ctl->empty);
   const int S = p.stages;
 
-  if (tid == 0) {
+  if (tid == kMoeConsumers) {
+    ptx::tma_prefetch_desc(&map_w);
+    if constexpr (kWhole) ptx::tma_prefetch_desc(&map_s);
     for (int s = 0; s < S; ++s) ptx::mbar_init(bar_full + s * 8, 1), ptx::mbar_init(bar_empty + s * 8, kMoeWarps);
     ctl->abort_flag = 0;
     ptx::mbar_fence_init();
@@ -389,7 +438,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
   const int tiles = (int)(p.rows / 16);  // of an expert (16 rows of w each)
   const int items = ctl->num_live * p.sets, turns = (p.steps + warps_k - 1) / warps_k;
   // A CTA takes neighbouring items, which are mostly of one expert.
-  const int item0 = (int)((int64_t)blockIdx.x * items / gridDim.x), item1 = (int)((int64_t)(blockIdx.x + 1) * items / gridDim.x);
+  const int each = (int)((uint32_t)items / gridDim.x), more = items - each * (int)gridDim.x;
+  const int item0 = (int)blockIdx.x * each + min((int)blockIdx.x, more), item1 = item0 + each + ((int)blockIdx.x < more ? 1 : 0);
 
   if (warp == kMoeWarps) {
     // ------------------------------ weights ------------------------------
@@ -474,11 +524,14 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
         };
         if constexpr (!kWhole) ask(sc[0]), ask(sc[1]);
         if (staged_live != live || staged_r0 != r0) {
-          stage_rows<T>(p, ctl, first + r0, n, stagings, xs);
+          stage_rows<T>(p, ctl, expert, first + r0, n, stagings, xs);
           ++stagings, staged_live = live, staged_r0 = r0;
         }
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        const uint4* b = xs + (wk * 8 * p.pass_rows + (g < n ? g : 0)) * 4 + t;  // (columns without a row are not looked at)
+        float acc[NT][4];
+#pragma unroll
+        for (int q = 0; q < NT; ++q) acc[q][0] = acc[q][1] = acc[q][2] = acc[q][3] = 0.f;
+        // (columns without a row are not looked at: they read what lies there, or row 0 where less than eight rows fit)
+        const uint4* b = xs + (wk * 8 * p.pass_rows + (g < p.pass_rows ? g : 0)) * 4 + t;
         const int stride = p.pass_rows * 4;
         const auto step = [&](uint32_t (&scale)[2], bool mine) {
           if (ok && !ptx::mbar_test(bar_full + s * 8, ph)) ok = ptx::mbar_wait_quiet(bar_full + s * 8, ph);
@@ -488,7 +541,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
           __syncwarp();
           ptx::mbar_arrive_if(bar_empty + s * 8, lane == 0);
           if (++s == S) s = 0, ph ^= 1;
-          if (mine) multiply(acc, code, scale, b, stride);
+          if (mine) multiply<NT>(acc, code, scale, b, stride);
           b += warps_k * 8 * stride;
           if constexpr (!kWhole) ask(scale);
         };
@@ -499,36 +552,39 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
         }
         // Lane (g, t) has rows g (acc 0, 1) and g + 8 (2, 3) of columns 2 t, 2 t + 1.  A warp of those that split K adds up two
         // values of each of their lanes.
-        const float alpha = p.alpha ? p.alpha[expert] : 1.f;
-        const auto finish = [&](int tile, int r, int row, float lo, float hi) {
+        const auto finish = [&](int tile, int r, float lo, float hi) {
           if (tile >= tiles || r >= n) return;
-          const float f = pow2(-row_shift<T>(ctl->amax[(stagings - 1) & 1][r]));
-          lo = lo * alpha * f, hi = hi * alpha * f;
+          const float f = ctl->factor[r], unscale = pow2(-row_shift<T>(ctl->amax[(stagings - 1) & 1][r]));
+          lo = lo * f * unscale, hi = hi * f * unscale;
           const int slot = ctl->slot[first + r0 + r];
           if constexpr (kUp) {
-            p.h[(int64_t)slot * (p.rows / 2) + tile * 8 + row] = lo / (1.f + expf(-lo)) * hi;
+            p.h[(int64_t)slot * (p.rows / 2) + tile * 8 + g] = lo / (1.f + expf(-lo)) * hi;
           } else {
-            const float weight = p.weights[slot];
-            float* at = p.h + (int64_t)slot * p.rows + tile * 16 + row;
-            at[0] = weight * lo, at[8] = weight * hi;
+            float* at = p.h + (int64_t)slot * p.rows + tile * 16 + g;
+            at[0] = lo, at[8] = hi;
           }
         };
         if (warps_k == 1) {
-          finish(my_tile, 2 * t, g, acc[0], acc[2]);
-          finish(my_tile, 2 * t + 1, g, acc[1], acc[3]);
+#pragma unroll
+          for (int q = 0; q < NT; ++q) {
+            finish(my_tile, 8 * q + 2 * t, acc[q][0], acc[q][2]);
+            finish(my_tile, 8 * q + 2 * t + 1, acc[q][1], acc[q][3]);
+          }
         } else {
           consumer_sync();  // (the sums before these have been read)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) red[(warp * 4 + j) * 32 + lane] = acc[j];
+          for (int q = 0; q < NT; ++q)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) red[((warp * NT + q) * 4 + j) * 32 + lane] = acc[q][j];
           consumer_sync();
-          for (int i = tid; i < warps_m * 64; i += kMoeConsumers) {
-            const int j = (i >> 5) & 1, m = i >> 6;  // (i % 32 == lane)
+          for (int i = tid; i < warps_m * NT * 64; i += kMoeConsumers) {
+            const int j = (i >> 5) & 1, q = (i >> 6) % NT, m = (i >> 6) / NT;  // (i % 32 == lane)
             float lo = 0.f, hi = 0.f;
             for (int k = 0; k < warps_k; ++k) {
-              const float* at = red + ((m * warps_k + k) * 4 + j) * 32 + lane;
+              const float* at = red + (((m * warps_k + k) * NT + q) * 4 + j) * 32 + lane;
               lo += at[0], hi += at[64];
             }
-            finish(set * warps_m + m, 2 * t + j, g, lo, hi);
+            finish(set * warps_m + m, 8 * q + 2 * t + j, lo, hi);
           }
         }
       }
@@ -564,7 +620,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
 }
 
 constexpr int64_t moe_smem(int steps, int pass_rows, int stages) {
-  return 1024 + (int64_t)stages * kStageBytes + (int64_t)steps * 512 * pass_rows + kMoeWarps * 512 + (int64_t)sizeof(MoeCtl);
+  return 1024 + (int64_t)stages * kStageBytes + (int64_t)steps * 512 * pass_rows + kMoeWarps * 512 * ((pass_rows + 7) / 8) + (int64_t)sizeof(MoeCtl);
 }
 constexpr int64_t kMoeMostSmem = 227 * 1024;
 
@@ -585,17 +641,19 @@ static int plan_product(MoeParams& p, int64_t K, int64_t rows) {
   while (p.warps_k < kMoeWarps && p.warps_k < p.steps && live * (double)(rows / 16) * p.warps_k / kMoeWarps < 0.85 * sm_count()) p.warps_k *= 2;
   const int per = kMoeWarps / p.warps_k;
   p.sets = (int)((rows / 16 + per - 1) / per);
-  p.pass_rows = kMoeRows;
-  while (p.pass_rows > 1 && (moe_smem(p.steps, p.pass_rows, 4) > kMoeMostSmem || p.pass_rows >= 2 * p.slots)) p.pass_rows /= 2;
+  // Rows per pass: every pass reads the weights again (from the L2), and rows take the place of stages.
+  const double rows_each = p.slots / live;
+  p.pass_rows = rows_each > 12 ? 32 : rows_each > 6 ? 16 : 8;
+  while (p.pass_rows > 1 && (moe_smem(p.steps, p.pass_rows, p.pass_rows > 8 ? 2 : 4) > kMoeMostSmem || p.pass_rows >= 2 * p.slots)) p.pass_rows /= 2;
   p.stages = kMoeMaxStages;
   while (p.stages > 2 && moe_smem(p.steps, p.pass_rows, p.stages) > kMoeMostSmem) --p.stages;
   SGLB_REQUIRE(moe_smem(p.steps, p.pass_rows, p.stages) <= kMoeMostSmem, "fused_experts_fp4: %lld columns are too many", (long long)K);
   return SGLB200_OK;
 }
 
-template <typename T, typename OutT, bool kUp, bool kWhole>
+template <typename T, typename OutT, bool kUp, bool kWhole, int NT>
 static int launch_experts(const CUtensorMap& map_w, const CUtensorMap& map_s, const MoeParams& p, cudaStream_t st) {
-  auto kern = fp4_experts_kernel<T, OutT, kUp, kWhole>;
+  auto kern = fp4_experts_kernel<T, OutT, kUp, kWhole, NT>;
   static thread_local bool attr_set[64] = {false};  // the opt-in is per function and per device
   int dev = 0;
   SGLB_CUDA(cudaGetDevice(&dev));
@@ -627,9 +685,12 @@ static int launch_product(const void* w, const MoeParams& p, cudaStream_t st) {
   CUtensorMap map_w, map_s;
   int rc = map_of(w, (uint64_t)p.K / 2, kStep / 2, true, &map_w);
   if (rc) return rc;
-  if (!whole) return launch_experts<T, OutT, kUp, false>(map_w, map_w, p, st);
-  rc = map_of(p.ws, (uint64_t)p.K / 16, kStep / 16, false, &map_s);
-  return rc ? rc : launch_experts<T, OutT, kUp, true>(map_w, map_s, p, st);
+  if (whole && (rc = map_of(p.ws, (uint64_t)p.K / 16, kStep / 16, false, &map_s)) != SGLB200_OK) return rc;
+#define GO(NT) return whole ? launch_experts<T, OutT, kUp, true, NT>(map_w, map_s, p, st) : launch_experts<T, OutT, kUp, false, NT>(map_w, map_w, p, st)
+  if (p.pass_rows <= 8) GO(1);
+  if (p.pass_rows <= 16) GO(2);
+  GO(4);
+#undef GO
 }
 
 }  // namespace fp4

@@ -1,9 +1,10 @@
 // Products of 4-bit operands:  C[m, n] = out_t( alpha * sum_k a[m, k] * b[n, k] + bias[n] ),  a and b e2m1 codes times the scale of
 // their group, on tcgen05.mma.kind::mxf4nvf4, which takes the scales from tensor memory and applies them inside the MMA.
 //
-// fp4_rows_kernel: the weights on the M side (128 of their rows), NT activation rows on the N side, so that nothing is multiplied
+// Many rows go to pairs of CTAs (fp4_pair.cu).  fp4_rows_kernel, for few rows or few tiles: the weights on the M side (128 of their rows), NT activation rows on the N side, so that nothing is multiplied
 // for padding of few rows up to 128; K split over the CTAs of a cluster, which add their partial sums through distributed shared
-// memory in a fixed order.
+// memory in a fixed order; without a split the sums go from tensor memory straight to the output.  Two CTAs an SM, each with a ring
+// of 80 to 100 KB: 1 x 36864 x 7168 takes 25.1 us (0.90 of the measured copy rate), 64 rows 28.8 (0.82), of which three are start and end.
 #include <algorithm>
 
 #include "fp4_gemm.cuh"
@@ -36,6 +37,44 @@ struct RowsCtl {
   uint32_t tmem_base;
   int abort_flag;
 };
+
+__device__ __forceinline__ float load_bias(const Params& p, int n) {
+  return p.out_fp16 ? __half2float(static_cast<const __half*>(p.bias)[n]) : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[n]);
+}
+__device__ __forceinline__ uint16_t round_out(const Params& p, float v) {
+  return p.out_fp16 ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+__device__ __forceinline__ void store_out(const Params& p, int64_t at, float v) { static_cast<uint16_t*>(p.C)[at] = round_out(p, v); }
+
+// The output of a tile whose K was split over the CTAs of a cluster: their partial sums ([column][kPartPitch weight rows] at `part` in
+// every CTA's shared memory) in ascending K order, the bias, one rounding.  CTA `rank` adds columns rank, rank + splits, ..; a thread
+// four neighbouring weight rows of a column, whose parts are all requested before the first is added.
+__device__ __forceinline__ void sum_parts(const Params& p, int n_tile, int row0, int cols, int rank, uint32_t part, int tid) {
+  const int splits = p.splits, mine = (cols - rank + splits - 1) / splits;
+  for (int i = tid; i < mine * 32; i += kRowsThreads) {
+    const int col = rank + (i >> 5) * splits, quad = (i & 31) * 4, n = n_tile * 128 + quad;
+    if (n >= p.N) continue;  // (N is a multiple of 8)
+    const uint32_t at = part + (col * kPartPitch + quad) * 4;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = 0; s0 < splits; s0 += 8) {
+      float4 v[8];
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+        if (s0 + s < splits) {
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v[s].x), "=f"(v[s].y), "=f"(v[s].z), "=f"(v[s].w)
+                       : "r"(ptx::cluster_map(at, s0 + s))
+                       : "memory");
+        }
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+        if (s0 + s < splits) sum.x += v[s].x, sum.y += v[s].y, sum.z += v[s].z, sum.w += v[s].w;
+    }
+    if (p.bias != nullptr) sum.x += load_bias(p, n), sum.y += load_bias(p, n + 1), sum.z += load_bias(p, n + 2), sum.w += load_bias(p, n + 3);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.C) + (int64_t)(row0 + col) * p.N + n) =
+        make_uint2(round_out(p, sum.x) | (uint32_t)round_out(p, sum.y) << 16, round_out(p, sum.z) | (uint32_t)round_out(p, sum.w) << 16);
+  }
+}
 
 template <class Cfg>
 __global__ void __launch_bounds__(kRowsThreads, 2)
@@ -129,27 +168,35 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
       *abort_flag = 1;
     } else {
       ptx::tc_fence_after();
-      const float alpha = p.alpha ? *p.alpha : 1.0f;
+      const float alpha = p.alpha ? __ldg(p.alpha) : 1.0f;
+      const int n = n_tile * 128 + warp * 32 + lane, m0 = m_tile * NT;
+      const float bias = splits == 1 && p.bias != nullptr && n < p.N ? load_bias(p, n) : 0.f;
       float* part = reinterpret_cast<float*>(ring) + warp * 32 + lane;  // the operands have been consumed
 #pragma unroll
       for (int c = 0; c < NT; c += 16) {
+        if (m0 + c >= p.M) break;  // (columns past the last row are nobody's)
         uint32_t r[16];
         ptx::tmem_ld_32x16(tmem + ((uint32_t)(warp * 32) << 16) + c, r);
         ptx::tmem_ld_wait();
+        if (splits == 1) {  // a warp stores 32 neighbouring values of a row
 #pragma unroll
-        for (int j = 0; j < 16; ++j) part[(c + j) * kPartPitch] = alpha * __uint_as_float(r[j]);
+          for (int j = 0; j < 16; ++j)
+            if (n < p.N && m0 + c + j < p.M) store_out(p, (int64_t)(m0 + c + j) * p.N + n, alpha * __uint_as_float(r[j]) + bias);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) part[(c + j) * kPartPitch] = alpha * __uint_as_float(r[j]);
+        }
       }
       ptx::tc_fence_before();
     }
   }
 
   __syncwarp();
-  RowsParams rp{};
-  rp.C = p.C, rp.bias = p.bias, rp.M = p.M, rp.N = p.N, rp.splits = splits, rp.out_fp16 = p.out_fp16;
-  const RowsTile t{n_tile, m_tile * NT, NT, 0};
-  if (splits > 1) ptx::cluster_sync(); else __syncthreads();
-  if (ctl->abort_flag == 0) rows_cluster_sum<kMostClusterCtas>(rp, t, rank, ptx::smem_u32(ring), tid, kRowsThreads);
-  if (splits > 1) ptx::cluster_sync();  // no CTA leaves while another reads its shared memory
+  if (splits > 1) {
+    ptx::cluster_sync();
+    if (ctl->abort_flag == 0) sum_parts(p, n_tile, m_tile * NT, min(NT, (int)p.M - m_tile * NT), rank, ptx::smem_u32(ring), tid);
+    ptx::cluster_sync();  // no CTA leaves while another reads its shared memory
+  }
 
   ptx::tc_fence_before();
   __syncthreads();
@@ -206,12 +253,31 @@ static int launch_rows(const void* A, const void* B, Params& p, cudaStream_t st)
   return SGLB200_OK;
 }
 
+// Columns of a pair's tile: as many waves of them as there are, times the time of a wave in hundredths of a microsecond (0.46 a slab
+// for 256 columns, 0.39 for 192, 0.33 for 128, and half a microsecond).  us over 256, 192 and 128: 4096 x 36864 x 7168 387, 433, 570;
+// 257 x 10240 x 8192 29.0, 27.6, 35.9; 1024 x 10240 x 8192 42, 40, 57; 1024 x 2112 x 7168 15.3, 15.3, 14.7; 257 x 36864 x 7168 56, 65, 78.
+static int pair_columns(const Params& p) {
+  const int64_t pairs = std::max<int64_t>(1, cluster_fits().alone[2]), tiles_m = (p.M + 255) / 256;
+  int best = 256;
+  int64_t best_cost = -1;
+  for (int bn = 256; bn >= 128; bn -= 64) {
+    const int64_t waves = (tiles_m * ((p.N + bn - 1) / bn) + pairs - 1) / pairs;
+    const int64_t cost = waves * (p.kb_total * (bn == 256 ? 46 : bn == 192 ? 39 : 33) + 50);
+    if (best_cost < 0 || cost < best_cost) best = bn, best_cost = cost;
+  }
+  return best;
+}
+
+// Up to 64 rows the weights on the M side.  Above that likewise, 64 rows a tile, where that makes no more tiles than SMs (their K is
+// then split over clusters: 128 x 512 x 8192 6.6 us, by pairs 14.2; 512 x 2112 x 7168 13.5 and 14.3; but 65 x 10240 x 8192, 160 tiles,
+// 22.6 and 17.0), and 128 rows a tile up to 128 rows (65 x 36864 x 7168 31.5 and 32.9; 128 rows 34.0 and 34.7); else pairs.
 template <int G>
 static int scaled_mm(const void* A, const void* B, Params& p, cudaStream_t st) {
   if (p.M <= 16) return launch_rows<RowsCfg<16, G>>(A, B, p, st);
   if (p.M <= 32) return launch_rows<RowsCfg<32, G>>(A, B, p, st);
-  if (p.M <= 64) return launch_rows<RowsCfg<64, G>>(A, B, p, st);
-  return launch_rows<RowsCfg<128, G>>(A, B, p, st);
+  if (p.M <= 64 || (p.M + 63) / 64 * ((p.N + 127) / 128) <= sm_count()) return launch_rows<RowsCfg<64, G>>(A, B, p, st);
+  if (p.M <= 128) return launch_rows<RowsCfg<128, G>>(A, B, p, st);
+  return pair_mm(A, B, p, G, pair_columns(p), st);
 }
 
 }  // namespace fp4
@@ -219,12 +285,12 @@ static int scaled_mm(const void* A, const void* B, Params& p, cudaStream_t st) {
 int fp4_gemm_status() {
   int v = 0;
   if (cudaMemcpyFromSymbol(&v, fp4::g_fp4_status, sizeof(int)) != cudaSuccess) return -1;
-  return v;
+  return v != 0 ? v : fp4_pair_status();
 }
 int fp4_gemm_status_clear() {
   const int zero = 0;
   SGLB_CUDA(cudaMemcpyToSymbol(fp4::g_fp4_status, &zero, sizeof(int)));
-  return SGLB200_OK;
+  return fp4_pair_status_clear();
 }
 
 }  // namespace sglb200

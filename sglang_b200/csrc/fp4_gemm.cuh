@@ -90,5 +90,12 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
   (p.wait_probes != ptx::kProbesNone && (ptx::mbar_test(bar, parity) || ptx::mbar_wait_quiet(bar, parity)))
 
 
+// fp4_pair.cu: the product by pairs of CTAs, in tiles of 256 rows x `bn` (128, 192 or 256) columns.
+int pair_mm(const void* A, const void* B, Params& p, int group_size, int bn, cudaStream_t st);
+
 }  // namespace fp4
+
+int fp4_pair_status();
+int fp4_pair_status_clear();
+
 }  // namespace sglb200

@@ -68,8 +68,16 @@ def test_matmul_large(M, N, K):
     _check(M, N, K, 16, torch.bfloat16, alpha=2.0**-12, bias=True, seed=3)
 
 
+# tiles of 256 rows by pairs of CTAs: 256, 192 and 128 columns, ragged ends of every kind, one tile and several a pair
 @pytest.mark.parametrize("group", [16, 32])
-@pytest.mark.parametrize("M,N,K", [(5, 136, 160), (64, 256, 1024), (200, 320, 608), (700, 1040, 1024)])
+@pytest.mark.parametrize("M,N,K,columns", [(257, 10240, 1056, 192), (129, 20000, 288, 256), (1024, 5000, 544, 256), (1100, 1928, 96, 128),
+                                           (8200, 520, 32, 128), (3000, 9224, 2080, 256), (513, 9432, 1312, 192)])
+def test_matmul_pairs(M, N, K, columns, group):
+    _check(M, N, K, group, torch.bfloat16, alpha=2.0**-10, bias=group == 16, seed=columns)
+
+
+@pytest.mark.parametrize("group", [16, 32])
+@pytest.mark.parametrize("M,N,K", [(5, 136, 160), (64, 256, 1024), (200, 320, 608), (700, 1040, 1024), (2048, 4104, 1024), (300, 9432, 544)])
 def test_matmul_exact(M, N, K, group):
     """Scales of one and values that are multiples of a half: every partial sum is a multiple of 1/4 below 2^22, so float32 sums
     are exact and the output is the exact sum, rounded once."""
@@ -154,7 +162,7 @@ def test_quantise_multiply_activate_multiply():
         assert (np.abs(hd.cpu().numpy() - exact) <= amax * (1 / 6 + 1 / 16)).all()
 
 
-@pytest.mark.parametrize("M,N,K", [(16, 7168, 4096), (64, 1024, 8192), (300, 512, 1024), (1024, 1024, 2048)])
+@pytest.mark.parametrize("M,N,K", [(16, 7168, 4096), (64, 1024, 8192), (300, 512, 1024), (2048, 4096, 2048), (300, 10240, 4096)])
 def test_wait_runs_out_and_recovers(M, N, K):
     from sglang_b200 import ops
     from sglang_b200._lib import check, lib
@@ -182,7 +190,7 @@ def test_captured_and_replayed_on_two_streams():
     """Two captured graphs and eager calls between them, each with inputs of its own."""
     from sglang_b200 import ops
     sets = []
-    for seed, (M, N, K) in enumerate([(8, 2112, 7168), (520, 1024, 2048)]):
+    for seed, (M, N, K) in enumerate([(8, 2112, 7168), (520, 10240, 2048)]):
         a, sa, _ = _operand(M, K, 16, 2 * seed)
         b, sb, _ = _operand(N, K, 16, 2 * seed + 1)
         want = ops.w4a4_group_fp4_matmul(a, b, sa, sb)

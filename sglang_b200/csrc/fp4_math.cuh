@@ -108,23 +108,39 @@ __device__ __forceinline__ uint32_t group_scale_e4m3(float amax, float g) {
   return lo;
 }
 
+// (a, b) times r, both products in one instruction.
+__device__ __forceinline__ void mul2(float& a, float& b, float x, float y, float r) {
+  asm("{\n\t.reg .b64 v, f, q;\n\t"
+      "mov.b64 v, {%2, %3};\n\t"
+      "mov.b64 f, {%4, %4};\n\t"
+      "mul.rn.f32x2 q, v, f;\n\t"
+      "mov.b64 {%0, %1}, q;\n\t}"
+      : "=f"(a), "=f"(b)
+      : "f"(x), "f"(y), "f"(r));
+}
+
+// x[i] of eight registers.
+__device__ __forceinline__ float pick(const float (&x)[8], uint32_t i) {
+  const bool b0 = i & 1, b1 = i & 2, b2 = i & 4;
+  const float a = b0 ? x[1] : x[0], b = b0 ? x[3] : x[2], c = b0 ? x[5] : x[4], d = b0 ? x[7] : x[6];
+  const float e = b1 ? b : a, f = b1 ? d : c;
+  return b2 ? f : e;
+}
+
 // Codes of eight values x under scale s (not 0) and the tensor's scale g: e2m1 nearest to x * g / s, decided likewise.
-// `r_lo`, `r_hi`: g / s a little too small and too large.
+// `r_lo`, `r_hi`: g / s a little too small and too large.  Where the two codes of a value differ the exact product decides, one value
+// after the other: g of few bits, or quotients of such as calibration gives, puts some value of a warp next to a border more often
+// than not, though seldom two of a thread (all eight unrolled: 8192 x 18432 in 117 us).
 __device__ __forceinline__ uint32_t codes_x8(const float (&x)[8], float r_lo, float r_hi, float s, float g) {
   float a[8], b[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a[i] = x[i] * r_lo, b[i] = x[i] * r_hi;
-  uint32_t lo = cvt_e2m1x8(a);
-  const uint32_t hi = cvt_e2m1x8(b);
-  if (lo != hi) {  // some value is within 2^-20 of a border
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t c = lo >> (4 * i) & 7;
-      if (c != (hi >> (4 * i) & 7)) {
-        const float over = fmaf(fabsf(x[i]), g, -e2m1_border(c) * s);
-        if (over > 0.f || (over == 0.f && (c & 1))) lo += 1u << (4 * i);
-      }
-    }
+  for (int i = 0; i < 8; i += 2) mul2(a[i], a[i + 1], x[i], x[i + 1], r_lo), mul2(b[i], b[i + 1], x[i], x[i + 1], r_hi);
+  uint32_t lo = cvt_e2m1x8(a), differ = lo ^ cvt_e2m1x8(b);
+  while (differ != 0) {
+    const uint32_t at = (__ffs(differ) - 1) & ~3u, c = lo >> at & 7;
+    const float over = fmaf(fabsf(pick(x, at >> 2)), g, -e2m1_border(c) * s);
+    if (over > 0.f || (over == 0.f && (c & 1))) lo += 1u << at;
+    differ &= ~(15u << at);
   }
   return lo;
 }

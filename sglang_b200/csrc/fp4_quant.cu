@@ -6,8 +6,10 @@
 // Every rounding is to nearest with ties to even and decided on exact numbers; a group whose scale is zero has zero codes, and one
 // that holds a NaN or an infinity has the scale NaN, so that no product hides it.
 //
-// All of them are bound by HBM: 2 bytes an element in and 0.5625 out (bf16, groups of 16).  A thread takes 16 columns of one row,
-// so a group of 16 needs no exchange and one of 32 a shuffle with the neighbour.
+// All of them are bound by HBM: 2 bytes an element in and 0.5625 out (bf16, groups of 16).  A thread takes 16 columns of a row, so a
+// group of 16 needs no exchange and one of 32 a shuffle with the neighbour.  A warp takes the 64 columns of a scale block in the
+// eight rows whose scales fill one 32-byte sector of it (rows r, r + 1 and those 32, 64 and 96 further), so that every sector it
+// touches, of values, codes and scales, is whole; with 32 columns a group it is 128 columns of four rows.
 #include <algorithm>
 #include <type_traits>
 
@@ -18,7 +20,7 @@ namespace sglb200 {
 namespace fp4 {
 
 constexpr int kThreads = 256;
-constexpr int64_t kMaxUnits = 1ll << 31;
+constexpr int64_t kMostScales = 1ll << 30;  // of a launch, in bytes (a block of 512 is at most 32 tasks)
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -26,44 +28,91 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// 16 consecutive elements as float32.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 32 bytes at once.
+__device__ __forceinline__ void ld_32(const void* p, uint32_t (&v)[8]) {
+  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void st_32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+               "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// 16 elements as they lie in memory.  kWide: they begin on 32 bytes.
 template <typename T>
-__device__ __forceinline__ void load16(const T* src, float (&v)[16]) {
-  if constexpr (sizeof(T) == 4) {
+struct Raw {
+  uint32_t w[sizeof(T) * 4];
+  template <bool kWide>
+  __device__ __forceinline__ void load(const T* src) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint4 q = ld_nc_16(src + 4 * j);
-      v[4 * j] = __uint_as_float(q.x), v[4 * j + 1] = __uint_as_float(q.y);
-      v[4 * j + 2] = __uint_as_float(q.z), v[4 * j + 3] = __uint_as_float(q.w);
+    for (int j = 0; j < (int)sizeof(T) / 2; ++j) {
+      uint32_t v[8];
+      if constexpr (kWide) {
+        ld_32(reinterpret_cast<const uint8_t*>(src) + 32 * j, v);
+      } else {
+        const uint4 a = ld_nc_16(reinterpret_cast<const uint8_t*>(src) + 32 * j), b = ld_nc_16(reinterpret_cast<const uint8_t*>(src) + 32 * j + 16);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[8 * j + i] = v[i];
     }
-  } else {
+  }
+  __device__ __forceinline__ void to_f32(float (&v)[16]) const {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const uint4 q = ld_nc_16(src + 8 * j);
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (std::is_same<T, __half>::value) {
-          const float2 f = f16x2_to_f32(w[i]);
-          v[8 * j + 2 * i] = f.x, v[8 * j + 2 * i + 1] = f.y;
-        } else {
-          v[8 * j + 2 * i] = __uint_as_float(w[i] << 16), v[8 * j + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        v[2 * i] = __uint_as_float(w[2 * i]), v[2 * i + 1] = __uint_as_float(w[2 * i + 1]);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = f16x2_to_f32(w[i]);
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+      } else {
+        v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
       }
     }
   }
-}
+};
 
-// Quantises this thread's 16 values and stores codes and scale.  All lanes of the warp take part where the group is 32.
+// Where a lane works: 16 columns of a row.  A warp's task is a block of scales (64 or 128 columns) in the rows of its block of 128
+// whose scales are neighbours.
 template <int kGroup>
-__device__ __forceinline__ void quantize16(const float (&v)[16], float g, uint2* codes, uint8_t* scales, int64_t row, int unit,
-                                           int units, int group_blocks, bool live) {
-  float amax = 0.f;
+struct Place {
+  static constexpr int kUnits = 4 * kGroup / kUnit;  // of a block in a row
+  static constexpr int kRows = 32 / kUnits;          // of a task: 8 or 4
+  static constexpr int kTasks = 128 / kRows;         // of a block of 128 rows and a block of scales
+  int64_t unit;                                      // of the tensor; the first one where this lane has none
+  uint32_t scale;                                    // where its scale lies, from the first of this launch
+  uint32_t column;                                   // of the row, in units
+  bool row_live, live;                               // whether there is such a row, and such columns in it
+  Place() = default;
+  // `rows`: of this launch.
+  __device__ __forceinline__ Place(uint32_t task, const FastDiv& blocks, uint32_t units, int rows) {
+    const uint32_t lane = threadIdx.x & 31, u = lane % kUnits, r = lane / kUnits;
+    const uint32_t set = blocks.quot(task), block = task - set * blocks.d;  // set: (block of rows, rows of it)
+    const uint32_t low = set % kTasks * (kRows / 4) + r / 4, quarter = r % 4, row = set / kTasks * 128 + quarter * 32 + low;
+    column = block * kUnits + u;
+    row_live = (int)row < rows, live = row_live && column < units;
+    unit = live ? (int64_t)((uint64_t)row * units + column) : 0;
+    scale = (set / kTasks * blocks.d + block) * kBlockBytes + low * 16 + quarter * 4 + u / (kGroup / kUnit);
+  }
+};
+
+// Quantises this thread's 16 values; the code of the scale.  The lanes of a warp whose group takes two of them go together.
+template <int kGroup>
+__device__ __forceinline__ uint32_t quantize16(const float (&v)[16], float g, uint2& out) {
+  float amax = max_nan(fabsf(v[0]), fabsf(v[1]));
 #pragma unroll
-  for (int i = 0; i < 16; ++i) amax = max_nan(amax, fabsf(v[i]));
+  for (int i = 2; i < 16; i += 2) amax = max3_nan(amax, fabsf(v[i]), fabsf(v[i + 1]));
   const float(&x0)[8] = *reinterpret_cast<const float(*)[8]>(&v[0]);
   const float(&x1)[8] = *reinterpret_cast<const float(*)[8]>(&v[8]);
-  uint2 out = make_uint2(0u, 0u);
+  out = make_uint2(0u, 0u);
   uint32_t code;
   if constexpr (kGroup == 32) {
     amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
@@ -74,7 +123,7 @@ __device__ __forceinline__ void quantize16(const float (&v)[16], float g, uint2*
     if (fine) {
       float a[8], b[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] = x0[i] * r, b[i] = x1[i] * r;
+      for (int i = 0; i < 8; i += 2) mul2(a[i], a[i + 1], x0[i], x0[i + 1], r), mul2(b[i], b[i + 1], x1[i], x1[i + 1], r);
       out = make_uint2(cvt_e2m1x8(a), cvt_e2m1x8(b));
     }
   } else {
@@ -86,108 +135,154 @@ __device__ __forceinline__ void quantize16(const float (&v)[16], float g, uint2*
       out = make_uint2(codes_x8(x0, r_lo, r_hi, s, g), codes_x8(x1, r_lo, r_hi, s, g));
     }
   }
-  if (!live) return;
-  *codes = out;
-  constexpr int kPer = kGroup / kUnit;
-  if (unit % kPer == 0) {
-    const int group = unit / kPer;
-    uint8_t* at = scales + scale_at(row, group, group_blocks);
-    *at = (uint8_t)code;
-    if (unit + kPer == units)  // the block's columns past the last group
-      for (int c = group + 1; c < 4 * group_blocks; ++c) at[c - group] = 0;
-  }
+  return code;
 }
 
-template <typename T, int kGroup, bool kSilu>
+// A warp takes kAhead tasks, whose values are all asked for before the first is quantised.
+template <typename T, int kGroup, bool kSilu, bool kWide, int kAhead>
 __global__ void __launch_bounds__(kThreads)
     quant_fp4_kernel(const T* __restrict__ x, uint2* __restrict__ codes, uint8_t* __restrict__ scales,
-                     const float* __restrict__ global_scale, uint32_t total, FastDiv units, int64_t first_row, int group_blocks) {
+                     const float* __restrict__ global_scale, uint32_t tasks, FastDiv blocks, uint32_t units, int rows) {
   ptx::grid_dependency_wait();
-  const uint32_t n = blockIdx.x * kThreads + threadIdx.x;
-  const bool live = n < total;
-  const uint32_t at = live ? n : total - 1;  // (total is even where a group takes two threads)
-  const uint32_t row = units.quot(at), unit = at - row * units.d;
-  const float g = global_scale ? *global_scale : 1.0f;
-  float v[16];
-  if constexpr (kSilu) {
-    const T* src = x + (int64_t)row * units.d * (2 * kUnit) + unit * kUnit;
-    float up[16];
-    load16(src, v);
-    load16(src + (int64_t)units.d * kUnit, up);
+  const uint32_t task0 = blockIdx.x * (kThreads / 32 * kAhead) + threadIdx.x / 32;
+  if (task0 >= tasks) return;
+  Place<kGroup> at[kAhead];
+  Raw<T> raw[kAhead][kSilu ? 2 : 1];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = v[i] / (1.0f + expf(-v[i])) * up[i];
-  } else {
-    load16(x + (int64_t)at * kUnit, v);
+  for (int k = 0; k < kAhead; ++k) {
+    at[k] = Place<kGroup>(min(task0 + k * (kThreads / 32), tasks - 1), blocks, units, rows);  // (the last one again rather than none)
+    const T* src = x + at[k].unit * kUnit;
+    if constexpr (kSilu) src += at[k].live ? (at[k].unit - at[k].column) * kUnit : 0;  // (rows of twice the columns)
+    raw[k][0].template load<kWide>(src);
+    if constexpr (kSilu) raw[k][1].template load<kWide>(src + (int64_t)units * kUnit);
   }
-  quantize16<kGroup>(v, g, codes + at, scales, first_row + row, (int)unit, (int)units.d, group_blocks, live);
+  const float g = global_scale ? __ldg(global_scale) : 1.0f;
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) {
+    if (task0 + k * (kThreads / 32) >= tasks) break;
+    float v[16];
+    raw[k][0].to_f32(v);
+    if constexpr (kSilu) {
+      float up[16];
+      raw[k][1].to_f32(up);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        // The quotient by a reciprocal and one correction: half a unit in the last place, and the instructions of a division are
+        // half of the kernel's.  Below -87, where the reciprocal is flushed to zero, it is zero.
+        const float d = fminf(1.0f + expf(-v[i]), 1e38f);
+        float r;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+        const float q = v[i] * r;
+        v[i] = fmaf(fmaf(-q, d, v[i]), r, q) * up[i];
+      }
+    }
+    uint2 c;
+    const uint32_t code = quantize16<kGroup>(v, g, c);
+    if (at[k].live) codes[at[k].unit] = c;
+    if (at[k].row_live && at[k].column % (kGroup / kUnit) == 0) scales[at[k].scale] = at[k].live ? (uint8_t)code : 0;  // (zeros for groups past the last)
+  }
 }
 
-template <typename T, int kGroup>
+template <typename T, int kGroup, bool kWide, int kAhead>
 __global__ void __launch_bounds__(kThreads)
     dequant_fp4_kernel(const uint2* __restrict__ codes, const uint8_t* __restrict__ scales, const float* __restrict__ global_scale,
-                       T* __restrict__ out, uint32_t total, FastDiv units, int64_t first_row, int group_blocks) {
+                       T* __restrict__ out, uint32_t tasks, FastDiv blocks, uint32_t units, int rows) {
   ptx::grid_dependency_wait();
-  const uint32_t n = blockIdx.x * kThreads + threadIdx.x;
-  if (n >= total) return;
-  const uint32_t row = units.quot(n), unit = n - row * units.d;
-  const uint2 c = __ldg(codes + n);
-  const uint32_t code = __ldg(scales + scale_at(first_row + row, (int)unit / (kGroup / kUnit), group_blocks));
-  float s = kGroup == 32 ? e8m0_to_f32(code) : f16x2_to_f32(cvt_f16x2_e4m3x2(code)).x;
-  if (global_scale) s = s / *global_scale;
-  uint32_t h[8];
-  cvt_f16x2_e2m1x8(c.x, *reinterpret_cast<uint32_t(*)[4]>(&h[0]));
-  cvt_f16x2_e2m1x8(c.y, *reinterpret_cast<uint32_t(*)[4]>(&h[4]));
-  T* dst = out + (int64_t)n * kUnit;
-  float v[16];
+  const uint32_t task0 = blockIdx.x * (kThreads / 32 * kAhead) + threadIdx.x / 32;
+  if (task0 >= tasks) return;
+  Place<kGroup> at[kAhead];
+  uint2 c[kAhead];
+  uint32_t code[kAhead];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 f = f16x2_to_f32(h[i]);
-    v[2 * i] = f.x * s, v[2 * i + 1] = f.y * s;
+  for (int k = 0; k < kAhead; ++k) {
+    at[k] = Place<kGroup>(min(task0 + k * (kThreads / 32), tasks - 1), blocks, units, rows);
+    c[k] = __ldg(codes + at[k].unit);
+    code[k] = at[k].live ? __ldg(scales + at[k].scale) : 0u;
   }
-  if constexpr (sizeof(T) == 4) {
+  const float g = global_scale ? __ldg(global_scale) : 1.0f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      reinterpret_cast<float4*>(dst)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-  } else {
-    union {
-      T t[16];
-      uint4 q[2];
-    } o;
+  for (int k = 0; k < kAhead; ++k) {
+    if (task0 + k * (kThreads / 32) >= tasks) break;
+    if (!at[k].live) continue;
+    float s = kGroup == 32 ? e8m0_to_f32(code[k]) : f16x2_to_f32(cvt_f16x2_e4m3x2(code[k])).x;
+    if (global_scale) s = s / g;
+    uint32_t h[8];
+    cvt_f16x2_e2m1x8(c[k].x, *reinterpret_cast<uint32_t(*)[4]>(&h[0]));
+    cvt_f16x2_e2m1x8(c[k].y, *reinterpret_cast<uint32_t(*)[4]>(&h[4]));
+    T* dst = out + at[k].unit * kUnit;
+    uint32_t o[sizeof(T) * 4];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o.t[i] = ElemTraits<T>::from_f32(v[i]);
-    reinterpret_cast<uint4*>(dst)[0] = o.q[0];
-    reinterpret_cast<uint4*>(dst)[1] = o.q[1];
+    for (int i = 0; i < 8; ++i) {
+      const float2 f = f16x2_to_f32(h[i]);
+      if constexpr (sizeof(T) == 4) {
+        o[2 * i] = __float_as_uint(f.x * s), o[2 * i + 1] = __float_as_uint(f.y * s);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        const __half2 p = __floats2half2_rn(f.x * s, f.y * s);
+        o[i] = *reinterpret_cast<const uint32_t*>(&p);
+      } else {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(f.x * s, f.y * s);
+        o[i] = *reinterpret_cast<const uint32_t*>(&p);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(T) / 2; ++j) {
+      const uint32_t(&part)[8] = *reinterpret_cast<const uint32_t(*)[8]>(&o[8 * j]);
+      if constexpr (kWide) {
+        st_32(reinterpret_cast<uint8_t*>(dst) + 32 * j, part);
+      } else {
+        reinterpret_cast<uint4*>(dst)[2 * j] = make_uint4(part[0], part[1], part[2], part[3]);
+        reinterpret_cast<uint4*>(dst)[2 * j + 1] = make_uint4(part[4], part[5], part[6], part[7]);
+      }
+    }
   }
 }
 
-// Rows per launch: their units are counted in 31 bits, and a launch starts at a block of 128 rows.
-static int64_t rows_per_launch(int64_t units) { return std::max<int64_t>(128, kMaxUnits / 2 / units / 128 * 128); }
+// Tasks and scales are counted in 31 bits; a launch starts at a block of 128 rows.  launch(tasks, blocks, first row, its rows, its
+// first scale).
+template <int kGroup, class Launch>
+static int over_rows(int64_t rows, int64_t hidden, Launch&& launch) {
+  const int64_t blocks = (hidden / kGroup + 3) / 4;
+  const int64_t step = std::max<int64_t>(1, kMostScales / (blocks * kBlockBytes)) * 128;
+  for (int64_t r = 0; r < rows; r += step) {
+    const int64_t left = std::min(step, rows - r), row_blocks = (left + 127) / 128;
+    // of a block with few rows, only the tasks that have one of them
+    const int64_t tail = std::min<int64_t>(left - (row_blocks - 1) * 128, 32);
+    const int64_t sets = (row_blocks - 1) * Place<kGroup>::kTasks + (tail + Place<kGroup>::kRows / 4 - 1) / (Place<kGroup>::kRows / 4);
+    SGLB_CUDA(launch((uint32_t)(sets * blocks), FastDiv((uint32_t)blocks), r, (int)left, r / 128 * blocks * kBlockBytes));
+  }
+  return SGLB200_OK;
+}
+
+// Tasks a warp takes: two where that still fills the SMs.
+constexpr int kAheadMany = 2;
+static bool many(uint32_t tasks) { return tasks >= (uint32_t)sm_count() * 64 * kAheadMany; }
+static unsigned grid_of(uint32_t tasks, int ahead) { return (tasks + kThreads / 32 * ahead - 1) / (kThreads / 32 * ahead); }
 
 template <typename T, int kGroup, bool kSilu>
 static int launch_quant(const void* x, void* codes, void* scales, const float* g, int64_t rows, int64_t hidden, cudaStream_t st) {
-  const int64_t units = hidden / kUnit, step = rows_per_launch(units);
-  const int group_blocks = (int)((hidden / kGroup + 3) / 4);
-  for (int64_t r = 0; r < rows; r += step) {
-    const int64_t total = std::min(step, rows - r) * units;
-    SGLB_CUDA(launch_pdl(quant_fp4_kernel<T, kGroup, kSilu>, (unsigned)((total + kThreads - 1) / kThreads), kThreads, 0, st,
-                         static_cast<const T*>(x) + r * hidden * (kSilu ? 2 : 1), static_cast<uint2*>(codes) + r * units,
-                         static_cast<uint8_t*>(scales), g, (uint32_t)total, FastDiv((uint32_t)units), r, group_blocks));
-  }
-  return SGLB200_OK;
+  const int units = (int)(hidden / kUnit);
+  return over_rows<kGroup>(rows, hidden, [&](uint32_t tasks, FastDiv blocks, int64_t r, int count, int64_t scale) {
+    const auto go = [&](auto kern, int ahead) {
+      return launch_pdl(kern, grid_of(tasks, ahead), kThreads, 0, st, static_cast<const T*>(x) + r * hidden * (kSilu ? 2 : 1),
+                        static_cast<uint2*>(codes) + r * units, static_cast<uint8_t*>(scales) + scale, g, tasks, blocks, (uint32_t)units, count);
+    };
+    if (reinterpret_cast<uintptr_t>(x) % 32) return go(quant_fp4_kernel<T, kGroup, kSilu, false, 1>, 1);
+    return many(tasks) ? go(quant_fp4_kernel<T, kGroup, kSilu, true, kAheadMany>, kAheadMany) : go(quant_fp4_kernel<T, kGroup, kSilu, true, 1>, 1);
+  });
 }
 
 template <typename T, int kGroup>
 static int launch_dequant(const void* codes, const void* scales, const float* g, void* out, int64_t rows, int64_t hidden,
                           cudaStream_t st) {
-  const int64_t units = hidden / kUnit, step = rows_per_launch(units);
-  const int group_blocks = (int)((hidden / kGroup + 3) / 4);
-  for (int64_t r = 0; r < rows; r += step) {
-    const int64_t total = std::min(step, rows - r) * units;
-    SGLB_CUDA(launch_pdl(dequant_fp4_kernel<T, kGroup>, (unsigned)((total + kThreads - 1) / kThreads), kThreads, 0, st,
-                         static_cast<const uint2*>(codes) + r * units, static_cast<const uint8_t*>(scales), g,
-                         static_cast<T*>(out) + r * hidden, (uint32_t)total, FastDiv((uint32_t)units), r, group_blocks));
-  }
-  return SGLB200_OK;
+  const int units = (int)(hidden / kUnit);
+  return over_rows<kGroup>(rows, hidden, [&](uint32_t tasks, FastDiv blocks, int64_t r, int count, int64_t scale) {
+    const auto go = [&](auto kern, int ahead) {
+      return launch_pdl(kern, grid_of(tasks, ahead), kThreads, 0, st, static_cast<const uint2*>(codes) + r * units,
+                        static_cast<const uint8_t*>(scales) + scale, g, static_cast<T*>(out) + r * hidden, tasks, blocks, (uint32_t)units, count);
+    };
+    if (reinterpret_cast<uintptr_t>(out) % 32) return go(dequant_fp4_kernel<T, kGroup, false, 1>, 1);
+    return many(tasks) ? go(dequant_fp4_kernel<T, kGroup, true, kAheadMany>, kAheadMany) : go(dequant_fp4_kernel<T, kGroup, true, 1>, 1);
+  });
 }
 
 // What the three entry points refuse alike.

@@ -33,7 +33,7 @@ def _check(x, g, group, q, s):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,hidden", [(1, 16), (1, 7168), (3, 48), (127, 272), (129, 2112), (300, 64), (33, 18432)])
+@pytest.mark.parametrize("rows,hidden", [(1, 16), (1, 7168), (3, 48), (127, 272), (129, 2112), (300, 64), (33, 18432), (2100, 4112)])
 @pytest.mark.parametrize("g", [None, 44.8, 32.0, 0.37])
 def test_quant_16(dtype, rows, hidden, g):
     from sglang_b200 import ops
@@ -44,7 +44,7 @@ def test_quant_16(dtype, rows, hidden, g):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,hidden", [(1, 32), (1, 7168), (5, 96), (129, 2112), (300, 64)])
+@pytest.mark.parametrize("rows,hidden", [(1, 32), (1, 7168), (5, 96), (129, 2112), (300, 64), (2100, 4128)])
 def test_quant_32(dtype, rows, hidden):
     from sglang_b200 import ops
     x = _rows(rows, hidden, dtype, rows + hidden)
@@ -84,7 +84,7 @@ def test_borders_and_special_values(dtype, group):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("group,g", [(16, None), (16, 44.8), (32, None)])
-@pytest.mark.parametrize("rows,hidden", [(1, 32), (131, 2112), (257, 160)])
+@pytest.mark.parametrize("rows,hidden", [(1, 32), (131, 2112), (257, 160), (2100, 4128)])
 def test_dequant(dtype, group, g, rows, hidden):
     from sglang_b200 import ops
     rng = np.random.default_rng(hidden)
@@ -145,6 +145,26 @@ def test_batched_shapes_empty_and_streams():
     side.synchronize()
     again = ops.per_token_group_quant_fp4(big * 2)
     assert torch.equal(again[0], q) and torch.equal(ops.per_token_group_dequant_fp4(*again), back)
+
+
+def test_values_that_begin_on_16_bytes():
+    """A view that is 16-byte but not 32-byte aligned takes narrower loads and stores."""
+    from sglang_b200 import ops
+    for dtype, off in ((torch.bfloat16, 8), (torch.float32, 4)):
+        x = _rows(70, 96, dtype, 4)
+        flat = torch.empty(70 * 96 + off, dtype=dtype, device="cuda")
+        flat[off:] = x.flatten().cuda()
+        view = flat[off:].view(70, 96)
+        assert view.data_ptr() % 32 == 16
+        q, s = ops.per_token_group_quant_fp4(view)
+        _check(x, None, 16, q, s)
+        q, s = ops.per_token_group_quant_fp4(view, None, 32)
+        _check(x, None, 32, q, s)
+    y = torch.empty(70 * 96 + 8, dtype=torch.bfloat16, device="cuda")[8:].view(70, 96)
+    from sglang_b200._lib import check, lib
+    check(lib.sglb200_per_token_group_dequant_fp4(q.data_ptr(), s.data_ptr(), None, y.data_ptr(), 0, 70, 96, 32,
+                                                  torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(y, ops.per_token_group_dequant_fp4(q, s))
 
 
 def test_rows_past_the_last_are_left_as_they_were():

@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
       *abort_flag = 1;
     } else {
       ptx::tc_fence_after();
-      const float alpha = p.alpha ? __ldg(p.alpha) : 1.0f;
+      const float alpha = p.alpha ? __ldcg(p.alpha) : 1.0f;
       const int n = n_tile * 128 + warp * 32 + lane, m0 = m_tile * NT;
       const float bias = splits == 1 && p.bias != nullptr && n < p.N ? load_bias(p, n) : 0.f;
       float* part = reinterpret_cast<float*>(ring) + warp * 32 + lane;  // the operands have been consumed

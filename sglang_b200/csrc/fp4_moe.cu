@@ -7,14 +7,24 @@
 // Few tokens name many experts once or twice each, so a layer is one read of those experts' weights: 0.5625 bytes a weight, and
 // the weights come in faster (12 T/s) than they could be expanded for anything but the matrix instructions.  A weight times its group's
 // scale has six significant bits and lies within fp16, so it goes into mma.m16n8k16 exactly; the weights are the 16-row side, read
-// straight from their rows in the order in which the instruction's lanes hold them (the order of k within a sum is free), and up to
-// eight activation rows are the other.  bf16 activations become fp16 under a power of two per row that brings the row's largest
-// magnitude to 2^14: exact down to 2^-28 of it and off by at most 2^-39 of it below.  h is kept in float32 and enters the second
-// product as fp16 likewise (2^-12 of a value, an eighth of what rounding the output to bf16 costs).
+// straight from their rows in the order in which the instruction's lanes hold them (the order of k within a sum is free), and eight
+// activation rows are the other; with more rows of an expert, 16 or 32 of them share what was expanded.  bf16 activations become fp16
+// under a power of two per row: 2^6 where the row's largest magnitude lies in [2^-5, 2^9), else what brings that to 2^14.  So they are
+// exact down to 2^-18 of that magnitude and off by at most 2^-26 of it below.  h is kept in float32 and enters the second product
+// as fp16 likewise (2^-12 of a value, an eighth of what rounding the output to bf16 costs).
 //
-// A CTA's item is one expert and a few 16-row tiles; its warps split the tiles and K.  Partial sums meet in shared memory in a fixed
-// order.  The second launch writes every slot's product to a scratch, and whichever CTA is the last of a set of columns adds the
-// slots of a token in their order, so results do not depend on the order of CTAs.
+// A CTA's item is one expert and a few 16-row tiles; its 16 warps split the tiles and K.  One more warp keeps a ring of 36 KB stages
+// (codes and scales of 256 columns of all 16 tiles, one TMA load each) full across items, so that the memory streams while rows are
+// staged and sums are taken.  Partial sums meet in shared memory in a fixed order.  The second launch writes every slot's product to a
+// scratch, and whichever CTA is the last of a set of columns adds the slots of a token in their order, so results do not depend on the
+// order of CTAs.
+//
+// 16 tokens, 8 of 256 experts of 7168 x 2048 (101 named, 2.5 GB): 450 to 490 us, 0.80 to 0.85 of the measured copy rate; the first product
+// streams at 0.96 of it, the second's items are shorter: a third of its time is their ends.  What bounds both is the expansion, 1500
+// clocks a stage against 1530 that the memory takes for it.  Small layers are bound by latency: two launches without weights to speak
+// of take 13 us (of which staging the rows 2 to 3 a launch, finding the experts 0.7, the count of items and the last sums 2), one
+// token through eighths of experts (25 MB) 21.  Not kept: weights straight into registers (16 warps, three steps deep: 570 us), two
+// tiles a warp (620; the ring is then two stages deep), two CTAs of eight warps an SM (520), a warp of its own that counts items (500).
 #include <algorithm>
 #include <type_traits>
 
@@ -292,14 +302,15 @@ __device__ __noinline__ void stage_rows(const MoeParams& p, MoeCtl* ctl, int exp
   if (turn > 0) consumer_sync();  // the rows before these have been used
   if (tid < kMoeRows) ctl->amax[(turn + 1) & 1][tid] = 0;
   if (tid < n) {
-    const float alpha = p.alpha ? __ldg(p.alpha + expert) : 1.f;
-    ctl->factor[tid] = std::is_same<T, float>::value ? alpha * __ldg(p.weights + ctl->slot[first + tid]) : alpha;
+    const float alpha = p.alpha ? __ldcg(p.alpha + expert) : 1.f;
+    ctl->factor[tid] = std::is_same<T, float>::value ? alpha * __ldcg(p.weights + ctl->slot[first + tid]) : alpha;
   }
   const int share = n > 8 ? 0 : n > 4 ? 1 : n > 2 ? 2 : n > 1 ? 3 : 4;  // 2^share warps to a row
-  constexpr int kAhead = 4;  // pieces that are asked for before the first is converted
+  constexpr int kAhead = 2;  // pieces that are asked for before the first is converted (four: 2 us more a layer, for the instructions)
   for (int r = warp >> share; r < n; r += kMoeWarps >> share) {
     const T* src = act_row<T>(p, ctl->slot[first + r]);
     uint32_t most = 0;
+#pragma unroll 1
     for (int q0 = (warp & ((1 << share) - 1)) * 32 + lane; q0 < pieces; q0 += (kAhead * 32) << share) {
       Piece<T> x[kAhead];
 #pragma unroll
@@ -323,12 +334,14 @@ __device__ __noinline__ void stage_rows(const MoeParams& p, MoeCtl* ctl, int exp
   consumer_sync();
   if constexpr (!std::is_same<T, __half>::value) {
     bool again = false;
+#pragma unroll 1
     for (int r = 0; r < n; ++r) {
       const int bits = amax[r], shift = row_shift<T>(bits);
       if (shift == kUsualShift) continue;
       again = true;
       const bool fine = bits < 0x7f800000;
       const T* src = act_row<T>(p, ctl->slot[first + r]);
+#pragma unroll 1
       for (int q = tid; q * 8 < K; q += kMoeConsumers) {
         Piece<T> x;
         x.load(src + q * 8);
@@ -360,7 +373,7 @@ __device__ __noinline__ void sum_slots(const MoeParams& p, int col0, int cols) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int s = token * p.topk + min(k0 + k, p.topk - 1);
-        v[k] = __ldcg(reinterpret_cast<const float4*>(p.h + (int64_t)s * p.rows + col)), id[k] = p.ids[s];
+        v[k] = __ldcg(reinterpret_cast<const float4*>(p.h + (int64_t)s * p.rows + col)), id[k] = __ldcg(p.ids + s);
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k)  // (a slot of no expert has not been written)

@@ -202,7 +202,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     constexpr int kFirst = BN == 128 ? 64 : 128;
     const int group = warp >> 2, q = warp & 3, cols = group == 0 ? kFirst : BN - kFirst;
     const uint32_t lead_aempty = ptx::cluster_map(bar_aempty, 0);
-    const float alpha = p.alpha ? __ldg(p.alpha) : 1.0f;
+    const float alpha = p.alpha ? __ldcg(p.alpha) : 1.0f;
     const uint32_t stage = ptx::smem_u32(out) + group * (128 * 128);
     const int row = q * 32 + lane;
     bool ok = true;
@@ -226,7 +226,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           for (int j = 0; j < 32; j += 8) {
             const int n = n0 + c + j;  // (N is a multiple of 8)
             uint4 bw = make_uint4(0, 0, 0, 0);
-            if (n < p.N) bw = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.bias) + n));
+            if (n < p.N) bw = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.bias) + n));
             const uint32_t b4[4] = {bw.x, bw.y, bw.z, bw.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {

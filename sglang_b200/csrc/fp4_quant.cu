@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kThreads)
     raw[k][0].template load<kWide>(src);
     if constexpr (kSilu) raw[k][1].template load<kWide>(src + (int64_t)units * kUnit);
   }
-  const float g = global_scale ? __ldg(global_scale) : 1.0f;
+  const float g = global_scale ? __ldcg(global_scale) : 1.0f;
 #pragma unroll
   for (int k = 0; k < kAhead; ++k) {
     if (task0 + k * (kThreads / 32) >= tasks) break;
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kThreads)
     c[k] = __ldg(codes + at[k].unit);
     code[k] = at[k].live ? __ldg(scales + at[k].scale) : 0u;
   }
-  const float g = global_scale ? __ldg(global_scale) : 1.0f;
+  const float g = global_scale ? __ldcg(global_scale) : 1.0f;
 #pragma unroll
   for (int k = 0; k < kAhead; ++k) {
     if (task0 + k * (kThreads / 32) >= tasks) break;

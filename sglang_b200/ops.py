@@ -596,8 +596,10 @@ def fused_experts_fp4(
     hidden_states [T, H] bf16 or fp16; w13 uint8 [E, 2I, H / 2] (G_e's rows, then U_e's), w2 uint8 [E, H, I / 2]; their scales
     float8_e4m3fn in rows' order, [E, 2I, H / 16] and [E, H, I / 16]; topk_weights and topk_ids [T, k].  An id outside
     [0, E) contributes nothing.  The alphas are float32 [E] (None: 1).  H and I divisible by 32."""
-    if topk_ids.dtype != torch.int32:  # (an id that does not fit an int32 names no expert)
+    if topk_ids.dtype == torch.int64:  # (an id that does not fit an int32 names no expert)
         topk_ids = topk_ids.clamp(-1, 2**31 - 1).to(torch.int32)
+    elif topk_ids.dtype != torch.int32:
+        raise RuntimeError("topk_ids must be int32 or int64")
     if topk_weights.dtype != torch.float32:
         topk_weights = topk_weights.float()
     out = host.fused_experts_fp4(hidden_states, w13, w2, w13_scale, w2_scale, topk_weights, topk_ids, w13_alpha, w2_alpha,

@@ -35,14 +35,21 @@
 namespace sglb200 {
 namespace fp4 {
 
-constexpr int kMoeWarps = 16, kMoeConsumers = kMoeWarps * 32, kMoeThreads = kMoeConsumers + 32;  // one more warp fetches the weights
+constexpr int kMoeWarps = 16, kMoeConsumers = kMoeWarps * 32;  // warps that multiply
+constexpr int kScaleWarps = 3;                // that fetch scales where K is not whole steps
+// One more warp fetches codes, and scales where K is whole steps.
+template <bool kWhole>
+constexpr int kMoeThreads = kMoeConsumers + 32 + (kWhole ? 0 : kScaleWarps * 32);
 constexpr int kMoeMaxExperts = 1024, kMoeMaxSlots = 1024;
 constexpr int kStep = 256;                    // columns per step: a lane takes 64 of a row, 32 bytes of codes and four scales
 constexpr int kMoeRows = 32;                  // activation rows per pass, at most: four times the eight of an instruction
 constexpr uint32_t kTileBytes = 16 * kStep / 2;                  // of a tile and step
-constexpr uint32_t kCodeBytes = kMoeWarps * kTileBytes;    // of a stage: 32 KB, and 4 KB of scales
-constexpr uint32_t kTileScales = 16 * kStep / 16;
-constexpr uint32_t kStageBytes = kCodeBytes + kMoeWarps * kTileScales;
+constexpr uint32_t kCodeBytes = kMoeWarps * kTileBytes;    // of a stage: 32 KB, and 4 or 5 KB of scales
+// Scales of a row and step in a stage: 16 bytes, or the five words that hold them where rows begin on two bytes.
+template <bool kWhole>
+constexpr uint32_t kScalePitch = kWhole ? 16 : 20;
+template <bool kWhole>
+constexpr uint32_t kStageBytes = kCodeBytes + kMoeWarps * 16 * kScalePitch<kWhole>;
 constexpr int kMoeMaxStages = 6;
 constexpr int kUsualShift = 6;                // rows whose largest magnitude lies in [2^-5, 2^9) are staged under 2^6
 
@@ -352,14 +359,6 @@ __device__ __noinline__ void stage_rows(const MoeParams& p, MoeCtl* ctl, int exp
   }
 }
 
-// A lane's scales of 64 columns of a row, of which `left` are there; zeros for the others.
-__device__ __forceinline__ uint32_t load_scales(const uint8_t* at, int left) {
-  uint32_t v = 0;
-  if (left > 0) v = __ldg(reinterpret_cast<const uint16_t*>(at));
-  if (left > 32) v |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(at) + 1) << 16;
-  return v;
-}
-
 // The tokens' slots of the columns [col0, col0 + cols), added in their order, by the CTA whose item was the last of those columns.
 template <typename OutT>
 __device__ __noinline__ void sum_slots(const MoeParams& p, int col0, int cols) {
@@ -417,12 +416,12 @@ __device__ __forceinline__ void multiply(float (&acc)[NT][4], const uint4 (&code
 
 // kWhole: K is a multiple of a step.  kUp: T is the activations' type and a tile is 8 gate and the 8 matching up rows; else T is float (h) and OutT the output's type.
 template <typename T, typename OutT, bool kUp, bool kWhole, int NT>
-__global__ void __launch_bounds__(kMoeThreads, 1)
+__global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
     fp4_experts_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s,
                        const __grid_constant__ MoeParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint4* xs = reinterpret_cast<uint4*>(ring + p.stages * kStageBytes);
+  uint4* xs = reinterpret_cast<uint4*>(ring + p.stages * kStageBytes<kWhole>);
   float* red = reinterpret_cast<float*>(xs + p.steps * 32 * p.pass_rows);  // [warp][4 NT][32]
   MoeCtl* ctl = reinterpret_cast<MoeCtl*>(red + kMoeWarps * NT * 128);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -432,7 +431,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
   if (tid == kMoeConsumers) {
     ptx::tma_prefetch_desc(&map_w);
     if constexpr (kWhole) ptx::tma_prefetch_desc(&map_s);
-    for (int s = 0; s < S; ++s) ptx::mbar_init(bar_full + s * 8, 1), ptx::mbar_init(bar_empty + s * 8, kMoeWarps);
+    for (int s = 0; s < S; ++s) ptx::mbar_init(bar_full + s * 8, kWhole ? 1 : 1 + kScaleWarps * 32), ptx::mbar_init(bar_empty + s * 8, kMoeWarps);
     ctl->abort_flag = 0;
     ptx::mbar_fence_init();
   }
@@ -443,7 +442,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     ptx::grid_dependency_wait();
     ptx::launch_dependents();
     if (blockIdx.x == 0)
-      for (int i = tid; i < p.done_count; i += kMoeThreads) p.done[i] = 0;
+      for (int i = tid; i < p.done_count; i += kMoeThreads<kWhole>) p.done[i] = 0;
   }
   route(p, ctl);
 
@@ -466,9 +465,9 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
         for (int i = 0, step0 = 0; i < passes * turns; ++i) {
           ok = p.wait_probes != ptx::kProbesNone && ptx::mbar_wait_quiet(bar_empty + s * 8, ph);
           if (!ok) break;
-          const uint32_t bar = bar_full + s * 8, at = ptx::smem_u32(ring) + s * kStageBytes;
+          const uint32_t bar = bar_full + s * 8, at = ptx::smem_u32(ring) + s * kStageBytes<kWhole>;
           if constexpr (kWhole) {  // one load for the codes of all parts of K, one for their scales (a box is counted whole)
-            ptx::mbar_arrive_expect_tx(bar, kStageBytes);
+            ptx::mbar_arrive_expect_tx(bar, kStageBytes<kWhole>);
             if constexpr (kUp) {
               tma_load_5d(at, &map_w, bar, 0, tile0 * 8, 0, step0, expert);
               tma_load_5d(at + kCodeBytes, &map_s, bar, 0, tile0 * 8, 0, step0, expert);
@@ -495,6 +494,76 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     }
     __syncwarp();
     if constexpr (!kUp) ptx::grid_dependency_wait();
+  } else if (!kWhole && warp > kMoeWarps) {
+    // ------------------------------ scales, where their rows do not begin on 16 bytes ------------------------------
+    // Words of four bytes by asynchronous copies, which arrive at the stage's barrier by themselves, so that they are as far ahead as the
+    // codes are.  A row that begins on two bytes takes five words to a step.  Where such a warp has few issue slots beside those that multiply,
+    // all that does not change from stage to stage is kept.  16 tokens, 8 of 256 experts of 7200 x 2080 take 660 us (whole steps, 7168 x
+    // 2048: 475), 32 tokens, 8 of 128 of 2080 x 800 131 (91); when the warps that multiply loaded them, two steps ahead, 683 and 141; by
+    // these through registers 840 and more.
+    constexpr int kWords = kScalePitch<kWhole> / 4, kAll = kMoeWarps * 16 * kWords;
+    constexpr int kTasks = (kAll + kScaleWarps * 32 - 1) / (kScaleWarps * 32);
+    const int h = (warp - kMoeWarps - 1) * 32 + lane, scale_row = (int)(p.K / 16), half_rows = warps_m * 8;
+    const int limit = kUp ? (int)(p.rows / 2) : (int)p.rows;  // rows of a half of w13, or of w2
+    uint32_t from[kTasks];  // where a task's word lies, from the set's first row and the stage's first column
+    int left_of[kTasks];    // bytes of the row from there on, for the first stage
+    const auto row_of = [&](int j, int& k, int& u) {  // a task's row of the set, its part of K, its half
+      const int r = (h + j * kScaleWarps * 32) / kWords, in = (k = r / (warps_m * 16), r - k * warps_m * 16);
+      u = kUp ? in / half_rows : 0;
+      return in - u * half_rows;
+    };
+#pragma unroll
+    for (int j = 0; j < kTasks; ++j) {
+      int k, u;
+      const int row = row_of(j, k, u), word = (h + j * kScaleWarps * 32) % kWords, back = (row & 1) * (scale_row & 2);
+      from[j] = (uint32_t)((row + u * limit) * scale_row + k * (kStep / 16) - back + word * 4);
+      left_of[j] = scale_row - k * (kStep / 16) + back - word * 4;
+    }
+    bool ok = p.wait_probes != ptx::kProbesNone;
+    int s = 0;
+    uint32_t ph = 1;
+    for (int item = item0; item < item1 && ok; ++item) {
+      const int live = item / p.sets, tile_row = (item - live * p.sets) * warps_m * (kUp ? 8 : 16);
+      const int passes = (ctl->begin[live + 1] - ctl->begin[live] + p.pass_rows - 1) / p.pass_rows;
+      const uint8_t* base = p.ws + ((int64_t)ctl->live[live] * p.rows + tile_row) * scale_row;
+      uint32_t rows_there = 0;  // of the tasks' rows, those that the expert has
+#pragma unroll
+      for (int j = 0; j < kTasks; ++j) {
+        int k, u;
+        const int row = row_of(j, k, u);
+        rows_there |= (h + j * kScaleWarps * 32 < kAll && tile_row + row < limit ? 1u : 0u) << j;
+      }
+      const bool all_there = tile_row + (kUp ? half_rows : warps_m * 16) <= limit;
+      for (int i = 0, step0 = 0; i < passes * turns; ++i) {
+        ok = ok && (ptx::mbar_test(bar_empty + s * 8, ph) || ptx::mbar_wait_quiet(bar_empty + s * 8, ph));
+        if (!ok) break;
+        const uint32_t at = ptx::smem_u32(ring) + s * kStageBytes<kWhole> + kCodeBytes + h * 4;
+        const uint8_t* src = base + step0 * (kStep / 16);
+        const int used = step0 * (kStep / 16);
+        if (all_there && used + warps_k * (kStep / 16) + 4 <= scale_row) {  // every word is whole
+#pragma unroll
+          for (int j = 0; j < kTasks; ++j)
+            if (j < kAll / (kScaleWarps * 32) || h + j * kScaleWarps * 32 < kAll)
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at + j * kScaleWarps * 128), "l"(src + from[j]) : "memory");
+        } else {
+#pragma unroll
+          for (int j = 0; j < kTasks; ++j)
+            if (h + j * kScaleWarps * 32 < kAll) {
+              const int bytes = rows_there >> j & 1 ? min(max(left_of[j] - used, 0), 4) : 0;  // (the rest of a word is filled with zeros)
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(at + j * kScaleWarps * 128),
+                           "l"(bytes > 0 ? src + from[j] : p.ws), "r"(bytes)
+                           : "memory");
+            }
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar_full + s * 8) : "memory");
+        step0 += warps_k;
+        if (step0 >= p.steps) step0 = 0;
+        if (++s == S) s = 0, ph ^= 1;
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (!ok) ctl->abort_flag = 1;
+    if constexpr (!kUp) ptx::grid_dependency_wait();
   } else {
     // ------------------------------ products ------------------------------
     const int wk = warp % warps_k, wm = warp / warps_k;
@@ -505,10 +574,13 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     const uint32_t code_lo = part + wm * tile_step + ((uint32_t)(2 * t) ^ g) * 16;
     const uint32_t code_hi = part + wm * tile_step + ((uint32_t)(2 * t + 1) ^ g) * 16;
     const uint32_t row_a = (kUp ? wm * 8 : wm * 16) + g, row_b = row_a + (kUp ? warps_m * 8 : 8);
-    const uint32_t scale_a = ptx::smem_u32(ring) + kCodeBytes + wk * warps_m * kTileScales + row_a * 16 + t * 4;
-    const uint32_t scale_b = scale_a + (row_b - row_a) * 16;
-    const int64_t scale_row = p.K / 16;
-    const int skip = warps_k * kStep;  // columns between two steps of this warp
+    const uint32_t scale_a = ptx::smem_u32(ring) + kCodeBytes + (wk * warps_m * 16 + row_a) * kScalePitch<kWhole> + t * 4;
+    const uint32_t scale_b = scale_a + (row_b - row_a) * kScalePitch<kWhole>;
+    const uint32_t halves = (g & 1) && p.K % 64 != 0 ? 0x5432 : 0x3210;  // of two words, where odd rows' scales begin in the middle of one
+    const auto read_scales = [&](uint32_t at) {
+      if constexpr (kWhole) return lds_32(at);
+      return __byte_perm(lds_32(at), lds_32(at + 4), halves);
+    };
 
     if constexpr (!kUp) ptx::grid_dependency_wait();
     const auto sum_set = [&](int set) {
@@ -522,20 +594,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
       const int live = item / p.sets, set = item - live * p.sets;
       const int expert = ctl->live[live], first = ctl->begin[live], rows_n = ctl->begin[live + 1] - first;
       const int my_tile = set * warps_m + wm;
-      // scales of this lane's rows (of the expert's first ones where there is no tile)
-      const int64_t row0 = (int64_t)expert * p.rows + (my_tile < tiles ? kUp ? (int64_t)my_tile * 8 + g : (int64_t)my_tile * 16 + g : 0);
-      const uint8_t* sp[2] = {p.ws + row0 * scale_row, p.ws + (row0 + (kUp ? p.rows / 2 : 8)) * scale_row};
       for (int r0 = 0; r0 < rows_n; r0 += p.pass_rows) {
         const int n = min(p.pass_rows, rows_n - r0);
-        // where K is not whole steps, scales are asked for in global memory, two steps ahead
-        uint32_t sc[2][2];
-        const uint8_t *sa = sp[0] + (wk * kStep + t * 64) / 16, *sb = sp[1] + (wk * kStep + t * 64) / 16;
-        int left = (int)p.K - (wk * kStep + t * 64);  // columns of the row from those whose scales are asked for next
-        const auto ask = [&](uint32_t (&to)[2]) {
-          to[0] = load_scales(sa, left), to[1] = load_scales(sb, left);
-          sa += skip / 16, sb += skip / 16, left -= skip;
-        };
-        if constexpr (!kWhole) ask(sc[0]), ask(sc[1]);
         if (staged_live != live || staged_r0 != r0) {
           stage_rows<T>(p, ctl, expert, first + r0, n, stagings, xs);
           ++stagings, staged_live = live, staged_r0 = r0;
@@ -546,22 +606,21 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
         // (columns without a row are not looked at: they read what lies there, or row 0 where less than eight rows fit)
         const uint4* b = xs + (wk * 8 * p.pass_rows + (g < p.pass_rows ? g : 0)) * 4 + t;
         const int stride = p.pass_rows * 4;
-        const auto step = [&](uint32_t (&scale)[2], bool mine) {
+        const auto step = [&](bool mine) {
           if (ok && !ptx::mbar_test(bar_full + s * 8, ph)) ok = ptx::mbar_wait_quiet(bar_full + s * 8, ph);
-          const uint32_t lo = code_lo + s * kStageBytes, hi = code_hi + s * kStageBytes;
+          const uint32_t lo = code_lo + s * kStageBytes<kWhole>, hi = code_hi + s * kStageBytes<kWhole>;
           const uint4 code[2][2] = {{ptx::lds_128(lo), ptx::lds_128(hi)}, {ptx::lds_128(lo + row_step), ptx::lds_128(hi + row_step)}};
-          if constexpr (kWhole) scale[0] = lds_32(scale_a + s * kStageBytes), scale[1] = lds_32(scale_b + s * kStageBytes);
+          const uint32_t scale[2] = {read_scales(scale_a + s * kStageBytes<kWhole>), read_scales(scale_b + s * kStageBytes<kWhole>)};
           __syncwarp();
           ptx::mbar_arrive_if(bar_empty + s * 8, lane == 0);
           if (++s == S) s = 0, ph ^= 1;
           if (mine) multiply<NT>(acc, code, scale, b, stride);
           b += warps_k * 8 * stride;
-          if constexpr (!kWhole) ask(scale);
         };
         const int mine = (p.steps - wk + warps_k - 1) / warps_k;  // (the last turn may have no step for this warp)
         for (int i = 0; i < turns; i += 2) {
-          step(sc[0], i < mine);
-          if (i + 1 < turns) step(sc[1], i + 1 < mine);
+          step(i < mine);
+          if (i + 1 < turns) step(i + 1 < mine);
         }
         // Lane (g, t) has rows g (acc 0, 1) and g + 8 (2, 3) of columns 2 t, 2 t + 1.  A warp of those that split K adds up two
         // values of each of their lanes.
@@ -632,8 +691,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
   }
 }
 
-constexpr int64_t moe_smem(int steps, int pass_rows, int stages) {
-  return 1024 + (int64_t)stages * kStageBytes + (int64_t)steps * 512 * pass_rows + kMoeWarps * 512 * ((pass_rows + 7) / 8) + (int64_t)sizeof(MoeCtl);
+constexpr int64_t moe_smem(int steps, int pass_rows, int stages) {  // (the larger stages: where K is whole steps a little is left over)
+  return 1024 + (int64_t)stages * kStageBytes<false> + (int64_t)steps * 512 * pass_rows + kMoeWarps * 512 * ((pass_rows + 7) / 8) + (int64_t)sizeof(MoeCtl);
 }
 constexpr int64_t kMoeMostSmem = 227 * 1024;
 
@@ -658,6 +717,7 @@ static int plan_product(MoeParams& p, int64_t K, int64_t rows) {
   const double rows_each = p.slots / live;
   p.pass_rows = rows_each > 12 ? 32 : rows_each > 6 ? 16 : 8;
   while (p.pass_rows > 1 && (moe_smem(p.steps, p.pass_rows, p.pass_rows > 8 ? 2 : 4) > kMoeMostSmem || p.pass_rows >= 2 * p.slots)) p.pass_rows /= 2;
+  SGLB_REQUIRE(rows * (K / 16) < (1ll << 31), "fused_experts_fp4: %lld x %lld weights are too many for an expert", (long long)rows, (long long)K);
   p.stages = kMoeMaxStages;
   while (p.stages > 2 && moe_smem(p.steps, p.pass_rows, p.stages) > kMoeMostSmem) --p.stages;
   SGLB_REQUIRE(moe_smem(p.steps, p.pass_rows, p.stages) <= kMoeMostSmem, "fused_experts_fp4: %lld columns are too many", (long long)K);
@@ -676,7 +736,7 @@ static int launch_experts(const CUtensorMap& map_w, const CUtensorMap& map_s, co
   }
   const int64_t most = (int64_t)std::min(p.slots, p.experts) * p.sets;
   const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, sm_count()));
-  SGLB_CUDA(launch_pdl(kern, grid, kMoeThreads, (size_t)moe_smem(p.steps, p.pass_rows, p.stages), st, map_w, map_s, p));
+  SGLB_CUDA(launch_pdl(kern, grid, kMoeThreads<kWhole>, (size_t)moe_smem(p.steps, p.pass_rows, p.stages), st, map_w, map_s, p));
   return SGLB200_OK;
 }
 

@@ -137,3 +137,35 @@ def test_experts_refuse():
     assert call(ws=None) == -4 and "workspace" in _err()
     assert call(ws_bytes=16) == -4 and call(ws=A + 8) == -4
     assert call(T=0) == 0
+
+
+def _code(name):
+    """A source file without its comments."""
+    import os
+    import re
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sglang_b200", "csrc", name)
+    return re.sub(r"//[^\n]*", "", re.sub(r"/\*.*?\*/", "", open(path).read(), flags=re.S))
+
+
+def test_tensor_memory_is_taken_after_the_kernel_in_front_and_before_the_one_behind():
+    """A CTA that held tensor memory while it waits for the kernel in front could keep that kernel's last CTAs from getting theirs;
+    one that let the next kernel in before it has its own could be kept waiting by it."""
+    for name, kernel, alloc in (("fp4_gemm.cu", "fp4_rows_kernel(", "tmem_alloc("), ("fp4_pair.cu", "fp4_pair_kernel(", "pair_tmem_alloc(")):
+        body = _code(name)
+        body = body[body.index(kernel):]
+        wait, take, let_in = (body.index(w) for w in ("grid_dependency_wait()", alloc, "launch_dependents()"))
+        assert wait < take < let_in
+        assert min(body.index("tma_load" if "rows" in kernel else "pair_load_2d("), body.index("p.alpha")) > let_in
+
+
+def test_the_down_launch_reads_nothing_of_the_up_launch_before_its_wait():
+    body = _code("fp4_moe.cu")
+    body = body[body.index("fp4_experts_kernel(const __grid_constant__"):]
+    products = body[body.index("const int wk = warp % warps_k"):]
+    wait = products.index("if constexpr (!kUp) ptx::grid_dependency_wait();")
+    assert wait < products.index("stage_rows") and wait < products.index("sum_slots") and wait < products.index("p.h")
+    assert "p.x" not in body[:body.index("const int wk = warp % warps_k")] and "act_row" not in body[:body.index("const int wk = warp % warps_k")]
+    # every thread of the down launch waits: a launch is over only when the one in front of it is
+    assert body.count("if constexpr (!kUp) ptx::grid_dependency_wait();") == 3
+    up = body[:body.index("route(p, ctl)")]
+    assert up.index("grid_dependency_wait()") < up.index("launch_dependents()") < up.index("p.done[i] = 0")

@@ -53,7 +53,7 @@ def _check(M, N, K, group, dtype, alpha=None, bias=False, seed=0):
 
 @pytest.mark.parametrize("group", [16, 32])
 @pytest.mark.parametrize("M,N,K", [(1, 8, 32), (1, 128, 64), (3, 136, 96), (16, 2112, 7168), (17, 264, 288), (32, 1000, 4096), (33, 512, 1056),
-                                   (64, 384, 544), (65, 256, 512), (128, 768, 256), (129, 392, 2080), (300, 1000, 1056), (515, 2112, 1536)])
+                                   (64, 384, 544), (65, 256, 512), (128, 768, 256), (129, 392, 2080), (300, 1000, 1056), (515, 2112, 1536), (9000, 104, 544)])
 def test_matmul(M, N, K, group):
     _check(M, N, K, group, torch.bfloat16, alpha=2.0**-10)
 

@@ -123,14 +123,11 @@ int sglb200_per_token_group_dequant_fp4(const void* input_q, const void* input_s
  * their scales in blocked order (bytes of groups past the last must be zero; bytes of rows past the last may be anything), both of
  * `group_size` 16 or 32.  Sums in float32, one rounding to out_dtype (0 bf16, 1 fp16).  alpha: one float32 in device memory (1 / (g of
  * A * g of B)), NULL = 1.  bias: N values of the output's type, or NULL.  K % 32 == 0, N % 8 == 0, K <= 2^20; every pointer 16-byte
- * aligned.  workspace: device scratch of at least sglb200_group_fp4_workspace_bytes(M, N, K) bytes, 16-byte aligned (NULL where that
- * is 0).  A wait inside the kernel that runs out sets sglb200_gemm_status().
+ * aligned.  A wait inside the kernel that runs out sets sglb200_gemm_status().
  * Stands beside sglb200_fp8_blockwise_scaled_mm; no counterpart in the reference's block-FP8 path.
  */
-int64_t sglb200_group_fp4_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int sglb200_group_fp4_scaled_mm(const void* A, const void* B, const void* a_s, const void* b_s, const float* alpha, void* C,
-                                const void* bias, int64_t M, int64_t N, int64_t K, int group_size, int out_dtype, void* workspace,
-                                int64_t workspace_bytes, void* stream);
+                                const void* bias, int64_t M, int64_t N, int64_t K, int group_size, int out_dtype, void* stream);
 
 /*
  * The routed experts of a few tokens with 4-bit weights (groups of 16) and 16-bit activations, in two launches:

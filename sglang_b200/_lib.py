@@ -33,8 +33,7 @@ SIGNATURES = {
     "sglb200_per_token_group_quant_fp4": (_i32, [_vp, _i32, _vp, _vp, _vp, _i64, _i64, _i32, _vp]),
     "sglb200_silu_and_mul_quant_fp4": (_i32, [_vp, _i32, _vp, _vp, _vp, _i64, _i64, _i32, _vp]),
     "sglb200_per_token_group_dequant_fp4": (_i32, [_vp, _vp, _vp, _vp, _i32, _i64, _i64, _i32, _vp]),
-    "sglb200_group_fp4_workspace_bytes": (_i64, [_i64, _i64, _i64]),
-    "sglb200_group_fp4_scaled_mm": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _i64, _vp]),
+    "sglb200_group_fp4_scaled_mm": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp]),
     "sglb200_fused_experts_fp4_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
     "sglb200_fused_experts_fp4": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i64, _i64, _f32, _vp, _i64, _vp]),
     "sglb200_moe_align_workspace_bytes": (_i64, [_i64, _i32]),

@@ -299,11 +299,8 @@ using namespace sglb200;
 
 extern "C" {
 
-int64_t sglb200_group_fp4_workspace_bytes(int64_t M, int64_t N, int64_t K) { return 0; }
-
 int sglb200_group_fp4_scaled_mm(const void* A, const void* B, const void* a_s, const void* b_s, const float* alpha, void* C,
-                                const void* bias, int64_t M, int64_t N, int64_t K, int group_size, int out_dtype, void* workspace,
-                                int64_t workspace_bytes, void* stream) {
+                                const void* bias, int64_t M, int64_t N, int64_t K, int group_size, int out_dtype, void* stream) {
   if (group_size != 16 && group_size != 32)
     return fail(SGLB200_E_UNSUPPORTED, "group_fp4_scaled_mm: group_size %d is neither 16 nor 32", group_size);
   if (out_dtype != 0 && out_dtype != 1)

@@ -29,7 +29,6 @@ namespace {
   X(sglb200_per_token_group_quant_fp4)   \
   X(sglb200_silu_and_mul_quant_fp4)      \
   X(sglb200_per_token_group_dequant_fp4) \
-  X(sglb200_group_fp4_workspace_bytes)   \
   X(sglb200_group_fp4_scaled_mm)         \
   X(sglb200_fused_experts_fp4_workspace_bytes) \
   X(sglb200_fused_experts_fp4)           \
@@ -352,14 +351,11 @@ PyObject* matmul_fp4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int64_t K = a->size(-1) * 2, N = b->size(0), M = a->numel() / a->size(-1);
   if (dt < 0 || dt > 1 || !bias_ok(args[6], N, out_t, &bias) || (bias && bias->device() != a->device())) Py_RETURN_NONE;
   return guarded([&]() -> PyObject* {
-    const int64_t scratch = abi.sglb200_group_fp4_workspace_bytes(M, N, K);
     c10::DimVector shape(a->sizes().begin(), a->sizes().end());
     shape.back() = N;
-    Tensor out = make(shape, out_t, a->device()), mem;
-    if (scratch) mem = workspace(scratch, a->device());
+    Tensor out = make(shape, out_t, a->device());
     const int rc = abi.sglb200_group_fp4_scaled_mm(a->data_ptr(), b->data_ptr(), as->data_ptr(), bs->data_ptr(), alpha, out.data_ptr(),
-                                                   bias ? bias->data_ptr() : nullptr, M, N, K, (int)group, dt,
-                                                   scratch ? mem.data_ptr() : nullptr, scratch, stream_of(*a));
+                                                   bias ? bias->data_ptr() : nullptr, M, N, K, (int)group, dt, stream_of(*a));
     if (rc) return raise_last(rc);
     return THPVariable_Wrap(std::move(out));
   });

@@ -546,13 +546,11 @@ def w4a4_group_fp4_matmul(
         bias = bias.to(output_dtype).contiguous()
         if not bias.is_cuda or bias.device != A.device or bias.numel() != N:
             raise RuntimeError(f"bias must be {N} values on A's device")
-    ws_bytes = lib.sglb200_group_fp4_workspace_bytes(M, N, K)
     with torch.cuda.device(A.device):
-        ws = torch.empty(ws_bytes, device=A.device, dtype=torch.uint8) if ws_bytes else None
         check(lib.sglb200_group_fp4_scaled_mm(
             A.data_ptr(), B.data_ptr(), As.data_ptr(), Bs.data_ptr(), a, C.data_ptr(),
             bias.data_ptr() if bias is not None else None, M, N, K, group, 0 if output_dtype == torch.bfloat16 else 1,
-            ws.data_ptr() if ws is not None else None, ws_bytes, _stream(A)))
+            _stream(A)))
     return C
 
 

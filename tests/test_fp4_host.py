@@ -98,7 +98,7 @@ def test_product_refuses():
     A = 4096
 
     def call(M=4, N=16, K=64, group=16, dt=0, a=A, b=A, sa=A, sb=A, alpha=None, c=A, bias=None):
-        return lib.sglb200_group_fp4_scaled_mm(a, b, sa, sb, alpha, c, bias, M, N, K, group, dt, None, 0, None)
+        return lib.sglb200_group_fp4_scaled_mm(a, b, sa, sb, alpha, c, bias, M, N, K, group, dt, None)
 
     assert call(group=64) == -2 and "group_size" in _err()
     assert call(dt=2) == -2 and "output dtype" in _err()

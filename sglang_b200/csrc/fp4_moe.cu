@@ -13,7 +13,9 @@
 // exact down to 2^-18 of that magnitude and off by at most 2^-26 of it below.  h is kept in float32 and enters the second product
 // as fp16 likewise (2^-12 of a value, an eighth of what rounding the output to bf16 costs).
 //
-// A CTA's item is one expert and a few 16-row tiles; its 16 warps split the tiles and K.  One more warp keeps a ring of 36 KB stages
+// A CTA's item is a pass (an expert and at most 32 of its slots) and a few 16-row tiles; its 16 warps split the tiles and K.  Passes of
+// one expert go to CTAs of their own, which read its weights from the L2 (64 tokens, 4 of 8 experts of 4096 x 1024: 106 us, against 148
+// where a CTA took all passes of its tiles in turn).  One more warp keeps a ring of 36 KB stages
 // (codes and scales of 256 columns of all 16 tiles, one TMA load each) full across items, so that the memory streams while rows are
 // staged and sums are taken.  Partial sums meet in shared memory in a fixed order.  The second launch writes every slot's product to a
 // scratch, and whichever CTA is the last of a set of columns adds the slots of a token in their order, so results do not depend on the
@@ -69,7 +71,7 @@ struct MoeParams {
   int slots, topk, experts, tokens;
   int steps;                // of K
   int warps_k;              // warps that split K; the others split tiles
-  int sets;                 // items per expert
+  int sets;                 // items per pass
   int pass_rows;            // activation rows per pass
   int stages;
   float factor;
@@ -79,13 +81,13 @@ struct MoeParams {
 struct MoeCtl {
   uint64_t full[kMoeMaxStages], empty[kMoeMaxStages];
   uint16_t count[kMoeMaxExperts];   // slots of an expert, then where they begin
-  uint16_t live[kMoeMaxExperts];    // experts that are named
-  uint16_t begin[kMoeMaxExperts + 1];
+  uint16_t live[kMoeMaxSlots];      // passes: their expert, and where their slots begin (at most pass_rows of them each)
+  uint16_t begin[kMoeMaxSlots + 1];
   uint16_t slot[kMoeMaxSlots];      // slots in experts' order
   int warp_sum[8];
   int amax[2][kMoeRows];            // largest magnitudes of the staged rows, as float bits; used in turn
   float factor[kMoeRows];           // of the staged rows: alpha (times the routing weight)
-  int num_live, complete[2], abort_flag;
+  int num_live, complete[2], abort_flag;  // num_live: passes
 };
 
 __device__ __forceinline__ int ld_fresh(const int32_t* at) {  // (past the first-level cache)
@@ -94,8 +96,9 @@ __device__ __forceinline__ int ld_fresh(const int32_t* at) {  // (past the first
   return v;
 }
 
-// Which experts are named and by which slots; ids outside the experts are skipped.  (The order of an expert's slots can depend on the
-// order of atomics; it decides only which column of an instruction a slot takes, and columns do not mix.)  All threads.
+// Which experts are named and by which slots, in passes of at most p.pass_rows slots; ids outside the experts are skipped.  All threads.
+// (The order of the slots of an expert with one pass can depend on the order of atomics; it decides only which column of an instruction
+// a slot takes, and columns do not mix.)
 __device__ __forceinline__ void route(const MoeParams& p, MoeCtl* ctl) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (p.slots <= 32) {  // a slot a lane: its expert's slots are those lanes whose id is the same
@@ -104,23 +107,26 @@ __device__ __forceinline__ void route(const MoeParams& p, MoeCtl* ctl) {
       const bool in = (uint32_t)id < (uint32_t)p.experts;
       const uint32_t same = __match_any_sync(0xffffffffu, in ? id : -1 - lane), before = (1u << lane) - 1;
       const bool first = in && (same & before) == 0;
-      const uint32_t firsts = __ballot_sync(0xffffffffu, first);
-      int incl = first ? __popc(same) : 0;
+      const int count = __popc(same), alone = first ? ((count + p.pass_rows - 1) / p.pass_rows << 16) + count : 0;  // (passes, slots)
+      int incl = alone;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int up = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += up;
       }
-      const int begin = __shfl_sync(0xffffffffu, incl - (first ? __popc(same) : 0), in ? __ffs(same) - 1 : lane);
-      if (first) {
-        const int j = __popc(firsts & before);
-        ctl->live[j] = (uint16_t)id;
-        ctl->begin[j] = (uint16_t)begin;
+      const int begin = __shfl_sync(0xffffffffu, incl - alone, in ? __ffs(same) - 1 : lane), rank = __popc(same & before);
+      if (in) {
+        const int at = (begin & 0xffff) + rank;
+        ctl->slot[at] = (uint16_t)lane;
+        if (rank % p.pass_rows == 0) {
+          const int j = (begin >> 16) + rank / p.pass_rows;
+          ctl->live[j] = (uint16_t)id;
+          ctl->begin[j] = (uint16_t)at;
+        }
       }
-      if (in) ctl->slot[begin + __popc(same & before)] = (uint16_t)lane;
       if (lane == 31) {
-        ctl->num_live = __popc(firsts);
-        ctl->begin[__popc(firsts)] = (uint16_t)incl;
+        ctl->num_live = incl >> 16;
+        ctl->begin[incl >> 16] = (uint16_t)(incl & 0xffff);
       }
     }
     __syncthreads();
@@ -147,13 +153,13 @@ __device__ __forceinline__ void route(const MoeParams& p, MoeCtl* ctl) {
     }
   }
   __syncthreads();
-  // exclusive scan over the experts, four a thread: (named, slots) packed
+  // exclusive scan over the experts, four a thread: (passes, slots) packed
   int mine = 0, c[kExperts], incl = 0;
   if (tid < kRouters) {
 #pragma unroll
     for (int k = 0; k < kExperts; ++k) {
       c[k] = ctl->count[tid * kExperts + k];
-      mine += c[k] ? (1 << 16) + c[k] : 0;
+      mine += ((c[k] + p.pass_rows - 1) / p.pass_rows << 16) + c[k];
     }
     incl = mine;
 #pragma unroll
@@ -169,12 +175,12 @@ __device__ __forceinline__ void route(const MoeParams& p, MoeCtl* ctl) {
     for (int w = 0; w < warp; ++w) before += ctl->warp_sum[w];
 #pragma unroll
     for (int k = 0; k < kExperts; ++k) {
-      if (c[k]) {
+      ctl->count[tid * kExperts + k] = (uint16_t)(before & 0xffff);
+      for (int r = 0; r < c[k]; r += p.pass_rows) {
         ctl->live[before >> 16] = (uint16_t)(tid * kExperts + k);
         ctl->begin[before >> 16] = (uint16_t)(before & 0xffff);
+        before += (1 << 16) + min(c[k] - r, p.pass_rows);
       }
-      ctl->count[tid * kExperts + k] = (uint16_t)(before & 0xffff);
-      before += c[k] ? (1 << 16) + c[k] : 0;
     }
     if (tid == kRouters - 1) {
       ctl->num_live = before >> 16;
@@ -182,10 +188,32 @@ __device__ __forceinline__ void route(const MoeParams& p, MoeCtl* ctl) {
     }
   }
   __syncthreads();
+  bool split = false;  // a slot of this thread is of an expert of several passes
+  int first[kIds], end[kIds];
+  if (tid < kRouters) {
+#pragma unroll
+    for (int j = 0; j < kIds; ++j) {
+      if (id[j] < 0) continue;
+      first[j] = ctl->count[id[j]], end[j] = id[j] + 1 < kMoeMaxExperts ? ctl->count[id[j] + 1] : ctl->begin[ctl->num_live];
+      ctl->slot[first[j] + place[j]] = (uint16_t)(tid + j * kRouters);
+      split |= end[j] - first[j] > p.pass_rows;
+    }
+  }
+  if (!__syncthreads_or(split)) return;
+  // CTAs have to agree on the slots of such an expert's passes: those are put into ascending order.
+  if (tid < kRouters) {
+#pragma unroll
+    for (int j = 0; j < kIds; ++j) {
+      if (id[j] < 0 || end[j] - first[j] <= p.pass_rows) continue;
+      place[j] = 0;
+      for (int i = first[j]; i < end[j]; ++i) place[j] += ctl->slot[i] < tid + j * kRouters;
+    }
+  }
+  __syncthreads();
   if (tid < kRouters) {
 #pragma unroll
     for (int j = 0; j < kIds; ++j)
-      if (id[j] >= 0) ctl->slot[ctl->count[id[j]] + place[j]] = (uint16_t)(tid + j * kRouters);
+      if (id[j] >= 0) ctl->slot[first[j] + place[j]] = (uint16_t)(tid + j * kRouters);
   }
   __syncthreads();
 }
@@ -449,7 +477,7 @@ __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
   const int warps_k = p.warps_k, warps_m = kMoeWarps / warps_k;
   const int tiles = (int)(p.rows / 16);  // of an expert (16 rows of w each)
   const int items = ctl->num_live * p.sets, turns = (p.steps + warps_k - 1) / warps_k;
-  // A CTA takes neighbouring items, which are mostly of one expert.
+  // A CTA takes neighbouring items, which are mostly of one pass.
   const int each = (int)((uint32_t)items / gridDim.x), more = items - each * (int)gridDim.x;
   const int item0 = (int)blockIdx.x * each + min((int)blockIdx.x, more), item1 = item0 + each + ((int)blockIdx.x < more ? 1 : 0);
 
@@ -461,8 +489,7 @@ __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
       uint32_t ph = 1, part_bytes = warps_m * kTileBytes;  // (the first round of stages is free)
       for (int item = item0; item < item1 && ok; ++item) {
         const int live = item / p.sets, tile0 = (item - live * p.sets) * warps_m, expert = ctl->live[live];
-        const int passes = (ctl->begin[live + 1] - ctl->begin[live] + p.pass_rows - 1) / p.pass_rows;
-        for (int i = 0, step0 = 0; i < passes * turns; ++i) {
+        for (int i = 0, step0 = 0; i < turns; ++i) {
           ok = p.wait_probes != ptx::kProbesNone && ptx::mbar_wait_quiet(bar_empty + s * 8, ph);
           if (!ok) break;
           const uint32_t bar = bar_full + s * 8, at = ptx::smem_u32(ring) + s * kStageBytes<kWhole>;
@@ -486,7 +513,6 @@ __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
             }
           }
           step0 += warps_k;
-          if (step0 >= p.steps) step0 = 0;
           if (++s == S) s = 0, ph ^= 1;
         }
       }
@@ -524,7 +550,6 @@ __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
     uint32_t ph = 1;
     for (int item = item0; item < item1 && ok; ++item) {
       const int live = item / p.sets, tile_row = (item - live * p.sets) * warps_m * (kUp ? 8 : 16);
-      const int passes = (ctl->begin[live + 1] - ctl->begin[live] + p.pass_rows - 1) / p.pass_rows;
       const uint8_t* base = p.ws + ((int64_t)ctl->live[live] * p.rows + tile_row) * scale_row;
       uint32_t rows_there = 0;  // of the tasks' rows, those that the expert has
 #pragma unroll
@@ -534,7 +559,7 @@ __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
         rows_there |= (h + j * kScaleWarps * 32 < kAll && tile_row + row < limit ? 1u : 0u) << j;
       }
       const bool all_there = tile_row + (kUp ? half_rows : warps_m * 16) <= limit;
-      for (int i = 0, step0 = 0; i < passes * turns; ++i) {
+      for (int i = 0, step0 = 0; i < turns; ++i) {
         ok = ok && (ptx::mbar_test(bar_empty + s * 8, ph) || ptx::mbar_wait_quiet(bar_empty + s * 8, ph));
         if (!ok) break;
         const uint32_t at = ptx::smem_u32(ring) + s * kStageBytes<kWhole> + kCodeBytes + h * 4;
@@ -557,7 +582,6 @@ __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
         }
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar_full + s * 8) : "memory");
         step0 += warps_k;
-        if (step0 >= p.steps) step0 = 0;
         if (++s == S) s = 0, ph ^= 1;
       }
     }
@@ -588,76 +612,73 @@ __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
       sum_slots<OutT>(p, col0, min(warps_m * 16, (int)p.rows - col0));
     };
     bool ok = p.wait_probes != ptx::kProbesNone;
-    int staged_live = -1, staged_r0 = -1, stagings = 0, s = 0;
+    int staged = -1, stagings = 0, s = 0;
     uint32_t ph = 0;
     for (int item = item0; item < item1; ++item) {
       const int live = item / p.sets, set = item - live * p.sets;
-      const int expert = ctl->live[live], first = ctl->begin[live], rows_n = ctl->begin[live + 1] - first;
+      const int expert = ctl->live[live], first = ctl->begin[live], n = ctl->begin[live + 1] - first;
       const int my_tile = set * warps_m + wm;
-      for (int r0 = 0; r0 < rows_n; r0 += p.pass_rows) {
-        const int n = min(p.pass_rows, rows_n - r0);
-        if (staged_live != live || staged_r0 != r0) {
-          stage_rows<T>(p, ctl, expert, first + r0, n, stagings, xs);
-          ++stagings, staged_live = live, staged_r0 = r0;
-        }
-        float acc[NT][4];
+      if (staged != live) {
+        stage_rows<T>(p, ctl, expert, first, n, stagings, xs);
+        ++stagings, staged = live;
+      }
+      float acc[NT][4];
 #pragma unroll
-        for (int q = 0; q < NT; ++q) acc[q][0] = acc[q][1] = acc[q][2] = acc[q][3] = 0.f;
-        // (columns without a row are not looked at: they read what lies there, or row 0 where less than eight rows fit)
-        const uint4* b = xs + (wk * 8 * p.pass_rows + (g < p.pass_rows ? g : 0)) * 4 + t;
-        const int stride = p.pass_rows * 4;
-        const auto step = [&](bool mine) {
-          if (ok && !ptx::mbar_test(bar_full + s * 8, ph)) ok = ptx::mbar_wait_quiet(bar_full + s * 8, ph);
-          const uint32_t lo = code_lo + s * kStageBytes<kWhole>, hi = code_hi + s * kStageBytes<kWhole>;
-          const uint4 code[2][2] = {{ptx::lds_128(lo), ptx::lds_128(hi)}, {ptx::lds_128(lo + row_step), ptx::lds_128(hi + row_step)}};
-          const uint32_t scale[2] = {read_scales(scale_a + s * kStageBytes<kWhole>), read_scales(scale_b + s * kStageBytes<kWhole>)};
-          __syncwarp();
-          ptx::mbar_arrive_if(bar_empty + s * 8, lane == 0);
-          if (++s == S) s = 0, ph ^= 1;
-          if (mine) multiply<NT>(acc, code, scale, b, stride);
-          b += warps_k * 8 * stride;
-        };
-        const int mine = (p.steps - wk + warps_k - 1) / warps_k;  // (the last turn may have no step for this warp)
-        for (int i = 0; i < turns; i += 2) {
-          step(i < mine);
-          if (i + 1 < turns) step(i + 1 < mine);
-        }
-        // Lane (g, t) has rows g (acc 0, 1) and g + 8 (2, 3) of columns 2 t, 2 t + 1.  A warp of those that split K adds up two
-        // values of each of their lanes.
-        const auto finish = [&](int tile, int r, float lo, float hi) {
-          if (tile >= tiles || r >= n) return;
-          const float f = ctl->factor[r], unscale = pow2(-row_shift<T>(ctl->amax[(stagings - 1) & 1][r]));
-          lo = lo * f * unscale, hi = hi * f * unscale;
-          const int slot = ctl->slot[first + r0 + r];
-          if constexpr (kUp) {
-            p.h[(int64_t)slot * (p.rows / 2) + tile * 8 + g] = lo / (1.f + expf(-lo)) * hi;
-          } else {
-            float* at = p.h + (int64_t)slot * p.rows + tile * 16 + g;
-            at[0] = lo, at[8] = hi;
-          }
-        };
-        if (warps_k == 1) {
-#pragma unroll
-          for (int q = 0; q < NT; ++q) {
-            finish(my_tile, 8 * q + 2 * t, acc[q][0], acc[q][2]);
-            finish(my_tile, 8 * q + 2 * t + 1, acc[q][1], acc[q][3]);
-          }
+      for (int q = 0; q < NT; ++q) acc[q][0] = acc[q][1] = acc[q][2] = acc[q][3] = 0.f;
+      // (columns without a row are not looked at: they read what lies there, or row 0 where less than eight rows fit)
+      const uint4* b = xs + (wk * 8 * p.pass_rows + (g < p.pass_rows ? g : 0)) * 4 + t;
+      const int stride = p.pass_rows * 4;
+      const auto step = [&](bool mine) {
+        if (ok && !ptx::mbar_test(bar_full + s * 8, ph)) ok = ptx::mbar_wait_quiet(bar_full + s * 8, ph);
+        const uint32_t lo = code_lo + s * kStageBytes<kWhole>, hi = code_hi + s * kStageBytes<kWhole>;
+        const uint4 code[2][2] = {{ptx::lds_128(lo), ptx::lds_128(hi)}, {ptx::lds_128(lo + row_step), ptx::lds_128(hi + row_step)}};
+        const uint32_t scale[2] = {read_scales(scale_a + s * kStageBytes<kWhole>), read_scales(scale_b + s * kStageBytes<kWhole>)};
+        __syncwarp();
+        ptx::mbar_arrive_if(bar_empty + s * 8, lane == 0);
+        if (++s == S) s = 0, ph ^= 1;
+        if (mine) multiply<NT>(acc, code, scale, b, stride);
+        b += warps_k * 8 * stride;
+      };
+      const int mine = (p.steps - wk + warps_k - 1) / warps_k;  // (the last turn may have no step for this warp)
+      for (int i = 0; i < turns; i += 2) {
+        step(i < mine);
+        if (i + 1 < turns) step(i + 1 < mine);
+      }
+      // Lane (g, t) has rows g (acc 0, 1) and g + 8 (2, 3) of columns 2 t, 2 t + 1.  A warp of those that split K adds up two
+      // values of each of their lanes.
+      const auto finish = [&](int tile, int r, float lo, float hi) {
+        if (tile >= tiles || r >= n) return;
+        const float f = ctl->factor[r], unscale = pow2(-row_shift<T>(ctl->amax[(stagings - 1) & 1][r]));
+        lo = lo * f * unscale, hi = hi * f * unscale;
+        const int slot = ctl->slot[first + r];
+        if constexpr (kUp) {
+          p.h[(int64_t)slot * (p.rows / 2) + tile * 8 + g] = lo / (1.f + expf(-lo)) * hi;
         } else {
-          consumer_sync();  // (the sums before these have been read)
+          float* at = p.h + (int64_t)slot * p.rows + tile * 16 + g;
+          at[0] = lo, at[8] = hi;
+        }
+      };
+      if (warps_k == 1) {
 #pragma unroll
-          for (int q = 0; q < NT; ++q)
+        for (int q = 0; q < NT; ++q) {
+          finish(my_tile, 8 * q + 2 * t, acc[q][0], acc[q][2]);
+          finish(my_tile, 8 * q + 2 * t + 1, acc[q][1], acc[q][3]);
+        }
+      } else {
+        consumer_sync();  // (the sums before these have been read)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) red[((warp * NT + q) * 4 + j) * 32 + lane] = acc[q][j];
-          consumer_sync();
-          for (int i = tid; i < warps_m * NT * 64; i += kMoeConsumers) {
-            const int j = (i >> 5) & 1, q = (i >> 6) % NT, m = (i >> 6) / NT;  // (i % 32 == lane)
-            float lo = 0.f, hi = 0.f;
-            for (int k = 0; k < warps_k; ++k) {
-              const float* at = red + (((m * warps_k + k) * NT + q) * 4 + j) * 32 + lane;
-              lo += at[0], hi += at[64];
-            }
-            finish(set * warps_m + m, 8 * q + 2 * t + j, lo, hi);
+        for (int q = 0; q < NT; ++q)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) red[((warp * NT + q) * 4 + j) * 32 + lane] = acc[q][j];
+        consumer_sync();
+        for (int i = tid; i < warps_m * NT * 64; i += kMoeConsumers) {
+          const int j = (i >> 5) & 1, q = (i >> 6) % NT, m = (i >> 6) / NT;  // (i % 32 == lane)
+          float lo = 0.f, hi = 0.f;
+          for (int k = 0; k < warps_k; ++k) {
+            const float* at = red + (((m * warps_k + k) * NT + q) * 4 + j) * 32 + lane;
+            lo += at[0], hi += at[64];
           }
+          finish(set * warps_m + m, 8 * q + 2 * t + j, lo, hi);
         }
       }
       if constexpr (!kUp) {
@@ -705,18 +726,19 @@ static double expected_live(const MoeParams& p) {
 
 static int plan_product(MoeParams& p, int64_t K, int64_t rows) {
   p.K = K, p.rows = rows, p.steps = (int)((K + kStep - 1) / kStep);
+  // Rows per pass: every pass of an expert reads its weights again (from the L2, by other CTAs at the same time), and rows take the place
+  // of stages.
+  const double live = expected_live(p), rows_each = p.slots / live;
+  p.pass_rows = rows_each > 12 ? 32 : rows_each > 6 ? 16 : 8;
+  while (p.pass_rows > 1 && (moe_smem(p.steps, p.pass_rows, p.pass_rows > 8 ? 2 : 4) > kMoeMostSmem || p.pass_rows >= 2 * p.slots)) p.pass_rows /= 2;
+  const double passes = rows_each > p.pass_rows / 2 ? live * std::max(1.0, rows_each / p.pass_rows + 0.5) : live;
   // Warps that split K, the others taking tiles of their own: as few as give nine in ten SMs an item (sums of a split K cost two
   // barriers and the shared memory between).  us over 1, 2, 4, 8 and 16 for the first product: 8 named experts of 7168 x 256 41, 31, 26,
   // 24, 24; 8 of 7168 x 2048 61, 62, 62, 65, 70; 101 of them 451, 475, 475, 497, 557.
-  const double live = expected_live(p);
   p.warps_k = 1;
-  while (p.warps_k < kMoeWarps && p.warps_k < p.steps && live * (double)(rows / 16) * p.warps_k / kMoeWarps < 0.85 * sm_count()) p.warps_k *= 2;
+  while (p.warps_k < kMoeWarps && p.warps_k < p.steps && passes * (double)(rows / 16) * p.warps_k / kMoeWarps < 0.85 * sm_count()) p.warps_k *= 2;
   const int per = kMoeWarps / p.warps_k;
   p.sets = (int)((rows / 16 + per - 1) / per);
-  // Rows per pass: every pass reads the weights again (from the L2), and rows take the place of stages.
-  const double rows_each = p.slots / live;
-  p.pass_rows = rows_each > 12 ? 32 : rows_each > 6 ? 16 : 8;
-  while (p.pass_rows > 1 && (moe_smem(p.steps, p.pass_rows, p.pass_rows > 8 ? 2 : 4) > kMoeMostSmem || p.pass_rows >= 2 * p.slots)) p.pass_rows /= 2;
   SGLB_REQUIRE(rows * (K / 16) < (1ll << 31), "fused_experts_fp4: %lld x %lld weights are too many for an expert", (long long)rows, (long long)K);
   p.stages = kMoeMaxStages;
   while (p.stages > 2 && moe_smem(p.steps, p.pass_rows, p.stages) > kMoeMostSmem) --p.stages;
@@ -734,7 +756,7 @@ static int launch_experts(const CUtensorMap& map_w, const CUtensorMap& map_s, co
     SGLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMoeMostSmem));
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  const int64_t most = (int64_t)std::min(p.slots, p.experts) * p.sets;
+  const int64_t most = (int64_t)std::min(p.slots, p.experts + p.slots / p.pass_rows) * p.sets;
   const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, sm_count()));
   SGLB_CUDA(launch_pdl(kern, grid, kMoeThreads<kWhole>, (size_t)moe_smem(p.steps, p.pass_rows, p.stages), st, map_w, map_s, p));
   return SGLB200_OK;

@@ -85,7 +85,9 @@ def _check(got, want, H, I, dtype):
 CASES = [(1, 8, 2, 256, 128), (1, 256, 8, 512, 96), (3, 4, 4, 288, 352), (16, 16, 4, 1024, 512), (33, 8, 2, 512, 160), (64, 4, 1, 416, 1056),
          (5, 3, 1, 7168, 64), (7, 6, 2, 64, 2048), (128, 8, 8, 128, 64), (2, 1, 1, 32, 32),
          # rows' scales on two bytes, on four, on eight; several turns of the ring, ragged sets of tiles
-         (6, 4, 2, 4128, 288), (6, 4, 2, 4160, 320), (6, 4, 2, 4224, 416), (1, 64, 8, 3104, 1056), (50, 6, 3, 2080, 800)]
+         (6, 4, 2, 4128, 288), (6, 4, 2, 4160, 320), (6, 4, 2, 4224, 416), (1, 64, 8, 3104, 1056), (50, 6, 3, 2080, 800),
+         # experts of many rows, whose slots are split among CTAs: few slots, one expert, the same experts for all, the most slots
+         (31, 1, 1, 2080, 256), (64, 1, 1, 4096, 256), (64, 2, 2, 2080, 800), (128, 3, 3, 1056, 96), (1024, 5, 1, 544, 64)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])

@@ -15,11 +15,11 @@
 //
 // A CTA's item is a pass (an expert and at most 32 of its slots) and a few 16-row tiles; its 16 warps split the tiles and K.  Passes of
 // one expert go to CTAs of their own, which read its weights from the L2 (64 tokens, 4 of 8 experts of 4096 x 1024: 106 us, against 148
-// where a CTA took all passes of its tiles in turn).  One more warp keeps a ring of 36 KB stages
-// (codes and scales of 256 columns of all 16 tiles, one TMA load each) full across items, so that the memory streams while rows are
-// staged and sums are taken.  Partial sums meet in shared memory in a fixed order.  The second launch writes every slot's product to a
-// scratch, and whichever CTA is the last of a set of columns adds the slots of a token in their order, so results do not depend on the
-// order of CTAs.
+// where a CTA took all passes of its tiles in turn; 82 with passes of eight rows instead of four).  One more warp keeps a ring of 36 KB
+// stages (codes and scales of 256 columns of all 16 tiles, one TMA load each) full across items, so that the memory streams while
+// rows are staged and sums are taken.  Partial sums meet in shared memory in a fixed order.  The second launch writes every slot's product
+// to a scratch, and whichever CTA is the last of a set of columns adds the slots of a token in their order, so results do not depend
+// on the order of CTAs.
 //
 // 16 tokens, 8 of 256 experts of 7168 x 2048 (101 named, 2.5 GB): 450 to 490 us, 0.80 to 0.85 of the measured copy rate; the first product
 // streams at 0.96 of it, the second's items are shorter: a third of its time is their ends.  What bounds both is the expansion, 1500
@@ -28,6 +28,7 @@
 // token through eighths of experts (25 MB) 21.  Not kept: weights straight into registers (16 warps, three steps deep: 570 us), two
 // tiles a warp (620; the ring is then two stages deep), two CTAs of eight warps an SM (520), a warp of its own that counts items (500).
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "fp4_math.cuh"
@@ -442,7 +443,8 @@ __device__ __forceinline__ void multiply(float (&acc)[NT][4], const uint4 (&code
   }
 }
 
-// kWhole: K is a multiple of a step.  kUp: T is the activations' type and a tile is 8 gate and the 8 matching up rows; else T is float (h) and OutT the output's type.
+// kWhole: K is a multiple of a step.  kUp: T is the activations' type and a tile is 8 gate and the 8 matching up rows; else T is float
+// (h) and OutT the output's type.
 template <typename T, typename OutT, bool kUp, bool kWhole, int NT>
 __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
     fp4_experts_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s,
@@ -724,21 +726,39 @@ static double expected_live(const MoeParams& p) {
   return p.experts * (1.0 - none);
 }
 
-static int plan_product(MoeParams& p, int64_t K, int64_t rows) {
+// Passes of those experts: one each, and one more for every further pass_rows rows (an expert's rows taken as normally distributed).
+static double expected_passes(const MoeParams& p, double live) {
+  const double mean = (double)p.slots / p.experts, sd = std::sqrt(mean * (1.0 - 1.0 / p.experts)) + 0.01;
+  double more = 0.0;
+  for (double rows = p.pass_rows + 0.5; rows < std::min(mean + 4.0 * sd, (double)p.slots); rows += p.pass_rows) {
+    more += 1.0 / (1.0 + std::exp(std::max(-30.0, 1.702 * (rows - mean) / sd)));
+  }
+  return live + p.experts * more;
+}
+
+static int plan_product(MoeParams& p, int64_t K, int64_t rows, bool up) {
   p.K = K, p.rows = rows, p.steps = (int)((K + kStep - 1) / kStep);
   // Rows per pass: every pass of an expert reads its weights again (from the L2, by other CTAs at the same time), and rows take the place
-  // of stages.
+  // of stages; eight columns of an instruction cost the same with one row in them as with eight.  us of a layer over 8, 16 and 32:
+  // 8 rows an expert (64 of 2048 x 1024) 98, 107, 114; 16 (32 of 7168 x 512) 160, 151, 163; 32 (8 of 4096 x 1024) 116, 105, 103.  Four instead
+  // of eight leave long rows more stages, which is worth 2 % where experts have a row or two (7168 x 512) and costs 14 % where they have four.
   const double live = expected_live(p), rows_each = p.slots / live;
-  p.pass_rows = rows_each > 12 ? 32 : rows_each > 6 ? 16 : 8;
-  while (p.pass_rows > 1 && (moe_smem(p.steps, p.pass_rows, p.pass_rows > 8 ? 2 : 4) > kMoeMostSmem || p.pass_rows >= 2 * p.slots)) p.pass_rows /= 2;
-  const double passes = rows_each > p.pass_rows / 2 ? live * std::max(1.0, rows_each / p.pass_rows + 0.5) : live;
-  // Warps that split K, the others taking tiles of their own: as few as give nine in ten SMs an item (sums of a split K cost two
-  // barriers and the shared memory between).  us over 1, 2, 4, 8 and 16 for the first product: 8 named experts of 7168 x 256 41, 31, 26,
-  // 24, 24; 8 of 7168 x 2048 61, 62, 62, 65, 70; 101 of them 451, 475, 475, 497, 557.
-  p.warps_k = 1;
-  while (p.warps_k < kMoeWarps && p.warps_k < p.steps && passes * (double)(rows / 16) * p.warps_k / kMoeWarps < 0.85 * sm_count()) p.warps_k *= 2;
-  const int per = kMoeWarps / p.warps_k;
-  p.sets = (int)((rows / 16 + per - 1) / per);
+  p.pass_rows = rows_each > 18 ? 32 : rows_each > 10 ? 16 : rows_each > 3 || moe_smem(p.steps, 8, 4) <= kMoeMostSmem ? 8 : 4;
+  while (p.pass_rows > 1 && (moe_smem(p.steps, p.pass_rows, 2) > kMoeMostSmem || p.pass_rows >= 2 * p.slots)) p.pass_rows /= 2;
+  const double passes = expected_passes(p, live);
+  // Warps that split K, the others taking tiles of their own: more of them make more and shorter items, which fill the GPU and its last
+  // round better, but each item has an end, of two barriers and the shared memory between where K is split and of a count where
+  // the slots are summed.  Times in turns of the ring: an end is 0.2 of one for the first product, 0.7 with a split K (the second: 0.5, 1.2);
+  // scales that come by asynchronous copies come slower in short runs.  us of a layer over 1, 2, 4 and 8 for the first product: one token,
+  // 8 experts of 7168 x 256 41, 31, 26, 24; 101 named of 7168 x 2048 451, 475, 475, 497; 11 of 4096 x 2048 62, 57, 54, 57; 24 of
+  // 7136 x 544 84, 78, 66, 67.  For the second: 106 of 7168 x 2048 580, 606, 642, 723.
+  double best = 0.0;
+  for (int k = 1; k <= kMoeWarps && k <= p.steps; k *= 2) {
+    const int per = kMoeWarps / k, sets = (int)((rows / 16 + per - 1) / per), turns = (p.steps + k - 1) / k;
+    const double rounds = passes * sets / sm_count(), slow = !up || K % kStep == 0 ? 1.0 : k == 1 ? 1.25 : k == 2 ? 1.08 : 1.0;
+    const double cost = (rounds <= 1.0 ? 1.0 : rounds + 0.5) * (turns * slow + (k == 1 ? 0.2 : 0.7) + (up ? 0.0 : k == 1 ? 0.3 : 0.5));
+    if (k == 1 || cost < best) best = cost, p.warps_k = k, p.sets = sets;
+  }
   SGLB_REQUIRE(rows * (K / 16) < (1ll << 31), "fused_experts_fp4: %lld x %lld weights are too many for an expert", (long long)rows, (long long)K);
   p.stages = kMoeMaxStages;
   while (p.stages > 2 && moe_smem(p.steps, p.pass_rows, p.stages) > kMoeMostSmem) --p.stages;
@@ -844,10 +864,10 @@ int sglb200_fused_experts_fp4(const void* x, int dtype, const void* w13, const v
   p.factor = factor;
   p.wait_probes = g_gemm_wait_probes;
   p.x = x, p.ws = static_cast<const uint8_t*>(w13_scale), p.alpha = w13_alpha, p.h = h;
-  int rc = fp4::plan_product(p, hidden, 2 * intermediate);
+  int rc = fp4::plan_product(p, hidden, 2 * intermediate, true);
   fp4::MoeParams q = p;
   q.x = h, q.ws = static_cast<const uint8_t*>(w2_scale), q.alpha = w2_alpha, q.h = y, q.out = out;
-  if (rc == SGLB200_OK) rc = fp4::plan_product(q, intermediate, hidden);
+  if (rc == SGLB200_OK) rc = fp4::plan_product(q, intermediate, hidden, false);
   if (rc != SGLB200_OK) return rc;
   rc = dtype == 0 ? fp4::launch_product<__nv_bfloat16, __nv_bfloat16, true>(w13, p, st) : fp4::launch_product<__half, __half, true>(w13, p, st);
   if (rc != SGLB200_OK) return rc;

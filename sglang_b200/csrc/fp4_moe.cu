@@ -342,12 +342,14 @@ __device__ __noinline__ void stage_rows(const MoeParams& p, MoeCtl* ctl, int exp
     ctl->factor[tid] = std::is_same<T, float>::value ? alpha * __ldcg(p.weights + ctl->slot[first + tid]) : alpha;
   }
   const int share = n > 8 ? 0 : n > 4 ? 1 : n > 2 ? 2 : n > 1 ? 3 : 4;  // 2^share warps to a row
+  // (Four lanes take pieces that lie side by side in shared memory and eight lanes those of two jj, which fall on the same banks twice
+  // at most; in the order of the columns it would be eight times.  1 to 3 % of a layer whose experts have many rows.)
   constexpr int kAhead = 2;  // pieces that are asked for before the first is converted (four: 2 us more a layer, for the instructions)
   for (int r = warp >> share; r < n; r += kMoeWarps >> share) {
     const T* src = act_row<T>(p, ctl->slot[first + r]);
     uint32_t most = 0;
 #pragma unroll 1
-    for (int q0 = (warp & ((1 << share) - 1)) * 32 + lane; q0 < pieces; q0 += (kAhead * 32) << share) {
+    for (int q0 = (warp & ((1 << share) - 1)) * 32 + (lane & 3) * 8 + (lane >> 2); q0 < pieces; q0 += (kAhead * 32) << share) {
       Piece<T> x[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {

@@ -138,7 +138,7 @@ int sglb200_group_fp4_scaled_mm(const void* A, const void* B, const void* a_s, c
  * float32 per expert (1 / the global scale of its weights), NULL = 1.  topk_ids int32 [tokens, topk]; an id outside [0, E) (an expert
  * of another rank) contributes nothing, the same id twice in a row counts twice.  Activations are not quantised: products with weights are exact in
  * fp16 (bf16 activations under a power of two per row; what is below 2^-18 of a row's largest magnitude is rounded to 2^-26 of
- * it), sums are float32, h is rounded to 11 bits for the second product, the output once.
+ * it), sums are float32, h is held to 23 bits for the second product (2^-23 of a value, 2^-37 of a row's largest), the output rounded once.
  * tokens * topk <= 1024, E <= 1024, hidden and intermediate divisible by 32; pointers 16-byte aligned.
  * A row with a NaN or an infinity gives NaN or infinities in that row only.  A wait inside a kernel that runs out sets
  * sglb200_gemm_status().

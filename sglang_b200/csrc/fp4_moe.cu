@@ -11,7 +11,8 @@
 // activation rows are the other; with more rows of an expert, 16 or 32 of them share what was expanded.  bf16 activations become fp16
 // under a power of two per row: 2^6 where the row's largest magnitude lies in [2^-5, 2^9), else what brings that to 2^14.  So they are
 // exact down to 2^-18 of that magnitude and off by at most 2^-26 of it below.  h is kept in float32 and enters the second product
-// as fp16 likewise (2^-12 of a value, an eighth of what rounding the output to bf16 costs).
+// under such a power of two as the sum of two fp16 terms, hi + 2^-11 lo, a column each: 23 bits, off by at most 2^-23 of a value or 2^-37 of
+// the row's largest.  (hi alone, 11 bits, moved one bf16 output in fifty by a step.)
 //
 // A CTA's item is a pass (an expert and at most 32 of its slots) and a few 16-row tiles; its 16 warps split the tiles and K.  Passes of
 // one expert go to CTAs of their own, which read its weights from the L2 (64 tokens, 4 of 8 experts of 4096 x 1024: 106 us, against 148
@@ -45,7 +46,11 @@ template <bool kWhole>
 constexpr int kMoeThreads = kMoeConsumers + 32 + (kWhole ? 0 : kScaleWarps * 32);
 constexpr int kMoeMaxExperts = 1024, kMoeMaxSlots = 1024;
 constexpr int kStep = 256;                    // columns per step: a lane takes 64 of a row, 32 bytes of codes and four scales
-constexpr int kMoeRows = 32;                  // activation rows per pass, at most: four times the eight of an instruction
+constexpr int kMoeRows = 32;                  // activation rows per pass, at most: four times the eight columns of an instruction
+// Columns of an instruction that an activation row takes: a float32 row has two, its terms.
+template <typename T>
+constexpr int kTerms = std::is_same<T, float>::value ? 2 : 1;
+constexpr float kLoTerm = 0x1p-11f;           // the second term's unit in the first one's
 constexpr uint32_t kTileBytes = 16 * kStep / 2;                  // of a tile and step
 constexpr uint32_t kCodeBytes = kMoeWarps * kTileBytes;    // of a stage: 32 KB, and 4 or 5 KB of scales
 // Scales of a row and step in a stage: 16 bytes, or the five words that hold them where rows begin on two bytes.
@@ -74,6 +79,7 @@ struct MoeParams {
   int warps_k;              // warps that split K; the others split tiles
   int sets;                 // items per pass
   int pass_rows;            // activation rows per pass
+  int cols;                 // columns of an instruction that they take
   int stages;
   float factor;
   uint32_t wait_probes;
@@ -312,7 +318,20 @@ __device__ __forceinline__ uint4 to_f16(const Piece<T>& x, float f) {
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-// The same of a row that is not finite: its finite values stay finite.
+// What that rounding left over, in units of kLoTerm: at most 2^14, as the first term is below 2^15.
+template <typename T>
+__device__ __forceinline__ uint4 rest_f16(const Piece<T>& x, float f, const uint4& first) {
+  const uint32_t had[4] = {first.x, first.y, first.z, first.w};
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = x.pair(i), h = f16x2_to_f32(had[i]);
+    const __half2 r = __floats2half2_rn(fmaf(v.x, f, -h.x) * (1.f / kLoTerm), fmaf(v.y, f, -h.y) * (1.f / kLoTerm));
+    w[i] = *reinterpret_cast<const uint32_t*>(&r);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The first term of a row that is not finite, whose second one is zero: its finite values stay finite.
 template <typename T>
 __device__ __forceinline__ uint4 to_f16_clamped(const Piece<T>& x) {
   uint32_t w[4];
@@ -327,13 +346,15 @@ __device__ __forceinline__ uint4 to_f16_clamped(const Piece<T>& x) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Rows [first, first + n) of the slots, as fp16 in the order in which lanes take them: 16-byte pieces of 8 columns, piece
-// (step, jj, row, t) = columns step * 256 + t * 64 + jj * 8 ..; columns past K are zeros.  The multiplying warps, which share out the
+// Rows [first, first + n) of the slots, as fp16 in the order in which lanes take them: 16-byte pieces of 8 columns of K, piece
+// (step, jj, column, t) = columns step * 256 + t * 64 + jj * 8 ..; what is past K is zeros.  A row of two terms has them in neighbouring columns,
+// or, where only one fits (`term` 0 or 1, else -1), that one in the row's column.  The multiplying warps, which share out the
 // rows, several to a row where there are few; ends with a barrier.
 template <typename T>
-__device__ __noinline__ void stage_rows(const MoeParams& p, MoeCtl* ctl, int expert, int first, int n, int turn, uint4* xs) {
+__device__ __noinline__ void stage_rows(const MoeParams& p, MoeCtl* ctl, int expert, int first, int n, int turn, int term, uint4* xs) {
+  constexpr bool kTwo = kTerms<T> == 2;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int pieces = p.steps * 32, K = (int)p.K, row_pitch = p.pass_rows * 4;
+  const int pieces = p.steps * 32, K = (int)p.K, pitch = p.cols * 4, row_pitch = kTwo && term < 0 ? 8 : 4;
   int* amax = ctl->amax[turn & 1];
   if (turn > 0) consumer_sync();  // the rows before these have been used
   if (tid < kMoeRows) ctl->amax[(turn + 1) & 1][tid] = 0;
@@ -341,6 +362,17 @@ __device__ __noinline__ void stage_rows(const MoeParams& p, MoeCtl* ctl, int exp
     const float alpha = p.alpha ? __ldcg(p.alpha + expert) : 1.f;
     ctl->factor[tid] = std::is_same<T, float>::value ? alpha * __ldcg(p.weights + ctl->slot[first + tid]) : alpha;
   }
+  const auto put = [&](int r, int q, const Piece<T>& x, float f, bool fine) {
+    uint4* at = xs + ((q >> 5) * 8 + (q & 7)) * pitch + r * row_pitch + ((q >> 3) & 3);
+    const uint4 hi = fine ? to_f16(x, f) : to_f16_clamped(x);
+    if constexpr (kTwo) {
+      const uint4 lo = fine ? rest_f16(x, f, hi) : make_uint4(0, 0, 0, 0);
+      if (term < 0) at[4] = lo;
+      *at = term == 1 ? lo : hi;
+    } else {
+      *at = hi;
+    }
+  };
   const int share = n > 8 ? 0 : n > 4 ? 1 : n > 2 ? 2 : n > 1 ? 3 : 4;  // 2^share warps to a row
   // (Four lanes take pieces that lie side by side in shared memory and eight lanes those of two jj, which fall on the same banks twice
   // at most; in the order of the columns it would be eight times.  1 to 3 % of a layer whose experts have many rows.)
@@ -360,7 +392,7 @@ __device__ __noinline__ void stage_rows(const MoeParams& p, MoeCtl* ctl, int exp
       for (int k = 0; k < kAhead; ++k) {
         const int q = q0 + ((k * 32) << share);
         if constexpr (!std::is_same<T, __half>::value) most = x[k].most(most);
-        if (q < pieces) xs[((q >> 5) * 8 + (q & 7)) * row_pitch + r * 4 + ((q >> 3) & 3)] = to_f16(x[k], pow2(kUsualShift));
+        if (q < pieces) put(r, q, x[k], pow2(kUsualShift), true);
       }
     }
     if constexpr (!std::is_same<T, __half>::value) {
@@ -377,13 +409,12 @@ __device__ __noinline__ void stage_rows(const MoeParams& p, MoeCtl* ctl, int exp
       const int bits = amax[r], shift = row_shift<T>(bits);
       if (shift == kUsualShift) continue;
       again = true;
-      const bool fine = bits < 0x7f800000;
       const T* src = act_row<T>(p, ctl->slot[first + r]);
 #pragma unroll 1
       for (int q = tid; q * 8 < K; q += kMoeConsumers) {
         Piece<T> x;
         x.load(src + q * 8);
-        xs[((q >> 5) * 8 + (q & 7)) * row_pitch + r * 4 + ((q >> 3) & 3)] = fine ? to_f16(x, pow2(shift)) : to_f16_clamped(x);
+        put(r, q, x, pow2(shift), bits < 0x7f800000);
       }
     }
     if (again) consumer_sync();  // (the same for all threads)
@@ -446,15 +477,15 @@ __device__ __forceinline__ void multiply(float (&acc)[NT][4], const uint4 (&code
 }
 
 // kWhole: K is a multiple of a step.  kUp: T is the activations' type and a tile is 8 gate and the 8 matching up rows; else T is float
-// (h) and OutT the output's type.
-template <typename T, typename OutT, bool kUp, bool kWhole, int NT>
+// (h) and OutT the output's type.  kTwice: both terms of a row of h do not fit, so an item takes K twice, first with the lesser ones.
+template <typename T, typename OutT, bool kUp, bool kWhole, int NT, bool kTwice>
 __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
     fp4_experts_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s,
                        const __grid_constant__ MoeParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint4* xs = reinterpret_cast<uint4*>(ring + p.stages * kStageBytes<kWhole>);
-  float* red = reinterpret_cast<float*>(xs + p.steps * 32 * p.pass_rows);  // [warp][4 NT][32]
+  float* red = reinterpret_cast<float*>(xs + p.steps * 32 * p.cols);  // [warp][values of a lane][32]
   MoeCtl* ctl = reinterpret_cast<MoeCtl*>(red + kMoeWarps * NT * 128);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const uint32_t bar_full = ptx::smem_u32(ctl->full), bar_empty = ptx::smem_u32(ctl->empty);
@@ -480,7 +511,7 @@ __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
 
   const int warps_k = p.warps_k, warps_m = kMoeWarps / warps_k;
   const int tiles = (int)(p.rows / 16);  // of an expert (16 rows of w each)
-  const int items = ctl->num_live * p.sets, turns = (p.steps + warps_k - 1) / warps_k;
+  const int items = ctl->num_live * p.sets, turns = (p.steps + warps_k - 1) / warps_k, all_turns = kTwice ? 2 * turns : turns;
   // A CTA takes neighbouring items, which are mostly of one pass.
   const int each = (int)((uint32_t)items / gridDim.x), more = items - each * (int)gridDim.x;
   const int item0 = (int)blockIdx.x * each + min((int)blockIdx.x, more), item1 = item0 + each + ((int)blockIdx.x < more ? 1 : 0);
@@ -493,7 +524,7 @@ __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
       uint32_t ph = 1, part_bytes = warps_m * kTileBytes;  // (the first round of stages is free)
       for (int item = item0; item < item1 && ok; ++item) {
         const int live = item / p.sets, tile0 = (item - live * p.sets) * warps_m, expert = ctl->live[live];
-        for (int i = 0, step0 = 0; i < turns; ++i) {
+        for (int i = 0, step0 = 0; i < all_turns; ++i) {
           ok = p.wait_probes != ptx::kProbesNone && ptx::mbar_wait_quiet(bar_empty + s * 8, ph);
           if (!ok) break;
           const uint32_t bar = bar_full + s * 8, at = ptx::smem_u32(ring) + s * kStageBytes<kWhole>;
@@ -516,7 +547,7 @@ __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
                 ptx::tma_load_3d(at + k * part_bytes, &map_w, bar, (step0 + k) * (kStep / 2), tile0 * 16, expert);
             }
           }
-          step0 += warps_k;
+          step0 = kTwice && i + 1 == turns ? 0 : step0 + warps_k;
           if (++s == S) s = 0, ph ^= 1;
         }
       }
@@ -563,7 +594,7 @@ __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
         rows_there |= (h + j * kScaleWarps * 32 < kAll && tile_row + row < limit ? 1u : 0u) << j;
       }
       const bool all_there = tile_row + (kUp ? half_rows : warps_m * 16) <= limit;
-      for (int i = 0, step0 = 0; i < turns; ++i) {
+      for (int i = 0, step0 = 0; i < all_turns; ++i) {
         ok = ok && (ptx::mbar_test(bar_empty + s * 8, ph) || ptx::mbar_wait_quiet(bar_empty + s * 8, ph));
         if (!ok) break;
         const uint32_t at = ptx::smem_u32(ring) + s * kStageBytes<kWhole> + kCodeBytes + h * 4;
@@ -585,7 +616,7 @@ __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
             }
         }
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar_full + s * 8) : "memory");
-        step0 += warps_k;
+        step0 = kTwice && i + 1 == turns ? 0 : step0 + warps_k;
         if (++s == S) s = 0, ph ^= 1;
       }
     }
@@ -622,34 +653,51 @@ __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
       const int live = item / p.sets, set = item - live * p.sets;
       const int expert = ctl->live[live], first = ctl->begin[live], n = ctl->begin[live + 1] - first;
       const int my_tile = set * warps_m + wm;
-      if (staged != live) {
-        stage_rows<T>(p, ctl, expert, first, n, stagings, xs);
-        ++stagings, staged = live;
-      }
       float acc[NT][4];
 #pragma unroll
       for (int q = 0; q < NT; ++q) acc[q][0] = acc[q][1] = acc[q][2] = acc[q][3] = 0.f;
-      // (columns without a row are not looked at: they read what lies there, or row 0 where less than eight rows fit)
-      const uint4* b = xs + (wk * 8 * p.pass_rows + (g < p.pass_rows ? g : 0)) * 4 + t;
-      const int stride = p.pass_rows * 4;
-      const auto step = [&](bool mine) {
-        if (ok && !ptx::mbar_test(bar_full + s * 8, ph)) ok = ptx::mbar_wait_quiet(bar_full + s * 8, ph);
-        const uint32_t lo = code_lo + s * kStageBytes<kWhole>, hi = code_hi + s * kStageBytes<kWhole>;
-        const uint4 code[2][2] = {{ptx::lds_128(lo), ptx::lds_128(hi)}, {ptx::lds_128(lo + row_step), ptx::lds_128(hi + row_step)}};
-        const uint32_t scale[2] = {read_scales(scale_a + s * kStageBytes<kWhole>), read_scales(scale_b + s * kStageBytes<kWhole>)};
-        __syncwarp();
-        ptx::mbar_arrive_if(bar_empty + s * 8, lane == 0);
-        if (++s == S) s = 0, ph ^= 1;
-        if (mine) multiply<NT>(acc, code, scale, b, stride);
-        b += warps_k * 8 * stride;
+      const int stride = p.cols * 4, mine = (p.steps - wk + warps_k - 1) / warps_k;  // (the last turn may have no step for this warp)
+      const auto take_all = [&](int term) {  // K of the staged rows, or of their one term
+        if (kTwice || staged != live) {
+          stage_rows<T>(p, ctl, expert, first, n, stagings, term, xs);
+          ++stagings, staged = live;
+        }
+        // (columns without a row are not looked at: they read what lies there, or column 0 where less than eight fit)
+        const uint4* b = xs + (wk * 8 * p.cols + (g < p.cols ? g : 0)) * 4 + t;
+        const auto step = [&](bool mine) {
+          if (ok && !ptx::mbar_test(bar_full + s * 8, ph)) ok = ptx::mbar_wait_quiet(bar_full + s * 8, ph);
+          const uint32_t lo = code_lo + s * kStageBytes<kWhole>, hi = code_hi + s * kStageBytes<kWhole>;
+          const uint4 code[2][2] = {{ptx::lds_128(lo), ptx::lds_128(hi)}, {ptx::lds_128(lo + row_step), ptx::lds_128(hi + row_step)}};
+          const uint32_t scale[2] = {read_scales(scale_a + s * kStageBytes<kWhole>), read_scales(scale_b + s * kStageBytes<kWhole>)};
+          __syncwarp();
+          ptx::mbar_arrive_if(bar_empty + s * 8, lane == 0);
+          if (++s == S) s = 0, ph ^= 1;
+          if (mine) multiply<NT>(acc, code, scale, b, stride);
+          b += warps_k * 8 * stride;
+        };
+        for (int i = 0; i < turns; i += 2) {
+          step(i < mine);
+          if (i + 1 < turns) step(i + 1 < mine);
+        }
       };
-      const int mine = (p.steps - wk + warps_k - 1) / warps_k;  // (the last turn may have no step for this warp)
-      for (int i = 0; i < turns; i += 2) {
-        step(i < mine);
-        if (i + 1 < turns) step(i + 1 < mine);
+      if constexpr (kTwice) {
+        take_all(1);
+#pragma unroll
+        for (int q = 0; q < NT; ++q)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[q][j] *= kLoTerm;
+        take_all(0);
+      } else {
+        take_all(-1);
       }
-      // Lane (g, t) has rows g (acc 0, 1) and g + 8 (2, 3) of columns 2 t, 2 t + 1.  A warp of those that split K adds up two
-      // values of each of their lanes.
+      // Lane (g, t) has rows g (acc 0, 1) and g + 8 (2, 3) of columns 2 t, 2 t + 1: of two activation rows, or both terms of one, which
+      // are added here.  A warp of those that split K adds up kVals values of each of their lanes.
+      constexpr bool kPairs = !kUp && !kTwice;
+      constexpr int kVals = kPairs ? 1 : 2;  // activation rows of a lane and eight columns
+      if constexpr (kPairs) {
+#pragma unroll
+        for (int q = 0; q < NT; ++q) acc[q][0] = fmaf(acc[q][1], kLoTerm, acc[q][0]), acc[q][1] = fmaf(acc[q][3], kLoTerm, acc[q][2]);
+      }
       const auto finish = [&](int tile, int r, float lo, float hi) {
         if (tile >= tiles || r >= n) return;
         const float f = ctl->factor[r], unscale = pow2(-row_shift<T>(ctl->amax[(stagings - 1) & 1][r]));
@@ -664,25 +712,24 @@ __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
       };
       if (warps_k == 1) {
 #pragma unroll
-        for (int q = 0; q < NT; ++q) {
-          finish(my_tile, 8 * q + 2 * t, acc[q][0], acc[q][2]);
-          finish(my_tile, 8 * q + 2 * t + 1, acc[q][1], acc[q][3]);
-        }
+        for (int q = 0; q < NT; ++q)
+#pragma unroll
+          for (int j = 0; j < kVals; ++j) finish(my_tile, kVals * (4 * q + t) + j, acc[q][j], acc[q][j + kVals]);
       } else {
         consumer_sync();  // (the sums before these have been read)
 #pragma unroll
         for (int q = 0; q < NT; ++q)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) red[((warp * NT + q) * 4 + j) * 32 + lane] = acc[q][j];
+          for (int j = 0; j < 2 * kVals; ++j) red[((warp * NT + q) * 2 * kVals + j) * 32 + lane] = acc[q][j];
         consumer_sync();
-        for (int i = tid; i < warps_m * NT * 64; i += kMoeConsumers) {
-          const int j = (i >> 5) & 1, q = (i >> 6) % NT, m = (i >> 6) / NT;  // (i % 32 == lane)
+        for (int i = tid; i < warps_m * NT * kVals * 32; i += kMoeConsumers) {
+          const int j = (i >> 5) % kVals, q = (i >> 5) / kVals % NT, m = (i >> 5) / kVals / NT;  // (i % 32 == lane)
           float lo = 0.f, hi = 0.f;
           for (int k = 0; k < warps_k; ++k) {
-            const float* at = red + (((m * warps_k + k) * NT + q) * 4 + j) * 32 + lane;
-            lo += at[0], hi += at[64];
+            const float* at = red + (((m * warps_k + k) * NT + q) * 2 * kVals + j) * 32 + lane;
+            lo += at[0], hi += at[kVals * 32];
           }
-          finish(set * warps_m + m, 8 * q + 2 * t + j, lo, hi);
+          finish(set * warps_m + m, kVals * (4 * q + t) + j, lo, hi);
         }
       }
       if constexpr (!kUp) {
@@ -716,8 +763,8 @@ __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
   }
 }
 
-constexpr int64_t moe_smem(int steps, int pass_rows, int stages) {  // (the larger stages: where K is whole steps a little is left over)
-  return 1024 + (int64_t)stages * kStageBytes<false> + (int64_t)steps * 512 * pass_rows + kMoeWarps * 512 * ((pass_rows + 7) / 8) + (int64_t)sizeof(MoeCtl);
+constexpr int64_t moe_smem(int steps, int cols, int stages) {  // (the larger stages: where K is whole steps a little is left over)
+  return 1024 + (int64_t)stages * kStageBytes<false> + (int64_t)steps * 512 * cols + kMoeWarps * 512 * ((cols + 7) / 8) + (int64_t)sizeof(MoeCtl);
 }
 constexpr int64_t kMoeMostSmem = 227 * 1024;
 
@@ -740,13 +787,17 @@ static double expected_passes(const MoeParams& p, double live) {
 
 static int plan_product(MoeParams& p, int64_t K, int64_t rows, bool up) {
   p.K = K, p.rows = rows, p.steps = (int)((K + kStep - 1) / kStep);
-  // Rows per pass: every pass of an expert reads its weights again (from the L2, by other CTAs at the same time), and rows take the place
-  // of stages; eight columns of an instruction cost the same with one row in them as with eight.  us of a layer over 8, 16 and 32:
-  // 8 rows an expert (64 of 2048 x 1024) 98, 107, 114; 16 (32 of 7168 x 512) 160, 151, 163; 32 (8 of 4096 x 1024) 116, 105, 103.  Four instead
-  // of eight leave long rows more stages, which is worth 2 % where experts have a row or two (7168 x 512) and costs 14 % where they have four.
-  const double live = expected_live(p), rows_each = p.slots / live;
-  p.pass_rows = rows_each > 18 ? 32 : rows_each > 10 ? 16 : rows_each > 3 || moe_smem(p.steps, 8, 4) <= kMoeMostSmem ? 8 : 4;
-  while (p.pass_rows > 1 && (moe_smem(p.steps, p.pass_rows, 2) > kMoeMostSmem || p.pass_rows >= 2 * p.slots)) p.pass_rows /= 2;
+  // Rows per pass, and the columns that they take (two a row of h): every pass of an expert reads its weights again (from the L2, by other
+  // CTAs at the same time), and columns take the place of stages; eight columns cost the same with one row in them as with all.
+  // us of a layer over 8, 16 and 32 columns of x: 8 rows an expert (64 of 2048 x 1024) 98, 107, 114; 16 (32 of 7168 x 512) 160, 151, 163; 32
+  // (8 of 4096 x 1024) 116, 105, 103; the same of h 113, 101, 117; 184, 150, 146; 97, 94, 89.  Four instead of eight leave long rows more stages,
+  // which is worth 2 % where experts have a row or two (7168 x 512) and costs 14 % where they have four.
+  const int terms = up ? 1 : 2;
+  const double live = expected_live(p), cols_each = p.slots / live * terms;
+  p.cols = cols_each > 18 ? 32 : cols_each > 10 ? 16 : cols_each > 3 || moe_smem(p.steps, 8, 4) <= kMoeMostSmem ? 8 : 4;
+  while (p.cols > terms && (moe_smem(p.steps, p.cols, 2) > kMoeMostSmem || p.cols >= 2 * terms * p.slots)) p.cols /= 2;
+  if (moe_smem(p.steps, p.cols, 2) > kMoeMostSmem) p.cols = 1;
+  p.pass_rows = std::max(1, p.cols / terms);
   const double passes = expected_passes(p, live);
   // Warps that split K, the others taking tiles of their own: more of them make more and shorter items, which fill the GPU and its last
   // round better, but each item has an end, of two barriers and the shared memory between where K is split and of a count where
@@ -763,14 +814,14 @@ static int plan_product(MoeParams& p, int64_t K, int64_t rows, bool up) {
   }
   SGLB_REQUIRE(rows * (K / 16) < (1ll << 31), "fused_experts_fp4: %lld x %lld weights are too many for an expert", (long long)rows, (long long)K);
   p.stages = kMoeMaxStages;
-  while (p.stages > 2 && moe_smem(p.steps, p.pass_rows, p.stages) > kMoeMostSmem) --p.stages;
-  SGLB_REQUIRE(moe_smem(p.steps, p.pass_rows, p.stages) <= kMoeMostSmem, "fused_experts_fp4: %lld columns are too many", (long long)K);
+  while (p.stages > 2 && moe_smem(p.steps, p.cols, p.stages) > kMoeMostSmem) --p.stages;
+  SGLB_REQUIRE(moe_smem(p.steps, p.cols, p.stages) <= kMoeMostSmem, "fused_experts_fp4: %lld columns are too many", (long long)K);
   return SGLB200_OK;
 }
 
-template <typename T, typename OutT, bool kUp, bool kWhole, int NT>
+template <typename T, typename OutT, bool kUp, bool kWhole, int NT, bool kTwice>
 static int launch_experts(const CUtensorMap& map_w, const CUtensorMap& map_s, const MoeParams& p, cudaStream_t st) {
-  auto kern = fp4_experts_kernel<T, OutT, kUp, kWhole, NT>;
+  auto kern = fp4_experts_kernel<T, OutT, kUp, kWhole, NT, kTwice>;
   static thread_local bool attr_set[64] = {false};  // the opt-in is per function and per device
   int dev = 0;
   SGLB_CUDA(cudaGetDevice(&dev));
@@ -780,7 +831,7 @@ static int launch_experts(const CUtensorMap& map_w, const CUtensorMap& map_s, co
   }
   const int64_t most = (int64_t)std::min(p.slots, p.experts + p.slots / p.pass_rows) * p.sets;
   const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, sm_count()));
-  SGLB_CUDA(launch_pdl(kern, grid, kMoeThreads<kWhole>, (size_t)moe_smem(p.steps, p.pass_rows, p.stages), st, map_w, map_s, p));
+  SGLB_CUDA(launch_pdl(kern, grid, kMoeThreads<kWhole>, (size_t)moe_smem(p.steps, p.cols, p.stages), st, map_w, map_s, p));
   return SGLB200_OK;
 }
 
@@ -803,10 +854,14 @@ static int launch_product(const void* w, const MoeParams& p, cudaStream_t st) {
   int rc = map_of(w, (uint64_t)p.K / 2, kStep / 2, true, &map_w);
   if (rc) return rc;
   if (whole && (rc = map_of(p.ws, (uint64_t)p.K / 16, kStep / 16, false, &map_s)) != SGLB200_OK) return rc;
-#define GO(NT) return whole ? launch_experts<T, OutT, kUp, true, NT>(map_w, map_s, p, st) : launch_experts<T, OutT, kUp, false, NT>(map_w, map_w, p, st)
-  if (p.pass_rows <= 8) GO(1);
-  if (p.pass_rows <= 16) GO(2);
-  GO(4);
+#define GO(NT, TWICE) return whole ? launch_experts<T, OutT, kUp, true, NT, TWICE>(map_w, map_s, p, st) \
+                                   : launch_experts<T, OutT, kUp, false, NT, TWICE>(map_w, map_w, p, st)
+  if constexpr (!kUp) {
+    if (p.cols == 1) GO(1, true);
+  }
+  if (p.cols <= 8) GO(1, false);
+  if (p.cols <= 16) GO(2, false);
+  GO(4, false);
 #undef GO
 }
 

@@ -108,6 +108,16 @@ __device__ __forceinline__ uint32_t group_scale_e4m3(float amax, float g) {
   return lo;
 }
 
+// silu(gate) * up in float32.  Below kSiluTail 1 + e^-gate and its reciprocal come to the ends of float32's range, while silu = gate e^gate,
+// times a large `up`, need not be small: e^(gate / 2) is taken twice there, with `up` in between.
+constexpr float kSiluTail = -87.0f;
+__device__ __forceinline__ float silu_mul(float gate, float up) {
+  if (gate < kSiluTail) {
+    const float e = expf(0.5f * gate);
+    return gate * e * up * e;
+  }
+  return gate / (1.f + expf(-gate)) * up;
+}
 // (a, b) times r, both products in one instruction.
 __device__ __forceinline__ void mul2(float& a, float& b, float x, float y, float r) {
   asm("{\n\t.reg .b64 v, f, q;\n\t"

@@ -704,7 +704,7 @@ __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
         lo = lo * f * unscale, hi = hi * f * unscale;
         const int slot = ctl->slot[first + r];
         if constexpr (kUp) {
-          p.h[(int64_t)slot * (p.rows / 2) + tile * 8 + g] = lo / (1.f + expf(-lo)) * hi;
+          p.h[(int64_t)slot * (p.rows / 2) + tile * 8 + g] = silu_mul(lo, hi);
         } else {
           float* at = p.h + (int64_t)slot * p.rows + tile * 16 + g;
           at[0] = lo, at[8] = hi;

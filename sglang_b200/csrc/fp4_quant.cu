@@ -138,6 +138,49 @@ __device__ __forceinline__ uint32_t quantize16(const float (&v)[16], float g, ui
   return code;
 }
 
+// Quantises 16 columns of silu(gate) * up, of a group of kGroup from `gate` on, once more in float64: rows whose values float32 does not do
+// for, few enough that neither this function's time nor its reading one value at a time shows.  `mine`: the 16 of the group.
+template <typename T, int kGroup>
+__device__ __noinline__ void quantize_silu_f64(const T* gate, const T* up, int mine, float g, uint2* codes, uint8_t* scale) {
+  double h[kGroup], amax = 0.0;
+  bool fine = true;
+#pragma unroll 1
+  for (int i = 0; i < kGroup; ++i) {
+    const double x = (double)ElemTraits<T>::to_f32(gate[i]);
+    h[i] = x / (1.0 + exp(-x)) * (double)ElemTraits<T>::to_f32(up[i]);
+    fine = fine && fabsf((float)h[i]) < __int_as_float(0x7f800000);
+    amax = fmax(amax, fabs(h[i]));
+  }
+  constexpr float kLess = 1.0f - 0x1p-20f, kMore = 1.0f + 0x1p-20f;
+  uint32_t code;
+  double s;  // of the values times g
+  if constexpr (kGroup == 32) {
+    const int e = amax > 0.0 ? max(ilogb(amax) - 2, -127) : -127;
+    code = (uint32_t)(e + 127), s = ldexp(1.0, e);
+  } else {
+    const float v = (float)(amax * (double)g / 6.0);
+    const uint32_t two = cvt_e4m3x2(v * kLess, v * kMore);
+    const float2 f = f16x2_to_f32(cvt_f16x2_e4m3x2(two));
+    const double border = 3.0 * ((double)f.x + (double)f.y), num = amax * (double)g;
+    const bool higher = (two & 0xff) != two >> 8 && (num > border || (num == border && (two & 1)));
+    code = higher ? two >> 8 : two & 0xff, s = higher ? f.y : f.x;
+  }
+  if (!fine) code = kGroup == 32 ? kNanE8m0 : kNanE4m3;
+  uint32_t word[2] = {0u, 0u};
+  if (fine && s > 0.0) {
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i) {
+      const double num = fabs(h[mine + i]) * (kGroup == 32 ? 1.0 : (double)g);
+      const float q = (float)fmin(num / s, 8.0);
+      uint32_t two = cvt_e2m1x2(q * kLess, q * kMore), c = two & 15;
+      if (c != two >> 4 && (num > (double)e2m1_border(c) * s || (num == (double)e2m1_border(c) * s && (c & 1)))) ++c;
+      word[i >> 3] |= (c | (signbit(h[mine + i]) ? 8u : 0u)) << 4 * (i & 7);
+    }
+  }
+  *codes = make_uint2(word[0], word[1]);
+  if (mine == 0) *scale = (uint8_t)code;
+}
+
 // A warp takes kAhead tasks, whose values are all asked for before the first is quantised.
 template <typename T, int kGroup, bool kSilu, bool kWide, int kAhead>
 __global__ void __launch_bounds__(kThreads)
@@ -157,6 +200,7 @@ __global__ void __launch_bounds__(kThreads)
     if constexpr (kSilu) raw[k][1].template load<kWide>(src + (int64_t)units * kUnit);
   }
   const float g = global_scale ? __ldcg(global_scale) : 1.0f;
+  uint32_t again = 0;  // tasks that float32 does not do for
 #pragma unroll
   for (int k = 0; k < kAhead; ++k) {
     if (task0 + k * (kThreads / 32) >= tasks) break;
@@ -165,11 +209,15 @@ __global__ void __launch_bounds__(kThreads)
     if constexpr (kSilu) {
       float up[16];
       raw[k][1].to_f32(up);
+      float least = fminf(v[0], v[1]);
+#pragma unroll
+      for (int i = 2; i < 16; ++i) least = fminf(least, v[i]);
+      if (least < kSiluTail) again |= 1u << k;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        // The quotient by a reciprocal and one correction: half a unit in the last place, and the instructions of a division are
-        // half of the kernel's.  Below -87, where the reciprocal is flushed to zero, it is zero.
-        const float d = fminf(1.0f + expf(-v[i]), 1e38f);
+        // The quotient by a reciprocal and one correction (Markstein's): half a unit in the last place, and the instructions of a division
+        // are half of the kernel's.  Not below kSiluTail.
+        const float d = 1.0f + expf(-v[i]);
         float r;
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
         const float q = v[i] * r;
@@ -180,6 +228,18 @@ __global__ void __launch_bounds__(kThreads)
     const uint32_t code = quantize16<kGroup>(v, g, c);
     if (at[k].live) codes[at[k].unit] = c;
     if (at[k].row_live && at[k].column % (kGroup / kUnit) == 0) scales[at[k].scale] = at[k].live ? (uint8_t)code : 0;  // (zeros for groups past the last)
+  }
+  if constexpr (kSilu) {
+    if constexpr (kGroup == 32) again |= __shfl_xor_sync(0xffffffffu, again, 1);  // (both halves of a group)
+    if (again == 0) return;
+#pragma unroll 1
+    for (int k = 0; k < kAhead; ++k) {
+      const Place<kGroup> place(min(task0 + k * (kThreads / 32), tasks - 1), blocks, units, rows);
+      if ((again >> k & 1) == 0 || !place.live) continue;
+      const uint32_t mine = place.column % (kGroup / kUnit);
+      const T* gate = x + (2 * place.unit - place.column - mine) * kUnit;  // the group's first: rows of twice the columns
+      quantize_silu_f64<T, kGroup>(gate, gate + (int64_t)units * kUnit, (int)mine * kUnit, g, codes + place.unit, scales + place.scale);
+    }
   }
 }
 

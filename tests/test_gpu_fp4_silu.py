@@ -8,6 +8,39 @@ from tests.test_gpu_fp4_moe import _run
 
 pytestmark = pytest.mark.gpu
 
+def _held(x, g, group):
+    """(codes, scale codes) of the operator as numpy."""
+    from sglang_b200 import ops
+    q, s = ops.silu_and_mul_quant_fp4(x.cuda(), None if g is None else torch.tensor([g], device="cuda"), group)
+    rows, d = x.shape[0], x.shape[1] // 2
+    return q.cpu().numpy(), F.unblocked(s.view(torch.uint8).cpu().numpy(), rows, d // group)
+
+
+@pytest.mark.parametrize("group,g", [(16, None), (16, 2.0**20), (32, None)])
+def test_gates_below_minus_87(group, g):
+    """e^-gate leaves float32 from 88.7 on, its reciprocal from 87.3; times a large `up` the product is an ordinary number."""
+    gates = np.array([-86.5, -87.0, -87.5, -88.0, -88.5, -89.0, -90.0, -92.0, -95.0, -100.0, -101.0, -103.0, -104.0, -110.0, -120.0, -150.0])
+    rows = []
+    for top in (1e38, 3e36, 1e30):
+        for first in (0, 3, 8):
+            gate = np.resize(gates[first:], 64)
+            up = np.where(np.arange(64) % 3 == 1, -1.0, 1.0) * top * (1 + np.arange(64) % 7 / 8)
+            rows.append(np.concatenate([gate, up]))
+    rows.append(np.concatenate([np.full(64, -88.0), np.full(64, 1e38)]))
+    x = torch.from_numpy(np.stack(rows)).to(torch.bfloat16)
+    codes, scales = _held(x, g, group)
+    want = F.silu_and_mul(x.double().numpy())
+    assert np.abs(want[-1]).min() > 40  # (an ordinary number)
+    # float32: an activation and a product good to 2^-21, which can move a value over a border that it is next to
+    gg, eps = 1.0 if g is None else np.float32(g), 2.0**-21
+    lo, hi = F.group_scales(want * (1 - eps), gg, group)[0], F.group_scales(want * (1 + eps), gg, group)[0]
+    assert ((lo <= scales) & (scales <= hi)).all()
+    sv = F.scale_values(scales, group)
+    got = F.unpack(codes)
+    lo, hi = (F.value_codes(want * f, sv, gg, group) % 8 for f in (1 - eps, 1 + eps))
+    assert ((lo <= got % 8) & (got % 8 <= hi)).all()
+    assert (got[-1] % 8 > 0).all()
+
 
 @pytest.mark.parametrize("gate", [-86, -88, -96, -100])
 def test_experts_gates_below_minus_87(gate):

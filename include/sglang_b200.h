@@ -111,7 +111,8 @@ int sglb200_silu_and_mul_masked_quant_fp8(const void* input, int dtype, void* ou
  */
 int sglb200_per_token_group_quant_fp4(const void* input, int in_dtype, void* output_q, void* output_s, const float* global_scale,
                                       int64_t num_tokens, int64_t hidden, int group_size, void* stream);
-/* h = silu(x[:, :d]) * x[:, d:], unrounded in float32, quantised as above; input [rows, 2d] (bf16, fp16). */
+/* h = silu(x[:, :d]) * x[:, d:], unrounded (codes and scales are those of the exact h), quantised as above; a group with an h beyond
+ * float32's range counts as one that holds an infinity; input [rows, 2d] (bf16, fp16). */
 int sglb200_silu_and_mul_quant_fp4(const void* input, int dtype, void* output_q, void* output_s, const float* global_scale,
                                    int64_t rows, int64_t d, int group_size, void* stream);
 /* output [num_tokens, hidden] (bf16, fp16, fp32) = code * s / g. */

@@ -137,15 +137,22 @@ __device__ __forceinline__ float pick(const float (&x)[8], uint32_t i) {
   return b2 ? f : e;
 }
 
+// Codes of eight values x under a factor a little too small and one a little too large; `differ`: where the two are not the same.
+__device__ __forceinline__ uint32_t codes_between(const float (&x)[8], float r_lo, float r_hi, uint32_t& differ) {
+  float a[8], b[8];
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) mul2(a[i], a[i + 1], x[i], x[i + 1], r_lo), mul2(b[i], b[i + 1], x[i], x[i + 1], r_hi);
+  const uint32_t lo = cvt_e2m1x8(a);
+  differ = lo ^ cvt_e2m1x8(b);
+  return lo;
+}
+
 // Codes of eight values x under scale s (not 0) and the tensor's scale g: e2m1 nearest to x * g / s, decided likewise.
 // `r_lo`, `r_hi`: g / s a little too small and too large.  Where the two codes of a value differ the exact product decides, one value
 // after the other: g of few bits, or quotients of such as calibration gives, puts some value of a warp next to a border more often
 // than not, though seldom two of a thread (all eight unrolled: 8192 x 18432 in 117 us).
 __device__ __forceinline__ uint32_t codes_x8(const float (&x)[8], float r_lo, float r_hi, float s, float g) {
-  float a[8], b[8];
-#pragma unroll
-  for (int i = 0; i < 8; i += 2) mul2(a[i], a[i + 1], x[i], x[i + 1], r_lo), mul2(b[i], b[i + 1], x[i], x[i + 1], r_hi);
-  uint32_t lo = cvt_e2m1x8(a), differ = lo ^ cvt_e2m1x8(b);
+  uint32_t differ, lo = codes_between(x, r_lo, r_hi, differ);
   while (differ != 0) {
     const uint32_t at = (__ffs(differ) - 1) & ~3u, c = lo >> at & 7;
     const float over = fmaf(fabsf(pick(x, at >> 2)), g, -e2m1_border(c) * s);

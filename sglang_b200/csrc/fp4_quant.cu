@@ -4,7 +4,8 @@
 //   groups of 32:  s = 2^(floor(log2 amax) - 2),  code = e2m1(x / s),  value = code * s
 //
 // Every rounding is to nearest with ties to even and decided on exact numbers; a group whose scale is zero has zero codes, and one
-// that holds a NaN or an infinity has the scale NaN, so that no product hides it.
+// that holds a NaN or an infinity has the scale NaN, so that no product hides it.  silu(gate) * up is taken in float32, and once more in
+// float64 where a rounding of it could matter.
 //
 // All of them are bound by HBM: 2 bytes an element in and 0.5625 out (bf16, groups of 16).  A thread takes 16 columns of a row, so a
 // group of 16 needs no exchange and one of 32 a shuffle with the neighbour.  A warp takes the 64 columns of a scale block in the
@@ -93,8 +94,8 @@ struct Place {
   bool row_live, live;                               // whether there is such a row, and such columns in it
   Place() = default;
   // `rows`: of this launch.
-  __device__ __forceinline__ Place(uint32_t task, const FastDiv& blocks, uint32_t units, int rows) {
-    const uint32_t lane = threadIdx.x & 31, u = lane % kUnits, r = lane / kUnits;
+  __device__ __forceinline__ Place(uint32_t task, const FastDiv& blocks, uint32_t units, int rows, uint32_t lane = threadIdx.x & 31) {
+    const uint32_t u = lane % kUnits, r = lane / kUnits;
     const uint32_t set = blocks.quot(task), block = task - set * blocks.d;  // set: (block of rows, rows of it)
     const uint32_t low = set % kTasks * (kRows / 4) + r / 4, quarter = r % 4, row = set / kTasks * 128 + quarter * 32 + low;
     column = block * kUnits + u;
@@ -105,8 +106,11 @@ struct Place {
 };
 
 // Quantises this thread's 16 values; the code of the scale.  The lanes of a warp whose group takes two of them go together.
-template <int kGroup>
-__device__ __forceinline__ uint32_t quantize16(const float (&v)[16], float g, uint2& out) {
+// kInexact: the values are rounded, off by at most 2^-21, and a rounded number cannot tell on which side of a border that it is next to
+// the exact one lies.  `near`: the scale or a code is so near, and whoever has the exact values has to decide.
+template <int kGroup, bool kInexact>
+__device__ __forceinline__ uint32_t quantize16(const float (&v)[16], float g, uint2& out, bool& near) {
+  constexpr float kLess = 1.0f - 0x1p-19f, kMore = 1.0f + 0x1p-19f;  // (where kInexact: what the values, g and its quotient are off by, twice)
   float amax = max_nan(fabsf(v[0]), fabsf(v[1]));
 #pragma unroll
   for (int i = 2; i < 16; i += 2) amax = max3_nan(amax, fabsf(v[i]), fabsf(v[i + 1]));
@@ -120,7 +124,13 @@ __device__ __forceinline__ uint32_t quantize16(const float (&v)[16], float g, ui
     const int e = max((int)(__float_as_uint(amax) >> 23) - 2, 0);
     code = fine ? (uint32_t)e : kNanE8m0;
     const float r = __uint_as_float((uint32_t)(254 - e) << 23);
-    if (fine) {
+    if constexpr (kInexact) {
+      if (fine) {
+        uint32_t differ[2];
+        out.x = codes_between(x0, r * kLess, r * kMore, differ[0]), out.y = codes_between(x1, r * kLess, r * kMore, differ[1]);
+        near = (__float_as_uint(amax * kLess) ^ __float_as_uint(amax * kMore)) >> 23 != 0 || (differ[0] | differ[1]) != 0;
+      }
+    } else if (fine) {
       float a[8], b[8];
 #pragma unroll
       for (int i = 0; i < 8; i += 2) mul2(a[i], a[i + 1], x0[i], x0[i + 1], r), mul2(b[i], b[i + 1], x1[i], x1[i + 1], r);
@@ -128,6 +138,19 @@ __device__ __forceinline__ uint32_t quantize16(const float (&v)[16], float g, ui
     }
   } else {
     const bool fine = amax < __int_as_float(0x7f800000);
+    if constexpr (kInexact) {
+      const float scaled = amax * g * 0.16666667f;
+      const uint32_t two = cvt_e4m3x2(scaled * kLess, scaled * kMore);
+      code = fine ? two & 0xff : kNanE4m3;
+      near = fine && (two & 0xff) != two >> 8;
+      if (fine && code != 0) {
+        const float r = g * __frcp_rn(f16x2_to_f32(cvt_f16x2_e4m3x2(code)).x);
+        uint32_t differ[2];
+        out.x = codes_between(x0, r * kLess, r * kMore, differ[0]), out.y = codes_between(x1, r * kLess, r * kMore, differ[1]);
+        near = near || (differ[0] | differ[1]) != 0;
+      }
+      return code;
+    }
     code = fine ? group_scale_e4m3(amax, g) : kNanE4m3;
     if (fine && code != 0) {
       const float s = f16x2_to_f32(cvt_f16x2_e4m3x2(code)).x;
@@ -138,47 +161,46 @@ __device__ __forceinline__ uint32_t quantize16(const float (&v)[16], float g, ui
   return code;
 }
 
-// Quantises 16 columns of silu(gate) * up, of a group of kGroup from `gate` on, once more in float64: rows whose values float32 does not do
-// for, few enough that neither this function's time nor its reading one value at a time shows.  `mine`: the 16 of the group.
+// Quantises a group of silu(gate) * up once more in float64, where float32 does not do: next to a border (a few in 10^5 groups) and
+// below kSiluTail.  A warp, one value a lane (by one thread, a value after the other, it took 10 us).  `gate`, `up`: the group's first values;
+// `codes`: where its codes go.
 template <typename T, int kGroup>
-__device__ __noinline__ void quantize_silu_f64(const T* gate, const T* up, int mine, float g, uint2* codes, uint8_t* scale) {
-  double h[kGroup], amax = 0.0;
-  bool fine = true;
-#pragma unroll 1
-  for (int i = 0; i < kGroup; ++i) {
-    const double x = (double)ElemTraits<T>::to_f32(gate[i]);
-    h[i] = x / (1.0 + exp(-x)) * (double)ElemTraits<T>::to_f32(up[i]);
-    fine = fine && fabsf((float)h[i]) < __int_as_float(0x7f800000);
-    amax = fmax(amax, fabs(h[i]));
-  }
+__device__ __noinline__ void quantize_silu_f64(const T* gate, const T* up, float g, uint32_t* codes, uint8_t* scale) {
+  const int lane = threadIdx.x & 31, i = lane % kGroup;
+  const double x = (double)ElemTraits<T>::to_f32(gate[i]), h = x / (1.0 + exp(-x)) * (double)ElemTraits<T>::to_f32(up[i]);
+  const bool fine = __all_sync(0xffffffffu, fabsf((float)h) < __int_as_float(0x7f800000));
+  double amax = fabs(h);
+#pragma unroll
+  for (int o = kGroup / 2; o > 0; o >>= 1) amax = fmax(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   constexpr float kLess = 1.0f - 0x1p-20f, kMore = 1.0f + 0x1p-20f;
+  const double factor = kGroup == 32 ? 1.0 : (double)g;
   uint32_t code;
-  double s;  // of the values times g
+  double s;
   if constexpr (kGroup == 32) {
     const int e = amax > 0.0 ? max(ilogb(amax) - 2, -127) : -127;
     code = (uint32_t)(e + 127), s = ldexp(1.0, e);
   } else {
-    const float v = (float)(amax * (double)g / 6.0);
+    const float v = (float)(amax * factor / 6.0);
     const uint32_t two = cvt_e4m3x2(v * kLess, v * kMore);
     const float2 f = f16x2_to_f32(cvt_f16x2_e4m3x2(two));
-    const double border = 3.0 * ((double)f.x + (double)f.y), num = amax * (double)g;
+    const double border = 3.0 * ((double)f.x + (double)f.y), num = amax * factor;
     const bool higher = (two & 0xff) != two >> 8 && (num > border || (num == border && (two & 1)));
     code = higher ? two >> 8 : two & 0xff, s = higher ? f.y : f.x;
   }
   if (!fine) code = kGroup == 32 ? kNanE8m0 : kNanE4m3;
-  uint32_t word[2] = {0u, 0u};
+  uint32_t word = 0;
   if (fine && s > 0.0) {
-#pragma unroll 1
-    for (int i = 0; i < 16; ++i) {
-      const double num = fabs(h[mine + i]) * (kGroup == 32 ? 1.0 : (double)g);
-      const float q = (float)fmin(num / s, 8.0);
-      uint32_t two = cvt_e2m1x2(q * kLess, q * kMore), c = two & 15;
-      if (c != two >> 4 && (num > (double)e2m1_border(c) * s || (num == (double)e2m1_border(c) * s && (c & 1)))) ++c;
-      word[i >> 3] |= (c | (signbit(h[mine + i]) ? 8u : 0u)) << 4 * (i & 7);
-    }
+    const double num = fabs(h) * factor;
+    const float q = (float)fmin(num / s, 8.0);
+    const uint32_t two = cvt_e2m1x2(q * kLess, q * kMore), c = two & 15;
+    const double border = (double)e2m1_border(c) * s;
+    const bool higher = c != two >> 4 && (num > border || (num == border && (c & 1)));
+    word = (c + (higher ? 1u : 0u) | (signbit(h) ? 8u : 0u)) << 4 * (i & 7);
   }
-  *codes = make_uint2(word[0], word[1]);
-  if (mine == 0) *scale = (uint8_t)code;
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
+  if (lane < kGroup && lane % 8 == 0) codes[lane / 8] = word;
+  if (lane == 0) *scale = (uint8_t)code;
 }
 
 // A warp takes kAhead tasks, whose values are all asked for before the first is quantised.
@@ -225,20 +247,25 @@ __global__ void __launch_bounds__(kThreads)
       }
     }
     uint2 c;
-    const uint32_t code = quantize16<kGroup>(v, g, c);
+    bool near = false;
+    const uint32_t code = quantize16<kGroup, kSilu>(v, g, c, near);
+    if (near) again |= 1u << k;
     if (at[k].live) codes[at[k].unit] = c;
     if (at[k].row_live && at[k].column % (kGroup / kUnit) == 0) scales[at[k].scale] = at[k].live ? (uint8_t)code : 0;  // (zeros for groups past the last)
   }
   if constexpr (kSilu) {
-    if constexpr (kGroup == 32) again |= __shfl_xor_sync(0xffffffffu, again, 1);  // (both halves of a group)
-    if (again == 0) return;
+    if (__ballot_sync(0xffffffffu, again != 0) == 0) return;
+    __syncwarp();  // (what one lane has stored another may store again)
 #pragma unroll 1
     for (int k = 0; k < kAhead; ++k) {
-      const Place<kGroup> place(min(task0 + k * (kThreads / 32), tasks - 1), blocks, units, rows);
-      if ((again >> k & 1) == 0 || !place.live) continue;
-      const uint32_t mine = place.column % (kGroup / kUnit);
-      const T* gate = x + (2 * place.unit - place.column - mine) * kUnit;  // the group's first: rows of twice the columns
-      quantize_silu_f64<T, kGroup>(gate, gate + (int64_t)units * kUnit, (int)mine * kUnit, g, codes + place.unit, scales + place.scale);
+      uint32_t left = __ballot_sync(0xffffffffu, again >> k & 1);
+      if constexpr (kGroup == 32) left = (left | left >> 1) & 0x55555555u;  // (a group's first lane)
+      for (; left != 0; left &= left - 1) {
+        const Place<kGroup> place(min(task0 + k * (kThreads / 32), tasks - 1), blocks, units, rows, __ffs(left) - 1);
+        if (!place.live) continue;
+        const T* gate = x + (2 * place.unit - place.column) * kUnit;  // (rows of twice the columns)
+        quantize_silu_f64<T, kGroup>(gate, gate + (int64_t)units * kUnit, g, reinterpret_cast<uint32_t*>(codes + place.unit), scales + place.scale);
+      }
     }
   }
 }

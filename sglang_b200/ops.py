@@ -168,7 +168,7 @@ def per_token_group_quant_fp4(
 def silu_and_mul_quant_fp4(
     x: torch.Tensor, global_scale: Optional[torch.Tensor] = None, group_size: int = 16,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """silu(x[..., :d]) * x[..., d:], unrounded in float32, quantised as `per_token_group_quant_fp4` does; x [..., 2d]."""
+    """silu(x[..., :d]) * x[..., d:], unrounded, quantised as `per_token_group_quant_fp4` does; x [..., 2d]."""
     out = host.silu_mul_quant_fp4(x, global_scale, group_size)
     return out if out is not None else _quant_fp4(x, global_scale, group_size, True, "silu_and_mul_quant_fp4")
 

@@ -8,6 +8,7 @@ from tests.test_gpu_fp4_moe import _run
 
 pytestmark = pytest.mark.gpu
 
+
 def _held(x, g, group):
     """(codes, scale codes) of the operator as numpy."""
     from sglang_b200 import ops
@@ -61,3 +62,64 @@ def test_experts_gates_below_minus_87(gate):
     assert 1e-36 < abs(want)
     # x[18] has 8 bits and is 2^-15 of its row's largest, so it and the gate are exact; the activation is good to 2^-20
     assert (np.abs(got - want) <= (2.0**-8 + 2.0**-19) * abs(want)).all(), (got[0, :3], want)
+
+
+def _near(targets, dtype, within):
+    """(gate, up) of `dtype` whose silu(gate) * up lies within that share of a target's magnitude, though never on it."""
+    gate = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16).view(dtype).double()
+    gate = gate[torch.isfinite(gate) & (gate.abs() < 80) & (gate.abs() > 2.0**-10)].numpy()
+    s = gate / (1 + np.exp(-gate))
+    found = []
+    for t in targets:
+        up = torch.from_numpy(t / s).to(dtype).double().numpy()
+        off = np.abs(s * up / t - 1)
+        for i in np.nonzero((off < within) & (off > 2.0**-44) & (np.abs(up) > 2.0**-10))[0]:
+            found.append((gate[i], up[i]))
+    return found
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("group,g", [(16, None), (16, 6.72), (32, None)])
+def test_values_next_to_borders(dtype, group, g):
+    """Codes and scales are those of the unrounded product, also where it lies nearer to a border than float32 resolves."""
+    gg = 1.0 if g is None else float(np.float32(g))
+    rows = []
+    scales = [1.0, 1.125, 1.25, 1.375, 1.5, 1.625, 1.75, 1.875] if group == 16 else [1.0]
+    borders = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    for s in scales:  # a group whose largest value has this scale, and one next to a border of codes
+        for gate, up in _near(borders * s / gg, dtype, 2.0**-22):
+            row = np.zeros(2 * group)
+            row[0], row[group] = 24.0, 6 * s / gg / 24
+            row[5], row[group + 5] = gate, up
+            rows.append(row)
+    if group == 16:  # the largest value next to a border of scales
+        targets = 6 * (F.E4M3[40:90] + F.E4M3[41:91]) / 2 / gg
+    else:
+        targets = 2.0 ** np.arange(-20, 12)
+    for gate, up in _near(targets, dtype, 2.0**-22):
+        row = np.zeros(2 * group)
+        row[9], row[group + 9] = gate, up
+        row[2::3], row[group + 2 :: 3] = 1.0, row[group + 2 :: 3] + 2.0**-6
+        rows.append(row)
+    x = torch.from_numpy(np.stack(rows)).to(dtype)
+    codes, scode = _held(x, g, group)
+    want_codes, want_scode = F.quantize(F.silu_and_mul(x.double().numpy()), gg, group)
+    wrong = (codes != want_codes).any(1) | (scode != want_scode).any(1)
+    print(f"{len(rows)} rows, {wrong.sum()} wrong")
+    assert not wrong.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("group,g", [(16, None), (16, 6.72), (32, None)])
+@pytest.mark.parametrize("rows,d", [(1, 64), (130, 352), (2600, 2112)])
+def test_bit_for_bit(dtype, group, g, rows, d):
+    """Ordinary rows, among them gates whose silu is the gate itself, so that products are short numbers and lie on borders."""
+    gen = torch.Generator().manual_seed(rows + d)
+    x = torch.randn(rows, 2 * d, generator=gen)
+    x = torch.where(torch.rand(x.shape, generator=gen) < 0.02, x * 40, x)
+    x[0] = torch.randint(-60, 60, (2 * d,), generator=gen).float() / 2
+    x = x.to(dtype)
+    codes, scode = _held(x, g, group)
+    h = F.silu_and_mul(x.double().numpy())
+    want_codes, want_scode = F.quantize(h, 1.0 if g is None else float(np.float32(g)), group)
+    assert np.array_equal(scode, want_scode) and np.array_equal(codes, want_codes)

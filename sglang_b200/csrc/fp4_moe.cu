@@ -701,7 +701,12 @@ __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
       const auto finish = [&](int tile, int r, float lo, float hi) {
         if (tile >= tiles || r >= n) return;
         const float f = ctl->factor[r], unscale = pow2(-row_shift<T>(ctl->amax[(stagings - 1) & 1][r]));
-        lo = lo * f * unscale, hi = hi * f * unscale;
+        // The factor and the row's power of two together, which is exact, so that neither of them by itself takes a sum out of range; where
+        // together they leave it, one after the other does not.
+        const float both = f * unscale;
+        const bool fits = fabsf(both) >= 0x1p-126f && fabsf(both) < __int_as_float(0x7f800000);
+        const float a = fits ? both : f, b = fits ? 1.f : unscale;
+        lo = lo * a * b, hi = hi * a * b;
         const int slot = ctl->slot[first + r];
         if constexpr (kUp) {
           p.h[(int64_t)slot * (p.rows / 2) + tile * 8 + g] = silu_mul(lo, hi);

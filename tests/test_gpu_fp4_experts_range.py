@@ -28,3 +28,30 @@ def test_large_and_small_factors(a13, a2, xs):
     tol = e1 * first + e2 * second + 2.0**-8 * 1.001 * np.abs(out)
     assert 1e-30 < np.abs(out).max() < 1e37
     assert (np.abs(got.double().cpu().numpy() - out) <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rows_of_all_magnitudes(dtype):
+    """Rows that are staged under another power of two than the usual one, as x and as h, each with an expert of its own whose factor brings the
+    output back to ordinary numbers; 2^6 would flush the small ones to zero and take the large ones to infinity."""
+    powers = [-60, -45, -30, -20, -12, -7, -3, 0, 4, 7, 9, 12, 16, 30, 45, 58] if dtype == torch.bfloat16 else [-9, -7, -5, -3, 0, 2, 4, 6, 8, 10]
+    n = len(powers)
+    x, w13, w2, weights, _ = _layer(n, n, 1, 512, 288, dtype, 22)
+    x = (x.double() * 2.0 ** torch.tensor(powers, dtype=torch.float64)[:, None]).to(dtype)
+    # silu(v) is v / 2 for small v: h goes as the square either way
+    w13 = w13[:2] + (np.full(n, 1e-2, dtype=np.float32),) + w13[3:]
+    w2 = w2[:2] + ((2.0 ** (-2.0 * np.array(powers)) * 1e-2).astype(np.float32),) + w2[3:]
+    ids = torch.arange(n, dtype=torch.int32)[:, None]
+    with np.errstate(over="ignore"):
+        out, first, second = _want(x, w13, w2, weights, ids)
+    got = _run(x, w13, w2, weights, ids).double().cpu().numpy()
+    # as above; fp16 outputs may be subnormal: half of their step
+    e1, e2 = (512 / 16 + 12) * 2.0**-23 + 2.0**-20, 2.0**-20 + (288 / 16 + 20) * 2.0**-23
+    tol = e1 * first + e2 * second + torch.finfo(dtype).eps / 2 * 1.001 * np.abs(out)
+    if dtype == torch.float16:
+        tol += 2.0**-25
+    err = np.abs(got - out)
+    assert (np.abs(out).max(1) > 1e-3).all() and (np.abs(out).max(1) < 6e4).all()
+    for row, p in enumerate(powers):
+        assert (err[row] <= tol[row]).all(), (p, (err[row] / tol[row]).max())
+        assert (err[row] ** 2).mean() <= (torch.finfo(dtype).eps / 2) ** 2 * (out[row] ** 2).mean(), p

@@ -71,3 +71,31 @@ def test_dequant(dtype, group, g, columns):
     # s / g and code * (s / g) in float32: each off by at most 2^-24 of the value; then one rounding to the output's type
     tol = (2 * 2.0**-24 + (torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0)) * np.abs(want) + torch.finfo(dtype).tiny * torch.finfo(dtype).eps
     assert (np.abs(got - want) <= tol).all()
+
+
+def test_more_rows_than_a_launch_takes():
+    """A launch takes 2^30 bytes of scales, 2^28 rows of one group: five more are a launch of their own.  Rows repeat, so that every part has
+    to give what the first one gives."""
+    from sglang_b200 import ops
+    base, times, more = 1 << 20, 1 << 8, 5
+    for silu in (False, True):
+        x = _x(base, 32 if silu else 16, torch.bfloat16, 4).cuda()
+        quantizer = ops.silu_and_mul_quant_fp4 if silu else ops.per_token_group_quant_fp4
+        q, s = quantizer(x)
+        want_q, want_s = q.clone(), s.view(torch.uint8).clone()
+        big = torch.cat([x.repeat(times, 1), x[:more]])
+        q, s = quantizer(big)
+        del big
+        s = s.view(torch.uint8)
+        for part in range(times):
+            assert torch.equal(q[part * base : (part + 1) * base], want_q)
+            assert torch.equal(s[part * base : (part + 1) * base], want_s)
+        assert torch.equal(q[times * base :], want_q[:more])
+        assert np.array_equal(F.unblocked(s[times * base :].cpu().numpy(), more, 4), F.unblocked(want_s[:128].cpu().numpy(), more, 4))
+        back = ops.per_token_group_dequant_fp4(q, s.view(torch.float8_e4m3fn))
+        want = ops.per_token_group_dequant_fp4(want_q, want_s.view(torch.float8_e4m3fn))
+        for part in range(times):
+            assert torch.equal(back[part * base : (part + 1) * base], want)
+        assert torch.equal(back[times * base :], want[:more])
+        del q, s, back
+        torch.cuda.empty_cache()

@@ -8,6 +8,7 @@
 #include <algorithm>
 
 #include "fp4_gemm.cuh"
+#include "fp4_rules.h"
 
 namespace sglb200 {
 namespace fp4 {
@@ -253,21 +254,6 @@ static int launch_rows(const void* A, const void* B, Params& p, cudaStream_t st)
   return SGLB200_OK;
 }
 
-// Columns of a pair's tile: as many waves of them as there are, times the time of a wave in hundredths of a microsecond (0.46 a slab
-// for 256 columns, 0.39 for 192, 0.33 for 128, and half a microsecond).  us over 256, 192 and 128: 4096 x 36864 x 7168 387, 433, 570;
-// 257 x 10240 x 8192 29.0, 27.6, 35.9; 1024 x 10240 x 8192 42, 40, 57; 1024 x 2112 x 7168 15.3, 15.3, 14.7; 257 x 36864 x 7168 56, 65, 78.
-static int pair_columns(const Params& p) {
-  const int64_t pairs = std::max<int64_t>(1, cluster_fits().alone[2]), tiles_m = (p.M + 255) / 256;
-  int best = 256;
-  int64_t best_cost = -1;
-  for (int bn = 256; bn >= 128; bn -= 64) {
-    const int64_t waves = (tiles_m * ((p.N + bn - 1) / bn) + pairs - 1) / pairs;
-    const int64_t cost = waves * (p.kb_total * (bn == 256 ? 46 : bn == 192 ? 39 : 33) + 50);
-    if (best_cost < 0 || cost < best_cost) best = bn, best_cost = cost;
-  }
-  return best;
-}
-
 // Up to 64 rows the weights on the M side.  Above that likewise, 64 rows a tile, where that makes no more tiles than SMs (their K is
 // then split over clusters: 128 x 512 x 8192 6.6 us, by pairs 14.2; 512 x 2112 x 7168 13.5 and 14.3; but 65 x 10240 x 8192, 160 tiles,
 // 22.6 and 17.0), and 128 rows a tile up to 128 rows (65 x 36864 x 7168 31.5 and 32.9; 128 rows 34.0 and 34.7); else pairs.
@@ -277,7 +263,7 @@ static int scaled_mm(const void* A, const void* B, Params& p, cudaStream_t st) {
   if (p.M <= 32) return launch_rows<RowsCfg<32, G>>(A, B, p, st);
   if (p.M <= 64 || (p.M + 63) / 64 * ((p.N + 127) / 128) <= sm_count()) return launch_rows<RowsCfg<64, G>>(A, B, p, st);
   if (p.M <= 128) return launch_rows<RowsCfg<128, G>>(A, B, p, st);
-  return pair_mm(A, B, p, G, pair_columns(p), st);
+  return pair_mm(A, B, p, G, pair_columns(p.M, p.N, p.kb_total, std::max<int64_t>(1, cluster_fits().alone[2])), st);
 }
 
 }  // namespace fp4

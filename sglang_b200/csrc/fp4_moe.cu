@@ -29,23 +29,22 @@
 // token through eighths of experts (25 MB) 21.  Not kept: weights straight into registers (16 warps, three steps deep: 570 us), two
 // tiles a warp (620; the ring is then two stages deep), two CTAs of eight warps an SM (520), a warp of its own that counts items (500).
 #include <algorithm>
-#include <cmath>
 #include <type_traits>
 
 #include "fp4_math.cuh"
+#include "fp4_rules.h"
 #include "gemm_common.cuh"
 #include "ptx_sm100.cuh"
 
 namespace sglb200 {
 namespace fp4 {
 
-constexpr int kMoeWarps = 16, kMoeConsumers = kMoeWarps * 32;  // warps that multiply
+constexpr int kMoeConsumers = kMoeWarps * 32;  // threads that multiply
 constexpr int kScaleWarps = 3;                // that fetch scales where K is not whole steps
 // One more warp fetches codes, and scales where K is whole steps.
 template <bool kWhole>
 constexpr int kMoeThreads = kMoeConsumers + 32 + (kWhole ? 0 : kScaleWarps * 32);
 constexpr int kMoeMaxExperts = 1024, kMoeMaxSlots = 1024;
-constexpr int kStep = 256;                    // columns per step: a lane takes 64 of a row, 32 bytes of codes and four scales
 constexpr int kMoeRows = 32;                  // activation rows per pass, at most: four times the eight columns of an instruction
 // Columns of an instruction that an activation row takes: a float32 row has two, its terms.
 template <typename T>
@@ -58,7 +57,6 @@ template <bool kWhole>
 constexpr uint32_t kScalePitch = kWhole ? 16 : 20;
 template <bool kWhole>
 constexpr uint32_t kStageBytes = kCodeBytes + kMoeWarps * 16 * kScalePitch<kWhole>;
-constexpr int kMoeMaxStages = 6;
 constexpr int kUsualShift = 6;                // rows whose largest magnitude lies in [2^-5, 2^9) are staged under 2^6
 
 __device__ int g_fp4_moe_status = 0;  // 0 ok, 1 = a wait for weights expired
@@ -96,6 +94,8 @@ struct MoeCtl {
   float factor[kMoeRows];           // of the staged rows: alpha (times the routing weight)
   int num_live, complete[2], abort_flag;  // num_live: passes
 };
+
+static_assert(sizeof(MoeCtl) == kMoeCtlBytes && kStageBytes<false> == kMoeStageBytes);
 
 __device__ __forceinline__ int ld_fresh(const int32_t* at) {  // (past the first-level cache)
   int v;
@@ -768,59 +768,12 @@ __global__ void __launch_bounds__(kMoeThreads<kWhole>, 1)
   }
 }
 
-constexpr int64_t moe_smem(int steps, int cols, int stages) {  // (the larger stages: where K is whole steps a little is left over)
-  return 1024 + (int64_t)stages * kStageBytes<false> + (int64_t)steps * 512 * cols + kMoeWarps * 512 * ((cols + 7) / 8) + (int64_t)sizeof(MoeCtl);
-}
-constexpr int64_t kMoeMostSmem = 227 * 1024;
-
-// Experts that `slots` picks name, taken as spread evenly.
-static double expected_live(const MoeParams& p) {
-  double none = 1.0;
-  for (int i = 0; i < p.slots; ++i) none *= 1.0 - 1.0 / p.experts;
-  return p.experts * (1.0 - none);
-}
-
-// Passes of those experts: one each, and one more for every further pass_rows rows (an expert's rows taken as normally distributed).
-static double expected_passes(const MoeParams& p, double live) {
-  const double mean = (double)p.slots / p.experts, sd = std::sqrt(mean * (1.0 - 1.0 / p.experts)) + 0.01;
-  double more = 0.0;
-  for (double rows = p.pass_rows + 0.5; rows < std::min(mean + 4.0 * sd, (double)p.slots); rows += p.pass_rows) {
-    more += 1.0 / (1.0 + std::exp(std::max(-30.0, 1.702 * (rows - mean) / sd)));
-  }
-  return live + p.experts * more;
-}
-
 static int plan_product(MoeParams& p, int64_t K, int64_t rows, bool up) {
-  p.K = K, p.rows = rows, p.steps = (int)((K + kStep - 1) / kStep);
-  // Rows per pass, and the columns that they take (two a row of h): every pass of an expert reads its weights again (from the L2, by other
-  // CTAs at the same time), and columns take the place of stages; eight columns cost the same with one row in them as with all.
-  // us of a layer over 8, 16 and 32 columns of x: 8 rows an expert (64 of 2048 x 1024) 98, 107, 114; 16 (32 of 7168 x 512) 160, 151, 163; 32
-  // (8 of 4096 x 1024) 116, 105, 103; the same of h 113, 101, 117; 184, 150, 146; 97, 94, 89.  Four instead of eight leave long rows more stages,
-  // which is worth 2 % where experts have a row or two (7168 x 512) and costs 14 % where they have four.
-  const int terms = up ? 1 : 2;
-  const double live = expected_live(p), cols_each = p.slots / live * terms;
-  p.cols = cols_each > 18 ? 32 : cols_each > 10 ? 16 : cols_each > 3 || moe_smem(p.steps, 8, 4) <= kMoeMostSmem ? 8 : 4;
-  while (p.cols > terms && (moe_smem(p.steps, p.cols, 2) > kMoeMostSmem || p.cols >= 2 * terms * p.slots)) p.cols /= 2;
-  if (moe_smem(p.steps, p.cols, 2) > kMoeMostSmem) p.cols = 1;
-  p.pass_rows = std::max(1, p.cols / terms);
-  const double passes = expected_passes(p, live);
-  // Warps that split K, the others taking tiles of their own: more of them make more and shorter items, which fill the GPU and its last
-  // round better, but each item has an end, of two barriers and the shared memory between where K is split and of a count where
-  // the slots are summed.  Times in turns of the ring: an end is 0.2 of one for the first product, 0.7 with a split K (the second: 0.5, 1.2);
-  // scales that come by asynchronous copies come slower in short runs.  us of a layer over 1, 2, 4 and 8 for the first product: one token,
-  // 8 experts of 7168 x 256 41, 31, 26, 24; 101 named of 7168 x 2048 451, 475, 475, 497; 11 of 4096 x 2048 62, 57, 54, 57; 24 of
-  // 7136 x 544 84, 78, 66, 67.  For the second: 106 of 7168 x 2048 580, 606, 642, 723.
-  double best = 0.0;
-  for (int k = 1; k <= kMoeWarps && k <= p.steps; k *= 2) {
-    const int per = kMoeWarps / k, sets = (int)((rows / 16 + per - 1) / per), turns = (p.steps + k - 1) / k;
-    const double rounds = passes * sets / sm_count(), slow = !up || K % kStep == 0 ? 1.0 : k == 1 ? 1.25 : k == 2 ? 1.08 : 1.0;
-    const double cost = (rounds <= 1.0 ? 1.0 : rounds + 0.5) * (turns * slow + (k == 1 ? 0.2 : 0.7) + (up ? 0.0 : k == 1 ? 0.3 : 0.5));
-    if (k == 1 || cost < best) best = cost, p.warps_k = k, p.sets = sets;
-  }
   SGLB_REQUIRE(rows * (K / 16) < (1ll << 31), "fused_experts_fp4: %lld x %lld weights are too many for an expert", (long long)rows, (long long)K);
-  p.stages = kMoeMaxStages;
-  while (p.stages > 2 && moe_smem(p.steps, p.cols, p.stages) > kMoeMostSmem) --p.stages;
-  SGLB_REQUIRE(moe_smem(p.steps, p.cols, p.stages) <= kMoeMostSmem, "fused_experts_fp4: %lld columns are too many", (long long)K);
+  const ExpertsPlan plan = plan_experts(p.slots, p.experts, K, rows, up, sm_count());
+  SGLB_REQUIRE(plan.stages > 0, "fused_experts_fp4: %lld columns are too many", (long long)K);
+  p.K = K, p.rows = rows, p.steps = plan.steps, p.cols = plan.cols, p.pass_rows = plan.pass_rows;
+  p.warps_k = plan.warps_k, p.sets = plan.sets, p.stages = plan.stages;
   return SGLB200_OK;
 }
 

@@ -65,7 +65,10 @@ def test_few_columns(T, E, topk, H, I, dtype):
     _check(_run(*args), _want(*args), H, I, dtype)
 
 
-@pytest.mark.parametrize("T,E,I", [(1, 1, 36096), (3, 2, 36000), (5, 1, 40992)])
+TWICE = [(1, 1, 36096), (3, 2, 36000), (5, 1, 40992)]
+
+
+@pytest.mark.parametrize("T,E,I", TWICE)
 def test_more_columns_than_fit_with_both_terms(T, E, I):
     """Second products whose rows fit shared memory with one term only: the weights are taken twice."""
     args = _layer(T, E, 1, 32, I, torch.bfloat16, I)

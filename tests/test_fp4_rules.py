@@ -1,4 +1,5 @@
-"""Which form of the 4-bit kernels a call takes (csrc/fp4_rules.h), compiled for the CPU."""
+"""Which form of the 4-bit kernels a call takes (csrc/fp4_rules.h), compiled for the CPU; the cases of test_gpu_fp4_forms.py reach all of
+them on a GPU of 148 SMs."""
 import ctypes
 import os
 import subprocess
@@ -90,3 +91,21 @@ def test_the_widths_of_pairs_tiles(rules):
     # figures of the rule's comment
     assert rules.columns(4096, 36864, 7168, PAIRS_OF_A_GPU) == 256 and rules.columns(1024, 10240, 8192, PAIRS_OF_A_GPU) == 192
     assert rules.columns(1024, 2112, 7168, PAIRS_OF_A_GPU) == 128
+
+
+def test_the_gpu_tests_reach_every_form(rules):
+    from tests.test_gpu_fp4_experts_terms import TWICE
+    from tests.test_gpu_fp4_forms import EXPERTS, PAIRS
+    from tests.test_gpu_fp4_moe import CASES
+    reached = {f for c in CASES + EXPERTS for f in forms(rules, *c)} | {f for T, E, I in TWICE for f in forms(rules, T, E, 1, 32, I)}
+    for whole in (False, True):
+        for split in (False, True):
+            for eights in (1, 2, 4):
+                assert ("up", whole, eights, split) in reached
+                assert ("down", whole, eights, split) in reached
+        assert any(f[:3] == ("down", whole, "twice") for f in reached)
+    for m, n, k, columns in PAIRS:
+        assert rules.columns(m, n, k, PAIRS_OF_A_GPU) == columns
+        assert -(-m // 64) * -(-n // 128) > SMS  # (pairs, not rows)
+        assert -(-m // 256) * -(-n // columns) > PAIRS_OF_A_GPU  # several tiles a pair
+    assert {c for *_, c in PAIRS} == {128, 192, 256}

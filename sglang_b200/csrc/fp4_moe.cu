@@ -448,11 +448,17 @@ __device__ __noinline__ void sum_slots(const MoeParams& p, int col0, int cols) {
   }
 }
 
-// acc += weights of a step times the staged rows, 8 NT of them (`b`: this lane's pieces, `stride` apart).  181 instructions with the loads from
-// shared memory, 64 of them conversions and 64 scalings, for 16 x 256 weights: an SM that does nothing else takes 8.2 TB/s of weights so
-// (two tiles a warp, which share the pieces of x: 9.3, but half as many stages fit).
+// acc += weights of a step times the staged rows, 8 NT of them (`b`: this lane's pieces, `stride` apart).  185 instructions with the loads from
+// shared memory, 64 of them conversions and 64 scalings, for 16 x 256 weights: an SM that does nothing else takes 8 TB/s of weights so
+// (two tiles a warp, which share the pieces of x: 9, but half as many stages fit).
+// A step's sums start from zero and are added in float32: the instructions cut off what does not fit their sum, and carried over all of 28
+// steps that moved one bf16 output in 350 by a step (16 tokens, 8 of 256 of 7168 x 2048); now one in 4400, as float32 sums do.  It costs nothing
+// with 8 columns, 1 to 2 % with 16 and 3 to 5 % with 32.
 template <int NT>
 __device__ __forceinline__ void multiply(float (&acc)[NT][4], const uint4 (&code)[2][2], const uint32_t (&scale)[2], const uint4* b, int stride) {
+  float sum[NT][4];
+#pragma unroll
+  for (int q = 0; q < NT; ++q) sum[q][0] = sum[q][1] = sum[q][2] = sum[q][3] = 0.f;
   uint32_t s2[2][2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) s2[u][0] = cvt_f16x2_e4m3x2(scale[u]), s2[u][1] = cvt_f16x2_e4m3x2(scale[u] >> 16);
@@ -470,10 +476,14 @@ __device__ __forceinline__ void multiply(float (&acc)[NT][4], const uint4 (&code
 #pragma unroll
     for (int q = 0; q < NT; ++q) {
       const uint4 x = b[jj * stride + q * 32];
-      mma_f16(acc[q], a[0][0], a[1][0], a[0][1], a[1][1], x.x, x.y);
-      mma_f16(acc[q], a[0][2], a[1][2], a[0][3], a[1][3], x.z, x.w);
+      mma_f16(sum[q], a[0][0], a[1][0], a[0][1], a[1][1], x.x, x.y);
+      mma_f16(sum[q], a[0][2], a[1][2], a[0][3], a[1][3], x.z, x.w);
     }
   }
+#pragma unroll
+  for (int q = 0; q < NT; ++q)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[q][j] += sum[q][j];
 }
 
 // kWhole: K is a multiple of a step.  kUp: T is the activations' type and a tile is 8 gate and the 8 matching up rows; else T is float

@@ -79,3 +79,35 @@ def test_more_columns_than_fit_with_both_terms(T, E, I):
     got = _run(*args)
     assert torch.isnan(got[0]).all()
     _check(got[1:], tuple(w[1:] for w in want), 32, I, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,H,I", [(1024, 7168, 1024), (300, 7168, 1024), (1024, 3616, 1024)])
+def test_long_sums(T, H, I, dtype):
+    """First products whose up sums climb over half of K and come back to zero: a sum that the matrix instructions carried all the way,
+    which cut off what does not fit instead of rounding it, would be left with a share of its peak."""
+    from sglang_b200 import ops
+    half = H // 2
+    gen = torch.Generator().manual_seed(H + T)
+    x = torch.randint(128, 256, (T, half), generator=gen).float() / 128
+    x[:, 0] = 4
+    x = torch.cat([x, x], 1).to(dtype).cuda()
+    up = torch.randint(1, 8, (I, half), generator=gen)  # codes of 0.5 to 6, under scales of 2^-4 to 2
+    scales = torch.randint(0x18, 0x40, (I, half // 16), generator=gen)
+    c13 = torch.zeros(2 * I, H, dtype=torch.uint8)
+    c13[:I, 0] = 7  # gate: 6 * 4
+    c13[I:] = torch.cat([up, up + 8], 1).to(torch.uint8)
+    c2 = torch.zeros(H, I, dtype=torch.uint8)
+    c2[torch.arange(I), torch.arange(I)] = 2  # output n is h of n
+    one = lambda n, k: torch.full((1, n, k // 16), 0x38, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)  # noqa: E731
+    s13 = torch.cat([torch.full((I, H // 16), 0x38), torch.cat([scales, scales], 1)]).to(torch.uint8).cuda().view(torch.float8_e4m3fn)[None]
+    pack = lambda c: torch.from_numpy(F.pack(c.numpy())).cuda()[None]  # noqa: E731
+    got = ops.fused_experts_fp4(x, pack(c13), pack(c2), s13, one(H, I), torch.ones(T, 1, device="cuda"),
+                                torch.zeros(T, 1, dtype=torch.int32, device="cuda")).double()
+    peak = x[:, :half].double() @ torch.from_numpy(F.E2M1[up] * np.repeat(F.E4M3[scales], 16, 1)).cuda().t()
+    # A step of 256 columns is 16 instructions, each off by at most 2^-23 of the step's sum so far, which is at most 256 / half of the peak;
+    # then a float32 addition of 2^-24 of the sum for each step, and four between warps.  silu(24) is 24 to 2^-34.
+    steps = -(-H // 256)
+    tol = 24.01 * peak * 2.0**-23 * (steps * 16 * min(1.0, 256 / half) + steps / 2 + 4)
+    assert (got[:, I:] == 0).all()
+    assert (got[:, :I].abs() <= tol).all(), (got[:, :I].abs() / tol).max()

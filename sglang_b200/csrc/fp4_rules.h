@@ -70,9 +70,10 @@ inline ExpertsPlan plan_experts(int64_t slots, int64_t experts, int64_t K, int64
   p.steps = (int)((K + kStep - 1) / kStep);
   // Rows per pass, and the columns that they take (two a row of h): every pass of an expert reads its weights again (from the L2, by other
   // CTAs at the same time), and columns take the place of stages; eight columns cost the same with one row in them as with all.
-  // us of a layer over 8, 16 and 32 columns of x: 8 rows an expert (64 of 2048 x 1024) 98, 107, 114; 16 (32 of 7168 x 512) 160, 151, 163; 32
-  // (8 of 4096 x 1024) 116, 105, 103; the same of h 113, 101, 117; 184, 150, 146; 97, 94, 89.  Four instead of eight leave long rows more stages,
-  // which is worth 2 % where experts have a row or two (7168 x 512) and costs 14 % where they have four.
+  // us of a layer over 8, 16 and 32 columns of x: 2 rows an expert (128 of 2048 x 768) 92, 102, 102; 4 (64 of 2048 x 1024) 85, 94, 93; 12 (32 of
+  // 1376 x 1440) 107, 106, 120; 16 (16 of 2080 x 1056) 95, 90, 90; 64 (4 of 2048 x 2048) 84, 79, 80.  Of h: 4 rows 85, 94, 105; 8 (64 of 2048 x 1024)
+  // 114, 104, 122; 16 (32 of 7168 x 512) 184, 158, 155; 32 (8 of 4096 x 1024) 96, 97, 93; 64 (one of 4096 x 1024) 53, 41, 38.  Four instead of eight
+  // leave long rows more stages, which is worth 2 % where experts have a row or two (7168 x 512) and costs 14 % where they have four.
   const int terms = up ? 1 : 2;
   const double live = expected_live(slots, experts), cols_each = slots / live * terms;
   p.cols = cols_each > 18 ? 32 : cols_each > 10 ? 16 : cols_each > 3 || moe_smem(p.steps, 8, 4) <= kMoeMostSmem ? 8 : 4;

@@ -237,7 +237,7 @@ static int launch_rows(const void* A, const void* B, Params& p, cudaStream_t st)
     SGLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  SGLB_REQUIRE(tiles * p.splits < (1ll << 31), "fp4_scaled_mm: %lld tiles are too many", (long long)tiles);
+  SGLB_REQUIRE(tiles * p.splits < (1ll << 31), "group_fp4_scaled_mm: %lld tiles are too many", (long long)tiles);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * p.splits), 1, 1);
   cfg.blockDim = dim3(kRowsThreads, 1, 1);

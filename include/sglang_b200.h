@@ -140,7 +140,8 @@ int sglb200_group_fp4_scaled_mm(const void* A, const void* B, const void* a_s, c
  * of another rank) contributes nothing, the same id twice in a row counts twice.  Activations are not quantised: products with weights are exact in
  * fp16 (bf16 activations under a power of two per row; what is below 2^-18 of a row's largest magnitude is rounded to 2^-26 of
  * it), sums are float32, h is held to 23 bits for the second product (2^-23 of a value, 2^-37 of a row's largest), the output rounded once.
- * tokens * topk <= 1024, E <= 1024, hidden and intermediate divisible by 32; pointers 16-byte aligned.
+ * tokens * topk <= 1024, E <= 1024, hidden and intermediate divisible by 32 and at most 69120 (a row of the staged activations has to fit the
+ * shared memory; more is refused), an expert's w13 and w2 below 2^31 groups; pointers 16-byte aligned.
  * A row with a NaN or an infinity gives NaN or infinities in that row only.  A wait inside a kernel that runs out sets
  * sglb200_gemm_status().
  * workspace: device scratch of at least sglb200_fused_experts_fp4_workspace_bytes, 16-byte aligned, needs no initialisation.

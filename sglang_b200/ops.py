@@ -593,7 +593,7 @@ def fused_experts_fp4(
 
     hidden_states [T, H] bf16 or fp16; w13 uint8 [E, 2I, H / 2] (G_e's rows, then U_e's), w2 uint8 [E, H, I / 2]; their scales
     float8_e4m3fn in rows' order, [E, 2I, H / 16] and [E, H, I / 16]; topk_weights and topk_ids [T, k].  An id outside
-    [0, E) contributes nothing.  The alphas are float32 [E] (None: 1).  H and I divisible by 32."""
+    [0, E) contributes nothing.  The alphas are float32 [E] (None: 1).  H and I divisible by 32, at most 69120."""
     if topk_ids.dtype == torch.int64:  # (an id that does not fit an int32 names no expert)
         topk_ids = topk_ids.clamp(-1, 2**31 - 1).to(torch.int32)
     elif topk_ids.dtype != torch.int32:

@@ -78,8 +78,15 @@ def test_plans_fit_and_cover_the_work(rules):
 
 
 def test_rows_that_do_not_fit(rules):
-    assert plan(rules, 4, 8, 69120, 64, 1).stages >= 2 and plan(rules, 4, 8, 80000, 64, 1).stages == 0
-    assert plan(rules, 4, 8, 69120, 64, 0).stages >= 2 and plan(rules, 4, 8, 80000, 64, 0).stages == 0
+    """69120 columns are the most that the header promises; what does not fit is refused before anything is launched."""
+    from sglang_b200._lib import lib
+    A, size = 4096, lib.sglb200_fused_experts_fp4_workspace_bytes  # A: an aligned address that is never touched
+    for slots in (1, 4, 1024):
+        for up in (0, 1):
+            assert plan(rules, slots, 8, 69120, 64, up).stages >= 2 and plan(rules, slots, 8, 69120 + 32, 64, up).stages == 0
+    for H, I in ((69120 + 32, 64), (64, 69120 + 32), (1 << 30, 32)):
+        rc = lib.sglb200_fused_experts_fp4(A, 0, A, A, None, A, A, None, A, A, A, 2, 2, 8, H, I, 1.0, A, size(2, 2, H, I), None)
+        assert rc == -1 and b"too many" in lib.sglb200_last_error()
 
 
 def test_the_widths_of_pairs_tiles(rules):

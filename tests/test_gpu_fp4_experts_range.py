@@ -55,3 +55,11 @@ def test_rows_of_all_magnitudes(dtype):
     for row, p in enumerate(powers):
         assert (err[row] <= tol[row]).all(), (p, (err[row] / tol[row]).max())
         assert (err[row] ** 2).mean() <= (torch.finfo(dtype).eps / 2) ** 2 * (out[row] ** 2).mean(), p
+
+
+@pytest.mark.parametrize("H,I", [(69120, 32), (69088, 64), (64, 69120), (32, 69088)])
+def test_longest_rows(H, I):
+    """The most columns of either product, where one row at a time is staged."""
+    from tests.test_gpu_fp4_experts_terms import _check
+    args = _layer(3, 1, 1, H, I, torch.bfloat16, 23)
+    _check(_run(*args), _want(*args), H, I, torch.bfloat16)

@@ -1,10 +1,19 @@
 // Products of 4-bit operands:  C[m, n] = out_t( alpha * sum_k a[m, k] * b[n, k] + bias[n] ),  a and b e2m1 codes times the scale of
 // their group, on tcgen05.mma.kind::mxf4nvf4, which takes the scales from tensor memory and applies them inside the MMA.
 //
-// Many rows go to pairs of CTAs (fp4_pair.cu).  fp4_rows_kernel, for few rows or few tiles: the weights on the M side (128 of their rows), NT activation rows on the N side, so that nothing is multiplied
-// for padding of few rows up to 128; K split over the CTAs of a cluster, which add their partial sums through distributed shared
-// memory in a fixed order; without a split the sums go from tensor memory straight to the output.  Two CTAs an SM, each with a ring
-// of 80 to 100 KB: 1 x 36864 x 7168 takes 25.1 us (0.90 of the measured copy rate), 64 rows 28.8 (0.82), of which three are start and end.
+// Many rows go to pairs of CTAs (fp4_pair.cu).  fp4_rows_kernel, for few rows or few tiles: the weights on the M side (128 of their
+// rows), NT activation rows on the N side, so that nothing is multiplied for padding of few rows up to 128; K split over the CTAs of a
+// cluster, which add their partial sums through distributed shared memory in a fixed order; without a split the sums go from tensor
+// memory straight to the output.  Two CTAs an SM, each with a ring of 80 to 100 KB: 1 x 36864 x 7168 takes 25.1 us (0.90 of the measured
+// copy rate), 64 rows 28.8 (0.82) with the same weights again and 30.4 with other ones in between, of which three are start and end.
+//
+// Over how many CTAs K is split follows the rule of the 8-bit kernel (rows_splits), whose slabs are as many bytes.  Measured for
+// this one, us over 1, 2, 3, 4, 6 and 8 CTAs: 33 rows, 2112 x 7168 15.2, 10.8, 9.0, 8.2, 7.6 (taken), 8.2; 4096 x 14336 26.9, 17.2,
+// 13.7, 12.5 (taken), 11.9, 11.6; 10240 x 8192 18.0, 15.3, 13.5 (taken), 19.0, 18.6, 23.3; 48 rows, 4096 x 4096 10.6, 9.1, 8.1, 7.6
+// (taken), 8.6, 9.2; 64 rows, 7168 x 2048 8.0, 8.4, 8.5, 8.4 (taken), 13.4, 14.8; 1536 x 7168 15.8, 11.8, 9.8, 8.4, 8.0, 7.9
+// (taken); 2816 x 16768 32.1, 20.4, 15.6, 13.4, 11.9 (taken), 12.5.  What it charges more than 32 rows for pushed sums, which this
+// kernel does not push, changes none of twelve shapes at 33, 48, 64 and 128 rows. It loses where tiles are one or two more than
+// SMs: 64 x 19200 x 7168 takes three CTAs, 25.1, and one would be 20.1.
 #include <algorithm>
 
 #include "fp4_gemm.cuh"

@@ -19,7 +19,7 @@ __host__ __device__ __forceinline__ int64_t scale_at(int64_t row, int group, int
   return ((row >> 7) * group_blocks + (group >> 2)) * kBlockBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (group & 3);
 }
 
-// n / d for n < 2^31 by a multiplication (d >= 1).
+// n / d for n < 2^31 by a multiplication (d >= 1): the reciprocal rounded up, with one bit more than a word (Granlund and Montgomery, 1994).
 struct FastDiv {
   uint32_t d, mul, shift;
   FastDiv() = default;

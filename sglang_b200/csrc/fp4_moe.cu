@@ -14,20 +14,21 @@
 // under such a power of two as the sum of two fp16 terms, hi + 2^-11 lo, a column each: 23 bits, off by at most 2^-23 of a value or 2^-37 of
 // the row's largest.  (hi alone, 11 bits, moved one bf16 output in fifty by a step.)
 //
-// A CTA's item is a pass (an expert and at most 32 of its slots) and a few 16-row tiles; its 16 warps split the tiles and K.  Passes of
-// one expert go to CTAs of their own, which read its weights from the L2 (64 tokens, 4 of 8 experts of 4096 x 1024: 106 us, against 148
-// where a CTA took all passes of its tiles in turn; 82 with passes of eight rows instead of four).  One more warp keeps a ring of 36 KB
-// stages (codes and scales of 256 columns of all 16 tiles, one TMA load each) full across items, so that the memory streams while
-// rows are staged and sums are taken.  Partial sums meet in shared memory in a fixed order.  The second launch writes every slot's product
-// to a scratch, and whichever CTA is the last of a set of columns adds the slots of a token in their order, so results do not depend
-// on the order of CTAs.
+// A CTA's item is a pass (an expert and at most 32 of its slots) and a few 16-row tiles; its 16 warps split the tiles and K.
+// Passes of one expert go to CTAs of their own, which read its weights from the L2 (64 tokens, 4 of 8 experts of 4096 x 1024: 106
+// us, against 148 where a CTA took all passes of its tiles in turn; 82 with passes of eight rows instead of four; 93 since a row of
+// h has two columns).  One more warp keeps a ring of 36 KB stages (codes and scales of 256 columns of all 16 tiles, one TMA load
+// each) full across items, so that the memory streams while rows are staged and sums are taken.  Partial sums meet in shared memory
+// in a fixed order.  The second launch writes every slot's product to a scratch, and whichever CTA is the last of a set of columns
+// adds the slots of a token in their order, so results do not depend on the order of CTAs.
 //
-// 16 tokens, 8 of 256 experts of 7168 x 2048 (101 named, 2.5 GB): 450 to 490 us, 0.80 to 0.85 of the measured copy rate; the first product
-// streams at 0.96 of it, the second's items are shorter: a third of its time is their ends.  What bounds both is the expansion, 1500
-// clocks a stage against 1530 that the memory takes for it.  Small layers are bound by latency: two launches without weights to speak
-// of take 13 us (of which staging the rows 2 to 3 a launch, finding the experts 0.7, the count of items and the last sums 2), one
-// token through eighths of experts (25 MB) 21.  Not kept: weights straight into registers (16 warps, three steps deep: 570 us), two
-// tiles a warp (620; the ring is then two stages deep), two CTAs of eight warps an SM (520), a warp of its own that counts items (500).
+// 16 tokens, 8 of 256 experts of 7168 x 2048 (101 named, 2.5 GB): 483 to 550 us with the weights of three layers in turn, 0.70 to
+// 0.79 of the measured copy rate; the first product streams at 0.96 of it, the second's items are shorter: a third of its time is
+// their ends.  What bounds both is the expansion, 1500 clocks a stage against 1530 that the memory takes for it.  Small layers are
+// bound by latency: two launches without weights to speak of take 13 us (of which staging the rows 2 to 3 a launch, finding the
+// experts 0.7, the count of items and the last sums 2), one token through eighths of experts (25 MB) 21.  Not kept: weights
+// straight into registers (16 warps, three steps deep: 570 us), two tiles a warp (620; the ring is then two stages deep), two CTAs
+// of eight warps an SM (520), a warp of its own that counts items (500).
 #include <algorithm>
 #include <type_traits>
 

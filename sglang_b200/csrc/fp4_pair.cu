@@ -6,9 +6,10 @@
 // The scales of a slab (in blocked order, so that they are contiguous) lie in the same stage; the thread that multiplies copies
 // them into tensor memory, two sets in turn, right in front of the instructions that read them.
 //
-// 4096 x 36864 x 7168 387 us: 5.6 PFLOP/s, 3.35 times the measured bf16 rate (cta_group::1, 128 x 128 tiles: 995 us).  What is left is
-// mostly power: the tensor cores are the load.  With a second staging area for the output there is room for four stages instead of
-// five: 405 us there, 4096 x 24576 x 1536 107 instead of 92, 4096 x 32768 x 512 88 instead of 91.
+// 4096 x 36864 x 7168 387 us in a burst: 5.6 PFLOP/s, 3.35 times the measured bf16 burst rate (cta_group::1, 128 x 128 tiles: 995
+// us); one after the other 463 to 468.  What is left is mostly power: the tensor cores are the load.  With a second staging area
+// for the output there is room for four stages instead of five: 405 us there, 4096 x 24576 x 1536 107 instead of 92, 4096 x 32768 x
+// 512 88 instead of 91.
 //
 // Persistent.  Warps: 0-7 epilogue (two groups of four, each half of the columns), 8 fetches, 9 multiplies (in the even CTA).  With
 // BN = 256 there is one accumulator, which the epilogue empties into registers, rounded, before it stores anything; with 192 and

@@ -251,7 +251,8 @@ __global__ void __launch_bounds__(kThreads)
     const uint32_t code = quantize16<kGroup, kSilu>(v, g, c, near);
     if (near) again |= 1u << k;
     if (at[k].live) codes[at[k].unit] = c;
-    if (at[k].row_live && at[k].column % (kGroup / kUnit) == 0) scales[at[k].scale] = at[k].live ? (uint8_t)code : 0;  // (zeros for groups past the last)
+    // (zeros for groups past the last)
+    if (at[k].row_live && at[k].column % (kGroup / kUnit) == 0) scales[at[k].scale] = at[k].live ? (uint8_t)code : 0;
   }
   if constexpr (kSilu) {
     if (__ballot_sync(0xffffffffu, again != 0) == 0) return;

@@ -68,12 +68,13 @@ struct ExpertsPlan {
 inline ExpertsPlan plan_experts(int64_t slots, int64_t experts, int64_t K, int64_t rows, bool up, int64_t sms) {
   ExpertsPlan p{};
   p.steps = (int)((K + kStep - 1) / kStep);
-  // Rows per pass, and the columns that they take (two a row of h): every pass of an expert reads its weights again (from the L2, by other
-  // CTAs at the same time), and columns take the place of stages; eight columns cost the same with one row in them as with all.
-  // us of a layer over 8, 16 and 32 columns of x: 2 rows an expert (128 of 2048 x 768) 92, 102, 102; 4 (64 of 2048 x 1024) 85, 94, 93; 12 (32 of
-  // 1376 x 1440) 107, 106, 120; 16 (16 of 2080 x 1056) 95, 90, 90; 64 (4 of 2048 x 2048) 84, 79, 80.  Of h: 4 rows 85, 94, 105; 8 (64 of 2048 x 1024)
-  // 114, 104, 122; 16 (32 of 7168 x 512) 184, 158, 155; 32 (8 of 4096 x 1024) 96, 97, 93; 64 (one of 4096 x 1024) 53, 41, 38.  Four instead of eight
-  // leave long rows more stages, which is worth 2 % where experts have a row or two (7168 x 512) and costs 14 % where they have four.
+  // Rows per pass, and the columns that they take (two a row of h): every pass of an expert reads its weights again (from the L2,
+  // by other CTAs at the same time), and columns take the place of stages; eight columns cost the same with one row in them as with
+  // all. us of a layer over 8, 16 and 32 columns of x: 2 rows an expert (128 of 2048 x 768) 92, 102, 102; 4 (64 of 2048 x 1024) 85,
+  // 94, 93; 12 (32 of 1376 x 1440) 107, 106, 120; 16 (16 of 2080 x 1056) 95, 90, 90; 64 (4 of 2048 x 2048) 84, 79, 80.  Of h: 4
+  // rows 85, 94, 105; 8 (64 of 2048 x 1024) 114, 104, 122; 16 (32 of 7168 x 512) 184, 158, 155; 32 (8 of 4096 x 1024) 96, 97, 93;
+  // 64 (one of 4096 x 1024) 53, 41, 38.  Four instead of eight leave long rows more stages, which is worth 2 % where experts have a
+  // row or two (7168 x 512) and costs 14 % where they have four.
   const int terms = up ? 1 : 2;
   const double live = expected_live(slots, experts), cols_each = slots / live * terms;
   p.cols = cols_each > 18 ? 32 : cols_each > 10 ? 16 : cols_each > 3 || moe_smem(p.steps, 8, 4) <= kMoeMostSmem ? 8 : 4;
@@ -81,12 +82,12 @@ inline ExpertsPlan plan_experts(int64_t slots, int64_t experts, int64_t K, int64
   if (moe_smem(p.steps, p.cols, 2) > kMoeMostSmem) p.cols = 1;
   p.pass_rows = std::max(1, p.cols / terms);
   const double passes = expected_passes(slots, experts, p.pass_rows, live);
-  // Warps that split K, the others taking tiles of their own: more of them make more and shorter items, which fill the GPU and its last
-  // round better, but each item has an end, of two barriers and the shared memory between where K is split and of a count where
-  // the slots are summed.  Times in turns of the ring: an end is 0.2 of one for the first product, 0.7 with a split K (the second: 0.5, 1.2);
-  // scales that come by asynchronous copies come slower in short runs.  us of a layer over 1, 2, 4 and 8 for the first product: one token,
-  // 8 experts of 7168 x 256 41, 31, 26, 24; 101 named of 7168 x 2048 451, 475, 475, 497; 11 of 4096 x 2048 62, 57, 54, 57; 24 of
-  // 7136 x 544 84, 78, 66, 67.  For the second: 106 of 7168 x 2048 580, 606, 642, 723.
+  // Warps that split K, the others taking tiles of their own: more of them make more and shorter items, which fill the GPU and its
+  // last round better, but each item has an end, of two barriers and the shared memory between where K is split and of a count
+  // where the slots are summed.  Times in turns of the ring: an end is 0.2 of one for the first product, 0.7 with a split K (the
+  // second: 0.5, 1.2); scales that come by asynchronous copies come slower in short runs.  us of a layer over 1, 2, 4 and 8 for the
+  // first product: one token, 8 experts of 7168 x 256 41, 31, 26, 24; 101 named of 7168 x 2048 451, 475, 475, 497; 11 of 4096 x
+  // 2048 62, 57, 54, 57; 24 of 7136 x 544 84, 78, 66, 67.  For the second: 106 of 7168 x 2048 580, 606, 642, 723.
   double best = 0.0;
   for (int k = 1; k <= kMoeWarps && k <= p.steps; k *= 2) {
     const int per = kMoeWarps / k, sets = (int)((rows / 16 + per - 1) / per), turns = (p.steps + k - 1) / k;

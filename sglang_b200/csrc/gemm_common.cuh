@@ -23,8 +23,8 @@ __device__ __forceinline__ void tile_coord(int t, int tiles_m, int tiles_n, int 
 // 128-byte swizzle, out-of-range elements read as zero.  Cached per argument tuple and thread.
 int get_tensor_map(const void* ptr, uint64_t d0, uint64_t d1, uint64_t d2, uint32_t box_rows, uint32_t rank, CUtensorMap* out);
 
-// uint8 tensor of `rank` (2 to 5) dimensions, innermost first, `strides` of all but the innermost in bytes; out-of-range elements read as zero; with `swizzled` the box's
-// rows are 128 bytes.  Cached likewise.
+// uint8 tensor of `rank` (2 to 5) dimensions, innermost first, `strides` of all but the innermost in bytes; out-of-range elements
+// read as zero; with `swizzled` the box's rows are 128 bytes.  Cached likewise.
 int get_tile_map(const void* ptr, uint32_t rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box, bool swizzled,
                  CUtensorMap* out);
 

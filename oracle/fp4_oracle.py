@@ -20,13 +20,6 @@ def nearest(num, den, grid):
     return code
 
 
-def nearest_sorted(num, grid):
-    """The same for den = 1 and long grids."""
-    mid = (grid[:-1] + grid[1:]) / 2
-    low, high = np.searchsorted(mid, num, side="left"), np.searchsorted(mid, num, side="right")
-    return np.where(low == high, low, low + low % 2)  # on the border between low and low + 1: the even one
-
-
 def group_scales(x, g, group):
     """x [rows, hidden] -> (scale codes uint8 [rows, groups], scale values, NaN where a group is not finite)."""
     a = np.abs(x.reshape(x.shape[0], -1, group).astype(np.float64))
@@ -104,14 +97,3 @@ def silu_and_mul(x):
     gate, up = x[..., :d].astype(np.float64), x[..., d:].astype(np.float64)
     with np.errstate(over="ignore"):
         return gate / (1 + np.exp(-gate)) * up
-
-
-def fused_experts(x, w13, w2, w13_alpha, w2_alpha, weights, ids, factor=1.0):
-    """x [T, H]; w13 [E, 2I, H], w2 [E, H, I] dequantised; ids outside [0, E) contribute nothing."""
-    out = np.zeros((x.shape[0], w2.shape[1]))
-    for t in range(x.shape[0]):
-        for j, e in enumerate(ids[t]):
-            if 0 <= e < len(w13):
-                h = silu_and_mul(w13_alpha[e] * (w13[e] @ x[t].astype(np.float64)))
-                out[t] += float(weights[t, j]) * w2_alpha[e] * (w2[e] @ h)
-    return out * factor

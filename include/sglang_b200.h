@@ -239,6 +239,43 @@ int sglb200_moe_fused_gate(const void* input, const void* bias, int dtype, int64
                            int32_t* topk_ids, void* stream);
 
 /*
+ * The router's product:  y[t, e] = sum_k x[t, k] w[e, k], float32 sums, unrounded.
+ * x [tokens, K] of dtype 0 or 1, rows `x_stride` elements apart; w [num_experts, K] of the same type, contiguous; y float32
+ * [tokens, num_experts].  K % 8 == 0, x_stride % 8 == 0; x, w and y 16-byte aligned.
+ */
+int sglb200_router_logits(const void* x, const void* w, int dtype, float* y, int64_t tokens, int64_t num_experts, int64_t K,
+                          int64_t x_stride, void* stream);
+
+/*
+ * Routing in general form, decided by the real numbers:  s = softmax(x) (softmax != 0) or sigmoid(x);  c = s + correction_bias (float32
+ * [num_experts] or NULL);  the value of each of the num_expert_group groups is the sum of its group_top (1 or 2) largest c; the
+ * topk_group best groups are kept (equal: lower group first) and the topk largest c in them picked (equal: lower expert first);
+ * weight = s, divided by the sum of the picks' s when renormalize, times routed_scaling_factor.
+ * An expert whose logit is NaN or -inf, or whose c is, is not available; a slot for which none is left gets the id -1 and weight 0.
+ * topk <= 32; at most 32 groups, and 1024 experts in all when each group's are 32 / (groups rounded up to a power of two) lanes of 32.
+ */
+int sglb200_route_topk(const void* logits, int dtype, int64_t rows, int num_experts, int topk, int softmax, const float* correction_bias,
+                       int num_expert_group, int topk_group, int group_top, int renormalize, float routed_scaling_factor,
+                       float* topk_weights, int32_t* topk_ids, void* stream);
+
+/*
+ * Low-rank adapters added to a shared projection:
+ *   out[t, n] = rnd( base[t, n] + scalings[l] * sum_{r < ranks[l]} lora_b[l, n, r] * sum_k x[t, k] lora_a[l, s(n) * rank + r, k] )
+ * with l = adapter_ids[t], and out = base where that names none (outside [0, num_adapters)).  s(n): the slice that column n is in, of
+ * num_slices (at most 8) merged projections of slice_sizes columns (host array), N in all.
+ * x [tokens, K], base and out [tokens, N]: dtype 0 or 1, rows their strides (in elements) apart; out may be base, and is not to overlap
+ * it otherwise.  lora_a [num_adapters, num_slices * rank, K], lora_b [num_adapters, N, rank]: the same type, contiguous.  scalings
+ * (float32), ranks (int32): [num_adapters] or NULL (1, rank); what lies beyond an adapter's rank is not used.  rank % 8 == 0, at most
+ * 256; K % 8 == 0; x_stride % 8 == 0; x, lora_a and lora_b 16-byte aligned.  workspace: 16-byte aligned, the bytes that the function
+ * beside it says.
+ */
+int64_t sglb200_lora_add_workspace_bytes(int64_t tokens, int num_adapters, int rank, int num_slices);
+int sglb200_lora_add(const void* x, const void* lora_a, const void* lora_b, const void* base, void* out, int dtype,
+                     const int32_t* adapter_ids, const float* scalings, const int32_t* ranks, int64_t tokens, int num_adapters, int rank,
+                     int64_t N, int64_t K, int64_t x_stride, int64_t base_stride, int64_t out_stride, int num_slices,
+                     const int64_t* slice_sizes, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * out[t, :] = bf16( scale * sum_k x[t, k, :] ), float32 accumulation in ascending k.
  * Replaces: torch.ops.sgl_kernel.moe_sum_reduce (sgl-kernel/csrc/moe/moe_sum_reduce.cu:56-116,
  *   schema common_extension.cc:234-235).  x [tokens, topk, hidden] contiguous, hidden % 8 == 0.

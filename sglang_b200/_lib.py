@@ -52,6 +52,10 @@ SIGNATURES = {
     "sglb200_topk_softmax": (_i32, [_vp, _i32, _i64, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _vp]),
     "sglb200_topk_sigmoid": (_i32, [_vp, _i32, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp]),
     "sglb200_moe_fused_gate": (_i32, [_vp, _vp, _i32, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _vp, _vp]),
+    "sglb200_router_logits": (_i32, [_vp, _vp, _i32, _vp, _i64, _i64, _i64, _i64, _vp]),
+    "sglb200_route_topk": (_i32, [_vp, _i32, _i64, _i32, _i32, _i32, _vp, _i32, _i32, _i32, _i32, _f32, _vp, _vp, _vp]),
+    "sglb200_lora_add_workspace_bytes": (_i64, [_i64, _i32, _i32, _i32]),
+    "sglb200_lora_add": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i32, C.POINTER(_i64), _vp, _i64, _vp]),
     "sglb200_gather_rows_fp8": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i64, _i64, _vp]),
     "sglb200_gemm_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "sglb200_fp8_blockwise_scaled_mm": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _vp, _i64, _vp]),

@@ -13,6 +13,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
+#include <limits.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -39,6 +40,10 @@ namespace {
   X(sglb200_fused_experts_workspace_bytes) \
   X(sglb200_fused_experts)               \
   X(sglb200_topk_softmax)                \
+  X(sglb200_router_logits)               \
+  X(sglb200_route_topk)                  \
+  X(sglb200_lora_add_workspace_bytes)    \
+  X(sglb200_lora_add)                    \
   X(sglb200_moe_fused_gate)
 
 struct Abi {
@@ -361,6 +366,16 @@ PyObject* matmul_fp4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
+// One float32 each on x's device, or absent.
+bool factors_ok(PyObject* o, int64_t n, const Tensor& x, const float** value) {
+  *value = nullptr;
+  if (o == Py_None) return true;
+  const Tensor* t = cuda_contig(o);
+  if (t == nullptr || t->numel() != n || t->scalar_type() != at::kFloat || t->device() != x.device()) return false;
+  *value = static_cast<const float*>(t->data_ptr());
+  return true;
+}
+
 // ---- routing --------------------------------------------------------------------------------------------------
 // topk_softmax(logits [T, E], k, renormalize) -> (weights, ids)
 PyObject* topk_softmax(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -401,6 +416,101 @@ PyObject* fused_gate(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                                               static_cast<float*>(w.data_ptr()), static_cast<int32_t*>(ids.data_ptr()), stream_of(*g));
     if (rc) return raise_last(rc);
     return pair(std::move(w), std::move(ids));
+  });
+}
+
+// route_topk(logits [T, E], k, softmax, bias [E] f32 | None, groups, topk_group, group_top, renormalize, factor) -> (weights, ids)
+PyObject* route_topk(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 9) Py_RETURN_NONE;
+  const Tensor* g = cuda_contig(args[0]);
+  const int64_t k = PyLong_AsLongLong(args[1]), groups = PyLong_AsLongLong(args[4]), kept = PyLong_AsLongLong(args[5]),
+                top = PyLong_AsLongLong(args[6]);
+  const bool softmax = flag(args[2]), renormalize = flag(args[7]);
+  const double factor = PyFloat_AsDouble(args[8]);
+  if (PyErr_Occurred()) return nullptr;
+  const float* bias;
+  if (g == nullptr || g->dim() != 2 || g->size(1) > INT_MAX || !here(*g) || !factors_ok(args[3], g->size(1), *g, &bias)) Py_RETURN_NONE;
+  const int dt = dtype_code(g->scalar_type());
+  // (numbers that the C ABI's ints do not hold go to the Python form, which names them)
+  if (dt < 0 || k < 1 || k > g->size(1) || groups < 1 || groups > g->size(1) || kept < 1 || kept > groups || top < 1 || top > 2)
+    Py_RETURN_NONE;
+  return guarded([&]() -> PyObject* {
+    Tensor w = make({g->size(0), k}, at::kFloat, g->device()), ids = make({g->size(0), k}, at::kInt, g->device());
+    const int rc = abi.sglb200_route_topk(g->data_ptr(), dt, g->size(0), (int)g->size(1), (int)k, softmax, bias, (int)groups, (int)kept,
+                                          (int)top, renormalize, (float)factor, static_cast<float*>(w.data_ptr()),
+                                          static_cast<int32_t*>(ids.data_ptr()), stream_of(*g));
+    if (rc) return raise_last(rc);
+    return pair(std::move(w), std::move(ids));
+  });
+}
+
+// router_logits(x [.., K] 16-bit, w [E, K]) -> float32 [.., E]
+PyObject* router_logits(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 2) Py_RETURN_NONE;
+  const Tensor *xp = cuda_contig(args[0]), *w = cuda_contig(args[1]);
+  if (!xp || !w || xp->dim() < 1 || w->dim() != 2 || w->scalar_type() != xp->scalar_type() || w->device() != xp->device() || !here(*xp))
+    Py_RETURN_NONE;
+  const Tensor& x = *xp;
+  const int dt = dtype_code(x.scalar_type());
+  const int64_t K = x.size(-1), E = w->size(0);
+  if (dt < 0 || dt > 1 || K == 0 || E == 0 || w->size(1) != K) Py_RETURN_NONE;
+  return guarded([&]() -> PyObject* {
+    c10::DimVector shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = E;
+    Tensor y = make(shape, at::kFloat, x.device());
+    const int rc = abi.sglb200_router_logits(x.data_ptr(), w->data_ptr(), dt, static_cast<float*>(y.data_ptr()), x.numel() / K, E, K, K,
+                                             stream_of(x));
+    if (rc) return raise_last(rc);
+    return THPVariable_Wrap(std::move(y));
+  });
+}
+
+// ---- low-rank adapters ----------------------------------------------------------------------------------------
+// lora_add(base [.., N], x [.., K], lora_a [L, S R, K], lora_b [L, N, R], ids i32, scalings f32 [L] | None, ranks i32 [L] | None,
+//          slices (tuple of S sizes) | None, out | None) -> [.., N]
+PyObject* lora_add(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 9) Py_RETURN_NONE;
+  const Tensor *base = cuda_contig(args[0]), *xp = cuda_contig(args[1]), *a = cuda_contig(args[2]), *b = cuda_contig(args[3]),
+               *ids = cuda_contig(args[4]);
+  const Tensor* into = args[8] != Py_None ? cuda_contig(args[8]) : nullptr;
+  if (!base || !xp || !a || !b || !ids || !here(*xp) || (args[8] != Py_None && !into)) Py_RETURN_NONE;
+  const Tensor& x = *xp;
+  if (into && (into->sizes() != base->sizes() || into->scalar_type() != x.scalar_type() || into->device() != x.device())) Py_RETURN_NONE;
+  const int dt = dtype_code(x.scalar_type());
+  for (const Tensor* t : {base, a, b})
+    if (t->scalar_type() != x.scalar_type() || t->device() != x.device()) Py_RETURN_NONE;
+  if (dt < 0 || dt > 1 || x.dim() < 1 || base->dim() != x.dim() || a->dim() != 3 || b->dim() != 3 || ids->scalar_type() != at::kInt ||
+      ids->device() != x.device())
+    Py_RETURN_NONE;
+  const int64_t K = x.size(-1), N = base->size(-1), L = a->size(0), R = b->size(2);
+  if (K == 0 || N == 0 || L == 0 || R == 0 || L > INT_MAX || R > INT_MAX || x.numel() / K != base->numel() / N || a->size(2) != K ||
+      b->size(0) != L || b->size(1) != N || ids->numel() != x.numel() / K || x.sizes().slice(0, x.dim() - 1) != base->sizes().slice(0, x.dim() - 1))
+    Py_RETURN_NONE;
+  int64_t sizes[8] = {N}, S = 1;
+  if (args[7] != Py_None) {
+    if (!PyTuple_CheckExact(args[7]) || PyTuple_GET_SIZE(args[7]) < 1 || PyTuple_GET_SIZE(args[7]) > 8) Py_RETURN_NONE;
+    S = PyTuple_GET_SIZE(args[7]);
+    for (int64_t s = 0; s < S; ++s) sizes[s] = PyLong_AsLongLong(PyTuple_GET_ITEM(args[7], s));
+    if (PyErr_Occurred()) return nullptr;
+  }
+  const float* scalings;
+  const int32_t* ranks = nullptr;
+  if (a->size(1) != S * R || !factors_ok(args[5], L, x, &scalings)) Py_RETURN_NONE;
+  if (args[6] != Py_None) {
+    const Tensor* t = cuda_contig(args[6]);
+    if (!t || t->numel() != L || t->scalar_type() != at::kInt || t->device() != x.device()) Py_RETURN_NONE;
+    ranks = static_cast<const int32_t*>(t->data_ptr());
+  }
+  return guarded([&]() -> PyObject* {
+    const int64_t T = x.numel() / K, bytes = abi.sglb200_lora_add_workspace_bytes(T, (int)L, (int)R, (int)S);
+    Tensor out = into ? *into : make(base->sizes(), x.scalar_type(), x.device());
+    if (T == 0) return THPVariable_Wrap(std::move(out));
+    Tensor mem = workspace(bytes, x.device());
+    const int rc = abi.sglb200_lora_add(x.data_ptr(), a->data_ptr(), b->data_ptr(), base->data_ptr(), out.data_ptr(), dt,
+                                        static_cast<const int32_t*>(ids->data_ptr()), scalings, ranks, T, (int)L, (int)R, N, K, K, N, N,
+                                        (int)S, sizes, mem.data_ptr(), bytes, stream_of(x));
+    if (rc) return raise_last(rc);
+    return THPVariable_Wrap(std::move(out));
   });
 }
 
@@ -446,16 +556,6 @@ bool experts_fp4_ok(const Tensor* w, const Tensor* s) {
          s->size(0) == w->size(0) && s->size(1) == w->size(1) && s->size(2) * 8 == w->size(2) && s->device() == w->device();
 }
 
-// One float32 per expert on x's device, or absent.
-bool factors_ok(PyObject* o, int64_t n, const Tensor& x, const float** value) {
-  *value = nullptr;
-  if (o == Py_None) return true;
-  const Tensor* t = cuda_contig(o);
-  if (t == nullptr || t->numel() != n || t->scalar_type() != at::kFloat || t->device() != x.device()) return false;
-  *value = static_cast<const float*>(t->data_ptr());
-  return true;
-}
-
 // fused_experts_fp4(x [T, H] 16-bit, w13, w2, w13_scale, w2_scale, weights [T, k] f32, ids [T, k] i32, w13_alpha | None,
 //                   w2_alpha | None, factor) -> [T, H]
 PyObject* fused_experts_fp4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -490,7 +590,7 @@ PyObject* fused_experts_fp4(PyObject*, PyObject* const* args, Py_ssize_t nargs) 
 PyMethodDef methods[] = {
     {"bind", bind, METH_O, "Bind the C ABI of the library at this path."},
 #define M(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-    M(quant), M(silu_mul_quant), M(quant_fp4), M(silu_mul_quant_fp4), M(dequant_fp4), M(linear), M(matmul), M(matmul_fp4), M(topk_softmax), M(fused_gate), M(fused_experts), M(fused_experts_fp4),
+    M(quant), M(silu_mul_quant), M(quant_fp4), M(silu_mul_quant_fp4), M(dequant_fp4), M(linear), M(matmul), M(matmul_fp4), M(topk_softmax), M(fused_gate), M(route_topk), M(router_logits), M(lora_add), M(fused_experts), M(fused_experts_fp4),
 #undef M
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -1,0 +1,173 @@
+// y[t, n] = sum_k x[t, k] w[n, k], few n, float32 sums (see narrow.cuh).
+//
+// narrow_kernel: the weights on the M side of mma.sync (16 of their rows), up to 64 activation rows on its N side, operands straight from
+// global memory into registers: a lane takes 16 consecutive bytes of its row, and as a sum does not mind the order of its terms, those are
+// its part of two instructions, of the weights' rows and the activations' alike.  K is split over the warps of a CTA and the CTAs of a
+// cluster, whose sums meet in a fixed order.
+#include <algorithm>
+
+#include "gemm_common.cuh"
+#include "narrow.cuh"
+#include "ptx_sm100.cuh"
+
+namespace sglb200 {
+namespace narrow {
+
+constexpr int kWarps = 8;
+constexpr int kStep = 32;  // columns of K a warp takes at a time
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// kG groups of 8 activation rows.
+template <typename T, int kG>
+__global__ void __launch_bounds__(kWarps * 32) narrow_kernel(const Params p) {
+  constexpr int kCols = kG * 8;
+  __shared__ float part[kWarps][16][kCols];
+  __shared__ float sums[16 * kCols];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
+  const int rank = (int)(blockIdx.x % p.splits), n0 = (int)(blockIdx.x / p.splits % p.n_tiles) * 16;
+  const int64_t block = blockIdx.x / p.splits / p.n_tiles;
+  ptx::grid_dependency_wait();
+  ptx::launch_dependents();
+  int64_t start = block * kBlock, adapter = 0;
+  int rows = (int)min((int64_t)kBlock, p.T - start);
+  if (p.blocks.order != nullptr) {  // (uniform over the cluster)
+    if (block >= *p.blocks.count) return;
+    start = p.blocks.start[block], rows = p.blocks.rows[block], adapter = p.blocks.adapter[block];
+    if (adapter < 0) return;
+  }
+  const int used = p.ranks != nullptr ? min(max(p.ranks[adapter], 0), p.rank_rows) : p.rank_rows;
+  const T* w = static_cast<const T*>(p.w) + adapter * p.N * p.K;
+  const int64_t na = n0 + g, nb = n0 + g + 8;
+  const bool a_on = na < p.N && na % p.rank_rows < used, b_on = nb < p.N && nb % p.rank_rows < used;
+  const T* wa = w + (a_on ? na : 0) * p.K;
+  const T* wb = w + (b_on ? nb : 0) * p.K;
+  const T* x[kG];
+  bool x_on[kG];
+#pragma unroll
+  for (int j = 0; j < kG; ++j) {
+    x_on[j] = j * 8 + g < rows;
+    const int64_t r = x_on[j] ? start + j * 8 + g : start;
+    x[j] = static_cast<const T*>(p.x) + (p.blocks.order != nullptr ? (int64_t)p.blocks.order[r] : r) * p.ldx;
+  }
+  float acc[kG][4] = {};
+  const int steps = (int)((p.K + kStep - 1) / kStep), parts = p.splits * kWarps, mine = rank * kWarps + warp;
+  const int s0 = (int)((int64_t)mine * steps / parts), s1 = (int)((int64_t)(mine + 1) * steps / parts);
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll 2
+  for (int s = s0; s < s1; ++s) {
+    const int64_t k = (int64_t)s * kStep + q * 8;
+    const bool in = k < p.K;  // (K is a multiple of 8)
+    const uint4 a = in && a_on ? __ldg(reinterpret_cast<const uint4*>(wa + k)) : zero;
+    const uint4 b = in && b_on ? __ldg(reinterpret_cast<const uint4*>(wb + k)) : zero;
+    const uint32_t first[4] = {a.x, b.x, a.y, b.y}, second[4] = {a.z, b.z, a.w, b.w};
+    uint4 v[kG];
+#pragma unroll
+    for (int j = 0; j < kG; ++j) v[j] = in && x_on[j] ? ld_nc_16(x[j] + k) : zero;
+#pragma unroll
+    for (int j = 0; j < kG; ++j)
+      if (j * 8 < rows) mma16816<T>(acc[j], first, v[j].x, v[j].y), mma16816<T>(acc[j], second, v[j].z, v[j].w);
+  }
+#pragma unroll
+  for (int j = 0; j < kG; ++j) {
+    *reinterpret_cast<float2*>(&part[warp][g][j * 8 + q * 2]) = make_float2(acc[j][0], acc[j][1]);
+    *reinterpret_cast<float2*>(&part[warp][g + 8][j * 8 + q * 2]) = make_float2(acc[j][2], acc[j][3]);
+  }
+  __syncthreads();
+  // The warps' sums, then the CTAs', each in ascending order of K.
+  for (int i = threadIdx.x; i < 16 * kCols; i += kWarps * 32) {
+    float v = 0.f;
+#pragma unroll
+    for (int u = 0; u < kWarps; ++u) v += (&part[u][0][0])[i];
+    sums[i] = v;
+  }
+  if (p.splits > 1) {
+    ptx::cluster_sync();
+  } else {
+    __syncthreads();
+  }
+  const uint32_t at = ptx::smem_u32(sums);
+  for (int i = threadIdx.x + rank * kWarps * 32; i < 16 * kCols; i += p.splits * kWarps * 32) {
+    // (neighbouring threads take neighbouring rows of the weights, which lie side by side in y)
+    const int n = i & 15, t = i >> 4;
+    if (t >= rows || n0 + n >= p.N) continue;
+    float v = 0.f;
+    if (p.splits > 1) {
+      for (int s = 0; s < p.splits; ++s) {
+        float o;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o) : "r"(ptx::cluster_map(at + (n * kCols + t) * 4, s)) : "memory");
+        v += o;
+      }
+    } else {
+      v = sums[n * kCols + t];
+    }
+    p.y[(start + t) * p.N + n0 + n] = v;
+  }
+  if (p.splits > 1) ptx::cluster_sync();  // no CTA leaves while another reads its shared memory
+}
+
+template <typename T, int kG>
+static int launch(const Params& p, int64_t blocks, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  const int64_t grid = blocks * p.n_tiles * p.splits;
+  SGLB_REQUIRE(grid < (1ll << 31), "narrow product: %lld tiles are too many", (long long)grid);
+  cfg.gridDim = dim3((unsigned)grid, 1, 1);
+  cfg.blockDim = dim3(kWarps * 32, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)p.splits, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  SGLB_CUDA(cudaLaunchKernelEx(&cfg, narrow_kernel<T, kG>, p));
+  return SGLB200_OK;
+}
+
+template <typename T>
+static int dispatch(Params& p, int64_t blocks, cudaStream_t st) {
+  p.n_tiles = (int)((p.N + 15) / 16);
+  const int64_t tiles = blocks * p.n_tiles, steps = (p.K + kStep - 1) / kStep;
+  p.splits = 1;
+  while (p.splits < 8 && tiles * p.splits * 2 <= 2 * sm_count() && steps >= p.splits * 2 * kWarps) p.splits *= 2;
+  if (p.T <= 8) return launch<T, 1>(p, blocks, st);
+  if (p.T <= 16) return launch<T, 2>(p, blocks, st);
+  return launch<T, 8>(p, blocks, st);
+}
+
+int product(Params p, int dtype, int64_t max_blocks, cudaStream_t st) {
+  return dtype == 0 ? dispatch<__nv_bfloat16>(p, max_blocks, st) : dispatch<__half>(p, max_blocks, st);
+}
+
+}  // namespace narrow
+}  // namespace sglb200
+
+using namespace sglb200;
+
+extern "C" int sglb200_router_logits(const void* x, const void* w, int dtype, float* y, int64_t tokens, int64_t num_experts, int64_t K,
+                                     int64_t x_stride, void* stream) {
+  if (dtype != 0 && dtype != 1) return fail(SGLB200_E_UNSUPPORTED, "router_logits: dtype %d (0 bf16, 1 fp16)", dtype);
+  SGLB_REQUIRE(tokens >= 0 && num_experts >= 1 && K >= 1, "router_logits: %lld tokens, %lld experts, K %lld", (long long)tokens,
+               (long long)num_experts, (long long)K);
+  SGLB_REQUIRE(K % 8 == 0 && x_stride % 8 == 0 && x_stride >= K, "router_logits: K (%lld) and the rows' stride (%lld) must be divisible by 8",
+               (long long)K, (long long)x_stride);
+  SGLB_REQUIRE(tokens < (1ll << 31) - 256 && num_experts <= 1 << 16 && K <= 1 << 20, "router_logits: %lld tokens, %lld experts or K %lld is too large",
+               (long long)tokens, (long long)num_experts, (long long)K);
+  if (tokens == 0) return SGLB200_OK;
+  SGLB_REQUIRE(x && w && y, "router_logits: null pointer");
+  SGLB_REQUIRE(aligned16(x) && aligned16(w) && aligned16(y), "router_logits: pointers must be 16-byte aligned");
+  narrow::Params p{};
+  p.x = x, p.w = w, p.y = y, p.T = tokens, p.N = num_experts, p.K = K, p.ldx = x_stride, p.rank_rows = (int)num_experts;
+  return narrow::product(p, dtype, (tokens + narrow::kBlock - 1) / narrow::kBlock, static_cast<cudaStream_t>(stream));
+}

@@ -7,6 +7,7 @@ here computes on the host and nothing synchronises the device.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Optional, Tuple
 
 import torch
@@ -384,6 +385,96 @@ def moe_fused_gate(input: torch.Tensor, bias: torch.Tensor, num_expert_group: in
     return w, ids
 
 
+def _same_device(like: torch.Tensor, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != like.device:
+            raise RuntimeError(f"{name} is on {t.device}, the other tensors on {like.device}")
+
+
+def _rows_view(t: torch.Tensor, name: str) -> torch.Tensor:
+    """`t` [..., n] as rows with neighbouring columns, any one distance apart: a view, never a copy."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if t.dim() < 1 or t.shape[-1] == 0:
+        raise RuntimeError(f"{name}: the last dimension is empty")
+    if t.dim() == 2:
+        rows = t
+    elif t.dim() == 1:
+        rows = t[None]
+    else:
+        try:
+            rows = t.view(-1, t.shape[-1]) if t.numel() else t.reshape(0, t.shape[-1])
+        except RuntimeError as e:
+            raise RuntimeError(f"{name}: its rows are not one distance apart") from e
+    if rows.shape[0] and (rows.stride(1) != 1 and rows.shape[1] > 1 or rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]):
+        raise RuntimeError(f"{name}: strides {t.stride()}; columns must be neighbours and rows not overlap")
+    return rows
+
+
+def _row_stride(rows: torch.Tensor) -> int:
+    return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
+
+
+def router_logits(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+    """The router's product: float32 [..., E] of x [..., K] and weight [E, K], both bf16 or both fp16; float32 sums, nothing rounded.
+    Rows of x may lie apart.  K % 8 == 0."""
+    out = host.router_logits(x, weight)
+    if out is not None:
+        return out
+    rows = _rows_view(x, "x")
+    _cuda_contig(weight, "weight")
+    _same_device(x, weight=weight)
+    if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or weight.dtype != x.dtype or weight.shape[0] == 0:
+        raise RuntimeError(f"router_logits: weight {tuple(weight.shape)} {weight.dtype} for x [..., {x.shape[-1]}] {x.dtype}")
+    dt = _dt(x)
+    with torch.cuda.device(x.device):
+        y = torch.empty(x.shape[:-1] + (weight.shape[0],), device=x.device, dtype=torch.float32)
+        check(lib.sglb200_router_logits(rows.data_ptr(), weight.data_ptr(), dt, y.data_ptr(), rows.shape[0], weight.shape[0],
+                                        x.shape[-1], _row_stride(rows), _stream(x)))
+    return y
+
+
+def route_topk(
+    gating_output: torch.Tensor, topk: int, scoring_func: str = "softmax", correction_bias: Optional[torch.Tensor] = None,
+    num_expert_group: int = 1, topk_group: int = 1, group_top: Optional[int] = None, renormalize: bool = True,
+    routed_scaling_factor: float = 1.0,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Experts and weights from the router's logits [T, E] (bf16, fp16, fp32) -> (float32 [T, topk], int32 [T, topk]), best first.
+
+    s = softmax or sigmoid of the logits, c = s + correction_bias (float32 [E]).  The experts form `num_expert_group` equal groups; a
+    group's value is the sum of its `group_top` (1 or 2; None: 2 with a bias, else 1) largest c, and the `topk` largest c of the
+    `topk_group` best groups are picked.  Weights are s, divided by the picks' sum if `renormalize`, times `routed_scaling_factor`.
+
+    The order is that of the real numbers, whatever the logits' type; ties go to the lower index.  An expert whose logit is NaN or -inf
+    (or whose bias is NaN or -inf) is not available; a slot for which none is left has the id -1 and the weight 0, which the experts'
+    operators skip.  topk and num_expert_group at most 32."""
+    if scoring_func not in ("softmax", "sigmoid"):
+        raise RuntimeError(f"route_topk: scoring_func must be 'softmax' or 'sigmoid', not {scoring_func!r}")
+    if group_top is None:
+        group_top = 1 if correction_bias is None else 2
+    out = host.route_topk(gating_output, topk, scoring_func == "softmax", correction_bias, num_expert_group, topk_group, group_top,
+                          renormalize, routed_scaling_factor)
+    if out is not None:
+        return out
+    _cuda_contig(gating_output, "gating_output")
+    if gating_output.dim() != 2:
+        raise RuntimeError("route_topk: gating_output must be [tokens, experts]")
+    rows, experts = gating_output.shape
+    dt, bias = _dt(gating_output, _GATE_DT), _gate_bias(correction_bias, experts, "route_topk")
+    _same_device(gating_output, correction_bias=correction_bias)
+    for n, v, most in (("topk", topk, experts), ("num_expert_group", num_expert_group, experts), ("topk_group", topk_group, num_expert_group),
+                       ("group_top", group_top, 2)):
+        if not 1 <= v <= most:
+            raise RuntimeError(f"route_topk: {n} is {v}, not one of 1 to {most}")
+    with torch.cuda.device(gating_output.device):
+        w = torch.empty(rows, topk, dtype=torch.float32, device=gating_output.device)
+        ids = torch.empty(rows, topk, dtype=torch.int32, device=gating_output.device)
+        check(lib.sglb200_route_topk(gating_output.data_ptr(), dt, rows, experts, int(topk), int(scoring_func == "softmax"), bias,
+                                     int(num_expert_group), int(topk_group), int(group_top), int(bool(renormalize)),
+                                     float(routed_scaling_factor), w.data_ptr(), ids.data_ptr(), _stream(gating_output)))
+    return w, ids
+
+
 def gather_rows_fp8(
     src_q: torch.Tensor, src_s: torch.Tensor, sorted_token_ids: torch.Tensor, num_rows: torch.Tensor,
     numel: int, topk: int, max_rows: Optional[int] = None,
@@ -552,6 +643,63 @@ def w4a4_group_fp4_matmul(
             bias.data_ptr() if bias is not None else None, M, N, K, group, 0 if output_dtype == torch.bfloat16 else 1,
             _stream(A)))
     return C
+
+
+def lora_add(
+    base: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapter_ids: torch.Tensor,
+    scalings: Optional[torch.Tensor] = None, ranks: Optional[torch.Tensor] = None, slices: Optional[Tuple[int, ...]] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Low-rank adapters of many requests beside a shared projection:
+
+        out[t] = base[t] + scalings[l] * lora_b[l] (lora_a[l] x[t]),   l = adapter_ids[t]
+
+    x [..., K], base [..., N] (the projection's output), both bf16 or both fp16, rows any distance apart; adapter_ids int32 [...], an
+    id outside [0, L): out = base.  lora_a [L, S * R, K], lora_b [L, N, R] of the same type: of S merged projections (`slices`, their
+    columns; None: one), the first takes rows 0 .. R - 1 of lora_a[l], and so on.  scalings float32 [L] (None: 1); ranks int32 [L]:
+    only that many rows (of each R) and columns of an adapter count (None: R).  `out` may be `base`; None: a new tensor.
+    Sums in float32, one rounding.  R % 8 == 0, at most 256; at most 1024 adapters and 8 slices; K % 8 == 0."""
+    got = host.lora_add(base, x, lora_a, lora_b, adapter_ids, scalings, ranks, slices, out)
+    if got is not None:
+        return got
+    xr, br = _rows_view(x, "x"), _rows_view(base, "base")
+    for t, n in ((lora_a, "lora_a"), (lora_b, "lora_b"), (adapter_ids, "adapter_ids")):
+        _cuda_contig(t, n)
+    _same_device(x, base=base, lora_a=lora_a, lora_b=lora_b, adapter_ids=adapter_ids, scalings=scalings, ranks=ranks, out=out)
+    dt = _dt(x)
+    for t, n in ((base, "base"), (lora_a, "lora_a"), (lora_b, "lora_b")):
+        if t.dtype != x.dtype:
+            raise RuntimeError(f"lora_add: {n} is {t.dtype}, x is {x.dtype}")
+    if base.shape[:-1] != x.shape[:-1]:
+        raise RuntimeError(f"lora_add: base {tuple(base.shape)} and x {tuple(x.shape)} have different rows")
+    T, K, N = xr.shape[0], x.shape[-1], base.shape[-1]
+    if lora_a.dim() != 3 or lora_b.dim() != 3 or lora_a.shape[2] != K or lora_b.shape[:2] != (lora_a.shape[0], N):
+        raise RuntimeError(f"lora_add: lora_a {tuple(lora_a.shape)} and lora_b {tuple(lora_b.shape)} do not fit K {K}, N {N}")
+    L, _, R = lora_b.shape
+    sizes = (N,) if slices is None else tuple(int(n) for n in slices)
+    if L == 0 or R == 0 or not sizes or lora_a.shape[1] != len(sizes) * R or sum(sizes) != N or min(sizes) < 1:
+        raise RuntimeError(f"lora_add: lora_a {tuple(lora_a.shape)} and slices {sizes} do not fit rank {R}, N {N}")
+    if adapter_ids.dtype != torch.int32 or adapter_ids.numel() != T:
+        raise RuntimeError(f"lora_add: adapter_ids must be {T} int32")
+    for t, n, d in ((scalings, "scalings", torch.float32), (ranks, "ranks", torch.int32)):
+        if t is not None and (not t.is_contiguous() or t.dtype != d or t.numel() != L):
+            raise RuntimeError(f"lora_add: {n} must be {L} contiguous {d}")
+    with torch.cuda.device(x.device):
+        if out is None:
+            out = torch.empty(base.shape, device=x.device, dtype=x.dtype)
+        orows = _rows_view(out, "out")
+        if out.dtype != x.dtype or out.shape != base.shape:
+            raise RuntimeError(f"lora_add: out {tuple(out.shape)} {out.dtype} is not like base")
+        if T == 0:
+            return out
+        bytes_ = lib.sglb200_lora_add_workspace_bytes(T, L, R, len(sizes))
+        ws = torch.empty(bytes_, device=x.device, dtype=torch.uint8)
+        check(lib.sglb200_lora_add(
+            xr.data_ptr(), lora_a.data_ptr(), lora_b.data_ptr(), br.data_ptr(), orows.data_ptr(), dt, adapter_ids.data_ptr(),
+            scalings.data_ptr() if scalings is not None else None, ranks.data_ptr() if ranks is not None else None, T, L, R, N, K,
+            _row_stride(xr), _row_stride(br), _row_stride(orows), len(sizes), (ctypes.c_int64 * len(sizes))(*sizes), ws.data_ptr(),
+            bytes_, _stream(x)))
+    return out
 
 
 def grouped_block_fp8_matmul(

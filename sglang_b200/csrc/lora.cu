@@ -2,7 +2,7 @@
 //   out[t, n] = rnd( base[t, n] + scaling[l] * sum_{r < rank[l]} B[l, n, r] h[t, s(n) R + r] ),   h[t, j] = sum_k x[t, k] A[l, j, k],
 // l the adapter that token t names (none: out = base) and s(n) the merged projection that column n belongs to.
 //
-// Three launches with programmatic serialization.  plan_kernel sorts the tokens by adapter into blocks of up to 64 (narrow.cuh).  The
+// Three launches with programmatic serialization.  plan_kernel sorts the tokens by adapter into blocks (narrow.cuh).  The
 // narrow product gives h in float32, in that order.  expand_kernel adds the second product.
 //
 // h keeps 16 bits and more in the second product: the row's values times a power of two that brings the largest to [1, 2) (float16 would
@@ -17,7 +17,6 @@
 namespace sglb200 {
 namespace lora {
 
-constexpr int kBlock = narrow::kBlock;
 constexpr int kMaxAdapters = 1024;
 constexpr int kMaxSlices = 8;
 constexpr int kMaxRank = 256;
@@ -27,8 +26,8 @@ constexpr int kPlanThreads = 1024;
 
 // One CTA.  Tokens of one adapter in any order: their rows do not meet.  Neighbours mostly name the same adapter, so that a warp counts
 // equal ids at once.
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __restrict__ ids, int T, int L, int32_t* order, int32_t* start,
-                                                            int32_t* rows, int32_t* adapter, int32_t* count) {
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __restrict__ ids, int T, int L, int block, int32_t* order,
+                                                            int32_t* start, int32_t* rows, int32_t* adapter, int32_t* count) {
   __shared__ int32_t cursor[kMaxAdapters + 1];
   const int tid = threadIdx.x, lane = tid & 31;
   for (int i = tid; i <= L; i += kPlanThreads) cursor[i] = 0;
@@ -46,7 +45,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __res
   if (tid < 32) {  // first token and first block of every adapter
     int tokens = 0, blocks = 0;
     for (int at = 0; at <= L; at += 32) {
-      const int l = at + lane, n = l <= L ? cursor[l] : 0, b = (n + kBlock - 1) / kBlock;
+      const int l = at + lane, n = l <= L ? cursor[l] : 0, b = (n + block - 1) / block;
       int sn = n, sb = b;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
@@ -56,8 +55,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __res
       if (l <= L) {
         for (int i = 0; i < b; ++i) {
           const int at_block = blocks + sb - b + i;
-          start[at_block] = tokens + sn - n + i * kBlock;
-          rows[at_block] = min(kBlock, n - i * kBlock);
+          start[at_block] = tokens + sn - n + i * block;
+          rows[at_block] = min(block, n - i * block);
           adapter[at_block] = l < L ? l : -1;
         }
         cursor[l] = tokens + sn - n;
@@ -91,7 +90,7 @@ struct Params {
   const int32_t* ranks;   // or nullptr
   narrow::Blocks blocks;
   int64_t N, ld_base, ld_out;
-  int R, S, max_blocks, passes, vec, in_place, pitch;
+  int R, S, block, max_blocks, passes, vec, in_place, pitch;
   int64_t col0[kMaxSlices + 1];  // first column of every merged projection, and the end
   int chunk0[kMaxSlices + 1];    // the first chunk of passes x 8 warps x columns of a warp, and the end
 };
@@ -144,9 +143,9 @@ __device__ __forceinline__ float split_row(const float* h, int used, float scali
 template <typename T, int kSteps, int kTiles>
 __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
   constexpr int kCols = 8 * kTiles, kMine = 2 * kTiles;
-  extern __shared__ __align__(16) uint8_t tile[];  // [kBlock][pitch]: a token's high terms, then its low terms
-  __shared__ float unscale[kBlock];
-  __shared__ int32_t token[kBlock];
+  extern __shared__ __align__(16) uint8_t tile[];  // [rows of a block][pitch]: a token's high terms, then its low terms
+  __shared__ float unscale[narrow::kTileBlock];
+  __shared__ int32_t token[narrow::kTileBlock];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
   const int block = (int)(blockIdx.x % p.max_blocks);
   const int chunk = (int)(blockIdx.x / p.max_blocks);
@@ -293,7 +292,7 @@ static int launch_expand(Params& p, cudaStream_t st) {
   p.chunk0[p.S] = chunks;
   // rows 32 bytes apart modulo 128: four rows of 32 bytes are read without a bank conflict
   p.pitch = (4 * p.R + 127) / 128 * 128 + 32;
-  const size_t smem = (size_t)kBlock * p.pitch;
+  const size_t smem = (size_t)p.block * p.pitch;
   SGLB_REQUIRE((int64_t)chunks * p.max_blocks < (1ll << 31), "lora_add: %lld tiles are too many", (long long)chunks * p.max_blocks);
   auto kern = expand_kernel<T, kSteps, kTiles>;
   if (smem > 48 * 1024) {
@@ -301,7 +300,7 @@ static int launch_expand(Params& p, cudaStream_t st) {
     int dev = 0;
     SGLB_CUDA(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-      SGLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBlock * (4 * kMaxRank + 160)));
+      SGLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, narrow::kTileBlock * (4 * kMaxRank + 160)));
       if (dev >= 0 && dev < 64) attr_set[dev] = true;
     }
   }
@@ -318,7 +317,7 @@ static int expand(Params& p, cudaStream_t st) {
   return launch_expand<T, 16, 2>(p, st);
 }
 
-static int64_t most_blocks(int64_t T, int L) { return T / kBlock + (T < L + 1 ? T : L + 1); }
+static int64_t most_blocks(int64_t T, int L, int block) { return T / block + (T < L + 1 ? T : L + 1); }
 static int64_t up(int64_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace lora
@@ -328,7 +327,8 @@ using namespace sglb200;
 
 extern "C" int64_t sglb200_lora_add_workspace_bytes(int64_t tokens, int num_adapters, int rank, int num_slices) {
   if (tokens <= 0 || num_adapters < 1 || rank < 1 || num_slices < 1) return 0;
-  const int64_t blocks = lora::most_blocks(tokens, num_adapters);
+  // (whichever blocks the call takes)
+  const int64_t blocks = lora::most_blocks(tokens, num_adapters, narrow::kSmallBlock);
   return lora::up(4 * tokens) + lora::up(4 * (3 * blocks + 1)) + lora::up(4 * tokens * num_slices * rank);
 }
 
@@ -369,21 +369,22 @@ extern "C" int sglb200_lora_add(const void* x, const void* lora_a, const void* l
   const int64_t bytes = sglb200_lora_add_workspace_bytes(tokens, num_adapters, rank, num_slices);
   if (workspace == nullptr || workspace_bytes < bytes || !aligned16(workspace))
     return fail(SGLB200_E_WORKSPACE, "lora_add: %lld bytes of workspace are needed, aligned to 16", (long long)bytes);
-  const int64_t blocks = lora::most_blocks(tokens, num_adapters);
+  const int block = narrow::block_rows(tokens, (int64_t)num_slices * rank, K, num_adapters);
+  const int64_t blocks = lora::most_blocks(tokens, num_adapters, block);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int32_t* order = static_cast<int32_t*>(workspace);
   int32_t* start = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + lora::up(4 * tokens));
   float* h = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(start) + lora::up(4 * (3 * blocks + 1)));
   p.blocks = {order, start, start + blocks, start + 2 * blocks, start + 3 * blocks};
-  SGLB_CUDA(launch_pdl(lora::plan_kernel, 1u, (unsigned)lora::kPlanThreads, (size_t)0, st, adapter_ids, (int)tokens, num_adapters, order, start,
+  SGLB_CUDA(launch_pdl(lora::plan_kernel, 1u, (unsigned)lora::kPlanThreads, (size_t)0, st, adapter_ids, (int)tokens, num_adapters, block, order, start,
                        start + blocks, start + 2 * blocks, start + 3 * blocks));
   narrow::Params n{};
   n.x = x, n.w = lora_a, n.y = h, n.ranks = ranks, n.blocks = p.blocks;
-  n.T = tokens, n.N = (int64_t)num_slices * rank, n.K = K, n.ldx = x_stride, n.rank_rows = rank;
+  n.T = tokens, n.N = (int64_t)num_slices * rank, n.K = K, n.ldx = x_stride, n.rank_rows = rank, n.adapters = num_adapters, n.block = block;
   int rc = narrow::product(n, dtype, blocks, st);
   if (rc) return rc;
   p.b = lora_b, p.base = base, p.out = out, p.h = h, p.scalings = scalings, p.ranks = ranks;
-  p.N = N, p.ld_base = base_stride, p.ld_out = out_stride, p.R = rank, p.S = num_slices, p.max_blocks = (int)blocks;
+  p.N = N, p.ld_base = base_stride, p.ld_out = out_stride, p.R = rank, p.S = num_slices, p.block = block, p.max_blocks = (int)blocks;
   p.in_place = base == out && base_stride == out_stride;
   p.vec = even && N % 8 == 0 && base_stride % 8 == 0 && out_stride % 8 == 0 && aligned16(base) && aligned16(out);
   return dtype == 0 ? lora::expand<__nv_bfloat16>(p, st) : lora::expand<__half>(p, st);

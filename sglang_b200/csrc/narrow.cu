@@ -39,8 +39,8 @@ __global__ void __launch_bounds__(kWarps * 32) narrow_kernel(const Params p) {
   const int64_t block = blockIdx.x / p.splits / p.n_tiles;
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
-  int64_t start = block * kBlock, adapter = 0;
-  int rows = (int)min((int64_t)kBlock, p.T - start);
+  int64_t start = block * kSmallBlock, adapter = 0;
+  int rows = (int)min((int64_t)kSmallBlock, p.T - start);
   if (p.blocks.order != nullptr) {  // (uniform over the cluster)
     if (block >= *p.blocks.count) return;
     start = p.blocks.start[block], rows = p.blocks.rows[block], adapter = p.blocks.adapter[block];
@@ -146,7 +146,13 @@ static int dispatch(Params& p, int64_t blocks, cudaStream_t st) {
   return launch<T, 8>(p, blocks, st);
 }
 
+#ifndef NARROW_TILE_FROM
+#define NARROW_TILE_FROM 129
+#endif
+int block_rows(int64_t T, int64_t N, int64_t K, int64_t adapters) { return T < NARROW_TILE_FROM ? kSmallBlock : kTileBlock; }
+
 int product(Params p, int dtype, int64_t max_blocks, cudaStream_t st) {
+  if (p.block == kTileBlock) return tile_product(p, dtype, max_blocks, st);
   return dtype == 0 ? dispatch<__nv_bfloat16>(p, max_blocks, st) : dispatch<__half>(p, max_blocks, st);
 }
 
@@ -169,5 +175,6 @@ extern "C" int sglb200_router_logits(const void* x, const void* w, int dtype, fl
   SGLB_REQUIRE(aligned16(x) && aligned16(w) && aligned16(y), "router_logits: pointers must be 16-byte aligned");
   narrow::Params p{};
   p.x = x, p.w = w, p.y = y, p.T = tokens, p.N = num_experts, p.K = K, p.ldx = x_stride, p.rank_rows = (int)num_experts;
-  return narrow::product(p, dtype, (tokens + narrow::kBlock - 1) / narrow::kBlock, static_cast<cudaStream_t>(stream));
+  p.adapters = 1, p.block = narrow::block_rows(tokens, num_experts, K, 1);
+  return narrow::product(p, dtype, (tokens + p.block - 1) / p.block, static_cast<cudaStream_t>(stream));
 }

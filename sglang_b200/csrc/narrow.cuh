@@ -5,8 +5,8 @@
 namespace sglb200 {
 namespace narrow {
 
-// Rows that share their weights come in blocks of up to kBlock.
-constexpr int kBlock = 64;
+// Rows that share their weights come in blocks: of 64 of them for narrow_kernel, of 128 for narrow_tile_kernel.
+constexpr int kSmallBlock = 64, kTileBlock = 128;
 
 // What the rows of a batch are sorted into: `order` the rows by adapter, then per block where it starts in the order, its rows and its
 // adapter (-1: rows that name none, behind the others); `count` the number of blocks.
@@ -25,12 +25,22 @@ struct Params {
   const int32_t* ranks;  // per adapter or nullptr: of every `rank_rows` rows of w the first ranks[adapter] count, the others give 0
   Blocks blocks;
   int64_t T, N, K, ldx;
+  int64_t adapters;
   int rank_rows;
+  int block;           // rows of a block
   int n_tiles, splits;
 };
 
-// y = x w^T, `max_blocks` the most blocks there can be.
+// Rows of a block for T rows and N weight rows of each of `adapters` adapters.
+int block_rows(int64_t T, int64_t N, int64_t K, int64_t adapters);
+
+// y = x w^T in blocks of p.block rows, `max_blocks` the most blocks there can be.
 int product(Params p, int dtype, int64_t max_blocks, cudaStream_t st);
+
+// narrow_tile.cu: the same for many rows; a status word as gemm_rows.cu's, and its reset.
+int tile_product(const Params& p, int dtype, int64_t max_blocks, cudaStream_t st);
+int tile_status();
+int tile_status_clear();
 
 }  // namespace narrow
 }  // namespace sglb200

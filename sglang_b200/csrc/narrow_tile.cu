@@ -1,0 +1,316 @@
+// y[t, n] = sum_k x[t, k] w[n, k] for many rows (see narrow.cuh), on tcgen05.mma.kind::f16.
+//
+// A tile is 128 activation rows by up to 256 weight rows; both operands come by TMA in stages of 64 columns, the activations of sorted rows
+// by gathers of four.  K is split over the CTAs of a cluster, which add their sums through distributed shared memory in a fixed order.
+//
+// The instruction cuts off what does not fit its sum, each time: over 7168 columns that would be off by more than a float32 product is.  So
+// the sums of 256 columns begin from zero, in two buffers of tensor memory in turn, and meet in the registers of eight warps.
+#include <algorithm>
+
+#include "gemm_common.cuh"
+#include "narrow.cuh"
+#include "ptx_sm100.cuh"
+
+namespace sglb200 {
+namespace narrow {
+
+__device__ int g_tile_status = 0;  // 0 ok, 1 = a pipeline wait expired
+
+constexpr int kThreads = 320;      // eight warps for the sums, one that loads, one that multiplies
+constexpr int kStageK = 64;        // columns of a stage: 128 bytes, one swizzle span
+constexpr int kChunk = 4;          // stages that are summed up in tensor memory
+constexpr int kMaxStages = 8;
+constexpr uint32_t kRing = 192 * 1024;
+constexpr uint32_t kXBytes = kTileBlock * kStageK * 2;
+
+struct Ctl {
+  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+struct TileParams {
+  Params p;
+  int nt;        // weight rows of a tile, a multiple of 16
+  int stages, kb_total, fp16;
+  uint32_t wait_probes;
+};
+
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);  // rows of 128 bytes, 128-byte swizzle
+__device__ __forceinline__ uint32_t desc_lo(uint32_t smem) { return ((smem & 0x3ffffu) >> 4) | (1u << 16); }
+
+// f32 += bf16 x bf16 (1) or f16 x f16 (0), both operands K-major.
+__device__ __forceinline__ uint32_t idesc(int n, int fp16) {
+  const uint32_t type = fp16 ? 0u : 1u;
+  return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTileBlock >> 4) << 24);
+}
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\t"
+               "setp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate)
+               : "memory");
+}
+
+#define NARROW_WAIT(bar, parity) \
+  (t.wait_probes != ptx::kProbesNone && (ptx::mbar_test(bar, parity) || ptx::mbar_wait_quiet(bar, parity)))
+
+// kUnits: groups of 16 columns of a tile that each of the two warpgroups adds up, at most.
+template <int kUnits>
+__global__ void __launch_bounds__(kThreads, 1)
+    narrow_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const TileParams t) {
+  constexpr uint32_t kBuf = kUnits * 32;  // columns of tensor memory of a buffer
+  const Params& p = t.p;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Ctl* ctl = reinterpret_cast<Ctl*>(ring + kRing);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int* abort_flag = &ctl->abort_flag;
+  const int rank = (int)(blockIdx.x % p.splits), n0 = (int)(blockIdx.x / p.splits % p.n_tiles) * t.nt;
+  const int64_t block = blockIdx.x / p.splits / p.n_tiles;
+  const uint32_t full = ptx::smem_u32(ctl->full), empty = ptx::smem_u32(ctl->empty), acc_full = ptx::smem_u32(ctl->acc_full),
+                 acc_empty = ptx::smem_u32(ctl->acc_empty);
+  if (tid == 0) {
+    for (int s = 0; s < t.stages; ++s) ptx::mbar_init(full + s * 8, 1), ptx::mbar_init(empty + s * 8, 1);
+    for (int b = 0; b < 2; ++b) ptx::mbar_init(acc_full + b * 8, 1), ptx::mbar_init(acc_empty + b * 8, 8);
+    ctl->abort_flag = 0;
+    ptx::mbar_fence_init();
+  }
+  // (tensor memory is taken once the kernel in front has ended; the kernel behind may start when every CTA has its own)
+  ptx::grid_dependency_wait();
+  int64_t start = block * kTileBlock;
+  int rows = (int)min((int64_t)kTileBlock, p.T - start), adapter = 0;
+  if (p.blocks.order != nullptr) {
+    const bool there = block < __ldcg(p.blocks.count);  // (uniform over the cluster)
+    adapter = there ? __ldcg(p.blocks.adapter + block) : -1;
+    if (adapter < 0) {
+      ptx::launch_dependents();
+      return;
+    }
+    start = __ldcg(p.blocks.start + block), rows = __ldcg(p.blocks.rows + block);
+  }
+  if (warp == 9) {
+    ptx::tmem_alloc(ptx::smem_u32(&ctl->tmem_base), 2 * kBuf);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  ptx::launch_dependents();
+  const uint32_t tmem = ctl->tmem_base;
+  const int kb0 = (int)((int64_t)rank * t.kb_total / p.splits), kb1 = (int)((int64_t)(rank + 1) * t.kb_total / p.splits);
+  const uint32_t w_bytes = (uint32_t)t.nt * kStageK * 2, stage_bytes = kXBytes + w_bytes, base = ptx::smem_u32(ring);
+  const int units = t.nt / 16, half = (units + 1) / 2;
+
+  if (warp == 8) {
+    const bool gather = p.blocks.order != nullptr;
+    int r[4];
+    if (gather)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = __ldcg(p.blocks.order + start + min(lane * 4 + i, rows - 1));
+    const bool mine = lane * 4 < rows;  // (rows past the last hold what they held; their sums are nobody's)
+    const uint32_t x_bytes = gather ? (uint32_t)((rows + 3) / 4 * 4) * kStageK * 2 : kXBytes;
+    for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+      const int s = i % t.stages;
+      bool ok = true;
+      if (i >= t.stages) ok = NARROW_WAIT(empty + s * 8, ((i / t.stages) & 1) ^ 1);
+      if (!__all_sync(0xffffffffu, ok)) {
+        if (lane == 0) *abort_flag = 1;
+        break;
+      }
+      const uint32_t at = base + s * stage_bytes, bar = full + s * 8;
+      if (lane == 0) {
+        ptx::mbar_arrive_expect_tx(bar, x_bytes + w_bytes);
+        ptx::tma_load_3d(at + kXBytes, &map_w, bar, kb * kStageK * 2, n0, adapter);
+        if (!gather) ptx::tma_load_2d(at, &map_x, bar, kb * kStageK * 2, (int)start);
+      }
+      __syncwarp();
+      if (gather && mine) ptx::tma_gather4(at + lane * (4 * kStageK * 2), &map_x, bar, kb * kStageK * 2, r[0], r[1], r[2], r[3]);
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    if (ptx::elect_one()) {
+      const uint32_t id = idesc(t.nt, t.fp16);
+      bool ok = true;
+      for (int kb = kb0, i = 0; kb < kb1 && ok; ++kb, ++i) {
+        const int s = i % t.stages, chunk = i / kChunk, buf = chunk & 1;
+        if (i % kChunk == 0 && chunk >= 2) ok = NARROW_WAIT(acc_empty + buf * 8, ((chunk >> 1) & 1) ^ 1);
+        if (ok) ok = NARROW_WAIT(full + s * 8, (i / t.stages) & 1);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        const uint32_t at = base + s * stage_bytes, x_lo = desc_lo(at), w_lo = desc_lo(at + kXBytes);
+#pragma unroll
+        for (int k = 0; k < kStageK / 16; ++k)
+          mma_f16(tmem + buf * kBuf, ptx::pack_f32x2(x_lo + 2 * k, kDescHi), ptx::pack_f32x2(w_lo + 2 * k, kDescHi), id,
+                  i % kChunk > 0 || k > 0 ? 1u : 0u);
+        ptx::mma_commit(empty + s * 8);
+        if (i % kChunk == kChunk - 1 || kb + 1 == kb1) ptx::mma_commit(acc_full + buf * 8);
+      }
+      if (!ok) *abort_flag = 1;
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------ sums: lane = activation row, column = weight row ------------------------------
+    float acc[kUnits * 16];
+#pragma unroll
+    for (int j = 0; j < kUnits * 16; ++j) acc[j] = 0.f;
+    const int first = warp < 4 ? 0 : half, mine = warp < 4 ? half : units - half;
+    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) * 32 << 16) + first * 16;
+    const int chunks = (kb1 - kb0 + kChunk - 1) / kChunk;
+    bool ok = true;
+    for (int c = 0; c < chunks; ++c) {
+      ok = NARROW_WAIT(acc_full + (c & 1) * 8, (c >> 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      ptx::tc_fence_after();
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        if (u >= mine) break;
+        uint32_t v[16];
+        ptx::tmem_ld_32x16(lanes + (c & 1) * kBuf + u * 16, v);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[u * 16 + j] += __uint_as_float(v[j]);
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(acc_empty + (c & 1) * 8);
+    }
+    if (!ok) {
+      *abort_flag = 1;
+    } else {  // the operands have been consumed
+      float* part = reinterpret_cast<float*>(ring) + ((warp & 3) * 32 + lane) * (t.nt + 4) + first * 16;
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        if (u >= mine) break;
+#pragma unroll
+        for (int j = 0; j < 16; j += 4)
+          *reinterpret_cast<float4*>(part + u * 16 + j) = make_float4(acc[u * 16 + j], acc[u * 16 + j + 1], acc[u * 16 + j + 2], acc[u * 16 + j + 3]);
+      }
+    }
+  }
+  __syncwarp();
+  if (p.splits > 1) ptx::cluster_sync(); else __syncthreads();
+  if (ctl->abort_flag == 0) {
+    // The CTAs' sums in ascending order of K; each CTA adds up its share of the rows.
+    const int row0 = rank * rows / p.splits, row1 = (rank + 1) * rows / p.splits, quads = t.nt / 4;
+    const bool vec = p.N % 4 == 0;
+    for (int i = tid; i < (row1 - row0) * quads; i += kThreads) {
+      const int row = row0 + i / quads, c = i % quads * 4;
+      if (n0 + c >= p.N) continue;
+      const uint32_t at = base + (uint32_t)(row * (t.nt + 4) + c) * 4;
+      float4 sum = ptx::lds_f32x4(at);
+      if (p.splits > 1) {
+        float4 v[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          if (s < p.splits)
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v[s].x), "=f"(v[s].y), "=f"(v[s].z), "=f"(v[s].w)
+                         : "r"(ptx::cluster_map(at, s))
+                         : "memory");
+        sum = v[0];
+#pragma unroll
+        for (int s = 1; s < 8; ++s)
+          if (s < p.splits) sum.x += v[s].x, sum.y += v[s].y, sum.z += v[s].z, sum.w += v[s].w;
+      }
+      float* to = p.y + (start + row) * p.N + n0 + c;
+      if (vec) {
+        *reinterpret_cast<float4*>(to) = sum;
+      } else {
+        const float one[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n0 + c + j < p.N) to[j] = one[j];
+      }
+    }
+  }
+  if (p.splits > 1) ptx::cluster_sync();  // no CTA leaves while another reads its shared memory
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (ctl->abort_flag != 0 && tid == 0) {
+    atomicExch(&g_tile_status, 1);
+    // give copies that may still be in flight time to land before the CTA's shared memory is released
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000ll) {
+    }
+  }
+  __syncthreads();
+  if (warp == 9) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, 2 * kBuf);
+  }
+}
+
+template <int kUnits>
+static int launch(const CUtensorMap& mx, const CUtensorMap& mw, const TileParams& t, int64_t blocks, cudaStream_t st) {
+  constexpr size_t kSmem = 1024 + kRing + sizeof(Ctl);
+  static_assert(kSmem <= 227 * 1024);
+  auto kern = narrow_tile_kernel<kUnits>;
+  static thread_local bool attr_set[64] = {false};  // the opt-in is per function and per device
+  int dev = 0;
+  SGLB_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    SGLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  const int64_t grid = blocks * t.p.n_tiles * t.p.splits;
+  SGLB_REQUIRE(grid < (1ll << 31), "narrow product: %lld tiles are too many", (long long)grid);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid, 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)t.p.splits, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  SGLB_CUDA(cudaLaunchKernelEx(&cfg, kern, mx, mw, t));
+  return SGLB200_OK;
+}
+
+int tile_product(const Params& given, int dtype, int64_t max_blocks, cudaStream_t st) {
+  TileParams t{};
+  t.p = given;
+  Params& p = t.p;
+  t.kb_total = (int)((p.K + kStageK - 1) / kStageK), t.fp16 = dtype, t.wait_probes = g_gemm_wait_probes;
+  // Up to 256 weight rows a tile, so that the activations are fetched once; fewer where there are few tiles, down to 32.
+  const ClusterFits& fits = cluster_fits();
+  int64_t n_tiles = (p.N + 255) / 256;
+  while (max_blocks * n_tiles * 8 <= fits.alone[1] && p.N > n_tiles * 32) n_tiles *= 2;
+  t.nt = (int)(((p.N + n_tiles - 1) / n_tiles + 15) / 16 * 16);
+  p.n_tiles = (int)((p.N + t.nt - 1) / t.nt);
+  const int64_t tiles = max_blocks * p.n_tiles;
+  p.splits = 1;
+  for (int s = 2; s <= 8; ++s)  // as many CTAs as run at once
+    if (tiles <= fits.alone[s] && t.kb_total >= s * kChunk) p.splits = s;
+  t.stages = (int)std::min<uint32_t>(kMaxStages, kRing / (kXBytes + (uint32_t)t.nt * kStageK * 2));
+  CUtensorMap mx, mw;
+  const bool gather = p.blocks.order != nullptr;
+  const uint64_t xd[2] = {(uint64_t)p.K * 2, (uint64_t)p.T}, xs[1] = {(uint64_t)p.ldx * 2};
+  const uint32_t xb[2] = {kStageK * 2, gather ? 1u : (uint32_t)kTileBlock};
+  int rc = get_tile_map(p.x, 2, xd, xs, xb, true, &mx);
+  if (rc) return rc;
+  const uint64_t wd[3] = {(uint64_t)p.K * 2, (uint64_t)p.N, (uint64_t)p.adapters}, ws[2] = {(uint64_t)p.K * 2, (uint64_t)(p.N * p.K * 2)};
+  const uint32_t wb[3] = {kStageK * 2, (uint32_t)t.nt, 1};
+  rc = get_tile_map(p.w, 3, wd, ws, wb, true, &mw);
+  if (rc) return rc;
+  if (t.nt <= 64) return launch<2>(mx, mw, t, max_blocks, st);
+  if (t.nt <= 128) return launch<4>(mx, mw, t, max_blocks, st);
+  return launch<8>(mx, mw, t, max_blocks, st);
+}
+
+int tile_status() {
+  int v = 0;
+  return cudaMemcpyFromSymbol(&v, g_tile_status, sizeof(int)) != cudaSuccess ? -1 : v;
+}
+int tile_status_clear() {
+  const int zero = 0;
+  SGLB_CUDA(cudaMemcpyToSymbol(g_tile_status, &zero, sizeof(int)));
+  return SGLB200_OK;
+}
+
+}  // namespace narrow
+}  // namespace sglb200

@@ -2,8 +2,8 @@
 //   out[t, n] = rnd( base[t, n] + scaling[l] * sum_{r < rank[l]} B[l, n, r] h[t, s(n) R + r] ),   h[t, j] = sum_k x[t, k] A[l, j, k],
 // l the adapter that token t names (none: out = base) and s(n) the merged projection that column n belongs to.
 //
-// Three launches with programmatic serialization.  plan_kernel sorts the tokens by adapter into blocks (narrow.cuh).  The
-// narrow product gives h in float32, in that order.  expand_kernel adds the second product.
+// Up to three launches with programmatic serialization.  plan_kernel sorts the tokens by adapter into blocks (narrow.cuh); up to 64 tokens
+// need none.  The narrow product gives h in float32.  expand_kernel adds the second product.
 //
 // h keeps 16 bits and more in the second product: the row's values times a power of two that brings the largest to [1, 2) (float16 would
 // overflow or lose small ones without it) enter as two 16-bit terms, 16 bits of bfloat16 or 22 of float16; the weights are what they are.
@@ -85,12 +85,13 @@ struct Params {
   const void* b;     // [L, N, R]
   const void* base;  // [T, N], rows ld_base apart
   void* out;         // rows ld_out apart; may be base
-  const float* h;    // [T, S R], in the blocks' order
+  const float* h;    // [T, S R]
   const float* scalings;  // or nullptr
   const int32_t* ranks;   // or nullptr
   narrow::Blocks blocks;
   int64_t N, ld_base, ld_out;
-  int R, S, block, max_blocks, passes, vec, in_place, pitch;
+  int R, S, max_blocks, passes, vec, in_place, pitch;
+  int sub, subs;     // rows of a block that a CTA takes, CTAs of a block
   int64_t col0[kMaxSlices + 1];  // first column of every merged projection, and the end
   int chunk0[kMaxSlices + 1];    // the first chunk of passes x 8 warps x columns of a warp, and the end
 };
@@ -139,21 +140,36 @@ __device__ __forceinline__ float split_row(const float* h, int used, float scali
 }
 
 // kSteps: instructions over the rank, at most; kTiles: groups of 8 columns of a warp.  A lane holds the same two kTiles neighbouring columns
-// of a token in all groups, so that base and out go by 4 kTiles bytes.
+// of a token in all groups, so that base and out go by 4 kTiles bytes.  A warp asks for the next 16 tokens' base before it multiplies these.
 template <typename T, int kSteps, int kTiles>
 __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
   constexpr int kCols = 8 * kTiles, kMine = 2 * kTiles;
-  extern __shared__ __align__(16) uint8_t tile[];  // [rows of a block][pitch]: a token's high terms, then its low terms
+  extern __shared__ __align__(16) uint8_t tile[];  // [rows of a CTA][pitch]: a token's high terms, then its low terms
   __shared__ float unscale[narrow::kTileBlock];
   __shared__ int32_t token[narrow::kTileBlock];
+  __shared__ int found[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
-  const int block = (int)(blockIdx.x % p.max_blocks);
-  const int chunk = (int)(blockIdx.x / p.max_blocks);
-  // The launch in front let this one in after its own wait for the plan, so only h is not there yet.
-  if (block >= __ldcg(p.blocks.count)) return;
-  const int adapter = __ldcg(p.blocks.adapter + block);
-  if (adapter < 0 && p.in_place) return;
-  const int start = __ldcg(p.blocks.start + block), rows = __ldcg(p.blocks.rows + block);
+  const int piece = (int)(blockIdx.x % (p.max_blocks * p.subs)), block = piece / p.subs, row0 = piece % p.subs * p.sub;
+  const int chunk = (int)(blockIdx.x / (p.max_blocks * p.subs));
+  // The launch in front let this one in after its own wait for all that came before it, so only h is not there yet.
+  int rows, adapter;
+  if (p.blocks.ids != nullptr) {
+    if (warp == 0) {
+      int n = 0, a = -1;
+      const bool there = narrow::scan_block(p.blocks, block, lane, token, n, a);
+      if (lane == 0) found[0] = there ? n : 0, found[1] = a;
+    }
+    __syncthreads();
+    rows = found[0], adapter = found[1];
+  } else {
+    if (block >= __ldcg(p.blocks.count)) return;
+    adapter = __ldcg(p.blocks.adapter + block);
+    const int start = __ldcg(p.blocks.start + block);
+    rows = __ldcg(p.blocks.rows + block);
+    if (tid < rows) token[tid] = __ldcg(p.blocks.order + start + tid);
+  }
+  if (row0 >= rows || (adapter < 0 && p.in_place)) return;
+  rows = min(rows - row0, p.sub);
   int slice = 0;
   while (slice + 1 < p.S && chunk >= p.chunk0[slice + 1]) ++slice;
   const int64_t end = p.col0[slice + 1];
@@ -162,7 +178,6 @@ __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
   const T* weights = static_cast<const T*>(p.b) + (adapter < 0 ? 0 : (int64_t)adapter * p.N * p.R);
   const T* base = static_cast<const T*>(p.base);
   T* out = static_cast<T*>(p.out);
-  if (tid < rows) token[tid] = __ldcg(p.blocks.order + start + tid);
 
   uint2 w[kSteps][kTiles];
   auto load_weights = [&](int64_t c) {
@@ -172,66 +187,85 @@ __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         const int r = s * 16 + q * 4;
-        uint2 v = make_uint2(0, 0);
-        if (n < end && r < used) {
-          v = __ldg(reinterpret_cast<const uint2*>(weights + n * p.R + r));
-          if (r + 1 >= used) v.x &= 0xffffu;  // (beyond the rank anything may stand)
-          if (r + 2 >= used) v.y = 0;
-          if (r + 3 >= used) v.y &= 0xffffu;
+        w[s][j] = n < end && r < used ? __ldg(reinterpret_cast<const uint2*>(weights + n * p.R + r)) : make_uint2(0, 0);
+      }
+    }
+    if (used % 4 != 0) {  // beyond the rank anything may stand
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int r = s * 16 + q * 4;
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) {
+          if (r + 1 >= used) w[s][j].x &= 0xffffu;
+          if (r + 2 >= used) w[s][j].y = 0;
+          if (r + 3 >= used) w[s][j].y &= 0xffffu;
         }
-        w[s][j] = v;
       }
     }
   };
+  // Two tokens' kMine columns at c, 16 bytes (8 for two groups) at a time where all lie so.
+  auto load_base = [&](int64_t c, int m, uint32_t (&old)[2][kTiles]) {
+    const int64_t mine = c + q * kMine;
+    const int cols = (int)max((int64_t)0, min((int64_t)kMine, end - mine));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = m + g + 8 * i;
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) old[i][j] = 0;
+      if (r >= rows || cols == 0) continue;
+      const T* from = base + (int64_t)token[row0 + r] * p.ld_base + mine;
+      if (p.vec) {
+        if constexpr (kTiles == 4)
+          *reinterpret_cast<uint4*>(old[i]) = *reinterpret_cast<const uint4*>(from);
+        else
+          *reinterpret_cast<uint2*>(old[i]) = *reinterpret_cast<const uint2*>(from);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kMine; ++j)
+          if (j < cols) old[i][j / 2] |= (uint32_t)bits(from[j]) << (j % 2 * 16);
+      }
+    }
+  };
+  uint32_t old[2][kTiles] = {};
   if (c0 < end) load_weights(c0);
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
+  __syncthreads();  // (the tokens)
+  if (c0 < end) load_base(c0, 0, old);
   const float scaling = adapter >= 0 && p.scalings != nullptr ? __ldg(p.scalings + adapter) : 1.f;
   for (int i = warp; i < rows; i += kWarps) {
     uint16_t* at = reinterpret_cast<uint16_t*>(tile + i * p.pitch);
-    const float inv = split_row<T>(p.h + (int64_t)(start + i) * p.S * p.R + slice * p.R, used, scaling, at, at + p.R, p.R, lane);
+    const float inv = split_row<T>(p.h + ((int64_t)token[row0 + i] * p.S + slice) * p.R, used, scaling, at, at + p.R, p.R, lane);
     if (lane == 0) unscale[i] = inv;
   }
   __syncthreads();
   const int steps = (used + 15) / 16;
-  const int tail = p.R % 16;  // (R is a multiple of 8: a last instruction may have half its columns)
 
   for (int pass = 0; pass < p.passes; ++pass) {
     const int64_t c = c0 + (int64_t)pass * kWarps * kCols;
     if (c >= end) break;
+    const int64_t next_c = c + kWarps * kCols;
+    const bool more = pass + 1 < p.passes && next_c < end;
     if (pass > 0) load_weights(c);
     const int64_t mine = c + q * kMine;
     const int cols = (int)max((int64_t)0, min((int64_t)kMine, end - mine));
     for (int m = 0; m < rows; m += 16) {
       const int ra = m + g, rb = m + g + 8;
-      const bool a_on = ra < rows && cols > 0, b_on = rb < rows && cols > 0;
-      const int64_t ta = a_on ? token[ra] : 0, tb = b_on ? token[rb] : 0;
-      uint32_t old[2][kTiles] = {};
-      const T* from[2] = {base + ta * p.ld_base + mine, base + tb * p.ld_base + mine};
-      const bool on[2] = {a_on, b_on};
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (!on[i]) continue;
-        if (p.vec) {
-          if constexpr (kTiles == 4)
-            *reinterpret_cast<uint4*>(old[i]) = *reinterpret_cast<const uint4*>(from[i]);
-          else
-            *reinterpret_cast<uint2*>(old[i]) = *reinterpret_cast<const uint2*>(from[i]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < kMine; ++j)
-            if (j < cols) old[i][j / 2] |= (uint32_t)bits(from[i][j]) << (j % 2 * 16);
-        }
+      uint32_t ahead[2][kTiles] = {};
+      if (m + 16 < rows) {
+        load_base(c, m + 16, ahead);
+      } else if (more) {
+        load_base(next_c, 0, ahead);
       }
       float acc[kTiles][4] = {};
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         if (s >= steps) break;
-        const bool in = s * 16 + q * 4 < p.R || tail == 0;
+        const bool in = s * 16 + q * 4 < p.R;  // (R is a multiple of 8: a last instruction may have half its columns)
         const uint8_t* pa = tile + ra * p.pitch + (s * 16 + q * 4) * 2;
         const uint8_t* pb = tile + rb * p.pitch + (s * 16 + q * 4) * 2;
         const uint2 zero = make_uint2(0, 0);
-        // (rows past the block's last are not written, and meet only their own sums)
+        // (rows past the last are not written, and meet only their own sums)
         const uint2 ah = in ? *reinterpret_cast<const uint2*>(pa) : zero, bh = in ? *reinterpret_cast<const uint2*>(pb) : zero;
         const uint2 al = in ? *reinterpret_cast<const uint2*>(pa + p.R * 2) : zero, bl = in ? *reinterpret_cast<const uint2*>(pb + p.R * 2) : zero;
 #pragma unroll
@@ -242,9 +276,10 @@ __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if (!on[i]) continue;
-        T* to = out + (i == 0 ? ta : tb) * p.ld_out + mine;
-        const float inv = unscale[i == 0 ? ra : rb];
+        const int r = m + g + 8 * i;
+        if (r >= rows || cols == 0) continue;
+        T* to = out + (int64_t)token[row0 + r] * p.ld_out + mine;
+        const float inv = unscale[r];
         uint32_t now[kTiles];
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) {
@@ -271,17 +306,25 @@ __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
             }
         }
       }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) old[i][j] = ahead[i][j];
     }
   }
 }
 
 template <typename T, int kSteps, int kTiles>
-static int launch_expand(Params& p, cudaStream_t st) {
+static int launch_expand(Params& p, int block, cudaStream_t st) {
   constexpr int kCols = 8 * kTiles * kWarps;
   int64_t units = 0;
   for (int s = 0; s < p.S; ++s) units += (p.col0[s + 1] - p.col0[s] + kCols - 1) / kCols;
-  // about eight CTAs' work for every SM, at most eight passes
-  int64_t passes = units * p.max_blocks / (8 * sm_count());
+  // Blocks are cut until there are four CTAs for every SM, then a CTA takes as many passes as leave that many.
+  const int64_t want = 4 * sm_count();
+  p.sub = block;
+  while (p.sub > 16 && units * p.max_blocks * (block / p.sub) < want) p.sub /= 2;
+  p.subs = block / p.sub;
+  const int64_t passes = units * p.max_blocks * p.subs / want;
   p.passes = (int)(passes < 1 ? 1 : passes > 8 ? 8 : passes);
   int chunks = 0;
   for (int s = 0; s < p.S; ++s) {
@@ -292,10 +335,11 @@ static int launch_expand(Params& p, cudaStream_t st) {
   p.chunk0[p.S] = chunks;
   // rows 32 bytes apart modulo 128: four rows of 32 bytes are read without a bank conflict
   p.pitch = (4 * p.R + 127) / 128 * 128 + 32;
-  const size_t smem = (size_t)p.block * p.pitch;
-  SGLB_REQUIRE((int64_t)chunks * p.max_blocks < (1ll << 31), "lora_add: %lld tiles are too many", (long long)chunks * p.max_blocks);
+  const size_t smem = (size_t)p.sub * p.pitch;
+  const int64_t grid = (int64_t)chunks * p.max_blocks * p.subs;
+  SGLB_REQUIRE(grid < (1ll << 31), "lora_add: %lld tiles are too many", (long long)grid);
   auto kern = expand_kernel<T, kSteps, kTiles>;
-  if (smem > 48 * 1024) {
+  if (smem > 40 * 1024) {  // (beside the static ones)
     static thread_local bool attr_set[64] = {false};  // the opt-in is per function and per device
     int dev = 0;
     SGLB_CUDA(cudaGetDevice(&dev));
@@ -304,20 +348,24 @@ static int launch_expand(Params& p, cudaStream_t st) {
       if (dev >= 0 && dev < 64) attr_set[dev] = true;
     }
   }
-  SGLB_CUDA(launch_pdl(kern, (unsigned)(chunks * p.max_blocks), kWarps * 32, smem, st, p));
+  SGLB_CUDA(launch_pdl(kern, (unsigned)grid, kWarps * 32, smem, st, p));
   return SGLB200_OK;
 }
 
 template <typename T>
-static int expand(Params& p, cudaStream_t st) {
-  if (p.R <= 16) return launch_expand<T, 1, 4>(p, st);
-  if (p.R <= 32) return launch_expand<T, 2, 4>(p, st);
-  if (p.R <= 64) return launch_expand<T, 4, 4>(p, st);
-  if (p.R <= 128) return launch_expand<T, 8, 4>(p, st);
-  return launch_expand<T, 16, 2>(p, st);
+static int expand(Params& p, int block, cudaStream_t st) {
+  if (p.R <= 16) return launch_expand<T, 1, 4>(p, block, st);
+  if (p.R <= 32) return launch_expand<T, 2, 4>(p, block, st);
+  if (p.R <= 64) return launch_expand<T, 4, 4>(p, block, st);
+  if (p.R <= 128) return launch_expand<T, 8, 4>(p, block, st);
+  return launch_expand<T, 16, 2>(p, block, st);
 }
 
-static int64_t most_blocks(int64_t T, int L, int block) { return T / block + (T < L + 1 ? T : L + 1); }
+// Every adapter (and "none") has at most one block that is not full.
+static int64_t most_blocks(int64_t T, int L, int block) {
+  const int64_t named = T < L + 1 ? T : L + 1;
+  return T <= block ? named : T / block + named;
+}
 static int64_t up(int64_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace lora
@@ -328,7 +376,7 @@ using namespace sglb200;
 extern "C" int64_t sglb200_lora_add_workspace_bytes(int64_t tokens, int num_adapters, int rank, int num_slices) {
   if (tokens <= 0 || num_adapters < 1 || rank < 1 || num_slices < 1) return 0;
   // (whichever blocks the call takes)
-  const int64_t blocks = lora::most_blocks(tokens, num_adapters, narrow::kSmallBlock);
+  const int64_t blocks = tokens / narrow::kSmallBlock + num_adapters + 1;
   return lora::up(4 * tokens) + lora::up(4 * (3 * blocks + 1)) + lora::up(4 * tokens * num_slices * rank);
 }
 
@@ -369,23 +417,28 @@ extern "C" int sglb200_lora_add(const void* x, const void* lora_a, const void* l
   const int64_t bytes = sglb200_lora_add_workspace_bytes(tokens, num_adapters, rank, num_slices);
   if (workspace == nullptr || workspace_bytes < bytes || !aligned16(workspace))
     return fail(SGLB200_E_WORKSPACE, "lora_add: %lld bytes of workspace are needed, aligned to 16", (long long)bytes);
-  const int block = narrow::block_rows(tokens, (int64_t)num_slices * rank, K, num_adapters);
+  const bool scan = tokens <= narrow::kScanRows;
+  const int block = scan ? narrow::kSmallBlock : narrow::block_rows(tokens, (int64_t)num_slices * rank, K, num_adapters);
   const int64_t blocks = lora::most_blocks(tokens, num_adapters, block);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int32_t* order = static_cast<int32_t*>(workspace);
   int32_t* start = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + lora::up(4 * tokens));
   float* h = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(start) + lora::up(4 * (3 * blocks + 1)));
-  p.blocks = {order, start, start + blocks, start + 2 * blocks, start + 3 * blocks};
-  SGLB_CUDA(launch_pdl(lora::plan_kernel, 1u, (unsigned)lora::kPlanThreads, (size_t)0, st, adapter_ids, (int)tokens, num_adapters, block, order, start,
-                       start + blocks, start + 2 * blocks, start + 3 * blocks));
+  if (scan) {
+    p.blocks.ids = adapter_ids, p.blocks.ids_rows = (int)tokens, p.blocks.adapters = num_adapters;
+  } else {
+    p.blocks = {order, start, start + blocks, start + 2 * blocks, start + 3 * blocks, nullptr, 0, 0};
+    SGLB_CUDA(launch_pdl(lora::plan_kernel, 1u, (unsigned)lora::kPlanThreads, (size_t)0, st, adapter_ids, (int)tokens, num_adapters, block, order,
+                         start, start + blocks, start + 2 * blocks, start + 3 * blocks));
+  }
   narrow::Params n{};
   n.x = x, n.w = lora_a, n.y = h, n.ranks = ranks, n.blocks = p.blocks;
   n.T = tokens, n.N = (int64_t)num_slices * rank, n.K = K, n.ldx = x_stride, n.rank_rows = rank, n.adapters = num_adapters, n.block = block;
   int rc = narrow::product(n, dtype, blocks, st);
   if (rc) return rc;
   p.b = lora_b, p.base = base, p.out = out, p.h = h, p.scalings = scalings, p.ranks = ranks;
-  p.N = N, p.ld_base = base_stride, p.ld_out = out_stride, p.R = rank, p.S = num_slices, p.block = block, p.max_blocks = (int)blocks;
+  p.N = N, p.ld_base = base_stride, p.ld_out = out_stride, p.R = rank, p.S = num_slices, p.max_blocks = (int)blocks;
   p.in_place = base == out && base_stride == out_stride;
   p.vec = even && N % 8 == 0 && base_stride % 8 == 0 && out_stride % 8 == 0 && aligned16(base) && aligned16(out);
-  return dtype == 0 ? lora::expand<__nv_bfloat16>(p, st) : lora::expand<__half>(p, st);
+  return dtype == 0 ? lora::expand<__nv_bfloat16>(p, block, st) : lora::expand<__half>(p, block, st);
 }

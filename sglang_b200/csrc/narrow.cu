@@ -28,43 +28,57 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// kG groups of 8 activation rows.
+// kG groups of 8 activation rows.  `part` and `sums` are padded so that neither their writes nor their reads meet in a bank: unpadded,
+// 64 rows x 256 x 7168 took 12.8 us.
 template <typename T, int kG>
 __global__ void __launch_bounds__(kWarps * 32) narrow_kernel(const Params p) {
-  constexpr int kCols = kG * 8;
-  __shared__ float part[kWarps][16][kCols];
-  __shared__ float sums[16 * kCols];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
+  constexpr int kCols = kG * 8, kPartPitch = kCols + 8, kSumPitch = 17;
+  __shared__ float part[kWarps][16][kPartPitch];
+  __shared__ float sums[kCols * kSumPitch];
+  __shared__ int32_t row[kSmallBlock];
+  __shared__ int found[2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
   const int rank = (int)(blockIdx.x % p.splits), n0 = (int)(blockIdx.x / p.splits % p.n_tiles) * 16;
   const int64_t block = blockIdx.x / p.splits / p.n_tiles;
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
   int64_t start = block * kSmallBlock, adapter = 0;
   int rows = (int)min((int64_t)kSmallBlock, p.T - start);
-  if (p.blocks.order != nullptr) {  // (uniform over the cluster)
+  const bool sorted = p.blocks.order != nullptr || p.blocks.ids != nullptr;
+  if (p.blocks.ids != nullptr) {
+    if (warp == 0) {
+      int n = 0, a = -1;
+      const bool there = scan_block(p.blocks, (int)block, lane, row, n, a);
+      if (lane == 0) found[0] = there ? n : 0, found[1] = a;
+    }
+    __syncthreads();
+    rows = found[0], adapter = found[1];
+    if (rows == 0 || adapter < 0) return;  // (uniform over the cluster)
+  } else if (p.blocks.order != nullptr) {
     if (block >= *p.blocks.count) return;
     start = p.blocks.start[block], rows = p.blocks.rows[block], adapter = p.blocks.adapter[block];
     if (adapter < 0) return;
+    if (tid < rows) row[tid] = p.blocks.order[start + tid];
+    __syncthreads();
   }
   const int used = p.ranks != nullptr ? min(max(p.ranks[adapter], 0), p.rank_rows) : p.rank_rows;
   const T* w = static_cast<const T*>(p.w) + adapter * p.N * p.K;
-  const int64_t na = n0 + g, nb = n0 + g + 8;
+  const int na = n0 + g, nb = n0 + g + 8;
   const bool a_on = na < p.N && na % p.rank_rows < used, b_on = nb < p.N && nb % p.rank_rows < used;
   const T* wa = w + (a_on ? na : 0) * p.K;
   const T* wb = w + (b_on ? nb : 0) * p.K;
   const T* x[kG];
-  bool x_on[kG];
 #pragma unroll
   for (int j = 0; j < kG; ++j) {
-    x_on[j] = j * 8 + g < rows;
-    const int64_t r = x_on[j] ? start + j * 8 + g : start;
-    x[j] = static_cast<const T*>(p.x) + (p.blocks.order != nullptr ? (int64_t)p.blocks.order[r] : r) * p.ldx;
+    const int i = min(j * 8 + g, rows - 1);
+    x[j] = static_cast<const T*>(p.x) + (sorted ? (int64_t)row[i] : start + i) * p.ldx;
   }
   float acc[kG][4] = {};
   const int steps = (int)((p.K + kStep - 1) / kStep), parts = p.splits * kWarps, mine = rank * kWarps + warp;
   const int s0 = (int)((int64_t)mine * steps / parts), s1 = (int)((int64_t)(mine + 1) * steps / parts);
   const uint4 zero = make_uint4(0, 0, 0, 0);
-#pragma unroll 2
+  constexpr int kAhead = kG <= 2 ? 4 : 2;
+#pragma unroll(kAhead)
   for (int s = s0; s < s1; ++s) {
     const int64_t k = (int64_t)s * kStep + q * 8;
     const bool in = k < p.K;  // (K is a multiple of 8)
@@ -73,23 +87,26 @@ __global__ void __launch_bounds__(kWarps * 32) narrow_kernel(const Params p) {
     const uint32_t first[4] = {a.x, b.x, a.y, b.y}, second[4] = {a.z, b.z, a.w, b.w};
     uint4 v[kG];
 #pragma unroll
-    for (int j = 0; j < kG; ++j) v[j] = in && x_on[j] ? ld_nc_16(x[j] + k) : zero;
+    for (int j = 0; j < kG; ++j) v[j] = in && j * 8 < rows ? ld_nc_16(x[j] + k) : zero;
 #pragma unroll
     for (int j = 0; j < kG; ++j)
       if (j * 8 < rows) mma16816<T>(acc[j], first, v[j].x, v[j].y), mma16816<T>(acc[j], second, v[j].z, v[j].w);
   }
 #pragma unroll
   for (int j = 0; j < kG; ++j) {
+    if (j * 8 >= rows) break;
     *reinterpret_cast<float2*>(&part[warp][g][j * 8 + q * 2]) = make_float2(acc[j][0], acc[j][1]);
     *reinterpret_cast<float2*>(&part[warp][g + 8][j * 8 + q * 2]) = make_float2(acc[j][2], acc[j][3]);
   }
   __syncthreads();
   // The warps' sums, then the CTAs', each in ascending order of K.
-  for (int i = threadIdx.x; i < 16 * kCols; i += kWarps * 32) {
+  for (int i = tid; i < 16 * kCols; i += kWarps * 32) {
+    const int t = i % kCols, n = i / kCols;
+    if (t >= rows) continue;
     float v = 0.f;
 #pragma unroll
-    for (int u = 0; u < kWarps; ++u) v += (&part[u][0][0])[i];
-    sums[i] = v;
+    for (int u = 0; u < kWarps; ++u) v += part[u][n][t];
+    sums[t * kSumPitch + n] = v;
   }
   if (p.splits > 1) {
     ptx::cluster_sync();
@@ -97,21 +114,24 @@ __global__ void __launch_bounds__(kWarps * 32) narrow_kernel(const Params p) {
     __syncthreads();
   }
   const uint32_t at = ptx::smem_u32(sums);
-  for (int i = threadIdx.x + rank * kWarps * 32; i < 16 * kCols; i += p.splits * kWarps * 32) {
+  for (int i = tid + rank * kWarps * 32; i < 16 * rows; i += p.splits * kWarps * 32) {
     // (neighbouring threads take neighbouring rows of the weights, which lie side by side in y)
     const int n = i & 15, t = i >> 4;
-    if (t >= rows || n0 + n >= p.N) continue;
+    if (n0 + n >= p.N) continue;
     float v = 0.f;
     if (p.splits > 1) {
-      for (int s = 0; s < p.splits; ++s) {
-        float o;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o) : "r"(ptx::cluster_map(at + (n * kCols + t) * 4, s)) : "memory");
-        v += o;
-      }
+      float o[8];
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+        if (s < p.splits)
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o[s]) : "r"(ptx::cluster_map(at + (t * kSumPitch + n) * 4, s)) : "memory");
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+        if (s < p.splits) v += o[s];
     } else {
-      v = sums[n * kCols + t];
+      v = sums[t * kSumPitch + n];
     }
-    p.y[(start + t) * p.N + n0 + n] = v;
+    p.y[(sorted ? (int64_t)row[t] : start + t) * p.N + n0 + n] = v;
   }
   if (p.splits > 1) ptx::cluster_sync();  // no CTA leaves while another reads its shared memory
 }
@@ -143,11 +163,12 @@ static int dispatch(Params& p, int64_t blocks, cudaStream_t st) {
   while (p.splits < 8 && tiles * p.splits * 2 <= 2 * sm_count() && steps >= p.splits * 2 * kWarps) p.splits *= 2;
   if (p.T <= 8) return launch<T, 1>(p, blocks, st);
   if (p.T <= 16) return launch<T, 2>(p, blocks, st);
+  if (p.T <= 32) return launch<T, 4>(p, blocks, st);
   return launch<T, 8>(p, blocks, st);
 }
 
 #ifndef NARROW_TILE_FROM
-#define NARROW_TILE_FROM 129
+#define NARROW_TILE_FROM 65
 #endif
 int block_rows(int64_t T, int64_t N, int64_t K, int64_t adapters) { return T < NARROW_TILE_FROM ? kSmallBlock : kTileBlock; }
 

@@ -8,20 +8,47 @@ namespace narrow {
 // Rows that share their weights come in blocks: of 64 of them for narrow_kernel, of 128 for narrow_tile_kernel.
 constexpr int kSmallBlock = 64, kTileBlock = 128;
 
-// What the rows of a batch are sorted into: `order` the rows by adapter, then per block where it starts in the order, its rows and its
-// adapter (-1: rows that name none, behind the others); `count` the number of blocks.
+// The blocks that the rows of a batch are sorted into by adapter.  Either a plan: `order` the rows, then per block where it starts in the
+// order, its rows and its adapter (-1: rows that name none), `count` the number of blocks.  Or, for up to kScanRows rows, which one warp
+// looks through faster than a launch of its own takes: `ids`, from which every CTA finds its block.
+constexpr int kScanRows = 64;
 struct Blocks {
-  const int32_t* order;    // or nullptr: the rows as they lie, all of one adapter
+  const int32_t* order;  // neither order nor ids: the rows as they lie, all of one adapter
   const int32_t* start;
   const int32_t* rows;
   const int32_t* adapter;
   const int32_t* count;
+  const int32_t* ids;
+  int ids_rows, adapters;
 };
+
+// One warp: block `block` in the order of the adapters' first rows, its rows to `row` (ascending); false: there are not so many.
+__device__ __forceinline__ bool scan_block(const Blocks& b, int block, int lane, int32_t* row, int& rows, int& adapter) {
+  auto key = [&](int t) {
+    const int id = t < b.ids_rows ? __ldg(b.ids + t) : -1;
+    return id >= 0 && id < b.adapters ? id : -1;
+  };
+  const int k0 = key(lane), k1 = key(lane + 32);
+  uint32_t left0 = b.ids_rows >= 32 ? 0xffffffffu : (1u << b.ids_rows) - 1;
+  uint32_t left1 = b.ids_rows >= 64 ? 0xffffffffu : b.ids_rows > 32 ? (1u << (b.ids_rows - 32)) - 1 : 0;
+  uint32_t in0 = 0, in1 = 0;
+  for (int i = 0; i <= block; ++i) {
+    if ((left0 | left1) == 0) return false;
+    adapter = left0 ? __shfl_sync(0xffffffffu, k0, __ffs(left0) - 1) : __shfl_sync(0xffffffffu, k1, __ffs(left1) - 1);
+    in0 = __ballot_sync(0xffffffffu, k0 == adapter) & left0, in1 = __ballot_sync(0xffffffffu, k1 == adapter) & left1;
+    left0 &= ~in0, left1 &= ~in1;
+  }
+  const uint32_t below = (1u << lane) - 1;
+  if (in0 >> lane & 1u) row[__popc(in0 & below)] = lane;
+  if (in1 >> lane & 1u) row[__popc(in0) + __popc(in1 & below)] = lane + 32;
+  rows = __popc(in0) + __popc(in1);
+  return true;
+}
 
 struct Params {
   const void* x;       // [T, K], rows `ldx` apart
   const void* w;       // [adapters, N, K]
-  float* y;            // [T, N], in the blocks' order
+  float* y;            // [T, N]
   const int32_t* ranks;  // per adapter or nullptr: of every `rank_rows` rows of w the first ranks[adapter] count, the others give 0
   Blocks blocks;
   int64_t T, N, K, ldx;

@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int s = 1; s < 8; ++s)
           if (s < p.splits) sum.x += v[s].x, sum.y += v[s].y, sum.z += v[s].z, sum.w += v[s].w;
       }
-      float* to = p.y + (start + row) * p.N + n0 + c;
+      float* to = p.y + (p.blocks.order != nullptr ? (int64_t)__ldcg(p.blocks.order + start + row) : start + row) * p.N + n0 + c;
       if (vec) {
         *reinterpret_cast<float4*>(to) = sum;
       } else {

@@ -52,7 +52,7 @@
 
 #include "common.cuh"
 #include "gemm_common.cuh"
-#include "narrow.cuh"
+#include "lora.cuh"
 #include "ptx_sm100.cuh"
 #include "quant_math.cuh"
 
@@ -1748,6 +1748,7 @@ extern "C" int sglb200_gemm_status_clear(void) {
   if (rc == SGLB200_OK) rc = fp4_gemm_status_clear();
   if (rc == SGLB200_OK) rc = fp4_moe_status_clear();
   if (rc == SGLB200_OK) rc = narrow::tile_status_clear();
+  if (rc == SGLB200_OK) rc = lora::tile_status_clear();
   return rc != SGLB200_OK ? rc : small_linear_status_clear();
 }
 
@@ -1758,6 +1759,7 @@ extern "C" int sglb200_gemm_status(void) {
   if (v == 0) v = fp4_gemm_status();
   if (v == 0) v = fp4_moe_status();
   if (v == 0) v = narrow::tile_status();
+  if (v == 0) v = lora::tile_status();
   return v != 0 ? v : small_linear_status();
 }
 

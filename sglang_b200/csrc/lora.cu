@@ -8,18 +8,12 @@
 // h keeps 16 bits and more in the second product: the row's values times a power of two that brings the largest to [1, 2) (float16 would
 // overflow or lose small ones without it) enter as two 16-bit terms, 16 bits of bfloat16 or 22 of float16; the weights are what they are.
 // A rounding to one term would be off by 2^-9 of h, as much as the rounding of the output.
-#include <type_traits>
-
-#include "common.cuh"
-#include "narrow.cuh"
+#include "gemm_common.cuh"
+#include "lora.cuh"
 #include "ptx_sm100.cuh"
 
 namespace sglb200 {
 namespace lora {
-
-constexpr int kMaxAdapters = 1024;
-constexpr int kMaxSlices = 8;
-constexpr int kMaxRank = 256;
 
 // ---- plan -----------------------------------------------------------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
@@ -81,21 +75,6 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __res
 // ---- second product -------------------------------------------------------------------------------------------------------------------
 constexpr int kWarps = 8;
 
-struct Params {
-  const void* b;     // [L, N, R]
-  const void* base;  // [T, N], rows ld_base apart
-  void* out;         // rows ld_out apart; may be base
-  const float* h;    // [T, S R]
-  const float* scalings;  // or nullptr
-  const int32_t* ranks;   // or nullptr
-  narrow::Blocks blocks;
-  int64_t N, ld_base, ld_out;
-  int R, S, max_blocks, passes, vec, in_place, pitch;
-  int sub, subs;     // rows of a block that a CTA takes, CTAs of a block
-  int64_t col0[kMaxSlices + 1];  // first column of every merged projection, and the end
-  int chunk0[kMaxSlices + 1];    // the first chunk of passes x 8 warps x columns of a warp, and the end
-};
-
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value)
@@ -106,37 +85,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-template <typename T>
-__device__ __forceinline__ uint16_t bits(T v) {
-  return *reinterpret_cast<const uint16_t*>(&v);
-}
-
-// Row of h -> two terms of a 16-bit type, times a power of two, whose inverse is returned.
-template <typename T>
-__device__ __forceinline__ float split_row(const float* h, int used, float scaling, uint16_t* hi, uint16_t* lo, int R, int lane) {
-  float v[kMaxRank / 32], most = 0.f;
-#pragma unroll
-  for (int j = 0; j < kMaxRank / 32; ++j) {
-    const int r = j * 32 + lane;
-    v[j] = r < used ? __ldcg(h + r) * scaling : 0.f;
-    most = fmaxf(most, fabsf(v[j]));
-  }
-  const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-  const uint32_t e = min(top >> 23, 253u);
-  const bool plain = e == 0 || top >= 0x7f800000u;  // nothing to bring anywhere
-  const float f = plain ? 1.f : __uint_as_float((254u - e) << 23);
-#pragma unroll
-  for (int j = 0; j < kMaxRank / 32; ++j) {
-    const int r = j * 32 + lane;
-    if (r >= R) break;
-    const float s = v[j] * f;
-    const T a = ElemTraits<T>::from_f32(s);
-    const float rest = s - ElemTraits<T>::to_f32(a);
-    hi[r] = bits(a), lo[r] = bits(ElemTraits<T>::from_f32(fabsf(s) < INFINITY ? rest : 0.f));
-  }
-  return plain ? 1.f : __uint_as_float(e << 23);
 }
 
 // kSteps: instructions over the rank, at most; kTiles: groups of 8 columns of a warp.  A lane holds the same two kTiles neighbouring columns
@@ -235,7 +183,8 @@ __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
   const float scaling = adapter >= 0 && p.scalings != nullptr ? __ldg(p.scalings + adapter) : 1.f;
   for (int i = warp; i < rows; i += kWarps) {
     uint16_t* at = reinterpret_cast<uint16_t*>(tile + i * p.pitch);
-    const float inv = split_row<T>(p.h + ((int64_t)token[row0 + i] * p.S + slice) * p.R, used, scaling, at, at + p.R, p.R, lane);
+    const float inv = split_row<T>(p.h + ((int64_t)token[row0 + i] * p.S + slice) * p.R, used, scaling, p.R, lane,
+                                   [&](int r, uint16_t hi, uint16_t lo) { at[r] = hi, at[p.R + r] = lo; });
     if (lane == 0) unscale[i] = inv;
   }
   __syncthreads();
@@ -440,5 +389,7 @@ extern "C" int sglb200_lora_add(const void* x, const void* lora_a, const void* l
   p.N = N, p.ld_base = base_stride, p.ld_out = out_stride, p.R = rank, p.S = num_slices, p.max_blocks = (int)blocks;
   p.in_place = base == out && base_stride == out_stride;
   p.vec = even && N % 8 == 0 && base_stride % 8 == 0 && out_stride % 8 == 0 && aligned16(base) && aligned16(out);
+  p.wait_probes = g_gemm_wait_probes;
+  if (block == narrow::kTileBlock && p.vec && rank <= lora::kTileRank) return lora::expand_tile(p, dtype, st);
   return dtype == 0 ? lora::expand<__nv_bfloat16>(p, block, st) : lora::expand<__half>(p, block, st);
 }

@@ -1,0 +1,70 @@
+// What the adapters' second-product kernels share (lora.cu, lora_tile.cu).
+#pragma once
+#include <type_traits>
+
+#include "common.cuh"
+#include "narrow.cuh"
+
+namespace sglb200 {
+namespace lora {
+
+constexpr int kMaxAdapters = 1024;
+constexpr int kMaxSlices = 8;
+constexpr int kMaxRank = 256;
+
+struct Params {
+  const void* b;     // [L, N, R]
+  const void* base;  // [T, N], rows ld_base apart
+  void* out;         // rows ld_out apart; may be base
+  const float* h;    // [T, S R]
+  const float* scalings;  // or nullptr
+  const int32_t* ranks;   // or nullptr
+  narrow::Blocks blocks;
+  int64_t N, ld_base, ld_out;
+  int R, S, max_blocks, passes, vec, in_place, pitch;
+  int sub, subs;     // rows of a block that a CTA takes, CTAs of a block
+  int64_t col0[kMaxSlices + 1];  // first column of every merged projection, and the end
+  int chunk0[kMaxSlices + 1];    // the first chunk of passes x 8 warps x columns of a warp (lora_tile.cu: of 128 columns), and the end
+  uint32_t wait_probes;
+};
+
+template <typename T>
+__device__ __forceinline__ uint16_t bits(T v) {
+  return *reinterpret_cast<const uint16_t*>(&v);
+}
+
+// A row of h times `scaling` -> two terms of a 16-bit type, times a power of two, whose inverse is returned; put(r, high, low) for r below
+// `width` (zeros from `used` on).  One warp.
+template <typename T, class Put>
+__device__ __forceinline__ float split_row(const float* h, int used, float scaling, int width, int lane, Put put) {
+  float v[kMaxRank / 32], most = 0.f;
+#pragma unroll
+  for (int j = 0; j < kMaxRank / 32; ++j) {
+    const int r = j * 32 + lane;
+    v[j] = r < used ? __ldcg(h + r) * scaling : 0.f;
+    most = fmaxf(most, fabsf(v[j]));
+  }
+  const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+  const uint32_t e = min(top >> 23, 253u);
+  const bool plain = e == 0 || top >= 0x7f800000u;  // nothing to bring anywhere
+  const float f = plain ? 1.f : __uint_as_float((254u - e) << 23);
+#pragma unroll
+  for (int j = 0; j < kMaxRank / 32; ++j) {
+    const int r = j * 32 + lane;
+    if (r >= width) break;
+    const float s = v[j] * f;
+    const T a = ElemTraits<T>::from_f32(s);
+    const float rest = s - ElemTraits<T>::to_f32(a);
+    put(r, bits(a), bits(ElemTraits<T>::from_f32(fabsf(s) < INFINITY ? rest : 0.f)));
+  }
+  return plain ? 1.f : __uint_as_float(e << 23);
+}
+
+// lora_tile.cu: the second product for blocks of 128 rows; rank at most kTileRank, p.vec.  A status word as gemm_rows.cu's, and its reset.
+constexpr int kTileRank = 128;
+int expand_tile(Params& p, int dtype, cudaStream_t st);
+int tile_status();
+int tile_status_clear();
+
+}  // namespace lora
+}  // namespace sglb200

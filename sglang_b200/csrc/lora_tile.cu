@@ -1,0 +1,356 @@
+// The adapters' second product for many rows, out = base + h B^T (lora.cu), on tcgen05.mma.kind::f16: bound by reading base and writing out.
+//
+// A tile is 128 sorted tokens by 128 columns.  The tiles of all blocks, columns fastest, are cut evenly over two CTAs an SM (one, where the
+// rank is above 64), whatever the blocks' sizes; a CTA builds the two terms of h anew where a block or a merged projection begins.  One warp
+// copies the weights into a ring, one multiplies into two buffers of tensor memory, eight add base and store.
+//
+// The columns of 32 are multiplied in the order i + 2 q + 8 j for column 8 q + 2 j + i: a lane that reads two neighbouring columns of each
+// eight from tensor memory then holds eight neighbouring ones of out, and base and out go by 16 bytes a lane, 64 a row.  The next tile's base is
+// asked for before this tile's sums are waited for.
+#include <algorithm>
+
+#include "gemm_common.cuh"
+#include "lora.cuh"
+#include "ptx_sm100.cuh"
+
+namespace sglb200 {
+namespace lora {
+
+__device__ int g_lora_tile_status = 0;  // 0 ok, 1 = a pipeline wait expired
+
+namespace {
+
+constexpr int kRows = narrow::kTileBlock, kCols = 128;
+constexpr int kThreads = 320;  // eight warps that add and store, one that copies weights, one that multiplies: 96 registers with two CTAs an SM
+constexpr int kStages = 3, kLag = 1;
+constexpr uint32_t kSpan = 128 * 128;  // 128 rows of 64 columns of the rank, one swizzle span wide
+
+// kKB: spans of 64 columns of the rank.
+template <int kKB>
+constexpr uint32_t kSmem = 1024 + kKB * kSpan * (2 + kStages);
+
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);  // rows of 128 bytes, 128-byte swizzle
+__device__ __forceinline__ uint32_t desc_lo(uint32_t smem) { return ((smem & 0x3ffffu) >> 4) | (1u << 16); }
+
+#define LORA_WAIT(bar, parity) \
+  (p.wait_probes != ptx::kProbesNone && (ptx::mbar_test(bar, parity) || ptx::mbar_wait_quiet(bar, parity)))
+
+// A run of tiles of one block and one merged projection.
+struct Run {
+  int adapter, rows, start, used;
+  int column, end;   // the first column, and the projection's end
+  int slice, count;  // tiles
+  bool multiply;     // (else out = base)
+};
+
+// The run that begins at tile `at` of all, of which `end` are this CTA's.
+__device__ __forceinline__ Run run_at(const Params& p, int at, int end) {
+  Run r;
+  const int per = p.chunk0[p.S], block = at / per, tile = at - block * per;
+  int s = 0;
+  while (s + 1 < p.S && tile >= p.chunk0[s + 1]) ++s;
+  r.slice = s;
+  r.column = (int)p.col0[s] + (tile - p.chunk0[s]) * kCols, r.end = (int)p.col0[s + 1];
+  r.count = min(p.chunk0[s + 1] - tile, end - at);
+  r.adapter = __ldcg(p.blocks.adapter + block);
+  r.rows = __ldcg(p.blocks.rows + block);
+  r.start = __ldcg(p.blocks.start + block);
+  r.used = r.adapter < 0 ? 0 : p.ranks != nullptr ? min(max(__ldg(p.ranks + r.adapter), 0), p.R) : p.R;
+  r.multiply = r.used > 0;
+  return r;
+}
+
+struct Ctl {
+  uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], h_full, h_empty;
+  uint32_t tmem_base;
+  int abort_flag;
+  float unscale[2][kRows];
+  int32_t token[2][kRows];
+  Run run[2];
+};
+
+template <typename T, int kKB>
+__global__ void __launch_bounds__(kThreads, kKB == 1 ? 2 : 1) expand_tile_kernel(const Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Ctl ctl;
+  uint8_t* spans = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t h_at = ptx::smem_u32(spans), ring = h_at + 2 * kKB * kSpan;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int* abort_flag = &ctl.abort_flag;
+  const uint32_t full = ptx::smem_u32(ctl.full), empty = ptx::smem_u32(ctl.empty), acc_full = ptx::smem_u32(ctl.acc_full),
+                 acc_empty = ptx::smem_u32(ctl.acc_empty), h_full = ptx::smem_u32(&ctl.h_full);
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) ptx::mbar_init(full + s * 8, 1), ptx::mbar_init(empty + s * 8, 1);
+    for (int b = 0; b < 2; ++b) ptx::mbar_init(acc_full + b * 8, 1), ptx::mbar_init(acc_empty + b * 8, 8);
+    ptx::mbar_init(h_full, 8);
+    ctl.abort_flag = 0;
+    ptx::mbar_fence_init();
+  }
+  ptx::grid_dependency_wait();
+  if (warp == 9) {
+    ptx::tmem_alloc(ptx::smem_u32(&ctl.tmem_base), 2 * kCols);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  ptx::launch_dependents();
+  const uint32_t tmem = ctl.tmem_base;
+  const int64_t all = (int64_t)__ldcg(p.blocks.count) * p.chunk0[p.S];
+  const int begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
+
+  if (warp == 8) {
+    // ------------------------------ weights: chunks of 16 bytes, row n to its place in the order above ------------------------------
+    int i = 0, landed = 0;
+    bool ok = true;
+    auto arrive = [&]() {
+      ptx::fence_async_smem();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(full + landed % kStages * 8);
+      ++landed;
+    };
+    for (int at = begin; at < end && ok;) {
+      const Run r = run_at(p, at, end);
+      at += r.count;
+      if (!r.multiply) continue;
+      const T* weights = static_cast<const T*>(p.b) + (int64_t)r.adapter * p.N * p.R;
+      const int chunks = (r.used + 15) / 16 * 2;  // of a row
+      for (int c = 0; c < r.count; ++c, ++i) {
+        const int s = i % kStages;
+        if (i >= kStages) ok = LORA_WAIT(empty + s * 8, ((i / kStages) & 1) ^ 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const int n0 = r.column + c * kCols, cols = min(kCols, r.end - n0);
+        const uint32_t to = ring + s * kKB * kSpan;
+        for (int id = lane; id < kCols * chunks; id += 32) {
+          const int n = id / chunks, k = id - n * chunks;
+          const int pos = (n & ~31) | ((n & 6) << 2) | ((n & 24) >> 2) | (n & 1);
+          const uint32_t dst = to + (k >> 3) * kSpan + pos * 128 + (((k & 7) ^ (pos & 7)) << 4);
+          const int left = n < cols ? r.used - k * 8 : 0;  // values that count of these eight
+          const T* src = weights + (int64_t)(n0 + n) * p.R + k * 8;
+          if (left <= 0 || left >= 8) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(left > 0 ? src : weights), "r"(left > 0 ? 16 : 0) : "memory");
+          } else {  // (beyond the rank anything may stand)
+            uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
+            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = 2 * j + 1 < left ? w[j] : 2 * j < left ? w[j] & 0xffffu : 0u;
+            ptx::sts_128(dst, v);
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (i >= kLag) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+          arrive();
+        }
+      }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (ok) {
+      while (landed < i) arrive();
+    } else if (lane == 0) {
+      *abort_flag = 1;
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    if (ptx::elect_one()) {
+      constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10) | ((kCols >> 3) << 17) | ((kRows >> 4) << 24);
+      int i = 0, runs = 0;
+      bool ok = true;
+      for (int at = begin; at < end && ok;) {
+        const Run r = run_at(p, at, end);
+        at += r.count;
+        if (!r.multiply) continue;
+        ok = LORA_WAIT(h_full, runs & 1);
+        ++runs;
+        const int steps = (r.used + 15) / 16;
+        for (int c = 0; c < r.count && ok; ++c, ++i) {
+          const int s = i % kStages, buf = i & 1;
+          if (i >= 2) ok = LORA_WAIT(acc_empty + buf * 8, ((i >> 1) & 1) ^ 1);
+          if (ok) ok = LORA_WAIT(full + s * 8, (i / kStages) & 1);
+          if (!ok) break;
+          ptx::tc_fence_after();
+#pragma unroll 1
+          for (int term = 1; term >= 0; --term)  // the low terms first
+#pragma unroll 1
+            for (int k = 0; k < steps; ++k) {
+              const uint32_t a = desc_lo(h_at + (term * kKB + k / 4) * kSpan) + 2 * (k % 4);
+              const uint32_t b = desc_lo(ring + (s * kKB + k / 4) * kSpan) + 2 * (k % 4);
+              asm volatile("{\n\t.reg .pred p;\n\t"
+                           "setp.ne.b32 p, %4, 0;\n\t"
+                           "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem + buf * kCols),
+                           "l"(ptx::pack_f32x2(a, kDescHi)), "l"(ptx::pack_f32x2(b, kDescHi)), "r"(kIdesc), "r"(term == 0 || k > 0 ? 1u : 0u)
+                           : "memory");
+            }
+          ptx::mma_commit(empty + s * 8);
+          ptx::mma_commit(acc_full + buf * 8);
+        }
+      }
+      if (!ok) *abort_flag = 1;
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------ out = base + sums ------------------------------
+    const int g = lane >> 2, q = lane & 3, quarter = warp & 3, wide = warp >> 2;  // 32 rows and 64 columns of a tile
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + wide * 64;
+    int i = 0, runs = 0;
+    bool ok = true;
+    uint4 old[2][2][2];  // [16 rows][+ 8 rows][32 columns]
+    // The run at tile `at` becomes the one of `set`: its rows' tokens and factors there, the terms of its h to shared memory.
+    auto build = [&](int at, int set) {
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // nobody is at the run before this one any more, whose set it takes
+      if (warp < 4) {
+        const Run r = run_at(p, at, end);
+        const int row = warp * 32 + lane;
+        ctl.token[set][row] = __ldcg(p.blocks.order + r.start + min(row, r.rows - 1));
+        if (row == 0) ctl.run[set] = r;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      const Run& r = ctl.run[set];
+      if (!r.multiply) return;
+      const int used = r.used, rows = r.rows;
+      const float scaling = p.scalings != nullptr ? __ldg(p.scalings + r.adapter) : 1.f;
+      const float* h = p.h + r.slice * p.R;
+      for (int row = warp; row < rows; row += 8) {
+        const uint32_t at_row = (uint32_t)row * 128;
+        const float inv = split_row<T>(h + (int64_t)ctl.token[set][row] * p.S * p.R, used, scaling, (used + 15) / 16 * 16, lane,
+                                       [&](int k, uint16_t hi, uint16_t lo) {
+                                         const uint32_t o = (k >> 6) * kSpan + at_row + ((((k >> 3) & 7) ^ (row & 7)) << 4) + (k & 7) * 2;
+                                         *reinterpret_cast<uint16_t*>(spans + o) = hi;
+                                         *reinterpret_cast<uint16_t*>(spans + kKB * kSpan + o) = lo;
+                                       });
+        if (lane == 0) ctl.unscale[set][row] = inv;
+      }
+      ptx::fence_async_smem();
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (lane == 0) ptx::mbar_arrive(h_full);
+    };
+    const int row_mine = quarter * 32 + g, col_mine = wide * 64 + q * 8;
+    // Base of tile c of the run of `set`.
+    auto load_base = [&](int c, int set) {
+      const Run& r = ctl.run[set];
+      if (!r.multiply && p.in_place) return;
+      const int n = r.column + c * kCols + col_mine, rows = r.rows, stop = r.end;
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = row_mine + hh * 16 + e * 8;
+          const T* from = static_cast<const T*>(p.base) + (int64_t)ctl.token[set][row] * p.ld_base + n;
+#pragma unroll
+          for (int a = 0; a < 2; ++a)
+            old[hh][e][a] = row < rows && n + a * 32 < stop ? *reinterpret_cast<const uint4*>(from + a * 32) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    if (begin < end) build(begin, 0), load_base(0, 0);
+    for (int at = begin; at < end; ++runs) {
+      const int set = runs & 1;
+      const Run& r = ctl.run[set];
+      const int count = r.count, rows = r.rows;
+      const bool multiply = r.multiply, keep = !multiply && p.in_place;
+      at += count;
+      for (int c = 0; c < count; ++c) {
+        const bool last = c + 1 == count;
+        const int buf = i & 1;
+        // (a wait that ran out ends the waiting and storing, not the loops: the warps meet in `build`)
+        if (multiply && ok) {
+          ok = LORA_WAIT(acc_full + buf * 8, (i >> 1) & 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) *abort_flag = 1;
+        }
+        if (last && at < end) build(at, set ^ 1);  // this run's products are done: the next one's h may take the place of its
+        if (ok) {
+          ptx::tc_fence_after();
+          const int n = r.column + c * kCols + col_mine, stop = r.end;
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+              uint32_t sum[16];
+              __syncwarp();
+              if (multiply) {
+                ptx::tmem_ld_16x256<4>(lanes + ((uint32_t)(hh * 16) << 16) + buf * kCols + a * 32, sum);
+                ptx::tmem_ld_wait();
+                if (hh == 1 && a == 1) {
+                  ptx::tc_fence_before();
+                  __syncwarp();
+                  if (lane == 0) ptx::mbar_arrive(acc_empty + buf * 8);
+                }
+              }
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int row = row_mine + hh * 16 + e * 8;
+                if (row < rows && n + a * 32 < stop && !keep) {
+                  uint4 now = old[hh][e][a];
+                  if (multiply) {
+                    const float inv = ctl.unscale[set][row];
+                    uint32_t* w = reinterpret_cast<uint32_t*>(&now);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                      const uint16_t lo = (uint16_t)w[j], hi = (uint16_t)(w[j] >> 16);
+                      const float v0 = ElemTraits<T>::to_f32(*reinterpret_cast<const T*>(&lo)) + __uint_as_float(sum[4 * j + 2 * e]) * inv;
+                      const float v1 = ElemTraits<T>::to_f32(*reinterpret_cast<const T*>(&hi)) + __uint_as_float(sum[4 * j + 2 * e + 1]) * inv;
+                      w[j] = bits(ElemTraits<T>::from_f32(v0)) | (uint32_t)bits(ElemTraits<T>::from_f32(v1)) << 16;
+                    }
+                  }
+                  *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)ctl.token[set][row] * p.ld_out + n + a * 32) = now;
+                }
+              }
+            }
+        }
+        if (multiply) ++i;
+        if (!last) load_base(c + 1, set); else if (at < end) load_base(0, set ^ 1);
+      }
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (ctl.abort_flag != 0 && tid == 0) atomicExch(&g_lora_tile_status, 1);
+  if (warp == 9) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, 2 * kCols);
+  }
+}
+
+template <typename T, int kKB>
+int launch(const Params& p, cudaStream_t st) {
+  auto kern = expand_tile_kernel<T, kKB>;
+  static thread_local bool attr_set[64] = {false};  // the opt-in is per function and per device
+  int dev = 0;
+  SGLB_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    SGLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem<kKB>));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  const int64_t tiles = (int64_t)p.max_blocks * p.chunk0[p.S], ctas = (kKB == 1 ? 2 : 1) * sm_count();
+  SGLB_REQUIRE(tiles < (1ll << 31), "lora_add: %lld tiles are too many", (long long)tiles);
+  SGLB_CUDA(launch_pdl(kern, (unsigned)std::min(tiles, ctas), kThreads, (size_t)kSmem<kKB>, st, p));
+  return SGLB200_OK;
+}
+
+}  // namespace
+
+int expand_tile(Params& p, int dtype, cudaStream_t st) {
+  int tiles = 0;
+  for (int s = 0; s < p.S; ++s) {
+    p.chunk0[s] = tiles;
+    tiles += (int)((p.col0[s + 1] - p.col0[s] + kCols - 1) / kCols);
+  }
+  p.chunk0[p.S] = tiles;
+  if (p.R <= 64) return dtype == 0 ? launch<__nv_bfloat16, 1>(p, st) : launch<__half, 1>(p, st);
+  return dtype == 0 ? launch<__nv_bfloat16, 2>(p, st) : launch<__half, 2>(p, st);
+}
+
+int tile_status() {
+  int v = 0;
+  return cudaMemcpyFromSymbol(&v, g_lora_tile_status, sizeof(int)) != cudaSuccess ? -1 : v;
+}
+int tile_status_clear() {
+  const int zero = 0;
+  SGLB_CUDA(cudaMemcpyToSymbol(g_lora_tile_status, &zero, sizeof(int)));
+  return SGLB200_OK;
+}
+
+}  // namespace lora
+}  // namespace sglb200

@@ -31,7 +31,7 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 // kG groups of 8 activation rows.  `part` and `sums` are padded so that neither their writes nor their reads meet in a bank: unpadded,
 // 64 rows x 256 x 7168 took 12.8 us.
 template <typename T, int kG>
-__global__ void __launch_bounds__(kWarps * 32) narrow_kernel(const Params p) {
+__global__ void __launch_bounds__(kWarps * 32, 2) narrow_kernel(const Params p) {
   constexpr int kCols = kG * 8, kPartPitch = kCols + 8, kSumPitch = 17;
   __shared__ float part[kWarps][16][kPartPitch];
   __shared__ float sums[kCols * kSumPitch];
@@ -160,7 +160,8 @@ static int dispatch(Params& p, int64_t blocks, cudaStream_t st) {
   p.n_tiles = (int)((p.N + 15) / 16);
   const int64_t tiles = blocks * p.n_tiles, steps = (p.K + kStep - 1) / kStep;
   p.splits = 1;
-  while (p.splits < 8 && tiles * p.splits * 2 <= 2 * sm_count() && steps >= p.splits * 2 * kWarps) p.splits *= 2;
+  // (two CTAs an SM: clusters that do not run at once would take a second round)
+  while (p.splits < 8 && tiles <= cluster_fits().paired[p.splits * 2] && steps >= p.splits * 2 * kWarps) p.splits *= 2;
   if (p.T <= 8) return launch<T, 1>(p, blocks, st);
   if (p.T <= 16) return launch<T, 2>(p, blocks, st);
   if (p.T <= 32) return launch<T, 4>(p, blocks, st);

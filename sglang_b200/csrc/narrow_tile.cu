@@ -1,7 +1,8 @@
 // y[t, n] = sum_k x[t, k] w[n, k] for many rows (see narrow.cuh), on tcgen05.mma.kind::f16.
 //
-// A tile is 128 activation rows by up to 256 weight rows; both operands come by TMA in stages of 64 columns, the activations of sorted rows
-// by gathers of four.  K is split over the CTAs of a cluster, which add their sums through distributed shared memory in a fixed order.
+// A tile is 128 activation rows by up to 256 weight rows, in stages of 64 columns.  The weights, and activations that lie one after the
+// other, come by TMA; sorted activations by asynchronous copies of 16 bytes of two warps (TMA gathers of four rows took 2 us a stage of 128
+// rows: 4096 rows of 7168 columns 55 us).  K is split over the CTAs of a cluster, which add their sums through distributed shared memory in a fixed order.
 //
 // The instruction cuts off what does not fit its sum, each time: over 7168 columns that would be off by more than a float32 product is.  So
 // the sums of 256 columns begin from zero, in two buffers of tensor memory in turn, and meet in the registers of eight warps.
@@ -16,10 +17,11 @@ namespace narrow {
 
 __device__ int g_tile_status = 0;  // 0 ok, 1 = a pipeline wait expired
 
-constexpr int kThreads = 320;      // eight warps for the sums, one that loads, one that multiplies
+constexpr int kThreads = 384;      // eight warps for the sums, one that loads, one that multiplies, two that copy sorted rows
+constexpr int kLag = 3;            // stages of copies in flight behind the one that is issued
 constexpr int kStageK = 64;        // columns of a stage: 128 bytes, one swizzle span
 constexpr int kChunk = 4;          // stages that are summed up in tensor memory
-constexpr int kMaxStages = 8;
+constexpr int kMaxStages = 8;      // (four at least: more than kLag)
 constexpr uint32_t kRing = 192 * 1024;
 constexpr uint32_t kXBytes = kTileBlock * kStageK * 2;
 
@@ -67,10 +69,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = &ctl->abort_flag;
   const int rank = (int)(blockIdx.x % p.splits), n0 = (int)(blockIdx.x / p.splits % p.n_tiles) * t.nt;
   const int64_t block = blockIdx.x / p.splits / p.n_tiles;
+  const bool sorted = p.blocks.order != nullptr;
   const uint32_t full = ptx::smem_u32(ctl->full), empty = ptx::smem_u32(ctl->empty), acc_full = ptx::smem_u32(ctl->acc_full),
                  acc_empty = ptx::smem_u32(ctl->acc_empty);
   if (tid == 0) {
-    for (int s = 0; s < t.stages; ++s) ptx::mbar_init(full + s * 8, 1), ptx::mbar_init(empty + s * 8, 1);
+    for (int s = 0; s < t.stages; ++s) ptx::mbar_init(full + s * 8, sorted ? 3 : 1), ptx::mbar_init(empty + s * 8, 1);
     for (int b = 0; b < 2; ++b) ptx::mbar_init(acc_full + b * 8, 1), ptx::mbar_init(acc_empty + b * 8, 8);
     ctl->abort_flag = 0;
     ptx::mbar_fence_init();
@@ -79,7 +82,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   ptx::grid_dependency_wait();
   int64_t start = block * kTileBlock;
   int rows = (int)min((int64_t)kTileBlock, p.T - start), adapter = 0;
-  if (p.blocks.order != nullptr) {
+  if (sorted) {
     const bool there = block < __ldcg(p.blocks.count);  // (uniform over the cluster)
     adapter = there ? __ldcg(p.blocks.adapter + block) : -1;
     if (adapter < 0) {
@@ -102,29 +105,64 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int units = t.nt / 16, half = (units + 1) / 2;
 
   if (warp == 8) {
-    const bool gather = p.blocks.order != nullptr;
-    int r[4];
-    if (gather)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = __ldcg(p.blocks.order + start + min(lane * 4 + i, rows - 1));
-    const bool mine = lane * 4 < rows;  // (rows past the last hold what they held; their sums are nobody's)
-    const uint32_t x_bytes = gather ? (uint32_t)((rows + 3) / 4 * 4) * kStageK * 2 : kXBytes;
-    for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
-      const int s = i % t.stages;
-      bool ok = true;
-      if (i >= t.stages) ok = NARROW_WAIT(empty + s * 8, ((i / t.stages) & 1) ^ 1);
-      if (!__all_sync(0xffffffffu, ok)) {
-        if (lane == 0) *abort_flag = 1;
-        break;
-      }
-      const uint32_t at = base + s * stage_bytes, bar = full + s * 8;
-      if (lane == 0) {
-        ptx::mbar_arrive_expect_tx(bar, x_bytes + w_bytes);
+    if (ptx::elect_one()) {
+      for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+        const int s = i % t.stages;
+        if (i >= t.stages && !NARROW_WAIT(empty + s * 8, ((i / t.stages) & 1) ^ 1)) {
+          *abort_flag = 1;
+          break;
+        }
+        const uint32_t at = base + s * stage_bytes, bar = full + s * 8;
+        ptx::mbar_arrive_expect_tx(bar, sorted ? w_bytes : kXBytes + w_bytes);
         ptx::tma_load_3d(at + kXBytes, &map_w, bar, kb * kStageK * 2, n0, adapter);
-        if (!gather) ptx::tma_load_2d(at, &map_x, bar, kb * kStageK * 2, (int)start);
+        if (!sorted) ptx::tma_load_2d(at, &map_x, bar, kb * kStageK * 2, (int)start);
       }
-      __syncwarp();
-      if (gather && mine) ptx::tma_gather4(at + lane * (4 * kStageK * 2), &map_x, bar, kb * kStageK * 2, r[0], r[1], r[2], r[3]);
+    }
+    __syncwarp();
+  } else if (warp >= 10) {
+    if (sorted) {
+      // Rows warp, + 2, .. of four at a time; a lane has 16 bytes of one of them.  (Rows past the last hold what they held; their sums are
+      // nobody's.)
+      const int c = lane & 7, r0 = (warp - 10) * 4 + (lane >> 3);
+      const uint8_t* from[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        from[j] = static_cast<const uint8_t*>(p.x) + (int64_t)__ldcg(p.blocks.order + start + min(r0 + j * 8, rows - 1)) * p.ldx * 2 + c * 16;
+      const uint32_t to = (uint32_t)(r0 * 128 + ((c ^ (r0 & 7)) << 4));  // (rows 8 apart have the same swizzle)
+      const int stages_here = kb1 - kb0;
+      auto landed = [&](int i) {
+        ptx::fence_async_smem();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(full + (i % t.stages) * 8);
+      };
+      bool ok = true;
+      int i = 0;
+      for (; i < stages_here; ++i) {
+        const int s = i % t.stages;
+        if (i >= t.stages) ok = NARROW_WAIT(empty + s * 8, ((i / t.stages) & 1) ^ 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const int64_t k = (int64_t)(kb0 + i) * kStageK;
+        const uint32_t bytes = k + c * 8 < p.K ? 16 : 0;  // (K is a multiple of 8; zeros beyond)
+        const int64_t off = bytes ? k * 2 : 0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (r0 + j * 8 < rows)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + s * stage_bytes + to + j * 1024), "l"(from[j] + off),
+                         "r"(bytes)
+                         : "memory");
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (i >= kLag) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+          landed(i - kLag);
+        }
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      if (ok) {
+        for (int j = max(0, stages_here - kLag); j < stages_here; ++j) landed(j);
+      } else if (lane == 0) {
+        *abort_flag = 1;
+      }
     }
     __syncwarp();
   } else if (warp == 9) {
@@ -288,9 +326,8 @@ int tile_product(const Params& given, int dtype, int64_t max_blocks, cudaStream_
     if (tiles <= fits.alone[s] && t.kb_total >= s * kChunk) p.splits = s;
   t.stages = (int)std::min<uint32_t>(kMaxStages, kRing / (kXBytes + (uint32_t)t.nt * kStageK * 2));
   CUtensorMap mx, mw;
-  const bool gather = p.blocks.order != nullptr;
   const uint64_t xd[2] = {(uint64_t)p.K * 2, (uint64_t)p.T}, xs[1] = {(uint64_t)p.ldx * 2};
-  const uint32_t xb[2] = {kStageK * 2, gather ? 1u : (uint32_t)kTileBlock};
+  const uint32_t xb[2] = {kStageK * 2, (uint32_t)kTileBlock};
   int rc = get_tile_map(p.x, 2, xd, xs, xb, true, &mx);
   if (rc) return rc;
   const uint64_t wd[3] = {(uint64_t)p.K * 2, (uint64_t)p.N, (uint64_t)p.adapters}, ws[2] = {(uint64_t)p.K * 2, (uint64_t)(p.N * p.K * 2)};

@@ -181,11 +181,24 @@ __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
   __syncthreads();  // (the tokens)
   if (c0 < end) load_base(c0, 0, old);
   const float scaling = adapter >= 0 && p.scalings != nullptr ? __ldg(p.scalings + adapter) : 1.f;
-  for (int i = warp; i < rows; i += kWarps) {
-    uint16_t* at = reinterpret_cast<uint16_t*>(tile + i * p.pitch);
-    const float inv = split_row<T>(p.h + ((int64_t)token[row0 + i] * p.S + slice) * p.R, used, scaling, p.R, lane,
-                                   [&](int r, uint16_t hi, uint16_t lo) { at[r] = hi, at[p.R + r] = lo; });
-    if (lane == 0) unscale[i] = inv;
+  // (two rows' loads at a time)
+  constexpr int kV = (kSteps + 1) / 2;
+  for (int i = warp; i < rows; i += 2 * kWarps) {
+    float v[2][kV];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float* h = p.h + ((int64_t)token[row0 + min(i + u * kWarps, rows - 1)] * p.S + slice) * p.R;
+#pragma unroll
+      for (int j = 0; j < kV; ++j) v[u][j] = j * 32 + lane < used ? __ldcg(h + j * 32 + lane) * scaling : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int row = i + u * kWarps;
+      if (row >= rows) break;
+      uint16_t* at = reinterpret_cast<uint16_t*>(tile + row * p.pitch);
+      const float inv = split_row<T>(v[u], p.R, lane, [&](int r, uint16_t hi, uint16_t lo) { at[r] = hi, at[p.R + r] = lo; });
+      if (lane == 0) unscale[row] = inv;
+    }
   }
   __syncthreads();
   const int steps = (used + 15) / 16;
@@ -232,13 +245,11 @@ __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
         uint32_t now[kTiles];
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) {
-          const uint16_t lo = (uint16_t)old[i][j], hi = (uint16_t)(old[i][j] >> 16);
           if (used == 0) {
             now[j] = old[i][j];
           } else {
-            const float v0 = ElemTraits<T>::to_f32(*reinterpret_cast<const T*>(&lo)) + acc[j][2 * i] * inv;
-            const float v1 = ElemTraits<T>::to_f32(*reinterpret_cast<const T*>(&hi)) + acc[j][2 * i + 1] * inv;
-            now[j] = bits(ElemTraits<T>::from_f32(v0)) | (uint32_t)bits(ElemTraits<T>::from_f32(v1)) << 16;
+            const float2 was = unpack2<T>(old[i][j]);
+            now[j] = pack2<T>(was.x + acc[j][2 * i] * inv, was.y + acc[j][2 * i + 1] * inv);
           }
         }
         if (p.vec) {

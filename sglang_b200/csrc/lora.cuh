@@ -33,23 +33,36 @@ __device__ __forceinline__ uint16_t bits(T v) {
   return *reinterpret_cast<const uint16_t*>(&v);
 }
 
-// A row of h times `scaling` -> two terms of a 16-bit type, times a power of two, whose inverse is returned; put(r, high, low) for r below
-// `width` (zeros from `used` on).  One warp.
-template <typename T, class Put>
-__device__ __forceinline__ float split_row(const float* h, int used, float scaling, int width, int lane, Put put) {
-  float v[kMaxRank / 32], most = 0.f;
-#pragma unroll
-  for (int j = 0; j < kMaxRank / 32; ++j) {
-    const int r = j * 32 + lane;
-    v[j] = r < used ? __ldcg(h + r) * scaling : 0.f;
-    most = fmaxf(most, fabsf(v[j]));
+// Two neighbouring 16-bit values as floats, and back, rounded to nearest.
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
   }
+}
+
+// A row of h times `scaling`, value j * 32 + lane in v[j] -> two terms of a 16-bit type, times a power of two, whose inverse is returned;
+// put(r, high, low) for r below `width`.  One warp.
+template <typename T, int kV, class Put>
+__device__ __forceinline__ float split_row(const float (&v)[kV], int width, int lane, Put put) {
+  float most = 0.f;
+#pragma unroll
+  for (int j = 0; j < kV; ++j) most = fmaxf(most, fabsf(v[j]));
   const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
   const uint32_t e = min(top >> 23, 253u);
   const bool plain = e == 0 || top >= 0x7f800000u;  // nothing to bring anywhere
   const float f = plain ? 1.f : __uint_as_float((254u - e) << 23);
 #pragma unroll
-  for (int j = 0; j < kMaxRank / 32; ++j) {
+  for (int j = 0; j < kV; ++j) {
     const int r = j * 32 + lane;
     if (r >= width) break;
     const float s = v[j] * f;

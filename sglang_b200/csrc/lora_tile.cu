@@ -22,7 +22,7 @@ namespace {
 
 constexpr int kRows = narrow::kTileBlock, kCols = 128;
 constexpr int kThreads = 320;  // eight warps that add and store, one that copies weights, one that multiplies: 96 registers with two CTAs an SM
-constexpr int kStages = 3, kLag = 1;
+constexpr int kStages = 3;
 constexpr uint32_t kSpan = 128 * 128;  // 128 rows of 64 columns of the rank, one swizzle span wide
 
 // kKB: spans of 64 columns of the rank.
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kThreads, kKB == 1 ? 2 : 1) expand_tile_kernel
   const uint32_t full = ptx::smem_u32(ctl.full), empty = ptx::smem_u32(ctl.empty), acc_full = ptx::smem_u32(ctl.acc_full),
                  acc_empty = ptx::smem_u32(ctl.acc_empty), h_full = ptx::smem_u32(&ctl.h_full);
   if (tid == 0) {
-    for (int s = 0; s < kStages; ++s) ptx::mbar_init(full + s * 8, 1), ptx::mbar_init(empty + s * 8, 1);
+    for (int s = 0; s < kStages; ++s) ptx::mbar_init(full + s * 8, 32), ptx::mbar_init(empty + s * 8, 1);
     for (int b = 0; b < 2; ++b) ptx::mbar_init(acc_full + b * 8, 1), ptx::mbar_init(acc_empty + b * 8, 8);
     ptx::mbar_init(h_full, 8);
     ctl.abort_flag = 0;
@@ -101,14 +101,8 @@ __global__ void __launch_bounds__(kThreads, kKB == 1 ? 2 : 1) expand_tile_kernel
 
   if (warp == 8) {
     // ------------------------------ weights: chunks of 16 bytes, row n to its place in the order above ------------------------------
-    int i = 0, landed = 0;
+    int i = 0;
     bool ok = true;
-    auto arrive = [&]() {
-      ptx::fence_async_smem();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(full + landed % kStages * 8);
-      ++landed;
-    };
     for (int at = begin; at < end && ok;) {
       const Run r = run_at(p, at, end);
       at += r.count;
@@ -122,35 +116,54 @@ __global__ void __launch_bounds__(kThreads, kKB == 1 ? 2 : 1) expand_tile_kernel
         if (!ok) break;
         const int n0 = r.column + c * kCols, cols = min(kCols, r.end - n0);
         const uint32_t to = ring + s * kKB * kSpan;
-        for (int id = lane; id < kCols * chunks; id += 32) {
-          const int n = id / chunks, k = id - n * chunks;
-          const int pos = (n & ~31) | ((n & 6) << 2) | ((n & 24) >> 2) | (n & 1);
-          const uint32_t dst = to + (k >> 3) * kSpan + pos * 128 + (((k & 7) ^ (pos & 7)) << 4);
-          const int left = n < cols ? r.used - k * 8 : 0;  // values that count of these eight
-          const T* src = weights + (int64_t)(n0 + n) * p.R + k * 8;
-          if (left <= 0 || left >= 8) {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(left > 0 ? src : weights), "r"(left > 0 ? 16 : 0) : "memory");
-          } else {  // (beyond the rank anything may stand)
-            uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
-            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+        if (cols == kCols && r.used % 8 == 0) {
+          // Lane l: 16 bytes l % 8 of every span of rows l / 8, + 4, ..; what the order makes of them differs by constants.
+          const int k = lane & 7, l = lane >> 3;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = 2 * j + 1 < left ? w[j] : 2 * j < left ? w[j] & 0xffffu : 0u;
-            ptx::sts_128(dst, v);
+          for (int span = 0; span < kKB; ++span) {
+            const int chunk = span * 8 + k;
+            if (chunk >= chunks) break;
+            const uint32_t bytes = chunk * 8 < r.used ? 16 : 0;
+            const T* src = bytes ? weights + (int64_t)(n0 + l) * p.R + chunk * 8 : weights;
+            const int64_t step = bytes ? 4 * p.R : 0;
+            const uint32_t dst = to + span * kSpan + ((l & 1) | (l & 2) << 2) * 128 + ((k ^ (l & 1)) << 4);
+#pragma unroll
+            for (int it = 0; it < kCols / 4; ++it) {
+              constexpr auto place = [](int n) { return (n & ~31) | ((n & 6) << 2) | ((n & 24) >> 2) | (n & 1); };
+              const uint32_t pos = place(it * 4);  // (a multiple of two, below 8 the bits that l does not set)
+              ptx::cp_async_16((dst + pos * 128) ^ ((pos & 7) << 4), src, bytes);
+              src += step;
+            }
+          }
+        } else {
+          for (int id = lane; id < kCols * chunks; id += 32) {
+            const int n = id / chunks, k = id - n * chunks;
+            const int pos = (n & ~31) | ((n & 6) << 2) | ((n & 24) >> 2) | (n & 1);
+            const uint32_t dst = to + (k >> 3) * kSpan + pos * 128 + (((k & 7) ^ (pos & 7)) << 4);
+            const int left = n < cols ? r.used - k * 8 : 0;  // values that count of these eight
+            const T* src = weights + (int64_t)(n0 + n) * p.R + k * 8;
+            if (left <= 0 || left >= 8) {
+              ptx::cp_async_16(dst, left > 0 ? src : weights, left > 0 ? 16 : 0);
+            } else {  // (beyond the rank anything may stand)
+              uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
+              uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) w[j] = 2 * j + 1 < left ? w[j] : 2 * j < left ? w[j] & 0xffffu : 0u;
+              ptx::sts_128(dst, v);
+            }
           }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (i >= kLag) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
-          arrive();
+        if (r.used % 8 == 0) {
+          ptx::cp_async_arrive(full + s * 8);
+        } else {  // (ordinary stores among them)
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          ptx::fence_async_smem();
+          ptx::mbar_arrive(full + s * 8);
         }
       }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (ok) {
-      while (landed < i) arrive();
-    } else if (lane == 0) {
-      *abort_flag = 1;
-    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (!ok && lane == 0) *abort_flag = 1;
     __syncwarp();
   } else if (warp == 9) {
     if (ptx::elect_one()) {
@@ -170,6 +183,7 @@ __global__ void __launch_bounds__(kThreads, kKB == 1 ? 2 : 1) expand_tile_kernel
           if (i >= 2) ok = LORA_WAIT(acc_empty + buf * 8, ((i >> 1) & 1) ^ 1);
           if (ok) ok = LORA_WAIT(full + s * 8, (i / kStages) & 1);
           if (!ok) break;
+          ptx::fence_async_smem();  // (the copies' writes, which the barrier has shown, before the tensor core's reads)
           ptx::tc_fence_after();
 #pragma unroll 1
           for (int term = 1; term >= 0; --term)  // the low terms first
@@ -212,38 +226,54 @@ __global__ void __launch_bounds__(kThreads, kKB == 1 ? 2 : 1) expand_tile_kernel
       const int used = r.used, rows = r.rows;
       const float scaling = p.scalings != nullptr ? __ldg(p.scalings + r.adapter) : 1.f;
       const float* h = p.h + r.slice * p.R;
-      for (int row = warp; row < rows; row += 8) {
-        const uint32_t at_row = (uint32_t)row * 128;
-        const float inv = split_row<T>(h + (int64_t)ctl.token[set][row] * p.S * p.R, used, scaling, (used + 15) / 16 * 16, lane,
-                                       [&](int k, uint16_t hi, uint16_t lo) {
-                                         const uint32_t o = (k >> 6) * kSpan + at_row + ((((k >> 3) & 7) ^ (row & 7)) << 4) + (k & 7) * 2;
-                                         *reinterpret_cast<uint16_t*>(spans + o) = hi;
-                                         *reinterpret_cast<uint16_t*>(spans + kKB * kSpan + o) = lo;
-                                       });
-        if (lane == 0) ctl.unscale[set][row] = inv;
+      // (eight rows' loads at a time: one after the other they took 16 us of a run)
+      for (int first = warp; first < rows; first += 64) {
+        float v[8][2 * kKB];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float* from = h + (int64_t)ctl.token[set][min(first + u * 8, rows - 1)] * p.S * p.R;
+#pragma unroll
+          for (int j = 0; j < 2 * kKB; ++j) v[u][j] = j * 32 + lane < used ? __ldcg(from + j * 32 + lane) : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int row = first + u * 8;
+          if (row >= rows) break;
+#pragma unroll
+          for (int j = 0; j < 2 * kKB; ++j) v[u][j] *= scaling;
+          const uint32_t at_row = (uint32_t)row * 128;
+          const float inv = split_row<T>(v[u], (used + 15) / 16 * 16, lane, [&](int k, uint16_t hi, uint16_t lo) {
+            const uint32_t o = (k >> 6) * kSpan + at_row + ((((k >> 3) & 7) ^ (row & 7)) << 4) + (k & 7) * 2;
+            *reinterpret_cast<uint16_t*>(spans + o) = hi;
+            *reinterpret_cast<uint16_t*>(spans + kKB * kSpan + o) = lo;
+          });
+          if (lane == 0) ctl.unscale[set][row] = inv;
+        }
       }
       ptx::fence_async_smem();
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (lane == 0) ptx::mbar_arrive(h_full);
     };
     const int row_mine = quarter * 32 + g, col_mine = wide * 64 + q * 8;
-    // Base of tile c of the run of `set`.
-    auto load_base = [&](int c, int set) {
+    // A quarter (16 rows, 32 columns) of the base of tile c of the run of `set`.
+    auto load_base = [&](int c, int set, int hh, int a) {
       const Run& r = ctl.run[set];
-      if (!r.multiply && p.in_place) return;
-      const int n = r.column + c * kCols + col_mine, rows = r.rows, stop = r.end;
+      const int n = r.column + c * kCols + col_mine + a * 32;
+      const bool on = n < r.end && (r.multiply || !p.in_place);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = row_mine + hh * 16 + e * 8;
+        old[hh][e][a] = on && row < r.rows ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + (int64_t)ctl.token[set][row] * p.ld_base + n)
+                                           : make_uint4(0, 0, 0, 0);
+      }
+    };
+    if (begin < end) {
+      build(begin, 0);
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int row = row_mine + hh * 16 + e * 8;
-          const T* from = static_cast<const T*>(p.base) + (int64_t)ctl.token[set][row] * p.ld_base + n;
-#pragma unroll
-          for (int a = 0; a < 2; ++a)
-            old[hh][e][a] = row < rows && n + a * 32 < stop ? *reinterpret_cast<const uint4*>(from + a * 32) : make_uint4(0, 0, 0, 0);
-        }
-    };
-    if (begin < end) build(begin, 0), load_base(0, 0);
+        for (int a = 0; a < 2; ++a) load_base(0, 0, hh, a);
+    }
     for (int at = begin; at < end; ++runs) {
       const int set = runs & 1;
       const Run& r = ctl.run[set];
@@ -260,47 +290,44 @@ __global__ void __launch_bounds__(kThreads, kKB == 1 ? 2 : 1) expand_tile_kernel
           if (!ok) *abort_flag = 1;
         }
         if (last && at < end) build(at, set ^ 1);  // this run's products are done: the next one's h may take the place of its
-        if (ok) {
-          ptx::tc_fence_after();
-          const int n = r.column + c * kCols + col_mine, stop = r.end;
+        ptx::tc_fence_after();
+        const int n = r.column + c * kCols + col_mine, stop = r.end;
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh)
+        for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-              uint32_t sum[16];
-              __syncwarp();
-              if (multiply) {
-                ptx::tmem_ld_16x256<4>(lanes + ((uint32_t)(hh * 16) << 16) + buf * kCols + a * 32, sum);
-                ptx::tmem_ld_wait();
-                if (hh == 1 && a == 1) {
-                  ptx::tc_fence_before();
-                  __syncwarp();
-                  if (lane == 0) ptx::mbar_arrive(acc_empty + buf * 8);
-                }
-              }
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int row = row_mine + hh * 16 + e * 8;
-                if (row < rows && n + a * 32 < stop && !keep) {
-                  uint4 now = old[hh][e][a];
-                  if (multiply) {
-                    const float inv = ctl.unscale[set][row];
-                    uint32_t* w = reinterpret_cast<uint32_t*>(&now);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                      const uint16_t lo = (uint16_t)w[j], hi = (uint16_t)(w[j] >> 16);
-                      const float v0 = ElemTraits<T>::to_f32(*reinterpret_cast<const T*>(&lo)) + __uint_as_float(sum[4 * j + 2 * e]) * inv;
-                      const float v1 = ElemTraits<T>::to_f32(*reinterpret_cast<const T*>(&hi)) + __uint_as_float(sum[4 * j + 2 * e + 1]) * inv;
-                      w[j] = bits(ElemTraits<T>::from_f32(v0)) | (uint32_t)bits(ElemTraits<T>::from_f32(v1)) << 16;
-                    }
-                  }
-                  *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)ctl.token[set][row] * p.ld_out + n + a * 32) = now;
-                }
+          for (int a = 0; a < 2; ++a) {
+            uint32_t sum[16];
+            __syncwarp();
+            if (multiply) {
+              ptx::tmem_ld_16x256<4>(lanes + ((uint32_t)(hh * 16) << 16) + buf * kCols + a * 32, sum);
+              ptx::tmem_ld_wait();
+              if (hh == 1 && a == 1) {
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(acc_empty + buf * 8);
               }
             }
-        }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int row = row_mine + hh * 16 + e * 8;
+              if (row < rows && n + a * 32 < stop && !keep && ok) {
+                uint4 now = old[hh][e][a];
+                if (multiply) {
+                  const float inv = ctl.unscale[set][row];
+                  uint32_t* w = reinterpret_cast<uint32_t*>(&now);
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) {
+                    const float2 was = unpack2<T>(w[j]);
+                    w[j] = pack2<T>(was.x + __uint_as_float(sum[4 * j + 2 * e]) * inv, was.y + __uint_as_float(sum[4 * j + 2 * e + 1]) * inv);
+                  }
+                }
+                *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)ctl.token[set][row] * p.ld_out + n + a * 32) = now;
+              }
+            }
+            // the quarter's place is free for the next tile's
+            if (!last) load_base(c + 1, set, hh, a); else if (at < end) load_base(0, set ^ 1, hh, a);
+          }
         if (multiply) ++i;
-        if (!last) load_base(c + 1, set); else if (at < end) load_base(0, set ^ 1);
       }
     }
   }

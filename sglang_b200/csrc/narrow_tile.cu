@@ -18,10 +18,9 @@ namespace narrow {
 __device__ int g_tile_status = 0;  // 0 ok, 1 = a pipeline wait expired
 
 constexpr int kThreads = 384;      // eight warps for the sums, one that loads, one that multiplies, two that copy sorted rows
-constexpr int kLag = 3;            // stages of copies in flight behind the one that is issued
 constexpr int kStageK = 64;        // columns of a stage: 128 bytes, one swizzle span
 constexpr int kChunk = 4;          // stages that are summed up in tensor memory
-constexpr int kMaxStages = 8;      // (four at least: more than kLag)
+constexpr int kMaxStages = 8;
 constexpr uint32_t kRing = 192 * 1024;
 constexpr uint32_t kXBytes = kTileBlock * kStageK * 2;
 
@@ -73,7 +72,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t full = ptx::smem_u32(ctl->full), empty = ptx::smem_u32(ctl->empty), acc_full = ptx::smem_u32(ctl->acc_full),
                  acc_empty = ptx::smem_u32(ctl->acc_empty);
   if (tid == 0) {
-    for (int s = 0; s < t.stages; ++s) ptx::mbar_init(full + s * 8, sorted ? 3 : 1), ptx::mbar_init(empty + s * 8, 1);
+    for (int s = 0; s < t.stages; ++s) ptx::mbar_init(full + s * 8, sorted ? 65 : 1), ptx::mbar_init(empty + s * 8, 1);
     for (int b = 0; b < 2; ++b) ptx::mbar_init(acc_full + b * 8, 1), ptx::mbar_init(acc_empty + b * 8, 8);
     ctl->abort_flag = 0;
     ptx::mbar_fence_init();
@@ -129,40 +128,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; j < 16; ++j)
         from[j] = static_cast<const uint8_t*>(p.x) + (int64_t)__ldcg(p.blocks.order + start + min(r0 + j * 8, rows - 1)) * p.ldx * 2 + c * 16;
       const uint32_t to = (uint32_t)(r0 * 128 + ((c ^ (r0 & 7)) << 4));  // (rows 8 apart have the same swizzle)
-      const int stages_here = kb1 - kb0;
-      auto landed = [&](int i) {
-        ptx::fence_async_smem();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(full + (i % t.stages) * 8);
-      };
-      bool ok = true;
-      int i = 0;
-      for (; i < stages_here; ++i) {
+      for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
         const int s = i % t.stages;
+        bool ok = true;
         if (i >= t.stages) ok = NARROW_WAIT(empty + s * 8, ((i / t.stages) & 1) ^ 1);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const int64_t k = (int64_t)(kb0 + i) * kStageK;
+        if (!__all_sync(0xffffffffu, ok)) {
+          if (lane == 0) *abort_flag = 1;
+          break;
+        }
+        const int64_t k = (int64_t)kb * kStageK;
         const uint32_t bytes = k + c * 8 < p.K ? 16 : 0;  // (K is a multiple of 8; zeros beyond)
         const int64_t off = bytes ? k * 2 : 0;
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-          if (r0 + j * 8 < rows)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + s * stage_bytes + to + j * 1024), "l"(from[j] + off),
-                         "r"(bytes)
-                         : "memory");
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (i >= kLag) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
-          landed(i - kLag);
-        }
+          if (r0 + j * 8 < rows) ptx::cp_async_16(base + s * stage_bytes + to + j * 1024, from[j] + off, bytes);
+        ptx::cp_async_arrive(full + s * 8);
       }
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-      if (ok) {
-        for (int j = max(0, stages_here - kLag); j < stages_here; ++j) landed(j);
-      } else if (lane == 0) {
-        *abort_flag = 1;
-      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
     __syncwarp();
   } else if (warp == 9) {
@@ -174,6 +156,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (i % kChunk == 0 && chunk >= 2) ok = NARROW_WAIT(acc_empty + buf * 8, ((chunk >> 1) & 1) ^ 1);
         if (ok) ok = NARROW_WAIT(full + s * 8, (i / t.stages) & 1);
         if (!ok) break;
+        if (sorted) ptx::fence_async_smem();  // (the copies' writes, which the barrier has shown, before the tensor core's reads)
         ptx::tc_fence_after();
         const uint32_t at = base + s * stage_bytes, x_lo = desc_lo(at), w_lo = desc_lo(at + kXBytes);
 #pragma unroll

@@ -28,6 +28,15 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// ---- asynchronous copies of 16 bytes (`bytes` of them read, the others zeros) that an mbarrier hears of -----------------------
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// One of the arrivals that the barrier was initialised for, once all copies that this thread has issued so far are in shared memory.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
 // Redistribution of the block's registers between warpgroups (four consecutive warps each, executed by all of them):
 // the sum over the warpgroups must not exceed what the block was launched with.
 template <int N>

@@ -401,6 +401,8 @@ extern "C" int sglb200_lora_add(const void* x, const void* lora_a, const void* l
   p.in_place = base == out && base_stride == out_stride;
   p.vec = even && N % 8 == 0 && base_stride % 8 == 0 && out_stride % 8 == 0 && aligned16(base) && aligned16(out);
   p.wait_probes = g_gemm_wait_probes;
-  if (block == narrow::kTileBlock && p.vec && rank <= lora::kTileRank) return lora::expand_tile(p, dtype, st);
+  // (its row pitches are 32-bit numbers of bytes)
+  if (block == narrow::kTileBlock && p.vec && rank <= lora::kTileRank && base_stride < 1ll << 30 && out_stride < 1ll << 30)
+    return lora::expand_tile(p, dtype, st);
   return dtype == 0 ? lora::expand<__nv_bfloat16>(p, block, st) : lora::expand<__half>(p, block, st);
 }

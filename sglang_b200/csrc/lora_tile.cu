@@ -1,12 +1,13 @@
 // The adapters' second product for many rows, out = base + h B^T (lora.cu), on tcgen05.mma.kind::f16: bound by reading base and writing out.
 //
-// A tile is 128 sorted tokens by 128 columns.  The tiles of all blocks, columns fastest, are cut evenly over two CTAs an SM (one, where the
-// rank is above 64), whatever the blocks' sizes; a CTA builds the two terms of h anew where a block or a merged projection begins.  One warp
-// copies the weights into a ring, one multiplies into two buffers of tensor memory, eight add base and store.
+// A tile is 128 sorted tokens by 128 columns.  The tiles of all blocks, columns fastest, are cut evenly over one CTA an SM, whatever the
+// blocks' sizes; a CTA builds the two terms of h anew where a block or a merged projection begins.  One warp copies the weights into a ring,
+// one multiplies into two buffers of tensor memory, sixteen add base and store.
 //
 // The columns of 32 are multiplied in the order i + 2 q + 8 j for column 8 q + 2 j + i: a lane that reads two neighbouring columns of each
-// eight from tensor memory then holds eight neighbouring ones of out, and base and out go by 16 bytes a lane, 64 a row.  The next tile's base is
-// asked for before this tile's sums are waited for.
+// eight from tensor memory then holds eight neighbouring ones of out, and base and out go by 16 bytes a lane, 64 a row.  Base comes by
+// asynchronous copies, each lane's to a place of its own, three tiles ahead (one, where the rank is above 64): loaded into registers, however
+// early, it was waited for in one piece, and 4096 tokens beside 36864 columns took 146 us and more.
 #include <algorithm>
 
 #include "gemm_common.cuh"
@@ -21,13 +22,17 @@ __device__ int g_lora_tile_status = 0;  // 0 ok, 1 = a pipeline wait expired
 namespace {
 
 constexpr int kRows = narrow::kTileBlock, kCols = 128;
-constexpr int kThreads = 320;  // eight warps that add and store, one that copies weights, one that multiplies: 96 registers with two CTAs an SM
-constexpr int kStages = 3;
+constexpr int kAdders = 16, kThreads = (kAdders + 2) * 32;  // warps that add and store, one that copies weights, one that multiplies
 constexpr uint32_t kSpan = 128 * 128;  // 128 rows of 64 columns of the rank, one swizzle span wide
 
 // kKB: spans of 64 columns of the rank.
 template <int kKB>
-constexpr uint32_t kSmem = 1024 + kKB * kSpan * (2 + kStages);
+struct Cfg {
+  static constexpr int kStages = kKB == 1 ? 3 : 2;  // of weights
+  static constexpr int kAhead = kKB == 1 ? 4 : 2;   // tiles of base
+  static constexpr uint32_t kBase = (2 + kStages) * kKB * kSpan, kSmem = 1024 + kBase + kAhead * kRows * kCols * 2;
+  static_assert(kSmem + 4096 <= 227 * 1024);
+};
 
 constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);  // rows of 128 bytes, 128-byte swizzle
 __device__ __forceinline__ uint32_t desc_lo(uint32_t smem) { return ((smem & 0x3ffffu) >> 4) | (1u << 16); }
@@ -61,16 +66,15 @@ __device__ __forceinline__ Run run_at(const Params& p, int at, int end) {
 }
 
 struct Ctl {
-  uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], h_full, h_empty;
+  uint64_t full[3], empty[3], acc_full[2], acc_empty[2], h_full;
   uint32_t tmem_base;
   int abort_flag;
   float unscale[2][kRows];
-  int32_t token[2][kRows];
-  Run run[2];
 };
 
 template <typename T, int kKB>
-__global__ void __launch_bounds__(kThreads, kKB == 1 ? 2 : 1) expand_tile_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 1) expand_tile_kernel(const Params p) {
+  constexpr int kStages = Cfg<kKB>::kStages, kAhead = Cfg<kKB>::kAhead;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Ctl ctl;
   uint8_t* spans = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -81,13 +85,13 @@ __global__ void __launch_bounds__(kThreads, kKB == 1 ? 2 : 1) expand_tile_kernel
                  acc_empty = ptx::smem_u32(ctl.acc_empty), h_full = ptx::smem_u32(&ctl.h_full);
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) ptx::mbar_init(full + s * 8, 32), ptx::mbar_init(empty + s * 8, 1);
-    for (int b = 0; b < 2; ++b) ptx::mbar_init(acc_full + b * 8, 1), ptx::mbar_init(acc_empty + b * 8, 8);
-    ptx::mbar_init(h_full, 8);
+    for (int b = 0; b < 2; ++b) ptx::mbar_init(acc_full + b * 8, 1), ptx::mbar_init(acc_empty + b * 8, kAdders);
+    ptx::mbar_init(h_full, kAdders);
     ctl.abort_flag = 0;
     ptx::mbar_fence_init();
   }
   ptx::grid_dependency_wait();
-  if (warp == 9) {
+  if (warp == kAdders + 1) {
     ptx::tmem_alloc(ptx::smem_u32(&ctl.tmem_base), 2 * kCols);
     ptx::tmem_relinquish();
   }
@@ -99,7 +103,7 @@ __global__ void __launch_bounds__(kThreads, kKB == 1 ? 2 : 1) expand_tile_kernel
   const int64_t all = (int64_t)__ldcg(p.blocks.count) * p.chunk0[p.S];
   const int begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
 
-  if (warp == 8) {
+  if (warp == kAdders) {
     // ------------------------------ weights: chunks of 16 bytes, row n to its place in the order above ------------------------------
     int i = 0;
     bool ok = true;
@@ -165,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, kKB == 1 ? 2 : 1) expand_tile_kernel
     asm volatile("cp.async.wait_all;" ::: "memory");
     if (!ok && lane == 0) *abort_flag = 1;
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp == kAdders + 1) {
     if (ptx::elect_one()) {
       constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
       constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10) | ((kCols >> 3) << 17) | ((kRows >> 4) << 24);
@@ -206,82 +210,93 @@ __global__ void __launch_bounds__(kThreads, kKB == 1 ? 2 : 1) expand_tile_kernel
     __syncwarp();
   } else {
     // ------------------------------ out = base + sums ------------------------------
-    const int g = lane >> 2, q = lane & 3, quarter = warp & 3, wide = warp >> 2;  // 32 rows and 64 columns of a tile
-    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + wide * 64;
-    int i = 0, runs = 0;
-    bool ok = true;
-    uint4 old[2][2][2];  // [16 rows][+ 8 rows][32 columns]
-    // The run at tile `at` becomes the one of `set`: its rows' tokens and factors there, the terms of its h to shared memory.
-    auto build = [&](int at, int set) {
-      asm volatile("bar.sync 1, 256;" ::: "memory");  // nobody is at the run before this one any more, whose set it takes
-      if (warp < 4) {
-        const Run r = run_at(p, at, end);
-        const int row = warp * 32 + lane;
-        ctl.token[set][row] = __ldcg(p.blocks.order + r.start + min(row, r.rows - 1));
-        if (row == 0) ctl.run[set] = r;
-      }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      const Run& r = ctl.run[set];
-      if (!r.multiply) return;
+    const int g = lane >> 2, q = lane & 3, quarter = warp & 3, wide = warp >> 2;  // 32 rows and 32 columns of a tile
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + wide * 32;
+    const int row_mine = quarter * 32 + g, col_mine = wide * 32 + q * 8;  // and the rows 8, 16 and 24 below
+    const uint32_t base_pitch = (uint32_t)(p.ld_base * 2), out_pitch = (uint32_t)(p.ld_out * 2);
+    const uint32_t mine = h_at + Cfg<kKB>::kBase + warp * 2048 + lane * 16;
+    // The terms of h of a run, and its rows' factors to `set`.
+    auto build = [&](const Run& r, int set) {
       const int used = r.used, rows = r.rows;
       const float scaling = p.scalings != nullptr ? __ldg(p.scalings + r.adapter) : 1.f;
       const float* h = p.h + r.slice * p.R;
-      // (eight rows' loads at a time: one after the other they took 16 us of a run)
-      for (int first = warp; first < rows; first += 64) {
-        float v[8][2 * kKB];
+      constexpr int kRowsHere = kRows / kAdders, kV = 2 * kKB;
+      float v[kRowsHere][kV];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const float* from = h + (int64_t)ctl.token[set][min(first + u * 8, rows - 1)] * p.S * p.R;
+      for (int u = 0; u < kRowsHere; ++u) {
+        const float* from = h + (int64_t)__ldcg(p.blocks.order + r.start + min(warp + u * kAdders, rows - 1)) * p.S * p.R;
 #pragma unroll
-          for (int j = 0; j < 2 * kKB; ++j) v[u][j] = j * 32 + lane < used ? __ldcg(from + j * 32 + lane) : 0.f;
-        }
+        for (int j = 0; j < kV; ++j) v[u][j] = j * 32 + lane < used ? __ldcg(from + j * 32 + lane) : 0.f;
+      }
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int row = first + u * 8;
-          if (row >= rows) break;
+      for (int u = 0; u < kRowsHere; ++u) {
+        const int row = warp + u * kAdders;
+        if (row >= rows) break;
 #pragma unroll
-          for (int j = 0; j < 2 * kKB; ++j) v[u][j] *= scaling;
-          const uint32_t at_row = (uint32_t)row * 128;
-          const float inv = split_row<T>(v[u], (used + 15) / 16 * 16, lane, [&](int k, uint16_t hi, uint16_t lo) {
-            const uint32_t o = (k >> 6) * kSpan + at_row + ((((k >> 3) & 7) ^ (row & 7)) << 4) + (k & 7) * 2;
-            *reinterpret_cast<uint16_t*>(spans + o) = hi;
-            *reinterpret_cast<uint16_t*>(spans + kKB * kSpan + o) = lo;
-          });
-          if (lane == 0) ctl.unscale[set][row] = inv;
-        }
+        for (int j = 0; j < kV; ++j) v[u][j] *= scaling;
+        const uint32_t at_row = (uint32_t)row * 128;
+        const float inv = split_row<T>(v[u], (used + 15) / 16 * 16, lane, [&](int k, uint16_t hi, uint16_t lo) {
+          const uint32_t o = (k >> 6) * kSpan + at_row + ((((k >> 3) & 7) ^ (row & 7)) << 4) + (k & 7) * 2;
+          *reinterpret_cast<uint16_t*>(spans + o) = hi;
+          *reinterpret_cast<uint16_t*>(spans + kKB * kSpan + o) = lo;
+        });
+        if (lane == 0) ctl.unscale[set][row] = inv;
       }
       ptx::fence_async_smem();
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(kAdders * 32) : "memory");
       if (lane == 0) ptx::mbar_arrive(h_full);
     };
-    const int row_mine = quarter * 32 + g, col_mine = wide * 64 + q * 8;
-    // A quarter (16 rows, 32 columns) of the base of tile c of the run of `set`.
-    auto load_base = [&](int c, int set, int hh, int a) {
-      const Run& r = ctl.run[set];
-      const int n = r.column + c * kCols + col_mine + a * 32;
-      const bool on = n < r.end && (r.multiply || !p.in_place);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int row = row_mine + hh * 16 + e * 8;
-        old[hh][e][a] = on && row < r.rows ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + (int64_t)ctl.token[set][row] * p.ld_base + n)
-                                           : make_uint4(0, 0, 0, 0);
-      }
+    // A run for a lane: its rows' tokens, its first column and where it stops (0: nothing to do).
+    struct Mine {
+      uint32_t token[4];
+      int rows, n, stop;
     };
-    if (begin < end) {
-      build(begin, 0);
+    auto open = [&](const Run& r, Mine& m) {
+      m.rows = r.rows - row_mine, m.n = r.column + col_mine, m.stop = r.multiply || !p.in_place ? r.end : 0;
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh)
+      for (int j = 0; j < 4; ++j) m.token[j] = j * 8 < m.rows ? (uint32_t)__ldcg(p.blocks.order + r.start + row_mine + j * 8) : 0u;
+    };
+    Mine ahead;
+    int ahead_at = begin, ahead_left = 0;
+    // Asks for the base of the next tile that has not been asked for, to place `slot`.
+    auto fetch = [&](int slot) {
+      if (ahead_at < end) {
+        if (ahead_left == 0) {
+          const Run r = run_at(p, ahead_at, end);
+          open(r, ahead);
+          ahead_left = r.count;
+        }
+        if (ahead.n < ahead.stop) {
+          const uint8_t* from = static_cast<const uint8_t*>(p.base) + (int64_t)ahead.n * 2;
 #pragma unroll
-        for (int a = 0; a < 2; ++a) load_base(0, 0, hh, a);
-    }
-    for (int at = begin; at < end; ++runs) {
-      const int set = runs & 1;
-      const Run& r = ctl.run[set];
-      const int count = r.count, rows = r.rows;
-      const bool multiply = r.multiply, keep = !multiply && p.in_place;
-      at += count;
-      for (int c = 0; c < count; ++c) {
-        const bool last = c + 1 == count;
+          for (int j = 0; j < 4; ++j)
+            if (j * 8 < ahead.rows) ptx::cp_async_16(mine + slot * (kRows * kCols * 2) + j * 512, from + (uint64_t)ahead.token[j] * base_pitch, 16);
+        }
+        ++ahead_at, --ahead_left, ahead.n += kCols;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int t = 0; t < kAhead - 1; ++t) fetch(t);
+    int i = 0, built = 0, slot = 0;
+    bool ok = true;
+    for (int at = begin; at < end;) {
+      const Run r = run_at(p, at, end);
+      Mine m;
+      open(r, m);
+      at += r.count;
+      const bool multiply = r.multiply;
+      float inv[4] = {};
+      if (multiply) {  // (the products of the run before are done: its last sums have been waited for)
+        build(r, built & 1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j * 8 < m.rows) inv[j] = ctl.unscale[built & 1][row_mine + j * 8];
+        ++built;
+      }
+      for (int c = 0; c < r.count; ++c, m.n += kCols) {
+        fetch(slot == 0 ? kAhead - 1 : slot - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
         const int buf = i & 1;
         // (a wait that ran out ends the waiting and storing, not the loops: the warps meet in `build`)
         if (multiply && ok) {
@@ -289,52 +304,50 @@ __global__ void __launch_bounds__(kThreads, kKB == 1 ? 2 : 1) expand_tile_kernel
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) *abort_flag = 1;
         }
-        if (last && at < end) build(at, set ^ 1);  // this run's products are done: the next one's h may take the place of its
         ptx::tc_fence_after();
-        const int n = r.column + c * kCols + col_mine, stop = r.end;
+        uint8_t* to = static_cast<uint8_t*>(p.out) + (int64_t)m.n * 2;
+        const bool store = m.n < m.stop && ok;
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-          for (int a = 0; a < 2; ++a) {
-            uint32_t sum[16];
-            __syncwarp();
-            if (multiply) {
-              ptx::tmem_ld_16x256<4>(lanes + ((uint32_t)(hh * 16) << 16) + buf * kCols + a * 32, sum);
-              ptx::tmem_ld_wait();
-              if (hh == 1 && a == 1) {
-                ptx::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(acc_empty + buf * 8);
-              }
+        for (int hh = 0; hh < 2; ++hh) {
+          uint32_t sum[16];
+          __syncwarp();
+          if (multiply) {
+            ptx::tmem_ld_16x256<4>(lanes + ((uint32_t)(hh * 16) << 16) + buf * kCols, sum);
+            ptx::tmem_ld_wait();
+            if (hh == 1) {
+              ptx::tc_fence_before();
+              __syncwarp();
+              if (lane == 0) ptx::mbar_arrive(acc_empty + buf * 8);
             }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int row = row_mine + hh * 16 + e * 8;
-              if (row < rows && n + a * 32 < stop && !keep && ok) {
-                uint4 now = old[hh][e][a];
-                if (multiply) {
-                  const float inv = ctl.unscale[set][row];
-                  uint32_t* w = reinterpret_cast<uint32_t*>(&now);
-#pragma unroll
-                  for (int j = 0; j < 4; ++j) {
-                    const float2 was = unpack2<T>(w[j]);
-                    w[j] = pack2<T>(was.x + __uint_as_float(sum[4 * j + 2 * e]) * inv, was.y + __uint_as_float(sum[4 * j + 2 * e + 1]) * inv);
-                  }
-                }
-                *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)ctl.token[set][row] * p.ld_out + n + a * 32) = now;
-              }
-            }
-            // the quarter's place is free for the next tile's
-            if (!last) load_base(c + 1, set, hh, a); else if (at < end) load_base(0, set ^ 1, hh, a);
           }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int j = 2 * hh + e;
+            if (store && j * 8 < m.rows) {
+              uint4 now = ptx::lds_128(mine + slot * (kRows * kCols * 2) + j * 512);
+              if (multiply) {
+                uint32_t* w = reinterpret_cast<uint32_t*>(&now);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  float2 v = unpack2<T>(w[k]);
+                  ptx::fma2(v.x, v.y, sum[4 * k + 2 * e], sum[4 * k + 2 * e + 1], inv[j]);
+                  w[k] = pack2<T>(v.x, v.y);
+                }
+              }
+              *reinterpret_cast<uint4*>(to + (uint64_t)m.token[j] * out_pitch) = now;
+            }
+          }
+        }
         if (multiply) ++i;
+        slot = slot + 1 == kAhead ? 0 : slot + 1;
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   ptx::tc_fence_before();
   __syncthreads();
   if (ctl.abort_flag != 0 && tid == 0) atomicExch(&g_lora_tile_status, 1);
-  if (warp == 9) {
+  if (warp == kAdders + 1) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem, 2 * kCols);
   }
@@ -347,12 +360,12 @@ int launch(const Params& p, cudaStream_t st) {
   int dev = 0;
   SGLB_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    SGLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem<kKB>));
+    SGLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<kKB>::kSmem));
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  const int64_t tiles = (int64_t)p.max_blocks * p.chunk0[p.S], ctas = (kKB == 1 ? 2 : 1) * sm_count();
+  const int64_t tiles = (int64_t)p.max_blocks * p.chunk0[p.S], ctas = sm_count();
   SGLB_REQUIRE(tiles < (1ll << 31), "lora_add: %lld tiles are too many", (long long)tiles);
-  SGLB_CUDA(launch_pdl(kern, (unsigned)std::min(tiles, ctas), kThreads, (size_t)kSmem<kKB>, st, p));
+  SGLB_CUDA(launch_pdl(kern, (unsigned)std::min(tiles, ctas), kThreads, (size_t)Cfg<kKB>::kSmem, st, p));
   return SGLB200_OK;
 }
 

@@ -5,11 +5,13 @@
 //
 // The order is that of the real numbers.  Without a bias it is the order of the logits.  Where scores decide it is taken in float32, which
 // tells two c apart that differ by more than `margin` (below); a row in which two neighbours of the order are closer than that, and are not
-// the same logit with the same bias, is decided once more in float64 by its warp.  With 256 experts that is one row in a few hundred.
+// the same logit with the same bias, is decided once more in float64 by its warp.  With 256 experts that is one row in some hundreds.
 //
-// One warp a row, the row in registers: lane l has consecutive experts of one group, so that a group's best come from its lanes' registers.
-// The picks are arg-maxima over the lanes' own best: one reduction over order-preserving bit patterns and one vote; a lane holds lower
-// experts than the next, so the lowest lane of equals has the lowest expert.
+// One warp a row, the row in registers: lane l has consecutive experts of one group.  It is bound by issue slots.  A lane sorts its
+// experts once, as integers: an order-preserving bit pattern of c, whose lowest bits give way to the expert's number in the lane (which the
+// margin allows for; 16-bit logits lose nothing).  A pick is then one reduction over the lanes' best, one vote and a shift of the winner's
+// list; a lane holds lower experts than the next, so the lowest lane of equals has the lowest expert.  16384 rows of 256 experts, best 8
+// in 4 of 8 groups: with the lanes' best looked for after every pick and scores by division, 1657 instructions a row and 33 us.
 #include <cfloat>
 
 #include "common.cuh"
@@ -53,13 +55,43 @@ __device__ __forceinline__ uint32_t to_ordered(float v) {
 }
 __device__ __forceinline__ float from_ordered(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
 
-// How far apart two c have to be for float32 to have their order right.  A sigmoid is off by at most s (1 - s) (2^-22 + 2^-24) of the
-// exponential (two units, and the sum beside it) and 2^-24 s of the quotient: below 2^-23.  A softmax by up to 2^-20 (the sum of up to
-// 1024 terms, the difference to the row's largest logit, the exponential, the quotient's two roundings).  Two of them, and a rounding of
-// each sum with the bias; a group's value is two c and one more rounding.
-__device__ __forceinline__ float margin(const Params& p, float a, float b) {
-  const float each = p.softmax ? 0x1p-20f : 0x1p-23f;
-  return (float)(2 * p.top) * (each + 0x1p-23f * fmaxf(fabsf(a), fabsf(b)));
+// How far apart two c have to be for float32 to have their order right.  A sigmoid is off by at most s (1 - s) of the exponential's relative
+// error (2^-22, and |x| 2^-24 from its argument, of which s (1 - s) |x| is below 1/4) and 2^-23 s of the reciprocal: below 2^-22.  A softmax
+// by up to 2^-19 (the sum of up to 1024 terms, the difference to the row's largest logit, the exponential, the quotient).  Scores of
+// logits whose lowest bits gave way: 2^-19 as well (up to 32 units of x, times s (1 - s)).  A rounding of the sum with the bias, and what the
+// number in the lane takes: `units` of 2^-23.  A group's value is up to two c, one more rounding and the group's number.
+__device__ __forceinline__ float margin(float each, int units, float a, float b) {
+  return 2.f * each + (float)(2 * units + 2) * 0x1p-23f * fmaxf(fabsf(a), fabsf(b));
+}
+
+// 2^x and 1 / x as the hardware gives them (2 units and 1 unit).
+__device__ __forceinline__ float fast_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kLog2e = 1.44269504f;
+
+// Descending, by Batcher's odd-even merges.
+template <int N>
+__device__ __forceinline__ void sort_keys(uint32_t (&v)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const uint32_t a = v[i + j], b = v[i + j + k];
+            v[i + j] = max(a, b), v[i + j + k] = min(a, b);
+          }
 }
 
 __device__ __forceinline__ double warp_max(double v) {
@@ -114,16 +146,23 @@ __device__ __forceinline__ V group_value(const Params& p, const V (&c)[kPer], V 
   return p.top == 2 && m2 > none ? m1 + m2 : m1;
 }
 
-// The row's picks in float64: lane i < k gets the i-th.  `kept_x`: the row's logits in shared memory.
-template <int kPer>
-__device__ __noinline__ int pick_exact(const Params& p, const float* kept_x, int lane) {
+// A logit as the order takes it: NaN is -inf, the largest is float32's.
+template <typename T>
+__device__ __forceinline__ float clean(T v) {
+  const float x = ElemTraits<T>::to_f32(v);
+  return x > kNone ? fminf(x, FLT_MAX) : kNone;
+}
+
+// The row's picks in float64: lane i < k gets the i-th.
+template <typename T, int kPer>
+__device__ __noinline__ int pick_exact(const Params& p, const T* x, int lane) {
   const Place at = place(p, lane);
   const double none = -INFINITY;
   double c[kPer];
   double mx = none, sum = 0.0;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    c[j] = j < at.count ? (double)kept_x[at.first + j] : none;
+    c[j] = j < at.count ? (double)clean(x[at.first + j]) : none;
     mx = fmax(mx, c[j]);
   }
   if (p.softmax) {
@@ -151,7 +190,7 @@ __device__ __noinline__ int pick_exact(const Params& p, const float* kept_x, int
   if (p.bias == nullptr) {  // (a score grows with its logit)
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
-      if (c[j] > none) c[j] = (double)kept_x[at.first + j];
+      if (c[j] > none) c[j] = (double)clean(x[at.first + j]);
   }
   int picked = -1;
   for (int i = 0; i < p.k; ++i) {
@@ -191,107 +230,125 @@ __device__ __forceinline__ void load_run(const T* at, int count, float (&v)[kPer
 
 template <typename T, int kPer>
 __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict__ logits, const Params p) {
-  extern __shared__ float smem[];  // per warp: the row's logits
+  constexpr uint32_t kIndex = kPer - 1;  // the bits of a key that hold the expert's number in the lane, the lowest on top
+  __shared__ int32_t picks[kWarps][kMaxTopk];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float* kept_x = smem + warp * p.E;
   const int64_t row = (int64_t)blockIdx.x * kWarps + warp;
   ptx::launch_dependents();
   ptx::grid_dependency_wait();
   if (row >= p.rows) return;
   const Place at = place(p, lane);
-  float x[kPer], c[kPer];
-  load_run<T, kPer>(logits + row * p.E + at.first, at.count, x);
-  const bool scored = p.bias != nullptr || p.top == 2;  // float32 decides, and may have to hand over to float64
-  float mx = kNone;
+  const T* logits_row = logits + row * p.E;
+  float x[kPer];
+  load_run<T, kPer>(logits_row + at.first, at.count, x);
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const bool live = j < at.count && x[j] > kNone;  // (false for a NaN)
-    x[j] = live ? fminf(x[j], FLT_MAX) : kNone;
-    if (j < at.count) kept_x[at.first + j] = x[j];
-    mx = fmaxf(mx, x[j]);
-  }
-  float inv = 0.f;
-  if (p.softmax && (scored || !p.renorm)) {
+  for (int j = 0; j < kPer; ++j) x[j] = j < at.count && x[j] > kNone ? fminf(x[j], FLT_MAX) : kNone;  // (false for a NaN)
+  const bool biased = p.bias != nullptr;
+  float mx = kNone, inv = 0.f;
+  if (p.softmax && (biased || p.top == 2 || !p.renorm)) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) mx = fmaxf(mx, x[j]);
     mx = warp_max(mx);
     float sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      c[j] = x[j] > kNone ? expf(x[j] - mx) : 0.f;
-      sum += c[j];
-    }
+    for (int j = 0; j < kPer; ++j) sum += x[j] > kNone ? fast_exp2((x[j] - mx) * kLog2e) : 0.f;
     sum = warp_sum(sum);
     inv = sum > 0.f ? 1.f / sum : 0.f;
   }
+  auto score = [&](float v) { return p.softmax ? fast_exp2((v - mx) * kLog2e) * inv : fast_rcp(1.f + fast_exp2(v * -kLog2e)); };
+  uint32_t key[kPer];  // descending; 0: not available
+  if (biased) {
+    float add[kPer];
+    load_run<float, kPer>(p.bias + at.first, at.count, add);
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    if (!scored) {
-      c[j] = x[j];
-    } else {
-      const float s = p.softmax ? c[j] * inv : 1.f / (1.f + expf(-x[j]));
-      const float v = s + (p.bias != nullptr && j < at.count ? p.bias[at.first + j] : 0.f);
-      c[j] = x[j] > kNone && v > kNone ? v : kNone;
+    for (int j = 0; j < kPer; ++j) {
+      const float c = score(x[j]) + add[j];
+      key[j] = x[j] > kNone && c > kNone ? (to_ordered(c) & ~kIndex) | (kIndex - j) : 0u;
     }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) key[j] = x[j] > kNone ? (to_ordered(x[j]) & ~kIndex) | (kIndex - j) : 0u;
   }
+  sort_keys<kPer>(key);
+
+  const float each = p.softmax ? 0x1p-19f : 0x1p-22f;
   bool close = false;
   if (p.groups > 1) {
-    const float value = group_value<kPer>(p, c, kNone);
-    float mine = __shfl_sync(kAll, value, (lane * p.group_lanes) & 31);
-    if (lane >= p.groups) mine = kNone;
-    const uint32_t keep = keep_groups<float>(p, mine, lane, kNone);
-    if (scored) {
-      const bool in = keep >> lane & 1u;
-      const float low = from_ordered(__reduce_min_sync(kAll, in ? to_ordered(mine) : kAll));
-      const float high = from_ordered(__reduce_max_sync(kAll, in ? 0u : to_ordered(mine)));
-      close = keep != kAll && high > kNone && !(low - high > margin(p, low, high));
+    // the group's two largest, in each of its lanes
+    uint32_t m1 = key[0], m2 = kPer > 1 ? key[kPer > 1 ? 1 : 0] : 0u;
+    for (int off = 1; off < p.group_lanes; off <<= 1) {
+      const uint32_t o1 = __shfl_xor_sync(kAll, m1, off), o2 = __shfl_xor_sync(kAll, m2, off);
+      m2 = max(max(m2, o2), min(m1, o1)), m1 = max(m1, o1);
+    }
+    m1 = __shfl_sync(kAll, m1, (lane * p.group_lanes) & 31), m2 = __shfl_sync(kAll, m2, (lane * p.group_lanes) & 31);
+    // lane g < groups: group g's value, the lower group on top of equals
+    float v1 = from_ordered(m1 & ~kIndex), v2 = from_ordered(m2 & ~kIndex);
+    // (the largest of what is added: a sum may be smaller than what it is off by)
+    const float reach = __uint_as_float(__reduce_max_sync(
+        kAll, lane < p.groups && m1 != 0u ? __float_as_uint(fmaxf(fabsf(v1), m2 != 0u && p.top == 2 ? fabsf(v2) : 0.f)) : 0u));
+    if (p.top == 2) {
+      if (!biased) v1 = score(v1), v2 = score(v2);
+      v1 = m2 != 0u ? v1 + v2 : v1;
+    }
+    const uint32_t exact = lane < p.groups && m1 != 0u ? to_ordered(v1) : 0u;
+    const uint32_t value = (exact & ~31u) | (31 - lane);
+    int beaten_by = 0;
+    for (int g = 0; g < p.groups; ++g) beaten_by += __shfl_sync(kAll, value, g) > value;
+    const uint32_t keep = __ballot_sync(kAll, lane < p.groups && beaten_by < p.kept);
+    // the last that stays and the first that goes have to be told apart
+    const bool in = keep >> lane & 1u;
+    const uint32_t low = __reduce_min_sync(kAll, in ? exact : kAll), high = __reduce_max_sync(kAll, in ? 0u : exact);
+    if (p.kept < p.groups && high != 0u) {
+      const float a = from_ordered(low), b = from_ordered(high);
+      if (biased) {
+        close = !(a - b > (float)p.top * margin(each, kPer + 34, reach, 0.f));
+      } else if (p.top == 2) {  // (scores of logits whose lowest bits gave way)
+        close = !(a - b > 2.f * margin(0x1p-19f + (p.softmax ? 0x1p-18f * reach : 0.f), kPer + 34, 1.f, 0.f));
+      } else if (sizeof(T) == 4) {
+        close = !(a - b > margin(0.f, kPer + 34, a, b));
+      }  // (16-bit logits lose nothing)
     }
     if (!(keep >> at.group & 1u))
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) c[j] = kNone;
+      for (int j = 0; j < kPer; ++j) key[j] = 0u;
   }
-  if (p.bias == nullptr && p.top == 2) {  // the groups' values were sums of scores; the logits order the experts
+
+  // The picks, best first: lane i keeps the i-th one's value, its expert goes through shared memory.
+  const bool inexact = biased || (sizeof(T) == 4 && kPer > 1);  // neighbours have to be told apart, the first that goes as well
+  const int looks = min(inexact ? p.k + 1 : p.k, 32);
+  uint32_t mine = 0u;
+  int count = 0;
+  for (; count < looks; ++count) {
+    const uint32_t head = key[0] & ~kIndex, top = __reduce_max_sync(kAll, head);
+    if (top == 0u) break;
+    const int winner = __ffs(__ballot_sync(kAll, head == top)) - 1;
+    if (lane == count) mine = top;
+    if (lane == winner) {
+      picks[warp][count] = at.first + (int)(kIndex - (key[0] & kIndex));
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) c[j] = c[j] > kNone ? x[j] : kNone;
+      for (int j = 0; j + 1 < kPer; ++j) key[j] = key[j + 1];
+      key[kPer - 1] = 0u;
+    }
   }
   __syncwarp();
-
-  float best;
-  int best_j;
-  auto look = [&]() {
-    best = kNone, best_j = 0;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if (c[j] > best) best = c[j], best_j = j;
-  };
-  look();
-  int picked = -1, last_e = 0;
-  float last = 0.f;
-  const int looks = p.bias != nullptr ? p.k + 1 : p.k;  // (the first that is not picked has to be told apart as well)
-  for (int i = 0; i < looks; ++i) {
-    const uint32_t key = to_ordered(best), top = __reduce_max_sync(kAll, key);
-    const float v = from_ordered(top);
-    if (!(v > kNone)) break;
-    const int winner = __ffs(__ballot_sync(kAll, key == top)) - 1;
-    const int e = __shfl_sync(kAll, at.first + best_j, winner);
-    if (p.bias != nullptr) {
-      if (i > 0 && !(last - v > margin(p, last, v)))
-        close = close || !(kept_x[last_e] == kept_x[e] && p.bias[last_e] == p.bias[e]);
-      last = v, last_e = e;
-    }
-    if (i == p.k) break;
-    if (lane == i) picked = e;
-    if (lane == winner) {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j)
-        if (j == best_j) c[j] = kNone;
-      look();
-    }
+  int picked = lane < count ? picks[warp][lane] : -1;
+  if (inexact) {
+    const uint32_t after = __shfl_down_sync(kAll, mine, 1);
+    const int after_e = __shfl_down_sync(kAll, picked, 1);
+    // (32 picks leave no lane for a 33rd look)
+    bool tell = lane + 1 < count && !(from_ordered(mine) - from_ordered(after) >
+                                      margin(biased ? each : 0.f, kPer, from_ordered(mine), from_ordered(after)));
+    if (tell)
+      tell = !(clean(logits_row[picked]) == clean(logits_row[after_e]) && (!biased || p.bias[picked] == p.bias[after_e]));
+    close = __any_sync(kAll, close || tell) || (p.k == 32 && count == 32);
   }
-  if (close) picked = pick_exact<kPer>(p, kept_x, lane);
+  if (close) picked = pick_exact<T, kPer>(p, logits_row, lane);
+  if (lane >= p.k) picked = -1;
 
   // Weights: the score, or its share of the picks' scores, for which the largest pick takes the place of the row's largest logit (softmax) or
   // of 0 (sigmoid = e^min(x, 0) / (1 + e^-|x|)): scores that are too small for float32 have shares all the same.
   const bool there = picked >= 0;
-  const float px = there ? kept_x[picked] : 0.f;
+  const float px = there ? clean(logits_row[picked]) : 0.f;
   float w;
   if (p.renorm) {
     const float num = p.softmax ? px : fminf(px, 0.f);
@@ -313,11 +370,10 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
 template <typename T>
 static int launch(const void* logits, const Params& p, cudaStream_t st) {
   const unsigned grid = (unsigned)((p.rows + kWarps - 1) / kWarps);
-  const size_t smem = (size_t)kWarps * p.E * sizeof(float);
   const T* x = static_cast<const T*>(logits);
 #define SGLB_ROUTE_CASE(P)                                                                    \
   if (p.per_lane <= P) {                                                                      \
-    SGLB_CUDA(launch_pdl(route_kernel<T, P>, grid, kWarps * 32, smem, st, x, p));             \
+    SGLB_CUDA(launch_pdl(route_kernel<T, P>, grid, kWarps * 32, (size_t)0, st, x, p));             \
     return SGLB200_OK;                                                                        \
   }
   SGLB_ROUTE_CASE(1) SGLB_ROUTE_CASE(2) SGLB_ROUTE_CASE(4) SGLB_ROUTE_CASE(8) SGLB_ROUTE_CASE(16) SGLB_ROUTE_CASE(32)

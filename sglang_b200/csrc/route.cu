@@ -12,6 +12,7 @@
 // margin allows for; 16-bit logits lose nothing).  A pick is then one reduction over the lanes' best, one vote and a shift of the winner's
 // list; a lane holds lower experts than the next, so the lowest lane of equals has the lowest expert.  16384 rows of 256 experts, best 8
 // in 4 of 8 groups: with the lanes' best looked for after every pick and scores by division, 1657 instructions a row and 33 us.
+#include <algorithm>
 #include <cfloat>
 
 #include "common.cuh"
@@ -94,12 +95,6 @@ __device__ __forceinline__ void sort_keys(uint32_t (&v)[N]) {
           }
 }
 
-__device__ __forceinline__ double warp_max(double v) {
-#pragma unroll
-  for (int m = 16; m > 0; m >>= 1) v = fmax(v, __shfl_xor_sync(kAll, v, m));
-  return v;
-}
-
 // Which group lane l's experts belong to, its first expert and how many it has.
 struct Place {
   int group, first, count;
@@ -113,37 +108,15 @@ __device__ __forceinline__ Place place(const Params& p, int lane) {
   return a;
 }
 
-// The kept groups, one bit each, by value and index.
+// The kept groups, one bit each, by value (lane g has group g's) and index.
 template <typename V>
-__device__ __forceinline__ uint32_t keep_groups(const Params& p, V mine, int lane, V none) {
+__device__ __forceinline__ uint32_t keep_groups(const Params& p, V mine, int lane) {
   int beaten_by = 0;
   for (int g = 0; g < p.groups; ++g) {
     const V other = __shfl_sync(kAll, mine, g);
     beaten_by += other > mine || (other == mine && g < lane);
   }
   return __ballot_sync(kAll, lane < p.groups && beaten_by < p.kept);
-}
-
-// The sum of a group's `top` largest values (of those that are there), in each of its lanes.
-template <int kPer, typename V>
-__device__ __forceinline__ V group_value(const Params& p, const V (&c)[kPer], V none) {
-  V m1 = none, m2 = none;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    if (c[j] > m1) {
-      m2 = m1, m1 = c[j];
-    } else if (c[j] > m2) {
-      m2 = c[j];
-    }
-  }
-  for (int off = 1; off < p.group_lanes; off <<= 1) {
-    const V o1 = __shfl_xor_sync(kAll, m1, off), o2 = __shfl_xor_sync(kAll, m2, off);
-    const V low = m1 < o1 ? m1 : o1;
-    m1 = m1 < o1 ? o1 : m1;
-    m2 = m2 < o2 ? o2 : m2;
-    m2 = m2 < low ? low : m2;
-  }
-  return p.top == 2 && m2 > none ? m1 + m2 : m1;
 }
 
 // A logit as the order takes it: NaN is -inf, the largest is float32's.
@@ -153,63 +126,112 @@ __device__ __forceinline__ float clean(T v) {
   return x > kNone ? fminf(x, FLT_MAX) : kNone;
 }
 
+// 64-bit patterns that compare like the doubles they come from; 0 is below them all.
+__device__ __forceinline__ uint64_t to_ordered64(double v) {
+  const uint64_t u = (uint64_t)__double_as_longlong(v + 0.0);
+  return u >> 63 ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ double from_ordered64(uint64_t u) { return __longlong_as_double((long long)(u >> 63 ? u & ~(1ull << 63) : ~u)); }
+__device__ __forceinline__ uint64_t warp_max64(uint64_t v) {
+  const uint32_t hi = __reduce_max_sync(kAll, (uint32_t)(v >> 32));
+  return (uint64_t)hi << 32 | __reduce_max_sync(kAll, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+}
+
+// c in float64, given the largest logit and the sum of a softmax.
+__device__ __forceinline__ double exact_c(const Params& p, float x, int e, double mx, double sum) {
+  const double s = p.softmax ? exp((double)x - mx) / sum : 1.0 / (1.0 + exp(-(double)x));
+  return p.bias != nullptr ? s + (double)p.bias[e] : s;
+}
+// The softmax's sum over the row.
+template <typename T>
+__device__ __forceinline__ double exact_sum(const Params& p, const T* x, double mx, int lane) {
+  double sum = 0.0;
+  for (int e = lane; e < p.E; e += 32) {
+    const float v = clean(x[e]);
+    if (v > kNone) sum += exp((double)v - mx);
+  }
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(kAll, sum, m);
+  return sum;
+}
+
 // The row's picks in float64: lane i < k gets the i-th.
 template <typename T, int kPer>
 __device__ __noinline__ int pick_exact(const Params& p, const T* x, int lane) {
   const Place at = place(p, lane);
-  const double none = -INFINITY;
-  double c[kPer];
-  double mx = none, sum = 0.0;
+  float v[kPer], mx = kNone;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    c[j] = j < at.count ? (double)clean(x[at.first + j]) : none;
-    mx = fmax(mx, c[j]);
+    v[j] = j < at.count ? clean(x[at.first + j]) : kNone;
+    mx = fmaxf(mx, v[j]);
   }
-  if (p.softmax) {
-    mx = warp_max(mx);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) sum += c[j] > none ? exp(c[j] - mx) : 0.0;
-#pragma unroll
-    for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(kAll, sum, m);
-  }
+  const bool biased = p.bias != nullptr, scored = biased || p.top == 2;
+  const double top = (double)warp_max(mx), sum = p.softmax && scored ? exact_sum(p, x, top, lane) : 0.0;
+  uint64_t c[kPer];  // (without a bias the logits' order: a score grows with its logit)
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    if (!(c[j] > none)) continue;
-    const double s = p.softmax ? exp(c[j] - mx) / sum : 1.0 / (1.0 + exp(-c[j]));
-    const double v = s + (p.bias != nullptr ? (double)p.bias[at.first + j] : 0.0);
-    c[j] = v > none ? v : none;
+    const double s = !(v[j] > kNone) ? -INFINITY : biased ? exact_c(p, v[j], at.first + j, top, sum) : (double)v[j];
+    c[j] = s > -INFINITY ? to_ordered64(s) : 0;
   }
   if (p.groups > 1) {
-    const double value = group_value<kPer>(p, c, none);
-    const double mine = __shfl_sync(kAll, value, (lane * p.group_lanes) & 31);
-    const uint32_t keep = keep_groups<double>(p, lane < p.groups ? mine : none, lane, none);
-    if (!(keep >> at.group & 1u))
+    uint64_t m1 = 0, m2 = 0;
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) c[j] = none;
-  }
-  if (p.bias == nullptr) {  // (a score grows with its logit)
+    for (int j = 0; j < kPer; ++j) m2 = max(m2, min(m1, c[j])), m1 = max(m1, c[j]);
+    for (int off = 1; off < p.group_lanes; off <<= 1) {
+      const uint64_t o1 = __shfl_xor_sync(kAll, m1, off), o2 = __shfl_xor_sync(kAll, m2, off);
+      m2 = max(max(m2, o2), min(m1, o1)), m1 = max(m1, o1);
+    }
+    uint64_t value = m1;
+    if (p.top == 2 && m1 != 0) {
+      double v1 = from_ordered64(m1), v2 = m2 != 0 ? from_ordered64(m2) : 0.0;
+      if (!biased) v1 = exact_c(p, (float)v1, 0, top, sum), v2 = m2 != 0 ? exact_c(p, (float)v2, 0, top, sum) : 0.0;
+      value = to_ordered64(v1 + v2);
+    }
+    const uint64_t mine = __shfl_sync(kAll, value, (lane * p.group_lanes) & 31);
+    if (!(keep_groups<uint64_t>(p, lane < p.groups ? mine : 0, lane) >> at.group & 1u))
 #pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if (c[j] > none) c[j] = (double)clean(x[at.first + j]);
+      for (int j = 0; j < kPer; ++j) c[j] = 0;
   }
   int picked = -1;
   for (int i = 0; i < p.k; ++i) {
-    double best = none;
-    int best_j = -1;
+    uint64_t best = 0;
+    int best_j = 0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
       if (c[j] > best) best = c[j], best_j = j;
-    const double top = warp_max(best);
-    if (!(top > none)) break;
-    const int winner = __ffs(__ballot_sync(kAll, best == top)) - 1;
+    const uint64_t winning = warp_max64(best);
+    if (winning == 0) break;
+    const int winner = __ffs(__ballot_sync(kAll, best == winning)) - 1;
     const int e = __shfl_sync(kAll, at.first + best_j, winner);
     if (lane == winner)
 #pragma unroll
       for (int j = 0; j < kPer; ++j)
-        if (j == best_j) c[j] = none;
+        if (j == best_j) c[j] = 0;
     if (lane == i) picked = e;
   }
   return picked;
+}
+
+// The `count` picks of the lanes (none left of those beyond in question) put in order by float64: lane i gets the i-th.
+template <typename T>
+__device__ __noinline__ int order_exact(const Params& p, const T* x, float mx, int picked, int count, int lane) {
+  const double sum = p.softmax && p.bias != nullptr ? exact_sum(p, x, (double)mx, lane) : 0.0;
+  uint64_t c = 0;
+  if (lane < count) {
+    const float v = clean(x[picked]);
+    c = to_ordered64(p.bias != nullptr ? exact_c(p, v, picked, (double)mx, sum) : (double)v);
+  }
+  int rank = 0, out = -1;
+  for (int i = 0; i < count; ++i) {
+    const uint64_t other = __shfl_sync(kAll, c, i);
+    const int e = __shfl_sync(kAll, picked, i);
+    rank += other > c || (other == c && e < picked);
+  }
+  for (int i = 0; i < count; ++i) {
+    const int r = __shfl_sync(kAll, rank, i), e = __shfl_sync(kAll, picked, i);
+    if (lane == r) out = e;
+  }
+  return out;
 }
 
 // A lane's `count` consecutive values at `at` of the row (the rest none), 16 bytes at a time where they lie so.
@@ -228,157 +250,172 @@ __device__ __forceinline__ void load_run(const T* at, int count, float (&v)[kPer
   }
 }
 
-template <typename T, int kPer>
+// kSoftmax: else sigmoid.
+template <typename T, int kPer, bool kSoftmax>
 __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict__ logits, const Params p) {
   constexpr uint32_t kIndex = kPer - 1;  // the bits of a key that hold the expert's number in the lane, the lowest on top
   __shared__ int32_t picks[kWarps][kMaxTopk];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = (int64_t)blockIdx.x * kWarps + warp;
   ptx::launch_dependents();
-  ptx::grid_dependency_wait();
-  if (row >= p.rows) return;
   const Place at = place(p, lane);
-  const T* logits_row = logits + row * p.E;
-  float x[kPer];
-  load_run<T, kPer>(logits_row + at.first, at.count, x);
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) x[j] = j < at.count && x[j] > kNone ? fminf(x[j], FLT_MAX) : kNone;  // (false for a NaN)
   const bool biased = p.bias != nullptr;
-  float mx = kNone, inv = 0.f;
-  if (p.softmax && (biased || p.top == 2 || !p.renorm)) {
+  const uint32_t there_mask = at.count >= 32 ? kAll : (1u << at.count) - 1;
+  ptx::grid_dependency_wait();
+  float add[kPer];
+  if (biased) load_run<float, kPer>(p.bias + at.first, at.count, add);
+  int64_t row = (int64_t)blockIdx.x * kWarps + warp;
+  const int64_t step = (int64_t)gridDim.x * kWarps;
+  float next[kPer];
+  if (row < p.rows) load_run<T, kPer>(logits + row * p.E + at.first, at.count, next);
+  for (; row < p.rows; row += step) {
+    const T* logits_row = logits + row * p.E;
+    float x[kPer];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) mx = fmaxf(mx, x[j]);
-    mx = warp_max(mx);
-    float sum = 0.f;
+    for (int j = 0; j < kPer; ++j) x[j] = (there_mask >> j & 1u) && next[j] > kNone ? fminf(next[j], FLT_MAX) : kNone;  // (false for a NaN)
+    if (row + step < p.rows) load_run<T, kPer>(logits_row + step * p.E + at.first, at.count, next);
+    float mx = kNone, inv = 0.f;
+    if (kSoftmax && (biased || p.top == 2 || !p.renorm)) {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) sum += x[j] > kNone ? fast_exp2((x[j] - mx) * kLog2e) : 0.f;
-    sum = warp_sum(sum);
-    inv = sum > 0.f ? 1.f / sum : 0.f;
-  }
-  auto score = [&](float v) { return p.softmax ? fast_exp2((v - mx) * kLog2e) * inv : fast_rcp(1.f + fast_exp2(v * -kLog2e)); };
-  uint32_t key[kPer];  // descending; 0: not available
-  if (biased) {
-    float add[kPer];
-    load_run<float, kPer>(p.bias + at.first, at.count, add);
+      for (int j = 0; j < kPer; ++j) mx = fmaxf(mx, x[j]);
+      mx = warp_max(mx);
+      float sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const float c = score(x[j]) + add[j];
-      key[j] = x[j] > kNone && c > kNone ? (to_ordered(c) & ~kIndex) | (kIndex - j) : 0u;
+      for (int j = 0; j < kPer; ++j) sum += x[j] > kNone ? fast_exp2((x[j] - mx) * kLog2e) : 0.f;
+      sum = warp_sum(sum);
+      inv = sum > 0.f ? 1.f / sum : 0.f;
     }
-  } else {
+    auto score = [&](float v) { return kSoftmax ? fast_exp2((v - mx) * kLog2e) * inv : fast_rcp(1.f + fast_exp2(v * -kLog2e)); };
+    uint32_t key[kPer];  // descending; 0: not available
+    if (biased) {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) key[j] = x[j] > kNone ? (to_ordered(x[j]) & ~kIndex) | (kIndex - j) : 0u;
-  }
-  sort_keys<kPer>(key);
+      for (int j = 0; j < kPer; ++j) {
+        const float c = score(x[j]) + add[j];
+        key[j] = x[j] > kNone && c > kNone ? (to_ordered(c) & ~kIndex) | (kIndex - j) : 0u;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) key[j] = x[j] > kNone ? (to_ordered(x[j]) & ~kIndex) | (kIndex - j) : 0u;
+    }
+    sort_keys<kPer>(key);
 
-  const float each = p.softmax ? 0x1p-19f : 0x1p-22f;
-  bool close = false;
-  if (p.groups > 1) {
-    // the group's two largest, in each of its lanes
-    uint32_t m1 = key[0], m2 = kPer > 1 ? key[kPer > 1 ? 1 : 0] : 0u;
-    for (int off = 1; off < p.group_lanes; off <<= 1) {
-      const uint32_t o1 = __shfl_xor_sync(kAll, m1, off), o2 = __shfl_xor_sync(kAll, m2, off);
-      m2 = max(max(m2, o2), min(m1, o1)), m1 = max(m1, o1);
-    }
-    m1 = __shfl_sync(kAll, m1, (lane * p.group_lanes) & 31), m2 = __shfl_sync(kAll, m2, (lane * p.group_lanes) & 31);
-    // lane g < groups: group g's value, the lower group on top of equals
-    float v1 = from_ordered(m1 & ~kIndex), v2 = from_ordered(m2 & ~kIndex);
-    // (the largest of what is added: a sum may be smaller than what it is off by)
-    const float reach = __uint_as_float(__reduce_max_sync(
-        kAll, lane < p.groups && m1 != 0u ? __float_as_uint(fmaxf(fabsf(v1), m2 != 0u && p.top == 2 ? fabsf(v2) : 0.f)) : 0u));
-    if (p.top == 2) {
-      if (!biased) v1 = score(v1), v2 = score(v2);
-      v1 = m2 != 0u ? v1 + v2 : v1;
-    }
-    const uint32_t exact = lane < p.groups && m1 != 0u ? to_ordered(v1) : 0u;
-    const uint32_t value = (exact & ~31u) | (31 - lane);
-    int beaten_by = 0;
-    for (int g = 0; g < p.groups; ++g) beaten_by += __shfl_sync(kAll, value, g) > value;
-    const uint32_t keep = __ballot_sync(kAll, lane < p.groups && beaten_by < p.kept);
-    // the last that stays and the first that goes have to be told apart
-    const bool in = keep >> lane & 1u;
-    const uint32_t low = __reduce_min_sync(kAll, in ? exact : kAll), high = __reduce_max_sync(kAll, in ? 0u : exact);
-    if (p.kept < p.groups && high != 0u) {
-      const float a = from_ordered(low), b = from_ordered(high);
-      if (biased) {
-        close = !(a - b > (float)p.top * margin(each, kPer + 34, reach, 0.f));
-      } else if (p.top == 2) {  // (scores of logits whose lowest bits gave way)
-        close = !(a - b > 2.f * margin(0x1p-19f + (p.softmax ? 0x1p-18f * reach : 0.f), kPer + 34, 1.f, 0.f));
-      } else if (sizeof(T) == 4) {
-        close = !(a - b > margin(0.f, kPer + 34, a, b));
-      }  // (16-bit logits lose nothing)
-    }
-    if (!(keep >> at.group & 1u))
+    constexpr float kEach = kSoftmax ? 0x1p-19f : 0x1p-22f;
+    bool redo = false;  // the row is decided in float64 from its groups on
+    if (p.groups > 1) {
+      // the group's two largest, in each of its lanes
+      uint32_t m1 = key[0], m2 = kPer > 1 ? key[kPer > 1 ? 1 : 0] : 0u;
+      for (int off = 1; off < p.group_lanes; off <<= 1) {
+        const uint32_t o1 = __shfl_xor_sync(kAll, m1, off), o2 = __shfl_xor_sync(kAll, m2, off);
+        m2 = max(max(m2, o2), min(m1, o1)), m1 = max(m1, o1);
+      }
+      m1 = __shfl_sync(kAll, m1, (lane * p.group_lanes) & 31), m2 = __shfl_sync(kAll, m2, (lane * p.group_lanes) & 31);
+      // lane g < groups: group g's value
+      float v1 = from_ordered(m1 & ~kIndex), v2 = from_ordered(m2 & ~kIndex);
+      // (the largest of what is added: a sum may be smaller than what it is off by)
+      const float reach = __uint_as_float(__reduce_max_sync(
+          kAll, lane < p.groups && m1 != 0u ? __float_as_uint(fmaxf(fabsf(v1), m2 != 0u && p.top == 2 ? fabsf(v2) : 0.f)) : 0u));
+      if (p.top == 2) {
+        if (!biased) v1 = score(v1), v2 = score(v2);
+        v1 = m2 != 0u ? v1 + v2 : v1;
+      }
+      const uint32_t value = lane < p.groups && m1 != 0u ? to_ordered(v1) : 0u;
+      const uint32_t keep = keep_groups<uint32_t>(p, value, lane);
+      // the last that stays and the first that goes have to be told apart
+      const bool in = keep >> lane & 1u;
+      const uint32_t low = __reduce_min_sync(kAll, in ? value : kAll), high = __reduce_max_sync(kAll, in ? 0u : value);
+      if (p.kept < p.groups && high != 0u) {
+        const float a = from_ordered(low), b = from_ordered(high);
+        if (biased) {
+          redo = !(a - b > (float)p.top * margin(kEach, kPer + 2, reach, 0.f));
+        } else if (p.top == 2) {  // (scores of logits whose lowest bits gave way)
+          redo = !(a - b > 2.f * margin(0x1p-19f + (kSoftmax ? 0x1p-18f * reach : 0.f), kPer + 2, 1.f, 0.f));
+        } else if (sizeof(T) == 4) {
+          redo = !(a - b > margin(0.f, kPer, a, b));
+        }  // (16-bit logits lose nothing)
+      }
+      if (!(keep >> at.group & 1u))
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) key[j] = 0u;
-  }
-
-  // The picks, best first: lane i keeps the i-th one's value, its expert goes through shared memory.
-  const bool inexact = biased || (sizeof(T) == 4 && kPer > 1);  // neighbours have to be told apart, the first that goes as well
-  const int looks = min(inexact ? p.k + 1 : p.k, 32);
-  uint32_t mine = 0u;
-  int count = 0;
-  for (; count < looks; ++count) {
-    const uint32_t head = key[0] & ~kIndex, top = __reduce_max_sync(kAll, head);
-    if (top == 0u) break;
-    const int winner = __ffs(__ballot_sync(kAll, head == top)) - 1;
-    if (lane == count) mine = top;
-    if (lane == winner) {
-      picks[warp][count] = at.first + (int)(kIndex - (key[0] & kIndex));
-#pragma unroll
-      for (int j = 0; j + 1 < kPer; ++j) key[j] = key[j + 1];
-      key[kPer - 1] = 0u;
+        for (int j = 0; j < kPer; ++j) key[j] = 0u;
     }
-  }
-  __syncwarp();
-  int picked = lane < count ? picks[warp][lane] : -1;
-  if (inexact) {
-    const uint32_t after = __shfl_down_sync(kAll, mine, 1);
-    const int after_e = __shfl_down_sync(kAll, picked, 1);
-    // (32 picks leave no lane for a 33rd look)
-    bool tell = lane + 1 < count && !(from_ordered(mine) - from_ordered(after) >
-                                      margin(biased ? each : 0.f, kPer, from_ordered(mine), from_ordered(after)));
-    if (tell)
-      tell = !(clean(logits_row[picked]) == clean(logits_row[after_e]) && (!biased || p.bias[picked] == p.bias[after_e]));
-    close = __any_sync(kAll, close || tell) || (p.k == 32 && count == 32);
-  }
-  if (close) picked = pick_exact<T, kPer>(p, logits_row, lane);
-  if (lane >= p.k) picked = -1;
 
-  // Weights: the score, or its share of the picks' scores, for which the largest pick takes the place of the row's largest logit (softmax) or
-  // of 0 (sigmoid = e^min(x, 0) / (1 + e^-|x|)): scores that are too small for float32 have shares all the same.
-  const bool there = picked >= 0;
-  const float px = there ? clean(logits_row[picked]) : 0.f;
-  float w;
-  if (p.renorm) {
-    const float num = p.softmax ? px : fminf(px, 0.f);
-    const float shift = warp_max(there ? num : kNone);
-    w = there ? expf(num - shift) : 0.f;
-    if (!p.softmax) w /= 1.f + expf(-fabsf(px));
-    const float sum = warp_sum(w);
-    w = there ? w / sum * p.factor : 0.f;
-  } else {
-    w = p.softmax ? expf(px - mx) * inv : 1.f / (1.f + expf(-px));
-    w = there ? w * p.factor : 0.f;
-  }
-  if (lane < p.k) {
-    p.out_w[row * p.k + lane] = w;
-    p.out_i[row * p.k + lane] = picked;
+    // The picks, best first: lane i keeps the i-th one's value, its expert goes through shared memory.
+    const bool inexact = biased || (sizeof(T) == 4 && kPer > 1);  // neighbours have to be told apart, two beyond the last as well
+    const int looks = min(inexact ? p.k + 2 : p.k, 32);
+    uint32_t mine = 0u;
+    int count = 0;
+    for (; count < looks; ++count) {
+      const uint32_t head = key[0] & ~kIndex, top = __reduce_max_sync(kAll, head);
+      if (top == 0u) break;
+      const int winner = __ffs(__ballot_sync(kAll, head == top)) - 1;
+      if (lane == count) mine = top;
+      if (lane == winner) {
+        picks[warp][count] = at.first + (int)(kIndex - (key[0] & kIndex));
+#pragma unroll
+        for (int j = 0; j + 1 < kPer; ++j) key[j] = key[j + 1];
+        key[kPer - 1] = 0u;
+      }
+    }
+    __syncwarp();
+    int picked = lane < count ? picks[warp][lane] : -1;
+    if (inexact) {
+      const uint32_t after = __shfl_down_sync(kAll, mine, 1);
+      const float a = from_ordered(mine), b = from_ordered(after);
+      bool tell = lane + 1 < count && lane < p.k + 1 && !(a - b > margin(biased ? kEach : 0.f, kPer, a, b));
+      uint32_t telling = __ballot_sync(kAll, tell);
+      if (telling != 0u) {  // equal logits with equal biases are in order
+        const int after_e = __shfl_down_sync(kAll, picked, 1);
+        if (tell) tell = !(clean(logits_row[picked]) == clean(logits_row[after_e]) && (!biased || p.bias[picked] == p.bias[after_e]));
+        telling = __ballot_sync(kAll, tell);
+      }
+      // Neighbours among the picks and the first that goes are put in order; where that one cannot be told from the next either, or (from 31
+      // picks on) could not be looked at, the row is decided anew.
+      const uint32_t border = 3u << (p.k - 1), among = p.k >= 32 ? kAll : (1u << p.k) - 1;
+      if ((telling & border) == border || (p.k > 30 && count == 32)) redo = true;
+      if ((telling & among) != 0u && !redo) picked = order_exact<T>(p, logits_row, mx, picked, min(count, p.k + 1), lane);
+    }
+    if (redo) picked = pick_exact<T, kPer>(p, logits_row, lane);
+    if (lane >= p.k) picked = -1;
+
+    // Weights: the score, or its share of the picks' scores, for which the largest pick takes the place of the row's largest logit (softmax)
+    // or of 0 (sigmoid = e^min(x, 0) / (1 + e^-|x|)): scores that are too small for float32 have shares all the same.
+    const bool there = picked >= 0;
+    const float px = there ? clean(logits_row[picked]) : 0.f;
+    float w;
+    if (p.renorm) {
+      const float num = kSoftmax ? px : fminf(px, 0.f);
+      const float shift = warp_max(there ? num : kNone);
+      w = there ? expf(num - shift) : 0.f;
+      if (!kSoftmax) w /= 1.f + expf(-fabsf(px));
+      const float sum = warp_sum(w);
+      w = there ? w / sum * p.factor : 0.f;
+    } else {
+      w = kSoftmax ? expf(px - mx) * inv : 1.f / (1.f + expf(-px));
+      w = there ? w * p.factor : 0.f;
+    }
+    if (lane < p.k) {
+      p.out_w[row * p.k + lane] = w;
+      p.out_i[row * p.k + lane] = picked;
+    }
+    __syncwarp();
   }
 }
 
-template <typename T>
+template <typename T, bool kSoftmax>
 static int launch(const void* logits, const Params& p, cudaStream_t st) {
-  const unsigned grid = (unsigned)((p.rows + kWarps - 1) / kWarps);
+  // (rows in rounds: the next row is asked for under this one)
+  const unsigned grid = (unsigned)std::min<int64_t>((p.rows + kWarps - 1) / kWarps, 4 * sm_count());
   const T* x = static_cast<const T*>(logits);
-#define SGLB_ROUTE_CASE(P)                                                                    \
-  if (p.per_lane <= P) {                                                                      \
-    SGLB_CUDA(launch_pdl(route_kernel<T, P>, grid, kWarps * 32, (size_t)0, st, x, p));             \
-    return SGLB200_OK;                                                                        \
+#define SGLB_ROUTE_CASE(P)                                                                              \
+  if (p.per_lane <= P) {                                                                                \
+    SGLB_CUDA(launch_pdl(route_kernel<T, P, kSoftmax>, grid, kWarps * 32, (size_t)0, st, x, p));        \
+    return SGLB200_OK;                                                                                  \
   }
   SGLB_ROUTE_CASE(1) SGLB_ROUTE_CASE(2) SGLB_ROUTE_CASE(4) SGLB_ROUTE_CASE(8) SGLB_ROUTE_CASE(16) SGLB_ROUTE_CASE(32)
 #undef SGLB_ROUTE_CASE
   return fail(SGLB200_E_UNSUPPORTED, "route_topk: %d groups of %d experts", p.groups, p.group_size);
+}
+template <typename T>
+static int launch(const void* logits, const Params& p, cudaStream_t st) {
+  return p.softmax ? launch<T, true>(logits, p, st) : launch<T, false>(logits, p, st);
 }
 
 }  // namespace route

@@ -61,6 +61,42 @@ def test_scores_that_float32_cannot_tell_apart(scoring, groups, kept):
             _check(x.repeat(3, 1), 8, scoring, bias, groups, kept, top)
 
 
+@pytest.mark.parametrize("topk", [1, 5, 30, 31, 32])
+def test_neighbours_at_the_border_of_the_picks(topk):
+    """Runs of experts a few float32 units apart, in any order, of which the border of the picks cuts one."""
+    for seed in range(6):
+        g = torch.Generator().manual_seed(100 + seed)
+        base = (torch.arange(96) // 3).float()[torch.randperm(96, generator=g)] * 0.125 - 2.0
+        x = base + torch.randint(-2, 3, (3, 96), generator=g) * 2.0**-23
+        _check(x, topk, "softmax")
+        _check(x, topk, "sigmoid", groups=4, kept=2, top=2)
+        _check(x, topk, "softmax", groups=8, kept=4, top=1)
+        bias = (torch.randint(0, 4, (96,), generator=g) * 0.25 - torch.sigmoid(x[0].double())).float()
+        _check(x, topk, "sigmoid", bias)
+        _check(x, topk, "softmax", bias * 0.01, 4, 2, 2, renorm=False)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_sums_of_large_biases_that_cancel(scoring):
+    """A group's two largest c of opposite signs: their sum is far smaller than what each is rounded by."""
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(20, 32, generator=g)
+    bias = torch.full((32,), -5000.0)
+    bias[0::4], bias[1::4] = 1000.0, -1000.0 + torch.arange(8) * 2.0**-13
+    _check(x, 4, scoring, bias, 8, 3, 2)
+
+
+def test_logits_far_from_zero():
+    """Differences that float32 logits hold in their last bits, far below a score's."""
+    g = torch.Generator().manual_seed(4)
+    x = (3.0e4 + torch.randint(0, 40, (30, 64), generator=g) * 2.0**-9).float()
+    for top in (1, 2):
+        _check(x, 6, "softmax", None, 8, 3, top)
+        _check(-x, 6, "softmax", None, 8, 3, top)
+    x = torch.where(torch.rand(30, 64, generator=g) < 0.7, x - 2000.0, x)  # most scores are nothing even in float64
+    _check(x, 6, "softmax", None, 8, 3, 1)
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 def test_ties_go_to_the_lower_index(scoring):
     x = torch.zeros(4, 64)

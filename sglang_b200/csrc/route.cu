@@ -5,13 +5,13 @@
 //
 // The order is that of the real numbers.  Without a bias it is the order of the logits.  Where scores decide it is taken in float32, which
 // tells two c apart that differ by more than `margin` (below); a row in which two neighbours of the order are closer than that, and are not
-// the same logit with the same bias, is decided once more in float64 by its warp.  With 256 experts that is one row in some hundreds.
+// the same logit with the same bias, is decided once more in float64 by its warp: the picks' order of one row in forty with 256 experts, a whole row of a few thousand.
 //
 // One warp a row, the row in registers: lane l has consecutive experts of one group.  It is bound by issue slots.  A lane sorts its
-// experts once, as integers: an order-preserving bit pattern of c, whose lowest bits give way to the expert's number in the lane (which the
-// margin allows for; 16-bit logits lose nothing).  A pick is then one reduction over the lanes' best, one vote and a shift of the winner's
-// list; a lane holds lower experts than the next, so the lowest lane of equals has the lowest expert.  16384 rows of 256 experts, best 8
-// in 4 of 8 groups: with the lanes' best looked for after every pick and scores by division, 1657 instructions a row and 33 us.
+// experts once, as integers: an order-preserving bit pattern of c, whose lowest bits give way to the expert's number in the lane and, for the
+// picks, to the lane's (which the margins allow for; 16-bit logits lose nothing).  A pick is then one reduction over the lanes' best and a
+// shift of the winner's list.  16384 rows of 256 experts, best 8 in 4 of 8 groups: with the lanes' best looked for after every pick and
+// scores by division, 1657 instructions a row and 33 us.
 #include <algorithm>
 #include <cfloat>
 
@@ -52,8 +52,9 @@ __device__ __forceinline__ float warp_sum(float v) {
 // Bit patterns that compare as unsigned integers like the floats they come from (-0 as +0), and the way back.
 __device__ __forceinline__ uint32_t to_ordered(float v) {
   const uint32_t u = __float_as_uint(v + 0.f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
+constexpr uint32_t kLeast = 0x00800000u;  // of the pattern of a finite number; -inf is below
 __device__ __forceinline__ float from_ordered(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
 
 // How far apart two c have to be for float32 to have their order right.  A sigmoid is off by at most s (1 - s) of the exponential's relative
@@ -234,45 +235,43 @@ __device__ __noinline__ int order_exact(const Params& p, const T* x, float mx, i
   return out;
 }
 
-// A lane's `count` consecutive values at `at` of the row (the rest none), 16 bytes at a time where they lie so.
+// A lane's `count` consecutive values at `at` of the row (the rest -inf), 16 bytes at a time where they lie so.
 template <typename T, int kPer>
 __device__ __forceinline__ void load_run(const T* at, int count, float (&v)[kPer]) {
   constexpr int kVec = 16 / (int)sizeof(T);
-  if (kPer % kVec == 0 && (count == kPer || count == 0) && (reinterpret_cast<uintptr_t>(at) & 15u) == 0) {
+  if (kPer % kVec == 0 && count == kPer && (reinterpret_cast<uintptr_t>(at) & 15u) == 0) {
     uint4 raw[kPer % kVec == 0 ? kPer / kVec : 1];
 #pragma unroll
-    for (int c = 0; c < kPer / kVec; ++c) raw[c] = count ? __ldg(reinterpret_cast<const uint4*>(at) + c) : make_uint4(0, 0, 0, 0);
+    for (int c = 0; c < kPer / kVec; ++c) raw[c] = __ldg(reinterpret_cast<const uint4*>(at) + c);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) v[j] = ElemTraits<T>::to_f32(reinterpret_cast<const T*>(raw)[j]);
   } else {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) v[j] = j < count ? ElemTraits<T>::to_f32(at[j]) : 0.f;
+    for (int j = 0; j < kPer; ++j) v[j] = j < count ? ElemTraits<T>::to_f32(at[j]) : kNone;
   }
 }
 
 // kSoftmax: else sigmoid.
 template <typename T, int kPer, bool kSoftmax>
-__global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict__ logits, const Params p) {
+__global__ void __launch_bounds__(kWarps * 32, kPer <= 8 ? 4 : 1) route_kernel(const T* __restrict__ logits, const Params p) {
   constexpr uint32_t kIndex = kPer - 1;  // the bits of a key that hold the expert's number in the lane, the lowest on top
-  __shared__ int32_t picks[kWarps][kMaxTopk];
+  constexpr uint32_t kUnits = 32 * kPer;  // and the lane
+  __shared__ uint32_t picks[kWarps][kMaxTopk];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   ptx::launch_dependents();
   const Place at = place(p, lane);
   const bool biased = p.bias != nullptr;
-  const uint32_t there_mask = at.count >= 32 ? kAll : (1u << at.count) - 1;
   ptx::grid_dependency_wait();
   float add[kPer];
   if (biased) load_run<float, kPer>(p.bias + at.first, at.count, add);
   int64_t row = (int64_t)blockIdx.x * kWarps + warp;
   const int64_t step = (int64_t)gridDim.x * kWarps;
-  float next[kPer];
-  if (row < p.rows) load_run<T, kPer>(logits + row * p.E + at.first, at.count, next);
   for (; row < p.rows; row += step) {
     const T* logits_row = logits + row * p.E;
     float x[kPer];
+    load_run<T, kPer>(logits_row + at.first, at.count, x);
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) x[j] = (there_mask >> j & 1u) && next[j] > kNone ? fminf(next[j], FLT_MAX) : kNone;  // (false for a NaN)
-    if (row + step < p.rows) load_run<T, kPer>(logits_row + step * p.E + at.first, at.count, next);
+    for (int j = 0; j < kPer; ++j) x[j] = fminf(fmaxf(x[j], kNone), FLT_MAX);  // (the larger of a NaN and -inf is -inf)
     float mx = kNone, inv = 0.f;
     if (kSoftmax && (biased || p.top == 2 || !p.renorm)) {
 #pragma unroll
@@ -285,16 +284,12 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
       inv = sum > 0.f ? 1.f / sum : 0.f;
     }
     auto score = [&](float v) { return kSoftmax ? fast_exp2((v - mx) * kLog2e) * inv : fast_rcp(1.f + fast_exp2(v * -kLog2e)); };
-    uint32_t key[kPer];  // descending; 0: not available
-    if (biased) {
+    uint32_t key[kPer];  // descending; below kLeast: not available
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const float c = score(x[j]) + add[j];
-        key[j] = x[j] > kNone && c > kNone ? (to_ordered(c) & ~kIndex) | (kIndex - j) : 0u;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) key[j] = x[j] > kNone ? (to_ordered(x[j]) & ~kIndex) | (kIndex - j) : 0u;
+    for (int j = 0; j < kPer; ++j) {
+      float c = x[j];
+      if (biased) c = c > kNone ? fmaxf(score(c) + add[j], kNone) : kNone;
+      key[j] = (to_ordered(c) & ~kIndex) | (kIndex - j);
     }
     sort_keys<kPer>(key);
 
@@ -312,12 +307,12 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
       float v1 = from_ordered(m1 & ~kIndex), v2 = from_ordered(m2 & ~kIndex);
       // (the largest of what is added: a sum may be smaller than what it is off by)
       const float reach = __uint_as_float(__reduce_max_sync(
-          kAll, lane < p.groups && m1 != 0u ? __float_as_uint(fmaxf(fabsf(v1), m2 != 0u && p.top == 2 ? fabsf(v2) : 0.f)) : 0u));
+          kAll, lane < p.groups && m1 >= kLeast ? __float_as_uint(fmaxf(fabsf(v1), m2 >= kLeast && p.top == 2 ? fabsf(v2) : 0.f)) : 0u));
       if (p.top == 2) {
         if (!biased) v1 = score(v1), v2 = score(v2);
-        v1 = m2 != 0u ? v1 + v2 : v1;
+        v1 = m2 >= kLeast ? v1 + v2 : v1;
       }
-      const uint32_t value = lane < p.groups && m1 != 0u ? to_ordered(v1) : 0u;
+      const uint32_t value = lane < p.groups && m1 >= kLeast ? to_ordered(v1) : 0u;
       const uint32_t keep = keep_groups<uint32_t>(p, value, lane);
       // the last that stays and the first that goes have to be told apart
       const bool in = keep >> lane & 1u;
@@ -337,29 +332,31 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
         for (int j = 0; j < kPer; ++j) key[j] = 0u;
     }
 
-    // The picks, best first: lane i keeps the i-th one's value, its expert goes through shared memory.
-    const bool inexact = biased || (sizeof(T) == 4 && kPer > 1);  // neighbours have to be told apart, two beyond the last as well
+    // The picks, best first, through shared memory to lane i.  With the lane in its lowest bits as well, the lower on top, a key is the row's
+    // only one of its kind, and a pick is a reduction and a comparison.
+    const bool inexact = biased || sizeof(T) == 4;  // neighbours have to be told apart, two beyond the last as well
     const int looks = min(inexact ? p.k + 2 : p.k, 32);
-    uint32_t mine = 0u;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) key[j] = (key[j] & ~(kUnits - kPer)) | (uint32_t)(31 - lane) * kPer;
     int count = 0;
     for (; count < looks; ++count) {
-      const uint32_t head = key[0] & ~kIndex, top = __reduce_max_sync(kAll, head);
-      if (top == 0u) break;
-      const int winner = __ffs(__ballot_sync(kAll, head == top)) - 1;
-      if (lane == count) mine = top;
-      if (lane == winner) {
-        picks[warp][count] = at.first + (int)(kIndex - (key[0] & kIndex));
+      const uint32_t top = __reduce_max_sync(kAll, key[0]);
+      if (top < kLeast) break;
+      if (lane == 0) picks[warp][count] = top;
+      if (key[0] == top) {
 #pragma unroll
         for (int j = 0; j + 1 < kPer; ++j) key[j] = key[j + 1];
         key[kPer - 1] = 0u;
       }
     }
     __syncwarp();
-    int picked = lane < count ? picks[warp][lane] : -1;
+    const uint32_t pick = picks[warp][lane], mine = pick & ~(kUnits - 1);
+    int picked = __shfl_sync(kAll, at.first, 31 - (int)(pick / kPer % 32)) + (int)(kIndex - (pick & kIndex));
+    if (lane >= count) picked = -1;
     if (inexact) {
       const uint32_t after = __shfl_down_sync(kAll, mine, 1);
       const float a = from_ordered(mine), b = from_ordered(after);
-      bool tell = lane + 1 < count && lane < p.k + 1 && !(a - b > margin(biased ? kEach : 0.f, kPer, a, b));
+      bool tell = lane + 1 < count && lane < p.k + 1 && !(a - b > margin(biased ? kEach : 0.f, kUnits, a, b));
       uint32_t telling = __ballot_sync(kAll, tell);
       if (telling != 0u) {  // equal logits with equal biases are in order
         const int after_e = __shfl_down_sync(kAll, picked, 1);
@@ -384,9 +381,9 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
       const float num = kSoftmax ? px : fminf(px, 0.f);
       const float shift = warp_max(there ? num : kNone);
       w = there ? expf(num - shift) : 0.f;
-      if (!kSoftmax) w /= 1.f + expf(-fabsf(px));
+      if (!kSoftmax) w = __fdividef(w, 1.f + expf(-fabsf(px)));
       const float sum = warp_sum(w);
-      w = there ? w / sum * p.factor : 0.f;
+      w = there ? __fdividef(w, sum) * p.factor : 0.f;
     } else {
       w = kSoftmax ? expf(px - mx) * inv : 1.f / (1.f + expf(-px));
       w = there ? w * p.factor : 0.f;

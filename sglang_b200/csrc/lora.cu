@@ -8,6 +8,8 @@
 // h keeps 16 bits and more in the second product: the row's values times a power of two that brings the largest to [1, 2) (float16 would
 // overflow or lose small ones without it) enter as two 16-bit terms, 16 bits of bfloat16 or 22 of float16; the weights are what they are.
 // A rounding to one term would be off by 2^-9 of h, as much as the rounding of the output.
+#include <algorithm>
+
 #include "gemm_common.cuh"
 #include "lora.cuh"
 #include "ptx_sm100.cuh"
@@ -18,57 +20,72 @@ namespace lora {
 // ---- plan -----------------------------------------------------------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
 
-// One CTA.  Tokens of one adapter in any order: their rows do not meet.  Neighbours mostly name the same adapter, so that a warp counts
-// equal ids at once.
+// One CTA.  The tokens of an adapter stay in their order, so that those of a long request lie one after the other.  Warp w takes the w-th part
+// of the tokens and counts them by adapter in a row of its own; neighbours mostly name the same adapter, so that it counts equal ids at once.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __restrict__ ids, int T, int L, int block, int32_t* order,
                                                             int32_t* start, int32_t* rows, int32_t* adapter, int32_t* count) {
-  __shared__ int32_t cursor[kMaxAdapters + 1];
-  const int tid = threadIdx.x, lane = tid & 31;
-  for (int i = tid; i <= L; i += kPlanThreads) cursor[i] = 0;
+  extern __shared__ int32_t counts[];  // [32 warps][L + 1], [L + 1] tokens and [L + 1] blocks before an adapter's
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, keys = L + 1;
+  int32_t *mine = counts + warp * keys, *tokens_before = counts + 32 * keys, *blocks_before = tokens_before + keys;
+  for (int i = tid; i < 32 * keys; i += kPlanThreads) counts[i] = 0;
   __syncthreads();
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
-  const int padded = (T + 31) & ~31;
-  for (int i = tid; i < padded; i += kPlanThreads) {
-    const int id = i < T ? ids[i] : -1;
-    const int key = i >= T ? L + 1 : id >= 0 && id < L ? id : L;
+  const int part = (T + kPlanThreads - 1) / kPlanThreads * 32, begin = min(warp * part, T), end = min(begin + part, T);
+  auto key_of = [&](int t) {  // (past the end: nobody's)
+    const int id = t < end ? ids[t] : 0;
+    return t >= end ? keys : id >= 0 && id < L ? id : L;
+  };
+  for (int t = begin; t < end; t += 32) {
+    const int key = key_of(t + lane);
     const uint32_t same = __match_any_sync(0xffffffffu, key);
-    if (i < T && (int)__ffs(same) - 1 == lane) atomicAdd(&cursor[key], __popc(same));
+    if (key < keys && __ffs(same) - 1 == lane) mine[key] += __popc(same);
+    __syncwarp();
   }
   __syncthreads();
-  if (tid < 32) {  // first token and first block of every adapter
+  for (int l = tid; l < keys; l += kPlanThreads) {  // every warp's tokens of an adapter begin behind the earlier warps'
+    int sum = 0;
+    for (int w = 0; w < 32; ++w) {
+      const int n = counts[w * keys + l];
+      counts[w * keys + l] = sum;
+      sum += n;
+    }
+    tokens_before[l] = sum;
+  }
+  __syncthreads();
+  if (warp == 0) {
     int tokens = 0, blocks = 0;
-    for (int at = 0; at <= L; at += 32) {
-      const int l = at + lane, n = l <= L ? cursor[l] : 0, b = (n + block - 1) / block;
+    for (int at = 0; at < keys; at += 32) {
+      const int l = at + lane, n = l < keys ? tokens_before[l] : 0, b = (n + block - 1) / block;
       int sn = n, sb = b;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
         const int un = __shfl_up_sync(0xffffffffu, sn, off), ub = __shfl_up_sync(0xffffffffu, sb, off);
         if (lane >= off) sn += un, sb += ub;
       }
-      if (l <= L) {
-        for (int i = 0; i < b; ++i) {
-          const int at_block = blocks + sb - b + i;
-          start[at_block] = tokens + sn - n + i * block;
-          rows[at_block] = min(block, n - i * block);
-          adapter[at_block] = l < L ? l : -1;
-        }
-        cursor[l] = tokens + sn - n;
-      }
+      if (l < keys) tokens_before[l] = tokens + sn - n, blocks_before[l] = blocks + sb - b;
       tokens += __shfl_sync(0xffffffffu, sn, 31), blocks += __shfl_sync(0xffffffffu, sb, 31);
     }
     if (lane == 0) *count = blocks;
   }
   __syncthreads();
-  for (int i = tid; i < padded; i += kPlanThreads) {
-    const int id = i < T ? ids[i] : -1;
-    const int key = i >= T ? L + 1 : id >= 0 && id < L ? id : L;
+  for (int l = warp; l < keys; l += 32) {
+    const int first = tokens_before[l], n = (l + 1 < keys ? tokens_before[l + 1] : T) - first;
+    for (int i = lane; i * block < n; i += 32) {
+      const int b = blocks_before[l] + i;
+      start[b] = first + i * block;
+      rows[b] = min(block, n - i * block);
+      adapter[b] = l < L ? l : -1;
+    }
+  }
+  for (int t = begin; t < end; t += 32) {
+    const int key = key_of(t + lane);
     const uint32_t same = __match_any_sync(0xffffffffu, key);
-    const int leader = __ffs(same) - 1;
-    int at = 0;
-    if (i < T && leader == lane) at = atomicAdd(&cursor[key], __popc(same));
-    at = __shfl_sync(0xffffffffu, at, leader) + __popc(same & ((1u << lane) - 1));
-    if (i < T) order[at] = i;
+    const int before = key < keys ? mine[key] : 0;
+    __syncwarp();
+    if (key < keys && __ffs(same) - 1 == lane) mine[key] = before + __popc(same);
+    if (key < keys) order[tokens_before[key] + before + __popc(same & ((1u << lane) - 1))] = t + lane;
+    __syncwarp();
   }
 }
 
@@ -87,12 +104,27 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// kSteps: instructions over the rank, at most; kTiles: groups of 8 columns of a warp.  A lane holds the same two kTiles neighbouring columns
-// of a token in all groups, so that base and out go by 4 kTiles bytes.  A warp asks for the next 16 tokens' base before it multiplies these.
-template <typename T, int kSteps, int kTiles>
+// A CTA takes up to `sub` rows of a block and `passes` times 8 warps' columns.  kPairs: 32 values of the rank at most, which are two
+// instructions; kTiles: groups of 8 columns of a warp.  As a sum does not mind the order of its terms, a lane's 16 consecutive bytes of a weight
+// row (and of a row of h alike) are its part of both.  A lane holds the same two kTiles neighbouring columns of a token in all groups, so that
+// base and out go by 4 kTiles bytes.  Weights, and base of the first 16 rows, come by asynchronous copies, each lane's to a place of its own,
+// kDepth - 1 passes ahead and before h is there: they are what bounds this kernel where few tokens name an adapter.
+template <int kPairs, int kTiles>
+struct ExpandCfg {
+  static constexpr int kLane = kPairs * kTiles * 16 + kTiles * 8;  // bytes of a lane and pass
+  static constexpr int kDepth = kPairs == 1 ? 4 : kPairs == 2 && kTiles == 4 ? 3 : 2;
+  static constexpr int kStage = kLane * kWarps * 32, kCols = 8 * kTiles * kWarps;
+  static constexpr int kPitch = kPairs * 128 + 64;  // of a token's two terms: two rows of 64 bytes are read without a bank conflict
+  static constexpr int kMostRows = (227 * 1024 - 4096 - kDepth * kStage) / kPitch >= 128 ? 128 : 64;
+  static_assert(kDepth * kStage + kMostRows * kPitch <= 227 * 1024 - 4096);
+};
+
+template <typename T, int kPairs, int kTiles>
 __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
-  constexpr int kCols = 8 * kTiles, kMine = 2 * kTiles;
-  extern __shared__ __align__(16) uint8_t tile[];  // [rows of a CTA][pitch]: a token's high terms, then its low terms
+  using Cfg = ExpandCfg<kPairs, kTiles>;
+  constexpr int kCols = 8 * kTiles, kMine = 2 * kTiles, kDepth = Cfg::kDepth;
+  extern __shared__ __align__(16) uint8_t tile[];  // [kDepth] stages, then [rows of a CTA][kPitch]
+  uint8_t* terms = tile + kDepth * Cfg::kStage;    // a token's high terms, then its low terms, 32 kPairs each
   __shared__ float unscale[narrow::kTileBlock];
   __shared__ int32_t token[narrow::kTileBlock];
   __shared__ int found[2];
@@ -115,140 +147,129 @@ __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
     const int start = __ldcg(p.blocks.start + block);
     rows = __ldcg(p.blocks.rows + block);
     if (tid < rows) token[tid] = __ldcg(p.blocks.order + start + tid);
+    __syncthreads();
   }
   if (row0 >= rows || (adapter < 0 && p.in_place)) return;
   rows = min(rows - row0, p.sub);
   int slice = 0;
   while (slice + 1 < p.S && chunk >= p.chunk0[slice + 1]) ++slice;
   const int64_t end = p.col0[slice + 1];
-  const int64_t c0 = p.col0[slice] + (int64_t)(chunk - p.chunk0[slice]) * p.passes * kWarps * kCols + warp * kCols;
+  const int64_t c0 = p.col0[slice] + (int64_t)(chunk - p.chunk0[slice]) * p.passes * Cfg::kCols + warp * kCols;
+  const int passes = c0 < end ? (int)min((int64_t)p.passes, (end - c0 + Cfg::kCols - 1) / Cfg::kCols) : 0;
   const int used = adapter < 0 ? 0 : p.ranks != nullptr ? min(max(__ldg(p.ranks + adapter), 0), p.R) : p.R;
-  const T* weights = static_cast<const T*>(p.b) + (adapter < 0 ? 0 : (int64_t)adapter * p.N * p.R);
+  const int pairs = (used + 31) / 32;
+  const uint8_t* weights = static_cast<const uint8_t*>(p.b) + (adapter < 0 ? 0 : (int64_t)adapter * p.N * p.R * 2);
   const T* base = static_cast<const T*>(p.base);
   T* out = static_cast<T*>(p.out);
+  const int64_t ta = token[row0 + min(g, rows - 1)], tb = token[row0 + min(g + 8, rows - 1)];
+  const uint32_t mine_at = ptx::smem_u32(tile) + tid * 16;  // (chunk i of a stage at i times 16 bytes of all threads)
+  constexpr uint32_t kChunk = kWarps * 32 * 16;
 
-  uint2 w[kSteps][kTiles];
-  auto load_weights = [&](int64_t c) {
+  auto fetch = [&](int pass) {
+    if (pass < passes) {
+      const int64_t c = c0 + (int64_t)pass * Cfg::kCols;
+      const uint32_t to = mine_at + pass % kDepth * Cfg::kStage;
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j) {
-      const int64_t n = c + (g >> 1) * kMine + j * 2 + (g & 1);
+      for (int j = 0; j < kTiles; ++j) {
+        const int64_t n = c + (g >> 1) * kMine + j * 2 + (g & 1);
+        const uint8_t* from = weights + (n < end ? n : c) * p.R * 2 + q * 16;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const int r = s * 16 + q * 4;
-        w[s][j] = n < end && r < used ? __ldg(reinterpret_cast<const uint2*>(weights + n * p.R + r)) : make_uint2(0, 0);
+        for (int s = 0; s < kPairs; ++s)
+          if (s < pairs) {  // (beyond the rank anything may stand: zeros instead)
+            const int there = n < end ? min(max((used - s * 32 - q * 8) * 2, 0), 16) : 0;
+            ptx::cp_async_16(to + (s * kTiles + j) * kChunk, there > 0 ? from + s * 64 : weights, there);
+          }
       }
-    }
-    if (used % 4 != 0) {  // beyond the rank anything may stand
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const int r = s * 16 + q * 4;
-#pragma unroll
-        for (int j = 0; j < kTiles; ++j) {
-          if (r + 1 >= used) w[s][j].x &= 0xffffu;
-          if (r + 2 >= used) w[s][j].y = 0;
-          if (r + 3 >= used) w[s][j].y &= 0xffffu;
+      if (p.vec) {
+        const int64_t n = c + q * kMine;
+        const uint32_t base_to = ptx::smem_u32(tile) + pass % kDepth * Cfg::kStage + kPairs * kTiles * kChunk;
+        if (n < end) {
+          if constexpr (kTiles == 4) {
+            if (g < rows) ptx::cp_async_16(base_to + tid * 16, base + ta * p.ld_base + n, 16);
+            if (g + 8 < rows) ptx::cp_async_16(base_to + kChunk + tid * 16, base + tb * p.ld_base + n, 16);
+          } else {
+            if (g < rows) ptx::cp_async_8(base_to + tid * 8, base + ta * p.ld_base + n);
+            if (g + 8 < rows) ptx::cp_async_8(base_to + kChunk / 2 + tid * 8, base + tb * p.ld_base + n);
+          }
         }
       }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  // Two tokens' kMine columns at c, 16 bytes (8 for two groups) at a time where all lie so.
-  auto load_base = [&](int64_t c, int m, uint32_t (&old)[2][kTiles]) {
-    const int64_t mine = c + q * kMine;
-    const int cols = (int)max((int64_t)0, min((int64_t)kMine, end - mine));
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = m + g + 8 * i;
-#pragma unroll
-      for (int j = 0; j < kTiles; ++j) old[i][j] = 0;
-      if (r >= rows || cols == 0) continue;
-      const T* from = base + (int64_t)token[row0 + r] * p.ld_base + mine;
-      if (p.vec) {
-        if constexpr (kTiles == 4)
-          *reinterpret_cast<uint4*>(old[i]) = *reinterpret_cast<const uint4*>(from);
-        else
-          *reinterpret_cast<uint2*>(old[i]) = *reinterpret_cast<const uint2*>(from);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kMine; ++j)
-          if (j < cols) old[i][j / 2] |= (uint32_t)bits(from[j]) << (j % 2 * 16);
-      }
-    }
-  };
-  uint32_t old[2][kTiles] = {};
-  if (c0 < end) load_weights(c0);
+  for (int i = 0; i < kDepth - 1; ++i) fetch(i);
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
-  __syncthreads();  // (the tokens)
-  if (c0 < end) load_base(c0, 0, old);
   const float scaling = adapter >= 0 && p.scalings != nullptr ? __ldg(p.scalings + adapter) : 1.f;
   // (two rows' loads at a time)
-  constexpr int kV = (kSteps + 1) / 2;
-  for (int i = warp; i < rows; i += 2 * kWarps) {
-    float v[2][kV];
+  for (int i = warp; i < rows && used > 0; i += 2 * kWarps) {
+    float v[2][kPairs];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const float* h = p.h + ((int64_t)token[row0 + min(i + u * kWarps, rows - 1)] * p.S + slice) * p.R;
 #pragma unroll
-      for (int j = 0; j < kV; ++j) v[u][j] = j * 32 + lane < used ? __ldcg(h + j * 32 + lane) * scaling : 0.f;
+      for (int j = 0; j < kPairs; ++j) v[u][j] = j * 32 + lane < used ? __ldcg(h + j * 32 + lane) * scaling : 0.f;
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int row = i + u * kWarps;
       if (row >= rows) break;
-      uint16_t* at = reinterpret_cast<uint16_t*>(tile + row * p.pitch);
-      const float inv = split_row<T>(v[u], p.R, lane, [&](int r, uint16_t hi, uint16_t lo) { at[r] = hi, at[p.R + r] = lo; });
+      uint16_t* at = reinterpret_cast<uint16_t*>(terms + row * Cfg::kPitch);
+      const float inv = split_row<T>(v[u], kPairs * 32, lane, [&](int r, uint16_t hi, uint16_t lo) { at[r] = hi, at[kPairs * 32 + r] = lo; });
       if (lane == 0) unscale[row] = inv;
     }
   }
   __syncthreads();
-  const int steps = (used + 15) / 16;
 
-  for (int pass = 0; pass < p.passes; ++pass) {
-    const int64_t c = c0 + (int64_t)pass * kWarps * kCols;
-    if (c >= end) break;
-    const int64_t next_c = c + kWarps * kCols;
-    const bool more = pass + 1 < p.passes && next_c < end;
-    if (pass > 0) load_weights(c);
-    const int64_t mine = c + q * kMine;
+  for (int pass = 0; pass < passes; ++pass) {
+    fetch(pass + kDepth - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+    const uint32_t from = mine_at + pass % kDepth * Cfg::kStage;
+    const int64_t mine = c0 + (int64_t)pass * Cfg::kCols + q * kMine;
     const int cols = (int)max((int64_t)0, min((int64_t)kMine, end - mine));
     for (int m = 0; m < rows; m += 16) {
-      const int ra = m + g, rb = m + g + 8;
-      uint32_t ahead[2][kTiles] = {};
-      if (m + 16 < rows) {
-        load_base(c, m + 16, ahead);
-      } else if (more) {
-        load_base(next_c, 0, ahead);
-      }
       float acc[kTiles][4] = {};
+      // (rows past the last are not written, and meet only their own sums)
+      const uint8_t *pa = terms + (m + g) * Cfg::kPitch + q * 16, *pb = pa + 8 * Cfg::kPitch;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        if (s >= steps) break;
-        const bool in = s * 16 + q * 4 < p.R;  // (R is a multiple of 8: a last instruction may have half its columns)
-        const uint8_t* pa = tile + ra * p.pitch + (s * 16 + q * 4) * 2;
-        const uint8_t* pb = tile + rb * p.pitch + (s * 16 + q * 4) * 2;
-        const uint2 zero = make_uint2(0, 0);
-        // (rows past the last are not written, and meet only their own sums)
-        const uint2 ah = in ? *reinterpret_cast<const uint2*>(pa) : zero, bh = in ? *reinterpret_cast<const uint2*>(pb) : zero;
-        const uint2 al = in ? *reinterpret_cast<const uint2*>(pa + p.R * 2) : zero, bl = in ? *reinterpret_cast<const uint2*>(pb + p.R * 2) : zero;
+      for (int s = 0; s < kPairs; ++s) {
+        if (s >= pairs) break;
+        const uint4 ah = *reinterpret_cast<const uint4*>(pa + s * 64), bh = *reinterpret_cast<const uint4*>(pb + s * 64);
+        const uint4 al = *reinterpret_cast<const uint4*>(pa + kPairs * 64 + s * 64), bl = *reinterpret_cast<const uint4*>(pb + kPairs * 64 + s * 64);
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) {
-          mma16816<T>(acc[j], al.x, bl.x, al.y, bl.y, w[s][j].x, w[s][j].y);
-          mma16816<T>(acc[j], ah.x, bh.x, ah.y, bh.y, w[s][j].x, w[s][j].y);
+          const uint4 w = ptx::lds_128(from + (s * kTiles + j) * kChunk);
+          mma16816<T>(acc[j], al.x, bl.x, al.y, bl.y, w.x, w.y);
+          mma16816<T>(acc[j], al.z, bl.z, al.w, bl.w, w.z, w.w);
+          mma16816<T>(acc[j], ah.x, bh.x, ah.y, bh.y, w.x, w.y);
+          mma16816<T>(acc[j], ah.z, bh.z, ah.w, bh.w, w.z, w.w);
         }
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int r = m + g + 8 * i;
         if (r >= rows || cols == 0) continue;
-        T* to = out + (int64_t)token[row0 + r] * p.ld_out + mine;
-        const float inv = unscale[r];
-        uint32_t now[kTiles];
-#pragma unroll
-        for (int j = 0; j < kTiles; ++j) {
-          if (used == 0) {
-            now[j] = old[i][j];
+        const int64_t t = token[row0 + r];
+        const T* had = base + t * p.ld_base + mine;
+        T* to = out + t * p.ld_out + mine;
+        uint32_t now[kTiles] = {};
+        if (p.vec) {
+          if constexpr (kTiles == 4) {
+            *reinterpret_cast<uint4*>(now) = m == 0 ? ptx::lds_128(from + (kPairs * kTiles + i) * kChunk) : *reinterpret_cast<const uint4*>(had);
           } else {
-            const float2 was = unpack2<T>(old[i][j]);
+            const uint8_t* staged = tile + pass % kDepth * Cfg::kStage + kPairs * kTiles * kChunk + i * (kChunk / 2) + tid * 8;
+            *reinterpret_cast<uint2*>(now) = m == 0 ? ptx::lds_64(ptx::smem_u32(staged)) : *reinterpret_cast<const uint2*>(had);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kMine; ++j)
+            if (j < cols) now[j / 2] |= (uint32_t)bits(had[j]) << (j % 2 * 16);
+        }
+        if (used > 0) {
+          const float inv = unscale[r];
+#pragma unroll
+          for (int j = 0; j < kTiles; ++j) {
+            const float2 was = unpack2<T>(now[j]);
             now[j] = pack2<T>(was.x + acc[j][2 * i] * inv, was.y + acc[j][2 * i + 1] * inv);
           }
         }
@@ -266,59 +287,49 @@ __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
             }
         }
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < kTiles; ++j) old[i][j] = ahead[i][j];
     }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-template <typename T, int kSteps, int kTiles>
+template <typename T, int kPairs, int kTiles>
 static int launch_expand(Params& p, int block, cudaStream_t st) {
-  constexpr int kCols = 8 * kTiles * kWarps;
+  using Cfg = ExpandCfg<kPairs, kTiles>;
   int64_t units = 0;
-  for (int s = 0; s < p.S; ++s) units += (p.col0[s + 1] - p.col0[s] + kCols - 1) / kCols;
-  // Blocks are cut until there are four CTAs for every SM, then a CTA takes as many passes as leave that many.
-  const int64_t want = 4 * sm_count();
-  p.sub = block;
+  for (int s = 0; s < p.S; ++s) units += (p.col0[s + 1] - p.col0[s] + Cfg::kCols - 1) / Cfg::kCols;
+  // Blocks are cut until there are as many CTAs as run at once, then a CTA takes as many passes as leave that many.
+  const int64_t want = (int64_t)std::min(4, (227 * 1024) / (Cfg::kDepth * Cfg::kStage + 16 * Cfg::kPitch + 3072)) * sm_count();
+  p.sub = std::min(block, Cfg::kMostRows);
   while (p.sub > 16 && units * p.max_blocks * (block / p.sub) < want) p.sub /= 2;
   p.subs = block / p.sub;
-  const int64_t passes = units * p.max_blocks * p.subs / want;
-  p.passes = (int)(passes < 1 ? 1 : passes > 8 ? 8 : passes);
+  p.passes = (int)std::min<int64_t>(16, (units * p.max_blocks * p.subs + want - 1) / want);
   int chunks = 0;
   for (int s = 0; s < p.S; ++s) {
     p.chunk0[s] = chunks;
-    const int64_t per = (int64_t)kCols * p.passes;
+    const int64_t per = (int64_t)Cfg::kCols * p.passes;
     chunks += (int)((p.col0[s + 1] - p.col0[s] + per - 1) / per);
   }
   p.chunk0[p.S] = chunks;
-  // rows 32 bytes apart modulo 128: four rows of 32 bytes are read without a bank conflict
-  p.pitch = (4 * p.R + 127) / 128 * 128 + 32;
-  const size_t smem = (size_t)p.sub * p.pitch;
   const int64_t grid = (int64_t)chunks * p.max_blocks * p.subs;
   SGLB_REQUIRE(grid < (1ll << 31), "lora_add: %lld tiles are too many", (long long)grid);
-  auto kern = expand_kernel<T, kSteps, kTiles>;
-  if (smem > 40 * 1024) {  // (beside the static ones)
-    static thread_local bool attr_set[64] = {false};  // the opt-in is per function and per device
-    int dev = 0;
-    SGLB_CUDA(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-      SGLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, narrow::kTileBlock * (4 * kMaxRank + 160)));
-      if (dev >= 0 && dev < 64) attr_set[dev] = true;
-    }
+  auto kern = expand_kernel<T, kPairs, kTiles>;
+  static thread_local bool attr_set[64] = {false};  // the opt-in is per function and per device
+  int dev = 0;
+  SGLB_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    SGLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kDepth * Cfg::kStage + Cfg::kMostRows * Cfg::kPitch));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  SGLB_CUDA(launch_pdl(kern, (unsigned)grid, kWarps * 32, smem, st, p));
+  SGLB_CUDA(launch_pdl(kern, (unsigned)grid, kWarps * 32, (size_t)(Cfg::kDepth * Cfg::kStage + p.sub * Cfg::kPitch), st, p));
   return SGLB200_OK;
 }
 
 template <typename T>
 static int expand(Params& p, int block, cudaStream_t st) {
-  if (p.R <= 16) return launch_expand<T, 1, 4>(p, block, st);
-  if (p.R <= 32) return launch_expand<T, 2, 4>(p, block, st);
-  if (p.R <= 64) return launch_expand<T, 4, 4>(p, block, st);
-  if (p.R <= 128) return launch_expand<T, 8, 4>(p, block, st);
-  return launch_expand<T, 16, 2>(p, block, st);
+  if (p.R <= 32) return launch_expand<T, 1, 4>(p, block, st);
+  if (p.R <= 64) return launch_expand<T, 2, 4>(p, block, st);
+  if (p.R <= 128) return launch_expand<T, 4, 4>(p, block, st);
+  return launch_expand<T, 8, 2>(p, block, st);
 }
 
 // Every adapter (and "none") has at most one block that is not full.
@@ -355,7 +366,7 @@ extern "C" int sglb200_lora_add(const void* x, const void* lora_a, const void* l
                (long long)K, (long long)x_stride);
   SGLB_REQUIRE(base_stride >= N && out_stride >= N, "lora_add: row strides %lld and %lld of %lld columns", (long long)base_stride,
                (long long)out_stride, (long long)N);
-  SGLB_REQUIRE(tokens < (1ll << 31) - 256 && N < (1ll << 31) - 65536 && K <= 1 << 20, "lora_add: %lld tokens, N %lld or K %lld is too large",
+  SGLB_REQUIRE(tokens < (1ll << 31) - 65536 && N < (1ll << 31) - 65536 && K <= 1 << 20, "lora_add: %lld tokens, N %lld or K %lld is too large",
                (long long)tokens, (long long)N, (long long)K);
   SGLB_REQUIRE(slice_sizes != nullptr, "lora_add: null slice_sizes");
   lora::Params p{};
@@ -388,7 +399,18 @@ extern "C" int sglb200_lora_add(const void* x, const void* lora_a, const void* l
     p.blocks.ids = adapter_ids, p.blocks.ids_rows = (int)tokens, p.blocks.adapters = num_adapters;
   } else {
     p.blocks = {order, start, start + blocks, start + 2 * blocks, start + 3 * blocks, nullptr, 0, 0};
-    SGLB_CUDA(launch_pdl(lora::plan_kernel, 1u, (unsigned)lora::kPlanThreads, (size_t)0, st, adapter_ids, (int)tokens, num_adapters, block, order,
+    const size_t smem = (size_t)34 * (num_adapters + 1) * sizeof(int32_t);
+    if (smem > 48 * 1024) {
+      static thread_local bool attr_set[64] = {false};  // the opt-in is per function and per device
+      int dev = 0;
+      SGLB_CUDA(cudaGetDevice(&dev));
+      if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+        SGLB_CUDA(cudaFuncSetAttribute(lora::plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       34 * (lora::kMaxAdapters + 1) * (int)sizeof(int32_t)));
+        if (dev >= 0 && dev < 64) attr_set[dev] = true;
+      }
+    }
+    SGLB_CUDA(launch_pdl(lora::plan_kernel, 1u, (unsigned)lora::kPlanThreads, smem, st, adapter_ids, (int)tokens, num_adapters, block, order,
                          start, start + blocks, start + 2 * blocks, start + 3 * blocks));
   }
   narrow::Params n{};
@@ -404,5 +426,6 @@ extern "C" int sglb200_lora_add(const void* x, const void* lora_a, const void* l
   // (its row pitches are 32-bit numbers of bytes)
   if (block == narrow::kTileBlock && p.vec && rank <= lora::kTileRank && base_stride < 1ll << 30 && out_stride < 1ll << 30)
     return lora::expand_tile(p, dtype, st);
-  return dtype == 0 ? lora::expand<__nv_bfloat16>(p, block, st) : lora::expand<__half>(p, block, st);
+  const int rows = tokens <= 16 ? 16 : tokens <= 32 ? 32 : block;  // the most that a block can have
+  return dtype == 0 ? lora::expand<__nv_bfloat16>(p, rows, st) : lora::expand<__half>(p, rows, st);
 }

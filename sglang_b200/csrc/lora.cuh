@@ -21,7 +21,7 @@ struct Params {
   const int32_t* ranks;   // or nullptr
   narrow::Blocks blocks;
   int64_t N, ld_base, ld_out;
-  int R, S, max_blocks, passes, vec, in_place, pitch;
+  int R, S, max_blocks, passes, vec, in_place;
   int sub, subs;     // rows of a block that a CTA takes, CTAs of a block
   int64_t col0[kMaxSlices + 1];  // first column of every merged projection, and the end
   int chunk0[kMaxSlices + 1];    // the first chunk of passes x 8 warps x columns of a warp (lora_tile.cu: of 128 columns), and the end

@@ -28,8 +28,41 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// kG groups of 8 activation rows.  `part` and `sums` are padded so that neither their writes nor their reads meet in a bank: unpadded,
-// 64 rows x 256 x 7168 took 12.8 us.
+// What a warp adds up of 16 weight rows and up to kG groups of 8 activation rows, `rows` in all, over steps s0 .. s1 of K, to
+// part[16][pitch]; `row_of(i)`: the i-th activation row.  kAhead steps are asked for at once.
+template <typename T, int kG, int kAhead, class RowOf>
+__device__ __forceinline__ void add_up(const Params& p, const T* wa, const T* wb, bool a_on, bool b_on, int rows, int s0, int s1, int lane,
+                                       float* part, int pitch, RowOf row_of) {
+  const int g = lane >> 2, q = lane & 3;
+  const T* x[kG];
+#pragma unroll
+  for (int j = 0; j < kG; ++j) x[j] = static_cast<const T*>(p.x) + row_of(min(j * 8 + g, rows - 1)) * p.ldx;
+  float acc[kG][4] = {};
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll(kAhead)
+  for (int s = s0; s < s1; ++s) {
+    const int64_t k = (int64_t)s * kStep + q * 8;
+    const bool in = k < p.K;  // (K is a multiple of 8)
+    const uint4 a = in && a_on ? __ldg(reinterpret_cast<const uint4*>(wa + k)) : zero;
+    const uint4 b = in && b_on ? __ldg(reinterpret_cast<const uint4*>(wb + k)) : zero;
+    const uint32_t first[4] = {a.x, b.x, a.y, b.y}, second[4] = {a.z, b.z, a.w, b.w};
+    uint4 v[kG];
+#pragma unroll
+    for (int j = 0; j < kG; ++j) v[j] = in && (kG == 1 || j * 8 < rows) ? ld_nc_16(x[j] + k) : zero;
+#pragma unroll
+    for (int j = 0; j < kG; ++j)
+      if (kG == 1 || j * 8 < rows) mma16816<T>(acc[j], first, v[j].x, v[j].y), mma16816<T>(acc[j], second, v[j].z, v[j].w);
+  }
+#pragma unroll
+  for (int j = 0; j < kG; ++j) {
+    if (j * 8 >= rows) break;
+    *reinterpret_cast<float2*>(part + g * pitch + j * 8 + q * 2) = make_float2(acc[j][0], acc[j][1]);
+    *reinterpret_cast<float2*>(part + (g + 8) * pitch + j * 8 + q * 2) = make_float2(acc[j][2], acc[j][3]);
+  }
+}
+
+// Up to kG groups of 8 activation rows.  `part` and `sums` are padded so that neither their writes nor their reads meet in a bank:
+// unpadded, 64 rows x 256 x 7168 took 12.8 us.
 template <typename T, int kG>
 __global__ void __launch_bounds__(kWarps * 32, 2) narrow_kernel(const Params p) {
   constexpr int kCols = kG * 8, kPartPitch = kCols + 8, kSumPitch = 17;
@@ -37,7 +70,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) narrow_kernel(const Params p) 
   __shared__ float sums[kCols * kSumPitch];
   __shared__ int32_t row[kSmallBlock];
   __shared__ int found[2];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2;
   const int rank = (int)(blockIdx.x % p.splits), n0 = (int)(blockIdx.x / p.splits % p.n_tiles) * 16;
   const int64_t block = blockIdx.x / p.splits / p.n_tiles;
   ptx::grid_dependency_wait();
@@ -67,37 +100,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) narrow_kernel(const Params p) 
   const bool a_on = na < p.N && na % p.rank_rows < used, b_on = nb < p.N && nb % p.rank_rows < used;
   const T* wa = w + (a_on ? na : 0) * p.K;
   const T* wb = w + (b_on ? nb : 0) * p.K;
-  const T* x[kG];
-#pragma unroll
-  for (int j = 0; j < kG; ++j) {
-    const int i = min(j * 8 + g, rows - 1);
-    x[j] = static_cast<const T*>(p.x) + (sorted ? (int64_t)row[i] : start + i) * p.ldx;
-  }
-  float acc[kG][4] = {};
   const int steps = (int)((p.K + kStep - 1) / kStep), parts = p.splits * kWarps, mine = rank * kWarps + warp;
   const int s0 = (int)((int64_t)mine * steps / parts), s1 = (int)((int64_t)(mine + 1) * steps / parts);
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  constexpr int kAhead = kG <= 2 ? 4 : 2;
-#pragma unroll(kAhead)
-  for (int s = s0; s < s1; ++s) {
-    const int64_t k = (int64_t)s * kStep + q * 8;
-    const bool in = k < p.K;  // (K is a multiple of 8)
-    const uint4 a = in && a_on ? __ldg(reinterpret_cast<const uint4*>(wa + k)) : zero;
-    const uint4 b = in && b_on ? __ldg(reinterpret_cast<const uint4*>(wb + k)) : zero;
-    const uint32_t first[4] = {a.x, b.x, a.y, b.y}, second[4] = {a.z, b.z, a.w, b.w};
-    uint4 v[kG];
-#pragma unroll
-    for (int j = 0; j < kG; ++j) v[j] = in && j * 8 < rows ? ld_nc_16(x[j] + k) : zero;
-#pragma unroll
-    for (int j = 0; j < kG; ++j)
-      if (j * 8 < rows) mma16816<T>(acc[j], first, v[j].x, v[j].y), mma16816<T>(acc[j], second, v[j].z, v[j].w);
-  }
-#pragma unroll
-  for (int j = 0; j < kG; ++j) {
-    if (j * 8 >= rows) break;
-    *reinterpret_cast<float2*>(&part[warp][g][j * 8 + q * 2]) = make_float2(acc[j][0], acc[j][1]);
-    *reinterpret_cast<float2*>(&part[warp][g + 8][j * 8 + q * 2]) = make_float2(acc[j][2], acc[j][3]);
-  }
+  auto row_of = [&](int i) { return sorted ? (int64_t)row[i] : start + i; };
+  float* to = &part[warp][0][0];
+  // (blocks of a batch of many adapters have few rows)
+  if (rows <= 8) add_up<T, 1, 6>(p, wa, wb, a_on, b_on, rows, s0, s1, lane, to, kPartPitch, row_of);
+  else if (kG > 2 && rows <= 16) add_up<T, 2, 4>(p, wa, wb, a_on, b_on, rows, s0, s1, lane, to, kPartPitch, row_of);
+  else add_up<T, kG, (kG <= 2 ? 4 : 2)>(p, wa, wb, a_on, b_on, rows, s0, s1, lane, to, kPartPitch, row_of);
   __syncthreads();
   // The warps' sums, then the CTAs', each in ascending order of K.
   for (int i = tid; i < 16 * kCols; i += kWarps * 32) {

@@ -29,18 +29,28 @@ __device__ __forceinline__ bool scan_block(const Blocks& b, int block, int lane,
     return id >= 0 && id < b.adapters ? id : -1;
   };
   const int k0 = key(lane), k1 = key(lane + 32);
-  uint32_t left0 = b.ids_rows >= 32 ? 0xffffffffu : (1u << b.ids_rows) - 1;
-  uint32_t left1 = b.ids_rows >= 64 ? 0xffffffffu : b.ids_rows > 32 ? (1u << (b.ids_rows - 32)) - 1 : 0;
-  uint32_t in0 = 0, in1 = 0;
-  for (int i = 0; i <= block; ++i) {
-    if ((left0 | left1) == 0) return false;
-    adapter = left0 ? __shfl_sync(0xffffffffu, k0, __ffs(left0) - 1) : __shfl_sync(0xffffffffu, k1, __ffs(left1) - 1);
-    in0 = __ballot_sync(0xffffffffu, k0 == adapter) & left0, in1 = __ballot_sync(0xffffffffu, k1 == adapter) & left1;
-    left0 &= ~in0, left1 &= ~in1;
+  const uint32_t all0 = b.ids_rows >= 32 ? 0xffffffffu : (1u << b.ids_rows) - 1;
+  const uint32_t all1 = b.ids_rows >= 64 ? 0xffffffffu : b.ids_rows > 32 ? (1u << (b.ids_rows - 32)) - 1 : 0;
+  // the first row of every adapter
+  const uint32_t before = (1u << lane) - 1, same0 = __match_any_sync(0xffffffffu, k0) & all0;
+  const uint32_t first0 = __ballot_sync(0xffffffffu, (same0 & before) == 0) & all0;
+  uint32_t first1 = 0;
+  if (all1 != 0) {
+    const uint32_t same1 = __match_any_sync(0xffffffffu, k1) & all1;
+    bool seen = (same1 & before) != 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) seen |= __shfl_sync(0xffffffffu, k0, i) == k1;
+    first1 = __ballot_sync(0xffffffffu, !seen) & all1;
   }
-  const uint32_t below = (1u << lane) - 1;
-  if (in0 >> lane & 1u) row[__popc(in0 & below)] = lane;
-  if (in1 >> lane & 1u) row[__popc(in0) + __popc(in1 & below)] = lane + 32;
+  const bool low = block < __popc(first0);
+  const uint32_t firsts = low ? first0 : first1;
+  const int nth = low ? block : block - __popc(first0);
+  const uint32_t it = __ballot_sync(0xffffffffu, (firsts >> lane & 1u) && __popc(firsts & before) == nth);
+  if (it == 0) return false;
+  adapter = __shfl_sync(0xffffffffu, low ? k0 : k1, __ffs(it) - 1);
+  const uint32_t in0 = __ballot_sync(0xffffffffu, k0 == adapter) & all0, in1 = __ballot_sync(0xffffffffu, k1 == adapter) & all1;
+  if (in0 >> lane & 1u) row[__popc(in0 & before)] = lane;
+  if (in1 >> lane & 1u) row[__popc(in0) + __popc(in1 & before)] = lane + 32;
   rows = __popc(in0) + __popc(in1);
   return true;
 }

@@ -1,8 +1,9 @@
 // y[t, n] = sum_k x[t, k] w[n, k] for many rows (see narrow.cuh), on tcgen05.mma.kind::f16.
 //
-// A tile is 128 activation rows by up to 256 weight rows, in stages of 64 columns.  The weights, and activations that lie one after the
-// other, come by TMA; sorted activations by asynchronous copies of 16 bytes of two warps (TMA gathers of four rows took 2 us a stage of 128
-// rows: 4096 rows of 7168 columns 55 us).  K is split over the CTAs of a cluster, which add their sums through distributed shared memory in a fixed order.
+// A tile is 128 activation rows by up to 256 weight rows, in stages of 64 columns.  The weights and activations that lie one after the other
+// come by TMA; of sorted activations 32 rows at a time that do (the tokens of a long request), the others by asynchronous copies of 16 bytes of
+// two warps, which take 0.65 us a stage of 128 rows (TMA gathers of four rows: 2 us).  K is split over the CTAs of a cluster, which add their
+// sums through distributed shared memory in a fixed order.
 //
 // The instruction cuts off what does not fit its sum, each time: over 7168 columns that would be off by more than a float32 product is.  So
 // the sums of 256 columns begin from zero, in two buffers of tensor memory in turn, and meet in the registers of eight warps.
@@ -28,6 +29,7 @@ struct Ctl {
   uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
   uint32_t tmem_base;
   int abort_flag;
+  int first[4];  // the first row of 32 of the tile that lie one after the other, else -1
 };
 
 struct TileParams {
@@ -71,12 +73,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const bool sorted = p.blocks.order != nullptr;
   const uint32_t full = ptx::smem_u32(ctl->full), empty = ptx::smem_u32(ctl->empty), acc_full = ptx::smem_u32(ctl->acc_full),
                  acc_empty = ptx::smem_u32(ctl->acc_empty);
-  if (tid == 0) {
-    for (int s = 0; s < t.stages; ++s) ptx::mbar_init(full + s * 8, sorted ? 65 : 1), ptx::mbar_init(empty + s * 8, 1);
-    for (int b = 0; b < 2; ++b) ptx::mbar_init(acc_full + b * 8, 1), ptx::mbar_init(acc_empty + b * 8, 8);
-    ctl->abort_flag = 0;
-    ptx::mbar_fence_init();
-  }
   // (tensor memory is taken once the kernel in front has ended; the kernel behind may start when every CTA has its own)
   ptx::grid_dependency_wait();
   int64_t start = block * kTileBlock;
@@ -89,6 +85,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       return;
     }
     start = __ldcg(p.blocks.start + block), rows = __ldcg(p.blocks.rows + block);
+    if (warp < 4) {
+      const int at = warp * 32 + lane, row = __ldcg(p.blocks.order + start + min(at, rows - 1)), first = __shfl_sync(0xffffffffu, row, 0);
+      const bool run = __all_sync(0xffffffffu, at >= rows || row == first + lane);
+      if (lane == 0) ctl->first[warp] = run ? first : -1;
+    }
+    __syncthreads();
+  }
+  // 32 rows that have to be copied one by one, a bit each; the number of 32 that hold rows
+  const int groups = (rows + 31) / 32;
+  int scattered = 0;
+  if (sorted)
+    for (int i = 0; i < groups; ++i) scattered |= ctl->first[i] < 0 ? 1 << i : 0;
+  if (tid == 0) {
+    for (int s = 0; s < t.stages; ++s) ptx::mbar_init(full + s * 8, scattered ? 65 : 1), ptx::mbar_init(empty + s * 8, 1);
+    for (int b = 0; b < 2; ++b) ptx::mbar_init(acc_full + b * 8, 1), ptx::mbar_init(acc_empty + b * 8, 8);
+    ctl->abort_flag = 0;
+    ptx::mbar_fence_init();
   }
   if (warp == 9) {
     ptx::tmem_alloc(ptx::smem_u32(&ctl->tmem_base), 2 * kBuf);
@@ -112,14 +125,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         const uint32_t at = base + s * stage_bytes, bar = full + s * 8;
-        ptx::mbar_arrive_expect_tx(bar, sorted ? w_bytes : kXBytes + w_bytes);
+        ptx::mbar_arrive_expect_tx(bar, w_bytes + (sorted ? (uint32_t)(groups - __popc(scattered)) * (kXBytes / 4) : kXBytes));
         ptx::tma_load_3d(at + kXBytes, &map_w, bar, kb * kStageK * 2, n0, adapter);
-        if (!sorted) ptx::tma_load_2d(at, &map_x, bar, kb * kStageK * 2, (int)start);
+        if (!sorted) {
+          ptx::tma_load_2d(at, &map_x, bar, kb * kStageK * 2, (int)start);
+        } else {
+          for (int j = 0; j < groups; ++j)
+            if (!(scattered >> j & 1)) ptx::tma_load_2d(at + j * (kXBytes / 4), &map_x, bar, kb * kStageK * 2, ctl->first[j]);
+        }
       }
     }
     __syncwarp();
   } else if (warp >= 10) {
-    if (sorted) {
+    if (scattered) {
       // Rows warp, + 2, .. of four at a time; a lane has 16 bytes of one of them.  (Rows past the last hold what they held; their sums are
       // nobody's.)
       const int c = lane & 7, r0 = (warp - 10) * 4 + (lane >> 3);
@@ -141,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int64_t off = bytes ? k * 2 : 0;
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-          if (r0 + j * 8 < rows) ptx::cp_async_16(base + s * stage_bytes + to + j * 1024, from[j] + off, bytes);
+          if ((scattered >> (j / 4) & 1) && r0 + j * 8 < rows) ptx::cp_async_16(base + s * stage_bytes + to + j * 1024, from[j] + off, bytes);
         ptx::cp_async_arrive(full + s * 8);
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
@@ -156,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (i % kChunk == 0 && chunk >= 2) ok = NARROW_WAIT(acc_empty + buf * 8, ((chunk >> 1) & 1) ^ 1);
         if (ok) ok = NARROW_WAIT(full + s * 8, (i / t.stages) & 1);
         if (!ok) break;
-        if (sorted) ptx::fence_async_smem();  // (the copies' writes, which the barrier has shown, before the tensor core's reads)
+        if (scattered) ptx::fence_async_smem();  // (the copies' writes, which the barrier has shown, before the tensor core's reads)
         ptx::tc_fence_after();
         const uint32_t at = base + s * stage_bytes, x_lo = desc_lo(at), w_lo = desc_lo(at + kXBytes);
 #pragma unroll
@@ -310,7 +328,7 @@ int tile_product(const Params& given, int dtype, int64_t max_blocks, cudaStream_
   t.stages = (int)std::min<uint32_t>(kMaxStages, kRing / (kXBytes + (uint32_t)t.nt * kStageK * 2));
   CUtensorMap mx, mw;
   const uint64_t xd[2] = {(uint64_t)p.K * 2, (uint64_t)p.T}, xs[1] = {(uint64_t)p.ldx * 2};
-  const uint32_t xb[2] = {kStageK * 2, (uint32_t)kTileBlock};
+  const uint32_t xb[2] = {kStageK * 2, p.blocks.order != nullptr ? kTileBlock / 4u : (uint32_t)kTileBlock};
   int rc = get_tile_map(p.x, 2, xd, xs, xb, true, &mx);
   if (rc) return rc;
   const uint64_t wd[3] = {(uint64_t)p.K * 2, (uint64_t)p.N, (uint64_t)p.adapters}, ws[2] = {(uint64_t)p.K * 2, (uint64_t)(p.N * p.K * 2)};

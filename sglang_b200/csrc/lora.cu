@@ -104,138 +104,181 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// A CTA takes up to `sub` rows of a block and `passes` times 8 warps' columns.  kPairs: 32 values of the rank at most, which are two
-// instructions; kTiles: groups of 8 columns of a warp.  As a sum does not mind the order of its terms, a lane's 16 consecutive bytes of a weight
-// row (and of a row of h alike) are its part of both.  A lane holds the same two kTiles neighbouring columns of a token in all groups, so that
-// base and out go by 4 kTiles bytes.  Weights, and base of the first 16 rows, come by asynchronous copies, each lane's to a place of its own,
-// kDepth - 1 passes ahead and before h is there: they are what bounds this kernel where few tokens name an adapter.
+// The units of 8 warps' columns of all blocks, columns fastest, are cut evenly over as many CTAs as run at once; a run is what a CTA has of one
+// block and one merged projection.  kPairs: 32 values of the rank at most, which are two instructions; kTiles: groups of 8 columns of a warp.
+// As a sum does not mind the order of its terms, a lane's 16 consecutive bytes of a weight row (and of a row of h alike) are its part of both
+// instructions.  A lane holds the same two kTiles neighbouring columns of a token in all groups, so that base and out go by 4 kTiles bytes.
+//
+// Weights and base bound this kernel.  They come by asynchronous copies, each lane's to a place of its own, kDepth - 1 steps (16 tokens of a
+// unit) ahead, and before h is there.
 template <int kPairs, int kTiles>
 struct ExpandCfg {
-  static constexpr int kLane = kPairs * kTiles * 16 + kTiles * 8;  // bytes of a lane and pass
+  static constexpr int kWeights = kPairs * kTiles * 16 * kWarps * 32, kBase = kTiles * 8 * kWarps * 32;  // bytes of a unit, of a step
   static constexpr int kDepth = kPairs == 1 ? 4 : kPairs == 2 && kTiles == 4 ? 3 : 2;
-  static constexpr int kStage = kLane * kWarps * 32, kCols = 8 * kTiles * kWarps;
+  static constexpr int kRing = kDepth * (kWeights + kBase), kCols = 8 * kTiles * kWarps;
   static constexpr int kPitch = kPairs * 128 + 64;  // of a token's two terms: two rows of 64 bytes are read without a bank conflict
-  static constexpr int kMostRows = (227 * 1024 - 4096 - kDepth * kStage) / kPitch >= 128 ? 128 : 64;
-  static_assert(kDepth * kStage + kMostRows * kPitch <= 227 * 1024 - 4096);
+  static constexpr int kMostRows = (227 * 1024 - 4096 - kRing) / kPitch >= 128 ? 128 : 64;
+  static_assert(kRing + kMostRows * kPitch <= 227 * 1024 - 4096);
 };
 
 template <typename T, int kPairs, int kTiles>
 __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
   using Cfg = ExpandCfg<kPairs, kTiles>;
   constexpr int kCols = 8 * kTiles, kMine = 2 * kTiles, kDepth = Cfg::kDepth;
-  extern __shared__ __align__(16) uint8_t tile[];  // [kDepth] stages, then [rows of a CTA][kPitch]
-  uint8_t* terms = tile + kDepth * Cfg::kStage;    // a token's high terms, then its low terms, 32 kPairs each
+  extern __shared__ __align__(16) uint8_t ring[];  // [kDepth] units' weights, [kDepth] steps' base, then [rows][kPitch]
+  uint8_t* terms = ring + Cfg::kRing;              // a token's high terms, then its low terms, 32 kPairs each
   __shared__ float unscale[narrow::kTileBlock];
   __shared__ int32_t token[narrow::kTileBlock];
-  __shared__ int found[2];
+  __shared__ int found[3];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
-  const int piece = (int)(blockIdx.x % (p.max_blocks * p.subs)), block = piece / p.subs, row0 = piece % p.subs * p.sub;
-  const int chunk = (int)(blockIdx.x / (p.max_blocks * p.subs));
+  const bool scan = p.blocks.ids != nullptr;
+  const int per = p.chunk0[p.S];  // units of a block
+  const uint8_t* base = static_cast<const uint8_t*>(p.base);
+  uint8_t* out = static_cast<uint8_t*>(p.out);
+  const uint32_t weights_at = ptx::smem_u32(ring) + tid * 16, base_at = ptx::smem_u32(ring) + kDepth * Cfg::kWeights + tid * (4 * kTiles);
+  constexpr uint32_t kChunk = kWarps * 32 * 16;
+  bool waited = false;
+
   // The launch in front let this one in after its own wait for all that came before it, so only h is not there yet.
-  int rows, adapter;
-  if (p.blocks.ids != nullptr) {
+  int block = -1, begin = 0, end = 0;
+  if (!scan) {
+    const int64_t all = (int64_t)__ldcg(p.blocks.count) * p.subs * per;
+    begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
+  } else {
     if (warp == 0) {
       int n = 0, a = -1;
-      const bool there = narrow::scan_block(p.blocks, block, lane, token, n, a);
-      if (lane == 0) found[0] = there ? n : 0, found[1] = a;
+      const int blocks = narrow::scan_block(p.blocks, 0, p.sub, lane, token, n, a);
+      if (lane == 0) found[0] = blocks;
     }
     __syncthreads();
-    rows = found[0], adapter = found[1];
-  } else {
-    if (block >= __ldcg(p.blocks.count)) return;
-    adapter = __ldcg(p.blocks.adapter + block);
-    const int start = __ldcg(p.blocks.start + block);
-    rows = __ldcg(p.blocks.rows + block);
-    if (tid < rows) token[tid] = __ldcg(p.blocks.order + start + tid);
-    __syncthreads();
+    const int64_t all = (int64_t)found[0] * p.subs * per;
+    begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
   }
-  if (row0 >= rows || (adapter < 0 && p.in_place)) return;
-  rows = min(rows - row0, p.sub);
-  int slice = 0;
-  while (slice + 1 < p.S && chunk >= p.chunk0[slice + 1]) ++slice;
-  const int64_t end = p.col0[slice + 1];
-  const int64_t c0 = p.col0[slice] + (int64_t)(chunk - p.chunk0[slice]) * p.passes * Cfg::kCols + warp * kCols;
-  const int passes = c0 < end ? (int)min((int64_t)p.passes, (end - c0 + Cfg::kCols - 1) / Cfg::kCols) : 0;
-  const int used = adapter < 0 ? 0 : p.ranks != nullptr ? min(max(__ldg(p.ranks + adapter), 0), p.R) : p.R;
-  const int pairs = (used + 31) / 32;
-  const uint8_t* weights = static_cast<const uint8_t*>(p.b) + (adapter < 0 ? 0 : (int64_t)adapter * p.N * p.R * 2);
-  const T* base = static_cast<const T*>(p.base);
-  T* out = static_cast<T*>(p.out);
-  const int64_t ta = token[row0 + min(g, rows - 1)], tb = token[row0 + min(g + 8, rows - 1)];
-  const uint32_t mine_at = ptx::smem_u32(tile) + tid * 16;  // (chunk i of a stage at i times 16 bytes of all threads)
-  constexpr uint32_t kChunk = kWarps * 32 * 16;
-
-  auto fetch = [&](int pass) {
-    if (pass < passes) {
-      const int64_t c = c0 + (int64_t)pass * Cfg::kCols;
-      const uint32_t to = mine_at + pass % kDepth * Cfg::kStage;
-#pragma unroll
-      for (int j = 0; j < kTiles; ++j) {
-        const int64_t n = c + (g >> 1) * kMine + j * 2 + (g & 1);
-        const uint8_t* from = weights + (n < end ? n : c) * p.R * 2 + q * 16;
-#pragma unroll
-        for (int s = 0; s < kPairs; ++s)
-          if (s < pairs) {  // (beyond the rank anything may stand: zeros instead)
-            const int there = n < end ? min(max((used - s * 32 - q * 8) * 2, 0), 16) : 0;
-            ptx::cp_async_16(to + (s * kTiles + j) * kChunk, there > 0 ? from + s * 64 : weights, there);
-          }
+  int all_rows = 0, adapter = -1;
+  for (int at = begin; at < end;) {
+    const int piece = at / per, unit0 = at - piece * per, row0 = piece % p.subs * p.sub;
+    int slice = 0;
+    while (slice + 1 < p.S && unit0 >= p.chunk0[slice + 1]) ++slice;
+    const int units = min(p.chunk0[slice + 1] - unit0, end - at);
+    at += units;
+    __syncthreads();  // (nobody is at the run before this one any more)
+    if (piece / p.subs != block) {
+      block = piece / p.subs;
+      if (scan) {
+        if (warp == 0) {
+          int n = 0, a = -1;
+          narrow::scan_block(p.blocks, block, p.sub, lane, token, n, a);
+          if (lane == 0) found[1] = n, found[2] = a;
+        }
+        __syncthreads();
+        all_rows = found[1], adapter = found[2];
+      } else {
+        adapter = __ldcg(p.blocks.adapter + block);
+        const int start = __ldcg(p.blocks.start + block);
+        all_rows = __ldcg(p.blocks.rows + block);
+        if (tid < all_rows) token[tid] = __ldcg(p.blocks.order + start + tid);
+        __syncthreads();
       }
-      if (p.vec) {
-        const int64_t n = c + q * kMine;
-        const uint32_t base_to = ptx::smem_u32(tile) + pass % kDepth * Cfg::kStage + kPairs * kTiles * kChunk;
-        if (n < end) {
-          if constexpr (kTiles == 4) {
-            if (g < rows) ptx::cp_async_16(base_to + tid * 16, base + ta * p.ld_base + n, 16);
-            if (g + 8 < rows) ptx::cp_async_16(base_to + kChunk + tid * 16, base + tb * p.ld_base + n, 16);
-          } else {
-            if (g < rows) ptx::cp_async_8(base_to + tid * 8, base + ta * p.ld_base + n);
-            if (g + 8 < rows) ptx::cp_async_8(base_to + kChunk / 2 + tid * 8, base + tb * p.ld_base + n);
+    }
+    if (row0 >= all_rows || (adapter < 0 && p.in_place)) continue;
+    const int rows = min(all_rows - row0, p.sub), steps = units * ((rows + 15) / 16);
+    const int64_t stop = p.col0[slice + 1];
+    const int64_t c0 = p.col0[slice] + (int64_t)(unit0 - p.chunk0[slice]) * Cfg::kCols + warp * kCols;
+    const int used = adapter < 0 ? 0 : p.ranks != nullptr ? min(max(__ldg(p.ranks + adapter), 0), p.R) : p.R;
+    const int pairs = (used + 31) / 32;
+    const uint8_t* weights = static_cast<const uint8_t*>(p.b) + (adapter < 0 ? 0 : (int64_t)adapter * p.N * p.R * 2);
+
+    // What a lane copies and stores, as far as it is the same for all units: its part of a weight row, the rows of the first 16 tokens.
+    uint32_t part[kPairs];  // bytes that count (beyond the rank anything may stand: zeros instead)
+#pragma unroll
+    for (int s = 0; s < kPairs; ++s) part[s] = (uint32_t)min(max((used - s * 32 - q * 8) * 2, 0), 16);
+    const int64_t row_bytes = (int64_t)p.R * 2;
+    const uint8_t* next_weights = weights + (c0 + (g >> 1) * kMine + (g & 1)) * row_bytes + q * 16;
+    auto row_of = [&](int m, int i) { return (int64_t)token[row0 + min(m + i * 8 + g, rows - 1)]; };
+    const int64_t first_row[2] = {row_of(0, 0), row_of(0, 1)};
+    const int64_t mine0 = c0 + q * kMine;
+    const uint8_t* base_row[2] = {base + (first_row[0] * p.ld_base + mine0) * 2, base + (first_row[1] * p.ld_base + mine0) * 2};
+    uint8_t* out_row[2] = {out + (first_row[0] * p.ld_out + mine0) * 2, out + (first_row[1] * p.ld_out + mine0) * 2};
+
+    // The step that is asked for next: its unit, 16 tokens and places.
+    int ahead_unit = 0, ahead_m = 0, ahead_left = (int)min((int64_t)units * Cfg::kCols, stop - c0);  // columns from the warp's first on
+    uint32_t weights_slot = 0, base_slot = 0;
+    auto fetch = [&]() {
+      if (ahead_unit < units) {
+        if (ahead_m == 0) {
+#pragma unroll
+          for (int j = 0; j < kTiles; ++j) {
+            const bool on = ahead_left >= kCols || (g >> 1) * kMine + j * 2 + (g & 1) < ahead_left;
+#pragma unroll
+            for (int s = 0; s < kPairs; ++s)
+              if (s < pairs)
+                ptx::cp_async_16(weights_at + weights_slot + (s * kTiles + j) * kChunk, on && part[s] ? next_weights + j * 2 * row_bytes + s * 64 : weights,
+                                 on ? part[s] : 0);
+          }
+          next_weights += Cfg::kCols * row_bytes;
+          weights_slot = weights_slot == (kDepth - 1) * Cfg::kWeights ? 0 : weights_slot + Cfg::kWeights;
+        }
+        if (p.vec && q * kMine < ahead_left) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (ahead_m + i * 8 + g >= rows) continue;
+            const uint8_t* from = base_row[i] + (int64_t)ahead_unit * (Cfg::kCols * 2);
+            if (ahead_m > 0) from += (row_of(ahead_m, i) - first_row[i]) * p.ld_base * 2;
+            if constexpr (kTiles == 4) ptx::cp_async_16(base_at + base_slot + i * (Cfg::kBase / 2), from, 16);
+            else ptx::cp_async_8(base_at + base_slot + i * (Cfg::kBase / 2), from);
           }
         }
+        base_slot = base_slot == (kDepth - 1) * Cfg::kBase ? 0 : base_slot + Cfg::kBase;
+        ahead_m += 16;
+        if (ahead_m >= rows) ahead_m = 0, ++ahead_unit, ahead_left -= Cfg::kCols;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < kDepth - 1; ++i) fetch();
+    if (!waited) {
+      ptx::grid_dependency_wait();
+      ptx::launch_dependents();
+      waited = true;
+    }
+    const float scaling = adapter >= 0 && p.scalings != nullptr ? __ldg(p.scalings + adapter) : 1.f;
+    // (two rows' loads at a time)
+    for (int i = warp; i < rows && used > 0; i += 2 * kWarps) {
+      float v[2][kPairs];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float* h = p.h + ((int64_t)token[row0 + min(i + u * kWarps, rows - 1)] * p.S + slice) * p.R;
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) v[u][j] = j * 32 + lane < used ? __ldcg(h + j * 32 + lane) * scaling : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int row = i + u * kWarps;
+        if (row >= rows) break;
+        uint16_t* to = reinterpret_cast<uint16_t*>(terms + row * Cfg::kPitch);
+        const float inv = split_row<T>(v[u], kPairs * 32, lane, [&](int r, uint16_t hi, uint16_t lo) { to[r] = hi, to[kPairs * 32 + r] = lo; });
+        if (lane == 0) unscale[row] = inv;
       }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-#pragma unroll
-  for (int i = 0; i < kDepth - 1; ++i) fetch(i);
-  ptx::grid_dependency_wait();
-  ptx::launch_dependents();
-  const float scaling = adapter >= 0 && p.scalings != nullptr ? __ldg(p.scalings + adapter) : 1.f;
-  // (two rows' loads at a time)
-  for (int i = warp; i < rows && used > 0; i += 2 * kWarps) {
-    float v[2][kPairs];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const float* h = p.h + ((int64_t)token[row0 + min(i + u * kWarps, rows - 1)] * p.S + slice) * p.R;
-#pragma unroll
-      for (int j = 0; j < kPairs; ++j) v[u][j] = j * 32 + lane < used ? __ldcg(h + j * 32 + lane) * scaling : 0.f;
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int row = i + u * kWarps;
-      if (row >= rows) break;
-      uint16_t* at = reinterpret_cast<uint16_t*>(terms + row * Cfg::kPitch);
-      const float inv = split_row<T>(v[u], kPairs * 32, lane, [&](int r, uint16_t hi, uint16_t lo) { at[r] = hi, at[kPairs * 32 + r] = lo; });
-      if (lane == 0) unscale[row] = inv;
-    }
-  }
-  __syncthreads();
+    __syncthreads();
 
-  for (int pass = 0; pass < passes; ++pass) {
-    fetch(pass + kDepth - 1);
-    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
-    const uint32_t from = mine_at + pass % kDepth * Cfg::kStage;
-    const int64_t mine = c0 + (int64_t)pass * Cfg::kCols + q * kMine;
-    const int cols = (int)max((int64_t)0, min((int64_t)kMine, end - mine));
-    for (int m = 0; m < rows; m += 16) {
+    int m = 0, left = (int)min((int64_t)units * Cfg::kCols, stop - c0);
+    int64_t along = 0;  // of the unit, in bytes
+    uint32_t from = weights_at, staged = base_at;
+    for (int step = 0; step < steps; ++step) {
+      fetch();
+      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+      const int cols = max(0, min(kMine, left - q * kMine));
+      const bool both = rows - m > 8;
       float acc[kTiles][4] = {};
       // (rows past the last are not written, and meet only their own sums)
       const uint8_t *pa = terms + (m + g) * Cfg::kPitch + q * 16, *pb = pa + 8 * Cfg::kPitch;
+      const uint4 zero = make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int s = 0; s < kPairs; ++s) {
         if (s >= pairs) break;
-        const uint4 ah = *reinterpret_cast<const uint4*>(pa + s * 64), bh = *reinterpret_cast<const uint4*>(pb + s * 64);
-        const uint4 al = *reinterpret_cast<const uint4*>(pa + kPairs * 64 + s * 64), bl = *reinterpret_cast<const uint4*>(pb + kPairs * 64 + s * 64);
+        const uint4 ah = *reinterpret_cast<const uint4*>(pa + s * 64), al = *reinterpret_cast<const uint4*>(pa + kPairs * 64 + s * 64);
+        const uint4 bh = both ? *reinterpret_cast<const uint4*>(pb + s * 64) : zero, bl = both ? *reinterpret_cast<const uint4*>(pb + kPairs * 64 + s * 64) : zero;
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) {
           const uint4 w = ptx::lds_128(from + (s * kTiles + j) * kChunk);
@@ -248,79 +291,80 @@ __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int r = m + g + 8 * i;
-        if (r >= rows || cols == 0) continue;
-        const int64_t t = token[row0 + r];
-        const T* had = base + t * p.ld_base + mine;
-        T* to = out + t * p.ld_out + mine;
-        uint32_t now[kTiles] = {};
-        if (p.vec) {
-          if constexpr (kTiles == 4) {
-            *reinterpret_cast<uint4*>(now) = m == 0 ? ptx::lds_128(from + (kPairs * kTiles + i) * kChunk) : *reinterpret_cast<const uint4*>(had);
+        if (r < rows && cols > 0) {
+          const int64_t down = m > 0 ? row_of(m, i) - first_row[i] : 0;
+          T* to = reinterpret_cast<T*>(out_row[i] + along + down * p.ld_out * 2);
+          uint32_t now[kTiles] = {};
+          if (p.vec) {
+            if constexpr (kTiles == 4) *reinterpret_cast<uint4*>(now) = ptx::lds_128(staged + i * (Cfg::kBase / 2));
+            else *reinterpret_cast<uint2*>(now) = ptx::lds_64(staged + i * (Cfg::kBase / 2));
           } else {
-            const uint8_t* staged = tile + pass % kDepth * Cfg::kStage + kPairs * kTiles * kChunk + i * (kChunk / 2) + tid * 8;
-            *reinterpret_cast<uint2*>(now) = m == 0 ? ptx::lds_64(ptx::smem_u32(staged)) : *reinterpret_cast<const uint2*>(had);
+            const T* had = reinterpret_cast<const T*>(base_row[i] + along + down * p.ld_base * 2);
+#pragma unroll
+            for (int j = 0; j < kMine; ++j)
+              if (j < cols) now[j / 2] |= (uint32_t)bits(had[j]) << (j % 2 * 16);
           }
-        } else {
+          if (used > 0) {
+            const float inv = unscale[r];
 #pragma unroll
-          for (int j = 0; j < kMine; ++j)
-            if (j < cols) now[j / 2] |= (uint32_t)bits(had[j]) << (j % 2 * 16);
-        }
-        if (used > 0) {
-          const float inv = unscale[r];
-#pragma unroll
-          for (int j = 0; j < kTiles; ++j) {
-            const float2 was = unpack2<T>(now[j]);
-            now[j] = pack2<T>(was.x + acc[j][2 * i] * inv, was.y + acc[j][2 * i + 1] * inv);
-          }
-        }
-        if (p.vec) {
-          if constexpr (kTiles == 4)
-            *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(now);
-          else
-            *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(now);
-        } else {
-#pragma unroll
-          for (int j = 0; j < kMine; ++j)
-            if (j < cols) {
-              const uint16_t v = (uint16_t)(now[j / 2] >> (j % 2 * 16));
-              to[j] = *reinterpret_cast<const T*>(&v);
+            for (int j = 0; j < kTiles; ++j) {
+              const float2 was = unpack2<T>(now[j]);
+              now[j] = pack2<T>(was.x + acc[j][2 * i] * inv, was.y + acc[j][2 * i + 1] * inv);
             }
+          }
+          if (p.vec) {
+            if constexpr (kTiles == 4)
+              *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(now);
+            else
+              *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(now);
+          } else {
+#pragma unroll
+            for (int j = 0; j < kMine; ++j)
+              if (j < cols) {
+                const uint16_t v = (uint16_t)(now[j / 2] >> (j % 2 * 16));
+                to[j] = *reinterpret_cast<const T*>(&v);
+              }
+          }
         }
       }
+      staged = staged == base_at + (kDepth - 1) * Cfg::kBase ? base_at : staged + Cfg::kBase;
+      m += 16;
+      if (m >= rows) {
+        m = 0, left -= Cfg::kCols, along += Cfg::kCols * 2;
+        from = from == weights_at + (kDepth - 1) * Cfg::kWeights ? weights_at : from + Cfg::kWeights;
+      }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (!waited) ptx::grid_dependency_wait();  // (no CTA ends before the launch in front: the one behind counts on that)
 }
 
 template <typename T, int kPairs, int kTiles>
 static int launch_expand(Params& p, int block, cudaStream_t st) {
   using Cfg = ExpandCfg<kPairs, kTiles>;
-  int64_t units = 0;
-  for (int s = 0; s < p.S; ++s) units += (p.col0[s + 1] - p.col0[s] + Cfg::kCols - 1) / Cfg::kCols;
-  // Blocks are cut until there are as many CTAs as run at once, then a CTA takes as many passes as leave that many.
-  const int64_t want = (int64_t)std::min(4, (227 * 1024) / (Cfg::kDepth * Cfg::kStage + 16 * Cfg::kPitch + 3072)) * sm_count();
-  p.sub = std::min(block, Cfg::kMostRows);
-  while (p.sub > 16 && units * p.max_blocks * (block / p.sub) < want) p.sub /= 2;
-  p.subs = block / p.sub;
-  p.passes = (int)std::min<int64_t>(16, (units * p.max_blocks * p.subs + want - 1) / want);
-  int chunks = 0;
+  int units = 0;
   for (int s = 0; s < p.S; ++s) {
-    p.chunk0[s] = chunks;
-    const int64_t per = (int64_t)Cfg::kCols * p.passes;
-    chunks += (int)((p.col0[s + 1] - p.col0[s] + per - 1) / per);
+    p.chunk0[s] = units;
+    units += (int)((p.col0[s + 1] - p.col0[s] + Cfg::kCols - 1) / Cfg::kCols);
   }
-  p.chunk0[p.S] = chunks;
-  const int64_t grid = (int64_t)chunks * p.max_blocks * p.subs;
-  SGLB_REQUIRE(grid < (1ll << 31), "lora_add: %lld tiles are too many", (long long)grid);
+  p.chunk0[p.S] = units;
+  p.sub = std::min(block, Cfg::kMostRows);
+  // Few tokens and few columns: blocks of fewer rows, so that every SM has some.  (With a plan that would leave empty ones.)
+  if (p.blocks.ids != nullptr)
+    while (p.sub > 16 && (int64_t)units * ((p.blocks.ids_rows + p.sub - 1) / p.sub) < 2 * sm_count()) p.sub /= 2;
+  p.subs = p.blocks.ids != nullptr ? 1 : block / p.sub;
+  const size_t smem = (size_t)(Cfg::kRing + p.sub * Cfg::kPitch);
+  const int64_t all = (int64_t)units * (p.blocks.ids != nullptr ? p.max_blocks + p.blocks.ids_rows / p.sub : p.max_blocks * p.subs), at_once = std::min<int64_t>(4, 227 * 1024 / (int64_t)(smem + 3072)) * sm_count();
+  SGLB_REQUIRE(all < (1ll << 31), "lora_add: %lld tiles are too many", (long long)all);
   auto kern = expand_kernel<T, kPairs, kTiles>;
   static thread_local bool attr_set[64] = {false};  // the opt-in is per function and per device
   int dev = 0;
   SGLB_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    SGLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kDepth * Cfg::kStage + Cfg::kMostRows * Cfg::kPitch));
+    SGLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kRing + Cfg::kMostRows * Cfg::kPitch));
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  SGLB_CUDA(launch_pdl(kern, (unsigned)grid, kWarps * 32, (size_t)(Cfg::kDepth * Cfg::kStage + p.sub * Cfg::kPitch), st, p));
+  SGLB_CUDA(launch_pdl(kern, (unsigned)std::min(all, at_once), kWarps * 32, smem, st, p));
   return SGLB200_OK;
 }
 

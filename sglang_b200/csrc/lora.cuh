@@ -21,10 +21,10 @@ struct Params {
   const int32_t* ranks;   // or nullptr
   narrow::Blocks blocks;
   int64_t N, ld_base, ld_out;
-  int R, S, max_blocks, passes, vec, in_place;
-  int sub, subs;     // rows of a block that a CTA takes, CTAs of a block
+  int R, S, max_blocks, vec, in_place;
+  int sub, subs;     // a block is taken `sub` rows at a time, in `subs` parts
   int64_t col0[kMaxSlices + 1];  // first column of every merged projection, and the end
-  int chunk0[kMaxSlices + 1];    // the first chunk of passes x 8 warps x columns of a warp (lora_tile.cu: of 128 columns), and the end
+  int chunk0[kMaxSlices + 1];    // the first unit of columns, and the end
   uint32_t wait_probes;
 };
 

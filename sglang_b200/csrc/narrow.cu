@@ -81,8 +81,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) narrow_kernel(const Params p) 
   if (p.blocks.ids != nullptr) {
     if (warp == 0) {
       int n = 0, a = -1;
-      const bool there = scan_block(p.blocks, (int)block, lane, row, n, a);
-      if (lane == 0) found[0] = there ? n : 0, found[1] = a;
+      scan_block(p.blocks, (int)block, kScanRows, lane, row, n, a);  // (0 rows: there is no such block)
+      if (lane == 0) found[0] = n, found[1] = a;
     }
     __syncthreads();
     rows = found[0], adapter = found[1];

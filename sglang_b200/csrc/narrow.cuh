@@ -22,8 +22,9 @@ struct Blocks {
   int ids_rows, adapters;
 };
 
-// One warp: block `block` in the order of the adapters' first rows, its rows to `row` (ascending); false: there are not so many.
-__device__ __forceinline__ bool scan_block(const Blocks& b, int block, int lane, int32_t* row, int& rows, int& adapter) {
+// One warp: how many blocks of up to `most` rows there are, and of block `block`, in the order of their first rows, its rows (to `row`,
+// ascending), if it is one of them.
+__device__ __forceinline__ int scan_block(const Blocks& b, int block, int most, int lane, int32_t* row, int& rows, int& adapter) {
   auto key = [&](int t) {
     const int id = t < b.ids_rows ? __ldg(b.ids + t) : -1;
     return id >= 0 && id < b.adapters ? id : -1;
@@ -31,28 +32,30 @@ __device__ __forceinline__ bool scan_block(const Blocks& b, int block, int lane,
   const int k0 = key(lane), k1 = key(lane + 32);
   const uint32_t all0 = b.ids_rows >= 32 ? 0xffffffffu : (1u << b.ids_rows) - 1;
   const uint32_t all1 = b.ids_rows >= 64 ? 0xffffffffu : b.ids_rows > 32 ? (1u << (b.ids_rows - 32)) - 1 : 0;
-  // the first row of every adapter
-  const uint32_t before = (1u << lane) - 1, same0 = __match_any_sync(0xffffffffu, k0) & all0;
-  const uint32_t first0 = __ballot_sync(0xffffffffu, (same0 & before) == 0) & all0;
-  uint32_t first1 = 0;
+  // which of its adapter's rows a row is; every `most`-th begins a block
+  const uint32_t before = (1u << lane) - 1;
+  const int nth0 = __popc(__match_any_sync(0xffffffffu, k0) & all0 & before);
+  int nth1 = 0;
   if (all1 != 0) {
-    const uint32_t same1 = __match_any_sync(0xffffffffu, k1) & all1;
-    bool seen = (same1 & before) != 0;
+    nth1 = __popc(__match_any_sync(0xffffffffu, k1) & all1 & before);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) seen |= __shfl_sync(0xffffffffu, k0, i) == k1;
-    first1 = __ballot_sync(0xffffffffu, !seen) & all1;
+    for (int i = 0; i < 32; ++i) nth1 += __shfl_sync(0xffffffffu, k0, i) == k1;
   }
+  const uint32_t first0 = __ballot_sync(0xffffffffu, nth0 % most == 0) & all0, first1 = __ballot_sync(0xffffffffu, nth1 % most == 0) & all1;
+  const int blocks = __popc(first0) + __popc(first1);
   const bool low = block < __popc(first0);
   const uint32_t firsts = low ? first0 : first1;
-  const int nth = low ? block : block - __popc(first0);
-  const uint32_t it = __ballot_sync(0xffffffffu, (firsts >> lane & 1u) && __popc(firsts & before) == nth);
-  if (it == 0) return false;
-  adapter = __shfl_sync(0xffffffffu, low ? k0 : k1, __ffs(it) - 1);
-  const uint32_t in0 = __ballot_sync(0xffffffffu, k0 == adapter) & all0, in1 = __ballot_sync(0xffffffffu, k1 == adapter) & all1;
-  if (in0 >> lane & 1u) row[__popc(in0 & before)] = lane;
-  if (in1 >> lane & 1u) row[__popc(in0) + __popc(in1 & before)] = lane + 32;
-  rows = __popc(in0) + __popc(in1);
-  return true;
+  const uint32_t it = __ballot_sync(0xffffffffu, (firsts >> lane & 1u) && __popc(firsts & before) == (low ? block : block - __popc(first0)));
+  if (it == 0) return blocks;
+  const int from = __ffs(it) - 1;
+  adapter = __shfl_sync(0xffffffffu, low ? k0 : k1, from);
+  const int nth = __shfl_sync(0xffffffffu, low ? nth0 : nth1, from);
+  const bool in0 = k0 == adapter && (all0 >> lane & 1u) && nth0 >= nth && nth0 < nth + most;
+  const bool in1 = k1 == adapter && (all1 >> lane & 1u) && nth1 >= nth && nth1 < nth + most;
+  if (in0) row[nth0 - nth] = lane;
+  if (in1) row[nth1 - nth] = lane + 32;
+  rows = __popc(__ballot_sync(0xffffffffu, in0)) + __popc(__ballot_sync(0xffffffffu, in1));
+  return blocks;
 }
 
 struct Params {

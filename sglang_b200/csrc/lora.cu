@@ -25,7 +25,7 @@ constexpr int kPlanThreads = 1024;
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __restrict__ ids, int T, int L, int block, int32_t* order,
                                                             int32_t* start, int32_t* rows, int32_t* adapter, int32_t* count) {
   extern __shared__ int32_t counts[];  // [32 warps][L + 1], [L + 1] tokens and [L + 1] blocks before an adapter's
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, keys = L + 1;
+  const int tid = threadIdx.x, lane = tid & 31, warp = ptx::warp_index(), keys = L + 1;
   int32_t *mine = counts + warp * keys, *tokens_before = counts + 32 * keys, *blocks_before = tokens_before + keys;
   for (int i = tid; i < 32 * keys; i += kPlanThreads) counts[i] = 0;
   __syncthreads();
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
   __shared__ float unscale[narrow::kTileBlock];
   __shared__ int32_t token[narrow::kTileBlock];
   __shared__ int found[3];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+  const int tid = threadIdx.x, lane = tid & 31, warp = ptx::warp_index(), g = lane >> 2, q = lane & 3;
   const bool scan = p.blocks.ids != nullptr;
   const int per = p.chunk0[p.S];  // units of a block
   const uint8_t* base = static_cast<const uint8_t*>(p.base);
@@ -140,19 +140,37 @@ __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
   bool waited = false;
 
   // The launch in front let this one in after its own wait for all that came before it, so only h is not there yet.
+  // This CTA's units, and its block's tokens, rows and adapter to shared memory.
   int block = -1, begin = 0, end = 0;
-  if (!scan) {
-    const int64_t all = (int64_t)__ldcg(p.blocks.count) * p.subs * per;
+  auto cut = [&](int blocks) {
+    const int64_t all = (int64_t)blocks * p.subs * per;
     begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
-  } else {
-    if (warp == 0) {
+  };
+  auto find = [&](int which) {
+    if (scan) {
+      if (warp != 0) return;
       int n = 0, a = -1;
-      const int blocks = narrow::scan_block(p.blocks, 0, p.sub, lane, token, n, a);
+      narrow::scan_block(p.blocks, which, p.sub, lane, token, n, a);
+      if (lane == 0) found[1] = n, found[2] = a;
+    } else {
+      const int start = __ldcg(p.blocks.start + which), n = __ldcg(p.blocks.rows + which);
+      if (tid < n) token[tid] = __ldcg(p.blocks.order + start + tid);
+      if (tid == 0) found[1] = n, found[2] = __ldcg(p.blocks.adapter + which);
+    }
+  };
+  if (!scan) {
+    cut(__ldcg(p.blocks.count));
+  } else {
+    if (warp == 0) {  // (one warp looks at the tokens once for both)
+      int n = 0, a = -1;
+      const int blocks = narrow::scan_block(p.blocks, -1, p.sub, lane, token, n, a);
+      cut(blocks);
+      if (begin < end) find(begin / per);
       if (lane == 0) found[0] = blocks;
     }
+    block = -2;  // found already
     __syncthreads();
-    const int64_t all = (int64_t)found[0] * p.subs * per;
-    begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
+    cut(found[0]);
   }
   int all_rows = 0, adapter = -1;
   for (int at = begin; at < end;) {
@@ -161,24 +179,16 @@ __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
     while (slice + 1 < p.S && unit0 >= p.chunk0[slice + 1]) ++slice;
     const int units = min(p.chunk0[slice + 1] - unit0, end - at);
     at += units;
-    __syncthreads();  // (nobody is at the run before this one any more)
     if (piece / p.subs != block) {
-      block = piece / p.subs;
-      if (scan) {
-        if (warp == 0) {
-          int n = 0, a = -1;
-          narrow::scan_block(p.blocks, block, p.sub, lane, token, n, a);
-          if (lane == 0) found[1] = n, found[2] = a;
-        }
-        __syncthreads();
-        all_rows = found[1], adapter = found[2];
-      } else {
-        adapter = __ldcg(p.blocks.adapter + block);
-        const int start = __ldcg(p.blocks.start + block);
-        all_rows = __ldcg(p.blocks.rows + block);
-        if (tid < all_rows) token[tid] = __ldcg(p.blocks.order + start + tid);
+      if (block != -2) {  // (else it has been found)
+        __syncthreads();  // (nobody is at the run before this one any more)
+        find(piece / p.subs);
         __syncthreads();
       }
+      block = piece / p.subs;
+      all_rows = found[1], adapter = found[2];
+    } else {
+      __syncthreads();
     }
     if (row0 >= all_rows || (adapter < 0 && p.in_place)) continue;
     const int rows = min(all_rows - row0, p.sub), steps = units * ((rows + 15) / 16);
@@ -470,6 +480,6 @@ extern "C" int sglb200_lora_add(const void* x, const void* lora_a, const void* l
   // (its row pitches are 32-bit numbers of bytes)
   if (block == narrow::kTileBlock && p.vec && rank <= lora::kTileRank && base_stride < 1ll << 30 && out_stride < 1ll << 30)
     return lora::expand_tile(p, dtype, st);
-  const int rows = tokens <= 16 ? 16 : tokens <= 32 ? 32 : block;  // the most that a block can have
+  const int rows = tokens <= 16 ? 16 : tokens <= 32 ? 32 : scan ? narrow::kScanRows : block;  // the most that a block can have
   return dtype == 0 ? lora::expand<__nv_bfloat16>(p, rows, st) : lora::expand<__half>(p, rows, st);
 }

@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kThreads, 1) expand_tile_kernel(const Params p
   __shared__ Ctl ctl;
   uint8_t* spans = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t h_at = ptx::smem_u32(spans), ring = h_at + 2 * kKB * kSpan;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = ptx::warp_index(), lane = tid & 31;
   volatile int* abort_flag = &ctl.abort_flag;
   const uint32_t full = ptx::smem_u32(ctl.full), empty = ptx::smem_u32(ctl.empty), acc_full = ptx::smem_u32(ctl.acc_full),
                  acc_empty = ptx::smem_u32(ctl.acc_empty), h_full = ptx::smem_u32(&ctl.h_full);

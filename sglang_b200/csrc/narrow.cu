@@ -1,6 +1,6 @@
 // y[t, n] = sum_k x[t, k] w[n, k], few n, float32 sums (see narrow.cuh).
 //
-// narrow_kernel: the weights on the M side of mma.sync (16 of their rows), up to 64 activation rows on its N side, operands straight from
+// narrow_kernel: the weights on the M side of mma.sync (16 of their rows), up to 32 activation rows on its N side, operands straight from
 // global memory into registers: a lane takes 16 consecutive bytes of its row, and as a sum does not mind the order of its terms, those are
 // its part of two instructions, of the weights' rows and the activations' alike.  K is split over the warps of a CTA and the CTAs of a
 // cluster, whose sums meet in a fixed order.
@@ -64,13 +64,13 @@ __device__ __forceinline__ void add_up(const Params& p, const T* wa, const T* wb
 // Up to kG groups of 8 activation rows.  `part` and `sums` are padded so that neither their writes nor their reads meet in a bank:
 // unpadded, 64 rows x 256 x 7168 took 12.8 us.
 template <typename T, int kG>
-__global__ void __launch_bounds__(kWarps * 32, 2) narrow_kernel(const Params p) {
+__global__ void __launch_bounds__(kWarps * 32, 3) narrow_kernel(const Params p) {
   constexpr int kCols = kG * 8, kPartPitch = kCols + 8, kSumPitch = 17;
   __shared__ float part[kWarps][16][kPartPitch];
   __shared__ float sums[kCols * kSumPitch];
   __shared__ int32_t row[kSmallBlock];
   __shared__ int found[2];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2;
+  const int tid = threadIdx.x, lane = tid & 31, warp = ptx::warp_index(), g = lane >> 2;
   const int rank = (int)(blockIdx.x % p.splits), n0 = (int)(blockIdx.x / p.splits % p.n_tiles) * 16;
   const int64_t block = blockIdx.x / p.splits / p.n_tiles;
   ptx::grid_dependency_wait();
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) narrow_kernel(const Params p) 
   if (p.blocks.ids != nullptr) {
     if (warp == 0) {
       int n = 0, a = -1;
-      scan_block(p.blocks, (int)block, kScanRows, lane, row, n, a);  // (0 rows: there is no such block)
+      scan_block(p.blocks, (int)block, kSmallBlock, lane, row, n, a);  // (0 rows: there is no such block)
       if (lane == 0) found[0] = n, found[1] = a;
     }
     __syncthreads();
@@ -105,9 +105,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) narrow_kernel(const Params p) 
   auto row_of = [&](int i) { return sorted ? (int64_t)row[i] : start + i; };
   float* to = &part[warp][0][0];
   // (blocks of a batch of many adapters have few rows)
-  if (rows <= 8) add_up<T, 1, 6>(p, wa, wb, a_on, b_on, rows, s0, s1, lane, to, kPartPitch, row_of);
-  else if (kG > 2 && rows <= 16) add_up<T, 2, 4>(p, wa, wb, a_on, b_on, rows, s0, s1, lane, to, kPartPitch, row_of);
-  else add_up<T, kG, (kG <= 2 ? 4 : 2)>(p, wa, wb, a_on, b_on, rows, s0, s1, lane, to, kPartPitch, row_of);
+  if (rows <= 8) add_up<T, 1, 4>(p, wa, wb, a_on, b_on, rows, s0, s1, lane, to, kPartPitch, row_of);
+  else if (kG > 2 && rows <= 16) add_up<T, 2, 2>(p, wa, wb, a_on, b_on, rows, s0, s1, lane, to, kPartPitch, row_of);
+  else add_up<T, kG, (kG <= 2 ? 3 : 1)>(p, wa, wb, a_on, b_on, rows, s0, s1, lane, to, kPartPitch, row_of);
   __syncthreads();
   // The warps' sums, then the CTAs', each in ascending order of K.
   for (int i = tid; i < 16 * kCols; i += kWarps * 32) {
@@ -174,8 +174,7 @@ static int dispatch(Params& p, int64_t blocks, cudaStream_t st) {
   while (p.splits < 8 && tiles <= cluster_fits().paired[p.splits * 2] && steps >= p.splits * 2 * kWarps) p.splits *= 2;
   if (p.T <= 8) return launch<T, 1>(p, blocks, st);
   if (p.T <= 16) return launch<T, 2>(p, blocks, st);
-  if (p.T <= 32) return launch<T, 4>(p, blocks, st);
-  return launch<T, 8>(p, blocks, st);
+  return launch<T, 4>(p, blocks, st);
 }
 
 #ifndef NARROW_TILE_FROM

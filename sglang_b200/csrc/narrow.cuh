@@ -5,8 +5,8 @@
 namespace sglb200 {
 namespace narrow {
 
-// Rows that share their weights come in blocks: of 64 of them for narrow_kernel, of 128 for narrow_tile_kernel.
-constexpr int kSmallBlock = 64, kTileBlock = 128;
+// Rows that share their weights come in blocks: of 32 of them for narrow_kernel, of 128 for narrow_tile_kernel.
+constexpr int kSmallBlock = 32, kTileBlock = 128;
 
 // The blocks that the rows of a batch are sorted into by adapter.  Either a plan: `order` the rows, then per block where it starts in the
 // order, its rows and its adapter (-1: rows that name none), `count` the number of blocks.  Or, for up to kScanRows rows, which one warp

@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Ctl* ctl = reinterpret_cast<Ctl*>(ring + kRing);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = ptx::warp_index(), lane = tid & 31;
   volatile int* abort_flag = &ctl->abort_flag;
   const int rank = (int)(blockIdx.x % p.splits), n0 = (int)(blockIdx.x / p.splits % p.n_tiles) * t.nt;
   const int64_t block = blockIdx.x / p.splits / p.n_tiles;

@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPer <= 8 ? 4 : 1) route_kernel(c
   constexpr uint32_t kIndex = kPer - 1;  // the bits of a key that hold the expert's number in the lane, the lowest on top
   constexpr uint32_t kUnits = 32 * kPer;  // and the lane
   __shared__ uint32_t picks[kWarps][kMaxTopk];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = ptx::warp_index();
   ptx::launch_dependents();
   const Place at = place(p, lane);
   const bool biased = p.bias != nullptr;

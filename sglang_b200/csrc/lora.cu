@@ -122,7 +122,7 @@ struct ExpandCfg {
 };
 
 template <typename T, int kPairs, int kTiles>
-__global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
+__global__ void __launch_bounds__(kWarps * 32, kPairs == 1 ? 3 : 2) expand_kernel(const Params p) {
   using Cfg = ExpandCfg<kPairs, kTiles>;
   constexpr int kCols = 8 * kTiles, kMine = 2 * kTiles, kDepth = Cfg::kDepth;
   extern __shared__ __align__(16) uint8_t ring[];  // [kDepth] units' weights, [kDepth] steps' base, then [rows][kPitch]
@@ -202,45 +202,61 @@ __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
     uint32_t part[kPairs];  // bytes that count (beyond the rank anything may stand: zeros instead)
 #pragma unroll
     for (int s = 0; s < kPairs; ++s) part[s] = (uint32_t)min(max((used - s * 32 - q * 8) * 2, 0), 16);
-    const int64_t row_bytes = (int64_t)p.R * 2;
+    const uint32_t row_bytes = (uint32_t)p.R * 2;
     const uint8_t* next_weights = weights + (c0 + (g >> 1) * kMine + (g & 1)) * row_bytes + q * 16;
     auto row_of = [&](int m, int i) { return (int64_t)token[row0 + min(m + i * 8 + g, rows - 1)]; };
-    const int64_t first_row[2] = {row_of(0, 0), row_of(0, 1)};
     const int64_t mine0 = c0 + q * kMine;
-    const uint8_t* base_row[2] = {base + (first_row[0] * p.ld_base + mine0) * 2, base + (first_row[1] * p.ld_base + mine0) * 2};
-    uint8_t* out_row[2] = {out + (first_row[0] * p.ld_out + mine0) * 2, out + (first_row[1] * p.ld_out + mine0) * 2};
+    const uint8_t *next_base0 = base + (row_of(0, 0) * p.ld_base + mine0) * 2, *next_base1 = base + (row_of(0, 1) * p.ld_base + mine0) * 2;
+    uint8_t *to0 = out + (row_of(0, 0) * p.ld_out + mine0) * 2, *to1 = out + (row_of(0, 1) * p.ld_out + mine0) * 2;
+    const bool tall = rows > 16;
 
     // The step that is asked for next: its unit, 16 tokens and places.
-    int ahead_unit = 0, ahead_m = 0, ahead_left = (int)min((int64_t)units * Cfg::kCols, stop - c0);  // columns from the warp's first on
-    uint32_t weights_slot = 0, base_slot = 0;
+    int ahead_left = (int)min((int64_t)units * Cfg::kCols, stop - c0), ahead_m = 0;  // columns from the warp's first on
+    int ahead_steps = steps;
+    uint32_t weights_slot = weights_at, base_slot = base_at;
     auto fetch = [&]() {
-      if (ahead_unit < units) {
+      if (ahead_steps > 0) {
+        --ahead_steps;
         if (ahead_m == 0) {
+          if (ahead_left >= kCols) {
 #pragma unroll
-          for (int j = 0; j < kTiles; ++j) {
-            const bool on = ahead_left >= kCols || (g >> 1) * kMine + j * 2 + (g & 1) < ahead_left;
+            for (int j = 0; j < kTiles; ++j)
 #pragma unroll
-            for (int s = 0; s < kPairs; ++s)
-              if (s < pairs)
-                ptx::cp_async_16(weights_at + weights_slot + (s * kTiles + j) * kChunk, on && part[s] ? next_weights + j * 2 * row_bytes + s * 64 : weights,
-                                 on ? part[s] : 0);
+              for (int s = 0; s < kPairs; ++s)
+                if (s < pairs) ptx::cp_async_16(weights_slot + (s * kTiles + j) * kChunk, next_weights + j * 2 * row_bytes + s * 64, part[s]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j) {
+              const bool on = (g >> 1) * kMine + j * 2 + (g & 1) < ahead_left;
+#pragma unroll
+              for (int s = 0; s < kPairs; ++s)
+                if (s < pairs)
+                  ptx::cp_async_16(weights_slot + (s * kTiles + j) * kChunk, on ? next_weights + j * 2 * row_bytes + s * 64 : weights, on ? part[s] : 0);
+            }
           }
           next_weights += Cfg::kCols * row_bytes;
-          weights_slot = weights_slot == (kDepth - 1) * Cfg::kWeights ? 0 : weights_slot + Cfg::kWeights;
+          weights_slot = weights_slot == weights_at + (kDepth - 1) * Cfg::kWeights ? weights_at : weights_slot + Cfg::kWeights;
         }
         if (p.vec && q * kMine < ahead_left) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (ahead_m + i * 8 + g >= rows) continue;
-            const uint8_t* from = base_row[i] + (int64_t)ahead_unit * (Cfg::kCols * 2);
-            if (ahead_m > 0) from += (row_of(ahead_m, i) - first_row[i]) * p.ld_base * 2;
-            if constexpr (kTiles == 4) ptx::cp_async_16(base_at + base_slot + i * (Cfg::kBase / 2), from, 16);
-            else ptx::cp_async_8(base_at + base_slot + i * (Cfg::kBase / 2), from);
+          const uint8_t *from0 = next_base0, *from1 = next_base1;
+          if (ahead_m > 0) {
+            from0 += (row_of(ahead_m, 0) - row_of(0, 0)) * p.ld_base * 2, from1 += (row_of(ahead_m, 1) - row_of(0, 1)) * p.ld_base * 2;
+          }
+          if (ahead_m + g < rows) {
+            if constexpr (kTiles == 4) ptx::cp_async_16(base_slot, from0, 16);
+            else ptx::cp_async_8(base_slot, from0);
+          }
+          if (ahead_m + 8 + g < rows) {
+            if constexpr (kTiles == 4) ptx::cp_async_16(base_slot + Cfg::kBase / 2, from1, 16);
+            else ptx::cp_async_8(base_slot + Cfg::kBase / 2, from1);
           }
         }
-        base_slot = base_slot == (kDepth - 1) * Cfg::kBase ? 0 : base_slot + Cfg::kBase;
-        ahead_m += 16;
-        if (ahead_m >= rows) ahead_m = 0, ++ahead_unit, ahead_left -= Cfg::kCols;
+        base_slot = base_slot == base_at + (kDepth - 1) * Cfg::kBase ? base_at : base_slot + Cfg::kBase;
+        if (tall && ahead_m + 16 < rows) {
+          ahead_m += 16;
+        } else {
+          ahead_m = 0, ahead_left -= Cfg::kCols, next_base0 += Cfg::kCols * 2, next_base1 += Cfg::kCols * 2;
+        }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -301,15 +317,16 @@ __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int r = m + g + 8 * i;
-        if (r < rows && cols > 0) {
-          const int64_t down = m > 0 ? row_of(m, i) - first_row[i] : 0;
-          T* to = reinterpret_cast<T*>(out_row[i] + along + down * p.ld_out * 2);
+        if ((i == 0 || both) && r < rows && cols > 0) {
+          uint8_t* to_bytes = (i == 0 ? to0 : to1) + along;
+          if (m > 0) to_bytes += (row_of(m, i) - row_of(0, i)) * p.ld_out * 2;
+          T* to = reinterpret_cast<T*>(to_bytes);
           uint32_t now[kTiles] = {};
           if (p.vec) {
             if constexpr (kTiles == 4) *reinterpret_cast<uint4*>(now) = ptx::lds_128(staged + i * (Cfg::kBase / 2));
             else *reinterpret_cast<uint2*>(now) = ptx::lds_64(staged + i * (Cfg::kBase / 2));
           } else {
-            const T* had = reinterpret_cast<const T*>(base_row[i] + along + down * p.ld_base * 2);
+            const T* had = reinterpret_cast<const T*>(base + (row_of(m, i) * p.ld_base + mine0) * 2 + along);
 #pragma unroll
             for (int j = 0; j < kMine; ++j)
               if (j < cols) now[j / 2] |= (uint32_t)bits(had[j]) << (j % 2 * 16);
@@ -318,8 +335,9 @@ __global__ void __launch_bounds__(kWarps * 32) expand_kernel(const Params p) {
             const float inv = unscale[r];
 #pragma unroll
             for (int j = 0; j < kTiles; ++j) {
-              const float2 was = unpack2<T>(now[j]);
-              now[j] = pack2<T>(was.x + acc[j][2 * i] * inv, was.y + acc[j][2 * i + 1] * inv);
+              float2 was = unpack2<T>(now[j]);
+              ptx::fma2(was.x, was.y, __float_as_uint(acc[j][2 * i]), __float_as_uint(acc[j][2 * i + 1]), inv);
+              now[j] = pack2<T>(was.x, was.y);
             }
           }
           if (p.vec) {

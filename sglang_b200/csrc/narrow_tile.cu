@@ -2,7 +2,7 @@
 //
 // A tile is 128 activation rows by up to 256 weight rows, in stages of 64 columns.  The weights and activations that lie one after the other
 // come by TMA; of sorted activations 32 rows at a time that do (the tokens of a long request), the others by asynchronous copies of 16 bytes of
-// two warps, which take 0.65 us a stage of 128 rows (TMA gathers of four rows: 2 us).  K is split over the CTAs of a cluster, which add their
+// four warps (two took 0.65 us a stage of 128 rows, TMA gathers of four rows 2 us).  K is split over the CTAs of a cluster, which add their
 // sums through distributed shared memory in a fixed order.
 //
 // The instruction cuts off what does not fit its sum, each time: over 7168 columns that would be off by more than a float32 product is.  So
@@ -18,7 +18,7 @@ namespace narrow {
 
 __device__ int g_tile_status = 0;  // 0 ok, 1 = a pipeline wait expired
 
-constexpr int kThreads = 384;      // eight warps for the sums, one that loads, one that multiplies, two that copy sorted rows
+constexpr int kThreads = 320, kSortedThreads = 448;  // eight warps for the sums, one that loads, one that multiplies, four that copy sorted rows
 constexpr int kStageK = 64;        // columns of a stage: 128 bytes, one swizzle span
 constexpr int kChunk = 4;          // stages that are summed up in tensor memory
 constexpr int kMaxStages = 8;
@@ -58,8 +58,8 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
   (t.wait_probes != ptx::kProbesNone && (ptx::mbar_test(bar, parity) || ptx::mbar_wait_quiet(bar, parity)))
 
 // kUnits: groups of 16 columns of a tile that each of the two warpgroups adds up, at most.
-template <int kUnits>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int kUnits, bool kSorted>
+__global__ void __launch_bounds__(kSorted ? kSortedThreads : kThreads, 1)
     narrow_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const TileParams t) {
   constexpr uint32_t kBuf = kUnits * 32;  // columns of tensor memory of a buffer
   const Params& p = t.p;
@@ -70,7 +70,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = &ctl->abort_flag;
   const int rank = (int)(blockIdx.x % p.splits), n0 = (int)(blockIdx.x / p.splits % p.n_tiles) * t.nt;
   const int64_t block = blockIdx.x / p.splits / p.n_tiles;
-  const bool sorted = p.blocks.order != nullptr;
+  constexpr bool sorted = kSorted;
+  constexpr int kAll = kSorted ? kSortedThreads : kThreads, kCopies = 4 * 32;
   const uint32_t full = ptx::smem_u32(ctl->full), empty = ptx::smem_u32(ctl->empty), acc_full = ptx::smem_u32(ctl->acc_full),
                  acc_empty = ptx::smem_u32(ctl->acc_empty);
   // (tensor memory is taken once the kernel in front has ended; the kernel behind may start when every CTA has its own)
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (sorted)
     for (int i = 0; i < groups; ++i) scattered |= ctl->first[i] < 0 ? 1 << i : 0;
   if (tid == 0) {
-    for (int s = 0; s < t.stages; ++s) ptx::mbar_init(full + s * 8, scattered ? 65 : 1), ptx::mbar_init(empty + s * 8, 1);
+    for (int s = 0; s < t.stages; ++s) ptx::mbar_init(full + s * 8, scattered ? kCopies + 1 : 1), ptx::mbar_init(empty + s * 8, 1);
     for (int b = 0; b < 2; ++b) ptx::mbar_init(acc_full + b * 8, 1), ptx::mbar_init(acc_empty + b * 8, 8);
     ctl->abort_flag = 0;
     ptx::mbar_fence_init();
@@ -138,14 +139,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp >= 10) {
     if (scattered) {
-      // Rows warp, + 2, .. of four at a time; a lane has 16 bytes of one of them.  (Rows past the last hold what they held; their sums are
+      // Rows warp, + 4, .. of four at a time; a lane has 16 bytes of one of them.  (Rows past the last hold what they held; their sums are
       // nobody's.)
       const int c = lane & 7, r0 = (warp - 10) * 4 + (lane >> 3);
-      const uint8_t* from[16];
+      const uint8_t* from[8];
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        from[j] = static_cast<const uint8_t*>(p.x) + (int64_t)__ldcg(p.blocks.order + start + min(r0 + j * 8, rows - 1)) * p.ldx * 2 + c * 16;
-      const uint32_t to = (uint32_t)(r0 * 128 + ((c ^ (r0 & 7)) << 4));  // (rows 8 apart have the same swizzle)
+      for (int j = 0; j < 8; ++j)
+        from[j] = static_cast<const uint8_t*>(p.x) + (int64_t)__ldcg(p.blocks.order + start + min(r0 + j * 16, rows - 1)) * p.ldx * 2 + c * 16;
+      const uint32_t to = (uint32_t)(r0 * 128 + ((c ^ (r0 & 7)) << 4));  // (rows 16 apart have the same swizzle)
       for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
         const int s = i % t.stages;
         bool ok = true;
@@ -158,8 +159,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t bytes = k + c * 8 < p.K ? 16 : 0;  // (K is a multiple of 8; zeros beyond)
         const int64_t off = bytes ? k * 2 : 0;
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if ((scattered >> (j / 4) & 1) && r0 + j * 8 < rows) ptx::cp_async_16(base + s * stage_bytes + to + j * 1024, from[j] + off, bytes);
+        for (int j = 0; j < 8; ++j)
+          if ((scattered >> (j / 2) & 1) && r0 + j * 16 < rows) ptx::cp_async_16(base + s * stage_bytes + to + j * 2048, from[j] + off, bytes);
         ptx::cp_async_arrive(full + s * 8);
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The CTAs' sums in ascending order of K; each CTA adds up its share of the rows.
     const int row0 = rank * rows / p.splits, row1 = (rank + 1) * rows / p.splits, quads = t.nt / 4;
     const bool vec = p.N % 4 == 0;
-    for (int i = tid; i < (row1 - row0) * quads; i += kThreads) {
+    for (int i = tid; i < (row1 - row0) * quads; i += kAll) {
       const int row = row0 + i / quads, c = i % quads * 4;
       if (n0 + c >= p.N) continue;
       const uint32_t at = base + (uint32_t)(row * (t.nt + 4) + c) * 4;
@@ -280,11 +281,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int kUnits>
+template <int kUnits, bool kSorted>
 static int launch(const CUtensorMap& mx, const CUtensorMap& mw, const TileParams& t, int64_t blocks, cudaStream_t st) {
   constexpr size_t kSmem = 1024 + kRing + sizeof(Ctl);
   static_assert(kSmem <= 227 * 1024);
-  auto kern = narrow_tile_kernel<kUnits>;
+  auto kern = narrow_tile_kernel<kUnits, kSorted>;
   static thread_local bool attr_set[64] = {false};  // the opt-in is per function and per device
   int dev = 0;
   SGLB_CUDA(cudaGetDevice(&dev));
@@ -296,7 +297,7 @@ static int launch(const CUtensorMap& mx, const CUtensorMap& mw, const TileParams
   SGLB_REQUIRE(grid < (1ll << 31), "narrow product: %lld tiles are too many", (long long)grid);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid, 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.blockDim = dim3(kSorted ? kSortedThreads : kThreads, 1, 1);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -315,10 +316,13 @@ int tile_product(const Params& given, int dtype, int64_t max_blocks, cudaStream_
   t.p = given;
   Params& p = t.p;
   t.kb_total = (int)((p.K + kStageK - 1) / kStageK), t.fp16 = dtype, t.wait_probes = g_gemm_wait_probes;
-  // Up to 256 weight rows a tile, so that the activations are fetched once; fewer where there are few tiles, down to 32.
+  // Up to 256 weight rows a tile, so that the activations are fetched once (128 for sorted rows, whose warps have fewer registers); where there are
+  // so few tiles that K can be split eight ways for twice as many, half as many rows, down to 32.
   const ClusterFits& fits = cluster_fits();
-  int64_t n_tiles = (p.N + 255) / 256;
-  while (max_blocks * n_tiles * 8 <= fits.alone[1] && p.N > n_tiles * 32) n_tiles *= 2;
+  const bool sorted = p.blocks.order != nullptr;
+  const int most = sorted ? 128 : 256;
+  int64_t n_tiles = (p.N + most - 1) / most;
+  while (max_blocks * n_tiles * 2 <= fits.alone[8] && p.N > n_tiles * 32) n_tiles *= 2;
   t.nt = (int)(((p.N + n_tiles - 1) / n_tiles + 15) / 16 * 16);
   p.n_tiles = (int)((p.N + t.nt - 1) / t.nt);
   const int64_t tiles = max_blocks * p.n_tiles;
@@ -328,16 +332,17 @@ int tile_product(const Params& given, int dtype, int64_t max_blocks, cudaStream_
   t.stages = (int)std::min<uint32_t>(kMaxStages, kRing / (kXBytes + (uint32_t)t.nt * kStageK * 2));
   CUtensorMap mx, mw;
   const uint64_t xd[2] = {(uint64_t)p.K * 2, (uint64_t)p.T}, xs[1] = {(uint64_t)p.ldx * 2};
-  const uint32_t xb[2] = {kStageK * 2, p.blocks.order != nullptr ? kTileBlock / 4u : (uint32_t)kTileBlock};
+  const uint32_t xb[2] = {kStageK * 2, sorted ? kTileBlock / 4u : (uint32_t)kTileBlock};
   int rc = get_tile_map(p.x, 2, xd, xs, xb, true, &mx);
   if (rc) return rc;
   const uint64_t wd[3] = {(uint64_t)p.K * 2, (uint64_t)p.N, (uint64_t)p.adapters}, ws[2] = {(uint64_t)p.K * 2, (uint64_t)(p.N * p.K * 2)};
   const uint32_t wb[3] = {kStageK * 2, (uint32_t)t.nt, 1};
   rc = get_tile_map(p.w, 3, wd, ws, wb, true, &mw);
   if (rc) return rc;
-  if (t.nt <= 64) return launch<2>(mx, mw, t, max_blocks, st);
-  if (t.nt <= 128) return launch<4>(mx, mw, t, max_blocks, st);
-  return launch<8>(mx, mw, t, max_blocks, st);
+  if (sorted) return t.nt <= 64 ? launch<2, true>(mx, mw, t, max_blocks, st) : launch<4, true>(mx, mw, t, max_blocks, st);
+  if (t.nt <= 64) return launch<2, false>(mx, mw, t, max_blocks, st);
+  if (t.nt <= 128) return launch<4, false>(mx, mw, t, max_blocks, st);
+  return launch<8, false>(mx, mw, t, max_blocks, st);
 }
 
 int tile_status() {

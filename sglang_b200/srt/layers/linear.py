@@ -64,6 +64,21 @@ class LinearBase(nn.Module):
         self.tp_size = get_tensor_model_parallel_world_size()
         self.tp_rank = get_tensor_model_parallel_rank()
         self.prefix = prefix
+        self.lora = None  # this rank's low-rank adapters (srt/lora)
+
+    # What `srt/lora` asks a layer: this rank's columns of every merged projection and of its input, and its part of an adapter's full A
+    # [rank, inputs] and B [outputs, rank] of projection `part`.
+    def lora_output_sizes(self) -> List[int]:
+        return [self.output_size]
+
+    def lora_input_size(self) -> int:
+        return self.input_size
+
+    def lora_shard(self, part: int, a: torch.Tensor, b: torch.Tensor):
+        return a, b
+
+    def _with_lora(self, out: torch.Tensor, x) -> torch.Tensor:
+        return out if self.lora is None else self.lora.add(out, x)
 
     def _attach_loaders(self) -> None:
         for name in ("weight", "weight_scale_inv"):
@@ -98,7 +113,7 @@ class ReplicatedLinear(LinearBase):
         _copy_checked(param.data, loaded_weight, self.prefix or "ReplicatedLinear")
 
     def forward(self, x):
-        return self.quant_method.apply(self, x, self.bias), None
+        return self._with_lora(self.quant_method.apply(self, x, self.bias), x), None
 
 
 class ColumnParallelLinear(LinearBase):
@@ -158,8 +173,19 @@ class ColumnParallelLinear(LinearBase):
         self.weight.data.copy_(torch.cat(w_parts, 0))
         self.weight_scale_inv.data.copy_(torch.cat(s_parts, 0))
 
+    def lora_output_sizes(self) -> List[int]:
+        return self.output_partition_sizes
+
+    def _source_block(self, part: int) -> int:
+        """Which of `part`'s equal blocks of outputs this rank holds."""
+        return self.tp_rank
+
+    def lora_shard(self, part: int, a: torch.Tensor, b: torch.Tensor):
+        n = self.output_partition_sizes[part]
+        return a, b.narrow(0, self._source_block(part) * n, n)
+
     def forward(self, x):
-        out = self.quant_method.apply(self, x, self.bias)
+        out = self._with_lora(self.quant_method.apply(self, x, self.bias), x)
         if self.gather_output and self.tp_size > 1:
             from ..distributed import get_tp_group
             out = get_tp_group().all_gather(out, dim=-1)
@@ -190,8 +216,10 @@ class QKVParallelLinear(ColumnParallelLinear):
         if loaded_shard_id is None:
             raise NotImplementedError("QKV weights stored fused on disk are not on this path; pass \"q\", \"k\" or \"v\"")
         part = {"q": 0, "k": 1, "v": 2}[loaded_shard_id]
-        src = self.tp_rank if part == 0 else self.tp_rank // self.num_kv_head_replicas
-        self._load_part(param, loaded_weight, part, src_block=src)
+        self._load_part(param, loaded_weight, part, src_block=self._source_block(part))
+
+    def _source_block(self, part: int) -> int:
+        return self.tp_rank if part == 0 else self.tp_rank // self.num_kv_head_replicas
 
     def load_full_weight(self, weight: torch.Tensor, weight_scale_inv: torch.Tensor, block: int = 128) -> None:
         """A full [q; k; v] weight (rows of the checkpoint's three projections one after the other) and its scales."""
@@ -232,13 +260,21 @@ class RowParallelLinear(LinearBase):
         self.weight.data.copy_(weight[:, lo : lo + k])
         self.weight_scale_inv.data.copy_(weight_scale_inv[:, lo // block : (lo + k + block - 1) // block])
 
+    def lora_input_size(self) -> int:
+        return self.input_size_per_partition
+
+    def lora_shard(self, part: int, a: torch.Tensor, b: torch.Tensor):
+        k = self.input_size_per_partition
+        return a.narrow(1, self.tp_rank * k, k), b
+
     def forward(self, x):
         if not self.input_is_parallel and self.tp_size > 1:
             k = self.input_size_per_partition
             x = x[..., self.tp_rank * k : (self.tp_rank + 1) * k].contiguous()
         # bias is added by rank 0 only so that the all-reduce counts it once (linear.py:1376-1378)
         bias = self.bias if (self.tp_rank == 0 or self.tp_size == 1) else None
-        fused = get_fused_row_parallel() if (self.reduce_results and self.tp_size > 1 and self.bias is None) else None
+        fused = get_fused_row_parallel() if (self.reduce_results and self.tp_size > 1 and self.bias is None
+                                            and self.lora is None) else None
         if fused is not None and getattr(self.quant_method, "block_quant", False):
             # GEMM with the reduce-scatter in its epilogue, then one reduce-and-gather kernel over peer memory
             xq, xs = x if isinstance(x, tuple) else (None, None)
@@ -255,7 +291,8 @@ class RowParallelLinear(LinearBase):
                     xq, xs, out_dtype = xq.reshape(rows, -1), xs.reshape(rows, -1), torch.bfloat16
                 out = fused.linear(xq, xs, self.weight, self.weight_scale_inv, out_dtype)
                 return out.view(*lead, self.output_size), None
-        out = self.quant_method.apply(self, x, bias)
+        # (a rank's part of an adapter's first product is a sum over its columns: added before the ranks' sums meet)
+        out = self._with_lora(self.quant_method.apply(self, x, bias), x)
         if self.reduce_results and self.tp_size > 1:
             out = tensor_model_parallel_all_reduce(out)
         return out, None

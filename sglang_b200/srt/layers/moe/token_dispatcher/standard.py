@@ -42,7 +42,8 @@ class StandardDispatcher:
                 m[lo : lo + self.num_local_experts] = torch.arange(
                     self.num_local_experts, dtype=torch.int32, device=hidden_states.device)
                 self.local_expert_mapping = m
-            ids = self.local_expert_mapping[topk_output.topk_ids.long()]
+            named = topk_output.topk_ids  # (a negative id names no expert: it stays one)
+            ids = torch.where(named < 0, -1, self.local_expert_mapping[named.clamp_min(0).long()]).to(torch.int32)
             topk_output = StandardTopKOutput(topk_output.topk_weights, ids, topk_output.router_logits)
         return StandardDispatchOutput(hidden_states, None, topk_output)
 

@@ -33,6 +33,21 @@ def fused_topk(gating_output: torch.Tensor, topk: int, renormalize: bool = True)
     return w, ids
 
 
+def route_experts(
+    gating_output: torch.Tensor, topk: int, renormalize: bool = True, num_expert_group: int = 1, topk_group: int = 1,
+    scoring_func: str = "softmax", correction_bias: Optional[torch.Tensor] = None, routed_scaling_factor: Optional[float] = None,
+    group_top: Optional[int] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Routing in its general form (`ops.route_topk`): softmax or sigmoid scores, a bias that only selects, groups by their best or best
+    two, masked experts, decided by the real numbers whatever the logits' type."""
+    from .... import ops
+
+    _need_cuda(gating_output, "route_experts")
+    return ops.route_topk(gating_output.contiguous(), topk, scoring_func,
+                          None if correction_bias is None else correction_bias.float().contiguous(), num_expert_group, topk_group, group_top,
+                          renormalize, 1.0 if routed_scaling_factor is None else routed_scaling_factor)
+
+
 def biased_grouped_topk(
     gating_output: torch.Tensor, correction_bias: Optional[torch.Tensor], topk: int, renormalize: bool,
     num_expert_group: int, topk_group: int, routed_scaling_factor: Optional[float] = None,

@@ -1,0 +1,106 @@
+"""Low-rank adapters of many requests beside the quantised linear layers (`srt/layers/linear.py`).
+
+A program keeps one `LoRABatch` for all its layers and writes into it, once per batch, which adapter every token names.  A layer
+gets its adapters' slots from `attach_lora(layer, ...)`; from then on its `forward` adds
+
+    scaling[l] * B[l] (A[l] x)          l = the adapter that the token names, none: nothing
+
+to what it returns (`ops.lora_add`, in place, before a row-parallel layer's all-reduce).  Slots are loaded and emptied while the
+program runs; their buffers stay where they are, so that captured graphs go on working.
+"""
+from __future__ import annotations
+
+from typing import List, Optional, Sequence
+
+import torch
+from torch import nn
+
+
+class LoRABatch:
+    """The adapters that the tokens of the batch in flight name: int32, in a buffer that stays where it is."""
+
+    def __init__(self, max_tokens: int, device=None):
+        self.buffer = torch.full((max_tokens,), -1, dtype=torch.int32, device=device)
+
+    def set(self, adapter_ids: torch.Tensor) -> None:
+        """`adapter_ids` [tokens] (any integer type; negative: no adapter); tokens behind them name none."""
+        n = adapter_ids.numel()
+        if n > self.buffer.numel():
+            raise RuntimeError(f"LoRABatch: {n} tokens, made for {self.buffer.numel()}")
+        self.buffer[:n].copy_(adapter_ids.reshape(-1))
+        self.buffer[n:].fill_(-1)
+
+    def ids(self, tokens: int) -> torch.Tensor:
+        if tokens > self.buffer.numel():
+            raise RuntimeError(f"LoRABatch: {tokens} tokens, made for {self.buffer.numel()}")
+        return self.buffer[:tokens]
+
+
+class LoRASlots(nn.Module):
+    """This rank's part of the adapters of one layer: `num_slots` of rank up to `max_rank`."""
+
+    def __init__(self, layer, batch: LoRABatch, num_slots: int, max_rank: int, dtype: torch.dtype, device=None):
+        super().__init__()
+        if max_rank % 8 or not 8 <= max_rank <= 256:
+            raise RuntimeError(f"max_rank is {max_rank}, not a multiple of 8 up to 256")
+        self.batch, self.max_rank, self.num_slots = batch, max_rank, num_slots
+        self.slices = tuple(layer.lora_output_sizes())
+        n, parts = sum(self.slices), len(self.slices)
+        self.register_buffer("lora_a", torch.zeros(num_slots, parts * max_rank, layer.lora_input_size(), dtype=dtype, device=device))
+        self.register_buffer("lora_b", torch.zeros(num_slots, n, max_rank, dtype=dtype, device=device))
+        self.register_buffer("scalings", torch.zeros(num_slots, dtype=torch.float32, device=device))
+        self.register_buffer("ranks", torch.zeros(num_slots, dtype=torch.int32, device=device))
+
+    def add(self, out: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+        """out += the adapters' part of x, in place."""
+        from ... import ops
+
+        if not isinstance(x, torch.Tensor):
+            raise RuntimeError("a layer with adapters takes 16-bit activations, not codes and scales")
+        ids = self.batch.ids(x.numel() // x.shape[-1]).view(x.shape[:-1])
+        return ops.lora_add(out, x, self.lora_a, self.lora_b, ids, self.scalings, self.ranks, self.slices, out=out)
+
+
+def attach_lora(layer, batch: LoRABatch, num_slots: int, max_rank: int, dtype: torch.dtype = torch.bfloat16) -> LoRASlots:
+    """Gives a linear layer `num_slots` empty slots for adapters of rank up to `max_rank`."""
+    layer.lora = LoRASlots(layer, batch, num_slots, max_rank, dtype, layer.weight.device)
+    return layer.lora
+
+
+def load_adapter(layer, slot: int, a_parts: Sequence[Optional[torch.Tensor]], b_parts: Sequence[Optional[torch.Tensor]],
+                 scaling: float) -> None:
+    """An adapter's FULL matrices into `slot` of a layer, of which this rank keeps its part: per merged projection A [rank, inputs] and
+    B [its outputs, rank], or None for a projection that the adapter leaves alone."""
+    s = layer.lora
+    if not 0 <= slot < s.num_slots:
+        raise RuntimeError(f"slot {slot} of {s.num_slots}")
+    if len(a_parts) != len(s.slices) or len(b_parts) != len(s.slices):
+        raise RuntimeError(f"{len(a_parts)} and {len(b_parts)} matrices for {len(s.slices)} merged projections")
+    ranks = {a.shape[0] for a in a_parts if a is not None} | {b.shape[1] for b in b_parts if b is not None}
+    if len(ranks) != 1 or not 0 < max(ranks) <= s.max_rank:
+        raise RuntimeError(f"ranks {sorted(ranks)}: one rank of at most {s.max_rank} for all of a layer's projections")
+    rank, R, row = ranks.pop(), s.max_rank, 0
+    a_new, b_new = torch.zeros_like(s.lora_a[slot]), torch.zeros_like(s.lora_b[slot])
+    for part, (a, b, width) in enumerate(zip(a_parts, b_parts, s.slices)):
+        if (a is None) != (b is None):
+            raise RuntimeError(f"projection {part} has one matrix of two")
+        if a is not None:
+            a, b = layer.lora_shard(part, a, b)
+            want = (rank, s.lora_a.shape[2]), (width, rank)
+            if tuple(a.shape) != want[0] or tuple(b.shape) != want[1]:
+                raise RuntimeError(f"projection {part}: A {tuple(a.shape)} and B {tuple(b.shape)}, expected {want[0]} and {want[1]}")
+            a_new[part * R : part * R + rank].copy_(a)
+            b_new[row : row + width, :rank].copy_(b)
+        row += width
+    s.lora_a[slot].copy_(a_new)
+    s.lora_b[slot].copy_(b_new)
+    s.scalings[slot] = scaling
+    s.ranks[slot] = rank
+
+
+def unload_adapter(layer, slot: int) -> None:
+    """Empties a slot: tokens that name it get nothing added."""
+    layer.lora.ranks[slot] = 0
+
+
+__all__: List[str] = ["LoRABatch", "LoRASlots", "attach_lora", "load_adapter", "unload_adapter"]

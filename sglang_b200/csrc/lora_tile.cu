@@ -346,7 +346,14 @@ __global__ void __launch_bounds__(kThreads, 1) expand_tile_kernel(const Params p
   }
   ptx::tc_fence_before();
   __syncthreads();
-  if (ctl.abort_flag != 0 && tid == 0) atomicExch(&g_lora_tile_status, 1);
+  if (ctl.abort_flag != 0 && tid == 0) {
+    atomicExch(&g_lora_tile_status, 1);
+    // give products that may still be in flight time to end before tensor and shared memory are released
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000ll) {
+    }
+  }
+  __syncthreads();
   if (warp == kAdders + 1) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem, 2 * kCols);

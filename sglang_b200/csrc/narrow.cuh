@@ -71,8 +71,8 @@ struct Params {
   int n_tiles, splits;
 };
 
-// Rows of a block for T rows and N weight rows of each of `adapters` adapters.
-int block_rows(int64_t T, int64_t N, int64_t K, int64_t adapters);
+// Rows of a block for T rows and N weight rows, of adapters or of one router.
+int block_rows(int64_t T, int64_t N, bool adapters);
 
 // y = x w^T in blocks of p.block rows, `max_blocks` the most blocks there can be.
 int product(Params p, int dtype, int64_t max_blocks, cudaStream_t st);

@@ -46,7 +46,7 @@ def test_whole_numbers_are_exact(T, E, K, dtype):
     assert torch.equal(got.double(), x.double() @ w.double().t())
 
 
-@pytest.mark.parametrize("T", [3, 70, 700])
+@pytest.mark.parametrize("T", [3, 70, 700, 1300])
 def test_rows_apart_and_leading_dimensions(T):
     from sglang_b200 import ops
     g = torch.Generator(device="cuda").manual_seed(T)
@@ -63,7 +63,7 @@ def test_no_tokens():
     assert tuple(ops.router_logits(torch.zeros(0, 64, device="cuda", dtype=torch.bfloat16), torch.zeros(4, 64, device="cuda", dtype=torch.bfloat16)).shape) == (0, 4)
 
 
-@pytest.mark.parametrize("T", [4, 100, 600])
+@pytest.mark.parametrize("T", [4, 100, 600, 1500])
 def test_infinities_and_nan_stay_in_their_rows(T):
     from sglang_b200 import ops
     g = torch.Generator(device="cuda").manual_seed(T)

@@ -23,7 +23,7 @@ constexpr int kPlanThreads = 1024;
 // One CTA.  The tokens of an adapter stay in their order, so that those of a long request lie one after the other.  Warp w takes the w-th part
 // of the tokens and counts them by adapter in a row of its own; neighbours mostly name the same adapter, so that it counts equal ids at once.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __restrict__ ids, int T, int L, int block, int32_t* order,
-                                                            int32_t* start, int32_t* rows, int32_t* adapter, int32_t* count) {
+                                                            int4* blocks, int most, int32_t* count) {
   extern __shared__ int32_t counts[];  // [32 warps][L + 1], [L + 1] tokens and [L + 1] blocks before an adapter's
   const int tid = threadIdx.x, lane = tid & 31, warp = ptx::warp_index(), keys = L + 1;
   int32_t *mine = counts + warp * keys, *tokens_before = counts + 32 * keys, *blocks_before = tokens_before + keys;
@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __res
   }
   __syncthreads();
   if (warp == 0) {
-    int tokens = 0, blocks = 0;
+    int tokens = 0, before = 0;
     for (int at = 0; at < keys; at += 32) {
       const int l = at + lane, n = l < keys ? tokens_before[l] : 0, b = (n + block - 1) / block;
       int sn = n, sb = b;
@@ -63,19 +63,17 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __res
         const int un = __shfl_up_sync(0xffffffffu, sn, off), ub = __shfl_up_sync(0xffffffffu, sb, off);
         if (lane >= off) sn += un, sb += ub;
       }
-      if (l < keys) tokens_before[l] = tokens + sn - n, blocks_before[l] = blocks + sb - b;
-      tokens += __shfl_sync(0xffffffffu, sn, 31), blocks += __shfl_sync(0xffffffffu, sb, 31);
+      if (l < keys) tokens_before[l] = tokens + sn - n, blocks_before[l] = before + sb - b;
+      tokens += __shfl_sync(0xffffffffu, sn, 31), before += __shfl_sync(0xffffffffu, sb, 31);
     }
-    if (lane == 0) *count = blocks;
+    for (int i = before + lane; i < most; i += 32) blocks[i] = make_int4(0, 0, -1, 0);
+    if (lane == 0) *count = before;
   }
   __syncthreads();
   for (int l = warp; l < keys; l += 32) {
     const int first = tokens_before[l], n = (l + 1 < keys ? tokens_before[l + 1] : T) - first;
     for (int i = lane; i * block < n; i += 32) {
-      const int b = blocks_before[l] + i;
-      start[b] = first + i * block;
-      rows[b] = min(block, n - i * block);
-      adapter[b] = l < L ? l : -1;
+      blocks[blocks_before[l] + i] = make_int4(first + i * block, min(block, n - i * block), l < L ? l : -1, 0);
     }
   }
   for (int t = begin; t < end; t += 32) {
@@ -153,9 +151,9 @@ __global__ void __launch_bounds__(kWarps * 32, kPairs == 1 ? 3 : 2) expand_kerne
       narrow::scan_block(p.blocks, which, p.sub, lane, token, n, a);
       if (lane == 0) found[1] = n, found[2] = a;
     } else {
-      const int start = __ldcg(p.blocks.start + which), n = __ldcg(p.blocks.rows + which);
-      if (tid < n) token[tid] = __ldcg(p.blocks.order + start + tid);
-      if (tid == 0) found[1] = n, found[2] = __ldcg(p.blocks.adapter + which);
+      const int4 at = __ldcg(p.blocks.at + which);
+      if (tid < at.y) token[tid] = __ldcg(p.blocks.order + at.x + tid);
+      if (tid == 0) found[1] = at.y, found[2] = at.z;
     }
   };
   if (!scan) {
@@ -420,7 +418,7 @@ extern "C" int64_t sglb200_lora_add_workspace_bytes(int64_t tokens, int num_adap
   if (tokens <= 0 || num_adapters < 1 || rank < 1 || num_slices < 1) return 0;
   // (whichever blocks the call takes)
   const int64_t blocks = tokens / narrow::kSmallBlock + num_adapters + 1;
-  return lora::up(4 * tokens) + lora::up(4 * (3 * blocks + 1)) + lora::up(4 * tokens * num_slices * rank);
+  return lora::up(4 * tokens) + lora::up(16 * blocks + 4) + lora::up(4 * tokens * num_slices * rank);
 }
 
 extern "C" int sglb200_lora_add(const void* x, const void* lora_a, const void* lora_b, const void* base, void* out, int dtype,
@@ -442,17 +440,17 @@ extern "C" int sglb200_lora_add(const void* x, const void* lora_a, const void* l
                (long long)tokens, (long long)N, (long long)K);
   SGLB_REQUIRE(slice_sizes != nullptr, "lora_add: null slice_sizes");
   lora::Params p{};
-  int64_t at = 0;
+  int64_t columns = 0;
   bool even = true;
   for (int s = 0; s < num_slices; ++s) {
     SGLB_REQUIRE(slice_sizes[s] >= 1, "lora_add: slice %d has %lld columns", s, (long long)slice_sizes[s]);
-    p.col0[s] = at;
-    even = even && at % 8 == 0;
-    at += slice_sizes[s];
-    SGLB_REQUIRE(at <= N, "lora_add: the slices have more than %lld columns", (long long)N);
+    p.col0[s] = columns;
+    even = even && columns % 8 == 0;
+    columns += slice_sizes[s];
+    SGLB_REQUIRE(columns <= N, "lora_add: the slices have more than %lld columns", (long long)N);
   }
-  p.col0[num_slices] = at;
-  SGLB_REQUIRE(at == N, "lora_add: the slices have %lld columns of %lld", (long long)at, (long long)N);
+  p.col0[num_slices] = columns;
+  SGLB_REQUIRE(columns == N, "lora_add: the slices have %lld columns of %lld", (long long)columns, (long long)N);
   if (tokens == 0) return SGLB200_OK;
   SGLB_REQUIRE(x && lora_a && lora_b && base && out && adapter_ids, "lora_add: null pointer");
   SGLB_REQUIRE(aligned16(x) && aligned16(lora_a) && aligned16(lora_b), "lora_add: x, lora_a and lora_b must be 16-byte aligned");
@@ -465,12 +463,13 @@ extern "C" int sglb200_lora_add(const void* x, const void* lora_a, const void* l
   const int64_t blocks = lora::most_blocks(tokens, num_adapters, block);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int32_t* order = static_cast<int32_t*>(workspace);
-  int32_t* start = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + lora::up(4 * tokens));
-  float* h = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(start) + lora::up(4 * (3 * blocks + 1)));
+  int4* at = reinterpret_cast<int4*>(static_cast<uint8_t*>(workspace) + lora::up(4 * tokens));
+  int32_t* count = reinterpret_cast<int32_t*>(at + blocks);
+  float* h = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(at) + lora::up(16 * blocks + 4));
   if (scan) {
     p.blocks.ids = adapter_ids, p.blocks.ids_rows = (int)tokens, p.blocks.adapters = num_adapters;
   } else {
-    p.blocks = {order, start, start + blocks, start + 2 * blocks, start + 3 * blocks, nullptr, 0, 0};
+    p.blocks = {order, at, count, nullptr, 0, 0};
     const size_t smem = (size_t)34 * (num_adapters + 1) * sizeof(int32_t);
     if (smem > 48 * 1024) {
       static thread_local bool attr_set[64] = {false};  // the opt-in is per function and per device
@@ -483,7 +482,7 @@ extern "C" int sglb200_lora_add(const void* x, const void* lora_a, const void* l
       }
     }
     SGLB_CUDA(launch_pdl(lora::plan_kernel, 1u, (unsigned)lora::kPlanThreads, smem, st, adapter_ids, (int)tokens, num_adapters, block, order,
-                         start, start + blocks, start + 2 * blocks, start + 3 * blocks));
+                         at, (int)blocks, count));
   }
   narrow::Params n{};
   n.x = x, n.w = lora_a, n.y = h, n.ranks = ranks, n.blocks = p.blocks;

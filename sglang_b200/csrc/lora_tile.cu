@@ -57,9 +57,8 @@ __device__ __forceinline__ Run run_at(const Params& p, int at, int end) {
   r.slice = s;
   r.column = (int)p.col0[s] + (tile - p.chunk0[s]) * kCols, r.end = (int)p.col0[s + 1];
   r.count = min(p.chunk0[s + 1] - tile, end - at);
-  r.adapter = __ldcg(p.blocks.adapter + block);
-  r.rows = __ldcg(p.blocks.rows + block);
-  r.start = __ldcg(p.blocks.start + block);
+  const int4 of = __ldcg(p.blocks.at + block);
+  r.start = of.x, r.rows = of.y, r.adapter = of.z;
   r.used = r.adapter < 0 ? 0 : p.ranks != nullptr ? min(max(__ldg(p.ranks + r.adapter), 0), p.R) : p.R;
   r.multiply = r.used > 0;
   return r;

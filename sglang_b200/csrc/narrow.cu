@@ -88,8 +88,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3) narrow_kernel(const Params p) 
     rows = found[0], adapter = found[1];
     if (rows == 0 || adapter < 0) return;  // (uniform over the cluster)
   } else if (p.blocks.order != nullptr) {
-    if (block >= *p.blocks.count) return;
-    start = p.blocks.start[block], rows = p.blocks.rows[block], adapter = p.blocks.adapter[block];
+    const int4 at = __ldcg(p.blocks.at + block);
+    start = at.x, rows = at.y, adapter = at.z;
     if (adapter < 0) return;
     if (tid < rows) row[tid] = p.blocks.order[start + tid];
     __syncthreads();

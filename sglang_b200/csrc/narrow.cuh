@@ -9,14 +9,12 @@ namespace narrow {
 constexpr int kSmallBlock = 32, kTileBlock = 128;
 
 // The blocks that the rows of a batch are sorted into by adapter.  Either a plan: `order` the rows, then per block where it starts in the
-// order, its rows and its adapter (-1: rows that name none), `count` the number of blocks.  Or, for up to kScanRows rows, which one warp
+// order, its rows and its adapter (-1: rows that name none), and for as many as there could be beyond the `count` that there are, 0 rows.  Or, for up to kScanRows rows, which one warp
 // looks through faster than a launch of its own takes: `ids`, from which every CTA finds its block.
 constexpr int kScanRows = 64;
 struct Blocks {
   const int32_t* order;  // neither order nor ids: the rows as they lie, all of one adapter
-  const int32_t* start;
-  const int32_t* rows;
-  const int32_t* adapter;
+  const int4* at;        // {start, rows, adapter, 0}
   const int32_t* count;
   const int32_t* ids;
   int ids_rows, adapters;

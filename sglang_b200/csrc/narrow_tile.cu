@@ -5,9 +5,6 @@
 // four warps (two took 0.65 us a stage of 128 rows, TMA gathers of four rows 2 us).  K is split over the CTAs of a cluster, which add their
 // sums through distributed shared memory in a fixed order.
 //
-// Many rows of one router: pairs of CTAs multiply 256 activation rows by the weight rows together, each fetching half of the weights, which is
-// what bounds it (some 60 bytes a clock arrive at an SM).
-//
 // The instruction cuts off what does not fit its sum, each time: over 7168 columns that would be off by more than a float32 product is.  So
 // the sums of 256 columns begin from zero, in two buffers of tensor memory in turn, and meet in the registers of eight warps.
 #include <algorithm>
@@ -26,11 +23,7 @@ constexpr int kStageK = 64;        // columns of a stage: 128 bytes, one swizzle
 constexpr int kChunk = 4;          // stages that are summed up in tensor memory
 constexpr int kMaxStages = 8;
 constexpr uint32_t kRing = 192 * 1024;
-#ifndef NARROW_PAIR_FROM
-#define NARROW_PAIR_FROM 16
-#endif
 constexpr uint32_t kXBytes = kTileBlock * kStageK * 2;
-enum class Form { kPlain, kSorted, kPair };
 
 struct Ctl {
   uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
@@ -51,46 +44,89 @@ constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);  // rows of
 __device__ __forceinline__ uint32_t desc_lo(uint32_t smem) { return ((smem & 0x3ffffu) >> 4) | (1u << 16); }
 
 // f32 += bf16 x bf16 (1) or f16 x f16 (0), both operands K-major.
-__device__ __forceinline__ uint32_t idesc(int m, int n, int fp16) {
+__device__ __forceinline__ uint32_t idesc(int n, int fp16) {
   const uint32_t type = fp16 ? 0u : 1u;
-  return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+  return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTileBlock >> 4) << 24);
 }
-template <bool kPair>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
-#define NARROW_MMA(CG)                                                                                                          \
-  asm volatile("{\n\t.reg .pred p;\n\t"                                                                                        \
-               "setp.ne.b32 p, %4, 0;\n\t"                                                                                     \
-               "tcgen05.mma.cta_group::" CG ".kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate) \
-               : "memory")
-  if constexpr (kPair) NARROW_MMA("2"); else NARROW_MMA("1");
-#undef NARROW_MMA
+  asm volatile("{\n\t.reg .pred p;\n\t"
+               "setp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate)
+               : "memory");
 }
 
 #define NARROW_WAIT(bar, parity) \
   (t.wait_probes != ptx::kProbesNone && (ptx::mbar_test(bar, parity) || ptx::mbar_wait_quiet(bar, parity)))
 
+// The sums of a tile out of the (up to kMost) CTAs' shared memory, in ascending order of K; each CTA adds up its share of the rows.  A thread
+// has four columns of every `step`-th row and asks for kAtOnce rows' parts at a time.
+template <int kMost, int kAtOnce, int kAll, bool kSorted>
+__device__ __forceinline__ void store_sums(const TileParams& t, uint32_t base, int rows, int rank, int n0, int64_t start, const int* row_of) {
+  const Params& p = t.p;
+  const int row0 = rank * rows / p.splits, row1 = (rank + 1) * rows / p.splits, quads = t.nt / 4, step = kAll / quads;
+  const int tid = threadIdx.x, c = tid % quads * 4;
+  const bool vec = p.N % 4 == 0;
+  if (n0 + c >= p.N || tid >= step * quads) return;
+  for (int row = row0 + tid / quads; row < row1; row += kAtOnce * step) {
+    float4 v[kAtOnce][kMost];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      if (row + u * step >= row1) break;
+      const uint32_t at = base + (uint32_t)((row + u * step) * (t.nt + 4) + c) * 4;
+      if constexpr (kMost == 1) {
+        v[u][0] = ptx::lds_f32x4(at);
+      } else {
+#pragma unroll
+        for (int s = 0; s < kMost; ++s)
+          if (s < p.splits)
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v[u][s].x), "=f"(v[u][s].y), "=f"(v[u][s].z), "=f"(v[u][s].w)
+                         : "r"(ptx::cluster_map(at, s))
+                         : "memory");
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int mine = row + u * step;
+      if (mine >= row1) break;
+      float4 sum = v[u][0];
+#pragma unroll
+      for (int s = 1; s < kMost; ++s)
+        if (s < p.splits) sum.x += v[u][s].x, sum.y += v[u][s].y, sum.z += v[u][s].z, sum.w += v[u][s].w;
+      float* to = p.y + (kSorted ? (int64_t)row_of[mine] : start + mine) * p.N + n0 + c;
+      if (vec) {
+        *reinterpret_cast<float4*>(to) = sum;
+      } else {
+        const float one[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n0 + c + j < p.N) to[j] = one[j];
+      }
+    }
+  }
+}
+
 // kUnits: groups of 16 columns of a tile that each of the two warpgroups adds up, at most.
-template <int kUnits, Form kForm>
-__global__ void __launch_bounds__(kForm == Form::kSorted ? kSortedThreads : kThreads, 1)
+template <int kUnits, bool kSorted>
+__global__ void __launch_bounds__(kSorted ? kSortedThreads : kThreads, 1)
     narrow_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const TileParams t) {
   constexpr uint32_t kBuf = kUnits * 32;  // columns of tensor memory of a buffer
-  constexpr bool sorted = kForm == Form::kSorted, kPair = kForm == Form::kPair;
-  constexpr int kAll = sorted ? kSortedThreads : kThreads, kCopies = 4 * 32, kCtas = kPair ? 2 : 1;
+  constexpr bool sorted = kSorted;
+  constexpr int kAll = kSorted ? kSortedThreads : kThreads, kCopies = 4 * 32;
   const Params& p = t.p;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Ctl* ctl = reinterpret_cast<Ctl*>(ring + kRing);
   const int tid = threadIdx.x, warp = ptx::warp_index(), lane = tid & 31;
   volatile int* abort_flag = &ctl->abort_flag;
-  const int in_cluster = (int)(blockIdx.x % (p.splits * kCtas)), rank = in_cluster / kCtas, odd = in_cluster % kCtas;
-  const int n0 = (int)(blockIdx.x / (p.splits * kCtas) % p.n_tiles) * t.nt;
-  const int64_t block = (int64_t)(blockIdx.x / (p.splits * kCtas) / p.n_tiles) * kCtas + odd;
+  const int rank = (int)(blockIdx.x % p.splits), n0 = (int)(blockIdx.x / p.splits % p.n_tiles) * t.nt;
+  const int64_t block = blockIdx.x / p.splits / p.n_tiles;
   const uint32_t full = ptx::smem_u32(ctl->full), empty = ptx::smem_u32(ctl->empty), acc_full = ptx::smem_u32(ctl->acc_full),
                  acc_empty = ptx::smem_u32(ctl->acc_empty);
   // (tensor memory is taken once the kernel in front has ended; the kernel behind may start when every CTA has its own)
   ptx::grid_dependency_wait();
   int64_t start = block * kTileBlock;
-  int rows = (int)max((int64_t)0, min((int64_t)kTileBlock, p.T - start)), adapter = 0;
+  int rows = (int)min((int64_t)kTileBlock, p.T - start), adapter = 0;
   if (sorted) {
     const int4 at = __ldcg(p.blocks.at + block);
     start = at.x, rows = at.y, adapter = at.z;
@@ -106,12 +142,8 @@ __global__ void __launch_bounds__(kForm == Form::kSorted ? kSortedThreads : kThr
     }
   }
   if (warp == 9) {
-    if constexpr (kPair) {
-      ptx::pair_tmem_alloc(ptx::smem_u32(&ctl->tmem_base), 2 * kBuf);
-    } else {
-      ptx::tmem_alloc(ptx::smem_u32(&ctl->tmem_base), 2 * kBuf);
-      ptx::tmem_relinquish();
-    }
+    ptx::tmem_alloc(ptx::smem_u32(&ctl->tmem_base), 2 * kBuf);
+    ptx::tmem_relinquish();
   }
   if (sorted) __syncthreads();
   // 32 rows that have to be copied one by one, a bit each; the number of 32 that hold rows
@@ -121,17 +153,17 @@ __global__ void __launch_bounds__(kForm == Form::kSorted ? kSortedThreads : kThr
     for (int i = 0; i < groups; ++i) scattered |= ctl->first[i] < 0 ? 1 << i : 0;
   if (tid == 0) {
     for (int s = 0; s < t.stages; ++s) ptx::mbar_init(full + s * 8, scattered ? kCopies + 1 : 1), ptx::mbar_init(empty + s * 8, 1);
-    for (int b = 0; b < 2; ++b) ptx::mbar_init(acc_full + b * 8, 1), ptx::mbar_init(acc_empty + b * 8, 8 * kCtas);
+    for (int b = 0; b < 2; ++b) ptx::mbar_init(acc_full + b * 8, 1), ptx::mbar_init(acc_empty + b * 8, 8);
     ctl->abort_flag = 0;
     ptx::mbar_fence_init();
   }
   ptx::tc_fence_before();
-  if constexpr (kPair) ptx::cluster_sync(); else __syncthreads();
+  __syncthreads();
   ptx::tc_fence_after();
   ptx::launch_dependents();
   const uint32_t tmem = ctl->tmem_base;
   const int kb0 = (int)((int64_t)rank * t.kb_total / p.splits), kb1 = (int)((int64_t)(rank + 1) * t.kb_total / p.splits);
-  const uint32_t w_bytes = (uint32_t)(t.nt / kCtas) * kStageK * 2, stage_bytes = kXBytes + w_bytes, base = ptx::smem_u32(ring);
+  const uint32_t w_bytes = (uint32_t)t.nt * kStageK * 2, stage_bytes = kXBytes + w_bytes, base = ptx::smem_u32(ring);
   const int units = t.nt / 16, half = (units + 1) / 2;
 
   if (warp == 8) {
@@ -146,13 +178,6 @@ __global__ void __launch_bounds__(kForm == Form::kSorted ? kSortedThreads : kThr
         }
         const uint32_t at = base + s * stage_bytes, bar = full + s * 8;
         if (++s == t.stages) s = 0, ph ^= 1;
-        if constexpr (kPair) {
-          if (odd == 0) ptx::mbar_arrive_expect_tx(bar, 2 * stage_bytes);  // of both CTAs
-          const uint32_t lead = ptx::cluster_map(bar, in_cluster - odd);
-          ptx::pair_load_3d(at + kXBytes, &map_w, lead, kb * kStageK * 2, n0 + odd * (t.nt / 2), 0);
-          ptx::pair_load_2d(at, &map_x, lead, kb * kStageK * 2, (int)start);
-          continue;
-        }
         ptx::mbar_arrive_expect_tx(bar, w_bytes + (sorted ? (uint32_t)(groups - __popc(scattered)) * (kXBytes / 4) : kXBytes));
         ptx::tma_load_3d(at + kXBytes, &map_w, bar, kb * kStageK * 2, n0, adapter);
         if (!sorted) {
@@ -195,14 +220,11 @@ __global__ void __launch_bounds__(kForm == Form::kSorted ? kSortedThreads : kThr
     }
     __syncwarp();
   } else if (warp == 9) {
-    if (odd == 0 && ptx::elect_one()) {
-      const uint32_t id = idesc(kTileBlock * kCtas, t.nt, t.fp16);
+    if (ptx::elect_one()) {
+      const uint32_t id = idesc(t.nt, t.fp16);
       bool ok = true;
       int s = 0, left = kChunk;  // stages of a chunk
       uint32_t ph = 0, buf = 0, acc_ph = 1;
-      auto commit = [&](uint32_t bar) {
-        if constexpr (kPair) ptx::pair_commit(bar, in_cluster); else ptx::mma_commit(bar);
-      };
       for (int kb = kb0; kb < kb1; ++kb) {
         if (left == kChunk) ok = NARROW_WAIT(acc_empty + buf * 8, acc_ph);
         if (ok) ok = NARROW_WAIT(full + s * 8, ph);
@@ -212,12 +234,12 @@ __global__ void __launch_bounds__(kForm == Form::kSorted ? kSortedThreads : kThr
         const uint32_t at = base + s * stage_bytes, x_lo = desc_lo(at), w_lo = desc_lo(at + kXBytes);
 #pragma unroll
         for (int k = 0; k < kStageK / 16; ++k)
-          mma_f16<kPair>(tmem + buf * kBuf, ptx::pack_f32x2(x_lo + 2 * k, kDescHi), ptx::pack_f32x2(w_lo + 2 * k, kDescHi), id,
+          mma_f16(tmem + buf * kBuf, ptx::pack_f32x2(x_lo + 2 * k, kDescHi), ptx::pack_f32x2(w_lo + 2 * k, kDescHi), id,
                          left < kChunk || k > 0 ? 1u : 0u);
-        commit(empty + s * 8);
+        ptx::mma_commit(empty + s * 8);
         if (++s == t.stages) s = 0, ph ^= 1;
         if (--left == 0 || kb + 1 == kb1) {
-          commit(acc_full + buf * 8);
+          ptx::mma_commit(acc_full + buf * 8);
           left = kChunk, acc_ph ^= buf, buf ^= 1;
         }
       }
@@ -249,10 +271,7 @@ __global__ void __launch_bounds__(kForm == Form::kSorted ? kSortedThreads : kThr
       }
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        if constexpr (kPair) ptx::cluster_arrive_bar(ptx::cluster_map(acc_empty + (c & 1) * 8, in_cluster - odd));
-        else ptx::mbar_arrive(acc_empty + (c & 1) * 8);
-      }
+      if (lane == 0) ptx::mbar_arrive(acc_empty + (c & 1) * 8);
     }
     if (!ok) {
       *abort_flag = 1;
@@ -268,55 +287,14 @@ __global__ void __launch_bounds__(kForm == Form::kSorted ? kSortedThreads : kThr
     }
   }
   __syncwarp();
-  if (p.splits > 1 || kPair) ptx::cluster_sync(); else __syncthreads();
+  if (p.splits > 1) ptx::cluster_sync(); else __syncthreads();
   if (ctl->abort_flag == 0) {
-    // The CTAs' sums in ascending order of K; each CTA adds up its share of the rows.  A thread has four columns of every `step`-th row and asks
-    // for two rows' parts at once.
-    const int row0 = rank * rows / p.splits, row1 = (rank + 1) * rows / p.splits, quads = t.nt / 4, step = kAll / quads;
-    const int c = tid % quads * 4, r0 = row0 + tid / quads;
-    const bool vec = p.N % 4 == 0;
-    if (n0 + c < p.N && tid < step * quads) {
-      constexpr int kRowsAtOnce = 2;
-      for (int row = r0; row < row1; row += kRowsAtOnce * step) {
-        float4 v[kRowsAtOnce][8];
-#pragma unroll
-        for (int u = 0; u < kRowsAtOnce; ++u) {
-          if (row + u * step >= row1) break;
-          const uint32_t at = base + (uint32_t)((row + u * step) * (t.nt + 4) + c) * 4;
-          if (p.splits == 1) {
-            v[u][0] = ptx::lds_f32x4(at);
-            continue;
-          }
-#pragma unroll
-          for (int s = 0; s < 8; ++s)
-            if (s < p.splits)
-              asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                           : "=f"(v[u][s].x), "=f"(v[u][s].y), "=f"(v[u][s].z), "=f"(v[u][s].w)
-                           : "r"(ptx::cluster_map(at, s * kCtas + odd))
-                           : "memory");
-        }
-#pragma unroll
-        for (int u = 0; u < kRowsAtOnce; ++u) {
-          const int mine = row + u * step;
-          if (mine >= row1) break;
-          float4 sum = v[u][0];
-#pragma unroll
-          for (int s = 1; s < 8; ++s)
-            if (s < p.splits) sum.x += v[u][s].x, sum.y += v[u][s].y, sum.z += v[u][s].z, sum.w += v[u][s].w;
-          float* to = p.y + (sorted ? (int64_t)ctl->row[mine] : start + mine) * p.N + n0 + c;
-          if (vec) {
-            *reinterpret_cast<float4*>(to) = sum;
-          } else {
-            const float one[4] = {sum.x, sum.y, sum.z, sum.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (n0 + c + j < p.N) to[j] = one[j];
-          }
-        }
-      }
-    }
+    if (p.splits == 1) store_sums<1, 4, kAll, kSorted>(t, base, rows, rank, n0, start, ctl->row);
+    else if (p.splits == 2) store_sums<2, 4, kAll, kSorted>(t, base, rows, rank, n0, start, ctl->row);
+    else if (p.splits <= 4) store_sums<4, 2, kAll, kSorted>(t, base, rows, rank, n0, start, ctl->row);
+    else store_sums<8, 2, kAll, kSorted>(t, base, rows, rank, n0, start, ctl->row);
   }
-  if (p.splits > 1 || kPair) ptx::cluster_sync();  // no CTA leaves while another reads its shared memory
+  if (p.splits > 1) ptx::cluster_sync_relaxed();  // no CTA leaves while another reads its shared memory
   ptx::tc_fence_before();
   __syncthreads();
   if (ctl->abort_flag != 0 && tid == 0) {
@@ -329,15 +307,15 @@ __global__ void __launch_bounds__(kForm == Form::kSorted ? kSortedThreads : kThr
   __syncthreads();
   if (warp == 9) {
     ptx::tc_fence_after();
-    if constexpr (kPair) ptx::pair_tmem_dealloc(tmem, 2 * kBuf); else ptx::tmem_dealloc(tmem, 2 * kBuf);
+    ptx::tmem_dealloc(tmem, 2 * kBuf);
   }
 }
 
-template <int kUnits, Form kForm>
+template <int kUnits, bool kSorted>
 static int launch(const CUtensorMap& mx, const CUtensorMap& mw, const TileParams& t, int64_t blocks, cudaStream_t st) {
   constexpr size_t kSmem = 1024 + kRing + sizeof(Ctl);
   static_assert(kSmem <= 227 * 1024);
-  auto kern = narrow_tile_kernel<kUnits, kForm>;
+  auto kern = narrow_tile_kernel<kUnits, kSorted>;
   static thread_local bool attr_set[64] = {false};  // the opt-in is per function and per device
   int dev = 0;
   SGLB_CUDA(cudaGetDevice(&dev));
@@ -345,19 +323,18 @@ static int launch(const CUtensorMap& mx, const CUtensorMap& mw, const TileParams
     SGLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  const unsigned cluster = (unsigned)t.p.splits * (kForm == Form::kPair ? 2 : 1);
-  const int64_t grid = blocks * t.p.n_tiles * cluster;
+  const int64_t grid = blocks * t.p.n_tiles * t.p.splits;
   SGLB_REQUIRE(grid < (1ll << 31), "narrow product: %lld tiles are too many", (long long)grid);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid, 1, 1);
-  cfg.blockDim = dim3(kForm == Form::kSorted ? kSortedThreads : kThreads, 1, 1);
+  cfg.blockDim = dim3(kSorted ? kSortedThreads : kThreads, 1, 1);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = cluster, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  attr[1].val.clusterDim.x = (unsigned)t.p.splits, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   SGLB_CUDA(cudaLaunchKernelEx(&cfg, kern, mx, mw, t));
@@ -377,29 +354,25 @@ int tile_product(const Params& given, int dtype, int64_t max_blocks, cudaStream_
   int64_t n_tiles = (p.N + most - 1) / most;
   while (max_blocks * n_tiles * 2 <= fits.alone[8] && p.N > n_tiles * 32) n_tiles *= 2;
   t.nt = (int)(((p.N + n_tiles - 1) / n_tiles + 15) / 16 * 16);
-  const bool pair = !sorted && t.nt > 128 && max_blocks >= NARROW_PAIR_FROM;
-  if (pair) t.nt = (t.nt + 31) / 32 * 32;  // (halves that are whole swizzle patterns, and M = 256 wants N in sixteens)
   p.n_tiles = (int)((p.N + t.nt - 1) / t.nt);
-  const int ctas = pair ? 2 : 1;
-  const int64_t blocks = (max_blocks + ctas - 1) / ctas, tiles = blocks * p.n_tiles;
+  const int64_t tiles = max_blocks * p.n_tiles;
   p.splits = 1;
-  for (int s = 2; s <= 8 / ctas; ++s)  // as many CTAs as run at once
-    if (tiles <= fits.alone[s * ctas] && t.kb_total >= s * kChunk) p.splits = s;
-  t.stages = (int)std::min<uint32_t>(kMaxStages, kRing / (kXBytes + (uint32_t)(t.nt / ctas) * kStageK * 2));
+  for (int s = 2; s <= 8; ++s)  // as many CTAs as run at once
+    if (tiles <= fits.alone[s] && t.kb_total >= s * kChunk) p.splits = s;
+  t.stages = (int)std::min<uint32_t>(kMaxStages, kRing / (kXBytes + (uint32_t)t.nt * kStageK * 2));
   CUtensorMap mx, mw;
   const uint64_t xd[2] = {(uint64_t)p.K * 2, (uint64_t)p.T}, xs[1] = {(uint64_t)p.ldx * 2};
   const uint32_t xb[2] = {kStageK * 2, sorted ? kTileBlock / 4u : (uint32_t)kTileBlock};
   int rc = get_tile_map(p.x, 2, xd, xs, xb, true, &mx);
   if (rc) return rc;
   const uint64_t wd[3] = {(uint64_t)p.K * 2, (uint64_t)p.N, (uint64_t)p.adapters}, ws[2] = {(uint64_t)p.K * 2, (uint64_t)(p.N * p.K * 2)};
-  const uint32_t wb[3] = {kStageK * 2, (uint32_t)(t.nt / ctas), 1};
+  const uint32_t wb[3] = {kStageK * 2, (uint32_t)t.nt, 1};
   rc = get_tile_map(p.w, 3, wd, ws, wb, true, &mw);
   if (rc) return rc;
-  if (pair) return launch<8, Form::kPair>(mx, mw, t, blocks, st);
-  if (sorted) return t.nt <= 64 ? launch<2, Form::kSorted>(mx, mw, t, blocks, st) : launch<4, Form::kSorted>(mx, mw, t, blocks, st);
-  if (t.nt <= 64) return launch<2, Form::kPlain>(mx, mw, t, blocks, st);
-  if (t.nt <= 128) return launch<4, Form::kPlain>(mx, mw, t, blocks, st);
-  return launch<8, Form::kPlain>(mx, mw, t, blocks, st);
+  if (sorted) return t.nt <= 64 ? launch<2, true>(mx, mw, t, max_blocks, st) : launch<4, true>(mx, mw, t, max_blocks, st);
+  if (t.nt <= 64) return launch<2, false>(mx, mw, t, max_blocks, st);
+  if (t.nt <= 128) return launch<4, false>(mx, mw, t, max_blocks, st);
+  return launch<8, false>(mx, mw, t, max_blocks, st);
 }
 
 int tile_status() {

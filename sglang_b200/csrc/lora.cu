@@ -22,7 +22,8 @@ constexpr int kPlanThreads = 1024;
 
 // One CTA.  The tokens of an adapter stay in their order, so that those of a long request lie one after the other.  Warp w takes the w-th part
 // of the tokens and counts them by adapter in a row of its own; neighbours mostly name the same adapter, so that it counts equal ids at once.
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __restrict__ ids, int T, int L, int block, int32_t* order,
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __restrict__ ids, const int32_t* __restrict__ ranks, int R, int T,
+                                                            int L, int block, int32_t* order,
                                                             int4* blocks, int most, int32_t* count) {
   extern __shared__ int32_t counts[];  // [32 warps][L + 1], [L + 1] tokens and [L + 1] blocks before an adapter's
   const int tid = threadIdx.x, lane = tid & 31, warp = ptx::warp_index(), keys = L + 1;
@@ -71,9 +72,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __res
   }
   __syncthreads();
   for (int l = warp; l < keys; l += 32) {
+    const int used = l == L ? 0 : ranks != nullptr ? min(max(ranks[l], 0), R) : R;
     const int first = tokens_before[l], n = (l + 1 < keys ? tokens_before[l + 1] : T) - first;
     for (int i = lane; i * block < n; i += 32) {
-      blocks[blocks_before[l] + i] = make_int4(first + i * block, min(block, n - i * block), l < L ? l : -1, 0);
+      blocks[blocks_before[l] + i] = make_int4(first + i * block, min(block, n - i * block), l < L ? l : -1, used);
     }
   }
   for (int t = begin; t < end; t += 32) {
@@ -127,7 +129,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPairs == 1 ? 3 : 2) expand_kerne
   uint8_t* terms = ring + Cfg::kRing;              // a token's high terms, then its low terms, 32 kPairs each
   __shared__ float unscale[narrow::kTileBlock];
   __shared__ int32_t token[narrow::kTileBlock];
-  __shared__ int found[3];
+  __shared__ int found[4];
   const int tid = threadIdx.x, lane = tid & 31, warp = ptx::warp_index(), g = lane >> 2, q = lane & 3;
   const bool scan = p.blocks.ids != nullptr;
   const int per = p.chunk0[p.S];  // units of a block
@@ -149,11 +151,11 @@ __global__ void __launch_bounds__(kWarps * 32, kPairs == 1 ? 3 : 2) expand_kerne
       if (warp != 0) return;
       int n = 0, a = -1;
       narrow::scan_block(p.blocks, which, p.sub, lane, token, n, a);
-      if (lane == 0) found[1] = n, found[2] = a;
+      if (lane == 0) found[1] = n, found[2] = a, found[3] = a < 0 ? 0 : p.ranks != nullptr ? min(max(__ldg(p.ranks + a), 0), p.R) : p.R;
     } else {
       const int4 at = __ldcg(p.blocks.at + which);
       if (tid < at.y) token[tid] = __ldcg(p.blocks.order + at.x + tid);
-      if (tid == 0) found[1] = at.y, found[2] = at.z;
+      if (tid == 0) found[1] = at.y, found[2] = at.z, found[3] = at.w;
     }
   };
   if (!scan) {
@@ -170,7 +172,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPairs == 1 ? 3 : 2) expand_kerne
     __syncthreads();
     cut(found[0]);
   }
-  int all_rows = 0, adapter = -1;
+  int all_rows = 0, adapter = -1, used = 0;
   for (int at = begin; at < end;) {
     const int piece = at / per, unit0 = at - piece * per, row0 = piece % p.subs * p.sub;
     int slice = 0;
@@ -184,7 +186,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPairs == 1 ? 3 : 2) expand_kerne
         __syncthreads();
       }
       block = piece / p.subs;
-      all_rows = found[1], adapter = found[2];
+      all_rows = found[1], adapter = found[2], used = found[3];
     } else {
       __syncthreads();
     }
@@ -192,7 +194,6 @@ __global__ void __launch_bounds__(kWarps * 32, kPairs == 1 ? 3 : 2) expand_kerne
     const int rows = min(all_rows - row0, p.sub), steps = units * ((rows + 15) / 16);
     const int64_t stop = p.col0[slice + 1];
     const int64_t c0 = p.col0[slice] + (int64_t)(unit0 - p.chunk0[slice]) * Cfg::kCols + warp * kCols;
-    const int used = adapter < 0 ? 0 : p.ranks != nullptr ? min(max(__ldg(p.ranks + adapter), 0), p.R) : p.R;
     const int pairs = (used + 31) / 32;
     const uint8_t* weights = static_cast<const uint8_t*>(p.b) + (adapter < 0 ? 0 : (int64_t)adapter * p.N * p.R * 2);
 
@@ -481,7 +482,7 @@ extern "C" int sglb200_lora_add(const void* x, const void* lora_a, const void* l
         if (dev >= 0 && dev < 64) attr_set[dev] = true;
       }
     }
-    SGLB_CUDA(launch_pdl(lora::plan_kernel, 1u, (unsigned)lora::kPlanThreads, smem, st, adapter_ids, (int)tokens, num_adapters, block, order,
+    SGLB_CUDA(launch_pdl(lora::plan_kernel, 1u, (unsigned)lora::kPlanThreads, smem, st, adapter_ids, ranks, rank, (int)tokens, num_adapters, block, order,
                          at, (int)blocks, count));
   }
   narrow::Params n{};

@@ -58,8 +58,7 @@ __device__ __forceinline__ Run run_at(const Params& p, int at, int end) {
   r.column = (int)p.col0[s] + (tile - p.chunk0[s]) * kCols, r.end = (int)p.col0[s + 1];
   r.count = min(p.chunk0[s + 1] - tile, end - at);
   const int4 of = __ldcg(p.blocks.at + block);
-  r.start = of.x, r.rows = of.y, r.adapter = of.z;
-  r.used = r.adapter < 0 ? 0 : p.ranks != nullptr ? min(max(__ldg(p.ranks + r.adapter), 0), p.R) : p.R;
+  r.start = of.x, r.rows = of.y, r.adapter = of.z, r.used = of.w;
   r.multiply = r.used > 0;
   return r;
 }
@@ -215,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1) expand_tile_kernel(const Params p
     const uint32_t base_pitch = (uint32_t)(p.ld_base * 2), out_pitch = (uint32_t)(p.ld_out * 2);
     const uint32_t mine = h_at + Cfg<kKB>::kBase + warp * 2048 + lane * 16;
     // The terms of h of a run, and its rows' factors to `set`.
-    auto build = [&](const Run& r, int set) {
+    auto build = [&](const Run& r, int of_rows, int set) {  // lane u of `of_rows`: the token of row warp + u * kAdders
       const int used = r.used, rows = r.rows;
       const float scaling = p.scalings != nullptr ? __ldg(p.scalings + r.adapter) : 1.f;
       const float* h = p.h + r.slice * p.R;
@@ -223,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1) expand_tile_kernel(const Params p
       float v[kRowsHere][kV];
 #pragma unroll
       for (int u = 0; u < kRowsHere; ++u) {
-        const float* from = h + (int64_t)__ldcg(p.blocks.order + r.start + min(warp + u * kAdders, rows - 1)) * p.S * p.R;
+        const float* from = h + (int64_t)__shfl_sync(0xffffffffu, of_rows, u) * p.S * p.R;
 #pragma unroll
         for (int j = 0; j < kV; ++j) v[u][j] = j * 32 + lane < used ? __ldcg(from + j * 32 + lane) : 0.f;
       }
@@ -248,22 +247,26 @@ __global__ void __launch_bounds__(kThreads, 1) expand_tile_kernel(const Params p
     // A run for a lane: its rows' tokens, its first column and where it stops (0: nothing to do).
     struct Mine {
       uint32_t token[4];
-      int rows, n, stop;
+      int rows, n, stop, of_rows;
     };
     auto open = [&](const Run& r, Mine& m) {
+      m.of_rows = __ldcg(p.blocks.order + r.start + min(warp + lane % (kRows / kAdders) * kAdders, r.rows - 1));
       m.rows = r.rows - row_mine, m.n = r.column + col_mine, m.stop = r.multiply || !p.in_place ? r.end : 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) m.token[j] = j * 8 < m.rows ? (uint32_t)__ldcg(p.blocks.order + r.start + row_mine + j * 8) : 0u;
     };
-    Mine ahead;
-    int ahead_at = begin, ahead_left = 0;
+    // The run that is asked for, and what the run behind this one is, if it has been opened already.
+    Run ahead_run{}, next_run{};
+    Mine ahead, next;
+    int ahead_at = begin, ahead_left = 0, next_at = -1;
     // Asks for the base of the next tile that has not been asked for, to place `slot`.
     auto fetch = [&](int slot) {
       if (ahead_at < end) {
         if (ahead_left == 0) {
-          const Run r = run_at(p, ahead_at, end);
-          open(r, ahead);
-          ahead_left = r.count;
+          ahead_run = run_at(p, ahead_at, end);
+          open(ahead_run, ahead);
+          ahead_left = ahead_run.count;
+          if (next_at < 0) next_at = ahead_at, next_run = ahead_run, next = ahead;
         }
         if (ahead.n < ahead.stop) {
           const uint8_t* from = static_cast<const uint8_t*>(p.base) + (int64_t)ahead.n * 2;
@@ -280,14 +283,20 @@ __global__ void __launch_bounds__(kThreads, 1) expand_tile_kernel(const Params p
     int i = 0, built = 0, slot = 0;
     bool ok = true;
     for (int at = begin; at < end;) {
-      const Run r = run_at(p, at, end);
+      Run r;
       Mine m;
-      open(r, m);
+      if (next_at == at) {
+        r = next_run, m = next;
+      } else {  // (runs shorter than what is asked for ahead)
+        r = run_at(p, at, end);
+        open(r, m);
+      }
+      next_at = -1;
       at += r.count;
       const bool multiply = r.multiply;
       float inv[4] = {};
       if (multiply) {  // (the products of the run before are done: its last sums have been waited for)
-        build(r, built & 1);
+        build(r, m.of_rows, built & 1);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (j * 8 < m.rows) inv[j] = ctl.unscale[built & 1][row_mine + j * 8];

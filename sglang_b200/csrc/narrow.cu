@@ -78,6 +78,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) narrow_kernel(const Params p) 
   int64_t start = block * kSmallBlock, adapter = 0;
   int rows = (int)min((int64_t)kSmallBlock, p.T - start);
   const bool sorted = p.blocks.order != nullptr || p.blocks.ids != nullptr;
+  int used = p.rank_rows;
   if (p.blocks.ids != nullptr) {
     if (warp == 0) {
       int n = 0, a = -1;
@@ -87,14 +88,14 @@ __global__ void __launch_bounds__(kWarps * 32, 3) narrow_kernel(const Params p) 
     __syncthreads();
     rows = found[0], adapter = found[1];
     if (rows == 0 || adapter < 0) return;  // (uniform over the cluster)
+    if (p.ranks != nullptr) used = min(max(__ldg(p.ranks + adapter), 0), p.rank_rows);
   } else if (p.blocks.order != nullptr) {
     const int4 at = __ldcg(p.blocks.at + block);
-    start = at.x, rows = at.y, adapter = at.z;
+    start = at.x, rows = at.y, adapter = at.z, used = at.w;
     if (adapter < 0) return;
     if (tid < rows) row[tid] = p.blocks.order[start + tid];
     __syncthreads();
   }
-  const int used = p.ranks != nullptr ? min(max(p.ranks[adapter], 0), p.rank_rows) : p.rank_rows;
   const T* w = static_cast<const T*>(p.w) + adapter * p.N * p.K;
   const int na = n0 + g, nb = n0 + g + 8;
   const bool a_on = na < p.N && na % p.rank_rows < used, b_on = nb < p.N && nb % p.rank_rows < used;

@@ -14,7 +14,7 @@ constexpr int kSmallBlock = 32, kTileBlock = 128;
 constexpr int kScanRows = 64;
 struct Blocks {
   const int32_t* order;  // neither order nor ids: the rows as they lie, all of one adapter
-  const int4* at;        // {start, rows, adapter, 0}
+  const int4* at;        // {start, rows, adapter, its rank}
   const int32_t* count;
   const int32_t* ids;
   int ids_rows, adapters;

@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) narrow_kernel(const Params p) 
     }
     p.y[(sorted ? (int64_t)row[t] : start + t) * p.N + n0 + n] = v;
   }
-  if (p.splits > 1) ptx::cluster_sync();  // no CTA leaves while another reads its shared memory
+  if (p.splits > 1) ptx::cluster_sync_relaxed();  // no CTA leaves while another reads its shared memory
 }
 
 template <typename T, int kG>

@@ -263,8 +263,8 @@ int sglb200_route_topk(const void* logits, int dtype, int64_t rows, int num_expe
  *   out[t, n] = rnd( base[t, n] + scalings[l] * sum_{r < ranks[l]} lora_b[l, n, r] * sum_k x[t, k] lora_a[l, s(n) * rank + r, k] )
  * with l = adapter_ids[t], and out = base where that names none (outside [0, num_adapters)).  s(n): the slice that column n is in, of
  * num_slices (at most 8) merged projections of slice_sizes columns (host array), N in all.
- * x [tokens, K], base and out [tokens, N]: dtype 0 or 1, rows their strides (in elements) apart; out may be base, and is not to overlap
- * it otherwise.  lora_a [num_adapters, num_slices * rank, K], lora_b [num_adapters, N, rank]: the same type, contiguous.  scalings
+ * x [tokens, K], base and out [tokens, N]: dtype 0 or 1, rows their strides (in elements) apart; out may be base; another
+ * overlap of the two is refused (of different strides: a byte between the other's ends).  An infinite lora_b may give NaN.  lora_a [num_adapters, num_slices * rank, K], lora_b [num_adapters, N, rank]: the same type, contiguous.  scalings
  * (float32), ranks (int32): [num_adapters] or NULL (1, rank); what lies beyond an adapter's rank is not used.  rank % 8 == 0, at most
  * 256; K % 8 == 0; x_stride % 8 == 0; x, lora_a and lora_b 16-byte aligned.  workspace: 16-byte aligned, the bytes that the function
  * beside it says.

@@ -408,6 +408,14 @@ static int64_t most_blocks(int64_t T, int L, int block) {
   const int64_t named = T < L + 1 ? T : L + 1;
   return T <= block ? named : T / block + named;
 }
+// Whether two arrays of 16-bit rows are one and the same or have no byte in common (rows of different strides: no byte between their ends).
+static bool apart(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t rows, int64_t n) {
+  const int64_t d = (int64_t)((intptr_t)b - (intptr_t)a);  // bytes
+  if (d == 0 && (lda == ldb || rows == 1)) return true;
+  if (d >= ((rows - 1) * lda + n) * 2 || -d >= ((rows - 1) * ldb + n) * 2) return true;
+  const int64_t within = (d % (lda * 2) + lda * 2) % (lda * 2);  // where in a row of a one of b begins
+  return lda == ldb && rows > 1 && within >= n * 2 && within <= (lda - n) * 2;
+}
 static int64_t up(int64_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace lora
@@ -456,6 +464,7 @@ extern "C" int sglb200_lora_add(const void* x, const void* lora_a, const void* l
   SGLB_REQUIRE(x && lora_a && lora_b && base && out && adapter_ids, "lora_add: null pointer");
   SGLB_REQUIRE(aligned16(x) && aligned16(lora_a) && aligned16(lora_b), "lora_add: x, lora_a and lora_b must be 16-byte aligned");
   SGLB_REQUIRE(((uintptr_t)base & 1) == 0 && ((uintptr_t)out & 1) == 0, "lora_add: base and out must be aligned to 2 bytes");
+  SGLB_REQUIRE(lora::apart(base, base_stride, out, out_stride, tokens, N), "lora_add: out overlaps base and is not base");
   const int64_t bytes = sglb200_lora_add_workspace_bytes(tokens, num_adapters, rank, num_slices);
   if (workspace == nullptr || workspace_bytes < bytes || !aligned16(workspace))
     return fail(SGLB200_E_WORKSPACE, "lora_add: %lld bytes of workspace are needed, aligned to 16", (long long)bytes);
@@ -492,7 +501,7 @@ extern "C" int sglb200_lora_add(const void* x, const void* lora_a, const void* l
   if (rc) return rc;
   p.b = lora_b, p.base = base, p.out = out, p.h = h, p.scalings = scalings, p.ranks = ranks;
   p.N = N, p.ld_base = base_stride, p.ld_out = out_stride, p.R = rank, p.S = num_slices, p.max_blocks = (int)blocks;
-  p.in_place = base == out && base_stride == out_stride;
+  p.in_place = base == out;
   p.vec = even && N % 8 == 0 && base_stride % 8 == 0 && out_stride % 8 == 0 && aligned16(base) && aligned16(out);
   p.wait_probes = g_gemm_wait_probes;
   // (its row pitches are 32-bit numbers of bytes)

@@ -657,8 +657,8 @@ def lora_add(
     x [..., K], base [..., N] (the projection's output), both bf16 or both fp16, rows any distance apart; adapter_ids int32 [...], an
     id outside [0, L): out = base.  lora_a [L, S * R, K], lora_b [L, N, R] of the same type: of S merged projections (`slices`, their
     columns; None: one), the first takes rows 0 .. R - 1 of lora_a[l], and so on.  scalings float32 [L] (None: 1); ranks int32 [L]:
-    only that many rows (of each R) and columns of an adapter count (None: R).  `out` may be `base`; None: a new tensor.
-    Sums in float32, one rounding.  R % 8 == 0, at most 256; at most 1024 adapters and 8 slices; K % 8 == 0."""
+    only that many rows (of each R) and columns of an adapter count (None: R).  `out` may be `base`, and not overlap it otherwise;
+    None: a new tensor.  Sums in float32, one rounding.  R % 8 == 0, at most 256; at most 1024 adapters and 8 slices; K % 8 == 0."""
     got = host.lora_add(base, x, lora_a, lora_b, adapter_ids, scalings, ranks, slices, out)
     if got is not None:
         return got

@@ -175,3 +175,44 @@ def test_leading_dimensions_and_no_tokens():
     assert torch.equal(got.view(24, 72), _run(c))
     none = ops.lora_add(d["base"][:0], d["x"][:0], d["a"], d["b"], d["ids"][:0])
     assert tuple(none.shape) == (0, 72)
+
+
+@pytest.mark.parametrize("T", [64, 65, 257, 3000])
+def test_most_adapters_and_slices(T):
+    c = _case(T, 64, [8, 16, 24, 8, 40, 8, 8, 16], 8, 1024, "bf16", T, "mixed", whole=True)
+    want, _ = _want(c)
+    np.testing.assert_array_equal(_run(c).cpu().double().numpy(), want)
+
+
+@pytest.mark.parametrize("T", [1, 70, 2100])
+def test_offsets_beyond_32_bits(T):
+    """An adapter behind 2^31 others' weights; 2100 tokens' rows of base and out pass 2^31 values as well."""
+    from sglang_b200 import ops
+    L, N, R, K = 40, 1 << 20, 56, 64
+    g = torch.Generator(device="cuda").manual_seed(T)
+    b = torch.zeros(L, N, R, device="cuda", dtype=torch.bfloat16)
+    a = torch.zeros(L, R, K, device="cuda", dtype=torch.bfloat16)
+    b[L - 1] = torch.randint(-1, 2, (N, R), generator=g, device="cuda").to(torch.bfloat16)
+    a[L - 1, torch.arange(R), torch.arange(R)] = 1  # h = the first R of x
+    x = torch.randint(-1, 2, (T, K), generator=g, device="cuda").to(torch.bfloat16)
+    base = torch.zeros(T, N, device="cuda", dtype=torch.bfloat16)
+    base[:, ::7] = 3
+    ids = torch.full((T,), L - 1, dtype=torch.int32, device="cuda")
+    got = ops.lora_add(base, x, a, b, ids)
+    for c0 in (0, N // 2 + 24, N - 1000):
+        cols = slice(c0, c0 + 1000)
+        want = base[:, cols].double() + x[:, :R].double() @ b[L - 1, cols].double().t()
+        assert torch.equal(got[:, cols].double(), want)
+
+
+def test_columns_of_one_buffer():
+    """base and out side by side in one buffer."""
+    from sglang_b200 import ops
+    c = _case(90, 128, [72], 16, 3, "bf16", 11, "mixed")
+    d = {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    both = torch.zeros(90, 160, device="cuda", dtype=torch.bfloat16)
+    both[:, :72] = d["base"]
+    ops.lora_add(both[:, :72], d["x"], d["a"], d["b"], d["ids"], d["scalings"], out=both[:, 80:152])
+    assert torch.equal(both[:, 80:152], _run(c)) and torch.equal(both[:, :72], d["base"]) and both[:, 72:80].eq(0).all()
+    with pytest.raises(RuntimeError, match="overlaps"):
+        ops.lora_add(both[:, :72], d["x"], d["a"], d["b"], d["ids"], d["scalings"], out=both[:, 8:80])

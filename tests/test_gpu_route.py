@@ -163,3 +163,24 @@ def test_no_rows():
     from sglang_b200 import ops
     w, ids = ops.route_topk(torch.zeros(0, 64, device="cuda"), 4)
     assert tuple(w.shape) == tuple(ids.shape) == (0, 4)
+
+
+def test_offsets_beyond_32_bits():
+    from sglang_b200 import ops
+    T, E = (1 << 21) + 77, 1024
+    x = torch.zeros(T, E, device="cuda", dtype=torch.bfloat16)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    tail = torch.randn(100, E, generator=g, device="cuda").to(torch.bfloat16)
+    x[-100:] = tail
+    w, i = ops.route_topk(x, 3)
+    want_w, want_i = ops.route_topk(tail, 3)
+    assert torch.equal(i[-100:], want_i) and torch.equal(w[-100:], want_w)
+    assert i[:-100].eq(torch.arange(3, device="cuda", dtype=torch.int32)).all()
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,groups,kept", [(32, 32, 5), (2, 2, 1), (31, 31, 31)])
+def test_groups_of_one_expert(E, groups, kept, scoring):
+    x = _logits(50, E, E)
+    for b, top in ((None, 1), (None, 2), (torch.linspace(-0.3, 0.3, E), 2)):
+        _check(x, min(kept, 4), scoring, b, groups, kept, top, True)

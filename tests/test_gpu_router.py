@@ -74,3 +74,15 @@ def test_infinities_and_nan_stay_in_their_rows(T):
     got = ops.router_logits(x, w)
     keep = [t for t in range(T) if t not in (1, 2)]
     assert torch.equal(got[keep], want[keep]) and got[1].isnan().all() and not got[2].isfinite().any()
+
+
+@pytest.mark.parametrize("E", [8, 512])
+def test_offsets_beyond_32_bits(E):
+    from sglang_b200 import ops
+    T, K, apart = 130, 64, (1 << 24) + 512  # the last rows begin behind 2^31 values
+    wide = torch.empty(T * apart, device="cuda", dtype=torch.bfloat16).view(T, apart)
+    g = torch.Generator(device="cuda").manual_seed(E)
+    x = torch.randn(T, K, generator=g, device="cuda").to(torch.bfloat16)
+    w = torch.randn(E, K, generator=g, device="cuda").to(torch.bfloat16)
+    wide[:, :K] = x
+    assert torch.equal(ops.router_logits(wide[:, :K], w), ops.router_logits(x, w))

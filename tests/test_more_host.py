@@ -77,6 +77,13 @@ def test_lora_add_refuses():
     assert call(x=None) == -1 and call(ids=None) == -1 and "null" in _err()
     assert call(a=A + 8) == -1 and "16-byte" in _err()
     assert call(out=A + 1) == -1 and "2 bytes" in _err()
+    for kw in (dict(out=A + 2), dict(out=A + 64), dict(out=A - 128), dict(ldo=72), dict(out=A + 100, ldb=200, ldo=200), dict(out=A + 320, ldb=200, ldo=200),
+               dict(out=A + 64, T=1), dict(out=A + 504)):
+        assert call(**kw) == -1 and "overlaps" in _err(), kw
+    # columns of one buffer, arrays behind one another, one row of any stride: no overlap, so the next check speaks
+    for kw in (dict(), dict(out=A + 128, ldb=128, ldo=128), dict(out=A + 272, ldb=200, ldo=200), dict(out=A + 512), dict(out=A - 512),
+               dict(ldo=72, T=1), dict(out=A + 128, T=1)):
+        assert call(ws=None, **kw) == -4, kw
     need = lib.sglb200_lora_add_workspace_bytes(4, 2, 16, 1)
     assert need > 0 and call(bytes=need - 1) == -4 and "workspace" in _err() and call(ws=None) == -4 and call(ws=A + 8) == -4
     assert call(T=0, x=None, base=None) == 0

@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __res
   __syncthreads();
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
-  const int part = (T + kPlanThreads - 1) / kPlanThreads * 32, begin = min(warp * part, T), end = min(begin + part, T);
+  const int part = (T + kPlanThreads - 1) / kPlanThreads * 32, shift = __ffs(block) - 1, begin = min(warp * part, T), end = min(begin + part, T);
   auto key_of = [&](int t) {  // (past the end: nobody's)
     const int id = t < end ? ids[t] : 0;
     return t >= end ? keys : id >= 0 && id < L ? id : L;
@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __res
   if (warp == 0) {
     int tokens = 0, before = 0;
     for (int at = 0; at < keys; at += 32) {
-      const int l = at + lane, n = l < keys ? tokens_before[l] : 0, b = (n + block - 1) / block;
+      const int l = at + lane, n = l < keys ? tokens_before[l] : 0, b = (n + block - 1) >> shift;
       int sn = n, sb = b;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
@@ -143,8 +143,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPairs == 1 ? 3 : 2) expand_kerne
   // This CTA's units, and its block's tokens, rows and adapter to shared memory.
   int block = -1, begin = 0, end = 0;
   auto cut = [&](int blocks) {
-    const int64_t all = (int64_t)blocks * p.subs * per;
-    begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
+    share(blocks * p.subs * per, begin, end);
   };
   auto find = [&](int which) {
     if (scan) {

@@ -28,6 +28,12 @@ struct Params {
   uint32_t wait_probes;
 };
 
+// This CTA's even share of `all` (below 2^31) units.  (A division in 64 bits takes a fifth of a microsecond, and a kernel's start was two of them.)
+__device__ __forceinline__ void share(int all, int& begin, int& end) {
+  const uint32_t each = (uint32_t)all / gridDim.x, more = (uint32_t)all - each * gridDim.x, i = blockIdx.x;
+  begin = (int)(each * i + min(i, more)), end = begin + (int)(each + (i < more ? 1 : 0));
+}
+
 template <typename T>
 __device__ __forceinline__ uint16_t bits(T v) {
   return *reinterpret_cast<const uint16_t*>(&v);

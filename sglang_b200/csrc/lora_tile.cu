@@ -98,8 +98,8 @@ __global__ void __launch_bounds__(kThreads, 1) expand_tile_kernel(const Params p
   ptx::tc_fence_after();
   ptx::launch_dependents();
   const uint32_t tmem = ctl.tmem_base;
-  const int64_t all = (int64_t)__ldcg(p.blocks.count) * p.chunk0[p.S];
-  const int begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
+  int begin, end;
+  share(__ldcg(p.blocks.count) * p.chunk0[p.S], begin, end);
 
   if (warp == kAdders) {
     // ------------------------------ weights: chunks of 16 bytes, row n to its place in the order above ------------------------------

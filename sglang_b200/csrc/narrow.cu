@@ -71,8 +71,9 @@ __global__ void __launch_bounds__(kWarps * 32, 3) narrow_kernel(const Params p) 
   __shared__ int32_t row[kSmallBlock];
   __shared__ int found[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = ptx::warp_index(), g = lane >> 2;
-  const int rank = (int)(blockIdx.x % p.splits), n0 = (int)(blockIdx.x / p.splits % p.n_tiles) * 16;
-  const int64_t block = blockIdx.x / p.splits / p.n_tiles;
+  const uint32_t tile = cluster_id(), of_block = tile / (uint32_t)p.n_tiles;
+  const int rank = cluster_rank(), n0 = (int)(tile - of_block * p.n_tiles) * 16;
+  const int64_t block = of_block;
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
   int64_t start = block * kSmallBlock, adapter = 0;
@@ -98,11 +99,12 @@ __global__ void __launch_bounds__(kWarps * 32, 3) narrow_kernel(const Params p) 
   }
   const T* w = static_cast<const T*>(p.w) + adapter * p.N * p.K;
   const int na = n0 + g, nb = n0 + g + 8;
-  const bool a_on = na < p.N && na % p.rank_rows < used, b_on = nb < p.N && nb % p.rank_rows < used;
+  const bool whole = used == p.rank_rows;
+  const bool a_on = na < p.N && (whole || na % p.rank_rows < used), b_on = nb < p.N && (whole || nb % p.rank_rows < used);
   const T* wa = w + (a_on ? na : 0) * p.K;
   const T* wb = w + (b_on ? nb : 0) * p.K;
   const int steps = (int)((p.K + kStep - 1) / kStep), parts = p.splits * kWarps, mine = rank * kWarps + warp;
-  const int s0 = (int)((int64_t)mine * steps / parts), s1 = (int)((int64_t)(mine + 1) * steps / parts);
+  const int s0 = mine * steps / parts, s1 = (mine + 1) * steps / parts;  // (at most 64 x 32768)
   auto row_of = [&](int i) { return sorted ? (int64_t)row[i] : start + i; };
   float* to = &part[warp][0][0];
   // (blocks of a batch of many adapters have few rows)

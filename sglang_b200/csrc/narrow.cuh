@@ -20,7 +20,7 @@ struct Blocks {
   int ids_rows, adapters;
 };
 
-// One warp: how many blocks of up to `most` rows there are, and of block `block`, in the order of their first rows, its rows (to `row`,
+// One warp: how many blocks of up to `most` (a power of two) rows there are, and of block `block`, in the order of their first rows, its rows (to `row`,
 // ascending), if it is one of them.
 __device__ __forceinline__ int scan_block(const Blocks& b, int block, int most, int lane, int32_t* row, int& rows, int& adapter) {
   auto key = [&](int t) {
@@ -39,7 +39,7 @@ __device__ __forceinline__ int scan_block(const Blocks& b, int block, int most, 
 #pragma unroll
     for (int i = 0; i < 32; ++i) nth1 += __shfl_sync(0xffffffffu, k0, i) == k1;
   }
-  const uint32_t first0 = __ballot_sync(0xffffffffu, nth0 % most == 0) & all0, first1 = __ballot_sync(0xffffffffu, nth1 % most == 0) & all1;
+  const uint32_t first0 = __ballot_sync(0xffffffffu, (nth0 & (most - 1)) == 0) & all0, first1 = __ballot_sync(0xffffffffu, (nth1 & (most - 1)) == 0) & all1;
   const int blocks = __popc(first0) + __popc(first1);
   const bool low = block < __popc(first0);
   const uint32_t firsts = low ? first0 : first1;
@@ -71,6 +71,18 @@ struct Params {
 
 // Rows of a block for T rows and N weight rows, of adapters or of one router.
 int block_rows(int64_t T, int64_t N, bool adapters);
+
+// A cluster has the K of one tile.  (Its number and a CTA's in it come without a division.)
+__device__ __forceinline__ uint32_t cluster_id() {
+  uint32_t v;
+  asm("mov.u32 %0, %%clusterid.x;" : "=r"(v));
+  return v;
+}
+__device__ __forceinline__ int cluster_rank() {
+  int v;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(v));
+  return v;
+}
 
 // y = x w^T in blocks of p.block rows, `max_blocks` the most blocks there can be.
 int product(Params p, int dtype, int64_t max_blocks, cudaStream_t st);

@@ -119,8 +119,9 @@ __global__ void __launch_bounds__(kSorted ? kSortedThreads : kThreads, 1)
   Ctl* ctl = reinterpret_cast<Ctl*>(ring + kRing);
   const int tid = threadIdx.x, warp = ptx::warp_index(), lane = tid & 31;
   volatile int* abort_flag = &ctl->abort_flag;
-  const int rank = (int)(blockIdx.x % p.splits), n0 = (int)(blockIdx.x / p.splits % p.n_tiles) * t.nt;
-  const int64_t block = blockIdx.x / p.splits / p.n_tiles;
+  const uint32_t tile = cluster_id(), of_block = tile / (uint32_t)p.n_tiles;
+  const int rank = cluster_rank(), n0 = (int)(tile - of_block * p.n_tiles) * t.nt;
+  const int64_t block = of_block;
   const uint32_t full = ptx::smem_u32(ctl->full), empty = ptx::smem_u32(ctl->empty), acc_full = ptx::smem_u32(ctl->acc_full),
                  acc_empty = ptx::smem_u32(ctl->acc_empty);
   // (tensor memory is taken once the kernel in front has ended; the kernel behind may start when every CTA has its own)
@@ -162,7 +163,7 @@ __global__ void __launch_bounds__(kSorted ? kSortedThreads : kThreads, 1)
   ptx::tc_fence_after();
   ptx::launch_dependents();
   const uint32_t tmem = ctl->tmem_base;
-  const int kb0 = (int)((int64_t)rank * t.kb_total / p.splits), kb1 = (int)((int64_t)(rank + 1) * t.kb_total / p.splits);
+  const int kb0 = rank * t.kb_total / p.splits, kb1 = (rank + 1) * t.kb_total / p.splits;
   const uint32_t w_bytes = (uint32_t)t.nt * kStageK * 2, stage_bytes = kXBytes + w_bytes, base = ptx::smem_u32(ring);
   const int units = t.nt / 16, half = (units + 1) / 2;
 

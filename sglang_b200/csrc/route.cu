@@ -34,7 +34,7 @@ struct Params {
   int32_t* out_i;
   int64_t rows;
   int E, k, groups, kept, top;
-  int group_size, group_lanes, per_lane;  // lanes of a group, experts of a lane
+  int group_size, group_lanes, group_shift, per_lane;  // lanes of a group (2^group_shift), experts of a lane
   int softmax, renorm;
   float factor;
 };
@@ -102,8 +102,8 @@ struct Place {
 };
 __device__ __forceinline__ Place place(const Params& p, int lane) {
   Place a;
-  a.group = lane / p.group_lanes;
-  const int at = (lane - a.group * p.group_lanes) * p.per_lane;
+  a.group = lane >> p.group_shift;
+  const int at = (lane & (p.group_lanes - 1)) * p.per_lane;
   a.first = a.group * p.group_size + at;
   a.count = a.group < p.groups ? max(0, min(p.per_lane, p.group_size - at)) : 0;
   return a;
@@ -439,7 +439,9 @@ extern "C" int sglb200_route_topk(const void* logits, int dtype, int64_t rows, i
   p.group_size = num_experts / num_expert_group;
   int lanes = 32;
   while (lanes * num_expert_group > 32) lanes >>= 1;
-  p.group_lanes = lanes, p.per_lane = (p.group_size + lanes - 1) / lanes;
+  p.group_lanes = lanes, p.group_shift = 0;
+  while (1 << p.group_shift < lanes) ++p.group_shift;
+  p.per_lane = (p.group_size + lanes - 1) / lanes;
   if (p.per_lane > route::kMaxPerLane)
     return fail(SGLB200_E_UNSUPPORTED, "route_topk: %d groups of %d experts (at most %d experts a group)", num_expert_group, p.group_size,
                 route::kMaxPerLane * lanes);

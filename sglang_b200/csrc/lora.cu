@@ -142,15 +142,15 @@ __global__ void __launch_bounds__(kWarps * 32, kPairs == 1 ? 3 : 2) expand_kerne
   // The launch in front let this one in after its own wait for all that came before it, so only h is not there yet.
   // This CTA's units, and its block's tokens, rows and adapter to shared memory.
   int block = -1, begin = 0, end = 0;
-  auto cut = [&](int blocks) {
-    share(blocks * p.subs * per, begin, end);
+  auto cut = [&](int blocks) { share(blocks * p.subs * per, begin, end); };
+  auto pick = [&](const narrow::Scan& s, int which) {
+    int n = 0, a = -1;
+    narrow::scan_pick(s, which, p.sub, lane, token, n, a);
+    if (lane == 0) found[1] = n, found[2] = a, found[3] = a < 0 ? 0 : p.ranks != nullptr ? min(max(__ldg(p.ranks + a), 0), p.R) : p.R;
   };
   auto find = [&](int which) {
     if (scan) {
-      if (warp != 0) return;
-      int n = 0, a = -1;
-      narrow::scan_block(p.blocks, which, p.sub, lane, token, n, a);
-      if (lane == 0) found[1] = n, found[2] = a, found[3] = a < 0 ? 0 : p.ranks != nullptr ? min(max(__ldg(p.ranks + a), 0), p.R) : p.R;
+      if (warp == 0) pick(narrow::scan_ids(p.blocks, p.sub, lane), which);
     } else {
       const int4 at = __ldcg(p.blocks.at + which);
       if (tid < at.y) token[tid] = __ldcg(p.blocks.order + at.x + tid);
@@ -161,11 +161,10 @@ __global__ void __launch_bounds__(kWarps * 32, kPairs == 1 ? 3 : 2) expand_kerne
     cut(__ldcg(p.blocks.count));
   } else {
     if (warp == 0) {  // (one warp looks at the tokens once for both)
-      int n = 0, a = -1;
-      const int blocks = narrow::scan_block(p.blocks, -1, p.sub, lane, token, n, a);
-      cut(blocks);
-      if (begin < end) find(begin / per);
-      if (lane == 0) found[0] = blocks;
+      const narrow::Scan s = narrow::scan_ids(p.blocks, p.sub, lane);
+      cut(s.blocks());
+      if (begin < end) pick(s, begin / per);
+      if (lane == 0) found[0] = s.blocks();
     }
     block = -2;  // found already
     __syncthreads();

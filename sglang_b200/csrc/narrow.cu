@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) narrow_kernel(const Params p) 
   if (p.blocks.ids != nullptr) {
     if (warp == 0) {
       int n = 0, a = -1;
-      scan_block(p.blocks, (int)block, kSmallBlock, lane, row, n, a);  // (0 rows: there is no such block)
+      scan_pick(scan_ids(p.blocks, kSmallBlock, lane), (int)block, kSmallBlock, lane, row, n, a);  // (0 rows: there is no such block)
       if (lane == 0) found[0] = n, found[1] = a;
     }
     __syncthreads();
@@ -104,7 +104,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3) narrow_kernel(const Params p) 
   const T* wa = w + (a_on ? na : 0) * p.K;
   const T* wb = w + (b_on ? nb : 0) * p.K;
   const int steps = (int)((p.K + kStep - 1) / kStep), parts = p.splits * kWarps, mine = rank * kWarps + warp;
-  const int s0 = mine * steps / parts, s1 = (mine + 1) * steps / parts;  // (at most 64 x 32768)
+  const int parts_log = 31 - __clz(parts);
+  const int s0 = mine * steps >> parts_log, s1 = (mine + 1) * steps >> parts_log;  // (at most 64 x 32768)
   auto row_of = [&](int i) { return sorted ? (int64_t)row[i] : start + i; };
   float* to = &part[warp][0][0];
   // (blocks of a batch of many adapters have few rows)

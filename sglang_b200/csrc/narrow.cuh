@@ -20,40 +20,49 @@ struct Blocks {
   int ids_rows, adapters;
 };
 
-// One warp: how many blocks of up to `most` (a power of two) rows there are, and of block `block`, in the order of their first rows, its rows (to `row`,
-// ascending), if it is one of them.
-__device__ __forceinline__ int scan_block(const Blocks& b, int block, int most, int lane, int32_t* row, int& rows, int& adapter) {
+// One warp's look at the rows' ids, lane l's rows l and l + 32, for blocks of up to `most` (a power of two) rows: the adapters, which of its
+// adapter's rows a row is, and the rows that begin a block.
+struct Scan {
+  int k0, k1, nth0, nth1;
+  uint32_t all0, all1, first0, first1;
+  __device__ __forceinline__ int blocks() const { return __popc(first0) + __popc(first1); }
+};
+__device__ __forceinline__ Scan scan_ids(const Blocks& b, int most, int lane) {
   auto key = [&](int t) {
     const int id = t < b.ids_rows ? __ldg(b.ids + t) : -1;
     return id >= 0 && id < b.adapters ? id : -1;
   };
-  const int k0 = key(lane), k1 = key(lane + 32);
-  const uint32_t all0 = b.ids_rows >= 32 ? 0xffffffffu : (1u << b.ids_rows) - 1;
-  const uint32_t all1 = b.ids_rows >= 64 ? 0xffffffffu : b.ids_rows > 32 ? (1u << (b.ids_rows - 32)) - 1 : 0;
-  // which of its adapter's rows a row is; every `most`-th begins a block
+  Scan s;
+  s.k0 = key(lane), s.k1 = key(lane + 32);
+  s.all0 = b.ids_rows >= 32 ? 0xffffffffu : (1u << b.ids_rows) - 1;
+  s.all1 = b.ids_rows >= 64 ? 0xffffffffu : b.ids_rows > 32 ? (1u << (b.ids_rows - 32)) - 1 : 0;
   const uint32_t before = (1u << lane) - 1;
-  const int nth0 = __popc(__match_any_sync(0xffffffffu, k0) & all0 & before);
-  int nth1 = 0;
-  if (all1 != 0) {
-    nth1 = __popc(__match_any_sync(0xffffffffu, k1) & all1 & before);
+  s.nth0 = __popc(__match_any_sync(0xffffffffu, s.k0) & s.all0 & before);
+  s.nth1 = 0;
+  if (s.all1 != 0) {
+    s.nth1 = __popc(__match_any_sync(0xffffffffu, s.k1) & s.all1 & before);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) nth1 += __shfl_sync(0xffffffffu, k0, i) == k1;
+    for (int i = 0; i < 32; ++i) s.nth1 += __shfl_sync(0xffffffffu, s.k0, i) == s.k1;
   }
-  const uint32_t first0 = __ballot_sync(0xffffffffu, (nth0 & (most - 1)) == 0) & all0, first1 = __ballot_sync(0xffffffffu, (nth1 & (most - 1)) == 0) & all1;
-  const int blocks = __popc(first0) + __popc(first1);
-  const bool low = block < __popc(first0);
-  const uint32_t firsts = low ? first0 : first1;
-  const uint32_t it = __ballot_sync(0xffffffffu, (firsts >> lane & 1u) && __popc(firsts & before) == (low ? block : block - __popc(first0)));
-  if (it == 0) return blocks;
+  s.first0 = __ballot_sync(0xffffffffu, (s.nth0 & (most - 1)) == 0) & s.all0;
+  s.first1 = __ballot_sync(0xffffffffu, (s.nth1 & (most - 1)) == 0) & s.all1;
+  return s;
+}
+// Block `block`, in the order of their first rows: its rows (to `row`, ascending) and its adapter, if it is one of them.
+__device__ __forceinline__ void scan_pick(const Scan& s, int block, int most, int lane, int32_t* row, int& rows, int& adapter) {
+  const uint32_t before = (1u << lane) - 1;
+  const bool low = block < __popc(s.first0);
+  const uint32_t firsts = low ? s.first0 : s.first1;
+  const uint32_t it = __ballot_sync(0xffffffffu, (firsts >> lane & 1u) && __popc(firsts & before) == (low ? block : block - __popc(s.first0)));
+  if (it == 0) return;
   const int from = __ffs(it) - 1;
-  adapter = __shfl_sync(0xffffffffu, low ? k0 : k1, from);
-  const int nth = __shfl_sync(0xffffffffu, low ? nth0 : nth1, from);
-  const bool in0 = k0 == adapter && (all0 >> lane & 1u) && nth0 >= nth && nth0 < nth + most;
-  const bool in1 = k1 == adapter && (all1 >> lane & 1u) && nth1 >= nth && nth1 < nth + most;
-  if (in0) row[nth0 - nth] = lane;
-  if (in1) row[nth1 - nth] = lane + 32;
+  adapter = __shfl_sync(0xffffffffu, low ? s.k0 : s.k1, from);
+  const int nth = __shfl_sync(0xffffffffu, low ? s.nth0 : s.nth1, from);
+  const bool in0 = s.k0 == adapter && (s.all0 >> lane & 1u) && s.nth0 >= nth && s.nth0 < nth + most;
+  const bool in1 = s.k1 == adapter && (s.all1 >> lane & 1u) && s.nth1 >= nth && s.nth1 < nth + most;
+  if (in0) row[s.nth0 - nth] = lane;
+  if (in1) row[s.nth1 - nth] = lane + 32;
   rows = __popc(__ballot_sync(0xffffffffu, in0)) + __popc(__ballot_sync(0xffffffffu, in1));
-  return blocks;
 }
 
 struct Params {

@@ -109,7 +109,8 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
 // As a sum does not mind the order of its terms, a lane's 16 consecutive bytes of a weight row (and of a row of h alike) are its part of both
 // instructions.  A lane holds the same two kTiles neighbouring columns of a token in all groups, so that base and out go by 4 kTiles bytes.
 //
-// Weights and base bound this kernel.  They come by asynchronous copies, each lane's to a place of its own, kDepth - 1 steps (16 tokens of a
+// Weights and base bound this kernel, and with few tokens a run's start: 64 tokens of 16 adapters beside 36864 columns take about 12 us, where the 48 MB
+// would take 7.5.  They come by asynchronous copies, each lane's to a place of its own, kDepth - 1 steps (16 tokens of a
 // unit) ahead, and before h is there.
 template <int kPairs, int kTiles>
 struct ExpandCfg {

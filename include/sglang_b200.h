@@ -247,7 +247,7 @@ int sglb200_router_logits(const void* x, const void* w, int dtype, float* y, int
                           int64_t x_stride, void* stream);
 
 /*
- * Routing in general form, decided by the real numbers:  s = softmax(x) (softmax != 0) or sigmoid(x);  c = s + correction_bias (float32
+ * Routing in general form, decided by the real numbers as far as float64 tells them (c that are equal there: by their logits):  s = softmax(x) (softmax != 0) or sigmoid(x);  c = s + correction_bias (float32
  * [num_experts] or NULL);  the value of each of the num_expert_group groups is the sum of its group_top (1 or 2) largest c; the
  * topk_group best groups are kept (equal: lower group first) and the topk largest c in them picked (equal: lower expert first);
  * weight = s, divided by the sum of the picks' s when renormalize, times routed_scaling_factor.

@@ -25,7 +25,8 @@ def lora_add(base, x, a, b, ids, scalings, ranks, slices):
 
 
 def route(x, topk, scoring, bias=None, groups=1, kept=1, top=1, renorm=True, factor=1.0):
-    """(weights float64, ids) of the logits x [T, E] (float64 values)."""
+    """(weights float64, ids) of the logits x [T, E] (float64 values).  c that float64 holds as equal go by their logits (which is the order of
+    the real numbers where their biases are equal), then by index; groups likewise where one c is their value."""
     T, E = x.shape
     w, ids = np.zeros((T, topk)), np.full((T, topk), -1, dtype=np.int32)
     for t in range(T):
@@ -45,15 +46,17 @@ def route(x, topk, scoring, bias=None, groups=1, kept=1, top=1, renorm=True, fac
         key = c if bias is not None else v
         allowed = np.ones(E, bool)
         if groups > 1:
-            value = np.full(groups, -np.inf)
+            value, second = np.full(groups, -np.inf), np.zeros(groups)
             for g in range(groups):
                 of = (v if bias is None and top == 1 else c)[g * (E // groups) : (g + 1) * (E // groups)]
                 best = sorted((z for z in of if z > -np.inf), reverse=True)[:top]
                 if best:
                     value[g] = sum(best)
-            order = sorted(range(groups), key=lambda g: (-value[g], g))[:kept]
+                    if top == 1:
+                        second[g] = max(z for z, cz in zip(v[g * (E // groups) : (g + 1) * (E // groups)], of) if cz == best[0])
+            order = sorted(range(groups), key=lambda g: (-value[g], -second[g], g))[:kept]
             allowed = np.repeat([g in order for g in range(groups)], E // groups)
-        order = sorted((e for e in range(E) if allowed[e] and c[e] > -np.inf), key=lambda e: (-key[e], e))[:topk]
+        order = sorted((e for e in range(E) if allowed[e] and c[e] > -np.inf), key=lambda e: (-key[e], -v[e], e))[:topk]
         ids[t, : len(order)] = order
         if order:
             if renorm:

@@ -6,6 +6,8 @@
 // The order is that of the real numbers.  Without a bias it is the order of the logits.  Where scores decide it is taken in float32, which
 // tells two c apart that differ by more than `margin` (below); a row in which two neighbours of the order are closer than that, and are not
 // the same logit with the same bias, is decided once more in float64 by its warp: the picks' order of one row in forty with 256 experts, a whole row of a few thousand.
+// c that float64 does not tell apart either (sigmoids of logits from 37 on are all 1) go by their logits, which is right wherever their biases
+// are equal; a group's sum of two is what float64 makes it.
 //
 // One warp a row, the row in registers: lane l has consecutive experts of one group.  It is bound by issue slots.  A lane sorts its
 // experts once, as integers: an order-preserving bit pattern of c, whose lowest bits give way to the expert's number in the lane and, for the
@@ -109,13 +111,14 @@ __device__ __forceinline__ Place place(const Params& p, int lane) {
   return a;
 }
 
-// The kept groups, one bit each, by value (lane g has group g's) and index.
+// The kept groups, one bit each, by value (lane g has group g's), what decides among equal values, and index.
 template <typename V>
-__device__ __forceinline__ uint32_t keep_groups(const Params& p, V mine, int lane) {
+__device__ __forceinline__ uint32_t keep_groups(const Params& p, V mine, int lane, float second = 0.f) {
   int beaten_by = 0;
   for (int g = 0; g < p.groups; ++g) {
     const V other = __shfl_sync(kAll, mine, g);
-    beaten_by += other > mine || (other == mine && g < lane);
+    const float other_second = sizeof(V) == 8 ? __shfl_sync(kAll, second, g) : second;
+    beaten_by += other > mine || (other == mine && (other_second > second || (other_second == second && g < lane)));
   }
   return __ballot_sync(kAll, lane < p.groups && beaten_by < p.kept);
 }
@@ -156,7 +159,7 @@ __device__ __forceinline__ double exact_sum(const Params& p, const T* x, double 
   return sum;
 }
 
-// The row's picks in float64: lane i < k gets the i-th.
+// The row's picks by c in float64, then by logit, then by index: lane i < k gets the i-th.
 template <typename T, int kPer>
 __device__ __noinline__ int pick_exact(const Params& p, const T* x, int lane) {
   const Place at = place(p, lane);
@@ -176,10 +179,16 @@ __device__ __noinline__ int pick_exact(const Params& p, const T* x, int lane) {
   }
   if (p.groups > 1) {
     uint64_t m1 = 0, m2 = 0;
+    float x1 = kNone;  // the largest logit of those with the largest c
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) m2 = max(m2, min(m1, c[j])), m1 = max(m1, c[j]);
+    for (int j = 0; j < kPer; ++j) {
+      if (c[j] != 0 && c[j] >= m1) x1 = c[j] > m1 ? clean(x[at.first + j]) : fmaxf(x1, clean(x[at.first + j]));
+      m2 = max(m2, min(m1, c[j])), m1 = max(m1, c[j]);
+    }
     for (int off = 1; off < p.group_lanes; off <<= 1) {
       const uint64_t o1 = __shfl_xor_sync(kAll, m1, off), o2 = __shfl_xor_sync(kAll, m2, off);
+      const float ox = __shfl_xor_sync(kAll, x1, off);
+      x1 = o1 > m1 ? ox : o1 == m1 ? fmaxf(x1, ox) : x1;
       m2 = max(max(m2, o2), min(m1, o1)), m1 = max(m1, o1);
     }
     uint64_t value = m1;
@@ -189,7 +198,8 @@ __device__ __noinline__ int pick_exact(const Params& p, const T* x, int lane) {
       value = to_ordered64(v1 + v2);
     }
     const uint64_t mine = __shfl_sync(kAll, value, (lane * p.group_lanes) & 31);
-    if (!(keep_groups<uint64_t>(p, lane < p.groups ? mine : 0, lane) >> at.group & 1u))
+    const float second = __shfl_sync(kAll, p.top == 2 ? 0.f : x1, (lane * p.group_lanes) & 31);
+    if (!(keep_groups<uint64_t>(p, lane < p.groups ? mine : 0, lane, second) >> at.group & 1u))
 #pragma unroll
       for (int j = 0; j < kPer; ++j) c[j] = 0;
   }
@@ -199,10 +209,11 @@ __device__ __noinline__ int pick_exact(const Params& p, const T* x, int lane) {
     int best_j = 0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
-      if (c[j] > best) best = c[j], best_j = j;
+      if (c[j] > best || (c[j] == best && best != 0 && clean(x[at.first + j]) > clean(x[at.first + best_j]))) best = c[j], best_j = j;
     const uint64_t winning = warp_max64(best);
     if (winning == 0) break;
-    const int winner = __ffs(__ballot_sync(kAll, best == winning)) - 1;
+    const uint32_t by_logit = best == winning ? to_ordered(clean(x[at.first + best_j])) : 0u, largest = __reduce_max_sync(kAll, by_logit);
+    const int winner = __ffs(__ballot_sync(kAll, by_logit == largest)) - 1;
     const int e = __shfl_sync(kAll, at.first + best_j, winner);
     if (lane == winner)
 #pragma unroll
@@ -213,20 +224,22 @@ __device__ __noinline__ int pick_exact(const Params& p, const T* x, int lane) {
   return picked;
 }
 
-// The `count` picks of the lanes (none left of those beyond in question) put in order by float64: lane i gets the i-th.
+// The `count` picks of the lanes (none left of those beyond in question) put in order in the same way: lane i gets the i-th.
 template <typename T>
 __device__ __noinline__ int order_exact(const Params& p, const T* x, float mx, int picked, int count, int lane) {
   const double sum = p.softmax && p.bias != nullptr ? exact_sum(p, x, (double)mx, lane) : 0.0;
   uint64_t c = 0;
+  float v = kNone;
   if (lane < count) {
-    const float v = clean(x[picked]);
+    v = clean(x[picked]);
     c = to_ordered64(p.bias != nullptr ? exact_c(p, v, picked, (double)mx, sum) : (double)v);
   }
   int rank = 0, out = -1;
   for (int i = 0; i < count; ++i) {
     const uint64_t other = __shfl_sync(kAll, c, i);
+    const float other_v = __shfl_sync(kAll, v, i);
     const int e = __shfl_sync(kAll, picked, i);
-    rank += other > c || (other == c && e < picked);
+    rank += other > c || (other == c && (other_v > v || (other_v == v && e < picked)));
   }
   for (int i = 0; i < count; ++i) {
     const int r = __shfl_sync(kAll, rank, i), e = __shfl_sync(kAll, picked, i);

@@ -445,7 +445,8 @@ def route_topk(
     group's value is the sum of its `group_top` (1 or 2; None: 2 with a bias, else 1) largest c, and the `topk` largest c of the
     `topk_group` best groups are picked.  Weights are s, divided by the picks' sum if `renormalize`, times `routed_scaling_factor`.
 
-    The order is that of the real numbers, whatever the logits' type; ties go to the lower index.  An expert whose logit is NaN or -inf
+    The order is that of the real numbers as far as float64 tells them, whatever the logits' type: c that are equal there go by their logits
+    (sigmoids of logits from 37 on are all 1), equal ones to the lower index; sums of two to the lower group.  An expert whose logit is NaN or -inf
     (or whose bias is NaN or -inf) is not available; a slot for which none is left has the id -1 and the weight 0, which the experts'
     operators skip.  topk and num_expert_group at most 32."""
     if scoring_func not in ("softmax", "sigmoid"):

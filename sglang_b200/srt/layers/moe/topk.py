@@ -39,7 +39,7 @@ def route_experts(
     group_top: Optional[int] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Routing in its general form (`ops.route_topk`): softmax or sigmoid scores, a bias that only selects, groups by their best or best
-    two, masked experts, decided by the real numbers whatever the logits' type."""
+    two, masked experts, decided by the real numbers, as far as float64 tells them, whatever the logits' type."""
     from .... import ops
 
     _need_cuda(gating_output, "route_experts")

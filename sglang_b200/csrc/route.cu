@@ -111,14 +111,13 @@ __device__ __forceinline__ Place place(const Params& p, int lane) {
   return a;
 }
 
-// The kept groups, one bit each, by value (lane g has group g's), what decides among equal values, and index.
+// The kept groups, one bit each, by value (lane g has group g's) and index.
 template <typename V>
-__device__ __forceinline__ uint32_t keep_groups(const Params& p, V mine, int lane, float second = 0.f) {
+__device__ __forceinline__ uint32_t keep_groups(const Params& p, V mine, int lane) {
   int beaten_by = 0;
   for (int g = 0; g < p.groups; ++g) {
     const V other = __shfl_sync(kAll, mine, g);
-    const float other_second = sizeof(V) == 8 ? __shfl_sync(kAll, second, g) : second;
-    beaten_by += other > mine || (other == mine && (other_second > second || (other_second == second && g < lane)));
+    beaten_by += other > mine || (other == mine && g < lane);
   }
   return __ballot_sync(kAll, lane < p.groups && beaten_by < p.kept);
 }
@@ -159,7 +158,76 @@ __device__ __forceinline__ double exact_sum(const Params& p, const T* x, double 
   return sum;
 }
 
-// The row's picks by c in float64, then by logit, then by index: lane i < k gets the i-th.
+// A pair that goes by its first and, where that is the same, by its second.
+struct Ranked {
+  uint64_t c;  // (0: none)
+  float x;
+};
+__device__ __forceinline__ bool above(Ranked a, Ranked b) { return a.c > b.c || (a.c == b.c && a.x > b.x); }
+
+// The row's picks by c in float64, then by logit, then by index, for a row with a bias: lane i < k gets the i-th.  Each is looked for anew
+// below the one before it, which is slow and small: few rows of few programs come here.
+template <typename T>
+__device__ __noinline__ int pick_by_logit(const Params& p, const T* x, int lane) {
+  const Place at = place(p, lane);
+  float mx = kNone;
+  for (int j = 0; j < at.count; ++j) mx = fmaxf(mx, clean(x[at.first + j]));
+  const double top = (double)warp_max(mx), sum = p.softmax ? exact_sum(p, x, top, lane) : 0.0;
+  auto ranked = [&](int e) {
+    Ranked r{0, clean(x[e])};
+    if (r.x > kNone) {
+      const double c = exact_c(p, r.x, e, top, sum);
+      if (c > -INFINITY) r.c = to_ordered64(c);
+    }
+    return r;
+  };
+  bool in = true;
+  if (p.groups > 1) {
+    Ranked m1{0, kNone};
+    uint64_t m2 = 0;
+    for (int j = 0; j < at.count; ++j) {
+      const Ranked r = ranked(at.first + j);
+      m2 = max(m2, min(m1.c, r.c));
+      if (above(r, m1)) m1 = r;
+    }
+    for (int off = 1; off < p.group_lanes; off <<= 1) {
+      const Ranked o{__shfl_xor_sync(kAll, m1.c, off), __shfl_xor_sync(kAll, m1.x, off)};
+      m2 = max(max(m2, __shfl_xor_sync(kAll, m2, off)), min(m1.c, o.c));
+      if (above(o, m1)) m1 = o;
+    }
+    if (p.top == 2) {  // (a sum is by itself)
+      if (m1.c != 0) m1.c = to_ordered64(from_ordered64(m1.c) + (m2 != 0 ? from_ordered64(m2) : 0.0));
+      m1.x = 0.f;
+    }
+    int beaten_by = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      const Ranked o{__shfl_sync(kAll, m1.c, g * p.group_lanes), __shfl_sync(kAll, m1.x, g * p.group_lanes)};
+      beaten_by += above(o, m1) || (!above(m1, o) && g < at.group);
+    }
+    in = beaten_by < p.kept;
+  }
+  Ranked last{~0ull, INFINITY};
+  int last_e = -1, picked = -1;
+  for (int i = 0; i < p.k; ++i) {
+    Ranked best{0, kNone};
+    int e_best = -1;
+    for (int j = 0; j < at.count && in; ++j) {
+      const int e = at.first + j;
+      const Ranked r = ranked(e);
+      const bool left = above(last, r) || (!above(r, last) && e > last_e);
+      if (left && r.c != 0 && above(r, best)) best = r, e_best = e;
+    }
+    last.c = warp_max64(best.c);
+    if (last.c == 0) break;
+    const uint32_t by_logit = best.c == last.c ? to_ordered(best.x) : 0u, largest = __reduce_max_sync(kAll, by_logit);
+    const int winner = __ffs(__ballot_sync(kAll, by_logit == largest)) - 1;
+    last.x = __shfl_sync(kAll, best.x, winner), last_e = __shfl_sync(kAll, e_best, winner);
+    if (lane == i) picked = last_e;
+  }
+  return picked;
+}
+
+// The row's picks in float64: lane i < k gets the i-th.
 template <typename T, int kPer>
 __device__ __noinline__ int pick_exact(const Params& p, const T* x, int lane) {
   const Place at = place(p, lane);
@@ -177,18 +245,13 @@ __device__ __noinline__ int pick_exact(const Params& p, const T* x, int lane) {
     const double s = !(v[j] > kNone) ? -INFINITY : biased ? exact_c(p, v[j], at.first + j, top, sum) : (double)v[j];
     c[j] = s > -INFINITY ? to_ordered64(s) : 0;
   }
+  bool by_logit = false;
   if (p.groups > 1) {
     uint64_t m1 = 0, m2 = 0;
-    float x1 = kNone;  // the largest logit of those with the largest c
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      if (c[j] != 0 && c[j] >= m1) x1 = c[j] > m1 ? clean(x[at.first + j]) : fmaxf(x1, clean(x[at.first + j]));
-      m2 = max(m2, min(m1, c[j])), m1 = max(m1, c[j]);
-    }
+    for (int j = 0; j < kPer; ++j) m2 = max(m2, min(m1, c[j])), m1 = max(m1, c[j]);
     for (int off = 1; off < p.group_lanes; off <<= 1) {
       const uint64_t o1 = __shfl_xor_sync(kAll, m1, off), o2 = __shfl_xor_sync(kAll, m2, off);
-      const float ox = __shfl_xor_sync(kAll, x1, off);
-      x1 = o1 > m1 ? ox : o1 == m1 ? fmaxf(x1, ox) : x1;
       m2 = max(max(m2, o2), min(m1, o1)), m1 = max(m1, o1);
     }
     uint64_t value = m1;
@@ -197,36 +260,56 @@ __device__ __noinline__ int pick_exact(const Params& p, const T* x, int lane) {
       if (!biased) v1 = exact_c(p, (float)v1, 0, top, sum), v2 = m2 != 0 ? exact_c(p, (float)v2, 0, top, sum) : 0.0;
       value = to_ordered64(v1 + v2);
     }
-    const uint64_t mine = __shfl_sync(kAll, value, (lane * p.group_lanes) & 31);
-    const float second = __shfl_sync(kAll, p.top == 2 ? 0.f : x1, (lane * p.group_lanes) & 31);
-    if (!(keep_groups<uint64_t>(p, lane < p.groups ? mine : 0, lane, second) >> at.group & 1u))
+    uint64_t mine = __shfl_sync(kAll, value, (lane * p.group_lanes) & 31);
+    if (lane >= p.groups) mine = 0;
+    const uint32_t keep = keep_groups<uint64_t>(p, mine, lane);
+    if (!(keep >> at.group & 1u))
 #pragma unroll
       for (int j = 0; j < kPer; ++j) c[j] = 0;
+    if (biased && p.top == 1) {  // does a group that goes have the value of one that stays?
+      const uint64_t most = warp_max64(keep >> lane & 1u ? 0 : mine);
+      by_logit = __any_sync(kAll, (keep >> lane & 1u) && mine == most && most != 0);
+    }
   }
-  int picked = -1;
+  int picked = -1, e = -1;
+  uint64_t last = 0;
   for (int i = 0; i < p.k; ++i) {
     uint64_t best = 0;
     int best_j = 0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
-      if (c[j] > best || (c[j] == best && best != 0 && clean(x[at.first + j]) > clean(x[at.first + best_j]))) best = c[j], best_j = j;
+      if (c[j] > best) best = c[j], best_j = j;
     const uint64_t winning = warp_max64(best);
     if (winning == 0) break;
-    const uint32_t by_logit = best == winning ? to_ordered(clean(x[at.first + best_j])) : 0u, largest = __reduce_max_sync(kAll, by_logit);
-    const int winner = __ffs(__ballot_sync(kAll, by_logit == largest)) - 1;
-    const int e = __shfl_sync(kAll, at.first + best_j, winner);
+    const int winner = __ffs(__ballot_sync(kAll, best == winning)) - 1, before = e;
+    e = __shfl_sync(kAll, at.first + best_j, winner);
     if (lane == winner)
 #pragma unroll
       for (int j = 0; j < kPer; ++j)
         if (j == best_j) c[j] = 0;
     if (lane == i) picked = e;
+    if (winning == last && biased) by_logit = by_logit || clean(x[e]) > clean(x[before]);
+    last = winning;
   }
-  return picked;
+  if (biased && last != 0) {  // is a larger logit left of the last one's c?
+    bool left = false;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) left = left || c[j] == last;
+    if (__any_sync(kAll, left)) {
+      bool larger = false;
+      for (int j = 0; j < at.count && left; ++j) {
+        const float other = clean(x[at.first + j]);
+        larger = larger || (other > clean(x[e]) && to_ordered64(exact_c(p, other, at.first + j, top, sum)) == last);
+      }
+      by_logit = by_logit || __any_sync(kAll, larger);
+    }
+  }
+  return by_logit ? pick_by_logit<T>(p, x, lane) : picked;
 }
 
-// The `count` picks of the lanes (none left of those beyond in question) put in order in the same way: lane i gets the i-th.
+// The `count` picks of the lanes (none left of those beyond in question) put in order in the same way, through `room`: lane i gets the i-th.
 template <typename T>
-__device__ __noinline__ int order_exact(const Params& p, const T* x, float mx, int picked, int count, int lane) {
+__device__ __noinline__ int order_exact(const Params& p, const T* x, float mx, int picked, int count, int lane, uint32_t* room) {
   const double sum = p.softmax && p.bias != nullptr ? exact_sum(p, x, (double)mx, lane) : 0.0;
   uint64_t c = 0;
   float v = kNone;
@@ -234,18 +317,22 @@ __device__ __noinline__ int order_exact(const Params& p, const T* x, float mx, i
     v = clean(x[picked]);
     c = to_ordered64(p.bias != nullptr ? exact_c(p, v, picked, (double)mx, sum) : (double)v);
   }
-  int rank = 0, out = -1;
+  int rank = 0, same = 0;
   for (int i = 0; i < count; ++i) {
     const uint64_t other = __shfl_sync(kAll, c, i);
-    const float other_v = __shfl_sync(kAll, v, i);
-    const int e = __shfl_sync(kAll, picked, i);
-    rank += other > c || (other == c && (other_v > v || (other_v == v && e < picked)));
+    rank += other > c, same += other == c;
   }
-  for (int i = 0; i < count; ++i) {
-    const int r = __shfl_sync(kAll, rank, i), e = __shfl_sync(kAll, picked, i);
-    if (lane == r) out = e;
-  }
-  return out;
+  if (__any_sync(kAll, lane < count && same > 1))
+    for (int i = 0; i < count; ++i) {
+      const uint64_t other = __shfl_sync(kAll, c, i);
+      const float other_v = __shfl_sync(kAll, v, i);
+      const int e = __shfl_sync(kAll, picked, i);
+      rank += other == c && (other_v > v || (other_v == v && e < picked));
+    }
+  __syncwarp();
+  if (lane < count) room[rank] = (uint32_t)picked;
+  __syncwarp();
+  return lane < count ? (int)room[lane] : -1;
 }
 
 // A lane's `count` consecutive values at `at` of the row (the rest -inf), 16 bytes at a time where they lie so.
@@ -266,7 +353,7 @@ __device__ __forceinline__ void load_run(const T* at, int count, float (&v)[kPer
 
 // kSoftmax: else sigmoid.
 template <typename T, int kPer, bool kSoftmax>
-__global__ void __launch_bounds__(kWarps * 32, kPer <= 8 ? 4 : 1) route_kernel(const T* __restrict__ logits, const Params p) {
+__global__ void __launch_bounds__(kWarps * 32, kPer <= 8 ? 4 : 1) route_kernel(const T* __restrict__ logits, const __grid_constant__ Params p) {
   constexpr uint32_t kIndex = kPer - 1;  // the bits of a key that hold the expert's number in the lane, the lowest on top
   constexpr uint32_t kUnits = 32 * kPer;  // and the lane
   __shared__ uint32_t picks[kWarps][kMaxTopk];
@@ -380,7 +467,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPer <= 8 ? 4 : 1) route_kernel(c
       // picks on) could not be looked at, the row is decided anew.
       const uint32_t border = 3u << (p.k - 1), among = p.k >= 32 ? kAll : (1u << p.k) - 1;
       if ((telling & border) == border || (p.k > 30 && count == 32)) redo = true;
-      if ((telling & among) != 0u && !redo) picked = order_exact<T>(p, logits_row, mx, picked, min(count, p.k + 1), lane);
+      if ((telling & among) != 0u && !redo) picked = order_exact<T>(p, logits_row, mx, picked, min(count, p.k + 1), lane, picks[warp]);
     }
     if (redo) picked = pick_exact<T, kPer>(p, logits_row, lane);
     if (lane >= p.k) picked = -1;

@@ -457,16 +457,36 @@ __global__ void __launch_bounds__(kWarps * 32, kPer <= 8 ? 4 : 1) route_kernel(c
       const uint32_t after = __shfl_down_sync(kAll, mine, 1);
       const float a = from_ordered(mine), b = from_ordered(after);
       bool tell = lane + 1 < count && lane < p.k + 1 && !(a - b > margin(biased ? kEach : 0.f, kUnits, a, b));
-      uint32_t telling = __ballot_sync(kAll, tell);
-      if (telling != 0u) {  // equal logits with equal biases are in order
+      const uint32_t close = __ballot_sync(kAll, tell);
+      uint32_t telling = close;
+      if (close != 0u) {  // equal logits with equal biases are in order
         const int after_e = __shfl_down_sync(kAll, picked, 1);
         if (tell) tell = !(clean(logits_row[picked]) == clean(logits_row[after_e]) && (!biased || p.bias[picked] == p.bias[after_e]));
         telling = __ballot_sync(kAll, tell);
       }
-      // Neighbours among the picks and the first that goes are put in order; where that one cannot be told from the next either, or (from 31
-      // picks on) could not be looked at, the row is decided anew.
-      const uint32_t border = 3u << (p.k - 1), among = p.k >= 32 ? kAll : (1u << p.k) - 1;
-      if ((telling & border) == border || (p.k > 30 && count == 32)) redo = true;
+      // Neighbours among the picks and the first that goes are put in order.  Where that one is close to the last pick and to the next as well,
+      // the run of close ones may go on behind what was looked at: the row is decided anew, unless all of the run are equal.  From 31 picks on the
+      // next cannot be looked at.
+      const uint32_t among = p.k >= 32 ? kAll : (1u << p.k) - 1;
+      if (p.k > 30) {
+        redo = redo || count == 32;
+      } else if ((close >> (p.k - 1) & 3u) == 3u) {
+        const int from = 32 - __clz(~close & among);  // where the run begins
+        bool differs = (telling & ((2u << p.k) - 1)) >> from != 0u;
+        if (!differs) {  // a lane's experts that are left, in descending order
+          const int tied = __shfl_sync(kAll, picked, p.k);
+          const float c = __shfl_sync(kAll, a, p.k);
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) {
+            const float left = from_ordered(key[j] & ~(kUnits - 1));
+            if (key[j] < kLeast || c - left > margin(biased ? kEach : 0.f, kUnits, c, left)) continue;
+            const int e = at.first + (int)(kIndex - (key[j] & kIndex));
+            if (!(clean(logits_row[e]) == clean(logits_row[tied]) && (!biased || p.bias[e] == p.bias[tied]))) differs = true;
+          }
+          differs = __any_sync(kAll, differs);
+        }
+        redo = redo || differs;
+      }
       if ((telling & among) != 0u && !redo) picked = order_exact<T>(p, logits_row, mx, picked, min(count, p.k + 1), lane, picks[warp]);
     }
     if (redo) picked = pick_exact<T, kPer>(p, logits_row, lane);

@@ -452,10 +452,10 @@ extern "C" int sglb200_lora_add(const void* x, const void* lora_a, const void* l
   bool even = true;
   for (int s = 0; s < num_slices; ++s) {
     SGLB_REQUIRE(slice_sizes[s] >= 1, "lora_add: slice %d has %lld columns", s, (long long)slice_sizes[s]);
+    SGLB_REQUIRE(slice_sizes[s] <= N - columns, "lora_add: the slices have more than %lld columns", (long long)N);
     p.col0[s] = columns;
     even = even && columns % 8 == 0;
     columns += slice_sizes[s];
-    SGLB_REQUIRE(columns <= N, "lora_add: the slices have more than %lld columns", (long long)N);
   }
   p.col0[num_slices] = columns;
   SGLB_REQUIRE(columns == N, "lora_add: the slices have %lld columns of %lld", (long long)columns, (long long)N);

@@ -446,6 +446,8 @@ extern "C" int sglb200_lora_add(const void* x, const void* lora_a, const void* l
                (long long)out_stride, (long long)N);
   SGLB_REQUIRE(tokens < (1ll << 31) - 65536 && N < (1ll << 31) - 65536 && K <= 1 << 20, "lora_add: %lld tokens, N %lld or K %lld is too large",
                (long long)tokens, (long long)N, (long long)K);
+  SGLB_REQUIRE(std::max({x_stride, base_stride, out_stride}) < std::min<int64_t>(1ll << 40, (1ll << 60) / std::max<int64_t>(tokens, 1)), "lora_add: row strides %lld, %lld or %lld are too large",
+               (long long)x_stride, (long long)base_stride, (long long)out_stride);
   SGLB_REQUIRE(slice_sizes != nullptr, "lora_add: null slice_sizes");
   lora::Params p{};
   int64_t columns = 0;

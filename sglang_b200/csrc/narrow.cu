@@ -211,6 +211,7 @@ extern "C" int sglb200_router_logits(const void* x, const void* w, int dtype, fl
                (long long)K, (long long)x_stride);
   SGLB_REQUIRE(tokens < (1ll << 31) - 256 && num_experts <= 1 << 16 && K <= 1 << 20, "router_logits: %lld tokens, %lld experts or K %lld is too large",
                (long long)tokens, (long long)num_experts, (long long)K);
+  SGLB_REQUIRE(x_stride < std::min<int64_t>(1ll << 40, (1ll << 60) / std::max<int64_t>(tokens, 1)), "router_logits: the rows' stride %lld is too large", (long long)x_stride);
   if (tokens == 0) return SGLB200_OK;
   SGLB_REQUIRE(x && w && y, "router_logits: null pointer");
   SGLB_REQUIRE(aligned16(x) && aligned16(w) && aligned16(y), "router_logits: pointers must be 16-byte aligned");

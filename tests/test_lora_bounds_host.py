@@ -19,3 +19,15 @@ def test_slices_whose_sum_wraps_around():
         assert (sum(sizes) + (1 << 63)) % (1 << 64) - (1 << 63) == 64
         rc, what = _call(sizes=sizes)
         assert rc == -1 and "more than 64 columns" in what, (sizes, rc, what)
+
+
+def test_strides_that_offsets_do_not_hold():
+    """64-bit offsets are rows x stride x 2 bytes: strides of 2^40 values and more are refused, before anything is multiplied by them."""
+    from sglang_b200._lib import lib
+    for T in (1, 4, 5, 100):
+        for kw in (dict(ldb=1 << 62, ldo=1 << 62), dict(ldb=1 << 40), dict(ldo=(1 << 63) - 8), dict(ldx=1 << 62)):
+            rc, what = _call(T=T, **kw)
+            assert rc == -1 and "too large" in what, (T, kw, rc, what)
+        assert lib.sglb200_router_logits(A, A, 0, A, T, 8, 64, 1 << 62, None) == -1 and "too large" in lib.sglb200_last_error().decode()
+    assert _call(T=1 << 30, ldb=1 << 31, ldo=1 << 31)[0] == -1
+    assert _call(ldb=(1 << 40) - 8, ldo=(1 << 40) - 8, ldx=(1 << 40) - 8, ws=None)[0] == -4  # (the next check speaks)

@@ -241,7 +241,8 @@ int sglb200_moe_fused_gate(const void* input, const void* bias, int dtype, int64
 /*
  * The router's product:  y[t, e] = sum_k x[t, k] w[e, k], float32 sums, unrounded.
  * x [tokens, K] of dtype 0 or 1, rows `x_stride` elements apart; w [num_experts, K] of the same type, contiguous; y float32
- * [tokens, num_experts].  K % 8 == 0, x_stride % 8 == 0; x, w and y 16-byte aligned.  Strides, here and below: below 2^40, and below 2^60 times the rows.
+ * [tokens, num_experts].  K % 8 == 0, x_stride % 8 == 0; x, w and y 16-byte aligned.  Strides, here and below: less than 2^40, and times the
+ * rows than 2^60.
  */
 int sglb200_router_logits(const void* x, const void* w, int dtype, float* y, int64_t tokens, int64_t num_experts, int64_t K,
                           int64_t x_stride, void* stream);

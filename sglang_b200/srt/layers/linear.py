@@ -66,13 +66,16 @@ class LinearBase(nn.Module):
         self.prefix = prefix
         self.lora = None  # this rank's low-rank adapters (srt/lora)
 
-    # What `srt/lora` asks a layer: this rank's columns of every merged projection and of its input, and its part of an adapter's full A
-    # [rank, inputs] and B [outputs, rank] of projection `part`.
+    # What `srt/lora` asks a layer: this rank's columns of every merged projection and of its input, the outputs of projection `part` over all
+    # ranks, and this rank's part of an adapter's full A [rank, inputs] and B [outputs, rank] of it.
     def lora_output_sizes(self) -> List[int]:
         return [self.output_size]
 
     def lora_input_size(self) -> int:
         return self.input_size
+
+    def lora_full_outputs(self, part: int) -> int:
+        return self.output_size
 
     def lora_shard(self, part: int, a: torch.Tensor, b: torch.Tensor):
         return a, b
@@ -176,6 +179,9 @@ class ColumnParallelLinear(LinearBase):
     def lora_output_sizes(self) -> List[int]:
         return self.output_partition_sizes
 
+    def lora_full_outputs(self, part: int) -> int:
+        return self.output_sizes[part]
+
     def _source_block(self, part: int) -> int:
         """Which of `part`'s equal blocks of outputs this rank holds."""
         return self.tp_rank
@@ -217,6 +223,9 @@ class QKVParallelLinear(ColumnParallelLinear):
             raise NotImplementedError("QKV weights stored fused on disk are not on this path; pass \"q\", \"k\" or \"v\"")
         part = {"q": 0, "k": 1, "v": 2}[loaded_shard_id]
         self._load_part(param, loaded_weight, part, src_block=self._source_block(part))
+
+    def lora_full_outputs(self, part: int) -> int:  # (a replicated head's once)
+        return self.output_sizes[part] // (1 if part == 0 else self.num_kv_head_replicas)
 
     def _source_block(self, part: int) -> int:
         return self.tp_rank if part == 0 else self.tp_rank // self.num_kv_head_replicas

@@ -85,10 +85,10 @@ def load_adapter(layer, slot: int, a_parts: Sequence[Optional[torch.Tensor]], b_
         if (a is None) != (b is None):
             raise RuntimeError(f"projection {part} has one matrix of two")
         if a is not None:
-            a, b = layer.lora_shard(part, a, b)
-            want = (rank, s.lora_a.shape[2]), (width, rank)
+            want = (rank, layer.input_size), (layer.lora_full_outputs(part), rank)
             if tuple(a.shape) != want[0] or tuple(b.shape) != want[1]:
                 raise RuntimeError(f"projection {part}: A {tuple(a.shape)} and B {tuple(b.shape)}, expected {want[0]} and {want[1]}")
+            a, b = layer.lora_shard(part, a, b)
             a_new[part * R : part * R + rank].copy_(a)
             b_new[row : row + width, :rank].copy_(b)
         row += width

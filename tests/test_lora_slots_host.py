@@ -1,0 +1,43 @@
+"""Matrices, slots and ids that a layer with adapters refuses, and what attaching leaves alone (no GPU needed)."""
+import pytest
+import torch
+
+
+def _as_rank(monkeypatch, rank, world):
+    from sglang_b200.srt import distributed
+    from sglang_b200.srt.layers import linear
+    from sglang_b200.srt.layers.quantization import fp8
+    for m in (linear, fp8, distributed):
+        for name, v in (("get_tensor_model_parallel_world_size", world), ("get_tensor_model_parallel_rank", rank)):
+            if hasattr(m, name):
+                monkeypatch.setattr(m, name, lambda v=v: v)
+
+
+def _layers():
+    from sglang_b200.srt.layers.linear import MergedColumnParallelLinear, QKVParallelLinear, ReplicatedLinear, RowParallelLinear
+    from sglang_b200.srt.layers.quantization.fp8 import Fp8Config
+    cfg = Fp8Config()
+    # with the full sizes of every projection: inputs, outputs
+    return [(MergedColumnParallelLinear(512, [256, 512], quant_config=cfg), [(512, 256), (512, 512)]),
+            (QKVParallelLinear(512, 128, 8, 1, quant_config=cfg), [(512, 1024), (512, 128), (512, 128)]),
+            (QKVParallelLinear(512, 128, 8, 2, quant_config=cfg), [(512, 1024), (512, 256), (512, 256)]),
+            (RowParallelLinear(512, 384, quant_config=cfg), [(512, 384)]), (ReplicatedLinear(512, 256, quant_config=cfg), [(512, 256)])]
+
+
+@pytest.mark.parametrize("rank,world", [(0, 1), (0, 2), (1, 2)])
+def test_matrices_that_are_not_the_whole(monkeypatch, rank, world):
+    """A and B are the adapter's full ones: a larger, a smaller or an already cut one is refused, and not cut to what fits."""
+    from sglang_b200.srt.lora import LoRABatch, attach_lora, load_adapter
+    _as_rank(monkeypatch, rank, world)
+    for layer, sizes in _layers():
+        s = attach_lora(layer, LoRABatch(4), 2, 16, torch.float32)
+        good = [(torch.ones(8, i), torch.ones(o, 8)) for i, o in sizes]
+        for part, (i, o) in enumerate(sizes):
+            for di, do in ((512, 0), (-256, 0), (0, 128), (0, o), (0, -o // 2), (8, 0), (0, 1)):
+                bad = list(good)
+                bad[part] = (torch.ones(8, i + di), torch.ones(o + do, 8))
+                with pytest.raises(RuntimeError, match="expected"):
+                    load_adapter(layer, 0, [m[0] for m in bad], [m[1] for m in bad], 1.0)
+        assert not s.ranks.any() and not s.lora_a.any() and not s.lora_b.any()
+        load_adapter(layer, 1, [m[0] for m in good], [m[1] for m in good], 1.0)
+        assert int(s.ranks[1]) == 8 and s.lora_b[1, :, :8].eq(1).all() and s.lora_b[1].sum() == s.lora_b.shape[1] * 8

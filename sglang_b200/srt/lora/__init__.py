@@ -41,6 +41,8 @@ class LoRASlots(nn.Module):
 
     def __init__(self, layer, batch: LoRABatch, num_slots: int, max_rank: int, dtype: torch.dtype, device=None):
         super().__init__()
+        if not 1 <= num_slots <= 1024:
+            raise RuntimeError(f"num_slots is {num_slots}, not 1 to 1024")
         if max_rank % 8 or not 8 <= max_rank <= 256:
             raise RuntimeError(f"max_rank is {max_rank}, not a multiple of 8 up to 256")
         self.batch, self.max_rank, self.num_slots = batch, max_rank, num_slots
@@ -67,15 +69,24 @@ def attach_lora(layer, batch: LoRABatch, num_slots: int, max_rank: int, dtype: t
     return layer.lora
 
 
+def _slots(layer, slot: int) -> LoRASlots:
+    if layer.lora is None:
+        raise RuntimeError("the layer has no slots for adapters (attach_lora)")
+    if not 0 <= slot < layer.lora.num_slots:
+        raise RuntimeError(f"slot {slot} of {layer.lora.num_slots}")
+    return layer.lora
+
+
 def load_adapter(layer, slot: int, a_parts: Sequence[Optional[torch.Tensor]], b_parts: Sequence[Optional[torch.Tensor]],
                  scaling: float) -> None:
     """An adapter's FULL matrices into `slot` of a layer, of which this rank keeps its part: per merged projection A [rank, inputs] and
     B [its outputs, rank], or None for a projection that the adapter leaves alone."""
-    s = layer.lora
-    if not 0 <= slot < s.num_slots:
-        raise RuntimeError(f"slot {slot} of {s.num_slots}")
+    s = _slots(layer, slot)
     if len(a_parts) != len(s.slices) or len(b_parts) != len(s.slices):
         raise RuntimeError(f"{len(a_parts)} and {len(b_parts)} matrices for {len(s.slices)} merged projections")
+    for m in (*a_parts, *b_parts):
+        if m is not None and m.dim() != 2:
+            raise RuntimeError(f"{tuple(m.shape)} is not a matrix")
     ranks = {a.shape[0] for a in a_parts if a is not None} | {b.shape[1] for b in b_parts if b is not None}
     if len(ranks) != 1 or not 0 < max(ranks) <= s.max_rank:
         raise RuntimeError(f"ranks {sorted(ranks)}: one rank of at most {s.max_rank} for all of a layer's projections")
@@ -100,7 +111,7 @@ def load_adapter(layer, slot: int, a_parts: Sequence[Optional[torch.Tensor]], b_
 
 def unload_adapter(layer, slot: int) -> None:
     """Empties a slot: tokens that name it get nothing added."""
-    layer.lora.ranks[slot] = 0
+    _slots(layer, slot).ranks[slot] = 0
 
 
 __all__: List[str] = ["LoRABatch", "LoRASlots", "attach_lora", "load_adapter", "unload_adapter"]

@@ -41,3 +41,31 @@ def test_matrices_that_are_not_the_whole(monkeypatch, rank, world):
         assert not s.ranks.any() and not s.lora_a.any() and not s.lora_b.any()
         load_adapter(layer, 1, [m[0] for m in good], [m[1] for m in good], 1.0)
         assert int(s.ranks[1]) == 8 and s.lora_b[1, :, :8].eq(1).all() and s.lora_b[1].sum() == s.lora_b.shape[1] * 8
+
+
+def test_slots_that_are_not_there():
+    """A slot out of range (-1 would be the last one), a layer without slots, numbers of slots that the operator does not take."""
+    from sglang_b200.srt.lora import LoRABatch, attach_lora, load_adapter, unload_adapter
+    layer, sizes = _layers()[4]
+    (i, o), = sizes
+    for call in (lambda: unload_adapter(layer, 0), lambda: load_adapter(layer, 0, [torch.ones(8, i)], [torch.ones(o, 8)], 1.0)):
+        with pytest.raises(RuntimeError, match="no slots"):
+            call()
+    for bad in (0, -1, 1025):
+        with pytest.raises(RuntimeError, match="num_slots"):
+            attach_lora(layer, LoRABatch(4), bad, 16)
+        assert layer.lora is None
+    s = attach_lora(layer, LoRABatch(4), 3, 16, torch.float32)
+    for slot in range(3):
+        load_adapter(layer, slot, [torch.ones(8, i)], [torch.ones(o, 8)], 1.0)
+    for bad in (-1, 3, -3):
+        with pytest.raises(RuntimeError, match="slot"):
+            unload_adapter(layer, bad)
+        with pytest.raises(RuntimeError, match="slot"):
+            load_adapter(layer, bad, [torch.ones(8, i)], [torch.ones(o, 8)], 1.0)
+    assert s.ranks.tolist() == [8, 8, 8]
+    unload_adapter(layer, 2)
+    assert s.ranks.tolist() == [8, 8, 0]
+    for a, b in ((torch.ones(8), torch.ones(o, 8)), (torch.ones(8, i), torch.ones(o)), (torch.ones(1, 8, i), torch.ones(1, o, 8))):
+        with pytest.raises(RuntimeError, match="matrix"):
+            load_adapter(layer, 0, [a], [b], 1.0)

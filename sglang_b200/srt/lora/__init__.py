@@ -23,11 +23,14 @@ class LoRABatch:
         self.buffer = torch.full((max_tokens,), -1, dtype=torch.int32, device=device)
 
     def set(self, adapter_ids: torch.Tensor) -> None:
-        """`adapter_ids` [tokens] (any integer type; negative: no adapter); tokens behind them name none."""
+        """`adapter_ids` [tokens] (any integer type; negative, or more than int32 holds: no adapter); tokens behind them name none."""
         n = adapter_ids.numel()
         if n > self.buffer.numel():
             raise RuntimeError(f"LoRABatch: {n} tokens, made for {self.buffer.numel()}")
-        self.buffer[:n].copy_(adapter_ids.reshape(-1))
+        if adapter_ids.dtype == torch.bool or adapter_ids.is_floating_point() or adapter_ids.is_complex():
+            raise RuntimeError(f"LoRABatch: ids of {adapter_ids.dtype}, not of an integer type")
+        ids = adapter_ids.reshape(-1)
+        self.buffer[:n].copy_(ids.clamp(-1, 2**31 - 1) if ids.dtype == torch.int64 else ids)
         self.buffer[n:].fill_(-1)
 
     def ids(self, tokens: int) -> torch.Tensor:

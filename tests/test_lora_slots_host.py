@@ -69,3 +69,18 @@ def test_slots_that_are_not_there():
     for a, b in ((torch.ones(8), torch.ones(o, 8)), (torch.ones(8, i), torch.ones(o)), (torch.ones(1, 8, i), torch.ones(1, o, 8))):
         with pytest.raises(RuntimeError, match="matrix"):
             load_adapter(layer, 0, [a], [b], 1.0)
+
+
+def test_ids_of_any_integer_type():
+    """Ids beyond int32 name no adapter (they wrapped around to one), and numbers that are no integers are refused."""
+    from sglang_b200.srt.lora import LoRABatch
+    b = LoRABatch(6)
+    b.set(torch.tensor([1 << 32, (1 << 32) + 3, -(1 << 32) + 2, 5, -(1 << 31) - 1, (1 << 31) + 1]))
+    assert [i if 0 <= i < 1024 else None for i in b.ids(6).tolist()] == [None, None, None, 5, None, None]
+    for dtype in (torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64):
+        b.set(torch.tensor([3, 0, 7], dtype=dtype))
+        assert b.ids(6).tolist() == [3, 0, 7, -1, -1, -1]
+    for bad in (torch.tensor([1.0]), torch.tensor([True]), torch.tensor([1.0], dtype=torch.bfloat16)):
+        with pytest.raises(RuntimeError, match="integer"):
+            b.set(bad)
+    assert b.ids(6).tolist() == [3, 0, 7, -1, -1, -1]

@@ -30,7 +30,7 @@ class LoRABatch:
         if adapter_ids.dtype == torch.bool or adapter_ids.is_floating_point() or adapter_ids.is_complex():
             raise RuntimeError(f"LoRABatch: ids of {adapter_ids.dtype}, not of an integer type")
         ids = adapter_ids.reshape(-1)
-        self.buffer[:n].copy_(ids.clamp(-1, 2**31 - 1) if ids.dtype == torch.int64 else ids)
+        self.buffer[:n].copy_(ids.to(torch.int64).clamp(-1, 2**31 - 1) if ids.element_size() == 8 else ids)
         self.buffer[n:].fill_(-1)
 
     def ids(self, tokens: int) -> torch.Tensor:

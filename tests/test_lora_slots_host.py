@@ -77,7 +77,9 @@ def test_ids_of_any_integer_type():
     b = LoRABatch(6)
     b.set(torch.tensor([1 << 32, (1 << 32) + 3, -(1 << 32) + 2, 5, -(1 << 31) - 1, (1 << 31) + 1]))
     assert [i if 0 <= i < 1024 else None for i in b.ids(6).tolist()] == [None, None, None, 5, None, None]
-    for dtype in (torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64):
+    b.set(torch.tensor([(1 << 32) + 3, (1 << 63) - 1], dtype=torch.int64).to(torch.uint64))
+    assert all(not 0 <= i < 1024 for i in b.ids(6).tolist())
+    for dtype in (torch.uint8, torch.int8, torch.uint32, torch.int16, torch.int32, torch.int64):
         b.set(torch.tensor([3, 0, 7], dtype=dtype))
         assert b.ids(6).tolist() == [3, 0, 7, -1, -1, -1]
     for bad in (torch.tensor([1.0]), torch.tensor([True]), torch.tensor([1.0], dtype=torch.bfloat16)):

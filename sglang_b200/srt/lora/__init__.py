@@ -51,10 +51,10 @@ class LoRASlots(nn.Module):
         self.batch, self.max_rank, self.num_slots = batch, max_rank, num_slots
         self.slices = tuple(layer.lora_output_sizes())
         n, parts = sum(self.slices), len(self.slices)
-        self.register_buffer("lora_a", torch.zeros(num_slots, parts * max_rank, layer.lora_input_size(), dtype=dtype, device=device))
-        self.register_buffer("lora_b", torch.zeros(num_slots, n, max_rank, dtype=dtype, device=device))
-        self.register_buffer("scalings", torch.zeros(num_slots, dtype=torch.float32, device=device))
-        self.register_buffer("ranks", torch.zeros(num_slots, dtype=torch.int32, device=device))
+        self.register_buffer("lora_a", torch.zeros(num_slots, parts * max_rank, layer.lora_input_size(), dtype=dtype, device=device), persistent=False)
+        self.register_buffer("lora_b", torch.zeros(num_slots, n, max_rank, dtype=dtype, device=device), persistent=False)
+        self.register_buffer("scalings", torch.zeros(num_slots, dtype=torch.float32, device=device), persistent=False)
+        self.register_buffer("ranks", torch.zeros(num_slots, dtype=torch.int32, device=device), persistent=False)
 
     def add(self, out: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
         """out += the adapters' part of x, in place."""

@@ -86,3 +86,15 @@ def test_ids_of_any_integer_type():
         with pytest.raises(RuntimeError, match="integer"):
             b.set(bad)
     assert b.ids(6).tolist() == [3, 0, 7, -1, -1, -1]
+
+
+def test_attaching_leaves_the_state_dict_alone():
+    """A checkpoint of the layer loads with and without slots, and holds no adapters: they come and go while a program runs."""
+    from sglang_b200.srt.lora import LoRABatch, attach_lora
+    for layer, _ in _layers():
+        before = layer.state_dict()
+        attach_lora(layer, LoRABatch(4), 2, 16, torch.float32)
+        assert list(layer.state_dict()) == list(before)
+        layer.load_state_dict(before)
+        moved = layer.to("meta")  # the slots still go where the layer goes
+        assert moved.lora.lora_a.device.type == moved.lora.ranks.device.type == "meta"

@@ -37,13 +37,13 @@ class StandardDispatcher:
     def dispatch(self, hidden_states: torch.Tensor, topk_output: StandardTopKOutput) -> StandardDispatchOutput:
         if self.ep_size > 1:
             if self.local_expert_mapping is None:
-                m = torch.full((self.num_experts,), -1, dtype=torch.int32, device=hidden_states.device)
+                # (a negative id names no expert, and reads an entry of the second half)
+                m = torch.full((2 * self.num_experts,), -1, dtype=torch.int32, device=hidden_states.device)
                 lo = self.ep_rank * self.num_local_experts
                 m[lo : lo + self.num_local_experts] = torch.arange(
                     self.num_local_experts, dtype=torch.int32, device=hidden_states.device)
                 self.local_expert_mapping = m
-            named = topk_output.topk_ids  # (a negative id names no expert: it stays one)
-            ids = torch.where(named < 0, -1, self.local_expert_mapping[named.clamp_min(0).long()]).to(torch.int32)
+            ids = self.local_expert_mapping[topk_output.topk_ids.long()]
             topk_output = StandardTopKOutput(topk_output.topk_weights, ids, topk_output.router_logits)
         return StandardDispatchOutput(hidden_states, None, topk_output)
 

@@ -5,9 +5,9 @@
 // Up to three launches with programmatic serialization.  plan_kernel sorts the tokens by adapter into blocks (narrow.cuh); up to 64 tokens
 // need none.  The narrow product gives h in float32.  expand_kernel adds the second product.
 //
-// h keeps 16 bits and more in the second product: the row's values times a power of two that brings the largest to [1, 2) (float16 would
-// overflow or lose small ones without it) enter as two 16-bit terms, 16 bits of bfloat16 or 22 of float16; the weights are what they are.
-// A rounding to one term would be off by 2^-9 of h, as much as the rounding of the output.
+// h keeps 16 bits and more in the second product: the row's values times a power of two (float16 would overflow or lose small ones without it)
+// enter as two 16-bit terms, 16 bits of bfloat16 or 22 of float16, there of values down to 2^-16 of the row's largest (split_row); the weights
+// are what they are.  A rounding to one term would be off by 2^-9 of h, as much as the rounding of the output.
 #include <algorithm>
 
 #include "gemm_common.cuh"

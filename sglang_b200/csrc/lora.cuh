@@ -58,15 +58,19 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 
 // A row of h times `scaling`, value j * 32 + lane in v[j] -> two terms of a 16-bit type, times a power of two, whose inverse is returned;
 // put(r, high, low) for r below `width`.  One warp.
+//
+// The power of two brings the row's largest to [1, 2) for bfloat16, whose two terms hold 16 bits of values of any size, and to [2^14, 2^15) for
+// float16, whose smallest step is 2^-24: 22 bits of values down to 2^-16 of the largest, and a bit less for every power of two below.
 template <typename T, int kV, class Put>
 __device__ __forceinline__ float split_row(const float (&v)[kV], int width, int lane, Put put) {
   float most = 0.f;
 #pragma unroll
   for (int j = 0; j < kV; ++j) most = fmaxf(most, fabsf(v[j]));
   const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-  const uint32_t e = min(top >> 23, 253u);
-  const bool plain = e == 0 || top >= 0x7f800000u;  // nothing to bring anywhere
-  const float f = plain ? 1.f : __uint_as_float((254u - e) << 23);
+  constexpr uint32_t kUp = std::is_same<T, __half>::value ? 14 : 0;
+  const bool plain = top < 0x00800000u || top >= 0x7f800000u;  // nothing to bring anywhere
+  const uint32_t e = min(max(top >> 23, kUp + 1), 253u);       // (float16's outputs end far above 2^-112)
+  const float f = plain ? 1.f : __uint_as_float((254u + kUp - e) << 23);
 #pragma unroll
   for (int j = 0; j < kV; ++j) {
     const int r = j * 32 + lane;
@@ -76,7 +80,7 @@ __device__ __forceinline__ float split_row(const float (&v)[kV], int width, int 
     const float rest = s - ElemTraits<T>::to_f32(a);
     put(r, bits(a), bits(ElemTraits<T>::from_f32(fabsf(s) < INFINITY ? rest : 0.f)));
   }
-  return plain ? 1.f : __uint_as_float(e << 23);
+  return plain ? 1.f : __uint_as_float((e - kUp) << 23);
 }
 
 // lora_tile.cu: the second product for blocks of 128 rows; rank at most kTileRank, p.vec.  A status word as gemm_rows.cu's, and its reset.

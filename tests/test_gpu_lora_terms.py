@@ -35,7 +35,7 @@ def _pairs(T, R, dtype, seed, spread):
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("T,R", FORMS)
-@pytest.mark.parametrize("spread", [0])
+@pytest.mark.parametrize("spread", [0, 14])
 def test_no_bit_of_two_terms_is_lost(T, R, dtype, spread):
     """Every out is the sum of two h (times the power of two that makes up for 2^-m) plus base = -(that sum, rounded): what is left are the
     bits behind the first p, which two terms hold and out holds as well.  h is up to 2^-`spread` of its row's largest.

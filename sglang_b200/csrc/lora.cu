@@ -12,6 +12,7 @@
 
 #include "gemm_common.cuh"
 #include "lora.cuh"
+#include "narrow_rule.h"
 #include "ptx_sm100.cuh"
 
 namespace sglb200 {
@@ -470,7 +471,7 @@ extern "C" int sglb200_lora_add(const void* x, const void* lora_a, const void* l
   if (workspace == nullptr || workspace_bytes < bytes || !aligned16(workspace))
     return fail(SGLB200_E_WORKSPACE, "lora_add: %lld bytes of workspace are needed, aligned to 16", (long long)bytes);
   const bool scan = tokens <= narrow::kScanRows;
-  const int block = scan ? narrow::kSmallBlock : narrow::block_rows(tokens, (int64_t)num_slices * rank, true);
+  const int block = scan || narrow::small_adapter_blocks(tokens, num_slices, rank, K, N) ? narrow::kSmallBlock : narrow::kTileBlock;
   const int64_t blocks = lora::most_blocks(tokens, num_adapters, block);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int32_t* order = static_cast<int32_t*>(workspace);

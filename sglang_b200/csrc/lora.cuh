@@ -4,6 +4,7 @@
 
 #include "common.cuh"
 #include "narrow.cuh"
+#include "narrow_rule.h"
 
 namespace sglb200 {
 namespace lora {
@@ -84,7 +85,7 @@ __device__ __forceinline__ float split_row(const float (&v)[kV], int width, int 
 }
 
 // lora_tile.cu: the second product for blocks of 128 rows; rank at most kTileRank, p.vec.  A status word as gemm_rows.cu's, and its reset.
-constexpr int kTileRank = 128;
+constexpr int kTileRank = narrow::kMostTileRank;
 int expand_tile(Params& p, int dtype, cudaStream_t st);
 int tile_status();
 int tile_status_clear();

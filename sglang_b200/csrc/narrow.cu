@@ -9,6 +9,7 @@
 
 #include "gemm_common.cuh"
 #include "narrow.cuh"
+#include "narrow_rule.h"
 #include "ptx_sm100.cuh"
 
 namespace sglb200 {
@@ -182,16 +183,6 @@ static int dispatch(Params& p, int64_t blocks, cudaStream_t st) {
   return launch<T, 4>(p, blocks, st);
 }
 
-// (Both sides as they were when the rule was set; the first has become 0.3 to 1 us faster since.)  narrow_kernel's share of the weights and activations is fetched anew by every 16 weight rows and every block, narrow_tile_kernel starts later
-// (tensor memory, a pipeline, 128 rows).  Router, us here / there: 128 x 256 x 7168 9.4 / 9.8, 160 11.3 / 10.3; 256 x 128 x 2048 5.9 / 6.0; 1024 x
-// 32 x 1024 5.0 / 5.9; 512 x 64 x 4096 7.4 / 7.5, 1024 10.0 / 8.2.  Adapters, with the second product that goes with each: 256 tokens beside 2112
-// columns of rank 16 13.1 / 20.4, 1024 20.9 / 25.8; 256 beside 10240 of three times 64 28 / 28, 192 27.0 / 30.0, 320 41.0 / 30.5; 256 beside
-// 36864 of twice 32 33 to 46 / 31 to 53, 512 48 to 60 / 36 to 57.
-int block_rows(int64_t T, int64_t N, bool adapters) {
-  const int64_t most = !adapters ? 32768 : T <= 256 ? 49152 : 16384;
-  return T * N <= most ? kSmallBlock : kTileBlock;
-}
-
 int product(Params p, int dtype, int64_t max_blocks, cudaStream_t st) {
   if (p.block == kTileBlock) return tile_product(p, dtype, max_blocks, st);
   return dtype == 0 ? dispatch<__nv_bfloat16>(p, max_blocks, st) : dispatch<__half>(p, max_blocks, st);
@@ -217,6 +208,6 @@ extern "C" int sglb200_router_logits(const void* x, const void* w, int dtype, fl
   SGLB_REQUIRE(aligned16(x) && aligned16(w) && aligned16(y), "router_logits: pointers must be 16-byte aligned");
   narrow::Params p{};
   p.x = x, p.w = w, p.y = y, p.T = tokens, p.N = num_experts, p.K = K, p.ldx = x_stride, p.rank_rows = (int)num_experts;
-  p.adapters = 1, p.block = narrow::block_rows(tokens, num_experts, false);
+  p.adapters = 1, p.block = narrow::small_blocks(tokens, num_experts, K) ? narrow::kSmallBlock : narrow::kTileBlock;
   return narrow::product(p, dtype, (tokens + p.block - 1) / p.block, static_cast<cudaStream_t>(stream));
 }

@@ -78,9 +78,6 @@ struct Params {
   int n_tiles, splits;
 };
 
-// Rows of a block for T rows and N weight rows, of adapters or of one router.
-int block_rows(int64_t T, int64_t N, bool adapters);
-
 // A cluster has the K of one tile.  (Its number and a CTA's in it come without a division.)
 __device__ __forceinline__ uint32_t cluster_id() {
   uint32_t v;

@@ -93,18 +93,6 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __res
 // ---- second product -------------------------------------------------------------------------------------------------------------------
 constexpr int kWarps = 8;
 
-template <typename T>
-__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
 // The units of 8 warps' columns of all blocks, columns fastest, are cut evenly over as many CTAs as run at once; a run is what a CTA has of one
 // block and one merged projection.  kPairs: 32 values of the rank at most, which are two instructions; kTiles: groups of 8 columns of a warp.
 // As a sum does not mind the order of its terms, a lane's 16 consecutive bytes of a weight row (and of a row of h alike) are its part of both
@@ -307,10 +295,10 @@ __global__ void __launch_bounds__(kWarps * 32, kPairs == 1 ? 3 : 2) expand_kerne
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) {
           const uint4 w = ptx::lds_128(from + (s * kTiles + j) * kChunk);
-          mma16816<T>(acc[j], al.x, bl.x, al.y, bl.y, w.x, w.y);
-          mma16816<T>(acc[j], al.z, bl.z, al.w, bl.w, w.z, w.w);
-          mma16816<T>(acc[j], ah.x, bh.x, ah.y, bh.y, w.x, w.y);
-          mma16816<T>(acc[j], ah.z, bh.z, ah.w, bh.w, w.z, w.w);
+          ptx::mma_16816<std::is_same<T, __half>::value>(acc[j], al.x, bl.x, al.y, bl.y, w.x, w.y);
+          ptx::mma_16816<std::is_same<T, __half>::value>(acc[j], al.z, bl.z, al.w, bl.w, w.z, w.w);
+          ptx::mma_16816<std::is_same<T, __half>::value>(acc[j], ah.x, bh.x, ah.y, bh.y, w.x, w.y);
+          ptx::mma_16816<std::is_same<T, __half>::value>(acc[j], ah.z, bh.z, ah.w, bh.w, w.z, w.w);
         }
       }
 #pragma unroll

@@ -35,9 +35,6 @@ struct Cfg {
   static_assert(kSmem + 4096 <= 227 * 1024);
 };
 
-constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);  // rows of 128 bytes, 128-byte swizzle
-__device__ __forceinline__ uint32_t desc_lo(uint32_t smem) { return ((smem & 0x3ffffu) >> 4) | (1u << 16); }
-
 #define LORA_WAIT(bar, parity) \
   (p.wait_probes != ptx::kProbesNone && (ptx::mbar_test(bar, parity) || ptx::mbar_wait_quiet(bar, parity)))
 
@@ -170,8 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1) expand_tile_kernel(const Params p
     __syncwarp();
   } else if (warp == kAdders + 1) {
     if (ptx::elect_one()) {
-      constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-      constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10) | ((kCols >> 3) << 17) | ((kRows >> 4) << 24);
+      const uint32_t id = ptx::idesc_f16(kRows, kCols, std::is_same<T, __half>::value);
       int i = 0, runs = 0;
       bool ok = true;
       for (int at = begin; at < end && ok;) {
@@ -192,13 +188,10 @@ __global__ void __launch_bounds__(kThreads, 1) expand_tile_kernel(const Params p
           for (int term = 1; term >= 0; --term)  // the low terms first
 #pragma unroll 1
             for (int k = 0; k < steps; ++k) {
-              const uint32_t a = desc_lo(h_at + (term * kKB + k / 4) * kSpan) + 2 * (k % 4);
-              const uint32_t b = desc_lo(ring + (s * kKB + k / 4) * kSpan) + 2 * (k % 4);
-              asm volatile("{\n\t.reg .pred p;\n\t"
-                           "setp.ne.b32 p, %4, 0;\n\t"
-                           "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem + buf * kCols),
-                           "l"(ptx::pack_f32x2(a, kDescHi)), "l"(ptx::pack_f32x2(b, kDescHi)), "r"(kIdesc), "r"(term == 0 || k > 0 ? 1u : 0u)
-                           : "memory");
+              const uint32_t a = ptx::desc_lo128(h_at + (term * kKB + k / 4) * kSpan) + 2 * (k % 4);
+              const uint32_t b = ptx::desc_lo128(ring + (s * kKB + k / 4) * kSpan) + 2 * (k % 4);
+              ptx::mma_f16(tmem + buf * kCols, ptx::pack_f32x2(a, ptx::kDescHi128), ptx::pack_f32x2(b, ptx::kDescHi128), id,
+                           term == 0 || k > 0 ? 1u : 0u);
             }
           ptx::mma_commit(empty + s * 8);
           ptx::mma_commit(acc_full + buf * 8);

@@ -18,23 +18,12 @@ namespace narrow {
 constexpr int kWarps = 8;
 constexpr int kStep = 32;  // columns of K a warp takes at a time
 
-template <typename T>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 // What a warp adds up of 16 weight rows and up to kG groups of 8 activation rows, `rows` in all, over steps s0 .. s1 of K, to
 // part[16][pitch]; `row_of(i)`: the i-th activation row.  kAhead steps are asked for at once.
 template <typename T, int kG, int kAhead, class RowOf>
 __device__ __forceinline__ void add_up(const Params& p, const T* wa, const T* wb, bool a_on, bool b_on, int rows, int s0, int s1, int lane,
                                        float* part, int pitch, RowOf row_of) {
+  constexpr bool kF16 = std::is_same<T, __half>::value;
   const int g = lane >> 2, q = lane & 3;
   const T* x[kG];
 #pragma unroll
@@ -47,13 +36,15 @@ __device__ __forceinline__ void add_up(const Params& p, const T* wa, const T* wb
     const bool in = k < p.K;  // (K is a multiple of 8)
     const uint4 a = in && a_on ? __ldg(reinterpret_cast<const uint4*>(wa + k)) : zero;
     const uint4 b = in && b_on ? __ldg(reinterpret_cast<const uint4*>(wb + k)) : zero;
-    const uint32_t first[4] = {a.x, b.x, a.y, b.y}, second[4] = {a.z, b.z, a.w, b.w};
     uint4 v[kG];
 #pragma unroll
     for (int j = 0; j < kG; ++j) v[j] = in && (kG == 1 || j * 8 < rows) ? ld_nc_16(x[j] + k) : zero;
 #pragma unroll
     for (int j = 0; j < kG; ++j)
-      if (kG == 1 || j * 8 < rows) mma16816<T>(acc[j], first, v[j].x, v[j].y), mma16816<T>(acc[j], second, v[j].z, v[j].w);
+      if (kG == 1 || j * 8 < rows) {
+        ptx::mma_16816<kF16>(acc[j], a.x, b.x, a.y, b.y, v[j].x, v[j].y);
+        ptx::mma_16816<kF16>(acc[j], a.z, b.z, a.w, b.w, v[j].z, v[j].w);
+      }
   }
 #pragma unroll
   for (int j = 0; j < kG; ++j) {

@@ -43,21 +43,6 @@ struct TileParams {
   uint32_t wait_probes;
 };
 
-constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);  // rows of 128 bytes, 128-byte swizzle
-__device__ __forceinline__ uint32_t desc_lo(uint32_t smem) { return ((smem & 0x3ffffu) >> 4) | (1u << 16); }
-
-// f32 += bf16 x bf16 (1) or f16 x f16 (0), both operands K-major.
-__device__ __forceinline__ uint32_t idesc(int n, int fp16) {
-  const uint32_t type = fp16 ? 0u : 1u;
-  return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTileBlock >> 4) << 24);
-}
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
-  asm volatile("{\n\t.reg .pred p;\n\t"
-               "setp.ne.b32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate)
-               : "memory");
-}
-
 #define NARROW_WAIT(bar, parity) \
   (t.wait_probes != ptx::kProbesNone && (ptx::mbar_test(bar, parity) || ptx::mbar_wait_quiet(bar, parity)))
 
@@ -225,7 +210,7 @@ __global__ void __launch_bounds__(kSorted ? kSortedThreads : kThreads, 1)
     __syncwarp();
   } else if (warp == 9) {
     if (ptx::elect_one()) {
-      const uint32_t id = idesc(t.nt, t.fp16);
+      const uint32_t id = ptx::idesc_f16(kTileBlock, t.nt, t.fp16);
       bool ok = true;
       int s = 0, left = kChunk;  // stages of a chunk
       uint32_t ph = 0, buf = 0, acc_ph = 1;
@@ -235,11 +220,11 @@ __global__ void __launch_bounds__(kSorted ? kSortedThreads : kThreads, 1)
         if (!ok) break;
         if (scattered) ptx::fence_async_smem();  // (the copies' writes, which the barrier has shown, before the tensor core's reads)
         ptx::tc_fence_after();
-        const uint32_t at = base + s * stage_bytes, x_lo = desc_lo(at), w_lo = desc_lo(at + kXBytes);
+        const uint32_t at = base + s * stage_bytes, x_lo = ptx::desc_lo128(at), w_lo = ptx::desc_lo128(at + kXBytes);
 #pragma unroll
         for (int k = 0; k < kStageK / 16; ++k)
-          mma_f16(tmem + buf * kBuf, ptx::pack_f32x2(x_lo + 2 * k, kDescHi), ptx::pack_f32x2(w_lo + 2 * k, kDescHi), id,
-                         left < kChunk || k > 0 ? 1u : 0u);
+          ptx::mma_f16(tmem + buf * kBuf, ptx::pack_f32x2(x_lo + 2 * k, ptx::kDescHi128), ptx::pack_f32x2(w_lo + 2 * k, ptx::kDescHi128), id,
+                       left < kChunk || k > 0 ? 1u : 0u);
         ptx::mma_commit(empty + s * 8);
         if (++s == t.stages) s = 0, ph ^= 1;
         if (--left == 0 || kb + 1 == kb1) {

@@ -3,8 +3,8 @@
 // narrow_kernel: the weights on the M side of mma.sync (16 of their rows), up to 32 activation rows on its N side, operands straight from
 // global memory into registers: a lane takes 16 consecutive bytes of its row, and as a sum does not mind the order of its terms, those are
 // its part of two instructions, of the weights' rows and the activations' alike.  K is split over the warps of a CTA and the CTAs of a
-// cluster, whose sums meet in a fixed order.  Bound by latency: 1 x 256 x 7168 takes 3.6 us (1.0 TB/s), of which first loads 1, the sums
-// and two cluster barriers 1.5; 64 x 128 x 2048 3.8 us.
+// cluster, whose sums meet in a fixed order.  Bound by latency: in a graph of calls 1 x 256 x 7168 takes 3.4 us (1.1 TB/s), of which first loads
+// 1, the sums and two cluster barriers 1.5; 64 x 128 x 2048 3.6 us.
 #include <algorithm>
 
 #include "gemm_common.cuh"

@@ -6,7 +6,7 @@ gets its adapters' slots from `attach_lora(layer, ...)`; from then on its `forwa
     scaling[l] * B[l] (A[l] x)          l = the adapter that the token names, none: nothing
 
 to what it returns (`ops.lora_add`, in place, before a row-parallel layer's all-reduce).  Slots are loaded and emptied while the
-program runs; their buffers stay where they are, so that captured graphs go on working.
+program runs; their buffers stay where they are, so that captured graphs go on working, and are no part of the layer's state_dict.
 """
 from __future__ import annotations
 

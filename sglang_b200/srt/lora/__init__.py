@@ -80,6 +80,7 @@ def _slots(layer, slot: int) -> LoRASlots:
     return layer.lora
 
 
+@torch.no_grad()
 def load_adapter(layer, slot: int, a_parts: Sequence[Optional[torch.Tensor]], b_parts: Sequence[Optional[torch.Tensor]],
                  scaling: float) -> None:
     """An adapter's FULL matrices into `slot` of a layer, of which this rank keeps its part: per merged projection A [rank, inputs] and
@@ -112,6 +113,7 @@ def load_adapter(layer, slot: int, a_parts: Sequence[Optional[torch.Tensor]], b_
     s.ranks[slot] = rank
 
 
+@torch.no_grad()
 def unload_adapter(layer, slot: int) -> None:
     """Empties a slot: tokens that name it get nothing added."""
     _slots(layer, slot).ranks[slot] = 0

@@ -98,3 +98,17 @@ def test_attaching_leaves_the_state_dict_alone():
         layer.load_state_dict(before)
         moved = layer.to("meta")  # the slots still go where the layer goes
         assert moved.lora.lora_a.device.type == moved.lora.ranks.device.type == "meta"
+
+
+def test_trained_matrices_leave_no_history():
+    """Matrices that require gradients, as a trained adapter's do: the slots are no part of their graph."""
+    from sglang_b200.srt.lora import LoRABatch, attach_lora, load_adapter, unload_adapter
+    layer, sizes = _layers()[4]
+    (i, o), = sizes
+    s = attach_lora(layer, LoRABatch(4), 2, 16, torch.float32)
+    a, b = torch.nn.Parameter(torch.ones(8, i)), torch.nn.Parameter(torch.ones(o, 8))
+    load_adapter(layer, 1, [a], [b * 2], torch.nn.Parameter(torch.tensor(0.5)))
+    unload_adapter(layer, 0)
+    for t in s.buffers():
+        assert not t.requires_grad and t.grad_fn is None
+    assert s.lora_b[1, :, :8].eq(2).all() and float(s.scalings[1]) == 0.5

@@ -5,16 +5,16 @@
 //
 // The order is that of the real numbers.  Without a bias it is the order of the logits.  Where scores decide it is taken in float32, which
 // tells two c apart that differ by more than `margin` (below); a row in which two neighbours of the order are closer than that, and are not
-// the same logit with the same bias, is decided once more in float64 by its warp: the picks' order of one row in forty with 256 experts, a whole row of a few thousand.
-// c that float64 does not tell apart either (sigmoids of logits from 37 on are all 1) go by their logits, which is right wherever their biases
-// are equal; a group's sum of two is what float64 makes it.
+// the same logit with the same bias, is decided once more in float64 by its warp: the picks' order (order_exact) of one row in forty with 256
+// experts, a whole row (pick_exact) of a few thousand.  c that float64 does not tell apart either (sigmoids of logits from 37 on are all 1) go
+// by their logits (pick_by_logit), which is right wherever their biases are equal; a group's sum of two is what float64 makes it.
 //
 // One warp a row, the row in registers: lane l has consecutive experts of one group.  It is bound by issue slots.  A lane sorts its
 // experts once, as integers: an order-preserving bit pattern of c, whose lowest bits give way to the expert's number in the lane and, for the
 // picks, to the lane's (which the margins allow for; 16-bit logits lose nothing).  A pick is then one reduction over the lanes' best and a
 // shift of the winner's list.  16384 rows of 256 experts, best 8 in 4 of 8 groups: 841 instructions a row and 21 us; with the lanes' best looked for
-// after every pick and scores by division 1657 and 33.  What decides close calls stands in functions of its own: they run in cold instructions,
-// and registers that they need would be the loop's.
+// after every pick and scores by division 1657 and 33.  The three that decide anew are functions of their own: they run in cold
+// instructions, and registers that they need would be the loop's.
 #include <algorithm>
 #include <cfloat>
 

@@ -52,7 +52,6 @@
 
 #include "common.cuh"
 #include "gemm_common.cuh"
-#include "lora.cuh"
 #include "ptx_sm100.cuh"
 #include "quant_math.cuh"
 
@@ -1741,14 +1740,27 @@ int grouped_act_mm(const void* A, const float* a_s, const void* w13, const float
 
 using namespace sglb200;
 
+int sglb200::gemm_status_word(int** word) {
+  static thread_local int* of[64] = {nullptr};  // per device
+  int dev = 0;
+  SGLB_CUDA(cudaGetDevice(&dev));
+  if (dev >= 0 && dev < 64 && of[dev] != nullptr) {
+    *word = of[dev];
+    return SGLB200_OK;
+  }
+  void* at = nullptr;
+  SGLB_CUDA(cudaGetSymbolAddress(&at, g_gemm_status));
+  *word = static_cast<int*>(at);
+  if (dev >= 0 && dev < 64) of[dev] = *word;
+  return SGLB200_OK;
+}
+
 extern "C" int sglb200_gemm_status_clear(void) {
   const int zero = 0;
   SGLB_CUDA(cudaMemcpyToSymbol(g_gemm_status, &zero, sizeof(int)));
   int rc = rows_gemm_status_clear();
   if (rc == SGLB200_OK) rc = fp4_gemm_status_clear();
   if (rc == SGLB200_OK) rc = fp4_moe_status_clear();
-  if (rc == SGLB200_OK) rc = narrow::tile_status_clear();
-  if (rc == SGLB200_OK) rc = lora::tile_status_clear();
   return rc != SGLB200_OK ? rc : small_linear_status_clear();
 }
 
@@ -1758,8 +1770,6 @@ extern "C" int sglb200_gemm_status(void) {
   if (v == 0) v = rows_gemm_status();
   if (v == 0) v = fp4_gemm_status();
   if (v == 0) v = fp4_moe_status();
-  if (v == 0) v = narrow::tile_status();
-  if (v == 0) v = lora::tile_status();
   return v != 0 ? v : small_linear_status();
 }
 

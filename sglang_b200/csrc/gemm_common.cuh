@@ -106,6 +106,9 @@ int rows_grouped_mm(const void* A, int64_t a_rows, int64_t as_stride, const floa
                     int32_t* next_tile, bool pdl, cudaStream_t st);
 bool rows_grouped_single(int64_t max_rows, int num_experts, int64_t N, int nt);
 
+// gemm.cu: where on the current device sglb200_gemm_status looks first, for kernels of other files to report a wait that ran out.
+int gemm_status_word(int** word);
+
 // gemm_small.cu: quantise + multiply in one launch; whether a problem is one for it.
 bool small_linear_fits(int64_t M, int64_t N, int64_t K);
 int small_linear(const void* x, int dtype, const void* B, const float* b_s, void* C, const void* bias, int64_t M, int64_t N,

@@ -27,6 +27,7 @@ struct Params {
   int64_t col0[kMaxSlices + 1];  // first column of every merged projection, and the end
   int chunk0[kMaxSlices + 1];    // the first unit of columns, and the end
   uint32_t wait_probes;
+  int* status;  // 1 where a pipeline wait has run out
 };
 
 // This CTA's even share of `all` (below 2^31) units.  (A division in 64 bits takes a fifth of a microsecond, and a kernel's start was two of them.)
@@ -84,11 +85,9 @@ __device__ __forceinline__ float split_row(const float (&v)[kV], int width, int 
   return plain ? 1.f : __uint_as_float((e - kUp) << 23);
 }
 
-// lora_tile.cu: the second product for blocks of 128 rows; rank at most kTileRank, p.vec.  A status word as gemm_rows.cu's, and its reset.
+// lora_tile.cu: the second product for blocks of 128 rows; rank at most kTileRank, p.vec.
 constexpr int kTileRank = narrow::kMostTileRank;
 int expand_tile(Params& p, int dtype, cudaStream_t st);
-int tile_status();
-int tile_status_clear();
 
 }  // namespace lora
 }  // namespace sglb200

@@ -18,8 +18,6 @@
 namespace sglb200 {
 namespace lora {
 
-__device__ int g_lora_tile_status = 0;  // 0 ok, 1 = a pipeline wait expired
-
 namespace {
 
 constexpr int kRows = narrow::kTileBlock, kCols = 128;
@@ -349,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1) expand_tile_kernel(const Params p
   ptx::tc_fence_before();
   __syncthreads();
   if (ctl.abort_flag != 0 && tid == 0) {
-    atomicExch(&g_lora_tile_status, 1);
+    atomicExch(p.status, 1);
     // give products that may still be in flight time to end before tensor and shared memory are released
     const long long t0 = clock64();
     while (clock64() - t0 < 2000000ll) {
@@ -387,18 +385,10 @@ int expand_tile(Params& p, int dtype, cudaStream_t st) {
     tiles += (int)((p.col0[s + 1] - p.col0[s] + kCols - 1) / kCols);
   }
   p.chunk0[p.S] = tiles;
+  const int rc = gemm_status_word(&p.status);
+  if (rc) return rc;
   if (p.R <= 64) return dtype == 0 ? launch<__nv_bfloat16, 1>(p, st) : launch<__half, 1>(p, st);
   return dtype == 0 ? launch<__nv_bfloat16, 2>(p, st) : launch<__half, 2>(p, st);
-}
-
-int tile_status() {
-  int v = 0;
-  return cudaMemcpyFromSymbol(&v, g_lora_tile_status, sizeof(int)) != cudaSuccess ? -1 : v;
-}
-int tile_status_clear() {
-  const int zero = 0;
-  SGLB_CUDA(cudaMemcpyToSymbol(g_lora_tile_status, &zero, sizeof(int)));
-  return SGLB200_OK;
 }
 
 }  // namespace lora

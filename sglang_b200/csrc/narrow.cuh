@@ -93,10 +93,8 @@ __device__ __forceinline__ int cluster_rank() {
 // y = x w^T in blocks of p.block rows, `max_blocks` the most blocks there can be.
 int product(Params p, int dtype, int64_t max_blocks, cudaStream_t st);
 
-// narrow_tile.cu: the same for many rows; a status word as gemm_rows.cu's, and its reset.
+// narrow_tile.cu: the same for many rows.
 int tile_product(const Params& p, int dtype, int64_t max_blocks, cudaStream_t st);
-int tile_status();
-int tile_status_clear();
 
 }  // namespace narrow
 }  // namespace sglb200

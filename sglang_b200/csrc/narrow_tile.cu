@@ -19,8 +19,6 @@
 namespace sglb200 {
 namespace narrow {
 
-__device__ int g_tile_status = 0;  // 0 ok, 1 = a pipeline wait expired
-
 constexpr int kThreads = 320, kSortedThreads = 448;  // eight warps for the sums, one that loads, one that multiplies, four that copy sorted rows
 constexpr int kStageK = 64;        // columns of a stage: 128 bytes, one swizzle span
 constexpr int kChunk = 4;          // stages that are summed up in tensor memory
@@ -41,6 +39,7 @@ struct TileParams {
   int nt;        // weight rows of a tile, a multiple of 16
   int stages, kb_total, fp16;
   uint32_t wait_probes;
+  int* status;   // 1 where a pipeline wait has run out
 };
 
 #define NARROW_WAIT(bar, parity) \
@@ -287,7 +286,7 @@ __global__ void __launch_bounds__(kSorted ? kSortedThreads : kThreads, 1)
   ptx::tc_fence_before();
   __syncthreads();
   if (ctl->abort_flag != 0 && tid == 0) {
-    atomicExch(&g_tile_status, 1);
+    atomicExch(t.status, 1);
     // give copies that may still be in flight time to land before the CTA's shared memory is released
     const long long t0 = clock64();
     while (clock64() - t0 < 2000000ll) {
@@ -335,6 +334,8 @@ int tile_product(const Params& given, int dtype, int64_t max_blocks, cudaStream_
   t.p = given;
   Params& p = t.p;
   t.kb_total = (int)((p.K + kStageK - 1) / kStageK), t.fp16 = dtype, t.wait_probes = g_gemm_wait_probes;
+  int rc = gemm_status_word(&t.status);
+  if (rc) return rc;
   // Up to 256 weight rows a tile, so that the activations are fetched once (128 for sorted rows, whose warps have fewer registers); where there are
   // so few tiles that K can be split eight ways for twice as many, half as many rows, down to 32.
   const ClusterFits& fits = cluster_fits();
@@ -352,7 +353,7 @@ int tile_product(const Params& given, int dtype, int64_t max_blocks, cudaStream_
   CUtensorMap mx, mw;
   const uint64_t xd[2] = {(uint64_t)p.K * 2, (uint64_t)p.T}, xs[1] = {(uint64_t)p.ldx * 2};
   const uint32_t xb[2] = {kStageK * 2, sorted ? kTileBlock / 4u : (uint32_t)kTileBlock};
-  int rc = get_tile_map(p.x, 2, xd, xs, xb, true, &mx);
+  rc = get_tile_map(p.x, 2, xd, xs, xb, true, &mx);
   if (rc) return rc;
   const uint64_t wd[3] = {(uint64_t)p.K * 2, (uint64_t)p.N, (uint64_t)p.adapters}, ws[2] = {(uint64_t)p.K * 2, (uint64_t)(p.N * p.K * 2)};
   const uint32_t wb[3] = {kStageK * 2, (uint32_t)t.nt, 1};
@@ -362,16 +363,6 @@ int tile_product(const Params& given, int dtype, int64_t max_blocks, cudaStream_
   if (t.nt <= 64) return launch<2, false>(mx, mw, t, max_blocks, st);
   if (t.nt <= 128) return launch<4, false>(mx, mw, t, max_blocks, st);
   return launch<8, false>(mx, mw, t, max_blocks, st);
-}
-
-int tile_status() {
-  int v = 0;
-  return cudaMemcpyFromSymbol(&v, g_tile_status, sizeof(int)) != cudaSuccess ? -1 : v;
-}
-int tile_status_clear() {
-  const int zero = 0;
-  SGLB_CUDA(cudaMemcpyToSymbol(g_tile_status, &zero, sizeof(int)));
-  return SGLB200_OK;
 }
 
 }  // namespace narrow

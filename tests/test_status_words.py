@@ -1,5 +1,5 @@
 """Where the kernels' bounded waits report that they ran out, from the sources: the expert-parallel layer asks after every exchange, and each word
-of its own is a synchronous copy of 13 us."""
+of its own is a synchronous copy of 12 us."""
 import os
 import re
 
